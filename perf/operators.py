@@ -174,11 +174,11 @@ def _plain_norm(s):
 
 
 def _plain_int8(s):
-    x = s["x"].float()
+    x = s["x"].double()                         # (32 bits would decide between two whole numbers where x / scale lies halfway)
     scale = x.abs().amax(1, keepdim=True) / 127
     q = torch.where(scale > 0, torch.round(x / scale), torch.zeros_like(x))
-    y = q.double() @ s["w"].double().T          # whole numbers beyond 2^24
-    y = y * scale.double() * s["ws"].double()
+    y = q @ s["w"].double().T                   # whole numbers beyond 2^24
+    y = y * scale * s["ws"].double()
     if s["b"] is not None:
         y = y + s["b"].double()
     return y.to(s["x"].dtype)
