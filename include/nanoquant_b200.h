@@ -41,7 +41,9 @@ typedef enum {
     NQ_ERR_TOO_LARGE = -9    /* size beyond a stated fixed maximum */
 } nq_status;
 
-typedef enum { NQ_F16 = 0, NQ_BF16 = 1 } nq_dtype;
+typedef enum { NQ_F16 = 0, NQ_BF16 = 1, NQ_F32 = 2 } nq_dtype; /* NQ_F32: weights of the norms only */
+/* What linear cross entropy returns: every token's loss, their sum, or the mean over the tokens that have a target. */
+typedef enum { NQ_REDUCE_NONE = 0, NQ_REDUCE_SUM = 1, NQ_REDUCE_MEAN = 2 } nq_reduction;
 
 /* Bit order inside a 32-column word.
  * reference: src/nanoquant/kernel/utils.py:99-104 */
@@ -345,6 +347,67 @@ int nq_linear_fwd(const void* x, const void* s_in, const void* v_tiles, const vo
 int nq_dense_gemv_max_tokens(void);
 int nq_dense_gemv_fwd(const void* x, const void* w, const void* bias, void* y, int T, int N, int V,
                       int64_t ldw, int64_t ldy, int dtype, nq_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * Behind the last decoder layer: norms, the head in 8 bits, the loss over the head
+ * ------------------------------------------------------------------------ */
+
+/* Layer norm (center != 0) or RMS norm of `rows` rows of N <= nq_norm_max_columns() 16-bit elements, ldx / ldy elements apart:
+ *     y = (x - m) r * weight + bias,   m = mean(x) (0 for RMS),   r = 1 / sqrt(mean((x - m)^2) + eps)
+ * weight and bias [N] are nullable and of `weight_dtype`: the activations' dtype or NQ_F32.  `stats` (nullable) receives
+ * (m, r) of every row, 2 * rows floats, which the backward pass reads.  fp32 arithmetic, one rounding of y.
+ * Any alignment; 16-byte loads where N, ldx and ldy are multiples of 8 and the pointers 16-byte aligned.
+ * No counterpart in the reference (its models' norms are torch's). */
+int nq_norm_max_columns(void);
+int nq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t rows, int64_t N,
+                int64_t ldx, int64_t ldy, float eps, int center, int dtype, int weight_dtype, nq_stream_t stream);
+
+/* Its backward pass: dx [rows, lddx], dweight and dbias [N] (weight_dtype), each nullable.  x may be read from where dx is
+ * written only if they are the same rows.  `scratch`: nq_norm_bwd_scratch_bytes() for the fp32 partial sums of dweight and dbias
+ * (not needed without them), 16-byte aligned, any contents.  The sums are added in an order that depends on the sizes alone. */
+size_t nq_norm_bwd_scratch_bytes(int64_t rows, int64_t N);
+int nq_norm_bwd(const void* dy, const void* x, const void* weight, const float* stats, void* dx, void* dweight, void* dbias,
+                void* scratch, size_t scratch_bytes, int64_t rows, int64_t N, int64_t lddy, int64_t ldx, int64_t lddx,
+                int center, int dtype, int weight_dtype, nq_stream_t stream);
+
+/* 16-bit rows -> signed bytes with one scale per row: scale = max|x| / 127, q = rint(127 x / max|x|) (ties to even; 0 for a row of zeros).
+ * A row with a NaN or an infinity has a NaN scale. */
+int nq_quantize_rows_s8(const void* x, int8_t* q, float* scale, int64_t rows, int64_t N, int64_t ldx, int64_t ldq, int dtype,
+                        nq_stream_t stream);
+
+/* y[t, v] = s_x[t] w_scale[v] sum_k q_x[t, k] w[v, k] (+ bias[v]): x [T, N] 16-bit, quantised per token as above within the call; w [V, ldw]
+ * signed bytes (rows of nq_quantize_rows_s8, ldw a multiple of 16), exact int32 sums (N <= 131072), fp32 scaling, one rounding of y.
+ * 16-byte aligned w, w_scale and scratch (nq_int8_linear_scratch_bytes(), any contents).  `status_word` as in nq_onebit_gemm_fwd.
+ * Few tokens stream w once, half the bytes of nq_dense_gemv_fwd; any number of tokens.  Weights may be read ahead of the completion of
+ * the kernel before the call (see nq_gemm_fwd). */
+size_t nq_int8_linear_scratch_bytes(int64_t T, int64_t N);
+int nq_int8_linear_fwd(const void* x, const int8_t* w, const float* w_scale, const void* bias, void* y, void* scratch, size_t scratch_bytes,
+                       void* status_word, int64_t T, int64_t N, int64_t V, int64_t ldx, int64_t ldw, int64_t ldy, int dtype,
+                       nq_stream_t stream);
+
+/* Cross entropy of T targets over a vocabulary of V words, from the hidden states h [T, ldh] and the weight w [V, ldw] of the head (one
+ * 16-bit dtype, N columns; N, ldh, ldw multiples of 8, 16-byte aligned), without the logits:
+ *     lse[t] = log sum_v exp(h[t] . w[v]),   loss[t] = lse[t] - h[t] . w[target[t]]
+ * `targets`: T int32 or int64 (target_bits).  A token whose target is ignore_index has no loss and no gradient, whatever its row holds; any
+ * other target outside 0..V-1 makes its loss and gradient NaN.  `loss`: T floats (NQ_REDUCE_NONE) or one; the mean of no tokens is NaN.
+ * lse [T] and count [1] (tokens with a target; not written for NQ_REDUCE_NONE) are what the backward pass reads.  `status_word` as in
+ * nq_onebit_gemm_fwd.  Scratch: 16-byte aligned, any contents.
+ * The reference evaluates perplexity and tunes its scales with this loss (src/nanoquant/utils/eval_utils.py:13-87,
+ * core/compress_model.py:125-286), by torch's product and cross entropy or another package's fused one. */
+size_t nq_linear_ce_fwd_scratch_bytes(int64_t T, int64_t N, int64_t V);
+int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int target_bits, int64_t ignore_index, float* loss, float* lse,
+                     float* count, void* scratch, size_t scratch_bytes, void* status_word, int64_t T, int64_t N, int64_t V, int64_t ldh,
+                     int64_t ldw, int reduction, int dtype, nq_stream_t stream);
+
+/* Its gradients dh [T, lddh] and dw [V, lddw] (nullable, same dtype) for grad_loss: one float, or for NQ_REDUCE_NONE T of them,
+ * grad_stride apart.  The vocabulary is processed in pieces whose gradients of the logits fit 256 MB of the scratch (more only where 256 words
+ * of all tokens do not), rounded there to the dtype (fp16: scaled by the largest |grad_loss|); sums in fp32, in an order that depends on
+ * the sizes alone.  The gradient of a mean over no tokens is zero. */
+size_t nq_linear_ce_bwd_scratch_bytes(int64_t T, int64_t N, int64_t V);
+int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int target_bits, int64_t ignore_index, const float* lse,
+                     const float* count, const float* grad_loss, int64_t grad_stride, void* dh, void* dw, void* scratch, size_t scratch_bytes,
+                     void* status_word, int64_t T, int64_t N, int64_t V, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw, int reduction,
+                     int dtype, nq_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
  * Measurement probes (no counterpart in the reference; nothing on the hot path calls them)

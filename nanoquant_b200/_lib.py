@@ -14,8 +14,9 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libnanoquant_b200.so")
 EXT_PATH = os.path.join(_PKG, "_nq_torch.so")
 
-NQ_F16, NQ_BF16 = 0, 1
+NQ_F16, NQ_BF16, NQ_F32 = 0, 1, 2
 NQ_LSB_FIRST, NQ_HALF2 = 0, 1
+REDUCTION_ID = {"none": 0, "sum": 1, "mean": 2}     # NQ_REDUCE_*
 ORDER_ID = {"lsb_first": NQ_LSB_FIRST, "half2": NQ_HALF2}
 
 GEMM_KERNELS = ("batch_stage_kernel", "wgemm_kernel", "pgemm_kernel")     # NQ_KERNEL_*
@@ -72,6 +73,19 @@ SIGNATURES = {
     "nq_allgather_set_wait_limit": (ctypes.c_uint, [ctypes.c_uint]),
     "nq_dense_gemv_max_tokens": (c_int, []),
     "nq_dense_gemv_fwd": (c_int, [c_void_p] * 4 + [c_int, c_int, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "nq_norm_max_columns": (c_int, []),
+    "nq_norm_fwd": (c_int, [c_void_p] * 5 + [c_int64] * 4 + [ctypes.c_float, c_int, c_int, c_int, c_void_p]),
+    "nq_norm_bwd_scratch_bytes": (c_size_t, [c_int64, c_int64]),
+    "nq_norm_bwd": (c_int, [c_void_p] * 8 + [c_size_t] + [c_int64] * 5 + [c_int, c_int, c_int, c_void_p]),
+    "nq_quantize_rows_s8": (c_int, [c_void_p] * 3 + [c_int64] * 4 + [c_int, c_void_p]),
+    "nq_int8_linear_scratch_bytes": (c_size_t, [c_int64, c_int64]),
+    "nq_int8_linear_fwd": (c_int, [c_void_p] * 6 + [c_size_t, c_void_p] + [c_int64] * 6 + [c_int, c_void_p]),
+    "nq_linear_ce_fwd_scratch_bytes": (c_size_t, [c_int64] * 3),
+    "nq_linear_ce_fwd": (c_int, [c_void_p] * 3 + [c_int, c_int64] + [c_void_p] * 4 + [c_size_t, c_void_p] + [c_int64] * 5 +
+                         [c_int, c_int, c_void_p]),
+    "nq_linear_ce_bwd_scratch_bytes": (c_size_t, [c_int64] * 3),
+    "nq_linear_ce_bwd": (c_int, [c_void_p] * 3 + [c_int, c_int64] + [c_void_p] * 3 + [c_int64] + [c_void_p] * 3 + [c_size_t, c_void_p] +
+                         [c_int64] * 7 + [c_int, c_int, c_void_p]),
     "nq_gemv_max_tokens": (c_int, []),
     "nq_linear_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "nq_linear_fwd": (c_int, [c_void_p] * 8 + [c_size_t, c_int, c_int, c_int, c_int, c_int, c_void_p]),

@@ -140,6 +140,20 @@ int encode_activations(CUtensorMap* map, const StageJob& S, int bf16, int T, int
     return r == CUDA_SUCCESS ? NQ_OK : NQ_ERR_UNSUPPORTED;
 }
 
+int mm_encode(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int box_inner, int box_outer) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return NQ_ERR_UNSUPPORTED;
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType dt = type == kMmS8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == kMmBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = enc(map, dt, 2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? NQ_OK : NQ_ERR_UNSUPPORTED;
+}
+
 // The kernel of a stage, with its plan.  (An intermediate in the GEMMs' column order is theirs.)
 static int pick_kernel(const StageJob* jobs, int n, int T, int order, WgemmPlan& w, PgemmPlan& p) {
     if (order == 0 && T <= batch_max_tokens(jobs, n)) return NQ_KERNEL_BATCH;

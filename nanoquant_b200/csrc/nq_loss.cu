@@ -1,0 +1,542 @@
+// Softmax cross entropy over the un-quantised head, without the logits:
+//
+//     l[t, v] = h[t] . w[v]        lse[t] = log sum_v exp(l[t, v])        loss[t] = lse[t] - l[t, target[t]]
+//     d[t, v] = g[t] (exp(l[t, v] - lse[t]) - [v = target[t]])            dh = d w        dw = d^T h
+//
+// Forward: one product whose epilogue keeps, for each token and each tile's half of the columns, the largest logit and the sum of exponentials
+// relative to it (fp32), and picks the target's logit; a second kernel joins the pieces of a token in a fixed order.
+//
+// Backward, over pieces of the vocabulary whose d fits the scratch (kLossPieceBytes): the logits of the piece once more, d from them and
+// the kept lse, rounded to the type of the operands (what the tensor cores multiply), then dw of the piece, complete, and the piece's part of
+// dh, added in fp32.  So four products in all, 8 T N V operations, and no more memory than a piece.
+//
+// Bound by the tensor cores from some 300 tokens on, below by reading w (each product once).
+#include "nq_common.cuh"
+#include "nq_mm.cuh"
+
+namespace nq {
+
+constexpr int64_t kLossPieceBytes = 256ll << 20;
+constexpr int kLossPieceUnit = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// fp16 holds d as multiples of this fraction of the largest |g|: probabilities down to 4e-9 of it are normal numbers.  (bf16 has the exponents of fp32.)
+constexpr float kLossHalfScale = 16384.f;
+
+__device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp, zero below 2^-126
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+struct LossTargets {
+    const void* p;
+    int wide;            // int64, not int32
+    long long ignore;
+};
+__device__ __forceinline__ long long loss_target(const LossTargets& t, int row) {
+    return t.wide ? __ldg(static_cast<const long long*>(t.p) + row) : (long long)__ldg(static_cast<const int*>(t.p) + row);
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+struct LseEpilogue {
+    static constexpr bool kS8 = false;
+    struct Params {
+        LossTargets targets;
+        float2* part;              // [2 n_tiles][T]: largest logit (times log2 e), sum
+        float* target_logit;       // [T]
+    };
+    const Params& p;
+    const MmShape& s;
+    int row, n0, slot;
+    long long target;
+    float top, sum;
+    __device__ LseEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_) {}
+    __device__ __forceinline__ void begin(int row_, int n0_, int set, int n_tile, int) {
+        row = row_;
+        n0 = n0_;
+        slot = 2 * n_tile + set;
+        target = row < s.M ? loss_target(p.targets, row) : -1;
+        top = -INFINITY;
+        sum = 0.f;
+    }
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char*) {
+        float cm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < cols) cm = fmaxf(cm, __uint_as_float(r[i]));
+        const float m = fmaxf(top, cm * kLog2e), base = m == -INFINITY ? 0.f : m;
+        sum *= exp2_fast(top - base);
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float a = exp2_fast(fmaf(__uint_as_float(r[i]), kLog2e, -base)), b = exp2_fast(fmaf(__uint_as_float(r[i + 1]), kLog2e, -base));
+            if (i < cols) s0 += a;
+            if (i + 1 < cols) s1 += b;
+        }
+        sum += s0 + s1;
+        top = m;
+        const long long at = target - (n0 + c);
+        if (at >= 0 && at < cols) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (at == i) p.target_logit[row] = __uint_as_float(r[i]);
+        }
+    }
+    __device__ __forceinline__ void end() {
+        if (row < s.M) p.part[(long long)slot * s.M + row] = make_float2(top, sum);
+    }
+};
+
+// 32 tokens a CTA, the pieces dealt to its warps.  A target that is no word of the vocabulary (and not `ignore`) makes its token NaN.
+__global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V) {
+    __shared__ float2 red[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto join = [](float2 a, float2 b) {
+        const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
+        return make_float2(m, a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base));
+    };
+    float2 v = make_float2(-INFINITY, 0.f);
+    if (row < T) {
+#pragma unroll 8
+        for (int i = warp; i < slots; i += 32) v = join(v, part[(long long)i * T + row]);
+    }
+    red[warp][lane] = v;
+    __syncthreads();
+    // warp w joins the 32 sums of token w
+    v = red[lane][warp];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+    const int r = blockIdx.x * 32 + warp;
+    if (lane == 0 && r < T) {
+        const long long t = loss_target(targets, r);
+        float l = v.x * kLn2 + logf(v.y), loss = 0.f;
+        if (t != targets.ignore) {
+            if (t >= 0 && t < V) loss = l - target_logit[r];
+            else loss = l = __int_as_float(0x7fffffff);
+        }
+        row_loss[r] = loss;
+        lse[r] = l;
+    }
+}
+
+// Sum (mean: of the tokens with a target) of the tokens' losses and the number of these tokens; one CTA, a fixed order, 64-bit sums.
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* row_loss, LossTargets targets, float* out, float* count, int T, int mean) {
+    __shared__ double sums[32];
+    __shared__ int counts[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    double s = 0;
+    int n = 0;
+    for (int i = threadIdx.x; i < T; i += 1024) {
+        if (row_loss) s += row_loss[i];
+        n += loss_target(targets, i) != targets.ignore;
+    }
+    auto reduce = [&]() {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
+    };
+    reduce();
+    if (lane == 0) { sums[warp] = s; counts[warp] = n; }
+    __syncthreads();
+    if (warp == 0) {
+        s = sums[lane];
+        n = counts[lane];
+        reduce();
+        if (lane == 0) {
+            *count = (float)n;
+            if (out) *out = mean ? (float)(s / n) : (float)s;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// row_scale[t]: what d of a token is multiplied by before it is rounded; final: what the products' sums are multiplied by.
+__global__ void __launch_bounds__(1024) loss_scales_kernel(const float* grad, long long grad_stride, const float* count, LossTargets targets, float* row_scale, float* final_scale,
+                                                           int T, int reduction, float unit) {
+    __shared__ float red[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float top = 0.f;
+    if (reduction == NQ_REDUCE_NONE && unit != 1.f) {
+        for (int i = threadIdx.x; i < T; i += 1024)
+            if (loss_target(targets, i) != targets.ignore) top = fmaxf(top, fabsf(grad[i * grad_stride]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) red[warp] = top;
+        __syncthreads();
+        top = red[lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (top == 0.f || top == INFINITY) top = 1.f;
+    } else {
+        top = 1.f;
+    }
+    for (int i = threadIdx.x; i < T; i += 1024) {
+        const bool live = loss_target(targets, i) != targets.ignore;
+        row_scale[i] = !live ? 0.f : reduction == NQ_REDUCE_NONE ? grad[i * grad_stride] / top * unit : unit;
+    }
+    if (threadIdx.x == 0) {
+        float f = reduction == NQ_REDUCE_NONE ? top : grad[0];
+        if (reduction == NQ_REDUCE_MEAN) f = *count > 0.f ? f / *count : 0.f;
+        *final_scale = f / unit;
+    }
+}
+// h with zeros in the rows of tokens without a target, whatever these hold (their d is zero, but zero times a NaN is not).
+__global__ void __launch_bounds__(256) loss_rows_kernel(const uint4* h, uint4* out, LossTargets targets, int T, int packs, long long ldh) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long total = (long long)T * packs;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int row = (int)(i / packs), c = (int)(i - (long long)row * packs);
+        out[i] = loss_target(targets, row) != targets.ignore ? __ldg(h + row * ldh + c) : make_uint4(0, 0, 0, 0);
+    }
+}
+
+// d of a piece of the vocabulary.
+template <int OUT>
+struct GradEpilogue {
+    static constexpr bool kS8 = false;
+    struct Params {
+        LossTargets targets;
+        const float *lse, *row_scale;
+        uint16_t* d;
+        long long ldd;
+        int v0;                    // first word of the piece
+    };
+    const Params& p;
+    const MmShape& s;
+    int row, n0, at;
+    float base, scale;
+    bool live;
+    __device__ GradEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_) {}
+    __device__ __forceinline__ void begin(int row_, int n0_, int, int, int) {
+        row = row_;
+        n0 = n0_;
+        live = false;
+        at = -1;
+        base = scale = 0.f;
+        if (row < s.M) {
+            const long long t = loss_target(p.targets, row);
+            live = t != p.targets.ignore;
+            const long long rel = t - p.v0 - n0;
+            at = rel >= 0 && rel < kMmAccCols ? (int)rel : -1;
+            base = __ldg(p.lse + row) * kLog2e;
+            scale = __ldg(p.row_scale + row);
+        }
+    }
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
+        const int row0 = row & ~31;
+        if (row0 >= s.M) return;                        // (the whole warp)
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float d[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float e = exp2_fast(fmaf(__uint_as_float(r[i + k]), kLog2e, -base));
+                if (at == c + i + k) e -= 1.f;
+                d[k] = live ? e * scale : 0.f;
+            }
+            w[i / 2] = pack_outputs<OUT>(d[0], d[1], 0);
+        }
+        mm_store_rows(stage, w, p.d + row0 * p.ldd + n0 + c, p.ldd, min(32, s.M - row0), cols, true);
+    }
+    __device__ __forceinline__ void end() {}
+};
+
+// dw of a piece: rows of words, times the final scale.
+template <int OUT>
+struct RowsEpilogue {
+    static constexpr bool kS8 = false;
+    struct Params {
+        const float* final_scale;
+        uint16_t* out;
+        long long ld;
+    };
+    const Params& p;
+    const MmShape& s;
+    int row0, n0;
+    float f;
+    __device__ RowsEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_), f(__ldg(p_.final_scale)) {}
+    __device__ __forceinline__ void begin(int row, int n0_, int, int, int) {
+        row0 = row & ~31;
+        n0 = n0_;
+    }
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
+        if (row0 >= s.M) return;                        // (the whole warp)
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = pack_outputs<OUT>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f, 0);
+        mm_store_rows(stage, w, p.out + row0 * p.ld + n0 + c, p.ld, min(32, s.M - row0), cols, true);
+    }
+    __device__ __forceinline__ void end() {}
+};
+
+// Partial sums of dh in fp32: [split][128 rows][4 columns][row], so that a warp's stores are whole lines.
+struct SumEpilogue {
+    static constexpr bool kS8 = false;
+    struct Params {
+        float4* sums;
+        int blocks, quads;         // of 128 rows; of 4 columns, padded to whole tiles
+        int add;                   // to what an earlier piece left
+    };
+    const Params& p;
+    const MmShape& s;
+    int n0;
+    float4* dst;
+    __device__ SumEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_) {}
+    __device__ __forceinline__ void begin(int row, int n0_, int, int, int split) {
+        n0 = n0_;
+        dst = p.sums + (((long long)split * p.blocks + (row >> 7)) * p.quads + (n0 >> 2)) * 128 + (row & 127);
+    }
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int, unsigned char*) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float4* q = dst + (long long)((c >> 2) + i) * 128;
+            float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+            if (p.add) {
+                const float4 o = *q;
+                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+            }
+            *q = v;
+        }
+    }
+    __device__ __forceinline__ void end() {}
+};
+
+// dh: the splits' sums, added in order, times the final scale.  32 tokens x 64 columns a CTA.
+template <int OUT>
+__global__ void __launch_bounds__(256) dh_kernel(const float4* sums, const float* final_scale, uint16_t* dh, long long ld, int T, int N, int blocks, int quads, int splits) {
+    __shared__ uint32_t tile[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = blockIdx.x * 32, col0 = blockIdx.y * 64;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const float f = *final_scale;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int qd = 2 * warp + k, quad = (col0 >> 2) + qd;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (quad < quads) {
+#pragma unroll 4
+            for (int sp = 0; sp < splits; ++sp) {
+                const float4 o = sums[(((long long)sp * blocks + (row0 >> 7)) * quads + quad) * 128 + (row0 & 127) + lane];
+                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+            }
+        }
+        tile[lane][2 * qd] = pack_outputs<OUT>(v.x * f, v.y * f, 0);
+        tile[lane][2 * qd + 1] = pack_outputs<OUT>(v.z * f, v.w * f, 0);
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 3, j = threadIdx.x & 7;
+    if (row0 + r < T && col0 + 8 * j < N)               // (N is a multiple of 8)
+        *reinterpret_cast<uint4*>(dh + (long long)(row0 + r) * ld + col0 + 8 * j) = make_uint4(tile[r][4 * j], tile[r][4 * j + 1], tile[r][4 * j + 2], tile[r][4 * j + 3]);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+static int launch_plain(const void* fn, dim3 grid, int threads, void** args, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    return launch_dependent(cfg, attr, 0, fn, args);
+}
+static bool loss_pairs(int64_t T) { return T > 128; }
+
+struct LossPlan {
+    int bn, slots;                       // forward
+    int64_t piece;                       // words
+    int d_bn, w_bn, h_bn, h_splits, h_blocks, h_quads;
+};
+static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
+    LossPlan p;
+    const int cg = loss_pairs(T) ? 2 : 1, groups = sm_count() / cg, m_tiles = (int)((T + 128 * cg - 1) / (128 * cg));
+    p.bn = mm_tile_cols((int)V, m_tiles, groups, 16 * cg, 64);
+    p.slots = 2 * (int)((V + p.bn - 1) / p.bn);
+    p.piece = kLossPieceBytes / 2 / T / kLossPieceUnit * kLossPieceUnit;
+    if (p.piece < kLossPieceUnit) p.piece = kLossPieceUnit;
+    const int64_t all = up(V, kLossPieceUnit);
+    if (p.piece > all) p.piece = all;
+    else {
+        const int64_t pieces = (V + p.piece - 1) / p.piece;      // of equal size
+        p.piece = up((V + pieces - 1) / pieces, kLossPieceUnit);
+    }
+    p.d_bn = mm_tile_cols((int)(p.piece < V ? p.piece : V), m_tiles, groups, 16 * cg, 64);
+    p.w_bn = N <= 128 ? 128 : 256;
+    // dh: few tiles over a long k.  Rounds of the longest tile, plus what writing and adding one more set of sums costs.
+    p.h_bn = cg == 2 ? (N <= 128 ? 128 : 256) : (N <= 64 ? 64 : N <= 128 ? 128 : 256);
+    const int64_t tiles = (int64_t)m_tiles * ((N + p.h_bn - 1) / p.h_bn), steps = ((p.piece < V ? p.piece : V) + 63) / 64;
+    p.h_splits = 1;
+    double best = 0;
+    for (int s = 1; s <= 32 && s <= steps; ++s) {
+        if (s > 1 && s * tiles * p.h_bn * 128 * cg * 4 > kLossPieceBytes) break;
+        const double cost = (double)((tiles * s + groups - 1) / groups) * (double)((steps + s - 1) / s + 8) + 0.12 * (double)(tiles * s) / groups * 32;
+        if (s == 1 || cost < best) { best = cost; p.h_splits = s; }
+    }
+    p.h_blocks = m_tiles * cg;
+    p.h_quads = (int)(up(N, p.h_bn) / 4);
+    return p;
+}
+struct LossScratch { int64_t d, h, sums, row_scale, final_scale, bytes; };
+static LossScratch loss_scratch(const LossPlan& p, int64_t T, int64_t N) {
+    LossScratch s;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t here = at; at += up(bytes, 256); return here; };
+    s.d = take(T * p.piece * 2);
+    s.h = take(T * N * 2);
+    s.sums = take((int64_t)p.h_splits * p.h_blocks * p.h_quads * 128 * 16);
+    s.row_scale = take(T * 4);
+    s.final_scale = take(4);
+    s.bytes = at;
+    return s;
+}
+static int check_loss(int64_t T, int64_t N, int64_t V, int64_t ldh, int64_t ldw, int dtype, int reduction, int target_bits) {
+    if (dtype != NQ_F16 && dtype != NQ_BF16) return NQ_ERR_DTYPE;
+    if (target_bits != 32 && target_bits != 64) return NQ_ERR_DTYPE;
+    if (reduction < NQ_REDUCE_NONE || reduction > NQ_REDUCE_MEAN) return NQ_ERR_UNSUPPORTED;
+    if (T < 1 || N < 1 || V < 1 || N % 8 || ldh < N || ldh % 8 || ldw < N || ldw % 8) return NQ_ERR_SHAPE;
+    if (T > (1 << 22) || N > (1 << 20) || V > (1 << 24)) return NQ_ERR_TOO_LARGE;
+    return NQ_OK;
+}
+
+template <int CG>
+static int launch_lse(const void* h, const void* w, const LseEpilogue::Params& e, int T, int N, int V, int64_t ldh, int64_t ldw, int type, int bn,
+                      unsigned* status, cudaStream_t stream) {
+    MmParams<LseEpilogue> P = {};
+    P.e = e;
+    return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 0, status, stream);
+}
+
+template <int CG, int OUT>
+static int launch_backward(const void* h, const void* w, const LossTargets& targets, const float* lse, void* dh, void* dw, char* scratch,
+                           const LossPlan& p, const LossScratch& at, int T, int N, int V, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw,
+                           unsigned* status, cudaStream_t stream) {
+    const int type = OUT == kOutFp16 ? kMmF16 : kMmBf16;
+    uint16_t* d = reinterpret_cast<uint16_t*>(scratch + at.d);
+    const float *row_scale = reinterpret_cast<float*>(scratch + at.row_scale), *final_scale = reinterpret_cast<float*>(scratch + at.final_scale);
+    int splits = p.h_splits;
+    for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+        const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece);
+        const char* wp = static_cast<const char*>(w) + v0 * ldw * 2;
+        {
+            MmParams<GradEpilogue<OUT>> P = {};
+            P.e = {targets, lse, row_scale, d, p.piece, (int)v0};
+            const int st = mm_launch<CG>(P, type, {h, ldh * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 0, status, stream);
+            if (st != NQ_OK) return st;
+        }
+        if (dw) {
+            MmParams<RowsEpilogue<OUT>> P = {};
+            P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
+            const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, status, stream);
+            if (st != NQ_OK) return st;
+        }
+        if (dh) {
+            MmParams<SumEpilogue> P = {};
+            P.e = {reinterpret_cast<float4*>(scratch + at.sums), p.h_blocks, p.h_quads, v0 > 0};
+            const int st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 0, status, stream);
+            if (st != NQ_OK) return st;
+            if (v0 == 0) splits = P.s.splits;                  // (the last piece may be shorter and have fewer)
+        }
+    }
+    if (dh) {
+        const void* fn = (const void*)dh_kernel<OUT>;
+        const float4* sums = reinterpret_cast<const float4*>(scratch + at.sums);
+        long long ld = lddh;
+        int blocks = p.h_blocks, quads = p.h_quads;
+        void* args[] = {&sums, &final_scale, &dh, &ld, &T, &N, &blocks, &quads, &splits};
+        return launch_plain(fn, dim3((T + 31) / 32, (N + 63) / 64), 256, args, stream);
+    }
+    return NQ_OK;
+}
+
+}  // namespace nq
+
+using namespace nq;
+
+extern "C" {
+
+size_t nq_linear_ce_fwd_scratch_bytes(int64_t T, int64_t N, int64_t V) {
+    if (check_loss(T, N, V, N, N, NQ_F16, NQ_REDUCE_NONE, 64) != NQ_OK) return 0;
+    return (size_t)(up((int64_t)plan_loss(T, N, V).slots * T * 8, 256) + 2 * up(T * 4, 256));
+}
+
+int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int target_bits, int64_t ignore_index, float* loss, float* lse,
+                     float* count, void* scratch, size_t scratch_bytes, void* status_word, int64_t T, int64_t N, int64_t V, int64_t ldh,
+                     int64_t ldw, int reduction, int dtype, nq_stream_t stream) {
+    if (!h || !w || !targets || !loss || !lse || !count || !scratch || !status_word) return NQ_ERR_NULL;
+    int st = check_loss(T, N, V, ldh, ldw, dtype, reduction, target_bits);
+    if (st != NQ_OK) return st;
+    if (!aligned16(h) || !aligned16(w) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
+    if (scratch_bytes < nq_linear_ce_fwd_scratch_bytes(T, N, V)) return NQ_ERR_SCRATCH;
+    cudaStream_t s = as_stream(stream);
+    unsigned* status = static_cast<unsigned*>(status_word) + 2;
+    const LossPlan p = plan_loss(T, N, V);
+    float2* part = static_cast<float2*>(scratch);
+    float* target_logit = reinterpret_cast<float*>(static_cast<char*>(scratch) + up((int64_t)p.slots * T * 8, 256));
+    float* row_loss = reduction == NQ_REDUCE_NONE ? loss : target_logit + up(T * 4, 256) / 4;
+    LossTargets tg = {targets, target_bits == 64, ignore_index};
+    const LseEpilogue::Params e = {tg, part, target_logit};
+    const int type = dtype == NQ_BF16 ? kMmBf16 : kMmF16;
+    st = loss_pairs(T) ? launch_lse<2>(h, w, e, (int)T, (int)N, (int)V, ldh, ldw, type, p.bn, status, s)
+                       : launch_lse<1>(h, w, e, (int)T, (int)N, (int)V, ldh, ldw, type, p.bn, status, s);
+    if (st != NQ_OK) return st;
+    int slots = p.slots, t = (int)T, v = (int)V, mean = reduction == NQ_REDUCE_MEAN;
+    void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v};
+    st = launch_plain((const void*)lse_join_kernel, dim3((unsigned)((T + 31) / 32)), 1024, join_args, s);
+    if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;
+    void* sum_args[] = {&row_loss, &tg, &loss, &count, &t, &mean};
+    return launch_plain((const void*)loss_sum_kernel, dim3(1), 1024, sum_args, s);
+}
+
+size_t nq_linear_ce_bwd_scratch_bytes(int64_t T, int64_t N, int64_t V) {
+    if (check_loss(T, N, V, N, N, NQ_F16, NQ_REDUCE_NONE, 64) != NQ_OK) return 0;
+    return (size_t)loss_scratch(plan_loss(T, N, V), T, N).bytes;
+}
+
+int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int target_bits, int64_t ignore_index, const float* lse,
+                     const float* count, const float* grad_loss, int64_t grad_stride, void* dh, void* dw, void* scratch, size_t scratch_bytes,
+                     void* status_word, int64_t T, int64_t N, int64_t V, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw, int reduction,
+                     int dtype, nq_stream_t stream) {
+    if (!h || !w || !targets || !lse || !count || !grad_loss || !scratch || !status_word) return NQ_ERR_NULL;
+    int st = check_loss(T, N, V, ldh, ldw, dtype, reduction, target_bits);
+    if (st != NQ_OK) return st;
+    if ((dh && (lddh < N || lddh % 8)) || (dw && (lddw < N || lddw % 8))) return NQ_ERR_SHAPE;
+    if (!aligned16(h) || !aligned16(w) || !aligned16(dh) || !aligned16(dw) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
+    if (scratch_bytes < nq_linear_ce_bwd_scratch_bytes(T, N, V)) return NQ_ERR_SCRATCH;
+    if (!dh && !dw) return NQ_OK;
+    cudaStream_t s = as_stream(stream);
+    unsigned* status = static_cast<unsigned*>(status_word) + 2;
+    const LossPlan p = plan_loss(T, N, V);
+    const LossScratch at = loss_scratch(p, T, N);
+    char* base = static_cast<char*>(scratch);
+    LossTargets tg = {targets, target_bits == 64, ignore_index};
+    int t = (int)T, red = reduction, packs = (int)(N / 8);
+    float unit = dtype == NQ_F16 ? kLossHalfScale : 1.f;
+    long long stride = grad_stride, ldp = ldh / 8;
+    float *row_scale = reinterpret_cast<float*>(base + at.row_scale), *final_scale = reinterpret_cast<float*>(base + at.final_scale);
+    void* scale_args[] = {&grad_loss, &stride, &count, &tg, &row_scale, &final_scale, &t, &red, &unit};
+    st = launch_plain((const void*)loss_scales_kernel, dim3(1), 1024, scale_args, s);
+    if (st != NQ_OK) return st;
+    if (dw) {
+        const uint4* hp = static_cast<const uint4*>(h);
+        uint4* hz = reinterpret_cast<uint4*>(base + at.h);
+        void* rows_args[] = {&hp, &hz, &tg, &t, &packs, &ldp};
+        const int64_t ctas = (T * packs + 1023) / 1024, most = 8 * sm_count();
+        st = launch_plain((const void*)loss_rows_kernel, dim3((unsigned)(ctas < most ? ctas : most)), 256, rows_args, s);
+        if (st != NQ_OK) return st;
+    }
+#define NQ_LOSS_BACKWARD(cg, out) launch_backward<cg, out>(h, w, tg, lse, dh, dw, base, p, at, (int)T, (int)N, (int)V, ldh, ldw, lddh, lddw, status, s)
+    if (dtype == NQ_BF16) return loss_pairs(T) ? NQ_LOSS_BACKWARD(2, kOutBf16) : NQ_LOSS_BACKWARD(1, kOutBf16);
+    return loss_pairs(T) ? NQ_LOSS_BACKWARD(2, kOutFp16) : NQ_LOSS_BACKWARD(1, kOutFp16);
+#undef NQ_LOSS_BACKWARD
+}
+
+}  // extern "C"

@@ -1,0 +1,403 @@
+// Products of two dense matrices on the 5th-generation tensor cores, with the epilogue of the operator that needs them:
+//
+//     acc[m, n] = sum_k A[m, k] B[n, k]        16-bit floats with fp32 sums, or signed bytes with int32 sums
+//
+// Either operand may lie with k contiguous (rows of A or B) or with m / n contiguous (the product of a transposed matrix needs no copy).
+//
+// One CTA (CG = 1, 128 rows), or a pair on neighbouring SMs (CG = 2, 256 rows, each CTA holding its half of A and of B), takes tiles
+// t, t + ctas, ... of `bn` columns:
+//
+//   warp 0       operands by TMA, 128 bytes of k per step, 128-byte swizzle
+//   warp 1       MMAs (the pair's first CTA), four per step
+//   warps 4-11   epilogue, two sets of four warps, 32 columns in turn; tensor memory holds two accumulators, so that the epilogue
+//                of a tile runs beside the main loop of the next
+//
+// `bn` is a multiple of 16 up to 256 that the host chooses so that the tiles fill whole rounds of the SMs.  A product over a long k and
+// few tiles is split: `splits` ranges of k are tiles of their own, whose partial sums the operator adds.
+#pragma once
+
+#include "nq_common.cuh"
+#include "nq_tcgen05.cuh"
+
+namespace nq {
+
+constexpr int kMmThreads = 32 * 12, kMmEpilogueWarps = 8;
+constexpr int kMmMaxStages = 8, kMmABytes = 128 * 128, kMmStageOut = 2048;   // (bytes of output staging per epilogue warp)
+constexpr int kMmBarOff = 0, kMmOutOff = 1024, kMmStageOff = kMmOutOff + kMmEpilogueWarps * kMmStageOut;
+constexpr int kMmSmemMost = 226 * 1024;
+constexpr int kMmAccCols = 256;
+
+struct MmShape {
+    int M, N;                      // rows and columns of the result
+    int m_tiles, n_tiles, bn;
+    int ksteps, steps_per_split, splits;
+    int stages, stage_bytes;
+    int m_fast;                    // consecutive tiles share their columns
+    int a_box, b_box;              // K-major: rows per load; MN-major: loads of 64 rows
+    int a_mn, b_mn;                // operand has m / n contiguous
+    int kel;                       // elements of k per step
+    int early_b;                   // B does not depend on the kernel before
+    uint32_t idesc;
+    unsigned wait_limit;
+    unsigned* status;
+};
+
+template <class Epi>
+struct alignas(64) MmParams {
+    CUtensorMap map_a, map_b;
+    MmShape s;
+    typename Epi::Params e;
+};
+
+// MN-major, 128-byte swizzle: 64 elements of m / n per 128-byte row, one row per k; 8-k groups 1024 bytes apart, the next 64 elements 8192.
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr) {
+    const uint32_t lo = ((smem_addr >> 4) & 0x3FFFu) | ((8192u >> 4) << 16);
+    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return ((uint64_t)hi << 32) | lo;
+}
+template <int CG, bool S8>
+__device__ __forceinline__ void mm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+#define NQ_MM_ISSUE(cg, kind)                                                   \
+    asm volatile("{\n\t.reg .pred p;\n\t"                                       \
+                 "setp.ne.b32 p, %4, 0;\n\t"                                    \
+                 "tcgen05.mma.cta_group::" cg ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" \
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory")
+    if constexpr (CG == 2 && S8) NQ_MM_ISSUE("2", "i8");
+    else if constexpr (CG == 2) NQ_MM_ISSUE("2", "f16");
+    else if constexpr (S8) NQ_MM_ISSUE("1", "i8");
+    else NQ_MM_ISSUE("1", "f16");
+#undef NQ_MM_ISSUE
+}
+template <int CG>
+__device__ __forceinline__ void mm_commit(uint32_t bar) {      // the barrier at this offset in every CTA of the group
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+    else
+        tma_load_2d(dst, map, c0, c1, bar);
+}
+// 32 columns of this warp's 32 rows: lane i has row i.
+__device__ __forceinline__ void mm_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"      // (the registers are operands, so that no use moves above it)
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+
+// 32 rows x 32 columns of 16-bit outputs, lane i holding row i as 16 words: through 2 KB of the warp's shared memory, so that four lanes
+// store a row's 64 bytes (whole sectors).  `rows` / `cols` of them exist; `wide`: the rows start at 16-byte boundaries.
+__device__ __forceinline__ void mm_store_rows(unsigned char* stage, const uint32_t (&w)[16], uint16_t* out, long long ld, int rows, int cols, bool wide) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+    if (wide) {
+        const int j = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+            if (r < rows) store_rows(out + r * ld + 8 * j, v, cols - 8 * j, 8 * j + 8 <= cols);
+        }
+    } else if (lane < cols) {
+        const int j = lane >> 3, b = (lane & 7) * 2;
+        for (int r = 0; r < rows; ++r)
+            out[r * ld + lane] = *reinterpret_cast<const uint16_t*>(stage + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + b);
+    }
+}
+
+// Epi: struct Params; kS8; an object per epilogue thread with
+//   Epi(const Params&, const MmShape&)
+//   begin(row, n0, m_tile, n_tile, split, ...)      a tile of this thread's row (row >= M: none)
+//   chunk(r, c, cols, stage)                        32 columns from n0 + c, `cols` of which exist (all lanes call it)
+//   end()
+template <int CG, class Epi>
+__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_kernel(const __grid_constant__ MmParams<Epi> P) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem), bars = sbase + kMmBarOff;
+    const MmShape& S = P.s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto bar_ready = [&](int s) { return bars + 8 * s; };                                  // used in the pair's first CTA
+    auto bar_free = [&](int s) { return bars + 8 * (kMmMaxStages + s); };
+    auto bar_acc_full = [&](int a) { return bars + 8 * (2 * kMmMaxStages + a); };
+    auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * kMmMaxStages + 2 + a); };     // used in the pair's first CTA
+    constexpr int kMisc = kMmBarOff + 8 * (2 * kMmMaxStages + 4);
+    static_assert(kMisc + 8 <= kMmOutOff, "shared memory map");
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kMisc + 4);
+    const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;
+    if (warp == 2) {
+        if (lane < kMmMaxStages) {
+            mbar_init(bar_ready(lane), 1);
+            mbar_init(bar_free(lane), 1);
+        }
+        if (lane < 2) {
+            mbar_init(bar_acc_full(lane), 1);
+            mbar_init(bar_acc_empty(lane), CG * kMmEpilogueWarps);
+        }
+        if (lane == 0) *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem_u32(const_cast<uint32_t*>(tmem_slot))), "r"(2u * kMmAccCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem_u32(const_cast<uint32_t*>(tmem_slot))), "r"(2u * kMmAccCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int groups = (int)gridDim.x / CG, first = (int)blockIdx.x / CG, plane = S.m_tiles * S.n_tiles, tiles = plane * S.splits;
+    struct Tile { int m, n, split, k0, k1; };
+    auto tile_of = [&](int t) {
+        Tile r;
+        r.split = t / plane;
+        const int u = t - r.split * plane;
+        if (S.m_fast) { r.n = u / S.m_tiles; r.m = u - r.n * S.m_tiles; }
+        else { r.m = u / S.n_tiles; r.n = u - r.m * S.n_tiles; }
+        r.k0 = r.split * S.steps_per_split;
+        r.k1 = min(S.ksteps, r.k0 + S.steps_per_split);
+        return r;
+    };
+    const uint32_t a_bytes = (uint32_t)(S.a_mn ? S.a_box * 8192 : S.a_box * 128), b_bytes = (uint32_t)(S.b_mn ? S.b_box * 8192 : S.b_box * 128);
+    const uint32_t stage0 = sbase + kMmStageOff;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- operands
+        auto load_a = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
+            const int m0 = (T.m * CG + rank) * 128;
+            if (S.a_mn) {
+                for (int i = 0; i < S.a_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_a, m0 + 64 * i, k * S.kel, bar);
+            } else {
+                mm_load<CG>(dst, &P.map_a, k * S.kel, m0, bar);
+            }
+        };
+        auto load_b = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
+            const int n0 = T.n * S.bn + rank * (S.bn / CG);
+            if (S.b_mn) {
+                for (int i = 0; i < S.b_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_b, n0 + 64 * i, k * S.kel, bar);
+            } else {
+                mm_load<CG>(dst, &P.map_b, k * S.kel, n0, bar);
+            }
+        };
+        auto ready_bar = [&](int s) { return CG == 2 ? cluster_map(bar_ready(s), 0) : bar_ready(s); };
+        int s = 0, pre = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        if (S.early_b && first < tiles) {      // the first tile's columns while the kernel before still writes the rows
+            const Tile T = tile_of(first);
+            pre = min(S.stages, T.k1 - T.k0);
+            if (elect_one())
+                for (int i = 0; i < pre; ++i) {
+                    if (rank == 0) mbar_expect_tx(bar_ready(i), (uint32_t)CG * (a_bytes + b_bytes));
+                    load_b(T, T.k0 + i, stage0 + (uint32_t)(i * S.stage_bytes) + kMmABytes, ready_bar(i));
+                }
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (pre) {
+            const Tile T = tile_of(first);
+            if (elect_one())
+                for (int i = 0; i < pre; ++i) load_a(T, T.k0 + i, stage0 + (uint32_t)(i * S.stage_bytes), ready_bar(i));
+            s = pre;
+            if (s == S.stages) { s = 0; ph = 1; }
+        }
+        for (int t = first; t < tiles && ok; t += groups) {
+            const Tile T = tile_of(t);
+            for (int k = T.k0 + pre; k < T.k1; ++k) {
+                ok = mbar_wait_warp<CG == 2>(bar_free(s), ph ^ 1, abort_flag, S.status, S.wait_limit);
+                if (!ok) break;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(bar_ready(s), (uint32_t)CG * (a_bytes + b_bytes));
+                    const uint32_t dst = stage0 + (uint32_t)(s * S.stage_bytes), bar = ready_bar(s);
+                    load_a(T, k, dst, bar);
+                    load_b(T, k, dst + kMmABytes, bar);
+                }
+                if (++s == S.stages) { s = 0; ph ^= 1; }
+            }
+            pre = 0;
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issue
+        if (rank == 0) {
+            const uint32_t a_step = S.a_mn ? 2048u >> 4 : 32u >> 4, b_step = S.b_mn ? 2048u >> 4 : 32u >> 4;
+            int s = 0, a = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += groups) {
+                const Tile T = tile_of(t);
+                const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols);
+                ok = mbar_wait_warp<CG == 2>(bar_acc_empty(a), aph ^ 1, abort_flag, S.status, S.wait_limit);
+                tc_fence_after();
+                for (int k = T.k0; k < T.k1 && ok; ++k) {
+                    ok = mbar_wait_warp<CG == 2>(bar_ready(s), ph, abort_flag, S.status, S.wait_limit);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t at = stage0 + (uint32_t)(s * S.stage_bytes), bt = at + kMmABytes;
+                        const uint64_t ad = S.a_mn ? umma_desc_mn(at) : umma_desc(at), bd = S.b_mn ? umma_desc_mn(bt) : umma_desc(bt);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mm_mma<CG, Epi::kS8>(d, ad + (uint64_t)(a_step * i), bd + (uint64_t)(b_step * i), S.idesc, k > T.k0 || i ? 1u : 0u);
+                        mm_commit<CG>(bar_free(s));
+                    }
+                    if (++s == S.stages) { s = 0; ph ^= 1; }
+                }
+                if (ok && elect_one()) mm_commit<CG>(bar_acc_full(a));
+                if (++a == 2) { a = 0; aph ^= 1; }
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------------------------------------------------------- epilogue
+        const int ew = warp & 3, set = (warp - 4) >> 2;
+        unsigned char* stage = smem + kMmOutOff + (warp - 4) * kMmStageOut;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        Epi epi(P.e, S);
+        int a = 0;
+        uint32_t aph = 0;
+        for (int t = first; t < tiles; t += groups) {
+            const Tile T = tile_of(t);
+            const int row = (T.m * CG + rank) * 128 + 32 * ew + lane, n0 = T.n * S.bn, live = min(S.bn, S.N - n0);
+            if (!mbar_wait_warp<CG == 2>(bar_acc_full(a), aph, abort_flag, S.status, S.wait_limit)) break;
+            tc_fence_after();
+            epi.begin(row, n0, set, T.n, T.split);
+            const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
+#pragma unroll 1
+            for (int c = 32 * set; c < live; c += 64) {
+                uint32_t r[32];
+                mm_tmem_ld32(d + (uint32_t)c, r);
+                epi.chunk(r, c, min(32, live - c), stage);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(bar_acc_empty(a), 0)) : "memory");
+                else mbar_arrive(bar_acc_empty(a));
+            }
+            epi.end();
+            if (++a == 2) { a = 0; aph ^= 1; }
+        }
+    }
+    // On an expired wait, give the copies in flight a bounded time to land before shared memory is released.
+    if (*abort_flag && threadIdx.x == 0) {
+        for (unsigned i = 0; i < (1u << 20); ++i) __nanosleep(64);
+    }
+    __syncwarp();
+    tc_fence_before();
+    if constexpr (CG == 2) {
+        // the other CTA may still signal barriers here, and its MMAs and epilogue use the pair's tensor memory
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * kMmAccCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * kMmAccCols) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// One operand: a matrix of `rows` (m or n) and K columns, or its transpose (`mn`: rows of K, `rows` contiguous elements each).
+struct MmOperand {
+    const void* p;
+    int64_t stride;       // bytes between its rows in memory
+    int mn;
+};
+
+// Width of the tiles: the multiple of `unit` up to 256 whose rounds over the `groups` waste least; a step costs its columns, or what the
+// loads of the 128 rows cost where these are more.
+inline int mm_tile_cols(int N, int m_tiles, int groups, int unit, int least) {
+    int best = 0;
+    double best_cost = 0;
+    for (int bn = 256; bn >= least; bn -= unit) {
+        const int64_t tiles = (int64_t)((N + bn - 1) / bn) * m_tiles, rounds = (tiles + groups - 1) / groups;
+        const double cost = (double)rounds * (bn + 16);      // (a tile's fill and drain as 16 columns)
+        if (!best || cost < best_cost * 0.995) { best = bn; best_cost = cost; }
+    }
+    return best;
+}
+
+template <int CG, class Epi>
+int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B, int M, int N, int64_t K, int bn, int splits,
+              int early_b, unsigned* status, cudaStream_t stream) {
+    static bool attr_set[64];
+    int dev = 0;
+    NQ_CUDA_TRY(cudaGetDevice(&dev));
+    const void* fn = (const void*)mm_kernel<CG, Epi>;
+    if (!attr_set[dev & 63]) {
+        NQ_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmemMost));
+        attr_set[dev & 63] = true;
+    }
+    MmShape& S = P.s;
+    const int esize = type == kMmS8 ? 1 : 2;
+    S.M = M; S.N = N; S.bn = bn;
+    S.m_tiles = (M + 128 * CG - 1) / (128 * CG);
+    S.n_tiles = (N + bn - 1) / bn;
+    S.m_fast = S.m_tiles <= S.n_tiles;
+    S.kel = 128 / esize;
+    S.ksteps = (int)((K + S.kel - 1) / S.kel);
+    if (splits > S.ksteps) splits = S.ksteps;
+    S.steps_per_split = (S.ksteps + splits - 1) / splits;
+    S.splits = (S.ksteps + S.steps_per_split - 1) / S.steps_per_split;
+    S.a_mn = A.mn; S.b_mn = B.mn;
+    S.a_box = A.mn ? 2 : CG == 2 || M >= 128 ? 128 : (M + 7) / 8 * 8;
+    S.b_box = B.mn ? bn / CG / 64 : bn / CG;
+    S.stage_bytes = kMmABytes + bn / CG * 128;
+    S.stages = (kMmSmemMost - 1024 - kMmStageOff) / S.stage_bytes;
+    if (S.stages > kMmMaxStages) S.stages = kMmMaxStages;
+    S.early_b = early_b;
+    const uint32_t fmt = type == kMmF16 ? 0u : 1u;           // kind::f16: 1 = bf16; kind::i8: 1 = signed
+    S.idesc = (type == kMmS8 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)A.mn << 15 | (uint32_t)B.mn << 16 |
+              (uint32_t)(bn >> 3) << 17 | (uint32_t)(128 * CG >> 4) << 24;
+    S.wait_limit = gemm_wait_limit();
+    S.status = status;
+    int st = A.mn ? mm_encode(&P.map_a, A.p, type, M, K, A.stride, 64, 64) : mm_encode(&P.map_a, A.p, type, K, M, A.stride, S.kel, S.a_box);
+    if (st != NQ_OK) return st;
+    st = B.mn ? mm_encode(&P.map_b, B.p, type, N, K, B.stride, 64, 64) : mm_encode(&P.map_b, B.p, type, K, N, B.stride, S.kel, S.b_box);
+    if (st != NQ_OK) return st;
+    const int64_t tiles = (int64_t)S.m_tiles * S.n_tiles * S.splits, most = sm_count() / CG;
+    if (tiles > 0x3fffffff) return NQ_ERR_TOO_LARGE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(CG * (tiles < most ? tiles : most)));
+    cfg.blockDim = dim3(kMmThreads);
+    cfg.dynamicSmemBytes = 1024 + kMmStageOff + S.stages * S.stage_bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    void* args[] = {&P};
+    return launch_dependent(cfg, attr, 0, fn, args);
+}
+
+}  // namespace nq

@@ -18,11 +18,15 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/as_strided.h>
+#include <ATen/ops/full.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/ops/zeros_like.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -516,6 +520,313 @@ PyObject* py_dense_gemv_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// behind the last decoder layer: norms, the head in 8 bits, the loss over the head
+// ---------------------------------------------------------------------------------------------------------------
+// A tensor as rows of its last dimension, `ld` elements apart; false: its leading dimensions are not evenly spaced, or the last is not dense.
+bool as_rows(const Tensor& t, int64_t& rows, int64_t& ld) {
+    const int64_t n = t.dim();
+    if (n < 1) return false;
+    const int64_t cols = t.size(n - 1);
+    if (cols > 1 && t.stride(n - 1) != 1) return false;
+    rows = 1;
+    ld = cols;
+    int64_t next = -1;      // stride that the next outer dimension has to have
+    for (int64_t k = n - 2; k >= 0; --k) {
+        if (t.size(k) == 1) continue;
+        if (next < 0) ld = t.stride(k);
+        else if (t.stride(k) != next) return false;
+        next = t.stride(k) * t.size(k);
+        rows *= t.size(k);
+    }
+    return ld >= 0;
+}
+Tensor dense_rows(const Tensor& t) {
+    int64_t rows, ld;
+    Tensor u = t.resolve_neg();
+    return as_rows(u, rows, ld) ? u : u.contiguous();
+}
+nq_stream_t stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+// The header of the device's scratch, whose status word an expired wait sets.
+void* status_header(int dev) {
+    Scratch s = scratch_of(dev);
+    if (!s.ptr) {
+        grow_scratch(dev, 256);
+        s = scratch_of(dev);
+    }
+    return s.ptr;
+}
+Tensor new_bytes(int64_t n, const Tensor& like) { return new_output({n}, like, at::kByte); }
+
+bool capturing(int dev) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(), &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+// A leaf's gradient is accumulated on the stream on which its accumulator was made.  While another graph holds an accumulator made on another
+// stream, a captured backward pass would have that stream wait for the capture, which ends the process: refuse the call instead.
+void check_capture(int dev, std::initializer_list<const Tensor*> inputs) {
+    if (!capturing(dev)) return;
+    const c10::Stream here = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).unwrap();
+    for (const Tensor* t : inputs) {
+        if (!t || !t->defined() || !t->requires_grad() || t->grad_fn()) continue;
+        const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
+        TORCH_CHECK(!acc || !acc->stream() || *acc->stream() == here,
+                    "a leaf of this captured call is held by an autograd graph made on another stream: its gradient cannot be captured; "
+                    "release that graph first, or make it on the capturing stream");
+    }
+}
+
+struct NormArgs {
+    int64_t rows, N;
+    double eps;
+    bool center;
+};
+Tensor norm_launch(const Tensor& x, const Tensor* w, const Tensor* b, const NormArgs& a, Tensor* stats) {
+    int64_t rows, ld;
+    as_rows(x, rows, ld);
+    Tensor y = new_output(x.sizes(), x);
+    if (stats) *stats = new_output({rows, 2}, x, at::kFloat);
+    if (rows * a.N == 0) return y;
+    const int dev = x.get_device(), dt = dtype_id(x.scalar_type());
+    OnDevice on(dev);
+    const int st = nq_norm_fwd(x.const_data_ptr(), w ? w->const_data_ptr() : nullptr, b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(),
+                               stats ? static_cast<float*>(stats->mutable_data_ptr()) : nullptr, rows, a.N, ld, a.N, (float)a.eps, a.center, dt,
+                               w && w->scalar_type() == at::kFloat ? (int)NQ_F32 : dt, stream_of(dev));
+    if (st < 0) fail(st, "nq_norm_fwd");
+    return y;
+}
+struct NormFunction : torch::autograd::Function<NormFunction> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t N, double eps, bool center) {
+        Tensor stats;
+        const NormArgs a{0, N, eps, center};
+        Tensor y = norm_launch(x, w ? &*w : nullptr, b ? &*b : nullptr, a, &stats);
+        ctx->save_for_backward({x, w ? *w : Tensor(), stats});
+        ctx->saved_data["center"] = center;
+        ctx->saved_data["bias"] = b.has_value();
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "the norms are differentiable once");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+        const bool center = ctx->saved_data["center"].toBool(), has_b = ctx->saved_data["bias"].toBool();
+        const bool want_x = ctx->needs_input_grad(0), want_w = w.defined() && ctx->needs_input_grad(1), want_b = has_b && ctx->needs_input_grad(2);
+        Tensor dx, dw, db;
+        int64_t rows, ldx, dy_rows, lddy;
+        as_rows(x, rows, ldx);
+        const int64_t N = x.size(-1);
+        if (grads[0].defined()) {
+            if (want_x) dx = new_output(x.sizes(), x);
+            if (want_w) dw = new_output({N}, w, w.scalar_type());
+            if (want_b) db = new_output({N}, w, w.scalar_type());
+            if (rows * N == 0) {
+                if (want_w) dw.zero_();
+                if (want_b) db.zero_();
+            } else {
+                const Tensor dy = dense_rows(grads[0]);
+                as_rows(dy, dy_rows, lddy);
+                const int dev = x.get_device(), dt = dtype_id(x.scalar_type());
+                OnDevice on(dev);
+                const size_t bytes = nq_norm_bwd_scratch_bytes(rows, N);
+                const Tensor scratch = want_w || want_b ? new_bytes((int64_t)bytes, x) : Tensor();
+                auto ptr = [](Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
+                const int st = nq_norm_bwd(dy.const_data_ptr(), x.const_data_ptr(), w.defined() ? w.const_data_ptr() : nullptr,
+                                           static_cast<const float*>(stats.const_data_ptr()), ptr(dx), ptr(dw), ptr(db),
+                                           scratch.defined() ? scratch.mutable_data_ptr() : nullptr, scratch.defined() ? bytes : 0, rows, N, lddy, ldx, N,
+                                           center, dt, w.defined() && w.scalar_type() == at::kFloat ? (int)NQ_F32 : dt, stream_of(dev));
+                if (st < 0) fail(st, "nq_norm_bwd");
+            }
+        }
+        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// norm(x, weight | None, bias | None, eps, center) -> y or None
+PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 5, "norm takes 5 arguments");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    const Tensor *x = plain(a[0]), *w = a[1] == Py_None ? nullptr : plain(a[1]), *b = a[2] == Py_None ? nullptr : plain(a[2]);
+    int64_t rows, ld;
+    if (!x || (a[1] != Py_None && !w) || (a[2] != Py_None && !b) || (b && !w) || !is_16bit(x->scalar_type()) || !as_rows(*x, rows, ld)) Py_RETURN_NONE;
+    const int64_t N = x->size(-1);
+    for (const Tensor* t : {w, b})
+        if (t && ((t->scalar_type() != x->scalar_type() && t->scalar_type() != at::kFloat) || t->scalar_type() != w->scalar_type() || t->dim() != 1 ||
+                  t->size(0) != N || !t->is_contiguous() || t->get_device() != x->get_device()))
+            Py_RETURN_NONE;
+    const double eps = PyFloat_AsDouble(a[3]);
+    const int center = PyObject_IsTrue(a[4]);
+    if (PyErr_Occurred()) return nullptr;
+    Tensor y;
+    if (at::GradMode::is_enabled() && (x->requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad()))) {
+        check_capture(x->get_device(), {x, w, b});
+        y = NormFunction::apply(*x, w ? OptTensor(*w) : std::nullopt, b ? OptTensor(*b) : std::nullopt, N, eps, center != 0);
+    } else {
+        y = norm_launch(*x, w, b, NormArgs{rows, N, eps, center != 0}, nullptr);
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// quantize_rows(x) -> (q, scale) or None; rows of q start at multiples of 16 bytes
+PyObject* py_quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 1, "quantize_rows takes 1 argument");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    const Tensor* x = plain(a[0]);
+    int64_t rows, ld;
+    if (!x || !is_16bit(x->scalar_type()) || x->dim() < 1 || x->size(-1) == 0 || !as_rows(*x, rows, ld)) Py_RETURN_NONE;
+    const int64_t N = x->size(-1), ldq = (N + 15) / 16 * 16;
+    c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end()), strides(shape.size()), lead(shape.begin(), shape.end() - 1);
+    strides.back() = 1;
+    int64_t step = ldq;
+    for (int k = (int)shape.size() - 2; k >= 0; --k) {
+        strides[k] = step;
+        step *= shape[k];
+    }
+    Tensor buf = new_output({rows, ldq}, *x, at::kChar), scale = new_output(lead, *x, at::kFloat);
+    if (rows > 0) {
+        const int dev = x->get_device();
+        OnDevice on(dev);
+        const int st = nq_quantize_rows_s8(x->const_data_ptr(), static_cast<int8_t*>(buf.mutable_data_ptr()), static_cast<float*>(scale.mutable_data_ptr()),
+                                           rows, N, ld, ldq, dtype_id(x->scalar_type()), stream_of(dev));
+        if (st < 0) fail(st, "nq_quantize_rows_s8");
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    PyObject* q = THPVariable_Wrap(buf.as_strided(shape, strides, 0));
+    PyObject* s = q ? THPVariable_Wrap(scale) : nullptr;
+    return s ? Py_BuildValue("(NN)", q, s) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
+// int8_linear_forward(x, weight, weight_scale, bias | None) -> y or None
+PyObject* py_int8_linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 4, "int8_linear_forward takes 4 arguments");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    const Tensor *x = plain(a[0]), *w = plain(a[1]), *ws = plain(a[2]), *b = a[3] == Py_None ? nullptr : plain(a[3]);
+    int64_t T, ldx;
+    if (!x || !w || !ws || (a[3] != Py_None && !b) || !is_16bit(x->scalar_type()) || w->scalar_type() != at::kChar || ws->scalar_type() != at::kFloat ||
+        w->dim() != 2 || w->size(0) == 0 || w->size(1) == 0 || w->stride(1) != 1 || !as_rows(*x, T, ldx) || x->size(-1) != w->size(1) || ws->dim() != 1 ||
+        ws->size(0) != w->size(0) || !ws->is_contiguous())
+        Py_RETURN_NONE;
+    const int64_t N = w->size(1), V = w->size(0), ldw = w->stride(0);
+    if (b && (b->scalar_type() != x->scalar_type() || b->dim() != 1 || !b->is_contiguous() || b->size(0) != V)) Py_RETURN_NONE;
+    // (one channel: its row stride means nothing)
+    if ((V > 1 && (ldw < N || ldw % 16 != 0)) || (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15) || (reinterpret_cast<uintptr_t>(ws->const_data_ptr()) & 15))
+        Py_RETURN_NONE;
+    const int dev = x->get_device();
+    for (const Tensor* t : {w, ws, b})
+        if (t && t->get_device() != dev) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = V;
+    Tensor y = new_output(shape, *x);
+    if (T == 0) return THPVariable_Wrap(y);
+    OnDevice on(dev);
+    void* status = status_header(dev);
+    const size_t bytes = nq_int8_linear_scratch_bytes(T, N);
+    const Tensor scratch = new_bytes((int64_t)bytes, *x);
+    const int st = nq_int8_linear_fwd(x->const_data_ptr(), static_cast<const int8_t*>(w->const_data_ptr()), static_cast<const float*>(ws->const_data_ptr()),
+                                      b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(), scratch.mutable_data_ptr(), bytes, status, T, N, V, ldx,
+                                      V > 1 ? ldw : (N + 15) / 16 * 16, V, dtype_id(x->scalar_type()), stream_of(dev));
+    if (st < 0) fail(st, "nq_int8_linear_fwd");
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+struct LossArgs {
+    int64_t ignore;
+    int reduction;
+};
+// Rows of a matrix that a stride means nothing for are taken as dense.
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 7) / 8 * 8; }
+// `lse`, `count`: what the backward pass needs.
+Tensor loss_launch(const Tensor& h, const Tensor& w, const Tensor& targets, const LossArgs& a, Tensor& lse, Tensor& count) {
+    const int64_t T = h.size(0), N = h.size(1), V = w.size(0);
+    const bool none = a.reduction == NQ_REDUCE_NONE;
+    lse = new_output({T}, h, at::kFloat);
+    count = new_output({1}, h, at::kFloat);
+    if (T == 0 && !none)
+        return at::full({}, a.reduction == NQ_REDUCE_MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0, lse.options());
+    Tensor loss = none ? new_output({T}, h, at::kFloat) : new_output({}, h, at::kFloat);
+    if (T == 0) return loss;
+    const int dev = h.get_device();
+    OnDevice on(dev);
+    void* status = status_header(dev);
+    const size_t bytes = nq_linear_ce_fwd_scratch_bytes(T, N, V);
+    const Tensor scratch = new_bytes((int64_t)bytes, h);
+    const int st = nq_linear_ce_fwd(h.const_data_ptr(), w.const_data_ptr(), targets.const_data_ptr(), targets.scalar_type() == at::kLong ? 64 : 32, a.ignore,
+                                    static_cast<float*>(loss.mutable_data_ptr()), static_cast<float*>(lse.mutable_data_ptr()),
+                                    static_cast<float*>(count.mutable_data_ptr()), scratch.mutable_data_ptr(), bytes, status, T, N, V, row_stride(h),
+                                    row_stride(w), a.reduction, dtype_id(h.scalar_type()), stream_of(dev));
+    if (st < 0) fail(st, "nq_linear_ce_fwd");
+    return loss;
+}
+struct LossFunction : torch::autograd::Function<LossFunction> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& targets, int64_t ignore, int64_t reduction) {
+        Tensor lse, count;
+        Tensor loss = loss_launch(h, w, targets, LossArgs{ignore, (int)reduction}, lse, count);
+        ctx->save_for_backward({h, w, targets, lse, count});
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy is differentiable once");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &h = saved[0], &w = saved[1], &targets = saved[2], &lse = saved[3], &count = saved[4];
+        const int reduction = (int)ctx->saved_data["reduction"].toInt();
+        Tensor dh, dw;
+        if (grads[0].defined()) {
+            const int64_t T = h.size(0), N = h.size(1), V = w.size(0);
+            if (ctx->needs_input_grad(0)) dh = new_output({T, N}, h);
+            if (ctx->needs_input_grad(1)) dw = T == 0 ? at::zeros({V, N}, w.options()) : new_output({V, N}, w);
+            if (T > 0 && (dh.defined() || dw.defined())) {
+                const Tensor g = grads[0].resolve_neg();
+                const int dev = h.get_device();
+                OnDevice on(dev);
+                void* status = status_header(dev);
+                const size_t bytes = nq_linear_ce_bwd_scratch_bytes(T, N, V);
+                const Tensor scratch = new_bytes((int64_t)bytes, h);
+                const int st = nq_linear_ce_bwd(h.const_data_ptr(), w.const_data_ptr(), targets.const_data_ptr(), targets.scalar_type() == at::kLong ? 64 : 32,
+                                                ctx->saved_data["ignore"].toInt(), static_cast<const float*>(lse.const_data_ptr()),
+                                                static_cast<const float*>(count.const_data_ptr()), static_cast<const float*>(g.const_data_ptr()),
+                                                g.dim() == 1 ? g.stride(0) : 0, dh.defined() ? dh.mutable_data_ptr() : nullptr,
+                                                dw.defined() ? dw.mutable_data_ptr() : nullptr, scratch.mutable_data_ptr(), bytes, status, T, N, V,
+                                                row_stride(h), row_stride(w), N, N, reduction, dtype_id(h.scalar_type()), stream_of(dev));
+                if (st < 0) fail(st, "nq_linear_ce_bwd");
+            }
+        }
+        return {dh, dw, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// linear_cross_entropy(h, weight, targets, ignore_index, reduction) -> loss or None
+PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 5, "linear_cross_entropy takes 5 arguments");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    const Tensor *h = plain(a[0]), *w = plain(a[1]), *t = plain(a[2]);
+    if (!h || !w || !t || !is_16bit(h->scalar_type()) || w->scalar_type() != h->scalar_type() || h->dim() != 2 || w->dim() != 2 || t->dim() != 1 ||
+        (t->scalar_type() != at::kLong && t->scalar_type() != at::kInt) || h->size(1) != w->size(1) || t->size(0) != h->size(0) || !t->is_contiguous() ||
+        h->stride(1) != 1 || w->stride(1) != 1 || w->get_device() != h->get_device() || t->get_device() != h->get_device())
+        Py_RETURN_NONE;
+    for (const Tensor* m : {h, w})
+        if ((reinterpret_cast<uintptr_t>(m->const_data_ptr()) & 15) || row_stride(*m) % 8 != 0 || row_stride(*m) < m->size(1)) Py_RETURN_NONE;
+    const int64_t ignore = PyLong_AsLongLong(a[3]), reduction = PyLong_AsLongLong(a[4]);
+    if (PyErr_Occurred()) return nullptr;
+    Tensor loss;
+    if (at::GradMode::is_enabled() && (h->requires_grad() || w->requires_grad())) {
+        check_capture(h->get_device(), {h, w});
+        loss = LossFunction::apply(*h, *w, *t, ignore, reduction);
+    } else {
+        Tensor lse, count;
+        loss = loss_launch(*h, *w, *t, LossArgs{ignore, (int)reduction}, lse, count);
+    }
+    return THPVariable_Wrap(loss);
+    END_HANDLE_TH_ERRORS
+}
+
 // The pack / layout kernels on a contiguous CUDA tensor.
 enum RepackOp : int { kPackRows, kUnpackRows, kRowsToTiles, kTilesToRows, kPackMarlin };
 Tensor repack(RepackOp op, const Tensor& src, int64_t rows, int64_t cols, int order) {
@@ -635,6 +946,10 @@ PyMethodDef kMethods[] = {
     {"linear_forward", (PyCFunction)(void*)py_linear_forward, METH_FASTCALL, nullptr},
     {"group_forward", (PyCFunction)(void*)py_group_forward, METH_FASTCALL, nullptr},
     {"dense_gemv_forward", (PyCFunction)(void*)py_dense_gemv_forward, METH_FASTCALL, nullptr},
+    {"norm", (PyCFunction)(void*)py_norm, METH_FASTCALL, nullptr},
+    {"quantize_rows", (PyCFunction)(void*)py_quantize_rows, METH_FASTCALL, nullptr},
+    {"int8_linear_forward", (PyCFunction)(void*)py_int8_linear_forward, METH_FASTCALL, nullptr},
+    {"linear_cross_entropy", (PyCFunction)(void*)py_linear_cross_entropy, METH_FASTCALL, nullptr},
     {"repack", (PyCFunction)(void*)py_repack, METH_FASTCALL, nullptr},
     {"pack_rows", (PyCFunction)(void*)py_pack_rows, METH_FASTCALL, nullptr},
     {"words_to", (PyCFunction)(void*)py_words_to, METH_FASTCALL, nullptr},

@@ -228,6 +228,146 @@ def dense_gemv_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     return y.reshape(*x.shape[:-1], V)
 
 
+# --- behind the last decoder layer: norms, the head in 8 bits, the loss over the head ---------------
+
+def _check_16bit(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("Support only Half or BFloat16")
+
+
+def _check_like(t: Optional[torch.Tensor], name: str, like: torch.Tensor, dtypes, shape) -> None:
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, the input on {like.device}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _not_plain(what: str) -> RuntimeError:
+    return RuntimeError(f"{what} takes plain CUDA tensors (no subclasses, no transforms of them)")
+
+
+def _norm(what: str, x, weight, bias, eps: float, center: bool) -> torch.Tensor:
+    y = _lib.ext().norm(x, weight, bias, eps, center)
+    if y is not None:
+        return y
+    _check_16bit(x, "x")
+    if x.dim() < 1:
+        raise RuntimeError("x needs at least one dimension")
+    if bias is not None and weight is None:
+        raise RuntimeError("bias needs a weight")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        _check_like(t, name, x, (x.dtype, torch.float32) if t is weight else (weight.dtype,), (x.size(-1),))
+    # rows that are not evenly spaced, columns that are not dense, lazily negated tensors
+    dense = lambda t: None if t is None else t.resolve_neg().contiguous()
+    y = _lib.ext().norm(dense(x), dense(weight), dense(bias), eps, center)
+    if y is None:
+        raise _not_plain(what)
+    return y
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of fp16 / bf16 ``x`` (``nq_norm_fwd``).
+
+    ``weight`` and ``bias`` ``[N]`` are in the type of ``x`` or fp32, and may be left out (a norm whose weight
+    ``NanoQuantLinear.fold_input_scale`` has taken).  Differentiable once in all three; at most ``nq_norm_max_columns()`` columns."""
+    return _norm("layer_norm", x, weight, bias, eps, True)
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """``x / sqrt(mean(x^2) + eps) * weight``, otherwise as :func:`layer_norm`."""
+    return _norm("rms_norm", x, weight, None, eps, False)
+
+
+def quantize_int8(x: torch.Tensor):
+    """``(q, scale)`` of fp16 / bf16 ``x [..., N]``: signed bytes and one fp32 scale for each row of the last dimension,
+    ``scale = max|x| / 127``, ``q = rint(127 x / max|x|)``.  For the weight of :func:`int8_linear_forward`: rows of ``q`` start at
+    multiples of 16 bytes.  A row with a NaN or an infinity gets a NaN scale."""
+    r = _lib.ext().quantize_rows(x)
+    if r is None:
+        _check_16bit(x, "x")
+        if x.dim() < 1 or x.size(-1) == 0:
+            raise RuntimeError("x needs a last dimension with columns")
+        r = _lib.ext().quantize_rows(x.resolve_neg().contiguous())
+        if r is None:
+            raise _not_plain("quantize_int8")
+    return r
+
+
+def int8_linear_forward(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                        bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``F.linear(x, weight * weight_scale[:, None], bias)`` with ``x`` quantised to signed bytes per token within the call
+    (``nq_int8_linear_fwd``).
+
+    A dense layer in 8 bits, above all the ``lm_head``, which :func:`dense_gemv_forward` streams in 16: ``weight`` ``[V, N]`` int8 with a
+    row stride that is a multiple of 16 and ``weight_scale`` ``[V]`` fp32, both from ``quantize_int8(lm_head.weight)``; ``x`` ``[..., N]``
+    fp16 / bf16 with any number of tokens, ``bias`` ``[V]`` in its type.  Sums are exact, the result is rounded once.  Inference: no
+    gradient.  A token with a NaN or an infinity is NaN in all its outputs."""
+    y = _lib.ext().int8_linear_forward(x, weight, weight_scale, bias)
+    if y is not None:
+        return y
+    _check_16bit(x, "x")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_cuda or weight.dtype != torch.int8:
+        raise RuntimeError("weight must be a CUDA [V, N] matrix of int8")
+    V, N = weight.shape
+    if x.dim() < 1 or x.size(-1) != N:
+        raise RuntimeError(f"x has shape {tuple(x.shape)}, weight expects {N} columns")
+    if V == 0 or N == 0:
+        raise RuntimeError("weight is empty")
+    if weight.device != x.device:
+        raise RuntimeError(f"weight is on {weight.device}, the input on {x.device}")
+    if weight.stride(1) != 1 or (V > 1 and (weight.stride(0) % 16 or weight.stride(0) < N)) or weight.data_ptr() % 16:
+        raise RuntimeError("rows of weight must be dense and start at multiples of 16 bytes (quantize_int8 lays them out so)")
+    _check_like(weight_scale, "weight_scale", x, (torch.float32,), (V,))
+    _check_like(bias, "bias", x, (x.dtype,), (V,))
+    dense = lambda t: None if t is None else t.resolve_neg().contiguous()
+    scale = dense(weight_scale)
+    y = _lib.ext().int8_linear_forward(dense(x), weight, scale if scale.data_ptr() % 16 == 0 else scale.clone(), dense(bias))
+    if y is None:
+        raise _not_plain("int8_linear_forward")
+    return y
+
+
+def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(F.linear(h, weight), targets, ignore_index=..., reduction=...)`` in fp32, without the logits
+    (``nq_linear_ce_fwd`` / ``nq_linear_ce_bwd``).
+
+    ``h`` ``[..., N]`` hidden states and ``weight`` ``[V, N]`` of the head in one type, fp16 or bf16, ``N`` and the row strides multiples
+    of 8; ``targets`` ``[...]`` int64 or int32.  A token whose target is ``ignore_index`` has no loss and no gradient, whatever its row
+    holds; any other target outside ``0..V-1`` makes its loss and gradient NaN (it is not checked on the host).  Returns one fp32 loss, or
+    with ``reduction="none"`` one for each token.  Differentiable once in ``h`` and ``weight``: the backward pass keeps one piece of the
+    vocabulary's gradients at a time (256 MB).  The mean over no tokens is NaN, its gradient zero."""
+    if reduction not in _lib.REDUCTION_ID:
+        raise ValueError(f"reduction should be one of [none, sum, mean], but {reduction} was given")
+    loss = _lib.ext().linear_cross_entropy(h, weight, targets, ignore_index, _lib.REDUCTION_ID[reduction])
+    if loss is not None:
+        return loss
+    _check_16bit(h, "h")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or h.dim() < 1 or h.size(-1) != weight.size(1):
+        raise RuntimeError("weight must be a [V, N] matrix, h [..., N]")
+    V, N = weight.shape
+    _check_like(weight, "weight", h, (h.dtype,), (V, N))
+    _check_like(targets, "targets", h, (torch.int64, torch.int32), h.shape[:-1])
+    if V == 0 or N == 0 or N % 8:
+        raise RuntimeError(f"weight has {V} words and {N} columns: at least one word, and a multiple of 8 columns")
+    dense = lambda t: t if t.dim() == 2 and t.stride(1) == 1 and (t.size(0) == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= N)) and \
+        t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    loss = _lib.ext().linear_cross_entropy(dense(h.resolve_neg().reshape(-1, N)), dense(weight.resolve_neg()),
+                                           targets.resolve_neg().reshape(-1).contiguous(), ignore_index, _lib.REDUCTION_ID[reduction])
+    if loss is None:
+        raise _not_plain("linear_cross_entropy")
+    return loss.reshape(targets.shape) if reduction == "none" else loss
+
+
 def _nanoquant_dyn_forward_cuda(x, scale_g, Ubits, scale_l, Vbits, scale_h,
                                 num_thread_stage1=128, num_thread_stage2=128,
                                 num_row_per_warp_stage1=2, num_row_per_warp_stage2=2,
