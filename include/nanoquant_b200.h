@@ -354,7 +354,7 @@ int nq_dense_gemv_fwd(const void* x, const void* w, const void* bias, void* y, i
 
 /* Layer norm (center != 0) or RMS norm of `rows` rows of N <= nq_norm_max_columns() 16-bit elements, ldx / ldy elements apart:
  *     y = (x - m) r * weight + bias,   m = mean(x) (0 for RMS),   r = 1 / sqrt(mean((x - m)^2) + eps)
- * weight and bias [N] are nullable and of `weight_dtype`: the activations' dtype or NQ_F32.  `stats` (nullable) receives
+ * weight and bias [N] (bias with center only) are nullable and of `weight_dtype`: the activations' dtype or NQ_F32.  `stats` (nullable) receives
  * (m, r) of every row, 2 * rows floats, which the backward pass reads.  fp32 arithmetic, one rounding of y.
  * Any alignment; 16-byte loads where N, ldx and ldy are multiples of 8 and the pointers 16-byte aligned.
  * No counterpart in the reference (its models' norms are torch's). */

@@ -5,18 +5,21 @@
 //     dw = sum_rows dy xhat        db = sum_rows dy
 //
 // Bound by memory: forward 2 bytes in and 2 out per element, backward 4 in and 2 out.  Every element is read once: a group of warps
-// holds a row in registers (the mean, then the sum of squares of the differences, all in fp32, cost no second read).  Groups are sized by
-// the row, and for few rows a thread takes fewer columns, so that one token's row is a single load per thread.
+// holds a row in registers (the mean, then the sum of squares of the differences, all in fp32, cost no second read).
 //
-// Backward.  A group takes rows `first, first + groups, ...`; a thread has the same columns of each and adds dy xhat and dy to fp32 sums
-// in registers.  One row of partial sums per CTA goes to the scratch; a second kernel adds these in a fixed order, so results do not
-// depend on timing.
+//   stream kernels   many rows at 16-byte boundaries.  As many CTAs as fit the SMs, each of one group or more; a group takes rows first, first +
+//                    groups, ...  A thread has the same columns of every row and copies the next rows' into its own part of shared memory
+//                    (cp.async), so that loads stay in flight across the reductions of a row, and no thread waits for another's copies.
+//   direct kernels   few rows (a CTA each, one load a thread: latency) and rows at any address (single elements).
+//
+// Backward: a thread adds dy xhat and dy of its columns to fp32 sums in registers.  One row of partial sums per CTA goes to the scratch; a
+// second kernel adds these in a fixed order, so results do not depend on timing.
 #include "nq_common.cuh"
 
 namespace nq {
 
 constexpr int kNormMaxCols = 16384;
-constexpr int kNormCtasPerSm = 4;          // of the backward kernel at most: rows of partial sums per SM
+constexpr int kNormCtasPerSm = 8;          // of the backward kernels at most: rows of partial sums per SM
 
 struct NormParams {
     const void *x, *w, *b, *dy;
@@ -250,10 +253,440 @@ __global__ void __launch_bounds__(32 * WARPS * norm_rows_per_cta<WARPS>()) norm_
     if (P.part_b) put(P.part_b, ab);
 }
 
-// out[c] = sum over the CTAs of part[i][c]: 32 columns a CTA, eight warps over the rows, then over the warps.
+// ---------------------------------------------------------------------------
+// stream kernels
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void norm_copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void norm_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void norm_copies_landed() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ uint4 norm_shared(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// Two fp32 numbers in one 64-bit register, and the instructions that work on both: with one element at a time the stream kernels were bound by
+// instruction issue (16384 x 5120: 28 instructions per element forward, 34 backward).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 template <bool BF16>
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* part_w, const float* part_b, void* dw, void* db, int ctas, int N, int w32) {
-    __shared__ float red[8][32];
+__device__ __forceinline__ f32x2 unpack2(uint32_t w) {
+    if constexpr (BF16) return pair2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pair2(f.x, f.y);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t repack2(f32x2 v) {
+    const float2 f = split2(v);
+    return norm_pack<BF16>(f.x, f.y);
+}
+// Weights of eight columns.
+template <bool BF16>
+__device__ __forceinline__ void weights2(const void* p, int w32, int c, f32x2 (&w)[4]) {
+    if (w32) {
+        const float4 *q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + c), a = q[0], b = q[1];
+        w[0] = pair2(a.x, a.y); w[1] = pair2(a.z, a.w); w[2] = pair2(b.x, b.y); w[3] = pair2(b.z, b.w);
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + c);
+        w[0] = unpack2<BF16>(v.x); w[1] = unpack2<BF16>(v.y); w[2] = unpack2<BF16>(v.z); w[3] = unpack2<BF16>(v.w);
+    }
+}
+// A group of G threads (whole warps) per batch of a few rows.  A batch's rows are all read for their sums, one exchange between the group's
+// warps serves all of them, and they are read again for the outputs; each time from shared memory, by the thread that copied them (cp.async).  The next
+// batch is on its way meanwhile.  16384 x 5120, layer norm, us: a row at a time 97 forward and 200 backward (waiting for reductions); batches with
+// addresses computed for every access 78 and 105 (20 and 30 instructions per element); rows PITCH bytes apart in shared memory, PITCH a constant, and
+// sums of several rows in one butterfly 59 and 90 (5.6 TB/s; RMS 60 and 83).
+template <int PITCH, bool BWD>
+struct NormShape {
+    static constexpr int kPacks = PITCH <= 4096 || (BWD && PITCH <= 10240) ? 1 : PITCH <= 16384 ? 2 : 4;      // times eight columns a thread
+    static constexpr int kRows = BWD ? (PITCH <= 10240 ? 4 : PITCH <= 16384 ? 2 : 1) : PITCH <= 16384 ? 4 : 2;
+    static constexpr int kThreads = PITCH <= 4096 ? 256 : PITCH / 16 / kPacks;                               // of a CTA at most
+    static constexpr int kCtas = BWD ? (PITCH <= 4096 ? 3 : 1) : PITCH <= 8192 ? 3 : PITCH <= 10240 ? 2 : 1;  // to an SM at least (registers)
+    static constexpr int kSlot = (BWD ? 2 : 1) * PITCH;                                                        // bytes of a row (x, then dy)
+    static constexpr int kGroupBytes = 2 * kRows * kSlot;
+};
+// Sums over the warp of NUM numbers, a power of two up to 8; lane i has number i / (32 / NUM).
+template <int NUM>
+__device__ __forceinline__ float warp_sums(const float (&v)[NUM]) {
+    const int lane = threadIdx.x & 31;
+    float t[NUM];
+#pragma unroll
+    for (int i = 0; i < NUM; ++i) t[i] = v[i];
+    int o = 16;
+#pragma unroll
+    for (int n = NUM; n > 1; n >>= 1, o >>= 1) {          // half of the numbers to either half of the lanes
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) {
+            const float keep = upper ? t[i + n / 2] : t[i], give = upper ? t[i] : t[i + n / 2];
+            t[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+#pragma unroll
+    for (; o > 0; o >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
+    return t[0];
+}
+struct NormGroup {
+    int G, id, tid, lane, warps;
+    float* red;
+    __device__ NormGroup(float (*red_)[2][8], int G_) : G(G_) {
+        id = threadIdx.x / G;
+        tid = threadIdx.x - id * G;
+        lane = threadIdx.x & 31;
+        warps = G >> 5;
+        red = &red_[id * warps][0][0];
+    }
+    // NUM numbers of every warp (as warp_sums leaves them) at OFF for all of the group to read, those of warp i at 16 i.
+    template <int NUM>
+    __device__ __forceinline__ void put(float v, int off, int parity) {
+        if ((lane & (32 / NUM - 1)) == 0) red[(tid >> 5) * 16 + 8 * parity + off + lane / (32 / NUM)] = v;
+    }
+    __device__ __forceinline__ void sync() { asm volatile("bar.sync %0, %1;" ::"r"(1 + id), "r"(G) : "memory"); }
+};
+__device__ __forceinline__ void unpack8(const uint4& v, uint32_t (&w)[4]) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+
+template <int PITCH, bool BF16, bool CENTER>
+__global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<PITCH, false>::kCtas) norm_fwd_stream_kernel(const NormParams P, int G) {
+    using Shape = NormShape<PITCH, false>;
+    constexpr int PACKS = Shape::kPacks, ROWS = Shape::kRows;
+    extern __shared__ __align__(16) unsigned char norm_smem[];
+    __shared__ float red[Shape::kThreads / 32][2][8];     // (two halves in turn, so that one barrier a batch is enough)
+    NormGroup g(red, G);
+    const int packs = P.N >> 3, groups = blockDim.x / G;
+    const long long batches = (P.rows + ROWS - 1) / ROWS, step = (long long)gridDim.x * groups, first = (long long)blockIdx.x * groups + g.id;
+    const uint32_t mine = smem_u32(norm_smem) + (uint32_t)(g.id * Shape::kGroupBytes + g.tid * 16);
+    auto live = [&](int p) { return p * G + g.tid < packs; };
+    const long long ldx = 2 * P.ldx, ldy = 2 * P.ldy, next_x = step * ROWS * ldx, next_y = step * ROWS * ldy;     // bytes
+    const char* x = static_cast<const char*>(P.x) + first * ROWS * ldx + g.tid * 16;          // of the next batch to be copied
+    char* y = static_cast<char*>(P.y) + first * ROWS * ldy + g.tid * 16;
+    long long ahead = first;                              // that batch
+    auto copy = [&](int stage) {
+        if (ahead < batches) {
+            const char* src = x;
+            const uint32_t dst = mine + (uint32_t)(stage * ROWS * PITCH);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                if (r == 0 || ahead * ROWS + r < P.rows) {
+#pragma unroll
+                    for (int p = 0; p < PACKS; ++p)
+                        if (live(p)) norm_copy16(dst + (uint32_t)(p * G * 16) + r * PITCH, src + p * G * 16);
+                }
+                src += ldx;
+            }
+        }
+        x += next_x;
+        ahead += step;
+        norm_commit();
+    };
+    auto count = [&](int warp) {                          // columns of a warp of the group (eight at least)
+        int n = 0;
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) n += max(0, min(32, packs - p * G - 32 * warp));
+        return 8.f * n;
+    };
+    const float inv_own = 1.f / count(g.tid >> 5);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    copy(0);
+    copy(1);
+    f32x2 w[PACKS][4], b[PACKS][4];                       // of the thread's columns, for all rows
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            w[p][k] = pair2(1.f, 1.f);
+            b[p][k] = 0;
+        }
+        if (live(p) && P.w) weights2<BF16>(P.w, P.w32, (p * G + g.tid) * 8, w[p]);
+        if (CENTER && live(p) && P.b) weights2<BF16>(P.b, P.w32, (p * G + g.tid) * 8, b[p]);
+    }
+    int stage = 0;
+    for (long long batch = first; batch < batches; batch += step, y += next_y) {
+        const int rows = (int)min((long long)ROWS, P.rows - batch * ROWS);
+        uint32_t at[PACKS];
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) at[p] = mine + (uint32_t)(stage * ROWS * PITCH + p * G * 16);
+        norm_copies_landed<1>();
+        // Layer norm: each warp's own mean and squares of the differences from it, then those of all warps, so that one exchange is enough and no
+        // small difference of large sums is taken: sum (x - m)^2 = sum_w [sum (x - m_w)^2 + n_w (m_w - m)^2].
+        float v[ROWS], own = 0.f;                         // own: of row lane / (32 / ROWS)
+        if constexpr (CENTER) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                f32x2 s = 0;
+#pragma unroll
+                for (int p = 0; p < PACKS; ++p)
+                    if (live(p)) {
+                        uint32_t xw[4];
+                        unpack8(norm_shared(at[p] + r * PITCH), xw);
+                        s = add2(s, add2(add2(unpack2<BF16>(xw[0]), unpack2<BF16>(xw[1])), add2(unpack2<BF16>(xw[2]), unpack2<BF16>(xw[3]))));
+                    }
+                v[r] = split2(s).x + split2(s).y;
+            }
+            own = warp_sums(v) * inv_own;
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            f32x2 s = 0, shift = 0;
+            if constexpr (CENTER) {
+                const float m = -__shfl_sync(0xffffffffu, own, r * (32 / ROWS));
+                shift = pair2(m, m);
+            }
+#pragma unroll
+            for (int p = 0; p < PACKS; ++p)
+                if (live(p)) {
+                    uint32_t xw[4];
+                    unpack8(norm_shared(at[p] + r * PITCH), xw);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const f32x2 d = CENTER ? add2(unpack2<BF16>(xw[k]), shift) : unpack2<BF16>(xw[k]);
+                        s = fma2(d, d, s);
+                    }
+                }
+            v[r] = split2(s).x + split2(s).y;
+        }
+        float squares = warp_sums(v), mean = own;
+        if (g.warps > 1) {
+            g.put<ROWS>(squares, 0, stage);
+            if constexpr (CENTER) g.put<ROWS>(own, ROWS, stage);
+            g.sync();
+            const float* all = g.red + 8 * stage + g.lane / (32 / ROWS);      // of the lane's row; its lanes share the warps
+            auto join = [](float t) {
+#pragma unroll
+                for (int o = 16 / ROWS; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                return t;
+            };
+            mean = squares = 0.f;
+            const int i0 = g.lane & (32 / ROWS - 1);
+            if constexpr (CENTER) {
+                for (int i = i0; i < g.warps; i += 32 / ROWS) mean = fmaf(count(i), all[16 * i + ROWS], mean);
+                mean = join(mean) * P.inv_n;
+                for (int i = i0; i < g.warps; i += 32 / ROWS) {
+                    const float d = all[16 * i + ROWS] - mean;
+                    squares += fmaf(count(i) * d, d, all[16 * i]);
+                }
+            } else {
+                for (int i = i0; i < g.warps; i += 32 / ROWS) squares += all[16 * i];
+            }
+            squares = join(squares);
+        }
+        const float rstd = 1.f / sqrtf(squares * P.inv_n + P.eps);
+        if (P.stats && g.tid < 32 && (g.lane & (32 / ROWS - 1)) == 0 && g.lane / (32 / ROWS) < rows)
+            P.stats[batch * ROWS + g.lane / (32 / ROWS)] = make_float2(mean, rstd);
+        char* dst = y;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const float rs = __shfl_sync(0xffffffffu, rstd, r * (32 / ROWS)), ms = CENTER ? -rs * __shfl_sync(0xffffffffu, mean, r * (32 / ROWS)) : 0.f;
+            const f32x2 r2 = pair2(rs, rs), shift = pair2(ms, ms);
+            if (r < rows) {
+#pragma unroll
+                for (int p = 0; p < PACKS; ++p)
+                    if (live(p)) {
+                        uint32_t xw[4];
+                        unpack8(norm_shared(at[p] + r * PITCH), xw);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            xw[k] = repack2<BF16>(CENTER ? fma2(fma2(unpack2<BF16>(xw[k]), r2, shift), w[p][k], b[p][k]) : mul2(mul2(unpack2<BF16>(xw[k]), r2), w[p][k]));
+                        *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+                    }
+            }
+            dst += ldy;
+        }
+        copy(stage);
+        stage ^= 1;
+    }
+}
+
+template <int PITCH, bool BF16, bool CENTER>
+__global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PITCH, true>::kCtas) norm_bwd_stream_kernel(const NormParams P, int G) {
+    using Shape = NormShape<PITCH, true>;
+    constexpr int PACKS = Shape::kPacks, ROWS = Shape::kRows, kSlot = Shape::kSlot;
+    constexpr int kSums = CENTER ? 2 * ROWS : ROWS;       // of g xhat, and of g
+    extern __shared__ __align__(16) unsigned char norm_smem[];
+    __shared__ float red[Shape::kThreads / 32][2][8];     // (two halves in turn, so that one barrier a batch is enough)
+    NormGroup g(red, G);
+    const int packs = P.N >> 3, groups = blockDim.x / G, tid = g.tid, lane = g.lane;
+    const long long batches = (P.rows + ROWS - 1) / ROWS, step = (long long)gridDim.x * groups, first = (long long)blockIdx.x * groups + g.id;
+    const uint32_t mine = smem_u32(norm_smem) + (uint32_t)(g.id * Shape::kGroupBytes + tid * 16);
+    auto live = [&](int p) { return p * G + tid < packs; };
+    const long long ldx = 2 * P.ldx, lddy = 2 * P.lddy, lddx = 2 * P.ldy, next_x = step * ROWS * ldx, next_dy = step * ROWS * lddy, next_dx = step * ROWS * lddx;
+    const char *x = static_cast<const char*>(P.x) + first * ROWS * ldx + tid * 16, *dy = static_cast<const char*>(P.dy) + first * ROWS * lddy + tid * 16;
+    char* dx = static_cast<char*>(P.y) + first * ROWS * lddx + tid * 16;
+    long long ahead = first;                              // the next batch to be copied
+    auto copy = [&](int stage) {
+        if (ahead < batches) {
+            const char *sx = x, *sd = dy;
+            const uint32_t dst = mine + (uint32_t)(stage * ROWS * kSlot);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                if (r == 0 || ahead * ROWS + r < P.rows) {
+#pragma unroll
+                    for (int p = 0; p < PACKS; ++p)
+                        if (live(p)) {
+                            norm_copy16(dst + (uint32_t)(p * G * 16) + r * kSlot, sx + p * G * 16);
+                            norm_copy16(dst + (uint32_t)(p * G * 16) + r * kSlot + PITCH, sd + p * G * 16);
+                        }
+                }
+                sx += ldx;
+                sd += lddy;
+            }
+        }
+        x += next_x;
+        dy += next_dy;
+        ahead += step;
+        norm_commit();
+    };
+    // mean and 1 / sigma of row `lane` of a batch
+    auto load_stats = [&](long long batch) {
+        return lane < ROWS && batch * ROWS + lane < P.rows ? __ldg(P.stats + batch * ROWS + lane) : make_float2(0.f, 0.f);
+    };
+    f32x2 aw[PACKS][4], ab[PACKS][4], w[PACKS][4];
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            aw[p][k] = ab[p][k] = 0;
+            w[p][k] = pair2(1.f, 1.f);
+        }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    copy(0);
+    copy(1);
+    float2 next = load_stats(first);
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p)
+        if (P.w && live(p)) weights2<BF16>(P.w, P.w32, (p * G + tid) * 8, w[p]);
+    int stage = 0;
+    for (long long batch = first; batch < batches; batch += step, dx += next_dx) {
+        const int rows = (int)min((long long)ROWS, P.rows - batch * ROWS);
+        const float rstd = next.y, shift = -next.x * next.y;       // of row `lane`
+        next = load_stats(batch + step);
+        uint32_t at[PACKS];
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) at[p] = mine + (uint32_t)(stage * ROWS * kSlot + p * G * 16);
+        norm_copies_landed<1>();
+        float sums[kSums];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const float r1 = __shfl_sync(0xffffffffu, rstd, r), s1 = __shfl_sync(0xffffffffu, shift, r);
+            const f32x2 r2 = pair2(r1, r1), s2 = pair2(s1, s1);
+            f32x2 sx = 0, sg = 0;
+            if (r < rows) {
+#pragma unroll
+                for (int p = 0; p < PACKS; ++p)
+                    if (live(p)) {
+                        uint32_t xw[4], dw[4];
+                        unpack8(norm_shared(at[p] + r * kSlot), xw);
+                        unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const f32x2 xh = fma2(unpack2<BF16>(xw[k]), r2, s2), d = unpack2<BF16>(dw[k]), gr = mul2(d, w[p][k]);
+                            sx = fma2(gr, xh, sx);
+                            aw[p][k] = fma2(d, xh, aw[p][k]);
+                            if constexpr (CENTER) {
+                                sg = add2(sg, gr);
+                                ab[p][k] = add2(ab[p][k], d);
+                            }
+                        }
+                    }
+            }
+            sums[r] = split2(sx).x + split2(sx).y;
+            if constexpr (CENTER) sums[ROWS + r] = split2(sg).x + split2(sg).y;
+        }
+        if (P.y) {
+            float total = warp_sums(sums);                // number lane / (32 / kSums)
+            if (g.warps > 1) {
+                g.put<kSums>(total, 0, stage);
+                g.sync();
+                const float* all = g.red + 8 * stage + lane / (32 / kSums);
+                total = 0.f;
+                for (int i = lane & (32 / kSums - 1); i < g.warps; i += 32 / kSums) total += all[16 * i];
+#pragma unroll
+                for (int o = 16 / kSums; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            }
+            total *= -P.inv_n;
+            char* dst = dx;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const float r1 = __shfl_sync(0xffffffffu, rstd, r), s1 = __shfl_sync(0xffffffffu, shift, r);
+                // dx = r g - (r mean(g)) - xhat (r mean(g xhat))
+                const float c1 = r1 * __shfl_sync(0xffffffffu, total, r * (32 / kSums)), c2 = CENTER ? r1 * __shfl_sync(0xffffffffu, total, (ROWS + r) * (32 / kSums)) : 0.f;
+                const f32x2 r2 = pair2(r1, r1), s2 = pair2(s1, s1), c1p = pair2(c1, c1), c2p = pair2(c2, c2);
+                if (r < rows) {
+#pragma unroll
+                    for (int p = 0; p < PACKS; ++p)
+                        if (live(p)) {
+                            uint32_t xw[4], dw[4];
+                            unpack8(norm_shared(at[p] + r * kSlot), xw);
+                            unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const f32x2 xh = fma2(unpack2<BF16>(xw[k]), r2, s2);
+                                xw[k] = repack2<BF16>(fma2(mul2(unpack2<BF16>(dw[k]), w[p][k]), r2, fma2(xh, c1p, c2p)));
+                            }
+                            *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+                        }
+                }
+                dst += lddx;
+            }
+        }
+        copy(stage);
+        stage ^= 1;
+    }
+    // One row of partial sums per CTA: the groups' in turn, in shared memory over the copies' (which have all landed and been read).
+    norm_copies_landed<0>();
+    float* sums = reinterpret_cast<float*>(norm_smem);
+    auto put = [&](float* part, const f32x2 (&a)[PACKS][4]) {
+        float* dst = part + (size_t)blockIdx.x * P.N;
+        for (int r = 0; r < groups; ++r) {
+            __syncthreads();
+            if (g.id == r) {
+#pragma unroll
+                for (int p = 0; p < PACKS; ++p) {
+                    const int c = (p * G + tid) * 8;
+                    if (live(p)) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const f32x2 v = r ? add2(a[p][k], *reinterpret_cast<const f32x2*>(sums + c + 2 * k)) : a[p][k];
+                            *reinterpret_cast<f32x2*>((r + 1 < groups ? sums : dst) + c + 2 * k) = v;
+                        }
+                    }
+                }
+            }
+        }
+    };
+    if (P.part_w) put(P.part_w, aw);
+    if (P.part_b) put(P.part_b, ab);
+}
+
+// out[c] = sum over the CTAs of part[i][c]: 32 columns a CTA, 32 warps over the rows (so that a warp's few loads are one round trip), then over the warps.
+template <bool BF16>
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* part_w, const float* part_b, void* dw, void* db, int ctas, int N, int w32) {
+    __shared__ float red[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float* part = blockIdx.y ? part_b : part_w;
@@ -261,16 +694,18 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const float* part_w, c
     if (!out) return;
     float s = 0.f;
     if (c < N) {
-#pragma unroll 4
-        for (int i = warp; i < ctas; i += 8) s += part[(size_t)i * N + c];
+#pragma unroll 8
+        for (int i = warp; i < ctas; i += 32) s += __ldcg(part + (size_t)i * N + c);
     }
     red[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < N) {
+    s = red[lane][warp];                   // warp w: column w
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += red[k][lane];
-        if (w32) static_cast<float*>(out)[c] = s;
-        else static_cast<uint16_t*>(out)[c] = (uint16_t)norm_pack<BF16>(s, 0.f);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int col = blockIdx.x * 32 + warp;
+    if (lane == 0 && col < N) {
+        if (w32) static_cast<float*>(out)[col] = s;
+        else static_cast<uint16_t*>(out)[col] = (uint16_t)norm_pack<BF16>(s, 0.f);
     }
 }
 
@@ -305,6 +740,57 @@ NormVariant choose_norm(bool bwd, bool bf16, bool center, bool vec, long long ro
     if (N <= 4096) return norm_variant<1, 8, 16>(bwd, bf16, center);
     return norm_variant<1, 32, 16>(bwd, bf16, center);
 }
+// How a stream kernel is launched.
+struct NormStream {
+    const void* fn;
+    int threads, smem, G, rows;
+    int64_t ctas;
+};
+template <int PITCH>
+NormStream norm_stream(bool bwd, bool bf16, bool center, int N) {
+    NormStream v = {};
+    if (bwd) v.fn = bf16 ? (center ? (const void*)norm_bwd_stream_kernel<PITCH, true, true> : (const void*)norm_bwd_stream_kernel<PITCH, true, false>)
+                         : (center ? (const void*)norm_bwd_stream_kernel<PITCH, false, true> : (const void*)norm_bwd_stream_kernel<PITCH, false, false>);
+    else v.fn = bf16 ? (center ? (const void*)norm_fwd_stream_kernel<PITCH, true, true> : (const void*)norm_fwd_stream_kernel<PITCH, true, false>)
+                     : (center ? (const void*)norm_fwd_stream_kernel<PITCH, false, true> : (const void*)norm_fwd_stream_kernel<PITCH, false, false>);
+    const int per = bwd ? NormShape<PITCH, true>::kPacks : NormShape<PITCH, false>::kPacks;
+    v.G = (N / 8 + 32 * per - 1) / (32 * per) * 32;
+    const int groups = v.G >= 256 ? 1 : 256 / v.G;
+    v.threads = groups * v.G;
+    v.smem = groups * (bwd ? NormShape<PITCH, true>::kGroupBytes : NormShape<PITCH, false>::kGroupBytes);
+    v.rows = groups * (bwd ? NormShape<PITCH, true>::kRows : NormShape<PITCH, false>::kRows);
+    return v;
+}
+int choose_stream(bool bwd, bool bf16, bool center, const NormParams& P, NormStream& v) {
+    const int N = P.N;
+    v = N <= 256    ? norm_stream<512>(bwd, bf16, center, N)
+        : N <= 512  ? norm_stream<1024>(bwd, bf16, center, N)
+        : N <= 1024 ? norm_stream<2048>(bwd, bf16, center, N)
+        : N <= 2048 ? norm_stream<4096>(bwd, bf16, center, N)
+        : N <= 4096 ? norm_stream<8192>(bwd, bf16, center, N)
+        : N <= 5120 ? norm_stream<10240>(bwd, bf16, center, N)
+        : N <= 8192 ? norm_stream<16384>(bwd, bf16, center, N)
+                    : norm_stream<32768>(bwd, bf16, center, N);
+    NQ_CUDA_TRY(cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem));
+    int per_sm = 1;
+    NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.fn, v.threads, v.smem));
+    per_sm = per_sm < 1 ? 1 : per_sm > kNormCtasPerSm ? kNormCtasPerSm : per_sm;
+    const int64_t units = (P.rows + v.rows - 1) / v.rows;
+    v.ctas = units < (int64_t)per_sm * sm_count() ? units : (int64_t)per_sm * sm_count();
+    return NQ_OK;
+}
+int launch_stream(const NormStream& v, const NormParams& P, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)v.ctas);
+    cfg.blockDim = dim3(v.threads);
+    cfg.dynamicSmemBytes = v.smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    NormParams p = P;
+    int G = v.G;
+    void* args[] = {&p, &G};
+    return launch_dependent(cfg, attr, 0, v.fn, args);
+}
 int launch_norm(const NormVariant& v, long long ctas, const NormParams& P, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
@@ -332,11 +818,17 @@ int nq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, fl
     if (weight_dtype != dtype && weight_dtype != NQ_F32) return NQ_ERR_DTYPE;
     if (rows < 1 || N < 1 || ldx < 0 || ldy < N) return NQ_ERR_SHAPE;
     if (N > kNormMaxCols || rows > 0x7fffffff) return NQ_ERR_TOO_LARGE;
+    if (bias && !center) return NQ_ERR_UNSUPPORTED;
     NormParams P = {};
     P.x = x; P.w = weight; P.b = bias; P.y = y; P.stats = reinterpret_cast<float2*>(stats);
     P.rows = rows; P.ldx = ldx; P.ldy = ldy; P.N = (int)N; P.w32 = weight_dtype == NQ_F32;
     P.eps = eps; P.inv_n = 1.f / (float)N;
     const bool vec = N % 8 == 0 && norm_rows_aligned(x, ldx) && norm_rows_aligned(y, ldy) && aligned16(weight) && aligned16(bias);
+    if (vec && rows > 2 * sm_count()) {
+        NormStream v = {};
+        const int st = choose_stream(false, dtype == NQ_BF16, center != 0, P, v);
+        return st != NQ_OK ? st : launch_stream(v, P, as_stream(stream));
+    }
     const NormVariant v = choose_norm(false, dtype == NQ_BF16, center != 0, vec, rows, (int)N);
     return launch_norm(v, (rows + v.rows_per_cta - 1) / v.rows_per_cta, P, as_stream(stream));
 }
@@ -355,6 +847,7 @@ int nq_norm_bwd(const void* dy, const void* x, const void* weight, const float* 
     if (weight_dtype != dtype && weight_dtype != NQ_F32) return NQ_ERR_DTYPE;
     if (rows < 1 || N < 1 || ldx < 0 || lddy < 0 || (dx && lddx < N)) return NQ_ERR_SHAPE;
     if (N > kNormMaxCols || rows > 0x7fffffff) return NQ_ERR_TOO_LARGE;
+    if (dbias && !center) return NQ_ERR_UNSUPPORTED;
     if (!dx && !dweight && !dbias) return NQ_OK;
     const bool sums = dweight || dbias;
     if (sums && !scratch) return NQ_ERR_NULL;
@@ -363,24 +856,34 @@ int nq_norm_bwd(const void* dy, const void* x, const void* weight, const float* 
     const bool bf16 = dtype == NQ_BF16;
     const bool vec = N % 8 == 0 && norm_rows_aligned(x, ldx) && norm_rows_aligned(dy, lddy) && (!dx || norm_rows_aligned(dx, lddx)) &&
                      aligned16(weight);
-    const NormVariant v = choose_norm(true, bf16, center != 0, vec, rows, (int)N);
-    int per_sm = 0;
-    NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, (const void*)v.fn, v.threads, 0));
-    per_sm = per_sm < 1 ? 1 : per_sm > kNormCtasPerSm ? kNormCtasPerSm : per_sm;
-    int64_t ctas = (rows + v.rows_per_cta - 1) / v.rows_per_cta;
-    if (ctas > (int64_t)per_sm * sm_count()) ctas = (int64_t)per_sm * sm_count();
+    const bool streamed = vec && rows > 2 * sm_count();
     NormParams P = {};
     P.x = x; P.w = weight; P.dy = dy; P.y = dx; P.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+    P.rows = rows; P.ldx = ldx; P.lddy = lddy; P.ldy = lddx; P.N = (int)N; P.w32 = weight_dtype == NQ_F32;
+    NormVariant v = {};
+    NormStream sv = {};
+    int64_t ctas = 0;
+    if (streamed) {
+        const int st = choose_stream(true, bf16, center != 0, P, sv);
+        if (st != NQ_OK) return st;
+        ctas = sv.ctas;
+    } else {
+        v = choose_norm(true, bf16, center != 0, vec, rows, (int)N);
+        int per_sm = 0;
+        NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, (const void*)v.fn, v.threads, 0));
+        per_sm = per_sm < 1 ? 1 : per_sm > kNormCtasPerSm ? kNormCtasPerSm : per_sm;
+        ctas = (rows + v.rows_per_cta - 1) / v.rows_per_cta;
+        if (ctas > (int64_t)per_sm * sm_count()) ctas = (int64_t)per_sm * sm_count();
+    }
     P.part_w = dweight ? static_cast<float*>(scratch) : nullptr;
     P.part_b = dbias ? static_cast<float*>(scratch) + (size_t)ctas * N : nullptr;
-    P.rows = rows; P.ldx = ldx; P.lddy = lddy; P.ldy = lddx; P.N = (int)N; P.w32 = weight_dtype == NQ_F32;
     P.inv_n = 1.f / (float)N;
-    const int st = launch_norm(v, ctas, P, as_stream(stream));
+    const int st = streamed ? launch_stream(sv, P, as_stream(stream)) : launch_norm(v, ctas, P, as_stream(stream));
     if (st != NQ_OK || !sums) return st;
     const void* fn = bf16 ? (const void*)norm_reduce_kernel<true> : (const void*)norm_reduce_kernel<false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((N + 31) / 32), dbias ? 2 : 1);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(1024);
     cfg.stream = as_stream(stream);
     cudaLaunchAttribute attr[1];
     int n_ctas = (int)ctas, cols = (int)N;
