@@ -40,7 +40,7 @@ __device__ __forceinline__ long long loss_target(const LossTargets& t, int row) 
 // forward
 // ---------------------------------------------------------------------------
 struct LseEpilogue {
-    static constexpr bool kS8 = false;
+    static constexpr bool kS8 = false, kBuildA = false;
     struct Params {
         LossTargets targets;
         float2* part;              // [2 n_tiles][T]: largest logit (times log2 e), sum
@@ -51,7 +51,7 @@ struct LseEpilogue {
     int row, n0, slot;
     long long target;
     float top, sum;
-    __device__ LseEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_) {}
+    __device__ LseEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_) {}
     __device__ __forceinline__ void begin(int row_, int n0_, int set, int n_tile, int) {
         row = row_;
         n0 = n0_;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const uint4* h, uint4* o
 // d of a piece of the vocabulary.
 template <int OUT>
 struct GradEpilogue {
-    static constexpr bool kS8 = false;
+    static constexpr bool kS8 = false, kBuildA = false;
     struct Params {
         LossTargets targets;
         const float *lse, *row_scale;
@@ -214,7 +214,7 @@ struct GradEpilogue {
     int row, n0, at;
     float base, scale;
     bool live;
-    __device__ GradEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_) {}
+    __device__ GradEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_) {}
     __device__ __forceinline__ void begin(int row_, int n0_, int, int, int) {
         row = row_;
         n0 = n0_;
@@ -232,7 +232,6 @@ struct GradEpilogue {
     }
     __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
         const int row0 = row & ~31;
-        if (row0 >= s.M) return;                        // (the whole warp)
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -253,7 +252,7 @@ struct GradEpilogue {
 // dw of a piece: rows of words, times the final scale.
 template <int OUT>
 struct RowsEpilogue {
-    static constexpr bool kS8 = false;
+    static constexpr bool kS8 = false, kBuildA = false;
     struct Params {
         const float* final_scale;
         uint16_t* out;
@@ -263,13 +262,12 @@ struct RowsEpilogue {
     const MmShape& s;
     int row0, n0;
     float f;
-    __device__ RowsEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_), f(__ldg(p_.final_scale)) {}
+    __device__ RowsEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_), f(__ldg(p_.final_scale)) {}
     __device__ __forceinline__ void begin(int row, int n0_, int, int, int) {
         row0 = row & ~31;
         n0 = n0_;
     }
     __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
-        if (row0 >= s.M) return;                        // (the whole warp)
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = pack_outputs<OUT>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f, 0);
@@ -280,7 +278,7 @@ struct RowsEpilogue {
 
 // Partial sums of dh in fp32: [split][128 rows][4 columns][row], so that a warp's stores are whole lines.
 struct SumEpilogue {
-    static constexpr bool kS8 = false;
+    static constexpr bool kS8 = false, kBuildA = false;
     struct Params {
         float4* sums;
         int blocks, quads;         // of 128 rows; of 4 columns, padded to whole tiles
@@ -290,7 +288,7 @@ struct SumEpilogue {
     const MmShape& s;
     int n0;
     float4* dst;
-    __device__ SumEpilogue(const Params& p_, const MmShape& s_) : p(p_), s(s_) {}
+    __device__ SumEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_) {}
     __device__ __forceinline__ void begin(int row, int n0_, int, int, int split) {
         n0 = n0_;
         dst = p.sums + (((long long)split * p.blocks + (row >> 7)) * p.quads + (n0 >> 2)) * 128 + (row & 127);
@@ -359,7 +357,7 @@ struct LossPlan {
 static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     LossPlan p;
     const int cg = loss_pairs(T) ? 2 : 1, groups = sm_count() / cg, m_tiles = (int)((T + 128 * cg - 1) / (128 * cg));
-    p.bn = mm_tile_cols((int)V, m_tiles, groups, 16 * cg, 64);
+    p.bn = mm_tile_cols((int)V, m_tiles, cg, 64);
     p.slots = 2 * (int)((V + p.bn - 1) / p.bn);
     p.piece = kLossPieceBytes / 2 / T / kLossPieceUnit * kLossPieceUnit;
     if (p.piece < kLossPieceUnit) p.piece = kLossPieceUnit;
@@ -369,7 +367,7 @@ static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
         const int64_t pieces = (V + p.piece - 1) / p.piece;      // of equal size
         p.piece = up((V + pieces - 1) / pieces, kLossPieceUnit);
     }
-    p.d_bn = mm_tile_cols((int)(p.piece < V ? p.piece : V), m_tiles, groups, 16 * cg, 64);
+    p.d_bn = mm_tile_cols((int)(p.piece < V ? p.piece : V), m_tiles, cg, 64);
     p.w_bn = N <= 128 ? 128 : 256;
     // dh: few tiles over a long k.  Rounds of the longest tile, plus what writing and adding one more set of sums costs.
     p.h_bn = cg == 2 ? (N <= 128 ? 128 : 256) : (N <= 64 ? 64 : N <= 128 ? 128 : 256);

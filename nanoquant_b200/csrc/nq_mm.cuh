@@ -22,8 +22,8 @@
 namespace nq {
 
 constexpr int kMmThreads = 32 * 12, kMmEpilogueWarps = 8;
-constexpr int kMmMaxStages = 8, kMmABytes = 128 * 128, kMmStageOut = 2048;   // (bytes of output staging per epilogue warp)
-constexpr int kMmBarOff = 0, kMmOutOff = 1024, kMmStageOff = kMmOutOff + kMmEpilogueWarps * kMmStageOut;
+constexpr int kMmMaxStages = 24, kMmABytes = 128 * 128, kMmStageOut = 2048;   // (bytes of output staging per epilogue warp)
+constexpr int kMmBarOff = 0, kMmFewOff = 512, kMmOutOff = 1024, kMmStageOff = kMmOutOff + kMmEpilogueWarps * kMmStageOut;
 constexpr int kMmSmemMost = 226 * 1024;
 constexpr int kMmAccCols = 256;
 
@@ -31,12 +31,13 @@ struct MmShape {
     int M, N;                      // rows and columns of the result
     int m_tiles, n_tiles, bn;
     int ksteps, steps_per_split, splits;
-    int stages, stage_bytes;
+    int stages, stage_bytes, a_stage;  // bytes of a stage, and of A in it
     int m_fast;                    // consecutive tiles share their columns
     int a_box, b_box;              // K-major: rows per load; MN-major: loads of 64 rows
     int a_mn, b_mn;                // operand has m / n contiguous
     int kel;                       // elements of k per step
     int early_b;                   // B does not depend on the kernel before
+    int few;                       // (kBuildA) bytes of A per step: 1024 for every eight rows
     uint32_t idesc;
     unsigned wait_limit;
     unsigned* status;
@@ -124,10 +125,12 @@ __device__ __forceinline__ void mm_store_rows(unsigned char* stage, const uint32
     }
 }
 
-// Epi: struct Params; kS8; an object per epilogue thread with
+// Epi: struct Params; kS8; kBuildA: the epilogue warps make A themselves, all of it before the first MMA (few rows: `build` writes its steps, each of
+// whole 8-row groups in the layout of umma_desc, and may leave up to 512 bytes at `few` for the epilogue; the MMA reads rows beyond as they
+// are, whose results nobody looks at); an object per epilogue thread with
 //   Epi(const Params&, const MmShape&)
 //   begin(row, n0, m_tile, n_tile, split, ...)      a tile of this thread's row (row >= M: none)
-//   chunk(r, c, cols, stage)                        32 columns from n0 + c, `cols` of which exist (all lanes call it)
+//   chunk(r, c, cols, stage)                        32 columns from n0 + c, `cols` of which exist (all lanes call it, if any of their rows exists)
 //   end()
 template <int CG, class Epi>
 __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_kernel(const __grid_constant__ MmParams<Epi> P) {
@@ -140,8 +143,9 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
     auto bar_free = [&](int s) { return bars + 8 * (kMmMaxStages + s); };
     auto bar_acc_full = [&](int a) { return bars + 8 * (2 * kMmMaxStages + a); };
     auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * kMmMaxStages + 2 + a); };     // used in the pair's first CTA
-    constexpr int kMisc = kMmBarOff + 8 * (2 * kMmMaxStages + 4);
-    static_assert(kMisc + 8 <= kMmOutOff, "shared memory map");
+    const uint32_t bar_built = bars + 8 * (2 * kMmMaxStages + 4);
+    constexpr int kMisc = kMmBarOff + 8 * (2 * kMmMaxStages + 5);
+    static_assert(kMisc + 8 <= kMmFewOff, "shared memory map");
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kMisc + 4);
     const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;
@@ -154,7 +158,10 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             mbar_init(bar_acc_full(lane), 1);
             mbar_init(bar_acc_empty(lane), CG * kMmEpilogueWarps);
         }
-        if (lane == 0) *abort_flag = 0;
+        if (lane == 0) {
+            mbar_init(bar_built, kMmEpilogueWarps);
+            *abort_flag = 0;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -189,12 +196,15 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         r.k1 = min(S.ksteps, r.k0 + S.steps_per_split);
         return r;
     };
-    const uint32_t a_bytes = (uint32_t)(S.a_mn ? S.a_box * 8192 : S.a_box * 128), b_bytes = (uint32_t)(S.b_mn ? S.b_box * 8192 : S.b_box * 128);
-    const uint32_t stage0 = sbase + kMmStageOff;
+    constexpr bool kBuildA = Epi::kBuildA;
+    const uint32_t a_bytes = kBuildA ? 0u : (uint32_t)(S.a_mn ? S.a_box * 8192 : S.a_box * 128), b_bytes = (uint32_t)(S.b_mn ? S.b_box * 8192 : S.b_box * 128);
+    const uint32_t built = sbase + kMmStageOff, stage0 = built + (kBuildA ? (uint32_t)(S.few * S.ksteps) : 0u);
+    const uint32_t a_stage = (uint32_t)S.a_stage;
 
     if (warp == 0) {
         // ---------------------------------------------------------------- operands
         auto load_a = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
+            if constexpr (kBuildA) return;
             const int m0 = (T.m * CG + rank) * 128;
             if (S.a_mn) {
                 for (int i = 0; i < S.a_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_a, m0 + 64 * i, k * S.kel, bar);
@@ -220,7 +230,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             if (elect_one())
                 for (int i = 0; i < pre; ++i) {
                     if (rank == 0) mbar_expect_tx(bar_ready(i), (uint32_t)CG * (a_bytes + b_bytes));
-                    load_b(T, T.k0 + i, stage0 + (uint32_t)(i * S.stage_bytes) + kMmABytes, ready_bar(i));
+                    load_b(T, T.k0 + i, stage0 + (uint32_t)(i * S.stage_bytes) + a_stage, ready_bar(i));
                 }
         }
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -240,7 +250,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                     if (rank == 0) mbar_expect_tx(bar_ready(s), (uint32_t)CG * (a_bytes + b_bytes));
                     const uint32_t dst = stage0 + (uint32_t)(s * S.stage_bytes), bar = ready_bar(s);
                     load_a(T, k, dst, bar);
-                    load_b(T, k, dst + kMmABytes, bar);
+                    load_b(T, k, dst + a_stage, bar);
                 }
                 if (++s == S.stages) { s = 0; ph ^= 1; }
             }
@@ -253,6 +263,10 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             int s = 0, a = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;
+            if constexpr (kBuildA) {
+                ok = mbar_wait_warp(bar_built, 0, abort_flag, S.status, S.wait_limit);
+                tc_fence_after();
+            }
             for (int t = first; t < tiles && ok; t += groups) {
                 const Tile T = tile_of(t);
                 const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols);
@@ -263,7 +277,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t at = stage0 + (uint32_t)(s * S.stage_bytes), bt = at + kMmABytes;
+                        const uint32_t st = stage0 + (uint32_t)(s * S.stage_bytes), at = kBuildA ? built + (uint32_t)(k * S.few) : st, bt = st + a_stage;
                         const uint64_t ad = S.a_mn ? umma_desc_mn(at) : umma_desc(at), bd = S.b_mn ? umma_desc_mn(bt) : umma_desc(bt);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -281,7 +295,13 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         const int ew = warp & 3, set = (warp - 4) >> 2;
         unsigned char* stage = smem + kMmOutOff + (warp - 4) * kMmStageOut;
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        Epi epi(P.e, S);
+        if constexpr (kBuildA) {
+            Epi::build(P.e, S, smem + kMmStageOff, smem + kMmFewOff);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_built);
+        }
+        Epi epi(P.e, S, smem + kMmFewOff);
         int a = 0;
         uint32_t aph = 0;
         for (int t = first; t < tiles; t += groups) {
@@ -292,7 +312,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             epi.begin(row, n0, set, T.n, T.split);
             const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
 #pragma unroll 1
-            for (int c = 32 * set; c < live; c += 64) {
+            for (int c = 32 * set; c < live && row - lane < S.M; c += 64) {
                 uint32_t r[32];
                 mm_tmem_ld32(d + (uint32_t)c, r);
                 epi.chunk(r, c, min(32, live - c), stage);
@@ -337,14 +357,19 @@ struct MmOperand {
     int mn;
 };
 
-// Width of the tiles: the multiple of `unit` up to 256 whose rounds over the `groups` waste least; a step costs its columns, or what the
-// loads of the 128 rows cost where these are more.
-inline int mm_tile_cols(int N, int m_tiles, int groups, int unit, int least) {
+// Width of the tiles: the multiple of `unit` up to 256 that takes least time, in columns of a k step.
+// Pairs of CTAs are bound by the tensor cores: whole rounds of tiles over the pairs, 16 columns for a tile's start.
+// Single CTAs have up to 128 rows and are bound by the memory that B streams from, as long as a step has enough of it: its four MMAs take as long for
+// 16 columns as for some 100 (they fetch 128 rows of A all the same).  The last tile's latency is what narrow tiles save.  One token, int8, us at
+// 32 / 64 / 96 / 128 / 176 / 208 / 256 columns: 128256 x 2048 106 / 58 / 47.5 / 44.2 / 48.6 / 51.9 / 48.3, 151936 x 4096 238 / 130 / 96.4 / 98.1 / 95.0 /
+// 95.4 / 99.7, 12288 x 4096 26 / 20 / 15.5 / 14.3 / 15.3 / 16.7 / 17.9.
+inline int mm_tile_cols(int N, int m_tiles, int cg, int least) {
+    const int groups = sm_count() / cg, unit = 16 * cg;
     int best = 0;
     double best_cost = 0;
     for (int bn = 256; bn >= least; bn -= unit) {
         const int64_t tiles = (int64_t)((N + bn - 1) / bn) * m_tiles, rounds = (tiles + groups - 1) / groups;
-        const double cost = (double)rounds * (bn + 16);      // (a tile's fill and drain as 16 columns)
+        const double cost = cg == 2 ? (double)rounds * (bn + 16) : (double)rounds * (bn > 100 ? bn : 100) + 0.4 * bn;
         if (!best || cost < best_cost * 0.995) { best = bn; best_cost = cost; }
     }
     return best;
@@ -369,14 +394,18 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
     S.m_fast = S.m_tiles <= S.n_tiles;
     S.kel = 128 / esize;
     S.ksteps = (int)((K + S.kel - 1) / S.kel);
+    S.few = Epi::kBuildA ? (M + 7) / 8 * 1024 : 0;
     if (splits > S.ksteps) splits = S.ksteps;
     S.steps_per_split = (S.ksteps + splits - 1) / splits;
     S.splits = (S.ksteps + S.steps_per_split - 1) / S.steps_per_split;
     S.a_mn = A.mn; S.b_mn = B.mn;
     S.a_box = A.mn ? 2 : CG == 2 || M >= 128 ? 128 : (M + 7) / 8 * 8;
     S.b_box = B.mn ? bn / CG / 64 : bn / CG;
-    S.stage_bytes = kMmABytes + bn / CG * 128;
-    S.stages = (kMmSmemMost - 1024 - kMmStageOff) / S.stage_bytes;
+    S.a_stage = Epi::kBuildA ? 0 : S.a_mn ? kMmABytes : S.a_box * 128;
+    S.stage_bytes = S.a_stage + bn / CG * 128;
+    // (a step's MMAs read 128 rows of A; what lies behind fewer is read as it is, and nobody looks at these rows' results)
+    const int fixed = 1024 + kMmStageOff + S.few * S.ksteps, slack = Epi::kBuildA || S.a_stage < kMmABytes ? kMmABytes : 0;
+    S.stages = (kMmSmemMost - fixed - slack) / S.stage_bytes;
     if (S.stages > kMmMaxStages) S.stages = kMmMaxStages;
     S.early_b = early_b;
     const uint32_t fmt = type == kMmF16 ? 0u : 1u;           // kind::f16: 1 = bf16; kind::i8: 1 = signed
@@ -384,7 +413,7 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
               (uint32_t)(bn >> 3) << 17 | (uint32_t)(128 * CG >> 4) << 24;
     S.wait_limit = gemm_wait_limit();
     S.status = status;
-    int st = A.mn ? mm_encode(&P.map_a, A.p, type, M, K, A.stride, 64, 64) : mm_encode(&P.map_a, A.p, type, K, M, A.stride, S.kel, S.a_box);
+    int st = Epi::kBuildA ? NQ_OK : A.mn ? mm_encode(&P.map_a, A.p, type, M, K, A.stride, 64, 64) : mm_encode(&P.map_a, A.p, type, K, M, A.stride, S.kel, S.a_box);
     if (st != NQ_OK) return st;
     st = B.mn ? mm_encode(&P.map_b, B.p, type, N, K, B.stride, 64, 64) : mm_encode(&P.map_b, B.p, type, K, N, B.stride, S.kel, S.b_box);
     if (st != NQ_OK) return st;
@@ -393,7 +422,7 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(CG * (tiles < most ? tiles : most)));
     cfg.blockDim = dim3(kMmThreads);
-    cfg.dynamicSmemBytes = 1024 + kMmStageOff + S.stages * S.stage_bytes;
+    cfg.dynamicSmemBytes = fixed + S.stages * S.stage_bytes + slack;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     void* args[] = {&P};

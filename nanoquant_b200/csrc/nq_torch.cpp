@@ -725,9 +725,9 @@ PyObject* py_int8_linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     OnDevice on(dev);
     void* status = status_header(dev);
     const size_t bytes = nq_int8_linear_scratch_bytes(T, N);
-    const Tensor scratch = new_bytes((int64_t)bytes, *x);
+    const Tensor scratch = bytes ? new_bytes((int64_t)bytes, *x) : Tensor();
     const int st = nq_int8_linear_fwd(x->const_data_ptr(), static_cast<const int8_t*>(w->const_data_ptr()), static_cast<const float*>(ws->const_data_ptr()),
-                                      b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(), scratch.mutable_data_ptr(), bytes, status, T, N, V, ldx,
+                                      b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(), bytes ? scratch.mutable_data_ptr() : nullptr, bytes, status, T, N, V, ldx,
                                       V > 1 ? ldw : (N + 15) / 16 * 16, V, dtype_id(x->scalar_type()), stream_of(dev));
     if (st < 0) fail(st, "nq_int8_linear_fwd");
     return THPVariable_Wrap(y);

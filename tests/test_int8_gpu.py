@@ -51,6 +51,23 @@ def test_quantize_is_exact(rows, cols, dtype):
     assert q.stride(0) % 16 == 0 and q.shape == x.shape and s.shape == (rows,)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_all_quotients(dtype):
+    """Every ratio of two significands, at ordinary magnitudes, the smallest and the largest: halves and their neighbours among them."""
+    from nanoquant_b200 import ops
+
+    bits = 8 if dtype == torch.bfloat16 else 11
+    x = torch.arange(1, 2 ** bits, device="cuda").double()
+    tops = (2 ** bits - 1 - torch.arange(0, 2 ** (bits - 1), 1 if bits == 8 else 13, device="cuda")).double()
+    for scale in (1.0, 2.0 ** -133, 2.0 ** 100) if dtype == torch.bfloat16 else (1.0, 2.0 ** -24, 2.0 ** 4):
+        m = torch.minimum(x, tops[:, None]) * scale        # every row: all values up to its largest
+        m[:, ::2] *= -1
+        m = m.to(dtype)
+        q, s = ops.quantize_int8(m)
+        q64, s64 = quantized(m)
+        assert torch.equal(q.double(), q64) and torch.equal(s.double(), s64)
+
+
 def test_quantize_ties_go_to_even():
     from nanoquant_b200 import ops
 
@@ -61,7 +78,8 @@ def test_quantize_ties_go_to_even():
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,N,V,bias", [
-    (1, 1, 1, True), (1, 4096, 512, False), (1, 16, 4, False), (3, 100, 33, False), (8, 128, 16, False), (37, 1003, 777, True), (127, 64, 130, True), (128, 256, 300, False),
+    (1, 1, 1, True), (2, 260, 77, True), (4, 1001, 40, False), (5, 384, 300, False), (9, 640, 200, True), (15, 4100, 64, False), (16, 6144, 50, True),
+    (16, 6272, 50, False), (8, 12288, 70, False), (8, 12300, 33, False), (1, 4096, 512, False), (1, 16, 4, False), (3, 100, 33, False), (8, 128, 16, False), (37, 1003, 777, True), (127, 64, 130, True), (128, 256, 300, False),
     (129, 512, 1000, True), (255, 200, 31, False), (257, 2048, 513, False), (16, 2048, 40001, False), (300, 1024, 2050, True),
     (1030, 4096, 1536, False), (2, 16384, 100, False)])
 def test_linear_matches_definition(T, N, V, bias, dtype):

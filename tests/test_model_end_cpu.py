@@ -45,9 +45,9 @@ def test_int8_refusals():
     for i, v, st in ((0, None, "NULL"), (1, None, "NULL"), (2, None, "NULL"), (3, 0, "SHAPE"), (4, 0, "SHAPE"), (6, 63, "SHAPE"), (7, F32, "DTYPE"),
                      (3, 1 << 31, "TOO_LARGE")):
         assert call("nq_quantize_rows_s8", good, i, v) == getattr(_lib, "NQ_ERR_" + st), (i, v)
-    need = L.nq_int8_linear_scratch_bytes(3, 100)
-    assert need == 256 + 3 * 112 and L.nq_int8_linear_scratch_bytes(0, 8) == 0
-    good = [P, P, P, P, P, P, need, P, 3, 100, 50, 100, 112, 50, BF16, None]   # x w ws bias y scratch bytes status T N V ldx ldw ldy dtype stream
+    need = L.nq_int8_linear_scratch_bytes(30, 100)
+    assert need == 256 + 30 * 112 and L.nq_int8_linear_scratch_bytes(0, 8) == 0 and L.nq_int8_linear_scratch_bytes(1, 4096) == 0
+    good = [P, P, P, P, P, P, need, P, 30, 100, 50, 100, 112, 50, BF16, None]   # x w ws bias y scratch bytes status T N V ldx ldw ldy dtype stream
     for i, v, st in ((0, None, "NULL"), (1, None, "NULL"), (2, None, "NULL"), (4, None, "NULL"), (5, None, "NULL"), (7, None, "NULL"), (6, need - 1, "SCRATCH"),
                      (1, ODD, "ALIGN"), (2, ODD, "ALIGN"), (5, ODD, "ALIGN"), (7, ODD, "ALIGN"), (8, 0, "SHAPE"), (9, 0, "SHAPE"), (10, 0, "SHAPE"), (12, 96, "SHAPE"),
                      (12, 120, "SHAPE"), (13, 49, "SHAPE"), (14, F32, "DTYPE"), (10, 1 << 30, "SHAPE")):
