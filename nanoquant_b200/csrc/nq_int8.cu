@@ -125,6 +125,7 @@ constexpr int kInt8Few = 2, kInt8FewBytes = 96 * 1024;       // tokens; bytes of
 template <int OUT, bool FEW>
 struct Int8Epilogue {
     static constexpr bool kS8 = true, kBuildA = FEW;
+    static constexpr int kChunk = 0;
     struct Params {
         const float *xs, *ws;
         const uint16_t* bias;
@@ -218,7 +219,7 @@ static int launch_int8(const typename Int8Epilogue<OUT, FEW>::Params& e, const i
     P.e = e;
     const int m_tiles = (T + 128 * CG - 1) / (128 * CG);
     const int bn = mm_tile_cols(V, m_tiles, CG, 16 * CG);
-    return mm_launch<CG>(P, kMmS8, {xq, ldq, 0}, {w, ldw, 0}, T, V, e.N, bn, 1, 1, status, stream);
+    return mm_launch<CG>(P, kMmS8, {xq, ldq, 0}, {w, ldw, 0}, T, V, e.N, bn, 1, 1, 0, status, stream);
 }
 static bool int8_few(int64_t T, int64_t N) { return T <= kInt8Few && 1024 * ((N + 127) / 128) <= kInt8FewBytes; }
 template <int OUT>

@@ -41,6 +41,7 @@ __device__ __forceinline__ long long loss_target(const LossTargets& t, int row) 
 // ---------------------------------------------------------------------------
 struct LseEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
+    static constexpr int kChunk = 8;           // 512 columns: 2048 x 4096 x 151936 level with a whole sum (1.60 ms), with 256 1.69
     struct Params {
         LossTargets targets;
         float2* part;              // [2 n_tiles][T]: largest logit (times log2 e), sum
@@ -88,10 +89,12 @@ struct LseEpilogue {
     }
 };
 
-// 32 tokens a CTA, the pieces dealt to its warps.  A target that is no word of the vocabulary (and not `ignore`) makes its token NaN.
-__global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V) {
-    __shared__ float2 red[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+// Eight tokens a CTA of 256 threads (so that the CTAs are there before the product's have left), 32 threads for each; the pieces of a token in the
+// same order whatever else there is.  A target that is no word of the vocabulary (and not `ignore`) makes its token NaN.
+__global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V) {
+    __shared__ float2 red[8][33];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int sub = threadIdx.x & 7, piece = threadIdx.x >> 3, row = blockIdx.x * 8 + sub;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto join = [](float2 a, float2 b) {
         const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
@@ -99,21 +102,27 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, cons
     };
     float2 v = make_float2(-INFINITY, 0.f);
     if (row < T) {
-#pragma unroll 8
-        for (int i = warp; i < slots; i += 32) v = join(v, part[(long long)i * T + row]);
+        int i = piece;
+        for (; i + 7 * 32 < slots; i += 8 * 32) {      // eight loads in flight
+            float2 p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = __ldcg(part + (long long)(i + 32 * k) * T + row);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v = join(v, p[k]);
+        }
+        for (; i < slots; i += 32) v = join(v, __ldcg(part + (long long)i * T + row));
     }
-    red[warp][lane] = v;
+    red[sub][piece] = v;
     __syncthreads();
-    // warp w joins the 32 sums of token w
-    v = red[lane][warp];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x * 8 + warp;
+    v = red[warp][lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
-    const int r = blockIdx.x * 32 + warp;
     if (lane == 0 && r < T) {
         const long long t = loss_target(targets, r);
         float l = v.x * kLn2 + logf(v.y), loss = 0.f;
         if (t != targets.ignore) {
-            if (t >= 0 && t < V) loss = l - target_logit[r];
+            if (t >= 0 && t < V) loss = l - __ldcg(target_logit + r);
             else loss = l = __int_as_float(0x7fffffff);
         }
         row_loss[r] = loss;
@@ -130,7 +139,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* row_loss, L
     double s = 0;
     int n = 0;
     for (int i = threadIdx.x; i < T; i += 1024) {
-        if (row_loss) s += row_loss[i];
+        s += __ldcg(row_loss + i);
         n += loss_target(targets, i) != targets.ignore;
     }
     auto reduce = [&]() {
@@ -149,7 +158,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* row_loss, L
         reduce();
         if (lane == 0) {
             *count = (float)n;
-            if (out) *out = mean ? (float)(s / n) : (float)s;
+            *out = mean ? (float)(s / n) : (float)s;
         }
     }
 }
@@ -157,44 +166,53 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* row_loss, L
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// row_scale[t]: what d of a token is multiplied by before it is rounded; final: what the products' sums are multiplied by.
-__global__ void __launch_bounds__(1024) loss_scales_kernel(const float* grad, long long grad_stride, const float* count, LossTargets targets, float* row_scale, float* final_scale,
-                                                           int T, int reduction, float unit) {
-    __shared__ float red[32];
+// What the products need, in one launch.  CTA 0: row_scale[t], what d of a token is multiplied by before it is rounded, and final_scale, what the
+// products' sums are multiplied by.  The others (where `out` is wanted): h with zeros in the rows of tokens without a target, whatever these hold (their
+// d is zero, but zero times a NaN is not).
+struct LossPrepare {
+    LossTargets targets;
+    const float *grad, *count;
+    long long grad_stride;
+    float *row_scale, *final_scale;
+    const uint4* h;
+    uint4* out;
+    long long ldh;                 // 16-byte units
+    int T, packs, reduction;
+    float unit;
+};
+__global__ void __launch_bounds__(512) loss_prepare_kernel(const LossPrepare P) {
+    __shared__ float red[16];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    float top = 0.f;
-    if (reduction == NQ_REDUCE_NONE && unit != 1.f) {
-        for (int i = threadIdx.x; i < T; i += 1024)
-            if (loss_target(targets, i) != targets.ignore) top = fmaxf(top, fabsf(grad[i * grad_stride]));
+    if (blockIdx.x > 0) {
+        const long long total = (long long)P.T * P.packs, step = (long long)(gridDim.x - 1) * 512;
+        for (long long i = (long long)(blockIdx.x - 1) * 512 + threadIdx.x; i < total; i += step) {
+            const int row = (int)(i / P.packs), c = (int)(i - (long long)row * P.packs);
+            P.out[i] = loss_target(P.targets, row) != P.targets.ignore ? __ldg(P.h + row * P.ldh + c) : make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
+    float top = 1.f;
+    if (P.reduction == NQ_REDUCE_NONE && P.unit != 1.f) {
+        top = 0.f;
+        for (int i = threadIdx.x; i < P.T; i += 512)
+            if (loss_target(P.targets, i) != P.targets.ignore) top = fmaxf(top, fabsf(P.grad[i * P.grad_stride]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) red[warp] = top;
         __syncthreads();
-        top = red[lane];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i]);
         if (top == 0.f || top == INFINITY) top = 1.f;
-    } else {
-        top = 1.f;
     }
-    for (int i = threadIdx.x; i < T; i += 1024) {
-        const bool live = loss_target(targets, i) != targets.ignore;
-        row_scale[i] = !live ? 0.f : reduction == NQ_REDUCE_NONE ? grad[i * grad_stride] / top * unit : unit;
+    for (int i = threadIdx.x; i < P.T; i += 512) {
+        const bool live = loss_target(P.targets, i) != P.targets.ignore;
+        P.row_scale[i] = !live ? 0.f : P.reduction == NQ_REDUCE_NONE ? P.grad[i * P.grad_stride] / top * P.unit : P.unit;
     }
     if (threadIdx.x == 0) {
-        float f = reduction == NQ_REDUCE_NONE ? top : grad[0];
-        if (reduction == NQ_REDUCE_MEAN) f = *count > 0.f ? f / *count : 0.f;
-        *final_scale = f / unit;
-    }
-}
-// h with zeros in the rows of tokens without a target, whatever these hold (their d is zero, but zero times a NaN is not).
-__global__ void __launch_bounds__(256) loss_rows_kernel(const uint4* h, uint4* out, LossTargets targets, int T, int packs, long long ldh) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const long long total = (long long)T * packs;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int row = (int)(i / packs), c = (int)(i - (long long)row * packs);
-        out[i] = loss_target(targets, row) != targets.ignore ? __ldg(h + row * ldh + c) : make_uint4(0, 0, 0, 0);
+        float f = P.reduction == NQ_REDUCE_NONE ? top : P.grad[0];
+        if (P.reduction == NQ_REDUCE_MEAN) f = *P.count > 0.f ? f / *P.count : 0.f;
+        *P.final_scale = f / P.unit;
     }
 }
 
@@ -202,6 +220,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const uint4* h, uint4* o
 template <int OUT>
 struct GradEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
+    static constexpr int kChunk = 0;
     struct Params {
         LossTargets targets;
         const float *lse, *row_scale;
@@ -253,6 +272,7 @@ struct GradEpilogue {
 template <int OUT>
 struct RowsEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
+    static constexpr int kChunk = 0;
     struct Params {
         const float* final_scale;
         uint16_t* out;
@@ -279,6 +299,7 @@ struct RowsEpilogue {
 // Partial sums of dh in fp32: [split][128 rows][4 columns][row], so that a warp's stores are whole lines.
 struct SumEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
+    static constexpr int kChunk = 0;
     struct Params {
         float4* sums;
         int blocks, quads;         // of 128 rows; of 4 columns, padded to whole tiles
@@ -410,7 +431,7 @@ static int launch_lse(const void* h, const void* w, const LseEpilogue::Params& e
                       unsigned* status, cudaStream_t stream) {
     MmParams<LseEpilogue> P = {};
     P.e = e;
-    return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 0, status, stream);
+    return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 1, 1, status, stream);
 }
 
 template <int CG, int OUT>
@@ -419,27 +440,27 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
                            unsigned* status, cudaStream_t stream) {
     const int type = OUT == kOutFp16 ? kMmF16 : kMmBf16;
     uint16_t* d = reinterpret_cast<uint16_t*>(scratch + at.d);
-    const float *row_scale = reinterpret_cast<float*>(scratch + at.row_scale), *final_scale = reinterpret_cast<float*>(scratch + at.final_scale);
+    const float* final_scale = reinterpret_cast<float*>(scratch + at.final_scale);
     int splits = p.h_splits;
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece);
         const char* wp = static_cast<const char*>(w) + v0 * ldw * 2;
         {
             MmParams<GradEpilogue<OUT>> P = {};
-            P.e = {targets, lse, row_scale, d, p.piece, (int)v0};
-            const int st = mm_launch<CG>(P, type, {h, ldh * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 0, status, stream);
+            P.e = {targets, lse, reinterpret_cast<float*>(scratch + at.row_scale), d, p.piece, (int)v0};
+            const int st = mm_launch<CG>(P, type, {h, ldh * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 1, 1, status, stream);
             if (st != NQ_OK) return st;
         }
         if (dw) {
             MmParams<RowsEpilogue<OUT>> P = {};
             P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
-            const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, status, stream);
+            const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
             if (st != NQ_OK) return st;
         }
         if (dh) {
             MmParams<SumEpilogue> P = {};
             P.e = {reinterpret_cast<float4*>(scratch + at.sums), p.h_blocks, p.h_quads, v0 > 0};
-            const int st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 0, status, stream);
+            const int st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 1, 1, status, stream);
             if (st != NQ_OK) return st;
             if (v0 == 0) splits = P.s.splits;                  // (the last piece may be shorter and have fewer)
         }
@@ -488,7 +509,7 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     if (st != NQ_OK) return st;
     int slots = p.slots, t = (int)T, v = (int)V, mean = reduction == NQ_REDUCE_MEAN;
     void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v};
-    st = launch_plain((const void*)lse_join_kernel, dim3((unsigned)((T + 31) / 32)), 1024, join_args, s);
+    st = launch_plain((const void*)lse_join_kernel, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
     if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;
     void* sum_args[] = {&row_loss, &tg, &loss, &count, &t, &mean};
     return launch_plain((const void*)loss_sum_kernel, dim3(1), 1024, sum_args, s);
@@ -516,21 +537,14 @@ int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int targ
     const LossScratch at = loss_scratch(p, T, N);
     char* base = static_cast<char*>(scratch);
     LossTargets tg = {targets, target_bits == 64, ignore_index};
-    int t = (int)T, red = reduction, packs = (int)(N / 8);
-    float unit = dtype == NQ_F16 ? kLossHalfScale : 1.f;
-    long long stride = grad_stride, ldp = ldh / 8;
-    float *row_scale = reinterpret_cast<float*>(base + at.row_scale), *final_scale = reinterpret_cast<float*>(base + at.final_scale);
-    void* scale_args[] = {&grad_loss, &stride, &count, &tg, &row_scale, &final_scale, &t, &red, &unit};
-    st = launch_plain((const void*)loss_scales_kernel, dim3(1), 1024, scale_args, s);
+    LossPrepare prep = {tg, grad_loss, count, grad_stride, reinterpret_cast<float*>(base + at.row_scale), reinterpret_cast<float*>(base + at.final_scale),
+                        static_cast<const uint4*>(h), reinterpret_cast<uint4*>(base + at.h), ldh / 8, (int)T, (int)(N / 8), reduction,
+                        dtype == NQ_F16 ? kLossHalfScale : 1.f};
+    int64_t ctas = dw ? (T * prep.packs + 2047) / 2048 : 0;
+    if (ctas > 4 * sm_count()) ctas = 4 * sm_count();
+    void* prepare_args[] = {&prep};
+    st = launch_plain((const void*)loss_prepare_kernel, dim3((unsigned)(1 + ctas)), 512, prepare_args, s);
     if (st != NQ_OK) return st;
-    if (dw) {
-        const uint4* hp = static_cast<const uint4*>(h);
-        uint4* hz = reinterpret_cast<uint4*>(base + at.h);
-        void* rows_args[] = {&hp, &hz, &tg, &t, &packs, &ldp};
-        const int64_t ctas = (T * packs + 1023) / 1024, most = 8 * sm_count();
-        st = launch_plain((const void*)loss_rows_kernel, dim3((unsigned)(ctas < most ? ctas : most)), 256, rows_args, s);
-        if (st != NQ_OK) return st;
-    }
 #define NQ_LOSS_BACKWARD(cg, out) launch_backward<cg, out>(h, w, tg, lse, dh, dw, base, p, at, (int)T, (int)N, (int)V, ldh, ldw, lddh, lddw, status, s)
     if (dtype == NQ_BF16) return loss_pairs(T) ? NQ_LOSS_BACKWARD(2, kOutBf16) : NQ_LOSS_BACKWARD(1, kOutBf16);
     return loss_pairs(T) ? NQ_LOSS_BACKWARD(2, kOutFp16) : NQ_LOSS_BACKWARD(1, kOutFp16);

@@ -37,6 +37,7 @@ struct MmShape {
     int a_mn, b_mn;                // operand has m / n contiguous
     int kel;                       // elements of k per step
     int early_b;                   // B does not depend on the kernel before
+    int release;                   // the kernel behind may start early (it is one of the same call and waits for this one's results)
     int few;                       // (kBuildA) bytes of A per step: 1024 for every eight rows
     uint32_t idesc;
     unsigned wait_limit;
@@ -49,6 +50,12 @@ struct alignas(64) MmParams {
     MmShape s;
     typename Epi::Params e;
 };
+
+// A split of the launch's registers between warpgroups (each call by all four warps of one).
+template <int REGS>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
 // MN-major, 128-byte swizzle: 64 elements of m / n per 128-byte row, one row per k; 8-k groups 1024 bytes apart, the next 64 elements 8192.
 __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr) {
@@ -86,7 +93,7 @@ __device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, in
         tma_load_2d(dst, map, c0, c1, bar);
 }
 // 32 columns of this warp's 32 rows: lane i has row i.
-__device__ __forceinline__ void mm_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void mm_tmem_start(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
                  "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
@@ -94,11 +101,20 @@ __device__ __forceinline__ void mm_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) 
                    "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;"      // (the registers are operands, so that no use moves above it)
+}
+__device__ __forceinline__ void mm_tmem_landed() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// (the registers are operands, so that no use moves above the wait in front of this)
+__device__ __forceinline__ void mm_tmem_use(uint32_t (&r)[32]) {
+    asm volatile(""
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
                    "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void mm_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    mm_tmem_start(taddr, r);
+    mm_tmem_landed();
+    mm_tmem_use(r);
 }
 
 // 32 rows x 32 columns of 16-bit outputs, lane i holding row i as 16 words: through 2 KB of the warp's shared memory, so that four lanes
@@ -132,6 +148,11 @@ __device__ __forceinline__ void mm_store_rows(unsigned char* stage, const uint32
 //   begin(row, n0, m_tile, n_tile, split, ...)      a tile of this thread's row (row >= M: none)
 //   chunk(r, c, cols, stage)                        32 columns from n0 + c, `cols` of which exist (all lanes call it, if any of their rows exists)
 //   end()
+// kChunk: steps of k after which the accumulator is added to fp32 sums in registers (0: never).  The tensor cores cut an accumulator off, towards zero, with every
+// instruction, so that the error of a long sum grows with its length, and has a sign: logits of 8 were 2.8e-5 low at 4096 columns, five times the
+// rms error of fp32 additions.  A sum of C chunks is off by a C-th of that.
+constexpr int kMmRegsLaunch = 168, kMmRegsIssue = 40, kMmRegsSums = 232;      // of a thread: at launch, and after the split with kChunk
+static_assert(128 * kMmRegsIssue + 256 * kMmRegsSums <= kMmThreads * kMmRegsLaunch, "register split");
 template <int CG, class Epi>
 __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_kernel(const __grid_constant__ MmParams<Epi> P) {
     extern __shared__ unsigned char smem_raw[];
@@ -183,7 +204,9 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     tc_fence_after();
+    if (S.release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+    constexpr int kChunk = Epi::kChunk ? Epi::kChunk : 1 << 30;
     const int groups = (int)gridDim.x / CG, first = (int)blockIdx.x / CG, plane = S.m_tiles * S.n_tiles, tiles = plane * S.splits;
     struct Tile { int m, n, split, k0, k1; };
     auto tile_of = [&](int t) {
@@ -201,6 +224,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
     const uint32_t built = sbase + kMmStageOff, stage0 = built + (kBuildA ? (uint32_t)(S.few * S.ksteps) : 0u);
     const uint32_t a_stage = (uint32_t)S.a_stage;
 
+    if (warp < 4) {
+    if constexpr (Epi::kChunk > 0) regs_down<kMmRegsIssue>();
     if (warp == 0) {
         // ---------------------------------------------------------------- operands
         auto load_a = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
@@ -269,10 +294,12 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             }
             for (int t = first; t < tiles && ok; t += groups) {
                 const Tile T = tile_of(t);
+                for (int c0 = T.k0; c0 < T.k1 && ok; c0 += kChunk) {
+                const int c1 = min(T.k1 - c0, kChunk) + c0;
                 const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols);
                 ok = mbar_wait_warp<CG == 2>(bar_acc_empty(a), aph ^ 1, abort_flag, S.status, S.wait_limit);
                 tc_fence_after();
-                for (int k = T.k0; k < T.k1 && ok; ++k) {
+                for (int k = c0; k < c1 && ok; ++k) {
                     ok = mbar_wait_warp<CG == 2>(bar_ready(s), ph, abort_flag, S.status, S.wait_limit);
                     if (!ok) break;
                     tc_fence_after();
@@ -281,17 +308,21 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                         const uint64_t ad = S.a_mn ? umma_desc_mn(at) : umma_desc(at), bd = S.b_mn ? umma_desc_mn(bt) : umma_desc(bt);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            mm_mma<CG, Epi::kS8>(d, ad + (uint64_t)(a_step * i), bd + (uint64_t)(b_step * i), S.idesc, k > T.k0 || i ? 1u : 0u);
+                            mm_mma<CG, Epi::kS8>(d, ad + (uint64_t)(a_step * i), bd + (uint64_t)(b_step * i), S.idesc, k > c0 || i ? 1u : 0u);
                         mm_commit<CG>(bar_free(s));
                     }
                     if (++s == S.stages) { s = 0; ph ^= 1; }
                 }
                 if (ok && elect_one()) mm_commit<CG>(bar_acc_full(a));
                 if (++a == 2) { a = 0; aph ^= 1; }
+                if (T.k1 - c0 <= kChunk) break;
+                }
             }
         }
-    } else if (warp >= 4) {
+    }
+    } else {
         // ---------------------------------------------------------------- epilogue
+        if constexpr (Epi::kChunk > 0) regs_up<kMmRegsSums>();
         const int ew = warp & 3, set = (warp - 4) >> 2;
         unsigned char* stage = smem + kMmOutOff + (warp - 4) * kMmStageOut;
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -307,24 +338,70 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         for (int t = first; t < tiles; t += groups) {
             const Tile T = tile_of(t);
             const int row = (T.m * CG + rank) * 128 + 32 * ew + lane, n0 = T.n * S.bn, live = min(S.bn, S.N - n0);
-            if (!mbar_wait_warp<CG == 2>(bar_acc_full(a), aph, abort_flag, S.status, S.wait_limit)) break;
-            tc_fence_after();
-            epi.begin(row, n0, set, T.n, T.split);
-            const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
+            auto full = [&]() {
+                const bool ok = mbar_wait_warp<CG == 2>(bar_acc_full(a), aph, abort_flag, S.status, S.wait_limit);
+                tc_fence_after();
+                return ok;
+            };
+            auto empty = [&]() {                          // this warp has read the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(bar_acc_empty(a), 0)) : "memory");
+                    else mbar_arrive(bar_acc_empty(a));
+                }
+                if (++a == 2) { a = 0; aph ^= 1; }
+            };
+            const bool some = row - lane < S.M;           // of the warp's rows exist
+            if constexpr (Epi::kChunk > 0) {
+                float sum[kMmAccCols / 64][32] = {};
+                bool ok = true;
+                for (int c0 = T.k0; c0 < T.k1; c0 += kChunk) {
+                    ok = full();
+                    if (!ok) break;
+                    const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
+#pragma unroll
+                    for (int j = 0; j < kMmAccCols / 64; j += 2) {        // (two loads under way)
+                        if (32 * set + 64 * j < live && some) {
+                            uint32_t r0[32], r1[32];
+                            mm_tmem_start(d + (uint32_t)(32 * set + 64 * j), r0);
+                            mm_tmem_start(d + (uint32_t)(32 * set + 64 * j + 64), r1);      // (within the accumulator, whatever the tile's width)
+                            mm_tmem_landed();
+                            mm_tmem_use(r0);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[j][i] += __uint_as_float(r0[i]);
+                            mm_tmem_use(r1);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[j + 1][i] += __uint_as_float(r1[i]);
+                        }
+                    }
+                    empty();
+                }
+                if (!ok) break;
+                epi.begin(row, n0, set, T.n, T.split);
+#pragma unroll
+                for (int j = 0; j < kMmAccCols / 64; ++j) {
+                    const int c = 32 * set + 64 * j;
+                    if (c < live && some) {
+                        uint32_t r[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sum[j][i]);
+                        epi.chunk(r, c, min(32, live - c), stage);
+                    }
+                }
+            } else {
+                if (!full()) break;
+                epi.begin(row, n0, set, T.n, T.split);
+                const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
 #pragma unroll 1
-            for (int c = 32 * set; c < live && row - lane < S.M; c += 64) {
-                uint32_t r[32];
-                mm_tmem_ld32(d + (uint32_t)c, r);
-                epi.chunk(r, c, min(32, live - c), stage);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(bar_acc_empty(a), 0)) : "memory");
-                else mbar_arrive(bar_acc_empty(a));
+                for (int c = 32 * set; c < live && some; c += 64) {
+                    uint32_t r[32];
+                    mm_tmem_ld32(d + (uint32_t)c, r);
+                    epi.chunk(r, c, min(32, live - c), stage);
+                }
+                empty();
             }
             epi.end();
-            if (++a == 2) { a = 0; aph ^= 1; }
         }
     }
     // On an expired wait, give the copies in flight a bounded time to land before shared memory is released.
@@ -377,7 +454,7 @@ inline int mm_tile_cols(int N, int m_tiles, int cg, int least) {
 
 template <int CG, class Epi>
 int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B, int M, int N, int64_t K, int bn, int splits,
-              int early_b, unsigned* status, cudaStream_t stream) {
+              int early_b, int release, unsigned* status, cudaStream_t stream) {
     static bool attr_set[64];
     int dev = 0;
     NQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -408,6 +485,7 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
     S.stages = (kMmSmemMost - fixed - slack) / S.stage_bytes;
     if (S.stages > kMmMaxStages) S.stages = kMmMaxStages;
     S.early_b = early_b;
+    S.release = release;
     const uint32_t fmt = type == kMmF16 ? 0u : 1u;           // kind::f16: 1 = bf16; kind::i8: 1 = signed
     S.idesc = (type == kMmS8 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)A.mn << 15 | (uint32_t)B.mn << 16 |
               (uint32_t)(bn >> 3) << 17 | (uint32_t)(128 * CG >> 4) << 24;
