@@ -70,8 +70,8 @@ __device__ __forceinline__ uint2 q8_pack(const uint4& u, const Q8Row& q) {
 template <bool BF16>
 __device__ __forceinline__ int8_t q8_one(uint16_t x, const Q8Row& q) { return q.live ? (int8_t)q8_exact(io_float(x, BF16), q.top) : (int8_t)0; }
 
-// VEC: elements per load (8: 16 bytes in, 8 out; 1: any alignment).
-template <bool BF16, int VEC>
+// A row per CTA.  PACKS > 0: 16-byte loads, PACKS of eight values a thread, kept in registers; 0: single values at any address, read twice.
+template <bool BF16, int PACKS>
 __global__ void __launch_bounds__(512) quantize_rows_kernel(const uint16_t* x, int8_t* q, float* scale, int N, long long ldx, long long ldq, int release) {
     __shared__ uint32_t red[16];
     const long long row = blockIdx.x;
@@ -82,10 +82,18 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const uint16_t* x, i
     // (behind the wait: what starts early may rely on everything before this kernel)
     if (release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     uint32_t top = 0;
+    uint4 v[PACKS > 0 ? PACKS : 1];
+    if constexpr (PACKS > 0) {
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) {
+            const int c = (p * (int)blockDim.x + tid) * 8;
+            v[p] = c < N ? __ldg(reinterpret_cast<const uint4*>(xr + c)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) top = q8_top(v[p], top);
+    } else {
 #pragma unroll 4
-    for (int c = tid * VEC; c < N; c += blockDim.x * VEC) {
-        if constexpr (VEC == 8) top = q8_top(__ldg(reinterpret_cast<const uint4*>(xr + c)), top);
-        else top = max(top, (uint32_t)(__ldg(xr + c) & 0x7fff));
+        for (int c = tid; c < N; c += blockDim.x) top = max(top, (uint32_t)(__ldg(xr + c) & 0x7fff));
     }
     top = warp_top(top);
     if (lane == 0) red[warp] = top;
@@ -93,20 +101,30 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const uint16_t* x, i
     for (int i = 0; i < (int)(blockDim.x >> 5); ++i) top = max(top, red[i]);
     const Q8Row by = q8_row<BF16>(top);
     if (tid == 0) scale[row] = by.scale;
+    if constexpr (PACKS > 0) {
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) {
+            const int c = (p * (int)blockDim.x + tid) * 8;
+            if (c < N) *reinterpret_cast<uint2*>(qr + c) = q8_pack<BF16>(v[p], by);
+        }
+    } else {
 #pragma unroll 4
-    for (int c = tid * VEC; c < N; c += blockDim.x * VEC) {
-        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(qr + c) = q8_pack<BF16>(__ldg(reinterpret_cast<const uint4*>(xr + c)), by);
-        else qr[c] = q8_one<BF16>(__ldg(xr + c), by);
+        for (int c = tid; c < N; c += blockDim.x) qr[c] = q8_one<BF16>(__ldg(xr + c), by);
     }
+}
+template <int PACKS>
+static const void* quantize_fn(int bf16) {
+    return bf16 ? (const void*)quantize_rows_kernel<true, PACKS> : (const void*)quantize_rows_kernel<false, PACKS>;
 }
 
 static int launch_quantize(const void* x, int8_t* q, float* scale, int64_t rows, int64_t N, int64_t ldx, int64_t ldq, int bf16, int release, cudaStream_t stream) {
-    const bool vec = aligned16(x) && ldx % 8 == 0 && N % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ldq % 8 == 0;
-    const int64_t per = vec ? 8 : 1;
-    int threads = (int)((N + per * 32 - 1) / (per * 32) * 32);
-    if (threads > 512) threads = 512;
-    const void* fn = vec ? (bf16 ? (const void*)quantize_rows_kernel<true, 8> : (const void*)quantize_rows_kernel<false, 8>)
-                         : (bf16 ? (const void*)quantize_rows_kernel<true, 1> : (const void*)quantize_rows_kernel<false, 1>);
+    // Many rows: four packs a thread, so that all rows' CTAs are there at once (2048 x 4096: 8.8 us); few: one.
+    const bool vec = aligned16(x) && ldx % 8 == 0 && N % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ldq % 8 == 0 && N <= 8 * 8 * 512;
+    const int64_t packs = (N + 7) / 8;
+    const int per = !vec ? 0 : packs > 4 * 512 ? 8 : packs > 512 || (rows > 2 * sm_count() && packs >= 128) ? 4 : 1;
+    const int64_t need = vec ? (packs + per - 1) / per : N;
+    const int threads = (int)(need > 512 ? 512 : (need + 31) / 32 * 32);
+    const void* fn = per == 8 ? quantize_fn<8>(bf16) : per == 4 ? quantize_fn<4>(bf16) : per == 1 ? quantize_fn<1>(bf16) : quantize_fn<0>(bf16);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows);
     cfg.blockDim = dim3(threads);

@@ -454,7 +454,7 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
         if (dw) {
             MmParams<RowsEpilogue<OUT>> P = {};
             P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
-            const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
+            const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
             if (st != NQ_OK) return st;
         }
         if (dh) {

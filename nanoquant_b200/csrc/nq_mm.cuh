@@ -34,7 +34,7 @@ struct MmShape {
     int stages, stage_bytes, a_stage;  // bytes of a stage, and of A in it
     int m_fast;                    // consecutive tiles share their columns
     int a_box, b_box;              // K-major: rows per load; MN-major: loads of 64 rows
-    int a_mn, b_mn;                // operand has m / n contiguous
+    int a_mn, b_mn;                // operand has m / n contiguous (2: its boxes in one load)
     int kel;                       // elements of k per step
     int early_b;                   // B does not depend on the kernel before
     int release;                   // the kernel behind may start early (it is one of the same call and waits for this one's results)
@@ -91,6 +91,15 @@ __device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, in
                      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
     else
         tma_load_2d(dst, map, c0, c1, bar);
+}
+template <int CG>
+__device__ __forceinline__ void mm_load_columns(uint32_t dst, const CUtensorMap* map, int c1, int c2, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 // 32 columns of this warp's 32 rows: lane i has row i.
 __device__ __forceinline__ void mm_tmem_start(uint32_t taddr, uint32_t (&r)[32]) {
@@ -231,7 +240,9 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         auto load_a = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
             if constexpr (kBuildA) return;
             const int m0 = (T.m * CG + rank) * 128;
-            if (S.a_mn) {
+            if (S.a_mn == 2) {
+                mm_load_columns<CG>(dst, &P.map_a, k * S.kel, m0 >> 6, bar);
+            } else if (S.a_mn) {
                 for (int i = 0; i < S.a_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_a, m0 + 64 * i, k * S.kel, bar);
             } else {
                 mm_load<CG>(dst, &P.map_a, k * S.kel, m0, bar);
@@ -239,7 +250,9 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         };
         auto load_b = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
             const int n0 = T.n * S.bn + rank * (S.bn / CG);
-            if (S.b_mn) {
+            if (S.b_mn == 2) {
+                mm_load_columns<CG>(dst, &P.map_b, k * S.kel, n0 >> 6, bar);
+            } else if (S.b_mn) {
                 for (int i = 0; i < S.b_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_b, n0 + 64 * i, k * S.kel, bar);
             } else {
                 mm_load<CG>(dst, &P.map_b, k * S.kel, n0, bar);
@@ -432,6 +445,7 @@ struct MmOperand {
     const void* p;
     int64_t stride;       // bytes between its rows in memory
     int mn;
+    int64_t extent = 0;   // (mn) `rows` that may be read, if more
 };
 
 // Width of the tiles: the multiple of `unit` up to 256 that takes least time, in columns of a k step.
@@ -475,7 +489,11 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
     if (splits > S.ksteps) splits = S.ksteps;
     S.steps_per_split = (S.ksteps + splits - 1) / splits;
     S.splits = (S.ksteps + S.steps_per_split - 1) / S.steps_per_split;
-    S.a_mn = A.mn; S.b_mn = B.mn;
+    // (all of an operand's columns of 64 by one load: by one load each, both operands' kept the producer busy longer than the MMAs; the gradient of
+    // 50688 x 4096 weights over 2048 tokens 612 us -> 524)
+    const int64_t am = A.extent > M ? A.extent : M, bm = B.extent > N ? B.extent : N;
+    S.a_mn = A.mn ? (am % 64 == 0 ? 2 : 1) : 0;
+    S.b_mn = B.mn ? (bm % 64 == 0 ? 2 : 1) : 0;
     S.a_box = A.mn ? 2 : CG == 2 || M >= 128 ? 128 : (M + 7) / 8 * 8;
     S.b_box = B.mn ? bn / CG / 64 : bn / CG;
     S.a_stage = Epi::kBuildA ? 0 : S.a_mn ? kMmABytes : S.a_box * 128;
@@ -491,9 +509,9 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
               (uint32_t)(bn >> 3) << 17 | (uint32_t)(128 * CG >> 4) << 24;
     S.wait_limit = gemm_wait_limit();
     S.status = status;
-    int st = Epi::kBuildA ? NQ_OK : A.mn ? mm_encode(&P.map_a, A.p, type, M, K, A.stride, 64, 64) : mm_encode(&P.map_a, A.p, type, K, M, A.stride, S.kel, S.a_box);
+    int st = Epi::kBuildA ? NQ_OK : S.a_mn == 2 ? mm_encode_columns(&P.map_a, A.p, type, am, K, A.stride, S.a_box) : A.mn ? mm_encode(&P.map_a, A.p, type, am, K, A.stride, 64, 64) : mm_encode(&P.map_a, A.p, type, K, M, A.stride, S.kel, S.a_box);
     if (st != NQ_OK) return st;
-    st = B.mn ? mm_encode(&P.map_b, B.p, type, N, K, B.stride, 64, 64) : mm_encode(&P.map_b, B.p, type, K, N, B.stride, S.kel, S.b_box);
+    st = S.b_mn == 2 ? mm_encode_columns(&P.map_b, B.p, type, bm, K, B.stride, S.b_box) : B.mn ? mm_encode(&P.map_b, B.p, type, bm, K, B.stride, 64, 64) : mm_encode(&P.map_b, B.p, type, K, N, B.stride, S.kel, S.b_box);
     if (st != NQ_OK) return st;
     const int64_t tiles = (int64_t)S.m_tiles * S.n_tiles * S.splits, most = sm_count() / CG;
     if (tiles > 0x3fffffff) return NQ_ERR_TOO_LARGE;

@@ -73,5 +73,7 @@ int launch_pgemm_stage(const StageJob* jobs, int n, int T, StageTypes ty, int sa
 // 128-byte swizzle.
 enum : int { kMmF16 = 0, kMmBf16 = 1, kMmS8 = 2 };
 int mm_encode(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int box_inner, int box_outer);
+// The same matrix as [inner / 64][outer][64], for one load of `boxes` columns of 64 x 64 elements (inner a multiple of 64).
+int mm_encode_columns(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int boxes);
 
 }  // namespace nq

@@ -38,7 +38,7 @@ def make(T, N, V, dtype, seed=0):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 17), (5, 1003), (64, 4096), (2, 40000)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 17), (5, 1003), (64, 4096), (2, 40000), (400, 128), (301, 1024), (300, 4104), (3, 16384), (2, 16392), (2, 32768)])
 def test_quantize_is_exact(rows, cols, dtype):
     from nanoquant_b200 import ops
 
