@@ -202,7 +202,7 @@ struct Int8Epilogue {
         row0 = row & ~31;
         sx = row < s.M ? (FEW ? few[row] : __ldcg(p.xs + row)) : 0.f;
     }
-    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage, int half) {
         const float* ws = p.ws + n0 + c;
         uint32_t w[16];
 #pragma unroll
@@ -225,7 +225,10 @@ struct Int8Epilogue {
             w[i / 2] = pack_outputs<OUT>(f[0], f[1], 0);
             w[i / 2 + 1] = pack_outputs<OUT>(f[2], f[3], 0);
         }
-        mm_store_rows(stage, w, p.y + row0 * p.ldy + n0 + c, p.ldy, min(32, s.M - row0), cols, p.wide);
+        mm_stage_row(stage, half, w);
+    }
+    __device__ __forceinline__ void flush(int c, int cols, const unsigned char* stage) {
+        mm_store_rows(stage, p.y + row0 * p.ldy + n0 + c, p.ldy, min(32, s.M - row0), cols, p.wide);
     }
     __device__ __forceinline__ void end() {}
 };

@@ -61,7 +61,7 @@ struct LseEpilogue {
         top = -INFINITY;
         sum = 0.f;
     }
-    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char*) {
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char*, int) {
         float cm = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -89,12 +89,14 @@ struct LseEpilogue {
     }
 };
 
-// Eight tokens a CTA of 256 threads (so that the CTAs are there before the product's have left), 32 threads for each; the pieces of a token in the
-// same order whatever else there is.  A target that is no word of the vocabulary (and not `ignore`) makes its token NaN.
+// ROWS tokens a CTA of 256 threads (so that the CTAs are there before the product's have left): eight, whose pieces lie side by side, or for few tokens
+// one, with all threads on its pieces (151936 words have some 1600).  A target that is no word of the vocabulary (and not `ignore`) makes its token NaN.
+template <int ROWS>
 __global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V) {
-    __shared__ float2 red[8][33];
+    constexpr int kPieces = 256 / ROWS;            // threads of a token
+    __shared__ float2 red[ROWS][kPieces / 32 > 1 ? kPieces / 32 : 33];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int sub = threadIdx.x & 7, piece = threadIdx.x >> 3, row = blockIdx.x * 8 + sub;
+    const int sub = threadIdx.x % ROWS, piece = threadIdx.x / ROWS, row = blockIdx.x * ROWS + sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto join = [](float2 a, float2 b) {
         const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
@@ -103,21 +105,33 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const
     float2 v = make_float2(-INFINITY, 0.f);
     if (row < T) {
         int i = piece;
-        for (; i + 7 * 32 < slots; i += 8 * 32) {      // eight loads in flight
+        for (; i + 7 * kPieces < slots; i += 8 * kPieces) {      // eight loads in flight
             float2 p[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) p[k] = __ldcg(part + (long long)(i + 32 * k) * T + row);
+            for (int k = 0; k < 8; ++k) p[k] = __ldcg(part + (long long)(i + kPieces * k) * T + row);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v = join(v, p[k]);
         }
-        for (; i < slots; i += 32) v = join(v, __ldcg(part + (long long)i * T + row));
+        for (; i < slots; i += kPieces) v = join(v, __ldcg(part + (long long)i * T + row));
     }
-    red[sub][piece] = v;
-    __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x * 8 + warp;
-    v = red[warp][lane];
+    auto warp_join = [&](float2 a) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+        for (int o = 16; o > 0; o >>= 1) a = join(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
+        return a;
+    };
+    int r = blockIdx.x;
+    if constexpr (ROWS == 1) {
+        v = warp_join(v);
+        if (lane == 0) red[0][warp] = v;
+        __syncthreads();
+        if (warp > 0) return;
+        v = warp_join(lane < 8 ? red[0][lane] : make_float2(-INFINITY, 0.f));
+    } else {
+        red[sub][piece] = v;
+        __syncthreads();
+        r = blockIdx.x * ROWS + warp;
+        v = warp_join(red[warp][lane]);
+    }
     if (lane == 0 && r < T) {
         const long long t = loss_target(targets, r);
         float l = v.x * kLn2 + logf(v.y), loss = 0.f;
@@ -249,8 +263,7 @@ struct GradEpilogue {
             scale = __ldg(p.row_scale + row);
         }
     }
-    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
-        const int row0 = row & ~31;
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int, unsigned char* stage, int half) {
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -263,7 +276,11 @@ struct GradEpilogue {
             }
             w[i / 2] = pack_outputs<OUT>(d[0], d[1], 0);
         }
-        mm_store_rows(stage, w, p.d + row0 * p.ldd + n0 + c, p.ldd, min(32, s.M - row0), cols, true);
+        mm_stage_row(stage, half, w);
+    }
+    __device__ __forceinline__ void flush(int c, int cols, const unsigned char* stage) {
+        const int row0 = row & ~31;
+        mm_store_rows(stage, p.d + row0 * p.ldd + n0 + c, p.ldd, min(32, s.M - row0), cols, true);
     }
     __device__ __forceinline__ void end() {}
 };
@@ -287,11 +304,14 @@ struct RowsEpilogue {
         row0 = row & ~31;
         n0 = n0_;
     }
-    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int cols, unsigned char* stage) {
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int, unsigned char* stage, int half) {
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = pack_outputs<OUT>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f, 0);
-        mm_store_rows(stage, w, p.out + row0 * p.ld + n0 + c, p.ld, min(32, s.M - row0), cols, true);
+        mm_stage_row(stage, half, w);
+    }
+    __device__ __forceinline__ void flush(int c, int cols, const unsigned char* stage) {
+        mm_store_rows(stage, p.out + row0 * p.ld + n0 + c, p.ld, min(32, s.M - row0), cols, true);
     }
     __device__ __forceinline__ void end() {}
 };
@@ -314,7 +334,7 @@ struct SumEpilogue {
         n0 = n0_;
         dst = p.sums + (((long long)split * p.blocks + (row >> 7)) * p.quads + (n0 >> 2)) * 128 + (row & 127);
     }
-    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int, unsigned char*) {
+    __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int, unsigned char*, int) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float4* q = dst + (long long)((c >> 2) + i) * 128;
@@ -326,6 +346,7 @@ struct SumEpilogue {
             *q = v;
         }
     }
+    __device__ __forceinline__ void flush(int, int, const unsigned char*) {}
     __device__ __forceinline__ void end() {}
 };
 
@@ -509,7 +530,8 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     if (st != NQ_OK) return st;
     int slots = p.slots, t = (int)T, v = (int)V, mean = reduction == NQ_REDUCE_MEAN;
     void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v};
-    st = launch_plain((const void*)lse_join_kernel, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
+    st = T <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)T), 256, join_args, s)
+                             : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
     if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;
     void* sum_args[] = {&row_loss, &tg, &loss, &count, &t, &mean};
     return launch_plain((const void*)loss_sum_kernel, dim3(1), 1024, sum_args, s);

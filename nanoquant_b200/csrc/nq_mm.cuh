@@ -9,7 +9,7 @@
 //
 //   warp 0       operands by TMA, 128 bytes of k per step, 128-byte swizzle
 //   warp 1       MMAs (the pair's first CTA), four per step
-//   warps 4-11   epilogue, two sets of four warps, 32 columns in turn; tensor memory holds two accumulators, so that the epilogue
+//   warps 4-11   epilogue, two sets of four warps, 64 columns in turn; tensor memory holds two accumulators, so that the epilogue
 //                of a tile runs beside the main loop of the next
 //
 // `bn` is a multiple of 16 up to 256 that the host chooses so that the tiles fill whole rounds of the SMs.  A product over a long k and
@@ -22,7 +22,7 @@
 namespace nq {
 
 constexpr int kMmThreads = 32 * 12, kMmEpilogueWarps = 8;
-constexpr int kMmMaxStages = 24, kMmABytes = 128 * 128, kMmStageOut = 2048;   // (bytes of output staging per epilogue warp)
+constexpr int kMmMaxStages = 24, kMmABytes = 128 * 128, kMmStageOut = 4096;   // (bytes of output staging per epilogue warp)
 constexpr int kMmBarOff = 0, kMmFewOff = 512, kMmOutOff = 1024, kMmStageOff = kMmOutOff + kMmEpilogueWarps * kMmStageOut;
 constexpr int kMmSmemMost = 226 * 1024;
 constexpr int kMmAccCols = 256;
@@ -120,33 +120,32 @@ __device__ __forceinline__ void mm_tmem_use(uint32_t (&r)[32]) {
                    "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
-__device__ __forceinline__ void mm_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    mm_tmem_start(taddr, r);
-    mm_tmem_landed();
-    mm_tmem_use(r);
-}
-
-// 32 rows x 32 columns of 16-bit outputs, lane i holding row i as 16 words: through 2 KB of the warp's shared memory, so that four lanes
-// store a row's 64 bytes (whole sectors).  `rows` / `cols` of them exist; `wide`: the rows start at 16-byte boundaries.
-__device__ __forceinline__ void mm_store_rows(unsigned char* stage, const uint32_t (&w)[16], uint16_t* out, long long ld, int rows, int cols, bool wide) {
+// 32 rows x 64 columns of 16-bit outputs through 4 KB of the warp's shared memory, so that eight lanes store a row's 128 bytes: lane i brings row i,
+// 32 columns (`half` 0 or 1) as 16 words at a time.
+__device__ __forceinline__ void mm_stage_row(unsigned char* stage, int half, const uint32_t (&w)[16]) {
     const int lane = threadIdx.x & 31;
-    __syncwarp();
+    if (half == 0) __syncwarp();          // the stores before have read theirs
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+// `rows` / `cols` of them exist; `wide`: the rows start at 16-byte boundaries.
+__device__ __forceinline__ void mm_store_rows(const unsigned char* stage, uint16_t* out, long long ld, int rows, int cols, bool wide) {
+    const int lane = threadIdx.x & 31;
     __syncwarp();
     if (wide) {
-        const int j = lane & 3;
+        const int j = lane & 7;
+        uint16_t* dst = out + (lane >> 3) * ld + 8 * j;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2);
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
-            if (r < rows) store_rows(out + r * ld + 8 * j, v, cols - 8 * j, 8 * j + 8 <= cols);
+        for (int i = 0; i < 8; ++i, dst += 4 * ld) {
+            const int r = 4 * i + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((j ^ (r & 7)) << 4));
+            if (r < rows) store_rows(dst, v, cols - 8 * j, 8 * j + 8 <= cols);
         }
-    } else if (lane < cols) {
-        const int j = lane >> 3, b = (lane & 7) * 2;
-        for (int r = 0; r < rows; ++r)
-            out[r * ld + lane] = *reinterpret_cast<const uint16_t*>(stage + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + b);
+    } else {
+        for (int c = lane; c < cols; c += 32)
+            for (int r = 0; r < rows; ++r)
+                out[r * ld + c] = *reinterpret_cast<const uint16_t*>(stage + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + 2 * (c & 7));
     }
 }
 
@@ -155,7 +154,8 @@ __device__ __forceinline__ void mm_store_rows(unsigned char* stage, const uint32
 // are, whose results nobody looks at); an object per epilogue thread with
 //   Epi(const Params&, const MmShape&)
 //   begin(row, n0, m_tile, n_tile, split, ...)      a tile of this thread's row (row >= M: none)
-//   chunk(r, c, cols, stage)                        32 columns from n0 + c, `cols` of which exist (all lanes call it, if any of their rows exists)
+//   chunk(r, c, cols, stage, half)                  32 columns from n0 + c, `cols` of which exist (all lanes call it, if any of their rows exists)
+//   flush(c, cols, stage)                           behind both halves of 64 columns
 //   end()
 // kChunk: steps of k after which the accumulator is added to fp32 sums in registers (0: never).  The tensor cores cut an accumulator off, towards zero, with every
 // instruction, so that the error of a long sum grows with its length, and has a sign: logits of 8 were 2.8e-5 low at 4096 columns, five times the
@@ -375,10 +375,10 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                     const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
 #pragma unroll
                     for (int j = 0; j < kMmAccCols / 64; j += 2) {        // (two loads under way)
-                        if (32 * set + 64 * j < live && some) {
+                        if (64 * set + 64 * j < live && some) {
                             uint32_t r0[32], r1[32];
-                            mm_tmem_start(d + (uint32_t)(32 * set + 64 * j), r0);
-                            mm_tmem_start(d + (uint32_t)(32 * set + 64 * j + 64), r1);      // (within the accumulator, whatever the tile's width)
+                            mm_tmem_start(d + (uint32_t)(64 * set + 64 * j), r0);
+                            mm_tmem_start(d + (uint32_t)(64 * set + 64 * j + 32), r1);      // (within the accumulator, whatever the tile's width)
                             mm_tmem_landed();
                             mm_tmem_use(r0);
 #pragma unroll
@@ -394,12 +394,12 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                 epi.begin(row, n0, set, T.n, T.split);
 #pragma unroll
                 for (int j = 0; j < kMmAccCols / 64; ++j) {
-                    const int c = 32 * set + 64 * j;
+                    const int c = 64 * set + 64 * (j & ~1) + 32 * (j & 1);
                     if (c < live && some) {
                         uint32_t r[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sum[j][i]);
-                        epi.chunk(r, c, min(32, live - c), stage);
+                        epi.chunk(r, c, min(32, live - c), stage, j & 1);
                     }
                 }
             } else {
@@ -407,10 +407,16 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                 epi.begin(row, n0, set, T.n, T.split);
                 const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols) + ((uint32_t)(32 * ew) << 16);
 #pragma unroll 1
-                for (int c = 32 * set; c < live && some; c += 64) {
-                    uint32_t r[32];
-                    mm_tmem_ld32(d + (uint32_t)c, r);
-                    epi.chunk(r, c, min(32, live - c), stage);
+                for (int c = 64 * set; c < live && some; c += 128) {
+                    uint32_t r0[32], r1[32];
+                    mm_tmem_start(d + (uint32_t)c, r0);
+                    mm_tmem_start(d + (uint32_t)c + 32u, r1);      // (within the accumulator, whatever the tile's width)
+                    mm_tmem_landed();
+                    mm_tmem_use(r0);
+                    epi.chunk(r0, c, min(32, live - c), stage, 0);
+                    mm_tmem_use(r1);
+                    if (c + 32 < live) epi.chunk(r1, c + 32, min(32, live - c - 32), stage, 1);
+                    epi.flush(c, min(64, live - c), stage);
                 }
                 empty();
             }
