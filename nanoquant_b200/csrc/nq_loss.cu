@@ -18,6 +18,7 @@ namespace nq {
 
 constexpr int64_t kLossPieceBytes = 256ll << 20;
 constexpr int kLossPieceUnit = 256;
+constexpr int kLossJoinHere = 8192;        // pieces of all tokens that one CTA joins
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // fp16 holds d as multiples of this fraction of the largest |g|: probabilities down to 4e-9 of it are normal numbers.  (bf16 has the exponents of fp32.)
 constexpr float kLossHalfScale = 16384.f;
@@ -89,8 +90,28 @@ struct LseEpilogue {
     }
 };
 
+__device__ __forceinline__ float2 lse_join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
+    return make_float2(m, a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base));
+}
+__device__ __forceinline__ float2 lse_warp_join(float2 a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = lse_join(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
+    return a;
+}
+// Loss and lse of token r from its joined pieces.  A target that is no word of the vocabulary (and not `ignore`) makes both NaN.
+__device__ __forceinline__ float lse_finish(float2 v, int r, const float* target_logit, const LossTargets& targets, int V, float* lse) {
+    const long long t = loss_target(targets, r);
+    float l = v.x * kLn2 + logf(v.y), loss = 0.f;
+    if (t != targets.ignore) {
+        if (t >= 0 && t < V) loss = l - __ldcg(target_logit + r);
+        else loss = l = __int_as_float(0x7fffffff);
+    }
+    lse[r] = l;
+    return loss;
+}
 // ROWS tokens a CTA of 256 threads (so that the CTAs are there before the product's have left): eight, whose pieces lie side by side, or for few tokens
-// one, with all threads on its pieces (151936 words have some 1600).  A target that is no word of the vocabulary (and not `ignore`) makes its token NaN.
+// one, with all threads on its pieces (151936 words have some 1600).
 template <int ROWS>
 __global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V) {
     constexpr int kPieces = 256 / ROWS;            // threads of a token
@@ -98,10 +119,6 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int sub = threadIdx.x % ROWS, piece = threadIdx.x / ROWS, row = blockIdx.x * ROWS + sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto join = [](float2 a, float2 b) {
-        const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
-        return make_float2(m, a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base));
-    };
     float2 v = make_float2(-INFINITY, 0.f);
     if (row < T) {
         int i = piece;
@@ -110,51 +127,51 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const
 #pragma unroll
             for (int k = 0; k < 8; ++k) p[k] = __ldcg(part + (long long)(i + kPieces * k) * T + row);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v = join(v, p[k]);
+            for (int k = 0; k < 8; ++k) v = lse_join(v, p[k]);
         }
-        for (; i < slots; i += kPieces) v = join(v, __ldcg(part + (long long)i * T + row));
+        for (; i < slots; i += kPieces) v = lse_join(v, __ldcg(part + (long long)i * T + row));
     }
-    auto warp_join = [&](float2 a) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a = join(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
-        return a;
-    };
     int r = blockIdx.x;
     if constexpr (ROWS == 1) {
-        v = warp_join(v);
+        v = lse_warp_join(v);
         if (lane == 0) red[0][warp] = v;
         __syncthreads();
         if (warp > 0) return;
-        v = warp_join(lane < 8 ? red[0][lane] : make_float2(-INFINITY, 0.f));
+        v = lse_warp_join(lane < 8 ? red[0][lane] : make_float2(-INFINITY, 0.f));
     } else {
         red[sub][piece] = v;
         __syncthreads();
         r = blockIdx.x * ROWS + warp;
-        v = warp_join(red[warp][lane]);
+        v = lse_warp_join(red[warp][lane]);
     }
-    if (lane == 0 && r < T) {
-        const long long t = loss_target(targets, r);
-        float l = v.x * kLn2 + logf(v.y), loss = 0.f;
-        if (t != targets.ignore) {
-            if (t >= 0 && t < V) loss = l - __ldcg(target_logit + r);
-            else loss = l = __int_as_float(0x7fffffff);
-        }
-        row_loss[r] = loss;
-        lse[r] = l;
-    }
+    if (lane == 0 && r < T) row_loss[r] = lse_finish(v, r, target_logit, targets, V, lse);
 }
 
-// Sum (mean: of the tokens with a target) of the tokens' losses and the number of these tokens; one CTA, a fixed order, 64-bit sums.
-__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* row_loss, LossTargets targets, float* out, float* count, int T, int mean) {
+// Sum (mean: of the tokens with a target) of the tokens' losses and the number of these tokens; one CTA, a fixed order, 64-bit sums.  With `part` the pieces
+// are joined here as well (a warp per token, few of them: one launch less).
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const float2* part, const float* target_logit, float* row_loss, float* lse, LossTargets targets, float* out, float* count,
+                                                        int slots, int T, int V, int mean) {
     __shared__ double sums[32];
     __shared__ int counts[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     double s = 0;
     int n = 0;
-    for (int i = threadIdx.x; i < T; i += 1024) {
-        s += __ldcg(row_loss + i);
-        n += loss_target(targets, i) != targets.ignore;
+    if (part) {
+        for (int r = warp; r < T; r += 32) {
+            float2 v = make_float2(-INFINITY, 0.f);
+            for (int i = lane; i < slots; i += 32) v = lse_join(v, __ldcg(part + (long long)i * T + r));
+            v = lse_warp_join(v);
+            if (lane == 0) {
+                s += lse_finish(v, r, target_logit, targets, V, lse);
+                n += loss_target(targets, r) != targets.ignore;
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < T; i += 1024) {
+            s += __ldcg(row_loss + i);
+            n += loss_target(targets, i) != targets.ignore;
+        }
     }
     auto reduce = [&]() {
 #pragma unroll
@@ -285,7 +302,7 @@ struct GradEpilogue {
     __device__ __forceinline__ void end() {}
 };
 
-// dw of a piece: rows of words, times the final scale.
+// dw of a piece (or dh): rows of words, times the final scale.
 template <int OUT>
 struct RowsEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
@@ -395,6 +412,7 @@ struct LossPlan {
     int bn, slots;                       // forward
     int64_t piece;                       // words
     int d_bn, w_bn, h_bn, h_splits, h_blocks, h_quads;
+    bool h_direct;                       // one piece, one split: dh as the product writes it
 };
 static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     LossPlan p;
@@ -411,15 +429,19 @@ static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     }
     p.d_bn = mm_tile_cols((int)(p.piece < V ? p.piece : V), m_tiles, cg, 64);
     p.w_bn = N <= 128 ? 128 : 256;
-    // dh: few tiles over a long k.  Rounds of the longest tile, plus what writing and adding one more set of sums costs.
+    // dh: few tiles over a long k, in us: rounds of the longest tile (a step takes 0.27, a tile's start and end as much as 8), the launch that adds the
+    // splits' sums, and what writing (with several pieces, also reading) and adding them moves.
     p.h_bn = cg == 2 ? (N <= 128 ? 128 : 256) : (N <= 64 ? 64 : N <= 128 ? 128 : 256);
     const int64_t tiles = (int64_t)m_tiles * ((N + p.h_bn - 1) / p.h_bn), steps = ((p.piece < V ? p.piece : V) + 63) / 64;
+    const bool one = p.piece >= V;
     p.h_splits = 1;
+    p.h_direct = one;
     double best = 0;
     for (int s = 1; s <= 32 && s <= steps; ++s) {
-        if (s > 1 && s * tiles * p.h_bn * 128 * cg * 4 > kLossPieceBytes) break;
-        const double cost = (double)((tiles * s + groups - 1) / groups) * (double)((steps + s - 1) / s + 8) + 0.12 * (double)(tiles * s) / groups * 32;
-        if (s == 1 || cost < best) { best = cost; p.h_splits = s; }
+        const int64_t bytes = s * tiles * p.h_bn * 128 * cg * 4;
+        if (s > 1 && bytes > kLossPieceBytes) break;
+        const double cost = 0.27 * (double)((tiles * s + groups - 1) / groups) * (double)((steps + s - 1) / s + 8) + (one && s == 1 ? 0. : 5. + (one ? 2 : 4) * (double)bytes * 1e-6 / 5.);
+        if (s == 1 || cost < best) { best = cost; p.h_splits = s; p.h_direct = one && s == 1; }
     }
     p.h_blocks = m_tiles * cg;
     p.h_quads = (int)(up(N, p.h_bn) / 4);
@@ -432,7 +454,7 @@ static LossScratch loss_scratch(const LossPlan& p, int64_t T, int64_t N) {
     auto take = [&](int64_t bytes) { const int64_t here = at; at += up(bytes, 256); return here; };
     s.d = take(T * p.piece * 2);
     s.h = take(T * N * 2);
-    s.sums = take((int64_t)p.h_splits * p.h_blocks * p.h_quads * 128 * 16);
+    s.sums = take(p.h_direct ? 0 : (int64_t)p.h_splits * p.h_blocks * p.h_quads * 128 * 16);
     s.row_scale = take(T * 4);
     s.final_scale = take(4);
     s.bytes = at;
@@ -477,6 +499,11 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
             P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
             const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
             if (st != NQ_OK) return st;
+        }
+        if (dh && p.h_direct) {
+            MmParams<RowsEpilogue<OUT>> P = {};
+            P.e = {final_scale, static_cast<uint16_t*>(dh), lddh};
+            return mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, 1, 1, 0, status, stream);
         }
         if (dh) {
             MmParams<SumEpilogue> P = {};
@@ -529,11 +556,16 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
                        : launch_lse<1>(h, w, e, (int)T, (int)N, (int)V, ldh, ldw, type, p.bn, status, s);
     if (st != NQ_OK) return st;
     int slots = p.slots, t = (int)T, v = (int)V, mean = reduction == NQ_REDUCE_MEAN;
-    void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v};
-    st = T <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)T), 256, join_args, s)
-                             : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
-    if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;
-    void* sum_args[] = {&row_loss, &tg, &loss, &count, &t, &mean};
+    const float2* joined = nullptr;
+    if (reduction != NQ_REDUCE_NONE && T <= 1024 && T * slots <= kLossJoinHere) {
+        joined = part;
+    } else {
+        void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v};
+        st = T <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)T), 256, join_args, s)
+                                 : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
+        if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;
+    }
+    void* sum_args[] = {&joined, &target_logit, &row_loss, &lse, &tg, &loss, &count, &slots, &t, &v, &mean};
     return launch_plain((const void*)loss_sum_kernel, dim3(1), 1024, sum_args, s);
 }
 
