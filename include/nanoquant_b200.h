@@ -378,8 +378,8 @@ int nq_quantize_rows_s8(const void* x, int8_t* q, float* scale, int64_t rows, in
 /* y[t, v] = s_x[t] w_scale[v] sum_k q_x[t, k] w[v, k] (+ bias[v]): x [T, N] 16-bit, quantised per token as above within the call; w [V, ldw]
  * signed bytes (rows of nq_quantize_rows_s8, ldw a multiple of 16), exact int32 sums (N <= 131072), fp32 scaling, one rounding of y.
  * 16-byte aligned w, w_scale and scratch (nq_int8_linear_scratch_bytes(), 0 for few tokens; any contents).  `status_word` as in nq_onebit_gemm_fwd.
- * Few tokens stream w once, half the bytes of nq_dense_gemv_fwd; any number of tokens.  Weights may be read ahead of the completion of
- * the kernel before the call (see nq_gemm_fwd). */
+ * Few tokens stream w once, half the bytes of nq_dense_gemv_fwd; any number of tokens.  Nothing is read before the kernels ahead of the
+ * call have completed. */
 size_t nq_int8_linear_scratch_bytes(int64_t T, int64_t N);
 int nq_int8_linear_fwd(const void* x, const int8_t* w, const float* w_scale, const void* bias, void* y, void* scratch, size_t scratch_bytes,
                        void* status_word, int64_t T, int64_t N, int64_t V, int64_t ldx, int64_t ldw, int64_t ldy, int dtype,

@@ -136,7 +136,7 @@ static int launch_quantize(const void* x, int8_t* q, float* scale, int64_t rows,
     return launch_dependent(cfg, attr, 0, fn, args);
 }
 
-// FEW: up to kInt8Few tokens, quantised by every CTA for itself while its first weights are on their way (one launch, no copy of the quantised
+// FEW: up to kInt8Few tokens, quantised by every CTA for itself, beside its first weights' loads (one launch, no copy of the quantised
 // activations); otherwise their bytes and scales are in memory.  us with and without: one token 97.6 and 102.5 (151936 x 4096), 8.0 and 11.7 (512 x
 // 2048); two 100.3 and 102.6; four 104.1 and 103.3, sixteen 32.7 and 16.6 (12288 x 4096: every SM reads and converts all tokens).
 constexpr int kInt8Few = 2, kInt8FewBytes = 96 * 1024;       // tokens; bytes of A in shared memory
@@ -240,7 +240,7 @@ static int launch_int8(const typename Int8Epilogue<OUT, FEW>::Params& e, const i
     P.e = e;
     const int m_tiles = (T + 128 * CG - 1) / (128 * CG);
     const int bn = mm_tile_cols(V, m_tiles, CG, 16 * CG);
-    return mm_launch<CG>(P, kMmS8, {xq, ldq, 0}, {w, ldw, 0}, T, V, e.N, bn, 1, 1, 0, status, stream);
+    return mm_launch<CG>(P, kMmS8, {xq, ldq, 0}, {w, ldw, 0}, T, V, e.N, bn, 1, !FEW, 0, status, stream);
 }
 static bool int8_few(int64_t T, int64_t N) { return T <= kInt8Few && 1024 * ((N + 127) / 128) <= kInt8FewBytes; }
 template <int OUT>

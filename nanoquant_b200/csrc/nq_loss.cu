@@ -113,12 +113,12 @@ __device__ __forceinline__ float lse_finish(float2 v, int r, const float* target
 // ROWS tokens a CTA of 256 threads (so that the CTAs are there before the product's have left): eight, whose pieces lie side by side, or for few tokens
 // one, with all threads on its pieces (151936 words have some 1600).
 template <int ROWS>
-__global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V) {
+__global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V, int release) {
     constexpr int kPieces = 256 / ROWS;            // threads of a token
     __shared__ float2 red[ROWS][kPieces / 32 > 1 ? kPieces / 32 : 33];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int sub = threadIdx.x % ROWS, piece = threadIdx.x / ROWS, row = blockIdx.x * ROWS + sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     float2 v = make_float2(-INFINITY, 0.f);
     if (row < T) {
         int i = piece;
@@ -214,8 +214,8 @@ struct LossPrepare {
 __global__ void __launch_bounds__(512) loss_prepare_kernel(const LossPrepare P) {
     __shared__ float red[16];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // (behind the wait: what starts early may rely on everything before)
     if (blockIdx.x > 0) {
         const long long total = (long long)P.T * P.packs, step = (long long)(gridDim.x - 1) * 512;
         for (long long i = (long long)(blockIdx.x - 1) * 512 + threadIdx.x; i < total; i += step) {
@@ -474,7 +474,7 @@ static int launch_lse(const void* h, const void* w, const LseEpilogue::Params& e
                       unsigned* status, cudaStream_t stream) {
     MmParams<LseEpilogue> P = {};
     P.e = e;
-    return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 1, 1, status, stream);
+    return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 0, 1, status, stream);
 }
 
 template <int CG, int OUT>
@@ -560,7 +560,8 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     if (reduction != NQ_REDUCE_NONE && T <= 1024 && T * slots <= kLossJoinHere) {
         joined = part;
     } else {
-        void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v};
+        int release = reduction != NQ_REDUCE_NONE;
+        void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v, &release};
         st = T <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)T), 256, join_args, s)
                                  : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
         if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;

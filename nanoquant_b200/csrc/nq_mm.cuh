@@ -36,8 +36,8 @@ struct MmShape {
     int a_box, b_box;              // K-major: rows per load; MN-major: loads of 64 rows
     int a_mn, b_mn;                // operand has m / n contiguous (2: its boxes in one load)
     int kel;                       // elements of k per step
-    int early_b;                   // B does not depend on the kernel before
-    int release;                   // the kernel behind may start early (it is one of the same call and waits for this one's results)
+    int early_b;                   // B does not depend on the kernel before, which is one of the same call and has waited for all before it
+    int release;                   // the kernel behind, one of the same call, may start early (but behind everything before this one)
     int few;                       // (kBuildA) bytes of A per step: 1024 for every eight rows
     uint32_t idesc;
     unsigned wait_limit;
@@ -213,7 +213,6 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     tc_fence_after();
-    if (S.release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
     constexpr int kChunk = Epi::kChunk ? Epi::kChunk : 1 << 30;
     const int groups = (int)gridDim.x / CG, first = (int)blockIdx.x / CG, plane = S.m_tiles * S.n_tiles, tiles = plane * S.splits;
@@ -272,6 +271,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                 }
         }
         asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (S.release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         if (pre) {
             const Tile T = tile_of(first);
             if (elect_one())

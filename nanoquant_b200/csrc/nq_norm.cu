@@ -19,7 +19,8 @@
 namespace nq {
 
 constexpr int kNormMaxCols = 16384;
-constexpr int kNormCtasPerSm = 8;          // of the backward kernels at most: rows of partial sums per SM
+// CTAs of a backward kernel to an SM at most: rows of partial sums.
+static int norm_ctas_per_sm(int64_t N) { return N <= 2048 ? 8 : N <= 4096 ? 4 : 2; }
 
 struct NormParams {
     const void *x, *w, *b, *dy;
@@ -774,7 +775,8 @@ int choose_stream(bool bwd, bool bf16, bool center, const NormParams& P, NormStr
     NQ_CUDA_TRY(cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem));
     int per_sm = 1;
     NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.fn, v.threads, v.smem));
-    per_sm = per_sm < 1 ? 1 : per_sm > kNormCtasPerSm ? kNormCtasPerSm : per_sm;
+    const int most = bwd ? norm_ctas_per_sm(N) : 8;
+    per_sm = per_sm < 1 ? 1 : per_sm > most ? most : per_sm;
     const int64_t units = (P.rows + v.rows - 1) / v.rows;
     v.ctas = units < (int64_t)per_sm * sm_count() ? units : (int64_t)per_sm * sm_count();
     return NQ_OK;
@@ -835,7 +837,7 @@ int nq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, fl
 
 size_t nq_norm_bwd_scratch_bytes(int64_t rows, int64_t N) {
     if (rows < 1 || N < 1 || N > kNormMaxCols) return 0;
-    const int64_t most = (int64_t)kNormCtasPerSm * sm_count(), ctas = rows < most ? rows : most;
+    const int64_t most = (int64_t)norm_ctas_per_sm(N) * sm_count(), ctas = rows < most ? rows : most;
     return (size_t)(ctas * N * 2 * 4);
 }
 
@@ -871,7 +873,8 @@ int nq_norm_bwd(const void* dy, const void* x, const void* weight, const float* 
         v = choose_norm(true, bf16, center != 0, vec, rows, (int)N);
         int per_sm = 0;
         NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, (const void*)v.fn, v.threads, 0));
-        per_sm = per_sm < 1 ? 1 : per_sm > kNormCtasPerSm ? kNormCtasPerSm : per_sm;
+        const int most = norm_ctas_per_sm(N);
+        per_sm = per_sm < 1 ? 1 : per_sm > most ? most : per_sm;
         ctas = (rows + v.rows_per_cta - 1) / v.rows_per_cta;
         if (ctas > (int64_t)per_sm * sm_count()) ctas = (int64_t)per_sm * sm_count();
     }

@@ -562,17 +562,18 @@ bool capturing(int dev) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     return cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(), &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
 }
-// A leaf's gradient is accumulated on the stream on which its accumulator was made.  While another graph holds an accumulator made on another
-// stream, a captured backward pass would have that stream wait for the capture, which ends the process: refuse the call instead.
+// A leaf's gradient is accumulated on the stream on which its accumulator was made.  While another graph holds an accumulator made on the
+// default stream, a captured backward pass would have that stream wait for the capture, which it cannot, and which ends the process: refuse the
+// call instead.  (Other streams join the capture and leave it again.)
 void check_capture(int dev, std::initializer_list<const Tensor*> inputs) {
     if (!capturing(dev)) return;
-    const c10::Stream here = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).unwrap();
+    const c10::Stream first = c10::cuda::getDefaultCUDAStream((c10::DeviceIndex)dev).unwrap();
     for (const Tensor* t : inputs) {
         if (!t || !t->defined() || !t->requires_grad() || t->grad_fn()) continue;
         const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
-        TORCH_CHECK(!acc || !acc->stream() || *acc->stream() == here,
-                    "a leaf of this captured call is held by an autograd graph made on another stream: its gradient cannot be captured; "
-                    "release that graph first, or make it on the capturing stream");
+        TORCH_CHECK(!acc || !acc->stream() || *acc->stream() != first,
+                    "a leaf of this captured call is held by an autograd graph made on the default stream: its gradient cannot be captured; "
+                    "release that graph first, or make it on another stream");
     }
 }
 

@@ -204,6 +204,37 @@ def test_linear_in_two_cuda_graphs_at_once():
     assert all(torch.equal(o, v) for o, v in zip(outs, want))
 
 
+def test_wait_that_runs_out():
+    """The epilogue of a tile waits for its main loop, 250 us; with a limit of one attempt after the first (10 us in all) it gives up.  The launch ends all the
+    same, drains what is in flight, gives its tensor memory back and reports; the next one on a zeroed status word is right."""
+    from nanoquant_b200 import _lib, ops
+
+    L = _lib.lib()
+    T, N, V = 256, 131072, 256
+    x, w, _ = make(T, N, V, torch.bfloat16, seed=2)
+    q, s = ops.quantize_int8(w)
+    y = torch.empty((T, V), dtype=torch.bfloat16, device="cuda")
+    nb = L.nq_int8_linear_scratch_bytes(T, N)
+    scratch, header = torch.empty(nb, dtype=torch.uint8, device="cuda"), torch.zeros(256, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    call = lambda: _lib.check(L.nq_int8_linear_fwd(x.data_ptr(), q.data_ptr(), s.data_ptr(), None, y.data_ptr(), scratch.data_ptr(), nb, header.data_ptr(),
+                                                   T, N, V, N, q.stride(0), V, _lib.NQ_BF16, st), "nq_int8_linear_fwd")
+    status = lambda: L.nq_scratch_status(header.data_ptr(), st)
+    call()
+    assert status() == 0
+    check(y, expected(x, q, s, None), None)
+    old = L.nq_gemm_set_wait_limit(1)
+    try:
+        call()
+        assert status() == _lib.NQ_ERR_TIMEOUT
+    finally:
+        assert L.nq_gemm_set_wait_limit(old) == 1
+    header.zero_()
+    call()
+    assert status() == 0
+    check(y, expected(x, q, s, None), None)
+
+
 def test_linear_against_the_dense_head():
     """Near the 16-bit head it stands in for: each factor is off by at most half a step of max / 127."""
     from nanoquant_b200 import ops

@@ -234,7 +234,7 @@ def test_same_bits_every_time_on_two_streams_and_in_a_graph():
     assert torch.equal(loss.detach(), fresh[0]) and torch.equal(dh, fresh[1]) and torch.equal(dw, fresh[2])
 
 
-def test_capture_that_another_stream_holds_is_refused():
+def test_capture_that_the_default_stream_holds_is_refused():
     from nanoquant_b200 import ops
 
     h, w, t = make(10, 64, 100, torch.bfloat16)
@@ -246,6 +246,36 @@ def test_capture_that_another_stream_holds_is_refused():
         with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
             ops.linear_cross_entropy(h, w, t)
     assert torch.isfinite(held)
+
+
+def test_training_step_captured_behind_a_warm_up_that_is_still_held():
+    """The usual way to capture a training step: warm-up on a side stream, whose loss lives on while the step is captured."""
+    from nanoquant_b200 import ops
+
+    h, w, t = make(50, 128, 700, torch.bfloat16, seed=14)
+    gamma = torch.ones(128, device="cuda", requires_grad=True)
+    w.requires_grad_()
+    step = lambda: ops.linear_cross_entropy(ops.rms_norm(h, gamma), w, t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            gamma.grad = w.grad = None
+            loss = step()
+            loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    want = [loss.detach().clone(), gamma.grad.clone(), w.grad.clone()]
+    gamma.grad = w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+        captured.backward()
+    for p in (gamma, w):
+        p.grad.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    # (a captured backward pass writes a fresh gradient, as an eager one with grad = None does)
+    assert all(torch.equal(a, b) for a, b in zip((captured.detach(), gamma.grad, w.grad), want))
 
 
 def test_offsets_beyond_31_bits():

@@ -169,7 +169,7 @@ def test_norm_same_bits_every_time_and_in_a_graph():
     assert torch.equal(y.detach(), a[0]) and all(torch.equal(g, -p) for g, p in zip(grads, a[1:]))
 
 
-def test_norm_refuses_a_capture_whose_gradient_another_stream_holds():
+def test_norm_refuses_a_capture_whose_gradient_the_default_stream_holds():
     from nanoquant_b200 import ops
 
     x, w, b, dy = make((4, 64), torch.bfloat16, seed=8)
