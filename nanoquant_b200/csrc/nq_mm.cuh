@@ -455,7 +455,9 @@ struct MmOperand {
 };
 
 // Width of the tiles: the multiple of `unit` up to 256 that takes least time, in columns of a k step.
-// Pairs of CTAs are bound by the tensor cores: whole rounds of tiles over the pairs, 16 columns for a tile's start.
+// Pairs of CTAs: whole rounds of tiles over the pairs; a tile costs its columns and some 220 more, for its rows pass through L2 to the SMs as often as
+// there are tiles.  us at 128 / 160 / 192 / 224 / 256 columns: int8 12288 x 4096, 512 tokens 35.0 / 36.7 / 30.9 / 31.5 / 33.1, 4096 tokens 194 / 174 / 158 / 148 /
+// 143, 4096 x 12288, 2048 tokens 120 / 100 / 101 / 101 / 87; the loss of 2048 tokens at 128256 x 2048 1025 / 890 / 790 / 723 / 689.
 // Single CTAs have up to 128 rows and are bound by the memory that B streams from, as long as a step has enough of it: its four MMAs take as long for
 // 16 columns as for some 100 (they fetch 128 rows of A all the same).  The last tile's latency is what narrow tiles save.  One token, int8, us at
 // 32 / 64 / 96 / 128 / 176 / 208 / 256 columns: 128256 x 2048 106 / 58 / 47.5 / 44.2 / 48.6 / 51.9 / 48.3, 151936 x 4096 238 / 130 / 96.4 / 98.1 / 95.0 /
@@ -466,7 +468,7 @@ inline int mm_tile_cols(int N, int m_tiles, int cg, int least) {
     double best_cost = 0;
     for (int bn = 256; bn >= least; bn -= unit) {
         const int64_t tiles = (int64_t)((N + bn - 1) / bn) * m_tiles, rounds = (tiles + groups - 1) / groups;
-        const double cost = cg == 2 ? (double)rounds * (bn + 16) : (double)rounds * (bn > 100 ? bn : 100) + 0.4 * bn;
+        const double cost = cg == 2 ? (double)rounds * (bn + 220) : (double)rounds * (bn > 100 ? bn : 100) + 0.4 * bn;
         if (!best || cost < best_cost * 0.995) { best = bn; best_cost = cost; }
     }
     return best;
