@@ -66,7 +66,8 @@ def run(x, w, b, dy, center, eps=1e-5):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [
     (1, 4096), (2, 8), (1, 1), (5, 3), (7, 33), (129, 128), (600, 512), (40, 1000), (33, 1001), (300, 1024), (50, 2048), (700, 2056),
-    (297, 4096), (9, 4104), (3, 8192), (310, 8200), (5, 16384), (6, 4999), (3, 16383)])
+    (297, 4096), (9, 4104), (3, 8192), (310, 8200), (5, 16384), (6, 4999), (3, 16383),
+    (1201, 1), (700, 7), (333, 33), (1500, 511), (601, 1001), (400, 4097), (302, 8191), (299, 9001), (310, 16383), (2000, 640), (303, 16384), (5000, 72)])
 def test_norm_matches_definition(rows, cols, dtype, center):
     x, w, b, dy = make((rows, cols), dtype, seed=rows * 7 + cols)
     b = b if center else None
@@ -94,6 +95,15 @@ def test_norm_strides():
         d = torch.randn(x.shape, device="cuda").half()
         want, mags = reference(x, wn, bn, d, 1e-5, True)
         check(run(x.detach(), wn, bn, d, True), want, mags)
+    # many rows
+    base = torch.randn((700, 1100), device="cuda").half()
+    for x in (base[:, :1024], base[:, 3:1003], base[:, 8:520], base[:, 1:], base[::2, 5:9]):
+        n = x.size(-1)
+        wn, bn = w[:n].contiguous(), b[:n].contiguous()
+        d = torch.randn((*x.shape[:-1], n + 3), device="cuda").half()[..., 1:n + 1]       # gradients at any address
+        want, mags = reference(x, wn, bn, d, 1e-5, True)
+        check(run(x.detach(), wn, bn, d, True), want, mags)
+    base = base[:64]
     # the gradient of a sum is broadcast in every dimension
     x = base[:, :1024].detach().requires_grad_()
     ops.layer_norm(x, w[:1024].contiguous().detach()).float().sum().backward()
