@@ -18,6 +18,7 @@ namespace nq {
 
 constexpr int64_t kLossPieceBytes = 256ll << 20;
 constexpr int kLossPieceUnit = 256;
+constexpr int kLossRows = 16384;           // tokens of a forward product: the scratch holds 8 bytes for each and every 64 to 128 words
 constexpr int kLossJoinHere = 8192;        // pieces of all tokens that one CTA joins
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // fp16 holds d as multiples of this fraction of the largest |g|: probabilities down to 4e-9 of it are normal numbers.  (bf16 has the exponents of fp32.)
@@ -276,8 +277,8 @@ struct GradEpilogue {
             live = t != p.targets.ignore;
             const long long rel = t - p.v0 - n0;
             at = rel >= 0 && rel < kMmAccCols ? (int)rel : -1;
-            base = __ldg(p.lse + row) * kLog2e;
-            scale = __ldg(p.row_scale + row);
+            base = __ldcg(p.lse + row) * kLog2e;
+            scale = __ldcg(p.row_scale + row);
         }
     }
     __device__ __forceinline__ void chunk(const uint32_t (&r)[32], int c, int, unsigned char* stage, int half) {
@@ -316,7 +317,7 @@ struct RowsEpilogue {
     const MmShape& s;
     int row0, n0;
     float f;
-    __device__ RowsEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_), f(__ldg(p_.final_scale)) {}
+    __device__ RowsEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_), f(__ldcg(p_.final_scale)) {}
     __device__ __forceinline__ void begin(int row, int n0_, int, int, int) {
         row0 = row & ~31;
         n0 = n0_;
@@ -357,7 +358,7 @@ struct SumEpilogue {
             float4* q = dst + (long long)((c >> 2) + i) * 128;
             float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
             if (p.add) {
-                const float4 o = *q;
+                const float4 o = __ldcg(q);
                 v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
             }
             *q = v;
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(256) dh_kernel(const float4* sums, const float
     __shared__ uint32_t tile[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = blockIdx.x * 32, col0 = blockIdx.y * 64;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const float f = *final_scale;
+    const float f = __ldcg(final_scale);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int qd = 2 * warp + k, quad = (col0 >> 2) + qd;
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(256) dh_kernel(const float4* sums, const float
         if (quad < quads) {
 #pragma unroll 4
             for (int sp = 0; sp < splits; ++sp) {
-                const float4 o = sums[(((long long)sp * blocks + (row0 >> 7)) * quads + quad) * 128 + (row0 & 127) + lane];
+                const float4 o = __ldcg(sums + (((long long)sp * blocks + (row0 >> 7)) * quads + quad) * 128 + (row0 & 127) + lane);
                 v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
             }
         }
@@ -460,6 +461,20 @@ static LossScratch loss_scratch(const LossPlan& p, int64_t T, int64_t N) {
     s.bytes = at;
     return s;
 }
+// Forward: the pieces and the targets' logits of kLossRows tokens, the losses of all.
+struct LossFwdScratch { int64_t target_logit, row_loss, bytes; };
+static LossFwdScratch loss_fwd_scratch(int64_t T, int64_t N, int64_t V) {
+    LossFwdScratch s;
+    int64_t part = 0;
+    for (int64_t t : {T < kLossRows ? T : (int64_t)kLossRows, T % kLossRows}) {      // (the last product may be another one)
+        const int64_t bytes = t > 0 ? plan_loss(t, N, V).slots * t * 8 : 0;
+        if (bytes > part) part = bytes;
+    }
+    s.target_logit = up(part, 256);
+    s.row_loss = s.target_logit + up((T < kLossRows ? T : kLossRows) * 4, 256);
+    s.bytes = s.row_loss + up(T * 4, 256);
+    return s;
+}
 static int check_loss(int64_t T, int64_t N, int64_t V, int64_t ldh, int64_t ldw, int dtype, int reduction, int target_bits) {
     if (dtype != NQ_F16 && dtype != NQ_BF16) return NQ_ERR_DTYPE;
     if (target_bits != 32 && target_bits != 64) return NQ_ERR_DTYPE;
@@ -532,7 +547,7 @@ extern "C" {
 
 size_t nq_linear_ce_fwd_scratch_bytes(int64_t T, int64_t N, int64_t V) {
     if (check_loss(T, N, V, N, N, NQ_F16, NQ_REDUCE_NONE, 64) != NQ_OK) return 0;
-    return (size_t)(up((int64_t)plan_loss(T, N, V).slots * T * 8, 256) + 2 * up(T * 4, 256));
+    return (size_t)loss_fwd_scratch(T, N, V).bytes;
 }
 
 int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int target_bits, int64_t ignore_index, float* loss, float* lse,
@@ -545,28 +560,37 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     if (scratch_bytes < nq_linear_ce_fwd_scratch_bytes(T, N, V)) return NQ_ERR_SCRATCH;
     cudaStream_t s = as_stream(stream);
     unsigned* status = static_cast<unsigned*>(status_word) + 2;
-    const LossPlan p = plan_loss(T, N, V);
-    float2* part = static_cast<float2*>(scratch);
-    float* target_logit = reinterpret_cast<float*>(static_cast<char*>(scratch) + up((int64_t)p.slots * T * 8, 256));
-    float* row_loss = reduction == NQ_REDUCE_NONE ? loss : target_logit + up(T * 4, 256) / 4;
-    LossTargets tg = {targets, target_bits == 64, ignore_index};
-    const LseEpilogue::Params e = {tg, part, target_logit};
+    const LossFwdScratch at = loss_fwd_scratch(T, N, V);
+    char* base = static_cast<char*>(scratch);
+    float2* part = reinterpret_cast<float2*>(base);
+    float* target_logit = reinterpret_cast<float*>(base + at.target_logit);
+    float* row_loss = reduction == NQ_REDUCE_NONE ? loss : reinterpret_cast<float*>(base + at.row_loss);
     const int type = dtype == NQ_BF16 ? kMmBf16 : kMmF16;
-    st = loss_pairs(T) ? launch_lse<2>(h, w, e, (int)T, (int)N, (int)V, ldh, ldw, type, p.bn, status, s)
-                       : launch_lse<1>(h, w, e, (int)T, (int)N, (int)V, ldh, ldw, type, p.bn, status, s);
-    if (st != NQ_OK) return st;
-    int slots = p.slots, t = (int)T, v = (int)V, mean = reduction == NQ_REDUCE_MEAN;
+    LossTargets all = {targets, target_bits == 64, ignore_index};
     const float2* joined = nullptr;
-    if (reduction != NQ_REDUCE_NONE && T <= 1024 && T * slots <= kLossJoinHere) {
-        joined = part;
-    } else {
-        int release = reduction != NQ_REDUCE_NONE;
-        void* join_args[] = {&part, &target_logit, &tg, &row_loss, &lse, &slots, &t, &v, &release};
-        st = T <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)T), 256, join_args, s)
-                                 : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((T + 7) / 8)), 256, join_args, s);
-        if (st != NQ_OK || reduction == NQ_REDUCE_NONE) return st;
+    int slots = 0, v = (int)V, mean = reduction == NQ_REDUCE_MEAN, all_t = (int)T;
+    for (int64_t t0 = 0; t0 < T; t0 += kLossRows) {
+        int t = (int)(T - t0 < kLossRows ? T - t0 : kLossRows), release = reduction != NQ_REDUCE_NONE || t0 + t < T;
+        const LossPlan p = plan_loss(t, N, V);
+        slots = p.slots;
+        const char* rows = static_cast<const char*>(h) + t0 * ldh * 2;
+        LossTargets tg = {static_cast<const char*>(targets) + t0 * (target_bits / 8), all.wide, ignore_index};
+        const LseEpilogue::Params e = {tg, part, target_logit};
+        st = loss_pairs(t) ? launch_lse<2>(rows, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s)
+                           : launch_lse<1>(rows, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s);
+        if (st != NQ_OK) return st;
+        if (reduction != NQ_REDUCE_NONE && T <= 1024 && T * slots <= kLossJoinHere) {
+            joined = part;
+            break;
+        }
+        float *loss_out = row_loss + t0, *lse_out = lse + t0;
+        void* join_args[] = {&part, &target_logit, &tg, &loss_out, &lse_out, &slots, &t, &v, &release};
+        st = t <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)t), 256, join_args, s)
+                                 : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((t + 7) / 8)), 256, join_args, s);
+        if (st != NQ_OK) return st;
     }
-    void* sum_args[] = {&joined, &target_logit, &row_loss, &lse, &tg, &loss, &count, &slots, &t, &v, &mean};
+    if (reduction == NQ_REDUCE_NONE) return NQ_OK;
+    void* sum_args[] = {&joined, &target_logit, &row_loss, &lse, &all, &loss, &count, &slots, &all_t, &v, &mean};
     return launch_plain((const void*)loss_sum_kernel, dim3(1), 1024, sum_args, s);
 }
 

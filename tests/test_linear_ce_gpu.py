@@ -110,6 +110,20 @@ def test_loss_in_several_pieces_of_the_vocabulary(dtype):
     assert ((got[2][-3000:].double() - dw).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_more_tokens_than_one_product_takes(reduction):
+    """Several products of tokens, the last one of another kind; a token's loss is that of its own product alone."""
+    from nanoquant_b200 import ops
+
+    for T in (16384 + 100, 2 * 16384 + 300):
+        h, w, t = make(T, 64, 700, torch.bfloat16, seed=T)
+        got = run(h, w, t, reduction, 8.0)
+        check(got, reference(h, w, t, reduction, 8.0))
+        if reduction == "none":
+            for rows in (slice(0, 16384), slice(T // 16384 * 16384, T)):
+                assert torch.equal(got[0][rows], ops.linear_cross_entropy(h[rows], w, t[rows], reduction="none"))
+
+
 def test_gradient_matches_differences():
     """<dh, a> and <dw, b> against differences of the loss, with steps that the type holds exactly."""
     from nanoquant_b200 import ops
