@@ -140,26 +140,26 @@ int encode_activations(CUtensorMap* map, const StageJob& S, int bf16, int T, int
     return r == CUDA_SUCCESS ? NQ_OK : NQ_ERR_UNSUPPORTED;
 }
 
-static int mm_encode_box(CUtensorMap* map, const void* p, int type, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+static int mm_encode_box(CUtensorMap* map, const void* p, int type, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return NQ_ERR_UNSUPPORTED;
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUtensorMapDataType dt = type == kMmS8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == kMmBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const CUresult r = enc(map, dt, rank, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUresult r = enc(map, dt, 3, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? NQ_OK : NQ_ERR_UNSUPPORTED;
 }
 
 int mm_encode(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int box_inner, int box_outer) {
-    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
-    return mm_encode_box(map, p, type, 2, dims, strides, box);
+    const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, 1}, strides[2] = {(cuuint64_t)stride, (cuuint64_t)stride};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1};
+    return mm_encode_box(map, p, type, dims, strides, box);
 }
 int mm_encode_columns(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int boxes) {
     const cuuint64_t dims[3] = {64, (cuuint64_t)outer, (cuuint64_t)(inner / 64)}, strides[2] = {(cuuint64_t)stride, 128};
     const cuuint32_t box[3] = {64, 64, (cuuint32_t)boxes};
-    return mm_encode_box(map, p, type, 3, dims, strides, box);
+    return mm_encode_box(map, p, type, dims, strides, box);
 }
 
 // The kernel of a stage, with its plan.  (An intermediate in the GEMMs' column order is theirs.)

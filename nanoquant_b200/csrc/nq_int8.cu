@@ -196,7 +196,7 @@ struct Int8Epilogue {
     const MmShape& s;
     float sx;
     int n0, row0;
-    __device__ Int8Epilogue(const Params& p_, const MmShape& s_, const unsigned char* few_) : few(reinterpret_cast<const float*>(few_)), p(p_), s(s_) {}
+    __device__ Int8Epilogue(const Params& p_, const MmShape& s_, const unsigned char* few_, const volatile MmDims*) : few(reinterpret_cast<const float*>(few_)), p(p_), s(s_) {}
     __device__ __forceinline__ void begin(int row, int n0_, int, int, int) {
         n0 = n0_;
         row0 = row & ~31;

@@ -39,6 +39,81 @@ __device__ __forceinline__ long long loss_target(const LossTargets& t, int row) 
 }
 
 // ---------------------------------------------------------------------------
+// tokens without a target
+// ---------------------------------------------------------------------------
+// They need no logits.  Larger calls (loss_packs) pack the rows of the others, so that prompts and padding in a batch cost no products; how many there are
+// is known on the device alone, and the products' kernels read it there.
+struct LossRows {
+    LossTargets targets;
+    const uint4* h;
+    uint4* out;
+    long long ldh;                 // 16-byte units
+    int *pos, *words, *live;       // nullable (no packing): [T] a token's row, -1 without a target; [rows] their targets, -1: no word of the vocabulary; number of rows
+    int T, V, packs;
+    int skip_all;                  // nothing to copy where all tokens have a target
+};
+__device__ __forceinline__ bool loss_has_target(const LossTargets& t, int row) { return loss_target(t, row) != t.ignore; }
+// One CTA of 512 threads takes the tokens first .. first + count - 1 (at most 512).  `each(token, row)` is called by one thread for each of them (row -1: none).
+// Every CTA counts the targets in front of its tokens and all of them for itself: no launch, and no wait, for a list.
+template <class Each>
+__device__ __forceinline__ void loss_copy_rows(const LossRows& R, int first, int count, Each each) {
+    __shared__ int sums[16], before[16], rows[512];
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int n = 0;                     // rows of all tokens
+    if (R.pos) {
+        int ahead = 0;
+#pragma unroll 4
+        for (int t = tid; t < R.T; t += 512) {
+            const int has = loss_has_target(R.targets, t);
+            n += has;
+            ahead += t < first ? has : 0;
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        ahead = __reduce_add_sync(0xffffffffu, ahead);
+        if (lane == 0) { sums[warp] = n; before[warp] = ahead; }
+        __syncthreads();
+        n = ahead = 0;
+        for (int i = 0; i < 16; ++i) { n += sums[i]; ahead += before[i]; }
+        __syncthreads();
+        const bool has = tid < count && loss_has_target(R.targets, first + tid);
+        const unsigned mask = __ballot_sync(0xffffffffu, has);
+        if (lane == 0) sums[warp] = __popc(mask);
+        __syncthreads();
+        for (int i = 0; i < warp; ++i) ahead += sums[i];
+        const int row = has ? ahead + __popc(mask & ((1u << lane) - 1)) : -1;
+        rows[tid] = row;
+        if (tid < count) {
+            R.pos[first + tid] = row;
+            if (has) {
+                const long long word = loss_target(R.targets, first + tid);
+                R.words[row] = word >= 0 && word < R.V ? (int)word : -1;
+            }
+            each(first + tid, row);
+        }
+        if (first == 0 && tid == 0) *R.live = n;
+    } else {
+        rows[tid] = tid < count && loss_has_target(R.targets, first + tid) ? first + tid : -1;
+        if (tid < count) each(first + tid, first + tid);
+    }
+    __syncthreads();
+    if (!R.out || (R.pos && R.skip_all && n == R.T)) return;
+    // Rows of the products.  Without packing a token's row is its own, zeros for one without a target, whatever it holds (its d is zero, but zero times a NaN
+    // is not); behind packed ones zeros up to a multiple of 64, which a step of the product over tokens reads.
+    const int zeros = (max(n, 1) + 63) & ~63;
+    for (int i = tid; i < count * R.packs; i += 512) {
+        const int k = i / R.packs, c = i - k * R.packs, t = first + k, row = rows[k];
+        if (row >= 0) R.out[(long long)row * R.packs + c] = __ldg(R.h + t * R.ldh + c);
+        if (R.pos ? t >= n && t < zeros : row < 0) R.out[(long long)t * R.packs + c] = make_uint4(0, 0, 0, 0);
+    }
+}
+__global__ void __launch_bounds__(512) loss_pack_kernel(const LossRows R, int per_cta) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // (behind the wait: what starts early may rely on everything before)
+    const int first = (int)blockIdx.x * per_cta;
+    loss_copy_rows(R, first, min(per_cta, R.T - first), [](int, int) {});
+}
+
+// ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
 struct LseEpilogue {
@@ -46,20 +121,22 @@ struct LseEpilogue {
     static constexpr int kChunk = 8;           // 512 columns: 2048 x 4096 x 151936 level with a whole sum (1.60 ms), with 256 1.69
     struct Params {
         LossTargets targets;
+        const int* words;          // nullable: the rows' targets (-1: none of the vocabulary's), else `targets` has them
         float2* part;              // [2 n_tiles][T]: largest logit (times log2 e), sum
         float* target_logit;       // [T]
     };
     const Params& p;
     const MmShape& s;
+    const volatile MmDims* dims;
     int row, n0, slot;
     long long target;
     float top, sum;
-    __device__ LseEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_) {}
+    __device__ LseEpilogue(const Params& p_, const MmShape& s_, const unsigned char*, const volatile MmDims* dims_) : p(p_), s(s_), dims(dims_) {}
     __device__ __forceinline__ void begin(int row_, int n0_, int set, int n_tile, int) {
         row = row_;
         n0 = n0_;
         slot = 2 * n_tile + set;
-        target = row < s.M ? loss_target(p.targets, row) : -1;
+        target = row >= dims->live ? -1 : p.words ? (long long)__ldcg(p.words + row) : loss_target(p.targets, row);
         top = -INFINITY;
         sum = 0.f;
     }
@@ -87,7 +164,7 @@ struct LseEpilogue {
         }
     }
     __device__ __forceinline__ void end() {
-        if (row < s.M) p.part[(long long)slot * s.M + row] = make_float2(top, sum);
+        if (row < dims->live) p.part[(long long)slot * s.M + row] = make_float2(top, sum);
     }
 };
 
@@ -100,12 +177,12 @@ __device__ __forceinline__ float2 lse_warp_join(float2 a) {
     for (int o = 16; o > 0; o >>= 1) a = lse_join(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
     return a;
 }
-// Loss and lse of token r from its joined pieces.  A target that is no word of the vocabulary (and not `ignore`) makes both NaN.
-__device__ __forceinline__ float lse_finish(float2 v, int r, const float* target_logit, const LossTargets& targets, int V, float* lse) {
+// Loss and lse of token r, whose logits are row `at`'s, from its joined pieces.  A target that is no word of the vocabulary (and not `ignore`) makes both NaN.
+__device__ __forceinline__ float lse_finish(float2 v, int r, int at, const float* target_logit, const LossTargets& targets, int V, float* lse) {
     const long long t = loss_target(targets, r);
     float l = v.x * kLn2 + logf(v.y), loss = 0.f;
     if (t != targets.ignore) {
-        if (t >= 0 && t < V) loss = l - __ldcg(target_logit + r);
+        if (t >= 0 && t < V) loss = l - __ldcg(target_logit + at);
         else loss = l = __int_as_float(0x7fffffff);
     }
     lse[r] = l;
@@ -114,23 +191,24 @@ __device__ __forceinline__ float lse_finish(float2 v, int r, const float* target
 // ROWS tokens a CTA of 256 threads (so that the CTAs are there before the product's have left): eight, whose pieces lie side by side, or for few tokens
 // one, with all threads on its pieces (151936 words have some 1600).
 template <int ROWS>
-__global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, int slots, int T, int V, int release) {
+__global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const float* target_logit, LossTargets targets, float* row_loss, float* lse, const int* pos, int slots, int T, int V, int release) {
     constexpr int kPieces = 256 / ROWS;            // threads of a token
     __shared__ float2 red[ROWS][kPieces / 32 > 1 ? kPieces / 32 : 33];
     const int sub = threadIdx.x % ROWS, piece = threadIdx.x / ROWS, row = blockIdx.x * ROWS + sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     float2 v = make_float2(-INFINITY, 0.f);
-    if (row < T) {
+    const int from = row >= T ? -1 : pos ? __ldcg(pos + row) : row;      // row of the logits (pos: -1 without a target)
+    if (from >= 0) {
         int i = piece;
         for (; i + 7 * kPieces < slots; i += 8 * kPieces) {      // eight loads in flight
             float2 p[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) p[k] = __ldcg(part + (long long)(i + kPieces * k) * T + row);
+            for (int k = 0; k < 8; ++k) p[k] = __ldcg(part + (long long)(i + kPieces * k) * T + from);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v = lse_join(v, p[k]);
         }
-        for (; i < slots; i += kPieces) v = lse_join(v, __ldcg(part + (long long)i * T + row));
+        for (; i < slots; i += kPieces) v = lse_join(v, __ldcg(part + (long long)i * T + from));
     }
     int r = blockIdx.x;
     if constexpr (ROWS == 1) {
@@ -145,7 +223,11 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const float2* part, const
         r = blockIdx.x * ROWS + warp;
         v = lse_warp_join(red[warp][lane]);
     }
-    if (lane == 0 && r < T) row_loss[r] = lse_finish(v, r, target_logit, targets, V, lse);
+    if (lane == 0 && r < T) {
+        const int at = pos ? __ldcg(pos + r) : r;
+        if (at < 0) row_loss[r] = lse[r] = 0.f;
+        else row_loss[r] = lse_finish(v, r, at, target_logit, targets, V, lse);
+    }
 }
 
 // Sum (mean: of the tokens with a target) of the tokens' losses and the number of these tokens; one CTA, a fixed order, 64-bit sums.  With `part` the pieces
@@ -164,7 +246,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float2* part, cons
             for (int i = lane; i < slots; i += 32) v = lse_join(v, __ldcg(part + (long long)i * T + r));
             v = lse_warp_join(v);
             if (lane == 0) {
-                s += lse_finish(v, r, target_logit, targets, V, lse);
+                s += lse_finish(v, r, r, target_logit, targets, V, lse);
                 n += loss_target(targets, r) != targets.ignore;
             }
         }
@@ -198,38 +280,29 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float2* part, cons
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// What the products need, in one launch.  CTA 0: row_scale[t], what d of a token is multiplied by before it is rounded, and final_scale, what the
-// products' sums are multiplied by.  The others (where `out` is wanted): h with zeros in the rows of tokens without a target, whatever these hold (their
-// d is zero, but zero times a NaN is not).
+// Backward: what the products need, in one launch: the rows of h; row_scale, what d of a row is multiplied by before it is rounded, and (with packing) its lse;
+// final_scale, what the products' sums are multiplied by.
 struct LossPrepare {
-    LossTargets targets;
-    const float *grad, *count;
+    LossRows rows;
+    const float *grad, *count, *lse;
     long long grad_stride;
-    float *row_scale, *final_scale;
-    const uint4* h;
-    uint4* out;
-    long long ldh;                 // 16-byte units
-    int T, packs, reduction;
+    float *row_scale, *final_scale, *row_lse;
+    int reduction;
     float unit;
 };
-__global__ void __launch_bounds__(512) loss_prepare_kernel(const LossPrepare P) {
+__global__ void __launch_bounds__(512) loss_prepare_kernel(const LossPrepare P, int per_cta) {
     __shared__ float red[16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const LossRows& R = P.rows;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, T = R.T, first = (int)blockIdx.x * per_cta;
+    const bool none = P.reduction == NQ_REDUCE_NONE;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // (behind the wait: what starts early may rely on everything before)
-    if (blockIdx.x > 0) {
-        const long long total = (long long)P.T * P.packs, step = (long long)(gridDim.x - 1) * 512;
-        for (long long i = (long long)(blockIdx.x - 1) * 512 + threadIdx.x; i < total; i += step) {
-            const int row = (int)(i / P.packs), c = (int)(i - (long long)row * P.packs);
-            P.out[i] = loss_target(P.targets, row) != P.targets.ignore ? __ldg(P.h + row * P.ldh + c) : make_uint4(0, 0, 0, 0);
-        }
-        return;
-    }
-    float top = 1.f;
-    if (P.reduction == NQ_REDUCE_NONE && P.unit != 1.f) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // (behind the wait, as above)
+    float top = 1.f;                       // the largest |grad|, which fp16 is relative to
+    if (none && P.unit != 1.f) {
         top = 0.f;
-        for (int i = threadIdx.x; i < P.T; i += 512)
-            if (loss_target(P.targets, i) != P.targets.ignore) top = fmaxf(top, fabsf(P.grad[i * P.grad_stride]));
+#pragma unroll 4
+        for (int i = threadIdx.x; i < T; i += 512)
+            if (loss_has_target(R.targets, i)) top = fmaxf(top, fabsf(P.grad[i * P.grad_stride]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) red[warp] = top;
@@ -237,15 +310,16 @@ __global__ void __launch_bounds__(512) loss_prepare_kernel(const LossPrepare P) 
         for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i]);
         if (top == 0.f || top == INFINITY) top = 1.f;
     }
-    for (int i = threadIdx.x; i < P.T; i += 512) {
-        const bool live = loss_target(P.targets, i) != P.targets.ignore;
-        P.row_scale[i] = !live ? 0.f : P.reduction == NQ_REDUCE_NONE ? P.grad[i * P.grad_stride] / top * P.unit : P.unit;
-    }
-    if (threadIdx.x == 0) {
-        float f = P.reduction == NQ_REDUCE_NONE ? top : P.grad[0];
+    if (first == 0 && threadIdx.x == 0) {
+        float f = none ? top : P.grad[0];
         if (P.reduction == NQ_REDUCE_MEAN) f = *P.count > 0.f ? f / *P.count : 0.f;
         *P.final_scale = f / P.unit;
     }
+    loss_copy_rows(R, first, min(per_cta, T - first), [&](int t, int row) {
+        if (row < 0) return;
+        P.row_scale[row] = !loss_has_target(R.targets, t) ? 0.f : none ? P.grad[t * P.grad_stride] / top * P.unit : P.unit;
+        if (R.pos) P.row_lse[row] = __ldcg(P.lse + t);
+    });
 }
 
 // d of a piece of the vocabulary.
@@ -255,6 +329,7 @@ struct GradEpilogue {
     static constexpr int kChunk = 0;
     struct Params {
         LossTargets targets;
+        const int* words;          // as in LseEpilogue; then all rows below `live` count
         const float *lse, *row_scale;
         uint16_t* d;
         long long ldd;
@@ -262,19 +337,20 @@ struct GradEpilogue {
     };
     const Params& p;
     const MmShape& s;
+    const volatile MmDims* dims;
     int row, n0, at;
     float base, scale;
     bool live;
-    __device__ GradEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_) {}
+    __device__ GradEpilogue(const Params& p_, const MmShape& s_, const unsigned char*, const volatile MmDims* dims_) : p(p_), s(s_), dims(dims_) {}
     __device__ __forceinline__ void begin(int row_, int n0_, int, int, int) {
         row = row_;
         n0 = n0_;
         live = false;
         at = -1;
         base = scale = 0.f;
-        if (row < s.M) {
-            const long long t = loss_target(p.targets, row);
-            live = t != p.targets.ignore;
+        if (row < dims->live) {
+            const long long t = p.words ? (long long)__ldcg(p.words + row) : loss_target(p.targets, row);
+            live = p.words || t != p.targets.ignore;
             const long long rel = t - p.v0 - n0;
             at = rel >= 0 && rel < kMmAccCols ? (int)rel : -1;
             base = __ldcg(p.lse + row) * kLog2e;
@@ -298,7 +374,7 @@ struct GradEpilogue {
     }
     __device__ __forceinline__ void flush(int c, int cols, const unsigned char* stage) {
         const int row0 = row & ~31;
-        mm_store_rows(stage, p.d + row0 * p.ldd + n0 + c, p.ldd, min(32, s.M - row0), cols, true);
+        mm_store_rows(stage, p.d + row0 * p.ldd + n0 + c, p.ldd, min(32, dims->rows - row0), cols, true);
     }
     __device__ __forceinline__ void end() {}
 };
@@ -317,7 +393,7 @@ struct RowsEpilogue {
     const MmShape& s;
     int row0, n0;
     float f;
-    __device__ RowsEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_), f(__ldcg(p_.final_scale)) {}
+    __device__ RowsEpilogue(const Params& p_, const MmShape& s_, const unsigned char*, const volatile MmDims*) : p(p_), s(s_), f(__ldcg(p_.final_scale)) {}
     __device__ __forceinline__ void begin(int row, int n0_, int, int, int) {
         row0 = row & ~31;
         n0 = n0_;
@@ -347,7 +423,7 @@ struct SumEpilogue {
     const MmShape& s;
     int n0;
     float4* dst;
-    __device__ SumEpilogue(const Params& p_, const MmShape& s_, const unsigned char*) : p(p_), s(s_) {}
+    __device__ SumEpilogue(const Params& p_, const MmShape& s_, const unsigned char*, const volatile MmDims*) : p(p_), s(s_) {}
     __device__ __forceinline__ void begin(int row, int n0_, int, int, int split) {
         n0 = n0_;
         dst = p.sums + (((long long)split * p.blocks + (row >> 7)) * p.quads + (n0 >> 2)) * 128 + (row & 127);
@@ -370,19 +446,20 @@ struct SumEpilogue {
 
 // dh: the splits' sums, added in order, times the final scale.  32 tokens x 64 columns a CTA.
 template <int OUT>
-__global__ void __launch_bounds__(256) dh_kernel(const float4* sums, const float* final_scale, uint16_t* dh, long long ld, int T, int N, int blocks, int quads, int splits) {
+__global__ void __launch_bounds__(256) dh_kernel(const float4* sums, const float* final_scale, uint16_t* dh, long long ld, const int* pos, int T, int N, int blocks, int quads, int splits) {
     __shared__ uint32_t tile[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = blockIdx.x * 32, col0 = blockIdx.y * 64;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float f = __ldcg(final_scale);
+    const int from = row0 + lane >= T ? -1 : pos ? __ldcg(pos + row0 + lane) : row0 + lane;      // the token's row, -1: zeros
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int qd = 2 * warp + k, quad = (col0 >> 2) + qd;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (quad < quads) {
+        if (quad < quads && from >= 0) {
 #pragma unroll 4
             for (int sp = 0; sp < splits; ++sp) {
-                const float4 o = __ldcg(sums + (((long long)sp * blocks + (row0 >> 7)) * quads + quad) * 128 + (row0 & 127) + lane);
+                const float4 o = __ldcg(sums + (((long long)sp * blocks + (from >> 7)) * quads + quad) * 128 + (from & 127));
                 v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
             }
         }
@@ -408,6 +485,9 @@ static int launch_plain(const void* fn, dim3 grid, int threads, void** args, cud
     return launch_dependent(cfg, attr, 0, fn, args);
 }
 static bool loss_pairs(int64_t T) { return T > 128; }
+// Whether a call packs the rows that have a target: forward a launch and a copy of h (where rows fall away), some 8 us, against products that take 150 us
+// and more and have several tiles of 256 rows.
+static bool loss_packs(int64_t T, int64_t N, int64_t V) { return T > 512 && 2.0 * (double)T * (double)N * (double)V > 2e11; }
 
 struct LossPlan {
     int bn, slots;                       // forward
@@ -434,7 +514,7 @@ static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     // splits' sums, and what writing (with several pieces, also reading) and adding them moves.
     p.h_bn = cg == 2 ? (N <= 128 ? 128 : 256) : (N <= 64 ? 64 : N <= 128 ? 128 : 256);
     const int64_t tiles = (int64_t)m_tiles * ((N + p.h_bn - 1) / p.h_bn), steps = ((p.piece < V ? p.piece : V) + 63) / 64;
-    const bool one = p.piece >= V;
+    const bool one = p.piece >= V && !loss_packs(T, N, V);
     p.h_splits = 1;
     p.h_direct = one;
     double best = 0;
@@ -448,8 +528,8 @@ static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     p.h_quads = (int)(up(N, p.h_bn) / 4);
     return p;
 }
-struct LossScratch { int64_t d, h, sums, row_scale, final_scale, bytes; };
-static LossScratch loss_scratch(const LossPlan& p, int64_t T, int64_t N) {
+struct LossScratch { int64_t d, h, sums, row_scale, final_scale, pos, words, row_lse, live, bytes; };
+static LossScratch loss_scratch(const LossPlan& p, int64_t T, int64_t N, bool packs) {
     LossScratch s;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t here = at; at += up(bytes, 256); return here; };
@@ -458,11 +538,15 @@ static LossScratch loss_scratch(const LossPlan& p, int64_t T, int64_t N) {
     s.sums = take(p.h_direct ? 0 : (int64_t)p.h_splits * p.h_blocks * p.h_quads * 128 * 16);
     s.row_scale = take(T * 4);
     s.final_scale = take(4);
+    s.pos = take(packs ? T * 4 : 0);
+    s.words = take(packs ? T * 4 : 0);
+    s.row_lse = take(packs ? T * 4 : 0);
+    s.live = take(packs ? 4 : 0);
     s.bytes = at;
     return s;
 }
-// Forward: the pieces and the targets' logits of kLossRows tokens, the losses of all.
-struct LossFwdScratch { int64_t target_logit, row_loss, bytes; };
+// Forward: the pieces and the targets' logits of kLossRows tokens, their packed rows, the losses of all.
+struct LossFwdScratch { int64_t target_logit, row_loss, h, pos, words, live, bytes; };
 static LossFwdScratch loss_fwd_scratch(int64_t T, int64_t N, int64_t V) {
     LossFwdScratch s;
     int64_t part = 0;
@@ -470,9 +554,15 @@ static LossFwdScratch loss_fwd_scratch(int64_t T, int64_t N, int64_t V) {
         const int64_t bytes = t > 0 ? plan_loss(t, N, V).slots * t * 8 : 0;
         if (bytes > part) part = bytes;
     }
+    const int64_t most = T < kLossRows ? T : (int64_t)kLossRows;
+    const bool packs = loss_packs(most, N, V);
     s.target_logit = up(part, 256);
-    s.row_loss = s.target_logit + up((T < kLossRows ? T : kLossRows) * 4, 256);
-    s.bytes = s.row_loss + up(T * 4, 256);
+    s.row_loss = s.target_logit + up(most * 4, 256);
+    s.h = s.row_loss + up(T * 4, 256);
+    s.pos = s.h + (packs ? up(most * N * 2, 256) : 0);
+    s.words = s.pos + (packs ? up(most * 4, 256) : 0);
+    s.live = s.words + (packs ? up(most * 4, 256) : 0);
+    s.bytes = s.live + (packs ? 256 : 0);
     return s;
 }
 static int check_loss(int64_t T, int64_t N, int64_t V, int64_t ldh, int64_t ldw, int dtype, int reduction, int target_bits) {
@@ -484,11 +574,24 @@ static int check_loss(int64_t T, int64_t N, int64_t V, int64_t ldh, int64_t ldw,
     return NQ_OK;
 }
 
+// Tokens of a CTA that copies rows: so many CTAs that a copy takes microseconds, no more than four to an SM.
+static int rows_per_cta(int64_t T) {
+    int64_t per = (T + 4 * sm_count() - 1) / (4 * sm_count());
+    return (int)(per < 4 ? 4 : per > 512 ? 512 : per);
+}
+
+// `packed` (with `live`): the rows of h that have a target, read where they are fewer than all.
 template <int CG>
-static int launch_lse(const void* h, const void* w, const LseEpilogue::Params& e, int T, int N, int V, int64_t ldh, int64_t ldw, int type, int bn,
-                      unsigned* status, cudaStream_t stream) {
+static int launch_lse(const void* h, const void* packed, const int* live, const void* w, const LseEpilogue::Params& e, int T, int N, int V, int64_t ldh, int64_t ldw,
+                      int type, int bn, unsigned* status, cudaStream_t stream) {
     MmParams<LseEpilogue> P = {};
     P.e = e;
+    if (live) {
+        P.s.live = live;
+        P.s.live_alt = 1;
+        const int st = mm_encode(&P.map_alt, packed, type, N, T, (int64_t)N * 2, 64, CG == 2 || T >= 128 ? 128 : (T + 7) / 8 * 8);
+        if (st != NQ_OK) return st;
+    }
     return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 0, 1, status, stream);
 }
 
@@ -499,19 +602,29 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
     const int type = OUT == kOutFp16 ? kMmF16 : kMmBf16;
     uint16_t* d = reinterpret_cast<uint16_t*>(scratch + at.d);
     const float* final_scale = reinterpret_cast<float*>(scratch + at.final_scale);
+    const bool packs = loss_packs(T, N, V);
+    const int *pos = packs ? reinterpret_cast<int*>(scratch + at.pos) : nullptr, *live = packs ? reinterpret_cast<int*>(scratch + at.live) : nullptr;
+    const int* words = packs ? reinterpret_cast<int*>(scratch + at.words) : nullptr;
+    const void* rows = packs ? scratch + at.h : h;      // of the logits
+    const int64_t ld_rows = packs ? N : ldh;
+    if (packs) lse = reinterpret_cast<float*>(scratch + at.row_lse);
     int splits = p.h_splits;
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece);
         const char* wp = static_cast<const char*>(w) + v0 * ldw * 2;
         {
             MmParams<GradEpilogue<OUT>> P = {};
-            P.e = {targets, lse, reinterpret_cast<float*>(scratch + at.row_scale), d, p.piece, (int)v0};
-            const int st = mm_launch<CG>(P, type, {h, ldh * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 1, 1, status, stream);
+            const typename GradEpilogue<OUT>::Params e = {targets, words, lse, reinterpret_cast<float*>(scratch + at.row_scale), d, p.piece, (int)v0};
+            P.e = e;
+            P.s.live = live;
+            const int st = mm_launch<CG>(P, type, {rows, ld_rows * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 1, 1, status, stream);
             if (st != NQ_OK) return st;
         }
         if (dw) {
             MmParams<RowsEpilogue<OUT>> P = {};
             P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
+            P.s.live = live;
+            P.s.live_k = 1;
             const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
             if (st != NQ_OK) return st;
         }
@@ -523,6 +636,7 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
         if (dh) {
             MmParams<SumEpilogue> P = {};
             P.e = {reinterpret_cast<float4*>(scratch + at.sums), p.h_blocks, p.h_quads, v0 > 0};
+            P.s.live = live;
             const int st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 1, 1, status, stream);
             if (st != NQ_OK) return st;
             if (v0 == 0) splits = P.s.splits;                  // (the last piece may be shorter and have fewer)
@@ -533,7 +647,7 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
         const float4* sums = reinterpret_cast<const float4*>(scratch + at.sums);
         long long ld = lddh;
         int blocks = p.h_blocks, quads = p.h_quads;
-        void* args[] = {&sums, &final_scale, &dh, &ld, &T, &N, &blocks, &quads, &splits};
+        void* args[] = {&sums, &final_scale, &dh, &ld, &pos, &T, &N, &blocks, &quads, &splits};
         return launch_plain(fn, dim3((T + 31) / 32, (N + 63) / 64), 256, args, stream);
     }
     return NQ_OK;
@@ -575,16 +689,28 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
         slots = p.slots;
         const char* rows = static_cast<const char*>(h) + t0 * ldh * 2;
         LossTargets tg = {static_cast<const char*>(targets) + t0 * (target_bits / 8), all.wide, ignore_index};
-        const LseEpilogue::Params e = {tg, part, target_logit};
-        st = loss_pairs(t) ? launch_lse<2>(rows, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s)
-                           : launch_lse<1>(rows, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s);
+        int *pos = nullptr, *words = nullptr, *live = nullptr;
+        char* packed = base + at.h;
+        if (loss_packs(t, N, V)) {
+            pos = reinterpret_cast<int*>(base + at.pos);
+            words = reinterpret_cast<int*>(base + at.words);
+            live = reinterpret_cast<int*>(base + at.live);
+            LossRows R = {tg, reinterpret_cast<const uint4*>(rows), reinterpret_cast<uint4*>(packed), ldh / 8, pos, words, live, t, v, (int)(N / 8), 1};
+            int per_cta = rows_per_cta(t);
+            void* pack_args[] = {&R, &per_cta};
+            st = launch_plain((const void*)loss_pack_kernel, dim3((unsigned)((t + per_cta - 1) / per_cta)), 512, pack_args, s);
+            if (st != NQ_OK) return st;
+        }
+        const LseEpilogue::Params e = {tg, words, part, target_logit};
+        st = loss_pairs(t) ? launch_lse<2>(rows, packed, live, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s)
+                           : launch_lse<1>(rows, packed, live, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s);
         if (st != NQ_OK) return st;
-        if (reduction != NQ_REDUCE_NONE && T <= 1024 && T * slots <= kLossJoinHere) {
+        if (reduction != NQ_REDUCE_NONE && !pos && T <= 1024 && T * slots <= kLossJoinHere) {
             joined = part;
             break;
         }
         float *loss_out = row_loss + t0, *lse_out = lse + t0;
-        void* join_args[] = {&part, &target_logit, &tg, &loss_out, &lse_out, &slots, &t, &v, &release};
+        void* join_args[] = {&part, &target_logit, &tg, &loss_out, &lse_out, &pos, &slots, &t, &v, &release};
         st = t <= 8 * sm_count() ? launch_plain((const void*)lse_join_kernel<1>, dim3((unsigned)t), 256, join_args, s)
                                  : launch_plain((const void*)lse_join_kernel<8>, dim3((unsigned)((t + 7) / 8)), 256, join_args, s);
         if (st != NQ_OK) return st;
@@ -596,7 +722,7 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
 
 size_t nq_linear_ce_bwd_scratch_bytes(int64_t T, int64_t N, int64_t V) {
     if (check_loss(T, N, V, N, N, NQ_F16, NQ_REDUCE_NONE, 64) != NQ_OK) return 0;
-    return (size_t)loss_scratch(plan_loss(T, N, V), T, N).bytes;
+    return (size_t)loss_scratch(plan_loss(T, N, V), T, N, loss_packs(T, N, V)).bytes;
 }
 
 int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int target_bits, int64_t ignore_index, const float* lse,
@@ -613,16 +739,22 @@ int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int targ
     cudaStream_t s = as_stream(stream);
     unsigned* status = static_cast<unsigned*>(status_word) + 2;
     const LossPlan p = plan_loss(T, N, V);
-    const LossScratch at = loss_scratch(p, T, N);
+    const bool packs = loss_packs(T, N, V);
+    const LossScratch at = loss_scratch(p, T, N, packs);
     char* base = static_cast<char*>(scratch);
     LossTargets tg = {targets, target_bits == 64, ignore_index};
-    LossPrepare prep = {tg, grad_loss, count, grad_stride, reinterpret_cast<float*>(base + at.row_scale), reinterpret_cast<float*>(base + at.final_scale),
-                        static_cast<const uint4*>(h), reinterpret_cast<uint4*>(base + at.h), ldh / 8, (int)T, (int)(N / 8), reduction,
-                        dtype == NQ_F16 ? kLossHalfScale : 1.f};
-    int64_t ctas = dw ? (T * prep.packs + 2047) / 2048 : 0;
-    if (ctas > 4 * sm_count()) ctas = 4 * sm_count();
-    void* prepare_args[] = {&prep};
-    st = launch_plain((const void*)loss_prepare_kernel, dim3((unsigned)(1 + ctas)), 512, prepare_args, s);
+    LossRows R = {tg, static_cast<const uint4*>(h), dw || packs ? reinterpret_cast<uint4*>(base + at.h) : nullptr, ldh / 8, nullptr, nullptr, nullptr, (int)T, (int)V,
+                  (int)(N / 8), 0};
+    if (packs) {
+        R.pos = reinterpret_cast<int*>(base + at.pos);
+        R.words = reinterpret_cast<int*>(base + at.words);
+        R.live = reinterpret_cast<int*>(base + at.live);
+    }
+    LossPrepare prep = {R, grad_loss, count, lse, grad_stride, reinterpret_cast<float*>(base + at.row_scale), reinterpret_cast<float*>(base + at.final_scale),
+                        reinterpret_cast<float*>(base + at.row_lse), reduction, dtype == NQ_F16 ? kLossHalfScale : 1.f};
+    int per_cta = rows_per_cta(T);
+    void* prepare_args[] = {&prep, &per_cta};
+    st = launch_plain((const void*)loss_prepare_kernel, dim3((unsigned)((T + per_cta - 1) / per_cta)), 512, prepare_args, s);
     if (st != NQ_OK) return st;
 #define NQ_LOSS_BACKWARD(cg, out) launch_backward<cg, out>(h, w, tg, lse, dh, dw, base, p, at, (int)T, (int)N, (int)V, ldh, ldw, lddh, lddw, status, s)
     if (dtype == NQ_BF16) return loss_pairs(T) ? NQ_LOSS_BACKWARD(2, kOutBf16) : NQ_LOSS_BACKWARD(1, kOutBf16);

@@ -27,26 +27,39 @@ constexpr int kMmBarOff = 0, kMmFewOff = 512, kMmOutOff = 1024, kMmStageOff = kM
 constexpr int kMmSmemMost = 226 * 1024;
 constexpr int kMmAccCols = 256;
 
+// How an operand's part of a step is fetched: `loads` boxes of its 3-d map, 64 of the first coordinate apart; the coordinates of k are (dx k, dy k), those
+// of row r (m or n) are (r if x_rows, r if y_rows, r / 64 if z_rows).
+struct MmLoad {
+    int bytes;                     // of all of it
+    int loads, dx, dy, x_rows, y_rows, z_rows;
+};
 struct MmShape {
     int M, N;                      // rows and columns of the result
     int m_tiles, n_tiles, bn;
     int ksteps, steps_per_split, splits;
-    int stages, stage_bytes, a_stage;  // bytes of a stage, and of A in it
+    int kel, stages, stage_bytes, a_stage;  // elements of k per step; bytes of a stage, and of A in it
     int m_fast;                    // consecutive tiles share their columns
-    int a_box, b_box;              // K-major: rows per load; MN-major: loads of 64 rows
-    int a_mn, b_mn;                // operand has m / n contiguous (2: its boxes in one load)
-    int kel;                       // elements of k per step
+    int a_mn, b_mn;                // operand has m / n contiguous
+    MmLoad a, b;
     int early_b;                   // B does not depend on the kernel before, which is one of the same call and has waited for all before it
     int release;                   // the kernel behind, one of the same call, may start early (but behind everything before this one)
     int few;                       // (kBuildA) bytes of A per step: 1024 for every eight rows
+    const int* live;               // nullable: how many of the rows of A (live_k: of the steps' k) there are, known on the device alone
+    int live_k, live_alt;          // (live_alt: A is map_alt's matrix where that is fewer than all)
     uint32_t idesc;
     unsigned wait_limit;
     unsigned* status;
 };
 
+// What a launch has to do: the host's numbers, or what the device knows better; in shared memory (registers are short in some epilogues).
+struct MmDims {
+    int rows, live;                // of A: that are taken (of a `live` number up to the next multiple of 64), and that count
+    int ksteps, m_tiles, tiles;
+};
+
 template <class Epi>
 struct alignas(64) MmParams {
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_a, map_b, map_alt;
     MmShape s;
     typename Epi::Params e;
 };
@@ -85,21 +98,26 @@ __device__ __forceinline__ void mm_commit(uint32_t bar) {      // the barrier at
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 template <int CG>
-__device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-    if constexpr (CG == 2)
-        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
-    else
-        tma_load_2d(dst, map, c0, c1, bar);
-}
-template <int CG>
-__device__ __forceinline__ void mm_load_columns(uint32_t dst, const CUtensorMap* map, int c1, int c2, uint32_t bar) {
+__device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
     if constexpr (CG == 2)
         asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                     ::"r"(dst), "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
     else
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                     ::"r"(dst), "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+// mbar_wait_warp for a thread of its own.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned* status, unsigned limit) {
+    auto done = [&]() { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity); };
+    if (done()) return true;
+    for (unsigned i = 0; i < limit; ++i) {
+        if (done()) return true;
+        if (*abort_flag != 0) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(status, (unsigned)(-NQ_ERR_TIMEOUT));
+    return false;
 }
 // 32 columns of this warp's 32 rows: lane i has row i.
 __device__ __forceinline__ void mm_tmem_start(uint32_t taddr, uint32_t (&r)[32]) {
@@ -152,7 +170,7 @@ __device__ __forceinline__ void mm_store_rows(const unsigned char* stage, uint16
 // Epi: struct Params; kS8; kBuildA: the epilogue warps make A themselves, all of it before the first MMA (few rows: `build` writes its steps, each of
 // whole 8-row groups in the layout of umma_desc, and may leave up to 512 bytes at `few` for the epilogue; the MMA reads rows beyond as they
 // are, whose results nobody looks at); an object per epilogue thread with
-//   Epi(const Params&, const MmShape&)
+//   Epi(const Params&, const MmShape&, few, dims)
 //   begin(row, n0, m_tile, n_tile, split, ...)      a tile of this thread's row (row >= M: none)
 //   chunk(r, c, cols, stage, half)                  32 columns from n0 + c, `cols` of which exist (all lanes call it, if any of their rows exists)
 //   flush(c, cols, stage)                           behind both halves of 64 columns
@@ -175,9 +193,10 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
     auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * kMmMaxStages + 2 + a); };     // used in the pair's first CTA
     const uint32_t bar_built = bars + 8 * (2 * kMmMaxStages + 4);
     constexpr int kMisc = kMmBarOff + 8 * (2 * kMmMaxStages + 5);
-    static_assert(kMisc + 8 <= kMmFewOff, "shared memory map");
+    static_assert(kMisc + 8 + (int)sizeof(MmDims) <= kMmFewOff, "shared memory map");
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kMisc + 4);
+    volatile MmDims* dims = reinterpret_cast<volatile MmDims*>(smem + kMisc + 8);
     const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;
     if (warp == 2) {
         if (lane < kMmMaxStages) {
@@ -206,6 +225,25 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
+    if (threadIdx.x == 0) {
+        int rows = S.M, live = S.M, ksteps = S.ksteps, m_tiles = S.m_tiles;
+        if (S.live) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            const int n = __ldcg(S.live), some = (max(n, 1) + 63) & ~63;      // (one step at least, of zeros)
+            if (S.live_k) {
+                ksteps = min(ksteps, some / 64);
+            } else {
+                live = n;
+                rows = min(rows, some);
+                m_tiles = (rows + 128 * CG - 1) / (128 * CG);
+            }
+        }
+        dims->rows = rows;
+        dims->live = live;
+        dims->ksteps = ksteps;
+        dims->m_tiles = m_tiles;
+        dims->tiles = m_tiles * S.n_tiles * S.splits;
+    }
     tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) {
@@ -215,124 +253,121 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     constexpr int kChunk = Epi::kChunk ? Epi::kChunk : 1 << 30;
-    const int groups = (int)gridDim.x / CG, first = (int)blockIdx.x / CG, plane = S.m_tiles * S.n_tiles, tiles = plane * S.splits;
+    const int groups = (int)gridDim.x / CG, first = (int)blockIdx.x / CG, tiles = dims->tiles;
     struct Tile { int m, n, split, k0, k1; };
     auto tile_of = [&](int t) {
+        const int m_tiles = dims->m_tiles, plane = m_tiles * S.n_tiles;
         Tile r;
         r.split = t / plane;
         const int u = t - r.split * plane;
-        if (S.m_fast) { r.n = u / S.m_tiles; r.m = u - r.n * S.m_tiles; }
+        if (S.m_fast) { r.n = u / m_tiles; r.m = u - r.n * m_tiles; }
         else { r.m = u / S.n_tiles; r.n = u - r.m * S.n_tiles; }
         r.k0 = r.split * S.steps_per_split;
-        r.k1 = min(S.ksteps, r.k0 + S.steps_per_split);
+        r.k1 = min(dims->ksteps, r.k0 + S.steps_per_split);
         return r;
     };
     constexpr bool kBuildA = Epi::kBuildA;
-    const uint32_t a_bytes = kBuildA ? 0u : (uint32_t)(S.a_mn ? S.a_box * 8192 : S.a_box * 128), b_bytes = (uint32_t)(S.b_mn ? S.b_box * 8192 : S.b_box * 128);
     const uint32_t built = sbase + kMmStageOff, stage0 = built + (kBuildA ? (uint32_t)(S.few * S.ksteps) : 0u);
     const uint32_t a_stage = (uint32_t)S.a_stage;
 
     if (warp < 4) {
-    if constexpr (Epi::kChunk > 0) regs_down<kMmRegsIssue>();
-    if (warp == 0) {
-        // ---------------------------------------------------------------- operands
-        auto load_a = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
-            if constexpr (kBuildA) return;
-            const int m0 = (T.m * CG + rank) * 128;
-            if (S.a_mn == 2) {
-                mm_load_columns<CG>(dst, &P.map_a, k * S.kel, m0 >> 6, bar);
-            } else if (S.a_mn) {
-                for (int i = 0; i < S.a_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_a, m0 + 64 * i, k * S.kel, bar);
-            } else {
-                mm_load<CG>(dst, &P.map_a, k * S.kel, m0, bar);
-            }
-        };
-        auto load_b = [&](const Tile& T, int k, uint32_t dst, uint32_t bar) {
-            const int n0 = T.n * S.bn + rank * (S.bn / CG);
-            if (S.b_mn == 2) {
-                mm_load_columns<CG>(dst, &P.map_b, k * S.kel, n0 >> 6, bar);
-            } else if (S.b_mn) {
-                for (int i = 0; i < S.b_box; ++i) mm_load<CG>(dst + 8192u * i, &P.map_b, n0 + 64 * i, k * S.kel, bar);
-            } else {
-                mm_load<CG>(dst, &P.map_b, k * S.kel, n0, bar);
-            }
-        };
-        auto ready_bar = [&](int s) { return CG == 2 ? cluster_map(bar_ready(s), 0) : bar_ready(s); };
-        int s = 0, pre = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        if (S.early_b && first < tiles) {      // the first tile's columns while the kernel before still writes the rows
-            const Tile T = tile_of(first);
-            pre = min(S.stages, T.k1 - T.k0);
-            if (elect_one())
+        if constexpr (Epi::kChunk > 0) regs_down<kMmRegsIssue>();
+        // One thread each for the loads and for the MMAs: a step takes some 450 cycles, and votes of the warp, branches and look-ups in every one cost a tenth
+        // of the tensor cores' time.
+        if (warp == 0 && elect_one()) {
+            // ------------------------------------------------------------ operands
+            const uint32_t step_bytes = (uint32_t)CG * (uint32_t)((kBuildA ? 0 : S.a.bytes) + S.b.bytes), stage_bytes = (uint32_t)S.stage_bytes;
+            const uint32_t ready0 = CG == 2 ? cluster_map(bar_ready(0), 0) : bar_ready(0);
+            const CUtensorMap *map_a = &P.map_a, *map_b = &P.map_b;
+            if (S.live_alt && dims->live < S.M) map_a = &P.map_alt;
+            int ax, ay, az, bx, by, bz;                    // of the tile's rows
+            auto tile_rows = [&](const Tile& T) {
+                const int m = (T.m * CG + rank) * 128, n = T.n * S.bn + rank * (S.bn / CG);
+                ax = S.a.x_rows ? m : 0; ay = S.a.y_rows ? m : 0; az = S.a.z_rows ? m >> 6 : 0;
+                bx = S.b.x_rows ? n : 0; by = S.b.y_rows ? n : 0; bz = S.b.z_rows ? n >> 6 : 0;
+            };
+            const int adx = S.a.dx, ady = S.a.dy, bdx = S.b.dx, bdy = S.b.dy;
+            auto load_a = [&](int k, uint32_t dst, uint32_t bar) {
+                if constexpr (kBuildA) return;
+                mm_load<CG>(dst, map_a, ax + k * adx, ay + k * ady, az, bar);
+                for (int i = 1; i < S.a.loads; ++i) mm_load<CG>(dst + 8192u * i, map_a, ax + 64 * i, ay + k * ady, az, bar);
+            };
+            auto load_b = [&](int k, uint32_t dst, uint32_t bar) {
+                mm_load<CG>(dst, map_b, bx + k * bdx, by + k * bdy, bz, bar);
+                for (int i = 1; i < S.b.loads; ++i) mm_load<CG>(dst + 8192u * i, map_b, bx + 64 * i, by + k * bdy, bz, bar);
+            };
+            int s = 0, pre = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            if (S.early_b && first < tiles) {      // the first tile's columns while the kernel before still writes the rows
+                const Tile T = tile_of(first);
+                tile_rows(T);
+                pre = min(S.stages, T.k1 - T.k0);
                 for (int i = 0; i < pre; ++i) {
-                    if (rank == 0) mbar_expect_tx(bar_ready(i), (uint32_t)CG * (a_bytes + b_bytes));
-                    load_b(T, T.k0 + i, stage0 + (uint32_t)(i * S.stage_bytes) + a_stage, ready_bar(i));
+                    if (rank == 0) mbar_expect_tx(bar_ready(i), step_bytes);
+                    load_b(T.k0 + i, stage0 + (uint32_t)i * stage_bytes + a_stage, ready0 + 8 * i);
                 }
-        }
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        if (S.release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        if (pre) {
-            const Tile T = tile_of(first);
-            if (elect_one())
-                for (int i = 0; i < pre; ++i) load_a(T, T.k0 + i, stage0 + (uint32_t)(i * S.stage_bytes), ready_bar(i));
-            s = pre;
-            if (s == S.stages) { s = 0; ph = 1; }
-        }
-        for (int t = first; t < tiles && ok; t += groups) {
-            const Tile T = tile_of(t);
-            for (int k = T.k0 + pre; k < T.k1; ++k) {
-                ok = mbar_wait_warp<CG == 2>(bar_free(s), ph ^ 1, abort_flag, S.status, S.wait_limit);
-                if (!ok) break;
-                if (elect_one()) {
-                    if (rank == 0) mbar_expect_tx(bar_ready(s), (uint32_t)CG * (a_bytes + b_bytes));
-                    const uint32_t dst = stage0 + (uint32_t)(s * S.stage_bytes), bar = ready_bar(s);
-                    load_a(T, k, dst, bar);
-                    load_b(T, k, dst + a_stage, bar);
-                }
-                if (++s == S.stages) { s = 0; ph ^= 1; }
             }
-            pre = 0;
-        }
-    } else if (warp == 1) {
-        // ---------------------------------------------------------------- MMA issue
-        if (rank == 0) {
-            const uint32_t a_step = S.a_mn ? 2048u >> 4 : 32u >> 4, b_step = S.b_mn ? 2048u >> 4 : 32u >> 4;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (S.release) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            if (pre) {
+                const int k0 = tile_of(first).k0;
+                for (int i = 0; i < pre; ++i) load_a(k0 + i, stage0 + (uint32_t)i * stage_bytes, ready0 + 8 * i);
+                s = pre;
+                if (s == S.stages) { s = 0; ph = 1; }
+            }
+            for (int t = first; t < tiles && ok; t += groups) {
+                const Tile T = tile_of(t);
+                tile_rows(T);
+                for (int k = T.k0 + pre; k < T.k1; ++k) {
+                    ok = mm_wait<CG == 2>(bar_free(s), ph ^ 1, abort_flag, S.status, S.wait_limit);
+                    if (!ok) break;
+                    if (rank == 0) mbar_expect_tx(bar_ready(s), step_bytes);
+                    const uint32_t dst = stage0 + (uint32_t)s * stage_bytes, bar = ready0 + 8 * s;
+                    load_a(k, dst, bar);
+                    load_b(k, dst + a_stage, bar);
+                    if (++s == S.stages) { s = 0; ph ^= 1; }
+                }
+                pre = 0;
+            }
+        } else if (warp == 1 && rank == 0 && elect_one()) {
+            // ------------------------------------------------------------ MMA issue
+            const uint32_t a_step = S.a_mn ? 2048u >> 4 : 32u >> 4, b_step = S.b_mn ? 2048u >> 4 : 32u >> 4, idesc = S.idesc;
+            const uint64_t a0 = S.a_mn ? umma_desc_mn(kBuildA ? built : stage0) : umma_desc(kBuildA ? built : stage0);
+            const uint64_t b0 = S.b_mn ? umma_desc_mn(stage0 + a_stage) : umma_desc(stage0 + a_stage);
+            const uint32_t stage_units = (uint32_t)S.stage_bytes >> 4, few_units = (uint32_t)S.few >> 4;
             int s = 0, a = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;
             if constexpr (kBuildA) {
-                ok = mbar_wait_warp(bar_built, 0, abort_flag, S.status, S.wait_limit);
+                ok = mm_wait<false>(bar_built, 0, abort_flag, S.status, S.wait_limit);
                 tc_fence_after();
             }
             for (int t = first; t < tiles && ok; t += groups) {
                 const Tile T = tile_of(t);
                 for (int c0 = T.k0; c0 < T.k1 && ok; c0 += kChunk) {
-                const int c1 = min(T.k1 - c0, kChunk) + c0;
-                const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols);
-                ok = mbar_wait_warp<CG == 2>(bar_acc_empty(a), aph ^ 1, abort_flag, S.status, S.wait_limit);
-                tc_fence_after();
-                for (int k = c0; k < c1 && ok; ++k) {
-                    ok = mbar_wait_warp<CG == 2>(bar_ready(s), ph, abort_flag, S.status, S.wait_limit);
-                    if (!ok) break;
+                    const int c1 = min(T.k1 - c0, kChunk) + c0;
+                    const uint32_t d = tmem_base + (uint32_t)(a * kMmAccCols);
+                    ok = mm_wait<CG == 2>(bar_acc_empty(a), aph ^ 1, abort_flag, S.status, S.wait_limit);
                     tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t st = stage0 + (uint32_t)(s * S.stage_bytes), at = kBuildA ? built + (uint32_t)(k * S.few) : st, bt = st + a_stage;
-                        const uint64_t ad = S.a_mn ? umma_desc_mn(at) : umma_desc(at), bd = S.b_mn ? umma_desc_mn(bt) : umma_desc(bt);
+                    for (int k = c0; k < c1 && ok; ++k) {
+                        ok = mm_wait<CG == 2>(bar_ready(s), ph, abort_flag, S.status, S.wait_limit);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t ad = a0 + (uint64_t)(kBuildA ? (uint32_t)k * few_units : (uint32_t)s * stage_units), bd = b0 + (uint64_t)((uint32_t)s * stage_units);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            mm_mma<CG, Epi::kS8>(d, ad + (uint64_t)(a_step * i), bd + (uint64_t)(b_step * i), S.idesc, k > c0 || i ? 1u : 0u);
+                            mm_mma<CG, Epi::kS8>(d, ad + (uint64_t)(a_step * i), bd + (uint64_t)(b_step * i), idesc, k > c0 || i ? 1u : 0u);
                         mm_commit<CG>(bar_free(s));
+                        if (++s == S.stages) { s = 0; ph ^= 1; }
                     }
-                    if (++s == S.stages) { s = 0; ph ^= 1; }
-                }
-                if (ok && elect_one()) mm_commit<CG>(bar_acc_full(a));
-                if (++a == 2) { a = 0; aph ^= 1; }
-                if (T.k1 - c0 <= kChunk) break;
+                    if (ok) mm_commit<CG>(bar_acc_full(a));
+                    if (++a == 2) { a = 0; aph ^= 1; }
+                    if (T.k1 - c0 <= kChunk) break;
                 }
             }
         }
-    }
+        __syncwarp();
     } else {
         // ---------------------------------------------------------------- epilogue
         if constexpr (Epi::kChunk > 0) regs_up<kMmRegsSums>();
@@ -345,7 +380,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_built);
         }
-        Epi epi(P.e, S, smem + kMmFewOff);
+        Epi epi(P.e, S, smem + kMmFewOff, dims);
         int a = 0;
         uint32_t aph = 0;
         for (int t = first; t < tiles; t += groups) {
@@ -365,7 +400,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                 }
                 if (++a == 2) { a = 0; aph ^= 1; }
             };
-            const bool some = row - lane < S.M;           // of the warp's rows exist
+            const bool some = row - lane < dims->rows;    // of the warp's rows exist
             if constexpr (Epi::kChunk > 0) {
                 float sum[kMmAccCols / 64][32] = {};
                 bool ok = true;
@@ -474,6 +509,24 @@ inline int mm_tile_cols(int N, int m_tiles, int cg, int least) {
     return best;
 }
 
+// Map and loads of an operand's `box` rows per step.
+inline int mm_operand(CUtensorMap* map, MmLoad& L, const MmOperand& O, int type, int64_t rows, int64_t K, int kel, int box) {
+    L = {box * 128, 1, 0, 0, 0, 0, 0};
+    if (!O.mn) {
+        L.dx = kel; L.y_rows = 1;
+        return mm_encode(map, O.p, type, K, rows, O.stride, kel, box);
+    }
+    // All of an operand's columns of 64 by one load (by one load each, both operands' kept the loading thread busy longer than the MMAs take; the gradient of
+    // 50688 x 4096 weights over 2048 tokens 612 us -> 524), where they are whole.
+    L.dy = 64;
+    if (rows % 64 == 0) {
+        L.z_rows = 1;
+        return mm_encode_columns(map, O.p, type, rows, K, O.stride, box / 64);
+    }
+    L.loads = box / 64; L.x_rows = 1;
+    return mm_encode(map, O.p, type, rows, K, O.stride, 64, 64);
+}
+// P.s.live, live_k and live_alt (with P.map_alt) are the caller's, or zero.
 template <int CG, class Epi>
 int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B, int M, int N, int64_t K, int bn, int splits,
               int early_b, int release, unsigned* status, cudaStream_t stream) {
@@ -491,35 +544,31 @@ int mm_launch(MmParams<Epi>& P, int type, const MmOperand& A, const MmOperand& B
     S.m_tiles = (M + 128 * CG - 1) / (128 * CG);
     S.n_tiles = (N + bn - 1) / bn;
     S.m_fast = S.m_tiles <= S.n_tiles;
-    S.kel = 128 / esize;
+    S.kel = 128 / esize;                                     // elements of k per step
     S.ksteps = (int)((K + S.kel - 1) / S.kel);
     S.few = Epi::kBuildA ? (M + 7) / 8 * 1024 : 0;
     if (splits > S.ksteps) splits = S.ksteps;
     S.steps_per_split = (S.ksteps + splits - 1) / splits;
     S.splits = (S.ksteps + S.steps_per_split - 1) / S.steps_per_split;
-    // (all of an operand's columns of 64 by one load: by one load each, both operands' kept the producer busy longer than the MMAs; the gradient of
-    // 50688 x 4096 weights over 2048 tokens 612 us -> 524)
     const int64_t am = A.extent > M ? A.extent : M, bm = B.extent > N ? B.extent : N;
-    S.a_mn = A.mn ? (am % 64 == 0 ? 2 : 1) : 0;
-    S.b_mn = B.mn ? (bm % 64 == 0 ? 2 : 1) : 0;
-    S.a_box = A.mn ? 2 : CG == 2 || M >= 128 ? 128 : (M + 7) / 8 * 8;
-    S.b_box = B.mn ? bn / CG / 64 : bn / CG;
-    S.a_stage = Epi::kBuildA ? 0 : S.a_mn ? kMmABytes : S.a_box * 128;
-    S.stage_bytes = S.a_stage + bn / CG * 128;
+    S.a_mn = A.mn; S.b_mn = B.mn;
+    const int a_rows = A.mn || CG == 2 || M >= 128 ? 128 : (M + 7) / 8 * 8, b_rows = bn / CG;
+    S.a_stage = Epi::kBuildA ? 0 : a_rows * 128;
+    S.stage_bytes = S.a_stage + b_rows * 128;
     // (a step's MMAs read 128 rows of A; what lies behind fewer is read as it is, and nobody looks at these rows' results)
     const int fixed = 1024 + kMmStageOff + S.few * S.ksteps, slack = Epi::kBuildA || S.a_stage < kMmABytes ? kMmABytes : 0;
     S.stages = (kMmSmemMost - fixed - slack) / S.stage_bytes;
     if (S.stages > kMmMaxStages) S.stages = kMmMaxStages;
-    S.early_b = early_b;
+    S.early_b = early_b && !S.live;
     S.release = release;
     const uint32_t fmt = type == kMmF16 ? 0u : 1u;           // kind::f16: 1 = bf16; kind::i8: 1 = signed
     S.idesc = (type == kMmS8 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)A.mn << 15 | (uint32_t)B.mn << 16 |
               (uint32_t)(bn >> 3) << 17 | (uint32_t)(128 * CG >> 4) << 24;
     S.wait_limit = gemm_wait_limit();
     S.status = status;
-    int st = Epi::kBuildA ? NQ_OK : S.a_mn == 2 ? mm_encode_columns(&P.map_a, A.p, type, am, K, A.stride, S.a_box) : A.mn ? mm_encode(&P.map_a, A.p, type, am, K, A.stride, 64, 64) : mm_encode(&P.map_a, A.p, type, K, M, A.stride, S.kel, S.a_box);
+    int st = Epi::kBuildA ? NQ_OK : mm_operand(&P.map_a, S.a, A, type, am, K, S.kel, a_rows);
     if (st != NQ_OK) return st;
-    st = S.b_mn == 2 ? mm_encode_columns(&P.map_b, B.p, type, bm, K, B.stride, S.b_box) : B.mn ? mm_encode(&P.map_b, B.p, type, bm, K, B.stride, 64, 64) : mm_encode(&P.map_b, B.p, type, K, N, B.stride, S.kel, S.b_box);
+    st = mm_operand(&P.map_b, S.b, B, type, bm, K, S.kel, b_rows);
     if (st != NQ_OK) return st;
     const int64_t tiles = (int64_t)S.m_tiles * S.n_tiles * S.splits, most = sm_count() / CG;
     if (tiles > 0x3fffffff) return NQ_ERR_TOO_LARGE;

@@ -69,8 +69,8 @@ PgemmPlan plan_pgemm(const StageJob* jobs, int n, int T, int order);
 int launch_pgemm_stage(const StageJob* jobs, int n, int T, StageTypes ty, int saturate, const PgemmPlan& plan, unsigned* status,
                        cudaStream_t stream);
 
-// Element types of a dense product (nq_mm.cuh), and a 2-D tensor map of one: `inner` contiguous elements, `outer` rows `stride` bytes apart,
-// 128-byte swizzle.
+// Element types of a dense product (nq_mm.cuh), and a tensor map [1][outer][inner] of one: `inner` contiguous elements, `outer` rows `stride` bytes
+// apart, 128-byte swizzle.
 enum : int { kMmF16 = 0, kMmBf16 = 1, kMmS8 = 2 };
 int mm_encode(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int box_inner, int box_outer);
 // The same matrix as [inner / 64][outer][64], for one load of `boxes` columns of 64 x 64 elements (inner a multiple of 64).

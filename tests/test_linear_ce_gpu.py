@@ -143,6 +143,63 @@ def test_gradient_matches_differences():
         assert abs(slope - diff) <= bound and bound < 0.5 * abs(slope) + 1, (slope, diff, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N,V,ignored", [(600, 1024, 200000, 0.5), (1030, 1024, 110000, 0.97), (2500, 2048, 20000, 0.1), (700, 2048, 80000, 0.0), (513, 2048, 100000, 1.0),
+                                           (20000, 128, 40000, 0.3)])
+def test_tokens_without_a_target_take_no_part(T, N, V, ignored, dtype):
+    """Sizes at which the rows that have a target are packed: a few, most, all and none of them (and one that is no word)."""
+    h, w, t = make(T, N, V, dtype, seed=T, ignored=ignored)
+    if ignored == 1.0:
+        t[:] = -100
+    else:
+        t[7:200] = -100                      # whole runs, the last row among them
+        t[-1] = -100
+        t[3], t[250] = 5, V // 2
+    if ignored == 0.0:
+        t[t == -100] = 1
+    live = t != -100
+    clean = h.clone()
+    h[~live] = float("nan")
+    g = torch.rand(T, device="cuda") * 16
+    got = run(h, w, t, "none", g)
+    assert not got[1][~live].any() and not got[0][~live].any()
+    rows = torch.cat([live.nonzero()[:40, 0], live.nonzero()[-40:, 0]])
+    if len(rows):
+        # 64 bits for some tokens, and for dw the words that are some tokens' targets and others
+        want = reference(clean[rows], w, t[rows], "none", g[rows])
+        u = torch.finfo(dtype).eps / 2
+        for name, x, (x64, bound) in zip(("loss", "dh"), got, want):
+            # (fp16: rounded relative to the largest |g| of all tokens)
+            extra = 2.0 ** -25 / 2 ** 14 * 16 * w.double().abs().sum(0) if name == "dh" and dtype == torch.float16 else 0
+            assert ((x[rows].double() - x64).abs() <= bound * (1 + 2.0 ** -9) + extra).all(), name
+        words = torch.cat([t[rows], torch.arange(64, device="cuda")])
+        hl, wl = clean[live].double(), w.double()
+        lse = torch.cat([torch.logsumexp(c.double() @ wl.T, 1) for c in clean[live].split(256)])
+        l = hl @ wl[words].T
+        d = ((l - lse[:, None]).exp() - (t[live][:, None] == words).double()) * g[live].double()[:, None]
+        E = (N / 16 + 16) * 2.0 ** -23 * (hl.abs() @ wl[words].abs().T)
+        dw = d.T @ hl
+        off = (d + (t[live][:, None] == words) * g[live][:, None]) * (2 * E + 2.0 ** -18 + 2 * E.amax(1, keepdim=True)) + d.abs() * u + 2.0 ** -25 / 2 ** 14 * 16
+        bound = off.T @ hl.abs() + (T / 16 + 64) * 2.0 ** -23 * (d.abs().T @ hl.abs()) + u * dw.abs() + TINY[dtype]
+        assert ((got[2][words].double() - dw).abs() <= bound * (1 + 2.0 ** -9)).all()
+    else:
+        assert not got[2].any()
+    # invalid targets among them
+    if len(rows):
+        t[rows[0]] = V
+        bad = run(h, w, t, "none", g)
+        assert torch.isnan(bad[0][rows[0]]) and torch.isnan(bad[1][rows[0]]).all()
+        others = torch.ones(T, dtype=torch.bool, device="cuda")
+        others[rows[0]] = False
+        assert torch.equal(bad[0][others], got[0][others]) and torch.equal(bad[1][others], got[1][others])
+    # the packed rows of one call are those of the tokens alone
+    if live.any() and ignored > 0:
+        alone = run(clean[live], w, t[live].clamp(max=V - 1), "sum", 2.0)
+        t2 = t.clamp(max=V - 1)
+        both = run(h, w, t2, "sum", 2.0)
+        assert abs(both[0] - alone[0]) <= 1e-5 * alone[0].abs() and ((both[1][live].double() - alone[1].double()).abs() <= 2.0 ** -7 * alone[1].double().abs() + 1e-4).all()
+
+
 def test_ignored_tokens_hold_anything():
     h, w, t = make(140, 64, 500, torch.bfloat16, seed=5, ignored=0.0)
     t[3::7] = 7

@@ -83,7 +83,8 @@ def test_loss_refusals():
 
 @pytest.mark.parametrize("T,N,V", [(1, 4096, 151936), (128, 4096, 151936), (2048, 4096, 151936), (4096, 4096, 32000), (77, 512, 1003), (30000, 64, 151936)])
 def test_loss_scratch_is_a_piece_and_not_the_logits(T, N, V):
-    """One piece of the vocabulary (256 MB, or 256 words), the hidden states once more and the partial sums of dh (256 MB)."""
+    """One piece of the vocabulary (256 MB, or 256 words), the hidden states once more and the partial sums of dh (256 MB); forward 8 bytes for every 64 words
+    and token of one product, and the hidden states of these."""
     piece = max(256 << 20, T * 256 * 2)
-    assert _lib.lib().nq_linear_ce_bwd_scratch_bytes(T, N, V) <= piece + 2 * T * N + 2 * (256 << 20) + 4 * T + 4096
-    assert _lib.lib().nq_linear_ce_fwd_scratch_bytes(T, N, V) <= 2 * (V // 64 + 1) * min(T, 16384) * 8 + 8 * T + 1024
+    assert _lib.lib().nq_linear_ce_bwd_scratch_bytes(T, N, V) <= piece + 2 * T * N + 2 * (256 << 20) + 16 * T + 4096
+    assert _lib.lib().nq_linear_ce_fwd_scratch_bytes(T, N, V) <= 2 * (V // 64 + 1) * min(T, 16384) * 8 + 2 * min(T, 16384) * N + 16 * T + 2048
