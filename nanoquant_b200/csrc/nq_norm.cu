@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(32 * WARPS * norm_rows_per_cta<WARPS>()) norm_
         for (int p = 0; p < PACKS; ++p)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s.x += norm_at<VEC, BF16>(v[p], e);
-        mean = group_sum2<WARPS>(s, red, turn).x * P.inv_n;
+        mean = group_sum2<WARPS>(s, red, turn).x / P.N;      // (exact where the sum is: a constant row's differences are zero)
     }
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
@@ -297,6 +297,9 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+// (x - m) r of two elements, from -m and r.  The difference first: x r - m r would round twice to the size of m r, many times the result's in rows far from zero.
+template <bool CENTER>
+__device__ __forceinline__ f32x2 norm_hat(f32x2 x, f32x2 shift, f32x2 r) { return mul2(CENTER ? add2(x, shift) : x, r); }
 template <bool BF16>
 __device__ __forceinline__ f32x2 unpack2(uint32_t w) {
     if constexpr (BF16) return pair2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -323,7 +326,7 @@ __device__ __forceinline__ void weights2(const void* p, int w32, int c, f32x2 (&
 // warps serves all of them, and they are read again for the outputs; each time from shared memory, by the thread that copied them (cp.async).  The next
 // batch is on its way meanwhile.  16384 x 5120, layer norm, us: a row at a time 97 forward and 200 backward (waiting for reductions); batches with
 // addresses computed for every access 78 and 105 (20 and 30 instructions per element); rows PITCH bytes apart in shared memory, PITCH a constant, and
-// sums of several rows in one butterfly 59 and 90 (5.6 TB/s; RMS 60 and 83).
+// sums of several rows in one butterfly 59 and 91; with the difference from the mean taken first (norm_hat) 61 and 93 (5.4 TB/s; RMS 61 and 84).
 template <int PITCH, bool BWD>
 struct NormShape {
     static constexpr int kPacks = PITCH <= 4096 || (BWD && PITCH <= 10240) ? 1 : PITCH <= 16384 ? 2 : 4;      // times eight columns a thread
@@ -386,8 +389,10 @@ __device__ __forceinline__ void group_moments(NormGroup& g, int parity, Count co
     mean = squares = 0.f;
     const int i0 = g.lane & (32 / ROWS - 1);
     if constexpr (CENTER) {
-        for (int i = i0; i < g.warps; i += 32 / ROWS) mean = fmaf(count(i), all[16 * i + ROWS], mean);
-        mean = join(mean) * inv_n;
+        // (by the distances from the first warp's: rounded once to the size of the mean, whose rounding counts 1 / sigma times)
+        const float start = all[ROWS];
+        for (int i = i0; i < g.warps; i += 32 / ROWS) mean = fmaf(count(i), all[16 * i + ROWS] - start, mean);
+        mean = fmaf(join(mean), inv_n, start);
         for (int i = i0; i < g.warps; i += 32 / ROWS) {
             const float d = all[16 * i + ROWS] - mean;
             squares += fmaf(count(i) * d, d, all[16 * i]);
@@ -452,7 +457,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
         for (int p = 0; p < PACKS; ++p) n += max(0, min(32, packs - p * G - 32 * warp));
         return 8.f * n;
     };
-    const float inv_own = 1.f / count(g.tid >> 5);
+    const float own_columns = count(g.tid >> 5);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     copy(0);
     copy(1);
@@ -490,7 +495,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
                     }
                 v[r] = split2(s).x + split2(s).y;
             }
-            own = warp_sums(v) * inv_own;
+            own = warp_sums(v) / own_columns;
         }
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
         char* dst = y;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const float rs = __shfl_sync(0xffffffffu, rstd, r * (32 / ROWS)), ms = CENTER ? -rs * __shfl_sync(0xffffffffu, mean, r * (32 / ROWS)) : 0.f;
+            const float rs = __shfl_sync(0xffffffffu, rstd, r * (32 / ROWS)), ms = CENTER ? -__shfl_sync(0xffffffffu, mean, r * (32 / ROWS)) : 0.f;
             const f32x2 r2 = pair2(rs, rs), shift = pair2(ms, ms);
             if (r < rows) {
 #pragma unroll
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
                         unpack8(norm_shared(at[p] + r * PITCH), xw);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            xw[k] = repack2<BF16>(CENTER ? fma2(fma2(unpack2<BF16>(xw[k]), r2, shift), w[p][k], b[p][k]) : mul2(mul2(unpack2<BF16>(xw[k]), r2), w[p][k]));
+                            xw[k] = repack2<BF16>(CENTER ? fma2(norm_hat<true>(unpack2<BF16>(xw[k]), shift, r2), w[p][k], b[p][k]) : mul2(mul2(unpack2<BF16>(xw[k]), r2), w[p][k]));
                         *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
                     }
             }
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
     int stage = 0;
     for (long long batch = first; batch < batches; batch += step, dx += next_dx) {
         const int rows = (int)min((long long)ROWS, P.rows - batch * ROWS);
-        const float rstd = next.y, shift = -next.x * next.y;       // of row `lane`
+        const float rstd = next.y, shift = -next.x;                // of row `lane`
         next = load_stats(batch + step);
         uint32_t at[PACKS];
 #pragma unroll
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
                         unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const f32x2 xh = fma2(unpack2<BF16>(xw[k]), r2, s2), d = unpack2<BF16>(dw[k]), gr = mul2(d, w[p][k]);
+                            const f32x2 xh = norm_hat<CENTER>(unpack2<BF16>(xw[k]), s2, r2), d = unpack2<BF16>(dw[k]), gr = mul2(d, w[p][k]);
                             sx = fma2(gr, xh, sx);
                             aw[p][k] = fma2(d, xh, aw[p][k]);
                             if constexpr (CENTER) {
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
                             unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                const f32x2 xh = fma2(unpack2<BF16>(xw[k]), r2, s2);
+                                const f32x2 xh = norm_hat<CENTER>(unpack2<BF16>(xw[k]), s2, r2);
                                 xw[k] = repack2<BF16>(fma2(mul2(unpack2<BF16>(dw[k]), w[p][k]), r2, fma2(xh, c1p, c2p)));
                             }
                             *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
@@ -698,7 +703,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
 // A row's 16-byte units (the first and the last hold elements of its neighbours, or what lies around the tensor in these units, which is ignored) are
 // copied as they are, and a thread takes the columns tid, tid + G, ...: single elements, but out of shared memory, and stores side by side.  A row is
 // read by others than copied it: one more barrier a batch, behind which the batch after this one is requested.  8000 x 5001, us: layer norm forward
-// 147 -> 107, backward 322 -> 118 against the direct kernels; bound by the loads of single elements from shared memory.
+// 147 -> 107, backward 322 -> 119 against the direct kernels; bound by the loads of single elements from shared memory.
 __device__ __forceinline__ uint16_t ragged_shared(uint32_t addr) {
     uint16_t h;
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr) : "memory");
@@ -743,7 +748,7 @@ __global__ void __launch_bounds__(512, 1) norm_fwd_ragged_kernel(const NormParam
         for (int e = 0; e < COLS; ++e) n += max(0, min(32, N - e * G - 32 * warp));
         return (float)n;
     };
-    const float inv_own = 1.f / count(tid >> 5);
+    const float own_columns = count(tid >> 5);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     copy(first, 0);
     uint32_t off[COLS];                    // bytes of the thread's columns
@@ -772,7 +777,7 @@ __global__ void __launch_bounds__(512, 1) norm_fwd_ragged_kernel(const NormParam
 #pragma unroll
                 for (int e = 0; e < COLS; ++e) v[r] += live(e) ? norm_float<BF16>(ragged_shared(at[r] + off[e])) : 0.f;
             }
-            own = warp_sums(v) * inv_own;
+            own = warp_sums(v) / own_columns;
         }
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -791,14 +796,14 @@ __global__ void __launch_bounds__(512, 1) norm_fwd_ragged_kernel(const NormParam
             P.stats[batch * ROWS + g.lane / (32 / ROWS)] = make_float2(mean, rstd);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const float rs = __shfl_sync(0xffffffffu, rstd, r * (32 / ROWS)), ms = CENTER ? -rs * __shfl_sync(0xffffffffu, mean, r * (32 / ROWS)) : 0.f;
+            const float rs = __shfl_sync(0xffffffffu, rstd, r * (32 / ROWS)), ms = CENTER ? -__shfl_sync(0xffffffffu, mean, r * (32 / ROWS)) : 0.f;
             const f32x2 r2 = pair2(rs, rs), shift = pair2(ms, ms);
             if (r < rows) {
                 char* dst = static_cast<char*>(P.y) + 2 * (batch * ROWS + r) * P.ldy;
 #pragma unroll
                 for (int e = 0; e < COLS; e += 2) {
                     const f32x2 xv = ragged_pair<BF16>(at[r] + off[e], at[r] + off[e + 1]);
-                    const uint32_t o = repack2<BF16>(CENTER ? fma2(fma2(xv, r2, shift), w[e / 2], b[e / 2]) : mul2(mul2(xv, r2), w[e / 2]));
+                    const uint32_t o = repack2<BF16>(CENTER ? fma2(norm_hat<true>(xv, shift, r2), w[e / 2], b[e / 2]) : mul2(mul2(xv, r2), w[e / 2]));
                     if (live(e)) *reinterpret_cast<uint16_t*>(dst + off[e]) = (uint16_t)o;
                     if (live(e + 1)) *reinterpret_cast<uint16_t*>(dst + off[e + 1]) = (uint16_t)(o >> 16);
                 }
@@ -844,7 +849,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ragged_kernel(const NormParam
     for (long long batch = first; batch < batches; batch += step) {
         const int rows = (int)min((long long)ROWS, P.rows - batch * ROWS);
         const float2 st = lane < rows ? __ldg(P.stats + batch * ROWS + lane) : make_float2(0.f, 0.f);
-        const float rstd = st.y, shift = -st.x * st.y;
+        const float rstd = st.y, shift = -st.x;
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         g.sync();                          // this batch is there for all, and all have left the one before
         copy(batch + step, stage ^ 1);
@@ -864,7 +869,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ragged_kernel(const NormParam
             if (r < rows) {
 #pragma unroll
                 for (int e = 0; e < COLS; e += 2) {
-                    const f32x2 xh = fma2(ragged_pair<BF16>(ax[r] + off[e], ax[r] + off[e + 1]), r2, s2), d = ragged_pair<BF16>(ad[r] + off[e], ad[r] + off[e + 1]);
+                    const f32x2 xh = norm_hat<CENTER>(ragged_pair<BF16>(ax[r] + off[e], ax[r] + off[e + 1]), s2, r2), d = ragged_pair<BF16>(ad[r] + off[e], ad[r] + off[e + 1]);
                     const f32x2 gr = mul2(d, w[e / 2]);
                     sx = fma2(gr, xh, sx);
                     aw[e / 2] = fma2(d, xh, aw[e / 2]);
@@ -888,7 +893,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ragged_kernel(const NormParam
                     char* dst = static_cast<char*>(P.y) + 2 * (batch * ROWS + r) * P.ldy;
 #pragma unroll
                     for (int e = 0; e < COLS; e += 2) {
-                        const f32x2 xh = fma2(ragged_pair<BF16>(ax[r] + off[e], ax[r] + off[e + 1]), r2, s2), d = ragged_pair<BF16>(ad[r] + off[e], ad[r] + off[e + 1]);
+                        const f32x2 xh = norm_hat<CENTER>(ragged_pair<BF16>(ax[r] + off[e], ax[r] + off[e + 1]), s2, r2), d = ragged_pair<BF16>(ad[r] + off[e], ad[r] + off[e + 1]);
                         const uint32_t o = repack2<BF16>(fma2(mul2(d, w[e / 2]), r2, fma2(xh, c1p, c2p)));
                         if (live(e)) *reinterpret_cast<uint16_t*>(dst + off[e]) = (uint16_t)o;
                         if (live(e + 1)) *reinterpret_cast<uint16_t*>(dst + off[e + 1]) = (uint16_t)(o >> 16);
@@ -1058,7 +1063,7 @@ int launch_norm(const NormVariant& v, long long ctas, const NormParams& P, cudaS
 }
 bool norm_rows_aligned(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
 // Direct kernels for few rows, and for short rows at any address (8192 x 1003 of layer norm, us: forward 18.0 and 21.1 ragged, backward 27.2 and 37.4;
-// 8000 x 5001: 147 and 107, 322 and 118).
+// 8000 x 5001: 147 and 107, 322 and 119).
 bool norm_streamed(bool vec, int64_t rows, int64_t N) { return rows > 2 * sm_count() && (vec || N > 1024); }
 
 }  // namespace nq

@@ -146,6 +146,29 @@ def test_norm_values_that_are_not_finite_stay_in_their_row():
     assert torch.equal(ops.rms_norm(big), torch.ones_like(big))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 40), (5, 1003), (400, 256), (400, 1000), (301, 5120), (333, 5001), (600, 8200)])
+def test_layer_norm_of_rows_far_from_zero(rows, cols, dtype):
+    """Rows c + k step, k = 0..3, which both types hold; c up to 250 steps.  All sums of x are whole steps below 2^24 and exact; a mean is rounded once per warp
+    and once over the warps, 3 2^-24 of it with what the distances between the warps' add, and x less the mean is exact.  Constant rows (k = 0) have no error."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    c = torch.randint(130, 250, (rows, 1), generator=g, device="cuda")
+    k = torch.randint(0, 4, (rows, cols), generator=g, device="cuda") * (torch.arange(rows, device="cuda") % 3 > 0)[:, None]
+    x = ((c + k) * 4).to(dtype)
+    _, w, b, dy = make((rows, cols), dtype, seed=4)
+    y, dx, dw, _ = run(x, w, b, dy, True)
+    m = x.detach().double().mean(-1, keepdim=True)
+    (want, _, _, _), _ = reference(x, w, b, dy, 1e-5, True)
+    r = 1 / (((x.detach().double() - m) ** 2).mean(-1, keepdim=True) + 1e-5).sqrt()
+    wd, bd = w.detach().double().abs(), b.detach().double().abs()
+    moved = (torch.arange(rows, device="cuda") % 3 > 0)[:, None]
+    bound = half_step(dtype) * want.abs() + moved * (3 * 2.0 ** -24 * m * r * wd + 2.0 ** -18 * (want.abs() + 2 * bd)) + TINY[dtype]
+    excess = ((y.double() - want).abs() - bound * (1 + 2.0 ** -10)).max().item()
+    assert excess <= 0, excess
+    flat = run(x[::3].detach().clone(), w, b, dy[::3], True)
+    assert torch.equal(flat[0], b.detach().expand_as(flat[0])) and not flat[2].any()
+
+
 def test_norm_no_rows():
     from nanoquant_b200 import ops
 
@@ -191,6 +214,24 @@ def test_norm_refuses_a_capture_whose_gradient_the_default_stream_holds():
     with pytest.raises(RuntimeError, match="held by an autograd graph"):
         with torch.cuda.graph(graph, stream=side):
             ops.layer_norm(x, w, b)
+    del held
+    torch.cuda.synchronize()
+    assert torch.isfinite(ops.layer_norm(x, w, b)).all()
+
+
+def test_norm_refuses_such_a_capture_behind_other_operations():
+    """The leaf whose accumulator the default stream made need not be an argument itself."""
+    from nanoquant_b200 import ops
+
+    x, w, b, dy = make((4, 64), torch.bfloat16, seed=8)
+    x.requires_grad_()
+    held = ops.layer_norm(x, w, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="held by an autograd graph"):
+        with torch.cuda.graph(graph, stream=side):
+            ops.layer_norm(x.view(2, 2, 64) * 2, w, b)
     del held
     torch.cuda.synchronize()
     assert torch.isfinite(ops.layer_norm(x, w, b)).all()
