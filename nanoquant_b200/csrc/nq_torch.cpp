@@ -27,6 +27,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -35,6 +36,7 @@
 
 #include <mutex>
 #include <optional>
+#include <unordered_set>
 #include <vector>
 
 #include "nanoquant_b200.h"
@@ -564,16 +566,32 @@ bool capturing(int dev) {
 }
 // A leaf's gradient is accumulated on the stream on which its accumulator was made.  While another graph holds an accumulator made on the
 // default stream, a captured backward pass would have that stream wait for the capture, which it cannot, and which ends the process: refuse the
-// call instead.  (Other streams join the capture and leave it again.)
+// call instead, wherever behind its inputs such a leaf is.  (Other streams join the capture and leave it again.)
 void check_capture(int dev, std::initializer_list<const Tensor*> inputs) {
     if (!capturing(dev)) return;
+    using torch::autograd::Node;
     const c10::Stream first = c10::cuda::getDefaultCUDAStream((c10::DeviceIndex)dev).unwrap();
+    std::vector<Node*> left;
+    std::unordered_set<Node*> seen;
+    auto visit = [&](Node* n) {
+        if (n && seen.insert(n).second) left.push_back(n);
+    };
+    std::shared_ptr<Node> held[3];          // (accumulators live only as long as a graph holds them)
+    size_t n = 0;
     for (const Tensor* t : inputs) {
-        if (!t || !t->defined() || !t->requires_grad() || t->grad_fn()) continue;
-        const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
-        TORCH_CHECK(!acc || !acc->stream() || *acc->stream() != first,
-                    "a leaf of this captured call is held by an autograd graph made on the default stream: its gradient cannot be captured; "
-                    "release that graph first, or make it on another stream");
+        if (!t || !t->defined() || !t->requires_grad()) continue;
+        if (t->grad_fn()) held[n] = t->grad_fn();
+        else held[n] = torch::autograd::impl::try_get_grad_accumulator(*t);
+        visit(held[n++].get());
+    }
+    while (!left.empty()) {
+        Node* node = left.back();
+        left.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node))
+            TORCH_CHECK(!node->stream() || *node->stream() != first,
+                        "a leaf of this captured call is held by an autograd graph made on the default stream: its gradient cannot be captured; "
+                        "release that graph first, or make it on another stream");
+        for (const auto& e : node->next_edges()) visit(e.function.get());
     }
 }
 

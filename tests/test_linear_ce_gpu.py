@@ -319,6 +319,21 @@ def test_capture_that_the_default_stream_holds_is_refused():
     assert torch.isfinite(held)
 
 
+def test_such_a_capture_is_refused_for_a_padded_batch_of_hidden_states():
+    """[batch, length, N] reaches the product as a view of the leaf."""
+    from nanoquant_b200 import ops
+
+    h, w, t = make(12, 64, 100, torch.bfloat16)
+    h, t = h.view(3, 4, 64).requires_grad_(), t.view(3, 4)
+    held = ops.linear_cross_entropy(h, w, t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="held by an autograd graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            ops.linear_cross_entropy(h, w, t)
+    assert torch.isfinite(held)
+
+
 def test_training_step_captured_behind_a_warm_up_that_is_still_held():
     """The usual way to capture a training step: warm-up on a side stream, whose loss lives on while the step is captured."""
     from nanoquant_b200 import ops
