@@ -390,8 +390,9 @@ int nq_int8_linear_fwd(const void* x, const int8_t* w, const float* w_scale, con
  *     lse[t] = log sum_v exp(h[t] . w[v]),   loss[t] = lse[t] - h[t] . w[target[t]]
  * `targets`: T int32 or int64 (target_bits).  A token whose target is ignore_index has no loss and no gradient, whatever its row holds; any
  * other target outside 0..V-1 makes its loss and gradient NaN.  `loss`: T floats (NQ_REDUCE_NONE) or one; the mean of no tokens is NaN.
- * lse [T] and count [1] (tokens with a target; not written for NQ_REDUCE_NONE) are what the backward pass reads.  `status_word` as in
- * nq_onebit_gemm_fwd.  Scratch: 16-byte aligned, any contents.
+ * lse [T] (without meaning for a token without a target) and count [1] (tokens with one; not written for NQ_REDUCE_NONE) are what the backward pass
+ * reads.  Calls of more than 512 tokens and 2e11 operations a product pack the rows that have a target, which the scratch holds a copy of: prompts and
+ * padding cost no products.  `status_word` as in nq_onebit_gemm_fwd.  Scratch: 16-byte aligned, any contents.
  * The reference evaluates perplexity and tunes its scales with this loss (src/nanoquant/utils/eval_utils.py:13-87,
  * core/compress_model.py:125-286), by torch's product and cross entropy or another package's fused one. */
 size_t nq_linear_ce_fwd_scratch_bytes(int64_t T, int64_t N, int64_t V);

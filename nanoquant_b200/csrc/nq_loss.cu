@@ -8,9 +8,11 @@
 //
 // Backward, over pieces of the vocabulary whose d fits the scratch (kLossPieceBytes): the logits of the piece once more, d from them and
 // the kept lse, rounded to the type of the operands (what the tensor cores multiply), then dw of the piece, complete, and the piece's part of
-// dh, added in fp32.  So four products in all, 8 T N V operations, and no more memory than a piece.
+// dh, added in fp32.  So four products in all, 8 T N V operations (T: the tokens that have a target, in larger calls), and no more memory than a piece.  The
+// logits in fp32 would save the fourth product, and take 4 T V bytes: 1.2 GB for 2048 tokens and 151936 words.
 //
-// Bound by the tensor cores from some 300 tokens on, below by reading w (each product once).
+// Bound by the tensor cores from some 300 tokens on, below by reading w (each product once).  2048 tokens, 51200 x 4096, all with a target, us: logits and
+// their sums 521, d 527, dw 534, dh 571, the tensor cores busy for 94 to 98 % of the cycles; packing 7, joining 10, preparing 12, adding dh 17.
 #include "nq_common.cuh"
 #include "nq_mm.cuh"
 
