@@ -269,6 +269,7 @@ __device__ __forceinline__ uint4 norm_shared(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ void norm_clear(uint32_t addr) { asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory"); }
 // Two fp32 numbers in one 64-bit register, and the instructions that work on both: with one element at a time the stream kernels were bound by
 // instruction issue (16384 x 5120: 28 instructions per element forward, 34 backward).
 typedef unsigned long long f32x2;
@@ -326,7 +327,8 @@ __device__ __forceinline__ void weights2(const void* p, int w32, int c, f32x2 (&
 // warps serves all of them, and they are read again for the outputs; each time from shared memory, by the thread that copied them (cp.async).  The next
 // batch is on its way meanwhile.  16384 x 5120, layer norm, us: a row at a time 97 forward and 200 backward (waiting for reductions); batches with
 // addresses computed for every access 78 and 105 (20 and 30 instructions per element); rows PITCH bytes apart in shared memory, PITCH a constant, and
-// sums of several rows in one butterfly 59 and 91; with the difference from the mean taken first (norm_hat) 61 and 93 (5.4 TB/s; RMS 61 and 84).
+// sums of several rows in one butterfly 59 and 91; with the difference from the mean taken first (norm_hat) 61 and 93; without branches for the columns beyond N
+// 59 and 92.5 (5.7 and 5.4 TB/s; RMS 60 and 84).
 template <int PITCH, bool BWD>
 struct NormShape {
     static constexpr int kPacks = PITCH <= 4096 || (BWD && PITCH <= 10240) ? 1 : PITCH <= 16384 ? 2 : 4;      // times eight columns a thread
@@ -458,6 +460,11 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
         return 8.f * n;
     };
     const float own_columns = count(g.tid >> 5);
+    // Slots of columns beyond N hold zeros, so that the loops below need no branches for them.
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p)
+        if (!live(p))
+            for (int i = 0; i < 2 * ROWS; ++i) norm_clear(mine + (uint32_t)(p * G * 16 + i * PITCH));
     asm volatile("griddepcontrol.wait;" ::: "memory");
     copy(0);
     copy(1);
@@ -487,12 +494,11 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
             for (int r = 0; r < ROWS; ++r) {
                 f32x2 s = 0;
 #pragma unroll
-                for (int p = 0; p < PACKS; ++p)
-                    if (live(p)) {
-                        uint32_t xw[4];
-                        unpack8(norm_shared(at[p] + r * PITCH), xw);
-                        s = add2(s, add2(add2(unpack2<BF16>(xw[0]), unpack2<BF16>(xw[1])), add2(unpack2<BF16>(xw[2]), unpack2<BF16>(xw[3]))));
-                    }
+                for (int p = 0; p < PACKS; ++p) {
+                    uint32_t xw[4];
+                    unpack8(norm_shared(at[p] + r * PITCH), xw);
+                    s = add2(s, add2(add2(unpack2<BF16>(xw[0]), unpack2<BF16>(xw[1])), add2(unpack2<BF16>(xw[2]), unpack2<BF16>(xw[3]))));
+                }
                 v[r] = split2(s).x + split2(s).y;
             }
             own = warp_sums(v) / own_columns;
@@ -505,16 +511,16 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
                 shift = pair2(m, m);
             }
 #pragma unroll
-            for (int p = 0; p < PACKS; ++p)
-                if (live(p)) {
-                    uint32_t xw[4];
-                    unpack8(norm_shared(at[p] + r * PITCH), xw);
+            for (int p = 0; p < PACKS; ++p) {
+                uint32_t xw[4];
+                unpack8(norm_shared(at[p] + r * PITCH), xw);
+                const f32x2 own_shift = live(p) ? shift : 0;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const f32x2 d = CENTER ? add2(unpack2<BF16>(xw[k]), shift) : unpack2<BF16>(xw[k]);
-                        s = fma2(d, d, s);
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    const f32x2 d = CENTER ? add2(unpack2<BF16>(xw[k]), own_shift) : unpack2<BF16>(xw[k]);
+                    s = fma2(d, d, s);
                 }
+            }
             v[r] = split2(s).x + split2(s).y;
         }
         float squares = warp_sums(v), mean = own;
@@ -527,17 +533,14 @@ __global__ void __launch_bounds__(NormShape<PITCH, false>::kThreads, NormShape<P
         for (int r = 0; r < ROWS; ++r) {
             const float rs = __shfl_sync(0xffffffffu, rstd, r * (32 / ROWS)), ms = CENTER ? -__shfl_sync(0xffffffffu, mean, r * (32 / ROWS)) : 0.f;
             const f32x2 r2 = pair2(rs, rs), shift = pair2(ms, ms);
-            if (r < rows) {
 #pragma unroll
-                for (int p = 0; p < PACKS; ++p)
-                    if (live(p)) {
-                        uint32_t xw[4];
-                        unpack8(norm_shared(at[p] + r * PITCH), xw);
+            for (int p = 0; p < PACKS; ++p) {
+                uint32_t xw[4];
+                unpack8(norm_shared(at[p] + r * PITCH), xw);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            xw[k] = repack2<BF16>(CENTER ? fma2(norm_hat<true>(unpack2<BF16>(xw[k]), shift, r2), w[p][k], b[p][k]) : mul2(mul2(unpack2<BF16>(xw[k]), r2), w[p][k]));
-                        *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
-                    }
+                for (int k = 0; k < 4; ++k)
+                    xw[k] = repack2<BF16>(CENTER ? fma2(norm_hat<true>(unpack2<BF16>(xw[k]), shift, r2), w[p][k], b[p][k]) : mul2(mul2(unpack2<BF16>(xw[k]), r2), w[p][k]));
+                if (r < rows && live(p)) *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
             }
             dst += ldy;
         }
@@ -597,6 +600,11 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
             aw[p][k] = ab[p][k] = 0;
             w[p][k] = pair2(1.f, 1.f);
         }
+    // Slots of columns beyond N hold zeros, so that the loops below need no branches for them.
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p)
+        if (!live(p))
+            for (int i = 0; i < 4 * ROWS; ++i) norm_clear(mine + (uint32_t)(p * G * 16 + i * PITCH));
     asm volatile("griddepcontrol.wait;" ::: "memory");
     copy(0);
     copy(1);
@@ -621,22 +629,21 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
             f32x2 sx = 0, sg = 0;
             if (r < rows) {
 #pragma unroll
-                for (int p = 0; p < PACKS; ++p)
-                    if (live(p)) {
-                        uint32_t xw[4], dw[4];
-                        unpack8(norm_shared(at[p] + r * kSlot), xw);
-                        unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
+                for (int p = 0; p < PACKS; ++p) {
+                    uint32_t xw[4], dw[4];
+                    unpack8(norm_shared(at[p] + r * kSlot), xw);
+                    unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const f32x2 xh = norm_hat<CENTER>(unpack2<BF16>(xw[k]), s2, r2), d = unpack2<BF16>(dw[k]), gr = mul2(d, w[p][k]);
-                            sx = fma2(gr, xh, sx);
-                            aw[p][k] = fma2(d, xh, aw[p][k]);
-                            if constexpr (CENTER) {
-                                sg = add2(sg, gr);
-                                ab[p][k] = add2(ab[p][k], d);
-                            }
+                    for (int k = 0; k < 4; ++k) {
+                        const f32x2 xh = norm_hat<CENTER>(unpack2<BF16>(xw[k]), s2, r2), d = unpack2<BF16>(dw[k]), gr = mul2(d, w[p][k]);
+                        sx = fma2(gr, xh, sx);
+                        aw[p][k] = fma2(d, xh, aw[p][k]);
+                        if constexpr (CENTER) {
+                            sg = add2(sg, gr);
+                            ab[p][k] = add2(ab[p][k], d);
                         }
                     }
+                }
             }
             sums[r] = split2(sx).x + split2(sx).y;
             if constexpr (CENTER) sums[ROWS + r] = split2(sg).x + split2(sg).y;
@@ -652,18 +659,17 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
                 const f32x2 r2 = pair2(r1, r1), s2 = pair2(s1, s1), c1p = pair2(c1, c1), c2p = pair2(c2, c2);
                 if (r < rows) {
 #pragma unroll
-                    for (int p = 0; p < PACKS; ++p)
-                        if (live(p)) {
-                            uint32_t xw[4], dw[4];
-                            unpack8(norm_shared(at[p] + r * kSlot), xw);
-                            unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
+                    for (int p = 0; p < PACKS; ++p) {
+                        uint32_t xw[4], dw[4];
+                        unpack8(norm_shared(at[p] + r * kSlot), xw);
+                        unpack8(norm_shared(at[p] + r * kSlot + PITCH), dw);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const f32x2 xh = norm_hat<CENTER>(unpack2<BF16>(xw[k]), s2, r2);
-                                xw[k] = repack2<BF16>(fma2(mul2(unpack2<BF16>(dw[k]), w[p][k]), r2, fma2(xh, c1p, c2p)));
-                            }
-                            *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+                        for (int k = 0; k < 4; ++k) {
+                            const f32x2 xh = norm_hat<CENTER>(unpack2<BF16>(xw[k]), s2, r2);
+                            xw[k] = repack2<BF16>(fma2(mul2(unpack2<BF16>(dw[k]), w[p][k]), r2, fma2(xh, c1p, c2p)));
                         }
+                        if (live(p)) *reinterpret_cast<uint4*>(dst + p * G * 16) = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+                    }
                 }
                 dst += lddx;
             }
