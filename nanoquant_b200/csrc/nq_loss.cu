@@ -18,6 +18,8 @@
 
 namespace nq {
 
+// Bytes of d of a piece.  Three products of the backward pass, us at 64 / 128 / 256 / 512 MB: 2048 tokens, 151936 x 4096 6027 / 5807 / 5826 / 5797, 8192 tokens 24631 /
+// 24534 / 24291 / 23708, 16384 tokens, 32000 x 4096 11291 / 9967 / 10297 / 11164, 1000 tokens, 128256 x 8192 5135 / 5150 / 5042 / 5052.
 constexpr int64_t kLossPieceBytes = 256ll << 20;
 constexpr int kLossPieceUnit = 256;
 constexpr int kLossRows = 16384;           // tokens of a forward product: the scratch holds 8 bytes for each and every 64 to 128 words
@@ -491,8 +493,14 @@ static bool loss_pairs(int64_t T) { return T > 128; }
 // and more and have several tiles of 256 rows.
 static bool loss_packs(int64_t T, int64_t N, int64_t V) { return T > 512 && 2.0 * (double)T * (double)N * (double)V > 2e11; }
 
+// Forward: columns of a tile, pieces of a token's logits.
+struct LossTiles { int bn, slots; };
+static LossTiles loss_tiles(int64_t T, int64_t V) {
+    const int cg = loss_pairs(T) ? 2 : 1, bn = mm_tile_cols((int)V, (int)((T + 128 * cg - 1) / (128 * cg)), cg, 64);
+    return {bn, 2 * (int)((V + bn - 1) / bn)};
+}
+// Backward.
 struct LossPlan {
-    int bn, slots;                       // forward
     int64_t piece;                       // words
     int d_bn, w_bn, h_bn, h_splits, h_blocks, h_quads;
     bool h_direct;                       // one piece, one split: dh as the product writes it
@@ -500,8 +508,6 @@ struct LossPlan {
 static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     LossPlan p;
     const int cg = loss_pairs(T) ? 2 : 1, groups = sm_count() / cg, m_tiles = (int)((T + 128 * cg - 1) / (128 * cg));
-    p.bn = mm_tile_cols((int)V, m_tiles, cg, 64);
-    p.slots = 2 * (int)((V + p.bn - 1) / p.bn);
     p.piece = kLossPieceBytes / 2 / T / kLossPieceUnit * kLossPieceUnit;
     if (p.piece < kLossPieceUnit) p.piece = kLossPieceUnit;
     const int64_t all = up(V, kLossPieceUnit);
@@ -514,6 +520,9 @@ static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     p.w_bn = N <= 128 ? 128 : 256;
     // dh: few tiles over a long k, in us: rounds of the longest tile (a step takes 0.27, a tile's start and end as much as 8), the launch that adds the
     // splits' sums, and what writing (with several pieces, also reading) and adding them moves.
+    // dh alone, us with 1 / 2 / 4 / 8 splits and as chosen: 128 tokens, 32000 x 2048 210 / 126 / 83 / 65, 66; 512 tokens, 128256 x 2048 761 / 580 / 508 / 519, 528; 1024
+    // tokens 1083 / 903 / 914 / 919, 902; 2048 tokens, 51200 x 4096 1341 / 1376 / 1369 / 1392, 1359; 8192 tokens, 32000 x 2048 936 / 965 / 984 / 1063, 937 (the
+    // logits' product included; large ones run at the power limit, where idle SMs leave the others a higher clock).
     p.h_bn = cg == 2 ? (N <= 128 ? 128 : 256) : (N <= 64 ? 64 : N <= 128 ? 128 : 256);
     const int64_t tiles = (int64_t)m_tiles * ((N + p.h_bn - 1) / p.h_bn), steps = ((p.piece < V ? p.piece : V) + 63) / 64;
     const bool one = p.piece >= V && !loss_packs(T, N, V);
@@ -553,7 +562,7 @@ static LossFwdScratch loss_fwd_scratch(int64_t T, int64_t N, int64_t V) {
     LossFwdScratch s;
     int64_t part = 0;
     for (int64_t t : {T < kLossRows ? T : (int64_t)kLossRows, T % kLossRows}) {      // (the last product may be another one)
-        const int64_t bytes = t > 0 ? plan_loss(t, N, V).slots * t * 8 : 0;
+        const int64_t bytes = t > 0 ? loss_tiles(t, V).slots * t * 8 : 0;
         if (bytes > part) part = bytes;
     }
     const int64_t most = T < kLossRows ? T : (int64_t)kLossRows;
@@ -673,10 +682,10 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     int st = check_loss(T, N, V, ldh, ldw, dtype, reduction, target_bits);
     if (st != NQ_OK) return st;
     if (!aligned16(h) || !aligned16(w) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
-    if (scratch_bytes < nq_linear_ce_fwd_scratch_bytes(T, N, V)) return NQ_ERR_SCRATCH;
+    const LossFwdScratch at = loss_fwd_scratch(T, N, V);
+    if (scratch_bytes < (size_t)at.bytes) return NQ_ERR_SCRATCH;
     cudaStream_t s = as_stream(stream);
     unsigned* status = static_cast<unsigned*>(status_word) + 2;
-    const LossFwdScratch at = loss_fwd_scratch(T, N, V);
     char* base = static_cast<char*>(scratch);
     float2* part = reinterpret_cast<float2*>(base);
     float* target_logit = reinterpret_cast<float*>(base + at.target_logit);
@@ -687,8 +696,8 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     int slots = 0, v = (int)V, mean = reduction == NQ_REDUCE_MEAN, all_t = (int)T;
     for (int64_t t0 = 0; t0 < T; t0 += kLossRows) {
         int t = (int)(T - t0 < kLossRows ? T - t0 : kLossRows), release = reduction != NQ_REDUCE_NONE || t0 + t < T;
-        const LossPlan p = plan_loss(t, N, V);
-        slots = p.slots;
+        const LossTiles tiles = loss_tiles(t, V);
+        slots = tiles.slots;
         const char* rows = static_cast<const char*>(h) + t0 * ldh * 2;
         LossTargets tg = {static_cast<const char*>(targets) + t0 * (target_bits / 8), all.wide, ignore_index};
         int *pos = nullptr, *words = nullptr, *live = nullptr;
@@ -704,8 +713,8 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
             if (st != NQ_OK) return st;
         }
         const LseEpilogue::Params e = {tg, words, part, target_logit};
-        st = loss_pairs(t) ? launch_lse<2>(rows, packed, live, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s)
-                           : launch_lse<1>(rows, packed, live, w, e, t, (int)N, v, ldh, ldw, type, p.bn, status, s);
+        st = loss_pairs(t) ? launch_lse<2>(rows, packed, live, w, e, t, (int)N, v, ldh, ldw, type, tiles.bn, status, s)
+                           : launch_lse<1>(rows, packed, live, w, e, t, (int)N, v, ldh, ldw, type, tiles.bn, status, s);
         if (st != NQ_OK) return st;
         if (reduction != NQ_REDUCE_NONE && !pos && T <= 1024 && T * slots <= kLossJoinHere) {
             joined = part;
@@ -736,13 +745,13 @@ int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int targ
     if (st != NQ_OK) return st;
     if ((dh && (lddh < N || lddh % 8)) || (dw && (lddw < N || lddw % 8))) return NQ_ERR_SHAPE;
     if (!aligned16(h) || !aligned16(w) || !aligned16(dh) || !aligned16(dw) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
-    if (scratch_bytes < nq_linear_ce_bwd_scratch_bytes(T, N, V)) return NQ_ERR_SCRATCH;
-    if (!dh && !dw) return NQ_OK;
-    cudaStream_t s = as_stream(stream);
-    unsigned* status = static_cast<unsigned*>(status_word) + 2;
     const LossPlan p = plan_loss(T, N, V);
     const bool packs = loss_packs(T, N, V);
     const LossScratch at = loss_scratch(p, T, N, packs);
+    if (scratch_bytes < (size_t)at.bytes) return NQ_ERR_SCRATCH;
+    if (!dh && !dw) return NQ_OK;
+    cudaStream_t s = as_stream(stream);
+    unsigned* status = static_cast<unsigned*>(status_word) + 2;
     char* base = static_cast<char*>(scratch);
     LossTargets tg = {targets, target_bits == 64, ignore_index};
     LossRows R = {tg, static_cast<const uint4*>(h), dw || packs ? reinterpret_cast<uint4*>(base + at.h) : nullptr, ldh / 8, nullptr, nullptr, nullptr, (int)T, (int)V,

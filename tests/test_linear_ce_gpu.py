@@ -200,6 +200,32 @@ def test_tokens_without_a_target_take_no_part(T, N, V, ignored, dtype):
         assert abs(both[0] - alone[0]) <= 1e-5 * alone[0].abs() and ((both[1][live].double() - alone[1].double()).abs() <= 2.0 ** -7 * alone[1].double().abs() + 1e-4).all()
 
 
+def test_packed_call_replayed_with_other_targets():
+    """How many rows are packed is the device's knowledge: a captured step follows its targets, from none to all of the tokens."""
+    from nanoquant_b200 import ops
+
+    T, N, V = 1200, 1024, 90000
+    h, w, t = make(T, N, V, torch.bfloat16, seed=31, ignored=0.0)
+    h.requires_grad_(), w.requires_grad_()
+    held = t.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.linear_cross_entropy(h, w, held, reduction="sum"), (h, w))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            loss = ops.linear_cross_entropy(h, w, held, reduction="sum")
+            grads = torch.autograd.grad(loss, (h, w))
+    torch.cuda.current_stream().wait_stream(side)
+    for ignored in (0.4, 0.0, 1.0, 0.99, 0.05):
+        with torch.no_grad():
+            held.copy_(torch.where(torch.rand(T, device="cuda") < ignored, -100, t))
+        graph.replay()
+        want = ops.linear_cross_entropy(h, w, held, reduction="sum")
+        for a, b in zip((loss, *grads), (want, *torch.autograd.grad(want, (h, w)))):
+            assert torch.equal(a, b), ignored
+
+
 def test_ignored_tokens_hold_anything():
     h, w, t = make(140, 64, 500, torch.bfloat16, seed=5, ignored=0.0)
     t[3::7] = 7
