@@ -43,8 +43,11 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t top_bits) {
 }
 // 127 x is exact and the division IEEE, so that the result is that of the definition: 16-bit x and max|x| have at most 11 significant bits, and
 // 127 x / max|x| is half a whole number exactly (x = max|x| / 2 is: 63.5, to 64) or further from it than the quotient's rounding.  (x / s in fp32
-// would decide such halves by the rounding of s.)
-__device__ __forceinline__ int q8_exact(float x, float top) { return (int)rintf(127.f * x / top); }
+// would decide such halves by the rounding of s.)  Both times 2^-8, exactly (bf16 has no unit below 2^-133), where 127 x could leave fp32.
+__device__ __forceinline__ int q8_exact(float x, float top) {
+    const float unit = top > 1e36f ? 0.00390625f : 1.f;
+    return (int)rintf(127.f * (x * unit) / (top * unit));
+}
 // Eight values, as bytes.  The products with `inv` are off by 2^-16 at most, so that only quotients within 2^-14 of a half need the division (or where
 // `inv` has overflowed); adding 1.5 2^23 leaves a whole number in the low bits.
 template <bool BF16>
