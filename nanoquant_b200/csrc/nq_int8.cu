@@ -4,7 +4,7 @@
 //
 // s = max|x| / 127 of the token (or, for weights, of the output channel) and q = rint(127 x / max|x|).  The activations are quantised in a kernel
 // of its own, one CTA per token; the product's CTAs load their first weights meanwhile.  Sums of products are exact (int32, K up to
-// 2^31 / 127^2); the two scales are multiplied and applied in fp32.
+// 2^31 / 127^2); the two scales are applied in fp32, the channel's first.
 //
 // Few tokens are bound by the memory that the weights stream from: K V bytes, half of the 16-bit head.  The tokens are the MMA's 128
 // rows and the output channels its columns, so any number of tokens up to 128 costs the same reads.  Prompts are bound by the tensor
@@ -219,7 +219,7 @@ struct Int8Epilogue {
                 for (int k = 0; k < 4; ++k) f[k] = i + k < cols ? __ldg(ws + i + k) : 0.f;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = (float)(int)r[i + k] * (sx * f[k]);
+            for (int k = 0; k < 4; ++k) f[k] = (float)(int)r[i + k] * f[k] * sx;      // (s_x s_w may leave fp32 where the result does not)
             if (p.bias) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)

@@ -1,4 +1,4 @@
-"""8-bit rows and products over the whole range of bf16: magnitudes whose products with 127 fp32 does not hold."""
+"""8-bit rows and products over the whole range of bf16: magnitudes whose products with 127 fp32 does not hold, and scales whose product it does not hold."""
 import pytest
 import torch
 
@@ -41,3 +41,22 @@ def test_linear_of_the_largest_tokens(T, N):
     y, want = ops.int8_linear_forward(x, q[:, :N], s), expected(x, w, s, None)
     # exact sums; a few roundings of 2^-24, and the output's own of half a step: bf16 has 8 significant bits, so 2^-8 of a value just above a power of two
     assert ((y.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want.abs()).all()
+
+
+@pytest.mark.parametrize("T", [1, 3, 200])
+def test_linear_where_the_product_of_the_scales_leaves_fp32(T):
+    """s_x s_w overflows, or falls below the normal numbers, where the result does not: the sum is multiplied by one scale and then by the other."""
+    from nanoquant_b200 import ops
+
+    N, V = 64, 24
+    q = torch.zeros((V, N), dtype=torch.int8, device="cuda")
+    q[1::2, :32] = 127
+    b = torch.randn(V, device="cuda").bfloat16()
+    x = torch.full((T, N), 2.0 ** 120, dtype=torch.bfloat16, device="cuda")
+    x[:, 16:32] = -x[:, :16]                       # sums of zero
+    s = torch.full((V,), 2.0 ** 20, device="cuda")
+    assert torch.equal(ops.int8_linear_forward(x, q, s, b), b.expand(T, V))
+    x = torch.full((T, N), 2.0 ** -105, dtype=torch.bfloat16, device="cuda")
+    s = torch.full((V,), 2.0 ** -32, device="cuda")
+    y, want = ops.int8_linear_forward(x, q, s), expected(x, q, s, None)
+    assert want.max() > 2.0 ** -126 and ((y.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want).all()
