@@ -13,6 +13,8 @@
 //
 // Bound by the tensor cores from some 300 tokens on, below by reading w (each product once).  2048 tokens, 51200 x 4096, all with a target, us: logits and
 // their sums 521, d 527, dw 534, dh 571, the tensor cores busy for 94 to 98 % of the cycles; packing 7, joining 10, preparing 12, adding dh 17.
+#include <type_traits>
+
 #include "nq_common.cuh"
 #include "nq_mm.cuh"
 
@@ -22,6 +24,11 @@ namespace nq {
 // 24534 / 24291 / 23708, 16384 tokens, 32000 x 4096 11291 / 9967 / 10297 / 11164, 1000 tokens, 128256 x 8192 5135 / 5150 / 5042 / 5052.
 constexpr int64_t kLossPieceBytes = 256ll << 20;
 constexpr int kLossPieceUnit = 256;
+// Steps of 64 products after which a sum leaves the tensor cores, which cut it off towards zero with every instruction (nq_mm.cuh).  Logits: the same in both
+// passes, so that the backward's are the numbers that lse came from.  (With whole sums there, p - 1 of a target with p = 0.999 was off by 6 to 19 % at 4096 columns and
+// by up to 38 % at 8192.)  Forward level with whole sums, with 256 columns 5 % slower; the backward's logits and d 9 to 15 % slower, 2 to 6 % of the pass: a tile's
+// outputs all come at its end.
+constexpr int kLossLogitsChunk = 8;
 constexpr int kLossRows = 16384;           // tokens of a forward product: the scratch holds 8 bytes for each and every 64 to 128 words
 constexpr int kLossJoinHere = 8192;        // pieces of all tokens that one CTA joins
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -122,7 +129,7 @@ __global__ void __launch_bounds__(512) loss_pack_kernel(const LossRows R, int pe
 // ---------------------------------------------------------------------------
 struct LseEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
-    static constexpr int kChunk = 8;           // 512 columns: 2048 x 4096 x 151936 level with a whole sum (1.60 ms), with 256 1.69
+    static constexpr int kChunk = kLossLogitsChunk;
     struct Params {
         LossTargets targets;
         const int* words;          // nullable: the rows' targets (-1: none of the vocabulary's), else `targets` has them
@@ -167,6 +174,7 @@ struct LseEpilogue {
                 if (at == i) p.target_logit[row] = __uint_as_float(r[i]);
         }
     }
+    __device__ __forceinline__ void flush(int, int, const unsigned char*) {}
     __device__ __forceinline__ void end() {
         if (row < dims->live) p.part[(long long)slot * s.M + row] = make_float2(top, sum);
     }
@@ -327,10 +335,10 @@ __global__ void __launch_bounds__(512) loss_prepare_kernel(const LossPrepare P, 
 }
 
 // d of a piece of the vocabulary.
-template <int OUT>
+template <int OUT, bool LONG>
 struct GradEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
-    static constexpr int kChunk = 0;
+    static constexpr int kChunk = LONG ? kLossLogitsChunk : 0;
     struct Params {
         LossTargets targets;
         const int* words;          // as in LseEpilogue; then all rows below `live` count
@@ -606,6 +614,13 @@ static int launch_lse(const void* h, const void* packed, const int* live, const 
     return mm_launch<CG>(P, type, {h, ldh * 2, 0}, {w, ldw * 2, 0}, T, V, N, bn, 1, 0, 1, status, stream);
 }
 
+// `run` with the kernels that add a sum of k products up by chunks of `steps`, or, where one chunk is all of it, with those that keep no sums in registers and
+// write outputs as they are loaded.
+template <class Run>
+static int by_length(int64_t k, int steps, Run run) {
+    return k > 64 * steps ? run(std::true_type()) : run(std::false_type());
+}
+
 template <int CG, int OUT>
 static int launch_backward(const void* h, const void* w, const LossTargets& targets, const float* lse, void* dh, void* dw, char* scratch,
                            const LossPlan& p, const LossScratch& at, int T, int N, int V, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw,
@@ -623,20 +638,20 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece);
         const char* wp = static_cast<const char*>(w) + v0 * ldw * 2;
-        {
-            MmParams<GradEpilogue<OUT>> P = {};
-            const typename GradEpilogue<OUT>::Params e = {targets, words, lse, reinterpret_cast<float*>(scratch + at.row_scale), d, p.piece, (int)v0};
+        int st = by_length(N, kLossLogitsChunk, [&](auto is_long) {
+            MmParams<GradEpilogue<OUT, is_long>> P = {};
+            const typename GradEpilogue<OUT, is_long>::Params e = {targets, words, lse, reinterpret_cast<float*>(scratch + at.row_scale), d, p.piece, (int)v0};
             P.e = e;
             P.s.live = live;
-            const int st = mm_launch<CG>(P, type, {rows, ld_rows * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 1, 1, status, stream);
-            if (st != NQ_OK) return st;
-        }
+            return mm_launch<CG>(P, type, {rows, ld_rows * 2, 0}, {wp, ldw * 2, 0}, T, vc, N, p.d_bn, 1, 1, 1, status, stream);
+        });
+        if (st != NQ_OK) return st;
         if (dw) {
             MmParams<RowsEpilogue<OUT>> P = {};
             P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
             P.s.live = live;
             P.s.live_k = 1;
-            const int st = mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
+            st = mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
             if (st != NQ_OK) return st;
         }
         if (dh && p.h_direct) {
@@ -648,7 +663,7 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
             MmParams<SumEpilogue> P = {};
             P.e = {reinterpret_cast<float4*>(scratch + at.sums), p.h_blocks, p.h_quads, v0 > 0};
             P.s.live = live;
-            const int st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 1, 1, status, stream);
+            st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 1, 1, status, stream);
             if (st != NQ_OK) return st;
             if (v0 == 0) splits = P.s.splits;                  // (the last piece may be shorter and have fewer)
         }

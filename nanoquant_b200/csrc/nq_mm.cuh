@@ -428,13 +428,17 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kMmThreads, 1) mm_k
                 if (!ok) break;
                 epi.begin(row, n0, set, T.n, T.split);
 #pragma unroll
-                for (int j = 0; j < kMmAccCols / 64; ++j) {
-                    const int c = 64 * set + 64 * (j & ~1) + 32 * (j & 1);
+                for (int j = 0; j < kMmAccCols / 64; j += 2) {
+                    const int c = 64 * set + 64 * j;
                     if (c < live && some) {
-                        uint32_t r[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sum[j][i]);
-                        epi.chunk(r, c, min(32, live - c), stage, j & 1);
+                        for (int half = 0; half < 2; ++half) {
+                            uint32_t r[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sum[j + half][i]);
+                            if (half == 0 || c + 32 < live) epi.chunk(r, c + 32 * half, min(32, live - c - 32 * half), stage, half);
+                        }
+                        epi.flush(c, min(64, live - c), stage);
                     }
                 }
             } else {
