@@ -27,8 +27,9 @@ constexpr int kLossPieceUnit = 256;
 // Steps of 64 products after which a sum leaves the tensor cores, which cut it off towards zero with every instruction (nq_mm.cuh).  Logits: the same in both
 // passes, so that the backward's are the numbers that lse came from.  (With whole sums there, p - 1 of a target with p = 0.999 was off by 6 to 19 % at 4096 columns and
 // by up to 38 % at 8192.)  Forward level with whole sums, with 256 columns 5 % slower; the backward's logits and d 9 to 15 % slower, 2 to 6 % of the pass: a tile's
-// outputs all come at its end.
-constexpr int kLossLogitsChunk = 8;
+// outputs all come at its end.  Sums over tokens and words: of 2048 products, whose error of 1.2e-5 at most is far below the outputs' rounding and does not grow
+// with their number (65536 tokens: 4.2e-4 of a whole sum); level with whole sums, with 512 9 % slower.
+constexpr int kLossLogitsChunk = 8, kLossSumsChunk = 32;
 constexpr int kLossRows = 16384;           // tokens of a forward product: the scratch holds 8 bytes for each and every 64 to 128 words
 constexpr int kLossJoinHere = 8192;        // pieces of all tokens that one CTA joins
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -392,10 +393,10 @@ struct GradEpilogue {
 };
 
 // dw of a piece (or dh): rows of words, times the final scale.
-template <int OUT>
+template <int OUT, bool LONG>
 struct RowsEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
-    static constexpr int kChunk = 0;
+    static constexpr int kChunk = LONG ? kLossSumsChunk : 0;
     struct Params {
         const float* final_scale;
         uint16_t* out;
@@ -423,9 +424,10 @@ struct RowsEpilogue {
 };
 
 // Partial sums of dh in fp32: [split][128 rows][4 columns][row], so that a warp's stores are whole lines.
+template <bool LONG>
 struct SumEpilogue {
     static constexpr bool kS8 = false, kBuildA = false;
-    static constexpr int kChunk = 0;
+    static constexpr int kChunk = LONG ? kLossSumsChunk : 0;
     struct Params {
         float4* sums;
         int blocks, quads;         // of 128 rows; of 4 columns, padded to whole tiles
@@ -615,7 +617,7 @@ static int launch_lse(const void* h, const void* packed, const int* live, const 
 }
 
 // `run` with the kernels that add a sum of k products up by chunks of `steps`, or, where one chunk is all of it, with those that keep no sums in registers and
-// write outputs as they are loaded.
+// write outputs as they are loaded (logits and dw of one token, 151936 x 4096, 490 us instead of 600).
 template <class Run>
 static int by_length(int64_t k, int steps, Run run) {
     return k > 64 * steps ? run(std::true_type()) : run(std::false_type());
@@ -647,25 +649,33 @@ static int launch_backward(const void* h, const void* w, const LossTargets& targ
         });
         if (st != NQ_OK) return st;
         if (dw) {
-            MmParams<RowsEpilogue<OUT>> P = {};
-            P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
-            P.s.live = live;
-            P.s.live_k = 1;
-            st = mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
+            st = by_length(T, kLossSumsChunk, [&](auto is_long) {
+                MmParams<RowsEpilogue<OUT, is_long>> P = {};
+                P.e = {final_scale, static_cast<uint16_t*>(dw) + v0 * lddw, lddw};
+                P.s.live = live;
+                P.s.live_k = 1;
+                return mm_launch<2>(P, type, {d, p.piece * 2, 1, up(vc, 64)}, {scratch + at.h, (int64_t)N * 2, 1}, vc, N, T, p.w_bn, 1, 0, dh || v0 + p.piece < V, status, stream);
+            });
             if (st != NQ_OK) return st;
         }
-        if (dh && p.h_direct) {
-            MmParams<RowsEpilogue<OUT>> P = {};
-            P.e = {final_scale, static_cast<uint16_t*>(dh), lddh};
-            return mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, 1, 1, 0, status, stream);
-        }
+        if (dh && p.h_direct)
+            return by_length(vc, kLossSumsChunk, [&](auto is_long) {
+                MmParams<RowsEpilogue<OUT, is_long>> P = {};
+                P.e = {final_scale, static_cast<uint16_t*>(dh), lddh};
+                return mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, 1, 1, 0, status, stream);
+            });
         if (dh) {
-            MmParams<SumEpilogue> P = {};
-            P.e = {reinterpret_cast<float4*>(scratch + at.sums), p.h_blocks, p.h_quads, v0 > 0};
-            P.s.live = live;
-            st = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 1, 1, status, stream);
+            int made = 0;
+            st = by_length((vc + splits - 1) / splits, kLossSumsChunk, [&](auto is_long) {
+                MmParams<SumEpilogue<is_long>> P = {};
+                P.e = {reinterpret_cast<float4*>(scratch + at.sums), p.h_blocks, p.h_quads, v0 > 0};
+                P.s.live = live;
+                const int r = mm_launch<CG>(P, type, {d, p.piece * 2, 0}, {wp, ldw * 2, 1}, T, N, vc, p.h_bn, splits, 1, 1, status, stream);
+                made = P.s.splits;
+                return r;
+            });
             if (st != NQ_OK) return st;
-            if (v0 == 0) splits = P.s.splits;                  // (the last piece may be shorter and have fewer)
+            if (v0 == 0) splits = made;                        // (the last piece may be shorter and have fewer)
         }
     }
     if (dh) {
