@@ -595,6 +595,12 @@ void check_capture(int dev, std::initializer_list<const Tensor*> inputs) {
     }
 }
 
+// A call that forward-mode differentiation follows: an output without a tangent would say that the tangent is zero.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        if (t) TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 struct NormArgs {
     int64_t rows, N;
     double eps;
@@ -676,6 +682,7 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double eps = PyFloat_AsDouble(a[3]);
     const int center = PyObject_IsTrue(a[4]);
     if (PyErr_Occurred()) return nullptr;
+    refuse_tangents(center ? "layer_norm" : "rms_norm", {x, w, b});
     Tensor y;
     if (at::GradMode::is_enabled() && (x->requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad()))) {
         check_capture(x->get_device(), {x, w, b});
@@ -834,6 +841,7 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if ((reinterpret_cast<uintptr_t>(m->const_data_ptr()) & 15) || row_stride(*m) % 8 != 0 || row_stride(*m) < m->size(1)) Py_RETURN_NONE;
     const int64_t ignore = PyLong_AsLongLong(a[3]), reduction = PyLong_AsLongLong(a[4]);
     if (PyErr_Occurred()) return nullptr;
+    refuse_tangents("linear_cross_entropy", {h, w});
     Tensor loss;
     if (at::GradMode::is_enabled() && (h->requires_grad() || w->requires_grad())) {
         check_capture(h->get_device(), {h, w});
