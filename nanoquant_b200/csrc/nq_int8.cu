@@ -73,6 +73,7 @@ __device__ __forceinline__ uint2 q8_pack(const uint4& u, const Q8Row& q) {
 template <bool BF16>
 __device__ __forceinline__ int8_t q8_one(uint16_t x, const Q8Row& q) { return q.live ? (int8_t)q8_exact(io_float(x, BF16), q.top) : (int8_t)0; }
 
+// (As in all kernels here, nothing is read by the non-coherent path: the kernel that writes the activations may have released this one early.)
 // A row per CTA.  PACKS > 0: 16-byte loads, PACKS of eight values a thread, kept in registers; 0: single values at any address, read twice.
 template <bool BF16, int PACKS>
 __global__ void __launch_bounds__(512) quantize_rows_kernel(const uint16_t* x, int8_t* q, float* scale, int N, long long ldx, long long ldq, int release) {
@@ -90,13 +91,13 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const uint16_t* x, i
 #pragma unroll
         for (int p = 0; p < PACKS; ++p) {
             const int c = (p * (int)blockDim.x + tid) * 8;
-            v[p] = c < N ? __ldg(reinterpret_cast<const uint4*>(xr + c)) : make_uint4(0u, 0u, 0u, 0u);
+            v[p] = c < N ? __ldcg(reinterpret_cast<const uint4*>(xr + c)) : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
         for (int p = 0; p < PACKS; ++p) top = q8_top(v[p], top);
     } else {
 #pragma unroll 4
-        for (int c = tid; c < N; c += blockDim.x) top = max(top, (uint32_t)(__ldg(xr + c) & 0x7fff));
+        for (int c = tid; c < N; c += blockDim.x) top = max(top, (uint32_t)(__ldca(xr + c) & 0x7fff));
     }
     top = warp_top(top);
     if (lane == 0) red[warp] = top;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const uint16_t* x, i
         }
     } else {
 #pragma unroll 4
-        for (int c = tid; c < N; c += blockDim.x) qr[c] = q8_one<BF16>(__ldg(xr + c), by);
+        for (int c = tid; c < N; c += blockDim.x) qr[c] = q8_one<BF16>(__ldca(xr + c), by);
     }
 }
 template <int PACKS>
@@ -170,10 +171,10 @@ struct Int8Epilogue {
             uint32_t top = 0;
             if (p.vec) {
 #pragma unroll 8
-                for (int c = (part * 32 + lane) * 8; c < p.N; c += share * 256) top = q8_top(__ldg(reinterpret_cast<const uint4*>(x + c)), top);
+                for (int c = (part * 32 + lane) * 8; c < p.N; c += share * 256) top = q8_top(__ldca(reinterpret_cast<const uint4*>(x + c)), top);
             } else {
 #pragma unroll 8
-                for (int c = part * 32 + lane; c < p.N; c += share * 32) top = max(top, (uint32_t)(__ldg(x + c) & 0x7fff));
+                for (int c = part * 32 + lane; c < p.N; c += share * 32) top = max(top, (uint32_t)(__ldca(x + c) & 0x7fff));
             }
             top = warp_top(top);
             if (lane == 0) tops[warp] = top;
@@ -187,9 +188,9 @@ struct Int8Epilogue {
             if (p.vec) {
 #pragma unroll 8
                 for (int c = (part * 32 + lane) * 8; c < p.N; c += share * 256)
-                    *reinterpret_cast<uint2*>(at(c)) = q8_pack<BF16>(__ldg(reinterpret_cast<const uint4*>(x + c)), by);
+                    *reinterpret_cast<uint2*>(at(c)) = q8_pack<BF16>(__ldca(reinterpret_cast<const uint4*>(x + c)), by);
             } else {
-                for (int c = part * 32 + lane; c < p.N; c += share * 32) *at(c) = (unsigned char)q8_one<BF16>(__ldg(x + c), by);
+                for (int c = part * 32 + lane; c < p.N; c += share * 32) *at(c) = (unsigned char)q8_one<BF16>(__ldca(x + c), by);
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kMmEpilogueWarps) : "memory");      // (the scales)
@@ -212,18 +213,18 @@ struct Int8Epilogue {
         for (int i = 0; i < 32; i += 4) {
             float f[4];
             if (i + 4 <= cols) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(ws + i));
+                const float4 v = __ldca(reinterpret_cast<const float4*>(ws + i));
                 f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
             } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = i + k < cols ? __ldg(ws + i + k) : 0.f;
+                for (int k = 0; k < 4; ++k) f[k] = i + k < cols ? __ldca(ws + i + k) : 0.f;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) f[k] = (float)(int)r[i + k] * f[k] * sx;      // (s_x s_w may leave fp32 where the result does not)
             if (p.bias) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (i + k < cols) f[k] += io_float(__ldg(p.bias + n0 + c + i + k), OUT != kOutFp16);
+                    if (i + k < cols) f[k] += io_float(__ldca(p.bias + n0 + c + i + k), OUT != kOutFp16);
             }
             w[i / 2] = pack_outputs<OUT>(f[0], f[1], 0);
             w[i / 2 + 1] = pack_outputs<OUT>(f[2], f[3], 0);

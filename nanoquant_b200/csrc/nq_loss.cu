@@ -46,8 +46,9 @@ struct LossTargets {
     int wide;            // int64, not int32
     long long ignore;
 };
+// (through L2, as h: whatever wrote them may have released this kernel early, which the non-coherent path does not allow)
 __device__ __forceinline__ long long loss_target(const LossTargets& t, int row) {
-    return t.wide ? __ldg(static_cast<const long long*>(t.p) + row) : (long long)__ldg(static_cast<const int*>(t.p) + row);
+    return t.wide ? __ldcg(static_cast<const long long*>(t.p) + row) : (long long)__ldcg(static_cast<const int*>(t.p) + row);
 }
 
 // ---------------------------------------------------------------------------
@@ -114,7 +115,7 @@ __device__ __forceinline__ void loss_copy_rows(const LossRows& R, int first, int
     const int zeros = (max(n, 1) + 63) & ~63;
     for (int i = tid; i < count * R.packs; i += 512) {
         const int k = i / R.packs, c = i - k * R.packs, t = first + k, row = rows[k];
-        if (row >= 0) R.out[(long long)row * R.packs + c] = __ldg(R.h + t * R.ldh + c);
+        if (row >= 0) R.out[(long long)row * R.packs + c] = __ldcg(R.h + t * R.ldh + c);
         if (R.pos ? t >= n && t < zeros : row < 0) R.out[(long long)t * R.packs + c] = make_uint4(0, 0, 0, 0);
     }
 }

@@ -49,16 +49,17 @@ __device__ __forceinline__ uint32_t norm_pack(float a, float b) {
     }
     return r;
 }
-// VEC consecutive elements (one 16-byte load, or a single element) as they are, and as floats.
+// VEC consecutive elements (one 16-byte load, or a single element) as they are, and as floats.  Nothing here is read by the non-coherent path: these kernels
+// may be on their SMs while a kernel that released them early still writes.  Rows come through L2, weights, which all rows read, through L1.
 template <int VEC> struct NormVec { uint32_t w[VEC / 2]; };
 template <> struct NormVec<1> { uint16_t h; };
 template <int VEC>
 __device__ __forceinline__ NormVec<VEC> norm_load(const void* p, long long i, bool live) {
     NormVec<VEC> v = {};
     if (live) {
-        if constexpr (VEC == 1) v.h = __ldg(static_cast<const uint16_t*>(p) + i);
+        if constexpr (VEC == 1) v.h = __ldcg(static_cast<const unsigned short*>(p) + i);
         else {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
             v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
         }
     }
@@ -80,15 +81,20 @@ template <int VEC, bool BF16>
 __device__ __forceinline__ void norm_weights(const void* p, int w32, int c, float (&f)[VEC]) {
     if (w32) {
         const float* q = static_cast<const float*>(p) + c;
-        if constexpr (VEC == 1) f[0] = __ldg(q);
+        if constexpr (VEC == 1) f[0] = *q;
         else {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(q)), b = __ldg(reinterpret_cast<const float4*>(q) + 1);
+            const float4 a = reinterpret_cast<const float4*>(q)[0], b = reinterpret_cast<const float4*>(q)[1];
             f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
         }
     } else {
-        const NormVec<VEC> v = norm_load<VEC>(p, c, true);
+        const uint16_t* q = static_cast<const uint16_t*>(p) + c;
+        if constexpr (VEC == 1) f[0] = norm_float<BF16>(*q);
+        else {
+            const uint4 u = *reinterpret_cast<const uint4*>(q);
+            const NormVec<VEC> v = {{u.x, u.y, u.z, u.w}};
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = norm_at<VEC, BF16>(v, e);
+            for (int e = 0; e < VEC; ++e) f[e] = norm_at<VEC, BF16>(v, e);
+        }
     }
 }
 __device__ __forceinline__ float2 warp_sum2(float2 v) {
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(32 * WARPS * norm_rows_per_cta<WARPS>()) norm_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (long long row = (long long)blockIdx.x * RPC + sub; row < P.rows; row += (long long)gridDim.x * RPC) {
         NormVec<VEC> x[PACKS], dy[PACKS];
-        const float2 st = __ldg(P.stats + row);
+        const float2 st = __ldcg(P.stats + row);
 #pragma unroll
         for (int p = 0; p < PACKS; ++p) {
             const int c = (p * G + tid) * VEC;
@@ -590,7 +596,7 @@ __global__ void __launch_bounds__(NormShape<PITCH, true>::kThreads, NormShape<PI
     };
     // mean and 1 / sigma of row `lane` of a batch
     auto load_stats = [&](long long batch) {
-        return lane < ROWS && batch * ROWS + lane < P.rows ? __ldg(P.stats + batch * ROWS + lane) : make_float2(0.f, 0.f);
+        return lane < ROWS && batch * ROWS + lane < P.rows ? __ldcg(P.stats + batch * ROWS + lane) : make_float2(0.f, 0.f);
     };
     f32x2 aw[PACKS][4], ab[PACKS][4], w[PACKS][4];
 #pragma unroll
@@ -728,7 +734,7 @@ template <bool BF16>
 __device__ __forceinline__ f32x2 ragged_pair(uint32_t a, uint32_t b) { return pair2(norm_float<BF16>(ragged_shared(a)), norm_float<BF16>(ragged_shared(b))); }
 template <bool BF16>
 __device__ __forceinline__ float ragged_weight(const void* p, int w32, int c) {
-    return w32 ? __ldg(static_cast<const float*>(p) + c) : norm_float<BF16>(__ldg(static_cast<const uint16_t*>(p) + c));
+    return w32 ? static_cast<const float*>(p)[c] : norm_float<BF16>(static_cast<const uint16_t*>(p)[c]);
 }
 
 // COLS columns a thread; dead ones (beyond N) read the row's first element and count for nothing.
@@ -854,7 +860,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ragged_kernel(const NormParam
     int stage = 0;
     for (long long batch = first; batch < batches; batch += step) {
         const int rows = (int)min((long long)ROWS, P.rows - batch * ROWS);
-        const float2 st = lane < rows ? __ldg(P.stats + batch * ROWS + lane) : make_float2(0.f, 0.f);
+        const float2 st = lane < rows ? __ldcg(P.stats + batch * ROWS + lane) : make_float2(0.f, 0.f);
         const float rstd = st.y, shift = -st.x;
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         g.sync();                          // this batch is there for all, and all have left the one before
@@ -1068,7 +1074,7 @@ int launch_norm(const NormVariant& v, long long ctas, const NormParams& P, cudaS
     return launch_dependent(cfg, attr, 0, (const void*)v.fn, args);
 }
 bool norm_rows_aligned(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
-// Direct kernels for few rows, and for short rows at any address (8192 x 1003 of layer norm, us: forward 18.0 and 21.1 ragged, backward 27.2 and 37.4;
+// Direct kernels for few rows, and for short rows at any address (8192 x 1003 of layer norm, us: forward 14.2 and 21.1 ragged, backward 24.8 and 37.4;
 // 8000 x 5001: 147 and 107, 322 and 119).
 bool norm_streamed(bool vec, int64_t rows, int64_t N) { return rows > 2 * sm_count() && (vec || N > 1024); }
 
