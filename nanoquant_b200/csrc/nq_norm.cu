@@ -15,6 +15,8 @@
 //
 // Backward: a thread adds dy xhat and dy of its columns to fp32 sums in registers.  One row of partial sums per CTA goes to the scratch; a
 // second kernel adds these in a fixed order, so results do not depend on timing.
+#include <atomic>
+
 #include "nq_common.cuh"
 
 namespace nq {
@@ -998,12 +1000,19 @@ NormVariant choose_norm(bool bwd, bool bf16, bool center, bool vec, long long ro
 // How a stream kernel is launched.
 struct NormStream {
     const void* fn;
+    std::atomic<unsigned long long>* ready;      // devices on which the kernel may use kNormSmemMost
     int threads, smem, G, rows, pitch;
     int64_t ctas;
 };
+// Shared memory of any of them at most.  A kernel's limit is set once per device and to this, not to a call's own size: it belongs to the process, and a
+// smaller call in another thread would lower it between a call's setting and its launch.
+constexpr int kNormSmemMost = 160 * 1024;
 template <int PITCH>
 NormStream norm_stream(bool bwd, bool bf16, bool center, int N) {
+    static std::atomic<unsigned long long> ready[8];
+    static_assert(NormShape<PITCH, true>::kGroupBytes * (PITCH <= 4096 ? 4096 / PITCH : 1) <= kNormSmemMost, "shared memory");
     NormStream v = {};
+    v.ready = &ready[4 * bwd + 2 * bf16 + center];
     if (bwd) v.fn = bf16 ? (center ? (const void*)norm_bwd_stream_kernel<PITCH, true, true> : (const void*)norm_bwd_stream_kernel<PITCH, true, false>)
                          : (center ? (const void*)norm_bwd_stream_kernel<PITCH, false, true> : (const void*)norm_bwd_stream_kernel<PITCH, false, false>);
     else v.fn = bf16 ? (center ? (const void*)norm_fwd_stream_kernel<PITCH, true, true> : (const void*)norm_fwd_stream_kernel<PITCH, true, false>)
@@ -1018,7 +1027,9 @@ NormStream norm_stream(bool bwd, bool bf16, bool center, int N) {
 }
 template <int COLS, int ROWS>
 NormStream norm_ragged(bool bwd, bool bf16, bool center, int N) {
+    static std::atomic<unsigned long long> ready[8];
     NormStream v = {};
+    v.ready = &ready[4 * bwd + 2 * bf16 + center];
     if (bwd) v.fn = bf16 ? (center ? (const void*)norm_bwd_ragged_kernel<COLS, ROWS, true, true> : (const void*)norm_bwd_ragged_kernel<COLS, ROWS, true, false>)
                          : (center ? (const void*)norm_bwd_ragged_kernel<COLS, ROWS, false, true> : (const void*)norm_bwd_ragged_kernel<COLS, ROWS, false, false>);
     else v.fn = bf16 ? (center ? (const void*)norm_fwd_ragged_kernel<COLS, ROWS, true, true> : (const void*)norm_fwd_ragged_kernel<COLS, ROWS, true, false>)
@@ -1042,8 +1053,13 @@ int choose_stream(bool bwd, bool bf16, bool center, bool vec, const NormParams& 
         : N <= 5120 ? norm_stream<10240>(bwd, bf16, center, N)
         : N <= 8192 ? norm_stream<16384>(bwd, bf16, center, N)
                     : norm_stream<32768>(bwd, bf16, center, N);
-    NQ_CUDA_TRY(cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem));
-    int per_sm = 1;
+    int dev = 0, per_sm = 1;
+    NQ_CUDA_TRY(cudaGetDevice(&dev));
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(*v.ready & bit)) {
+        NQ_CUDA_TRY(cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmemMost));
+        *v.ready |= bit;
+    }
     NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.fn, v.threads, v.smem));
     const int most = bwd ? norm_ctas_per_sm(N) : 8;
     per_sm = per_sm < 1 ? 1 : per_sm > most ? most : per_sm;

@@ -1,8 +1,51 @@
-"""Calls behind the last decoder layer next to other calls: kernels that release the next one early."""
+"""Calls behind the last decoder layer next to other calls: host threads, kernels that release the next one early."""
+import threading
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("cols,other", [((4001, 4001), (1100, 1300)), ((4096, 2056), (256, 520))])
+def test_norms_of_different_widths_in_two_threads(cols, other):
+    """Both threads use the same kernels with other sizes of shared memory."""
+    from nanoquant_b200 import _lib
+
+    L = _lib.lib()
+    rows = 400
+    errors, gate = [], threading.Barrier(2)
+
+    def work(widths, seed):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            sets = []
+            for n in widths:
+                x = torch.randn((rows, n), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").bfloat16()
+                sets.append((n, x, torch.empty_like(x), torch.empty((rows, 2), device="cuda"), torch.empty_like(x)))
+        torch.cuda.synchronize()
+        gate.wait()
+        for i in range(4000):
+            n, x, y, stats, dx = sets[i % 2]
+            st = L.nq_norm_fwd(x.data_ptr(), None, None, y.data_ptr(), stats.data_ptr(), rows, n, n, n, 1e-5, 1, _lib.NQ_BF16, _lib.NQ_BF16, stream.cuda_stream)
+            st2 = L.nq_norm_bwd(y.data_ptr(), x.data_ptr(), None, stats.data_ptr(), dx.data_ptr(), None, None, None, 0, rows, n, n, n, n, 1, _lib.NQ_BF16, _lib.NQ_BF16,
+                                stream.cuda_stream)
+            if st or st2:
+                errors.append((n, st, st2, L.nq_last_cuda_error()))
+                return
+        stream.synchronize()
+        for n, x, y, _, _ in sets:
+            d = x.double()
+            want = (d - d.mean(1, keepdim=True)) / (d.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+            if not ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -17).all():
+                errors.append((n, "values"))
+
+    threads = [threading.Thread(target=work, args=a) for a in ((cols, 1), (other, 2))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors[:2]
 
 
 @pytest.mark.parametrize("T", [1, 6, 40, 600])
