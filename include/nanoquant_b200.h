@@ -33,7 +33,7 @@ typedef enum {
     NQ_ERR_NULL = -1,        /* a required pointer is NULL */
     NQ_ERR_SHAPE = -2,       /* a dimension is <= 0 or violates a divisibility rule */
     NQ_ERR_DTYPE = -3,       /* dtype is not NQ_F16 / NQ_BF16, or method id unknown */
-    NQ_ERR_ALIGN = -4,       /* a pointer is not aligned as required (16 bytes) */
+    NQ_ERR_ALIGN = -4,       /* a pointer is not aligned as required (16 bytes, where nothing else is said; always to its elements) */
     NQ_ERR_SCRATCH = -5,     /* scratch / workspace buffer too small */
     NQ_ERR_CUDA = -6,        /* a CUDA runtime call failed; see nq_last_cuda_error() */
     NQ_ERR_TIMEOUT = -7,     /* a bounded device-side wait gave up (read from a status word) */
@@ -356,7 +356,8 @@ int nq_dense_gemv_fwd(const void* x, const void* w, const void* bias, void* y, i
  *     y = (x - m) r * weight + bias,   m = mean(x) (0 for RMS),   r = 1 / sqrt(mean((x - m)^2) + eps)
  * weight and bias [N] (bias with center only) are nullable and of `weight_dtype`: the activations' dtype or NQ_F32.  `stats` (nullable) receives
  * (m, r) of every row, 2 * rows floats, which the backward pass reads.  fp32 arithmetic, one rounding of y.
- * Any alignment; 16-byte loads where N, ldx and ldy are multiples of 8 and the pointers 16-byte aligned.
+ * Rows and weights at any address of their type, stats at a multiple of 8 bytes; 16-byte loads where N, ldx and ldy are multiples of 8 and the pointers
+ * 16-byte aligned.
  * No counterpart in the reference (its models' norms are torch's). */
 int nq_norm_max_columns(void);
 int nq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t rows, int64_t N,

@@ -30,6 +30,9 @@ inline int check_cuda(cudaError_t e, const char* where) {
 #define NQ_LAUNCH_CHECK() NQ_CUDA_TRY(cudaGetLastError())
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Addresses that elements of `bytes` (a power of two) can have, each null or a multiple of it.
+template <class... P>
+inline bool aligned_to(unsigned bytes, const P*... p) { return (((reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0) && ...); }
 
 inline cudaStream_t as_stream(nq_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 

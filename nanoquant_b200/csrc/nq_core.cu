@@ -57,7 +57,7 @@ const char* nq_strerror(int status) {
         case NQ_ERR_NULL: return "a required pointer is NULL";
         case NQ_ERR_SHAPE: return "invalid shape (non-positive or not a required multiple)";
         case NQ_ERR_DTYPE: return "unsupported dtype or layout id";
-        case NQ_ERR_ALIGN: return "pointer not 16-byte aligned";
+        case NQ_ERR_ALIGN: return "pointer not aligned as the entry point asks";
         case NQ_ERR_SCRATCH: return "scratch or workspace buffer too small";
         case NQ_ERR_CUDA: return "CUDA runtime error (see nq_last_cuda_error)";
         case NQ_ERR_TIMEOUT: return "a bounded device-side wait gave up";

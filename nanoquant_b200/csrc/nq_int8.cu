@@ -284,6 +284,7 @@ int nq_quantize_rows_s8(const void* x, int8_t* q, float* scale, int64_t rows, in
     if (dtype != NQ_F16 && dtype != NQ_BF16) return NQ_ERR_DTYPE;
     if (rows < 1 || N < 1 || ldx < 0 || ldq < N) return NQ_ERR_SHAPE;
     if (rows > 0x7fffffff || N > 0x7fffffff) return NQ_ERR_TOO_LARGE;
+    if (!aligned_to(2, x) || !aligned_to(4, scale)) return NQ_ERR_ALIGN;
     return launch_quantize(x, q, scale, rows, N, ldx, ldq, dtype == NQ_BF16, 0, as_stream(stream));
 }
 
@@ -299,7 +300,7 @@ int nq_int8_linear_fwd(const void* x, const int8_t* w, const float* w_scale, con
     if (dtype != NQ_F16 && dtype != NQ_BF16) return NQ_ERR_DTYPE;
     if (T < 1 || N < 1 || V < 1 || ldx < 0 || ldw < N || ldw % 16 || ldy < V) return NQ_ERR_SHAPE;
     if (N > kInt8MaxCols || T > 0x1fffffff || V > 0x1fffffff) return NQ_ERR_TOO_LARGE;
-    if (!aligned16(w) || !aligned16(w_scale) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
+    if (!aligned16(w) || !aligned16(w_scale) || !aligned16(scratch) || !aligned16(status_word) || !aligned_to(2, x, bias, y)) return NQ_ERR_ALIGN;
     const size_t need = nq_int8_linear_scratch_bytes(T, N);
     if (need && !scratch) return NQ_ERR_NULL;
     if (scratch_bytes < need) return NQ_ERR_SCRATCH;

@@ -708,6 +708,7 @@ int nq_linear_ce_fwd(const void* h, const void* w, const void* targets, int targ
     int st = check_loss(T, N, V, ldh, ldw, dtype, reduction, target_bits);
     if (st != NQ_OK) return st;
     if (!aligned16(h) || !aligned16(w) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
+    if (!aligned_to(target_bits / 8, targets) || !aligned_to(4, loss, lse, count)) return NQ_ERR_ALIGN;
     const LossFwdScratch at = loss_fwd_scratch(T, N, V);
     if (scratch_bytes < (size_t)at.bytes) return NQ_ERR_SCRATCH;
     cudaStream_t s = as_stream(stream);
@@ -771,6 +772,7 @@ int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int targ
     if (st != NQ_OK) return st;
     if ((dh && (lddh < N || lddh % 8)) || (dw && (lddw < N || lddw % 8))) return NQ_ERR_SHAPE;
     if (!aligned16(h) || !aligned16(w) || !aligned16(dh) || !aligned16(dw) || !aligned16(scratch) || !aligned16(status_word)) return NQ_ERR_ALIGN;
+    if (!aligned_to(target_bits / 8, targets) || !aligned_to(4, lse, count, grad_loss)) return NQ_ERR_ALIGN;
     const LossPlan p = plan_loss(T, N, V);
     const bool packs = loss_packs(T, N, V);
     const LossScratch at = loss_scratch(p, T, N, packs);

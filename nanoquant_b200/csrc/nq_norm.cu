@@ -1110,6 +1110,7 @@ int nq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, fl
     if (rows < 1 || N < 1 || ldx < 0 || ldy < N) return NQ_ERR_SHAPE;
     if (N > kNormMaxCols || rows > 0x7fffffff) return NQ_ERR_TOO_LARGE;
     if (bias && !center) return NQ_ERR_UNSUPPORTED;
+    if (!aligned_to(2, x, y) || !aligned_to(weight_dtype == NQ_F32 ? 4 : 2, weight, bias) || !aligned_to(8, stats)) return NQ_ERR_ALIGN;
     NormParams P = {};
     P.x = x; P.w = weight; P.b = bias; P.y = y; P.stats = reinterpret_cast<float2*>(stats);
     P.rows = rows; P.ldx = ldx; P.ldy = ldy; P.N = (int)N; P.w32 = weight_dtype == NQ_F32;
@@ -1139,6 +1140,7 @@ int nq_norm_bwd(const void* dy, const void* x, const void* weight, const float* 
     if (rows < 1 || N < 1 || ldx < 0 || lddy < 0 || (dx && lddx < N)) return NQ_ERR_SHAPE;
     if (N > kNormMaxCols || rows > 0x7fffffff) return NQ_ERR_TOO_LARGE;
     if (dbias && !center) return NQ_ERR_UNSUPPORTED;
+    if (!aligned_to(2, dy, x, dx) || !aligned_to(weight_dtype == NQ_F32 ? 4 : 2, weight, dweight, dbias) || !aligned_to(8, stats)) return NQ_ERR_ALIGN;
     if (!dx && !dweight && !dbias) return NQ_OK;
     const bool sums = dweight || dbias;
     if (sums && !scratch) return NQ_ERR_NULL;
