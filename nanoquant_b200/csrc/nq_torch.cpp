@@ -56,6 +56,7 @@ PyObject* g_raise_status = nullptr;    // (status, what): raises
 PyObject* g_grow_scratch = nullptr;    // (device index, bytes): makes the scratch hold that many bytes, or raises
 PyObject* g_dyn_general = nullptr;     // Python implementations of the operators (reference operand layouts)
 PyObject* g_marlin_general = nullptr;
+PyObject* g_thread_scratch = nullptr;  // () -> the tensor that this thread runs on instead of the device's scratch
 
 // What module_call compares with: NanoQuantLinear and its forward, nn.Module and its way from a call to forward, the hooks on every module.
 struct ModuleClass {
@@ -549,6 +550,20 @@ Tensor dense_rows(const Tensor& t) {
     return as_rows(u, rows, ld) ? u : u.contiguous();
 }
 nq_stream_t stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+// A backward pass runs on a thread of autograd's: it keeps the scratch that the forward call's thread ran on, alive too, and runs on it.
+Tensor thread_scratch() {
+    if (!t_override.ptr) return Tensor();
+    pybind11::gil_scoped_acquire gil;
+    THPObjectPtr r(call_python(g_thread_scratch, PyTuple_New(0)));
+    return THPVariable_Check(r.get()) ? THPVariable_Unpack(r.get()) : Tensor();
+}
+struct OnScratch {
+    explicit OnScratch(const Tensor& t) : before(t_override) {
+        t_override = t.defined() ? Scratch{t.data_ptr(), (size_t)t.numel()} : Scratch{};
+    }
+    ~OnScratch() { t_override = before; }
+    Scratch before;
+};
 // The header of the device's scratch, whose status word an expired wait sets.
 void* status_header(int dev) {
     Scratch s = scratch_of(dev);
@@ -793,6 +808,7 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
         Tensor lse, count;
         Tensor loss = loss_launch(h, w, targets, LossArgs{ignore, (int)reduction}, lse, count);
         ctx->save_for_backward({h, w, targets, lse, count});
+        if (const Tensor own = thread_scratch(); own.defined()) ctx->saved_data["scratch"] = own;
         ctx->saved_data["ignore"] = ignore;
         ctx->saved_data["reduction"] = reduction;
         return loss;
@@ -811,6 +827,8 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
                 const Tensor g = grads[0].resolve_neg();
                 const int dev = h.get_device();
                 OnDevice on(dev);
+                const auto own = ctx->saved_data.find("scratch");
+                const OnScratch on_scratch(own == ctx->saved_data.end() ? Tensor() : own->second.toTensor());
                 void* status = status_header(dev);
                 const size_t bytes = nq_linear_ce_bwd_scratch_bytes(T, N, V);
                 const Tensor scratch = new_bytes((int64_t)bytes, h);
@@ -956,12 +974,12 @@ PyObject* py_set_thread_scratch(PyObject*, PyObject* args) {
     t_override = Scratch{reinterpret_cast<void*>(ptr), (size_t)bytes};
     Py_RETURN_NONE;
 }
-// set_callbacks(raise_status, grow_scratch, dyn_general, marlin_general)
+// set_callbacks(raise_status, grow_scratch, dyn_general, marlin_general, thread_scratch)
 PyObject* py_set_callbacks(PyObject*, PyObject* args) {
-    PyObject* f[4];
-    if (!PyArg_ParseTuple(args, "OOOO", &f[0], &f[1], &f[2], &f[3])) return nullptr;
-    PyObject** slot[4] = {&g_raise_status, &g_grow_scratch, &g_dyn_general, &g_marlin_general};
-    for (int i = 0; i < 4; ++i) {
+    PyObject* f[5];
+    if (!PyArg_ParseTuple(args, "OOOOO", &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
+    PyObject** slot[5] = {&g_raise_status, &g_grow_scratch, &g_dyn_general, &g_marlin_general, &g_thread_scratch};
+    for (int i = 0; i < 5; ++i) {
         Py_INCREF(f[i]);
         Py_XDECREF(*slot[i]);
         *slot[i] = f[i];

@@ -82,7 +82,7 @@ def connect_host_path(ext) -> None:
     """Give the C++ host path (``csrc/nq_torch.cpp``) what it calls back for: errors, scratch growth and the Python
     implementations of the operators."""
     ext.set_callbacks(_lib.check, lambda idx, nbytes: scratch_for(torch.device("cuda", idx), nbytes),
-                      _nanoquant_dyn_forward_cuda, _marlin_nanoquant_forward_cuda)
+                      _nanoquant_dyn_forward_cuda, _marlin_nanoquant_forward_cuda, lambda: getattr(_override, "buf", None))
     from .modules import linear
     ext.set_module_class(*linear.module_class())
     for idx, buf in _scratch.items():
@@ -123,7 +123,8 @@ def scratch_for(device: torch.device, nbytes: int) -> torch.Tensor:
 @contextlib.contextmanager
 def private_scratch(buf: torch.Tensor):
     """Run the enclosed launches of this thread on `buf` (uint8, zeroed once by the caller, 16-byte aligned)
-    instead of the device's shared scratch: for concurrent streams."""
+    instead of the device's shared scratch: for concurrent streams.  The backward pass of a call in here runs on `buf` as well, which the
+    call's graph keeps alive."""
     prev = getattr(_override, "buf", None)
     _set_override(buf)
     try:

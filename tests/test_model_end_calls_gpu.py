@@ -1,4 +1,4 @@
-"""Calls behind the last decoder layer next to other calls: host threads, kernels that release the next one early."""
+"""Calls behind the last decoder layer next to other calls: host threads, scratch of their own, kernels that release the next one early."""
 import threading
 
 import pytest
@@ -46,6 +46,33 @@ def test_norms_of_different_widths_in_two_threads(cols, other):
     for th in threads:
         th.join()
     assert not errors, errors[:2]
+
+
+def test_backward_keeps_the_scratch_of_its_forward():
+    """The backward pass runs on a thread of autograd's; its status word is the one that the forward call was given, also when the caller has left the block."""
+    from nanoquant_b200 import _lib, ops
+
+    dev = torch.cuda.current_device()
+    h = torch.randn((20, 64), device="cuda").bfloat16().requires_grad_()
+    w = torch.randn((100, 64), device="cuda").bfloat16()
+    t = torch.arange(20, device="cuda")
+    want = torch.autograd.grad(ops.linear_cross_entropy(h, w, t), h)[0]
+    shared = ops._scratch.pop(dev)
+    _lib.ext().set_scratch(dev, 0, 0)
+    try:
+        mine = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+        with ops.private_scratch(mine):
+            loss = ops.linear_cross_entropy(h, w, t)
+        address = mine.data_ptr()
+        del mine
+        taken = torch.full((4096,), 7, dtype=torch.uint8, device="cuda")        # (what the allocator hands out next is not the block that the graph still uses)
+        assert taken.data_ptr() != address
+        assert torch.equal(torch.autograd.grad(loss, h)[0], want)
+        assert dev not in ops._scratch                                          # nothing has asked for the shared one
+    finally:
+        ops._scratch[dev] = shared
+        _lib.ext().set_scratch(dev, shared.data_ptr(), shared.numel())
+    assert torch.equal(torch.autograd.grad(ops.linear_cross_entropy(h, w, t), h)[0], want)
 
 
 @pytest.mark.parametrize("T", [1, 6, 40, 600])
