@@ -566,9 +566,10 @@ struct OnScratch {
 };
 // The header of the device's scratch, whose status word an expired wait sets.
 void* status_header(int dev) {
+    constexpr size_t kHeader = 256;
     Scratch s = scratch_of(dev);
-    if (!s.ptr) {
-        grow_scratch(dev, 256);
+    if (!s.ptr || s.bytes < kHeader) {
+        grow_scratch(dev, kHeader);
         s = scratch_of(dev);
     }
     return s.ptr;

@@ -75,6 +75,21 @@ def test_backward_keeps_the_scratch_of_its_forward():
     assert torch.equal(torch.autograd.grad(ops.linear_cross_entropy(h, w, t), h)[0], want)
 
 
+def test_private_scratch_without_room_for_the_header_is_refused():
+    """An expired wait would set a status word behind its end."""
+    from nanoquant_b200 import ops
+
+    h = torch.randn((3, 64), device="cuda").bfloat16()
+    w = torch.randn((100, 64), device="cuda").bfloat16()
+    q, s = ops.quantize_int8(w)
+    with ops.private_scratch(torch.zeros(64, dtype=torch.uint8, device="cuda")):
+        with pytest.raises(RuntimeError, match="too small"):
+            ops.int8_linear_forward(h, q, s)
+        with pytest.raises(RuntimeError, match="too small"):
+            ops.linear_cross_entropy(h, w, torch.arange(3, device="cuda"))
+        assert torch.isfinite(ops.rms_norm(h)).all()        # (needs none)
+
+
 @pytest.mark.parametrize("T", [1, 6, 40, 600])
 def test_behind_kernels_that_release_the_next_one_early(T):
     """A quantised linear starts the kernel behind it before its outputs are written.  The same buffers again and again with other values: each step has to give
