@@ -975,12 +975,13 @@ PyObject* py_set_thread_scratch(PyObject*, PyObject* args) {
     t_override = Scratch{reinterpret_cast<void*>(ptr), (size_t)bytes};
     Py_RETURN_NONE;
 }
-// set_callbacks(raise_status, grow_scratch, dyn_general, marlin_general, thread_scratch)
+// set_callbacks(raise_status, grow_scratch, dyn_general, marlin_general[, thread_scratch])
 PyObject* py_set_callbacks(PyObject*, PyObject* args) {
-    PyObject* f[5];
-    if (!PyArg_ParseTuple(args, "OOOOO", &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
+    PyObject* f[5] = {};
+    if (!PyArg_ParseTuple(args, "OOOO|O", &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
     PyObject** slot[5] = {&g_raise_status, &g_grow_scratch, &g_dyn_general, &g_marlin_general, &g_thread_scratch};
     for (int i = 0; i < 5; ++i) {
+        if (!f[i]) continue;
         Py_INCREF(f[i]);
         Py_XDECREF(*slot[i]);
         *slot[i] = f[i];
