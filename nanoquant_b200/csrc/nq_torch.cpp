@@ -273,7 +273,8 @@ const Tensor* plain(PyObject* o) {
     const Tensor& t = THPVariable_Unpack(o);
     return t.is_cuda() && (t.key_set().raw_repr() & ~kPlainKeys) == 0 ? &t : nullptr;
 }
-bool exact_plain(PyObject* o) { return THPVariable_CheckExact(o) && !c10::impl::dispatch_mode_enabled(); }
+// (what torch.jit.trace records are calls of the dispatcher: a result of any other call is a constant to it)
+bool exact_plain(PyObject* o) { return THPVariable_CheckExact(o) && !c10::impl::dispatch_mode_enabled() && !torch::jit::tracer::isTracing(); }
 
 // (s_in, v_tiles, s_mid | None, u_tiles, s_out, rank, bias | None) from `a[0..6]`; false: not the plain case.
 bool parse_linear(PyObject* const* a, at::ScalarType dt, int64_t N, Linear& l) {
@@ -351,7 +352,7 @@ PyObject* py_module_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!cls.type || Py_TYPE(a[0]) != cls.type || _PyType_Lookup(cls.type, key[5]) != cls.forward ||
         _PyType_Lookup(cls.type, key[12]) != cls.call_impl || _PyType_Lookup(cls.base, key[13]) != cls.call)
         Py_RETURN_NONE;
-    if (!exact_plain(a[1]) || torch::jit::tracer::isTracing()) Py_RETURN_NONE;
+    if (!exact_plain(a[1])) Py_RETURN_NONE;
     // A profiler that records modules knows them by the frame of nn.Module.__call__; a debugger steps into forward.
     const PyThreadState* const thread = PyThreadState_Get();
     if (thread->c_profilefunc || thread->c_tracefunc) Py_RETURN_NONE;
@@ -499,27 +500,31 @@ PyObject* py_group_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+bool dense_gemv_takes(const Tensor& x, const Tensor& w, const Tensor* b) {
+    return is_16bit(x.scalar_type()) && w.scalar_type() == x.scalar_type() && w.dim() == 2 && w.stride(1) == 1 && x.is_contiguous() && x.dim() >= 1 &&
+           x.size(-1) == w.size(1) && x.numel() > 0 && (!b || (b->scalar_type() == x.scalar_type() && b->is_contiguous() && b->numel() == w.size(0)));
+}
+Tensor dense_gemv_launch(const Tensor& x, const Tensor& w, const Tensor* b) {
+    const int64_t V = w.size(0), N = w.size(1), T = x.numel() / N;
+    c10::SmallVector<int64_t, 4> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = V;
+    Tensor y = new_output(shape, x);
+    const int dev = x.get_device();
+    OnDevice on(dev);
+    const int st = nq_dense_gemv_fwd(x.const_data_ptr(), w.const_data_ptr(), b ? b->const_data_ptr() : nullptr,
+                                     y.mutable_data_ptr(), (int)T, (int)N, (int)V, w.stride(0), V, dtype_id(x.scalar_type()),
+                                     c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream());
+    if (st < 0) fail(st, "nq_dense_gemv_fwd");
+    return y;
+}
 // dense_gemv_forward(x, weight, bias | None) -> y or None
 PyObject* py_dense_gemv_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 3, "dense_gemv_forward takes 3 arguments");
     if (!exact_plain(a[0])) Py_RETURN_NONE;
     const Tensor *x = plain(a[0]), *w = plain(a[1]), *b = a[2] == Py_None ? nullptr : plain(a[2]);
-    if (!x || !w || (a[2] != Py_None && !b) || !is_16bit(x->scalar_type()) || w->scalar_type() != x->scalar_type() ||
-        w->dim() != 2 || w->stride(1) != 1 || !x->is_contiguous() || x->dim() < 1 || x->size(-1) != w->size(1) || x->numel() == 0)
-        Py_RETURN_NONE;
-    const int64_t V = w->size(0), N = w->size(1), T = x->numel() / N;
-    if (b && (b->scalar_type() != x->scalar_type() || !b->is_contiguous() || b->numel() != V)) Py_RETURN_NONE;
-    c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
-    shape.back() = V;
-    Tensor y = new_output(shape, *x);
-    const int dev = x->get_device();
-    OnDevice on(dev);
-    const int st = nq_dense_gemv_fwd(x->const_data_ptr(), w->const_data_ptr(), b ? b->const_data_ptr() : nullptr,
-                                     y.mutable_data_ptr(), (int)T, (int)N, (int)V, w->stride(0), V, dtype_id(x->scalar_type()),
-                                     c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream());
-    if (st < 0) fail(st, "nq_dense_gemv_fwd");
-    return THPVariable_Wrap(y);
+    if (!x || !w || (a[2] != Py_None && !b) || !dense_gemv_takes(*x, *w, b)) Py_RETURN_NONE;
+    return THPVariable_Wrap(dense_gemv_launch(*x, *w, b));
     END_HANDLE_TH_ERRORS
 }
 
@@ -618,7 +623,7 @@ void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inpu
 }
 
 struct NormArgs {
-    int64_t rows, N;
+    int64_t N;
     double eps;
     bool center;
 };
@@ -636,10 +641,38 @@ Tensor norm_launch(const Tensor& x, const Tensor* w, const Tensor* b, const Norm
     if (st < 0) fail(st, "nq_norm_fwd");
     return y;
 }
+// (dx, dw, db), undefined where not wanted
+std::array<Tensor, 3> norm_gradients(const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& stats, bool center, std::array<bool, 3> want) {
+    int64_t rows, ldx, dy_rows, lddy;
+    as_rows(x, rows, ldx);
+    const int64_t N = x.size(-1);
+    std::array<Tensor, 3> d;
+    if (want[0]) d[0] = new_output(x.sizes(), x);
+    for (int i = 1; i < 3; ++i)
+        if (want[i]) d[i] = new_output({N}, w, w.scalar_type());
+    if (rows * N == 0) {
+        for (int i = 1; i < 3; ++i)
+            if (want[i]) d[i].zero_();
+        return d;
+    }
+    const Tensor dy = dense_rows(grad);
+    as_rows(dy, dy_rows, lddy);
+    const int dev = x.get_device(), dt = dtype_id(x.scalar_type());
+    OnDevice on(dev);
+    const size_t bytes = nq_norm_bwd_scratch_bytes(rows, N);
+    const Tensor scratch = want[1] || want[2] ? new_bytes((int64_t)bytes, x) : Tensor();
+    auto ptr = [](Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
+    const int st = nq_norm_bwd(dy.const_data_ptr(), x.const_data_ptr(), w.defined() ? w.const_data_ptr() : nullptr,
+                               static_cast<const float*>(stats.const_data_ptr()), ptr(d[0]), ptr(d[1]), ptr(d[2]),
+                               scratch.defined() ? scratch.mutable_data_ptr() : nullptr, scratch.defined() ? bytes : 0, rows, N, lddy, ldx, N,
+                               center, dt, w.defined() && w.scalar_type() == at::kFloat ? (int)NQ_F32 : dt, stream_of(dev));
+    if (st < 0) fail(st, "nq_norm_bwd");
+    return d;
+}
 struct NormFunction : torch::autograd::Function<NormFunction> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t N, double eps, bool center) {
         Tensor stats;
-        const NormArgs a{0, N, eps, center};
+        const NormArgs a{N, eps, center};
         Tensor y = norm_launch(x, w ? &*w : nullptr, b ? &*b : nullptr, a, &stats);
         ctx->save_for_backward({x, w ? *w : Tensor(), stats});
         ctx->saved_data["center"] = center;
@@ -649,38 +682,23 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "the norms are differentiable once");
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
-        const bool center = ctx->saved_data["center"].toBool(), has_b = ctx->saved_data["bias"].toBool();
-        const bool want_x = ctx->needs_input_grad(0), want_w = w.defined() && ctx->needs_input_grad(1), want_b = has_b && ctx->needs_input_grad(2);
-        Tensor dx, dw, db;
-        int64_t rows, ldx, dy_rows, lddy;
-        as_rows(x, rows, ldx);
-        const int64_t N = x.size(-1);
-        if (grads[0].defined()) {
-            if (want_x) dx = new_output(x.sizes(), x);
-            if (want_w) dw = new_output({N}, w, w.scalar_type());
-            if (want_b) db = new_output({N}, w, w.scalar_type());
-            if (rows * N == 0) {
-                if (want_w) dw.zero_();
-                if (want_b) db.zero_();
-            } else {
-                const Tensor dy = dense_rows(grads[0]);
-                as_rows(dy, dy_rows, lddy);
-                const int dev = x.get_device(), dt = dtype_id(x.scalar_type());
-                OnDevice on(dev);
-                const size_t bytes = nq_norm_bwd_scratch_bytes(rows, N);
-                const Tensor scratch = want_w || want_b ? new_bytes((int64_t)bytes, x) : Tensor();
-                auto ptr = [](Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
-                const int st = nq_norm_bwd(dy.const_data_ptr(), x.const_data_ptr(), w.defined() ? w.const_data_ptr() : nullptr,
-                                           static_cast<const float*>(stats.const_data_ptr()), ptr(dx), ptr(dw), ptr(db),
-                                           scratch.defined() ? scratch.mutable_data_ptr() : nullptr, scratch.defined() ? bytes : 0, rows, N, lddy, ldx, N,
-                                           center, dt, w.defined() && w.scalar_type() == at::kFloat ? (int)NQ_F32 : dt, stream_of(dev));
-                if (st < 0) fail(st, "nq_norm_bwd");
-            }
-        }
-        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+        const Tensor& w = saved[1];
+        std::array<Tensor, 3> d;
+        if (grads[0].defined())
+            d = norm_gradients(grads[0], saved[0], w, saved[2], ctx->saved_data["center"].toBool(),
+                               {ctx->needs_input_grad(0), w.defined() && ctx->needs_input_grad(1), ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2)});
+        return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor()};
     }
 };
+bool norm_takes(const Tensor& x, const Tensor* w, const Tensor* b) {
+    int64_t rows, ld;
+    if ((b && !w) || !is_16bit(x.scalar_type()) || !as_rows(x, rows, ld)) return false;
+    for (const Tensor* t : {w, b})
+        if (t && ((t->scalar_type() != x.scalar_type() && t->scalar_type() != at::kFloat) || t->scalar_type() != w->scalar_type() || t->dim() != 1 ||
+                  t->size(0) != x.size(-1) || !t->is_contiguous() || t->get_device() != x.get_device()))
+            return false;
+    return true;
+}
 
 // norm(x, weight | None, bias | None, eps, center) -> y or None
 PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -688,13 +706,8 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK(n == 5, "norm takes 5 arguments");
     if (!exact_plain(a[0])) Py_RETURN_NONE;
     const Tensor *x = plain(a[0]), *w = a[1] == Py_None ? nullptr : plain(a[1]), *b = a[2] == Py_None ? nullptr : plain(a[2]);
-    int64_t rows, ld;
-    if (!x || (a[1] != Py_None && !w) || (a[2] != Py_None && !b) || (b && !w) || !is_16bit(x->scalar_type()) || !as_rows(*x, rows, ld)) Py_RETURN_NONE;
+    if (!x || (a[1] != Py_None && !w) || (a[2] != Py_None && !b) || !norm_takes(*x, w, b)) Py_RETURN_NONE;
     const int64_t N = x->size(-1);
-    for (const Tensor* t : {w, b})
-        if (t && ((t->scalar_type() != x->scalar_type() && t->scalar_type() != at::kFloat) || t->scalar_type() != w->scalar_type() || t->dim() != 1 ||
-                  t->size(0) != N || !t->is_contiguous() || t->get_device() != x->get_device()))
-            Py_RETURN_NONE;
     const double eps = PyFloat_AsDouble(a[3]);
     const int center = PyObject_IsTrue(a[4]);
     if (PyErr_Occurred()) return nullptr;
@@ -704,75 +717,93 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         check_capture(x->get_device(), {x, w, b});
         y = NormFunction::apply(*x, w ? OptTensor(*w) : std::nullopt, b ? OptTensor(*b) : std::nullopt, N, eps, center != 0);
     } else {
-        y = norm_launch(*x, w, b, NormArgs{rows, N, eps, center != 0}, nullptr);
+        y = norm_launch(*x, w, b, NormArgs{N, eps, center != 0}, nullptr);
     }
     return THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS
 }
 
-// quantize_rows(x) -> (q, scale) or None; rows of q start at multiples of 16 bytes
-PyObject* py_quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 1, "quantize_rows takes 1 argument");
-    if (!exact_plain(a[0])) Py_RETURN_NONE;
-    const Tensor* x = plain(a[0]);
+bool quantize_takes(const Tensor& x) {
     int64_t rows, ld;
-    if (!x || !is_16bit(x->scalar_type()) || x->dim() < 1 || x->size(-1) == 0 || !as_rows(*x, rows, ld)) Py_RETURN_NONE;
-    const int64_t N = x->size(-1), ldq = (N + 15) / 16 * 16;
-    c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end()), strides(shape.size()), lead(shape.begin(), shape.end() - 1);
+    return is_16bit(x.scalar_type()) && x.dim() >= 1 && x.size(-1) > 0 && as_rows(x, rows, ld);
+}
+// (q, scale); rows of q start at multiples of 16 bytes
+std::tuple<Tensor, Tensor> quantize_launch(const Tensor& x) {
+    int64_t rows, ld;
+    as_rows(x, rows, ld);
+    const int64_t N = x.size(-1), ldq = (N + 15) / 16 * 16;
+    c10::SmallVector<int64_t, 4> shape(x.sizes().begin(), x.sizes().end()), strides(shape.size()), lead(shape.begin(), shape.end() - 1);
     strides.back() = 1;
     int64_t step = ldq;
     for (int k = (int)shape.size() - 2; k >= 0; --k) {
         strides[k] = step;
         step *= shape[k];
     }
-    Tensor buf = new_output({rows, ldq}, *x, at::kChar), scale = new_output(lead, *x, at::kFloat);
+    Tensor buf = new_output({rows, ldq}, x, at::kChar), scale = new_output(lead, x, at::kFloat);
     if (rows > 0) {
-        const int dev = x->get_device();
+        const int dev = x.get_device();
         OnDevice on(dev);
-        const int st = nq_quantize_rows_s8(x->const_data_ptr(), static_cast<int8_t*>(buf.mutable_data_ptr()), static_cast<float*>(scale.mutable_data_ptr()),
-                                           rows, N, ld, ldq, dtype_id(x->scalar_type()), stream_of(dev));
+        const int st = nq_quantize_rows_s8(x.const_data_ptr(), static_cast<int8_t*>(buf.mutable_data_ptr()), static_cast<float*>(scale.mutable_data_ptr()),
+                                           rows, N, ld, ldq, dtype_id(x.scalar_type()), stream_of(dev));
         if (st < 0) fail(st, "nq_quantize_rows_s8");
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    PyObject* q = THPVariable_Wrap(buf.as_strided(shape, strides, 0));
+    return {buf.as_strided(shape, strides, 0), scale};
+}
+// quantize_rows(x) -> (q, scale) or None
+PyObject* py_quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 1, "quantize_rows takes 1 argument");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    const Tensor* x = plain(a[0]);
+    if (!x || !quantize_takes(*x)) Py_RETURN_NONE;
+    const auto [buf, scale] = quantize_launch(*x);
+    PyObject* q = THPVariable_Wrap(buf);
     PyObject* s = q ? THPVariable_Wrap(scale) : nullptr;
     return s ? Py_BuildValue("(NN)", q, s) : nullptr;
     END_HANDLE_TH_ERRORS
 }
 
+bool int8_takes(const Tensor& x, const Tensor& w, const Tensor& ws, const Tensor* b) {
+    int64_t T, ldx;
+    if (!is_16bit(x.scalar_type()) || w.scalar_type() != at::kChar || ws.scalar_type() != at::kFloat || w.dim() != 2 || w.size(0) == 0 || w.size(1) == 0 ||
+        w.stride(1) != 1 || !as_rows(x, T, ldx) || x.size(-1) != w.size(1) || ws.dim() != 1 || ws.size(0) != w.size(0) || !ws.is_contiguous())
+        return false;
+    const int64_t N = w.size(1), V = w.size(0), ldw = w.stride(0);
+    if (b && (b->scalar_type() != x.scalar_type() || b->dim() != 1 || !b->is_contiguous() || b->size(0) != V)) return false;
+    // (one channel: its row stride means nothing)
+    if ((V > 1 && (ldw < N || ldw % 16 != 0)) || (reinterpret_cast<uintptr_t>(w.const_data_ptr()) & 15) || (reinterpret_cast<uintptr_t>(ws.const_data_ptr()) & 15))
+        return false;
+    const int dev = x.get_device();
+    return w.get_device() == dev && ws.get_device() == dev && (!b || b->get_device() == dev);
+}
+Tensor int8_launch(const Tensor& x, const Tensor& w, const Tensor& ws, const Tensor* b) {
+    int64_t T, ldx;
+    as_rows(x, T, ldx);
+    const int64_t N = w.size(1), V = w.size(0);
+    const int dev = x.get_device();
+    c10::SmallVector<int64_t, 4> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = V;
+    Tensor y = new_output(shape, x);
+    if (T == 0) return y;
+    OnDevice on(dev);
+    void* status = status_header(dev);
+    const size_t bytes = nq_int8_linear_scratch_bytes(T, N);
+    const Tensor scratch = bytes ? new_bytes((int64_t)bytes, x) : Tensor();
+    const int st = nq_int8_linear_fwd(x.const_data_ptr(), static_cast<const int8_t*>(w.const_data_ptr()), static_cast<const float*>(ws.const_data_ptr()),
+                                      b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(), bytes ? scratch.mutable_data_ptr() : nullptr, bytes, status, T, N, V, ldx,
+                                      V > 1 ? w.stride(0) : (N + 15) / 16 * 16, V, dtype_id(x.scalar_type()), stream_of(dev));
+    if (st < 0) fail(st, "nq_int8_linear_fwd");
+    return y;
+}
 // int8_linear_forward(x, weight, weight_scale, bias | None) -> y or None
 PyObject* py_int8_linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 4, "int8_linear_forward takes 4 arguments");
     if (!exact_plain(a[0])) Py_RETURN_NONE;
     const Tensor *x = plain(a[0]), *w = plain(a[1]), *ws = plain(a[2]), *b = a[3] == Py_None ? nullptr : plain(a[3]);
-    int64_t T, ldx;
-    if (!x || !w || !ws || (a[3] != Py_None && !b) || !is_16bit(x->scalar_type()) || w->scalar_type() != at::kChar || ws->scalar_type() != at::kFloat ||
-        w->dim() != 2 || w->size(0) == 0 || w->size(1) == 0 || w->stride(1) != 1 || !as_rows(*x, T, ldx) || x->size(-1) != w->size(1) || ws->dim() != 1 ||
-        ws->size(0) != w->size(0) || !ws->is_contiguous())
-        Py_RETURN_NONE;
-    const int64_t N = w->size(1), V = w->size(0), ldw = w->stride(0);
-    if (b && (b->scalar_type() != x->scalar_type() || b->dim() != 1 || !b->is_contiguous() || b->size(0) != V)) Py_RETURN_NONE;
-    // (one channel: its row stride means nothing)
-    if ((V > 1 && (ldw < N || ldw % 16 != 0)) || (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15) || (reinterpret_cast<uintptr_t>(ws->const_data_ptr()) & 15))
-        Py_RETURN_NONE;
-    const int dev = x->get_device();
-    for (const Tensor* t : {w, ws, b})
-        if (t && t->get_device() != dev) Py_RETURN_NONE;
-    c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
-    shape.back() = V;
-    Tensor y = new_output(shape, *x);
-    if (T == 0) return THPVariable_Wrap(y);
-    OnDevice on(dev);
-    void* status = status_header(dev);
-    const size_t bytes = nq_int8_linear_scratch_bytes(T, N);
-    const Tensor scratch = bytes ? new_bytes((int64_t)bytes, *x) : Tensor();
-    const int st = nq_int8_linear_fwd(x->const_data_ptr(), static_cast<const int8_t*>(w->const_data_ptr()), static_cast<const float*>(ws->const_data_ptr()),
-                                      b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(), bytes ? scratch.mutable_data_ptr() : nullptr, bytes, status, T, N, V, ldx,
-                                      V > 1 ? ldw : (N + 15) / 16 * 16, V, dtype_id(x->scalar_type()), stream_of(dev));
-    if (st < 0) fail(st, "nq_int8_linear_fwd");
-    return THPVariable_Wrap(y);
+    if (!x || !w || !ws || (a[3] != Py_None && !b) || !int8_takes(*x, *w, *ws, b)) Py_RETURN_NONE;
+    return THPVariable_Wrap(int8_launch(*x, *w, *ws, b));
     END_HANDLE_TH_ERRORS
 }
 
@@ -804,6 +835,28 @@ Tensor loss_launch(const Tensor& h, const Tensor& w, const Tensor& targets, cons
     if (st < 0) fail(st, "nq_linear_ce_fwd");
     return loss;
 }
+// (dh, dw), undefined where not wanted
+std::array<Tensor, 2> loss_gradients(const Tensor& grad, const Tensor& h, const Tensor& w, const Tensor& targets, const Tensor& lse, const Tensor& count, const LossArgs& a,
+                                     std::array<bool, 2> want) {
+    const int64_t T = h.size(0), N = h.size(1), V = w.size(0);
+    std::array<Tensor, 2> d;
+    if (want[0]) d[0] = new_output({T, N}, h);
+    if (want[1]) d[1] = T == 0 ? at::zeros({V, N}, w.options()) : new_output({V, N}, w);
+    if (T == 0 || !(want[0] || want[1])) return d;
+    const Tensor g = grad.resolve_neg();
+    const int dev = h.get_device();
+    OnDevice on(dev);
+    void* status = status_header(dev);
+    const size_t bytes = nq_linear_ce_bwd_scratch_bytes(T, N, V);
+    const Tensor scratch = new_bytes((int64_t)bytes, h);
+    const int st = nq_linear_ce_bwd(h.const_data_ptr(), w.const_data_ptr(), targets.const_data_ptr(), targets.scalar_type() == at::kLong ? 64 : 32, a.ignore,
+                                    static_cast<const float*>(lse.const_data_ptr()), static_cast<const float*>(count.const_data_ptr()),
+                                    static_cast<const float*>(g.const_data_ptr()), g.dim() == 1 ? g.stride(0) : 0, want[0] ? d[0].mutable_data_ptr() : nullptr,
+                                    want[1] ? d[1].mutable_data_ptr() : nullptr, scratch.mutable_data_ptr(), bytes, status, T, N, V, row_stride(h), row_stride(w), N, N,
+                                    a.reduction, dtype_id(h.scalar_type()), stream_of(dev));
+    if (st < 0) fail(st, "nq_linear_ce_bwd");
+    return d;
+}
 struct LossFunction : torch::autograd::Function<LossFunction> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& targets, int64_t ignore, int64_t reduction) {
         Tensor lse, count;
@@ -817,34 +870,25 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy is differentiable once");
         const auto saved = ctx->get_saved_variables();
-        const Tensor &h = saved[0], &w = saved[1], &targets = saved[2], &lse = saved[3], &count = saved[4];
-        const int reduction = (int)ctx->saved_data["reduction"].toInt();
-        Tensor dh, dw;
+        std::array<Tensor, 2> d;
         if (grads[0].defined()) {
-            const int64_t T = h.size(0), N = h.size(1), V = w.size(0);
-            if (ctx->needs_input_grad(0)) dh = new_output({T, N}, h);
-            if (ctx->needs_input_grad(1)) dw = T == 0 ? at::zeros({V, N}, w.options()) : new_output({V, N}, w);
-            if (T > 0 && (dh.defined() || dw.defined())) {
-                const Tensor g = grads[0].resolve_neg();
-                const int dev = h.get_device();
-                OnDevice on(dev);
-                const auto own = ctx->saved_data.find("scratch");
-                const OnScratch on_scratch(own == ctx->saved_data.end() ? Tensor() : own->second.toTensor());
-                void* status = status_header(dev);
-                const size_t bytes = nq_linear_ce_bwd_scratch_bytes(T, N, V);
-                const Tensor scratch = new_bytes((int64_t)bytes, h);
-                const int st = nq_linear_ce_bwd(h.const_data_ptr(), w.const_data_ptr(), targets.const_data_ptr(), targets.scalar_type() == at::kLong ? 64 : 32,
-                                                ctx->saved_data["ignore"].toInt(), static_cast<const float*>(lse.const_data_ptr()),
-                                                static_cast<const float*>(count.const_data_ptr()), static_cast<const float*>(g.const_data_ptr()),
-                                                g.dim() == 1 ? g.stride(0) : 0, dh.defined() ? dh.mutable_data_ptr() : nullptr,
-                                                dw.defined() ? dw.mutable_data_ptr() : nullptr, scratch.mutable_data_ptr(), bytes, status, T, N, V,
-                                                row_stride(h), row_stride(w), N, N, reduction, dtype_id(h.scalar_type()), stream_of(dev));
-                if (st < 0) fail(st, "nq_linear_ce_bwd");
-            }
+            const auto own = ctx->saved_data.find("scratch");
+            const OnScratch on_scratch(own == ctx->saved_data.end() ? Tensor() : own->second.toTensor());
+            d = loss_gradients(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+                               LossArgs{ctx->saved_data["ignore"].toInt(), (int)ctx->saved_data["reduction"].toInt()}, {ctx->needs_input_grad(0), ctx->needs_input_grad(1)});
         }
-        return {dh, dw, Tensor(), Tensor(), Tensor()};
+        return {d[0], d[1], Tensor(), Tensor(), Tensor()};
     }
 };
+bool loss_takes(const Tensor& h, const Tensor& w, const Tensor& t) {
+    if (!is_16bit(h.scalar_type()) || w.scalar_type() != h.scalar_type() || h.dim() != 2 || w.dim() != 2 || t.dim() != 1 ||
+        (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt) || h.size(1) != w.size(1) || t.size(0) != h.size(0) || !t.is_contiguous() ||
+        h.stride(1) != 1 || w.stride(1) != 1 || w.get_device() != h.get_device() || t.get_device() != h.get_device())
+        return false;
+    for (const Tensor* m : {&h, &w})
+        if ((reinterpret_cast<uintptr_t>(m->const_data_ptr()) & 15) || row_stride(*m) % 8 != 0 || row_stride(*m) < m->size(1)) return false;
+    return true;
+}
 
 // linear_cross_entropy(h, weight, targets, ignore_index, reduction) -> loss or None
 PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -852,12 +896,7 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK(n == 5, "linear_cross_entropy takes 5 arguments");
     if (!exact_plain(a[0])) Py_RETURN_NONE;
     const Tensor *h = plain(a[0]), *w = plain(a[1]), *t = plain(a[2]);
-    if (!h || !w || !t || !is_16bit(h->scalar_type()) || w->scalar_type() != h->scalar_type() || h->dim() != 2 || w->dim() != 2 || t->dim() != 1 ||
-        (t->scalar_type() != at::kLong && t->scalar_type() != at::kInt) || h->size(1) != w->size(1) || t->size(0) != h->size(0) || !t->is_contiguous() ||
-        h->stride(1) != 1 || w->stride(1) != 1 || w->get_device() != h->get_device() || t->get_device() != h->get_device())
-        Py_RETURN_NONE;
-    for (const Tensor* m : {h, w})
-        if ((reinterpret_cast<uintptr_t>(m->const_data_ptr()) & 15) || row_stride(*m) % 8 != 0 || row_stride(*m) < m->size(1)) Py_RETURN_NONE;
+    if (!h || !w || !t || !loss_takes(*h, *w, *t)) Py_RETURN_NONE;
     const int64_t ignore = PyLong_AsLongLong(a[3]), reduction = PyLong_AsLongLong(a[4]);
     if (PyErr_Occurred()) return nullptr;
     refuse_tangents("linear_cross_entropy", {h, w});
@@ -871,6 +910,82 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     return THPVariable_Wrap(loss);
     END_HANDLE_TH_ERRORS
+}
+
+// The same as operators of the dispatcher, for what records calls (torch.compile, torch.jit.trace); schemas, shapes for tracing and derivatives: nanoquant_b200/ops.py.
+Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
+OptTensor dense(const OptTensor& t) { return t ? OptTensor(dense(*t)) : t; }
+const Tensor* pointer(const OptTensor& t) { return t ? &*t : nullptr; }
+Tensor or_none(const Tensor& t, const Tensor& like) { return t.defined() ? t : new_output({0}, like); }
+
+std::tuple<Tensor, Tensor> op_norm(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps, bool center) {
+    const Tensor x = dense_rows(x_);
+    const OptTensor w = dense(w_), b = dense(b_);
+    TORCH_CHECK(norm_takes(x, pointer(w), pointer(b)), "nanoquant_b200::norm: 16-bit rows, and weight and bias of their columns in that type or fp32");
+    Tensor stats, y = norm_launch(x, pointer(w), pointer(b), NormArgs{x.size(-1), eps, center}, &stats);
+    return {y, stats};
+}
+std::tuple<Tensor, Tensor, Tensor> op_norm_backward(const Tensor& dy, const Tensor& x_, const OptTensor& w_, const Tensor& stats, bool center, std::array<bool, 3> want) {
+    const Tensor x = dense_rows(x_);
+    const OptTensor w = dense(w_);
+    TORCH_CHECK(norm_takes(x, pointer(w), nullptr) && dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && (w || !(want[1] || want[2])) &&
+                    stats.scalar_type() == at::kFloat && stats.is_contiguous() && (x.size(-1) == 0 || stats.numel() == 2 * (x.numel() / x.size(-1))),
+                "nanoquant_b200::norm_backward: operands of nanoquant_b200::norm and its second result");
+    const auto d = norm_gradients(dy, x, w ? *w : Tensor(), stats, center, want);
+    return {or_none(d[0], x), or_none(d[1], x), or_none(d[2], x)};
+}
+std::tuple<Tensor, Tensor> op_quantize_rows(const Tensor& x_) {
+    const Tensor x = x_.dim() ? dense_rows(x_) : x_;
+    TORCH_CHECK(quantize_takes(x), "nanoquant_b200::quantize_rows: 16-bit rows of at least one column");
+    return quantize_launch(x);
+}
+Tensor op_int8_linear(const Tensor& x_, const Tensor& w_, const Tensor& ws_, const OptTensor& b_) {
+    const Tensor x = dense_rows(x_), w = w_.resolve_neg();
+    Tensor ws = dense(ws_);
+    if (reinterpret_cast<uintptr_t>(ws.const_data_ptr()) & 15) ws = ws.clone();
+    const OptTensor b = dense(b_);
+    TORCH_CHECK(int8_takes(x, w, ws, pointer(b)),
+                "nanoquant_b200::int8_linear: 16-bit rows, an int8 weight whose rows start at multiples of 16 bytes, its fp32 scales, a bias in the type of the rows");
+    return int8_launch(x, w, ws, pointer(b));
+}
+Tensor op_dense_gemv(const Tensor& x_, const Tensor& w_, const OptTensor& b_) {
+    const Tensor x = dense(x_), w = w_.resolve_neg();
+    const OptTensor b = dense(b_);
+    TORCH_CHECK(dense_gemv_takes(x, w, pointer(b)), "nanoquant_b200::dense_gemv: 16-bit rows and weight, the weight's columns dense");
+    return dense_gemv_launch(x, w, pointer(b));
+}
+// What the loss reads in place: rows at multiples of 16 bytes.
+Tensor loss_matrix(const Tensor& t_) {
+    const Tensor t = t_.resolve_neg();
+    const bool in_place = t.dim() == 2 && t.stride(1) == 1 && row_stride(t) % 8 == 0 && row_stride(t) >= t.size(1) && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0;
+    return in_place ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+const char* const kLossOperands = "nanoquant_b200::linear_cross_entropy: 16-bit matrices of one type with a multiple of 8 columns, one int64 or int32 target for each row";
+std::tuple<Tensor, Tensor, Tensor> op_linear_cross_entropy(const Tensor& h_, const Tensor& w_, const Tensor& t_, int64_t ignore, int64_t reduction) {
+    const Tensor h = loss_matrix(h_), w = loss_matrix(w_), t = dense(t_);
+    TORCH_CHECK(loss_takes(h, w, t), kLossOperands);
+    Tensor lse, count, loss = loss_launch(h, w, t, LossArgs{ignore, (int)reduction}, lse, count);
+    return {loss, lse, count};
+}
+std::tuple<Tensor, Tensor> op_linear_cross_entropy_backward(const Tensor& grad, const Tensor& h_, const Tensor& w_, const Tensor& t_, const Tensor& lse, const Tensor& count,
+                                                            int64_t ignore, int64_t reduction, std::array<bool, 2> want) {
+    const Tensor h = loss_matrix(h_), w = loss_matrix(w_), t = dense(t_);
+    TORCH_CHECK(loss_takes(h, w, t), kLossOperands);
+    const int64_t T = h.size(0);
+    TORCH_CHECK(grad.scalar_type() == at::kFloat && lse.scalar_type() == at::kFloat && count.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == T &&
+                    count.numel() == 1 && (reduction == NQ_REDUCE_NONE ? grad.dim() == 1 && grad.size(0) == T : grad.dim() == 0),
+                "nanoquant_b200::linear_cross_entropy_backward: the gradient of the first result of nanoquant_b200::linear_cross_entropy, and the other two");
+    const auto d = loss_gradients(grad, h, w, t, lse, count, LossArgs{ignore, (int)reduction}, want);
+    return {or_none(d[0], h), or_none(d[1], h)};
+}
+TORCH_LIBRARY_IMPL(nanoquant_b200, CUDA, m) {
+    m.impl("norm", op_norm);
+    m.impl("norm_backward", op_norm_backward);
+    m.impl("quantize_rows", op_quantize_rows);
+    m.impl("int8_linear", op_int8_linear);
+    m.impl("dense_gemv", op_dense_gemv);
+    m.impl("linear_cross_entropy", op_linear_cross_entropy);
+    m.impl("linear_cross_entropy_backward", op_linear_cross_entropy_backward);
 }
 
 // The pack / layout kernels on a contiguous CUDA tensor.

@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import os
 import threading
 from typing import Optional
 
@@ -198,15 +199,21 @@ def gemv_forward(x: torch.Tensor, s_in: torch.Tensor, v_tiles: torch.Tensor, s_m
     return y
 
 
+def _recorded() -> bool:
+    """The call is recorded (``torch.compile``, ``torch.jit.trace``): it has to be one of the dispatcher's."""
+    return torch.compiler.is_compiling() or torch.jit.is_tracing()
+
+
 def dense_gemv_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``F.linear(x, weight, bias)`` for the few tokens of a decode step through ``nq_dense_gemv_fwd``.
 
     For the layers the reference leaves as ``nn.Linear`` (``lm_head``, ``utils/load_utils.py:322``): ``weight``
     ``[V, N]`` fp16/bf16 with a unit inner stride, ``x`` ``[..., N]`` with at most ``nq_dense_gemv_max_tokens()``
     rows in total; more rows raise (a batched GEMM is the right tool there)."""
-    y = _lib.ext().dense_gemv_forward(x, weight, bias)
-    if y is not None:
-        return y
+    if not torch.compiler.is_compiling():
+        y = _lib.ext().dense_gemv_forward(x, weight, bias)
+        if y is not None:
+            return y
     _check_cuda_cont(x, "x", weight.dtype, str(weight.dtype))
     if weight.dim() != 2 or weight.stride(1) != 1 or not weight.is_cuda:
         raise RuntimeError("weight must be a CUDA [V, N] matrix with a unit inner stride")
@@ -214,6 +221,8 @@ def dense_gemv_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
         raise RuntimeError(f"x has {x.size(-1)} columns, weight expects {weight.size(1)}")
     if bias is not None:
         _check_cuda_cont(bias, "bias", weight.dtype, str(weight.dtype))
+    if _recorded() and x.numel() > 0:
+        return torch.ops.nanoquant_b200.dense_gemv(x, weight, bias)
     x, weight, bias = _stored(x), _stored(weight), _stored(bias)
     V, N = weight.shape
     x2 = x.reshape(-1, N)
@@ -256,9 +265,10 @@ def _not_plain(what: str) -> RuntimeError:
 
 
 def _norm(what: str, x, weight, bias, eps: float, center: bool) -> torch.Tensor:
-    y = _lib.ext().norm(x, weight, bias, eps, center)
-    if y is not None:
-        return y
+    if not torch.compiler.is_compiling():
+        y = _lib.ext().norm(x, weight, bias, eps, center)
+        if y is not None:
+            return y
     _check_16bit(x, "x")
     if x.dim() < 1:
         raise RuntimeError("x needs at least one dimension")
@@ -266,6 +276,8 @@ def _norm(what: str, x, weight, bias, eps: float, center: bool) -> torch.Tensor:
         raise RuntimeError("bias needs a weight")
     for t, name in ((weight, "weight"), (bias, "bias")):
         _check_like(t, name, x, (x.dtype, torch.float32) if t is weight else (weight.dtype,), (x.size(-1),))
+    if _recorded():
+        return torch.ops.nanoquant_b200.norm(x, weight, bias, eps, center)[0]
     # rows that are not evenly spaced, columns that are not dense, lazily negated tensors
     dense = lambda t: None if t is None else t.resolve_neg().contiguous()
     y = _lib.ext().norm(dense(x), dense(weight), dense(bias), eps, center)
@@ -292,14 +304,18 @@ def quantize_int8(x: torch.Tensor):
     """``(q, scale)`` of fp16 / bf16 ``x [..., N]``: signed bytes and one fp32 scale for each row of the last dimension,
     ``scale = max|x| / 127``, ``q = rint(127 x / max|x|)``.  For the weight of :func:`int8_linear_forward`: rows of ``q`` start at
     multiples of 16 bytes.  A row with a NaN or an infinity gets a NaN scale."""
-    r = _lib.ext().quantize_rows(x)
+    if not torch.compiler.is_compiling():
+        r = _lib.ext().quantize_rows(x)
+        if r is not None:
+            return r
+    _check_16bit(x, "x")
+    if x.dim() < 1 or x.size(-1) == 0:
+        raise RuntimeError("x needs a last dimension with columns")
+    if _recorded():
+        return torch.ops.nanoquant_b200.quantize_rows(x)
+    r = _lib.ext().quantize_rows(x.resolve_neg().contiguous())
     if r is None:
-        _check_16bit(x, "x")
-        if x.dim() < 1 or x.size(-1) == 0:
-            raise RuntimeError("x needs a last dimension with columns")
-        r = _lib.ext().quantize_rows(x.resolve_neg().contiguous())
-        if r is None:
-            raise _not_plain("quantize_int8")
+        raise _not_plain("quantize_int8")
     return r
 
 
@@ -312,9 +328,10 @@ def int8_linear_forward(x: torch.Tensor, weight: torch.Tensor, weight_scale: tor
     row stride that is a multiple of 16 and ``weight_scale`` ``[V]`` fp32, both from ``quantize_int8(lm_head.weight)``; ``x`` ``[..., N]``
     fp16 / bf16 with any number of tokens, ``bias`` ``[V]`` in its type.  Sums are exact, the result is rounded once.  Inference: no
     gradient.  A token with a NaN or an infinity is NaN in all its outputs."""
-    y = _lib.ext().int8_linear_forward(x, weight, weight_scale, bias)
-    if y is not None:
-        return y
+    if not torch.compiler.is_compiling():
+        y = _lib.ext().int8_linear_forward(x, weight, weight_scale, bias)
+        if y is not None:
+            return y
     _check_16bit(x, "x")
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_cuda or weight.dtype != torch.int8:
         raise RuntimeError("weight must be a CUDA [V, N] matrix of int8")
@@ -325,10 +342,12 @@ def int8_linear_forward(x: torch.Tensor, weight: torch.Tensor, weight_scale: tor
         raise RuntimeError("weight is empty")
     if weight.device != x.device:
         raise RuntimeError(f"weight is on {weight.device}, the input on {x.device}")
-    if weight.stride(1) != 1 or (V > 1 and (weight.stride(0) % 16 or weight.stride(0) < N)) or weight.data_ptr() % 16:
+    if weight.stride(1) != 1 or (V > 1 and (weight.stride(0) % 16 or weight.stride(0) < N)) or (not _recorded() and weight.data_ptr() % 16):
         raise RuntimeError("rows of weight must be dense and start at multiples of 16 bytes (quantize_int8 lays them out so)")
     _check_like(weight_scale, "weight_scale", x, (torch.float32,), (V,))
     _check_like(bias, "bias", x, (x.dtype,), (V,))
+    if _recorded():
+        return torch.ops.nanoquant_b200.int8_linear(x, weight, weight_scale, bias)
     dense = lambda t: None if t is None else t.resolve_neg().contiguous()
     scale = dense(weight_scale)
     y = _lib.ext().int8_linear_forward(dense(x), weight, scale if scale.data_ptr() % 16 == 0 else scale.clone(), dense(bias))
@@ -349,9 +368,10 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     vocabulary's gradients at a time (256 MB).  The mean over no tokens is NaN, its gradient zero."""
     if reduction not in _lib.REDUCTION_ID:
         raise ValueError(f"reduction should be one of [none, sum, mean], but {reduction} was given")
-    loss = _lib.ext().linear_cross_entropy(h, weight, targets, ignore_index, _lib.REDUCTION_ID[reduction])
-    if loss is not None:
-        return loss
+    if not torch.compiler.is_compiling():
+        loss = _lib.ext().linear_cross_entropy(h, weight, targets, ignore_index, _lib.REDUCTION_ID[reduction])
+        if loss is not None:
+            return loss
     _check_16bit(h, "h")
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or h.dim() < 1 or h.size(-1) != weight.size(1):
         raise RuntimeError("weight must be a [V, N] matrix, h [..., N]")
@@ -360,6 +380,9 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     _check_like(targets, "targets", h, (torch.int64, torch.int32), h.shape[:-1])
     if V == 0 or N == 0 or N % 8:
         raise RuntimeError(f"weight has {V} words and {N} columns: at least one word, and a multiple of 8 columns")
+    if _recorded():
+        loss = torch.ops.nanoquant_b200.linear_cross_entropy(h.reshape(-1, N), weight, targets.reshape(-1), ignore_index, _lib.REDUCTION_ID[reduction])[0]
+        return loss.reshape(targets.shape) if reduction == "none" else loss
     dense = lambda t: t if t.dim() == 2 and t.stride(1) == 1 and (t.size(0) == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= N)) and \
         t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
     loss = _lib.ext().linear_cross_entropy(dense(h.resolve_neg().reshape(-1, N)), dense(weight.resolve_neg()),
@@ -367,6 +390,101 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     if loss is None:
         raise _not_plain("linear_cross_entropy")
     return loss.reshape(targets.shape) if reduction == "none" else loss
+
+
+# The same calls as operators of the dispatcher, for what records calls: implementations in csrc/nq_torch.cpp, shapes for tracing and derivatives here.
+_RECORDED_OPS = {
+    "norm": "(Tensor x, Tensor? weight, Tensor? bias, float eps, bool center) -> (Tensor, Tensor)",
+    "norm_backward": "(Tensor dy, Tensor x, Tensor? weight, Tensor stats, bool center, bool[3] want) -> (Tensor, Tensor, Tensor)",
+    "quantize_rows": "(Tensor x) -> (Tensor, Tensor)",
+    "int8_linear": "(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias) -> Tensor",
+    "dense_gemv": "(Tensor x, Tensor weight, Tensor? bias) -> Tensor",
+    "linear_cross_entropy": "(Tensor h, Tensor weight, Tensor targets, int ignore_index, int reduction) -> (Tensor, Tensor, Tensor)",
+    "linear_cross_entropy_backward": "(Tensor grad, Tensor h, Tensor weight, Tensor targets, Tensor lse, Tensor count, int ignore_index, int reduction, "
+                                     "bool[2] want) -> (Tensor, Tensor)",
+}
+
+
+def _rows(x):
+    n = 1
+    for k in x.shape[:-1]:
+        n = n * k
+    return n
+
+
+def _norm_fake(x, weight, bias, eps, center):
+    return x.new_empty(x.shape), x.new_empty((_rows(x), 2), dtype=torch.float32)
+
+
+def _norm_backward_fake(dy, x, weight, stats, center, want):
+    some = lambda wanted, like: like.new_empty(like.shape) if wanted else x.new_empty((0,))
+    return some(want[0], x), some(want[1], weight), some(want[2], weight)
+
+
+def _norm_setup(ctx, inputs, output):
+    x, weight, bias, _, center = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.mark_non_differentiable(output[1])
+    ctx.center = center
+
+
+def _norm_gradients(ctx, dy, _):
+    if torch.is_grad_enabled():
+        raise RuntimeError("the norms are differentiable once")
+    x, weight, stats = ctx.saved_tensors
+    want = list(ctx.needs_input_grad[:3])
+    d = torch.ops.nanoquant_b200.norm_backward(dy, x, weight, stats, ctx.center, want)
+    return (*(t if wanted else None for t, wanted in zip(d, want)), None, None)
+
+
+def _quantize_rows_fake(x):
+    strides, step = [1], (x.shape[-1] + 15) // 16 * 16
+    for k in reversed(x.shape[:-1]):
+        strides.insert(0, step)
+        step = step * k
+    return x.new_empty_strided(x.shape, strides, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+def _head_fake(x, weight, *_):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+def _linear_cross_entropy_fake(h, weight, targets, ignore_index, reduction):
+    number = lambda *shape: h.new_empty(shape, dtype=torch.float32)
+    return number(h.shape[0]) if reduction == _lib.REDUCTION_ID["none"] else number(), number(h.shape[0]), number(1)
+
+
+def _linear_cross_entropy_backward_fake(grad, h, weight, targets, lse, count, ignore_index, reduction, want):
+    return tuple(t.new_empty(t.shape) if wanted else h.new_empty((0,)) for t, wanted in zip((h, weight), want))
+
+
+def _linear_cross_entropy_setup(ctx, inputs, output):
+    h, weight, targets, ctx.ignore_index, ctx.reduction = inputs
+    ctx.save_for_backward(h, weight, targets, *output[1:])
+    ctx.mark_non_differentiable(*output[1:])
+
+
+def _linear_cross_entropy_gradients(ctx, grad, *_):
+    if torch.is_grad_enabled():
+        raise RuntimeError("linear_cross_entropy is differentiable once")
+    want = list(ctx.needs_input_grad[:2])
+    d = torch.ops.nanoquant_b200.linear_cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index, ctx.reduction, want)
+    return (*(t if wanted else None for t, wanted in zip(d, want)), None, None, None)
+
+
+def _define_recorded_ops() -> None:
+    name = "nanoquant_b200::{}".format
+    for op, schema in _RECORDED_OPS.items():
+        torch.library.define(name(op), schema)
+    for op, fake in (("norm", _norm_fake), ("norm_backward", _norm_backward_fake), ("quantize_rows", _quantize_rows_fake), ("int8_linear", _head_fake),
+                     ("dense_gemv", _head_fake), ("linear_cross_entropy", _linear_cross_entropy_fake),
+                     ("linear_cross_entropy_backward", _linear_cross_entropy_backward_fake)):
+        torch.library.register_fake(name(op))(fake)
+    torch.library.register_autograd(name("norm"), _norm_gradients, setup_context=_norm_setup)
+    torch.library.register_autograd(name("linear_cross_entropy"), _linear_cross_entropy_gradients, setup_context=_linear_cross_entropy_setup)
+
+
+_define_recorded_ops()
 
 
 def _nanoquant_dyn_forward_cuda(x, scale_g, Ubits, scale_l, Vbits, scale_h,
@@ -634,7 +752,11 @@ def define_ops() -> None:
     torch.library.register_fake("binary_kernels::marlin_nanoquant_forward")(_marlin_nanoquant_forward_fake)
     # the CUDA implementations of the other two operators; without the built extension (schemas and tracing only) a
     # call on CUDA tensors fails in the dispatcher
-    import os
     if os.path.exists(_lib.EXT_PATH):
         _lib.ext()
     _DEFINED = True
+
+
+# The CUDA implementations of the operators above; without the built extension (schemas and tracing only) a call on CUDA tensors fails in the dispatcher.
+if os.path.exists(_lib.EXT_PATH):
+    _lib.ext()
