@@ -980,14 +980,13 @@ NormVariant norm_variant(bool bwd, bool bf16, bool center) {
     return {k, 32 * WARPS * norm_rows_per_cta<WARPS>(), norm_rows_per_cta<WARPS>()};
 }
 // Direct kernels: the smallest group that holds a row.  16-byte loads where every row starts at a 16-byte boundary, single elements otherwise.
-NormVariant choose_norm(bool bwd, bool bf16, bool center, bool vec, long long rows, int N) {
+// (vec: at most 2 sm_count() rows, more are streamed)
+NormVariant choose_norm(bool bwd, bool bf16, bool center, bool vec, int N) {
     if (vec) {
         const int packs = (N + 7) / 8;
         if (packs <= 64) return norm_variant<8, 2, 1>(bwd, bf16, center);
-        if (rows <= 2 * sm_count() && packs <= 512)      // few rows: one load a thread
-            return packs <= 128 ? norm_variant<8, 1, 4>(bwd, bf16, center) : norm_variant<8, 1, 16>(bwd, bf16, center);
-        if (packs <= 256) return norm_variant<8, 2, 4>(bwd, bf16, center);
-        if (packs <= 512) return norm_variant<8, 2, 8>(bwd, bf16, center);
+        if (packs <= 128) return norm_variant<8, 1, 4>(bwd, bf16, center);
+        if (packs <= 512) return norm_variant<8, 1, 16>(bwd, bf16, center);
         if (packs <= 1024) return norm_variant<8, 2, 16>(bwd, bf16, center);
         return norm_variant<8, 4, 16>(bwd, bf16, center);
     }
@@ -1121,7 +1120,7 @@ int nq_norm_fwd(const void* x, const void* weight, const void* bias, void* y, fl
         const int st = choose_stream(false, dtype == NQ_BF16, center != 0, vec, P, v);
         return st != NQ_OK ? st : launch_stream(v, P, as_stream(stream));
     }
-    const NormVariant v = choose_norm(false, dtype == NQ_BF16, center != 0, vec, rows, (int)N);
+    const NormVariant v = choose_norm(false, dtype == NQ_BF16, center != 0, vec, (int)N);
     return launch_norm(v, (rows + v.rows_per_cta - 1) / v.rows_per_cta, P, as_stream(stream));
 }
 
@@ -1161,7 +1160,7 @@ int nq_norm_bwd(const void* dy, const void* x, const void* weight, const float* 
         if (st != NQ_OK) return st;
         ctas = sv.ctas;
     } else {
-        v = choose_norm(true, bf16, center != 0, vec, rows, (int)N);
+        v = choose_norm(true, bf16, center != 0, vec, (int)N);
         int per_sm = 0;
         NQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, (const void*)v.fn, v.threads, 0));
         const int most = norm_ctas_per_sm(N);
