@@ -8,7 +8,7 @@
 //
 // Few tokens are bound by the memory that the weights stream from: K V bytes, half of the 16-bit head.  The tokens are the MMA's 128
 // rows and the output channels its columns, so any number of tokens up to 128 costs the same reads.  Prompts are bound by the tensor
-// cores, pairs of CTAs on 256 x 256 tiles.
+// cores, pairs of CTAs on tiles of 256 rows and up to 256 columns.
 #include "nq_common.cuh"
 #include "nq_mm.cuh"
 

@@ -12,7 +12,7 @@
 // logits in fp32 would save the fourth product, and take 4 T V bytes: 1.2 GB for 2048 tokens and 151936 words.
 //
 // Bound by the tensor cores from some 300 tokens on, below by reading w (each product once).  2048 tokens, 51200 x 4096, all with a target, us: logits and
-// their sums 521, d 527, dw 534, dh 571, the tensor cores busy for 94 to 98 % of the cycles; packing 7, joining 10, preparing 12, adding dh 17.
+// their sums 521, d 560, dw 535, dh 571, the tensor cores busy for 98, 90, 94 and 98 % of the cycles; packing 7, joining 11, preparing 13, adding dh 17.
 #include <type_traits>
 
 #include "nq_common.cuh"
@@ -20,15 +20,16 @@
 
 namespace nq {
 
-// Bytes of d of a piece.  Three products of the backward pass, us at 64 / 128 / 256 / 512 MB: 2048 tokens, 151936 x 4096 6027 / 5807 / 5826 / 5797, 8192 tokens 24631 /
-// 24534 / 24291 / 23708, 16384 tokens, 32000 x 4096 11291 / 9967 / 10297 / 11164, 1000 tokens, 128256 x 8192 5135 / 5150 / 5042 / 5052.
+// Bytes of d of a piece.  Three products of the backward pass, us at 64 / 128 / 256 / 512 MB: 2048 tokens, 151936 x 4096 6224 / 6079 / 6091 / 5967, 8192 tokens 25478 /
+// 25419 / 24933 / 24271, 16384 tokens, 32000 x 4096 11319 / 10386 / 11144 / 11167, 1000 tokens, 128256 x 8192 5357 / 5245 / 5155 / 5170.
 constexpr int64_t kLossPieceBytes = 256ll << 20;
 constexpr int kLossPieceUnit = 256;
 // Steps of 64 products after which a sum leaves the tensor cores, which cut it off towards zero with every instruction (nq_mm.cuh).  Logits: the same in both
 // passes, so that the backward's are the numbers that lse came from.  (With whole sums there, p - 1 of a target with p = 0.999 was off by 6 to 19 % at 4096 columns and
-// by up to 38 % at 8192.)  Forward level with whole sums, with 256 columns 5 % slower; the backward's logits and d 9 to 15 % slower, 2 to 6 % of the pass: a tile's
-// outputs all come at its end.  Sums over tokens and words: of 2048 products, whose error of 1.2e-5 at most is far below the outputs' rounding and does not grow
-// with their number (65536 tokens: 4.2e-4 of a whole sum); level with whole sums, with 512 9 % slower.
+// by up to 38 % at 8192.)  Forward level with whole sums, with 256 columns 5 % slower; the backward's logits and d 6 % (4096 columns) to 15 % (2048)
+// slower, 2 to 6 % of the pass: a tile's outputs all come at its end.  Sums over tokens and words: of 2048 products, whose error of 1.2e-5
+// is far below the outputs' rounding and does not grow with their number (65536 tokens: 4.2e-4 of a whole sum); level with whole sums, with 512 products 9 %
+// slower.
 constexpr int kLossLogitsChunk = 8, kLossSumsChunk = 32;
 constexpr int kLossRows = 16384;           // tokens of a forward product: the scratch holds 8 bytes for each and every 64 to 128 words
 constexpr int kLossJoinHere = 8192;        // pieces of all tokens that one CTA joins
@@ -531,9 +532,9 @@ static LossPlan plan_loss(int64_t T, int64_t N, int64_t V) {
     p.w_bn = N <= 128 ? 128 : 256;
     // dh: few tiles over a long k, in us: rounds of the longest tile (a step takes 0.27, a tile's start and end as much as 8), the launch that adds the
     // splits' sums, and what writing (with several pieces, also reading) and adding them moves.
-    // dh alone, us with 1 / 2 / 4 / 8 splits and as chosen: 128 tokens, 32000 x 2048 210 / 126 / 83 / 65, 66; 512 tokens, 128256 x 2048 761 / 580 / 508 / 519, 528; 1024
-    // tokens 1083 / 903 / 914 / 919, 902; 2048 tokens, 51200 x 4096 1341 / 1376 / 1369 / 1392, 1359; 8192 tokens, 32000 x 2048 936 / 965 / 984 / 1063, 937 (the
-    // logits' product included; large ones run at the power limit, where idle SMs leave the others a higher clock).
+    // dh alone (the logits' product included), us with 1 / 2 / 4 / 8 splits and as chosen: 128 tokens, 32000 x 2048 212 / 128 / 86 / 68, 66; 512 tokens, 128256 x 2048
+    // 779 / 600 / 512 / 501, 499; 1024 tokens 1161 / 927 / 930 / 956, 939; 2048 tokens, 51200 x 4096 1411 / 1427 / 1404 / 1446, 1402; 8192 tokens, 32000 x 2048 1815 /
+    // 1814 / 1852 / 1998, 1794 (large ones run at the power limit, where idle SMs leave the others a higher clock).
     p.h_bn = cg == 2 ? (N <= 128 ? 128 : 256) : (N <= 64 ? 64 : N <= 128 ? 128 : 256);
     const int64_t tiles = (int64_t)m_tiles * ((N + p.h_bn - 1) / p.h_bn), steps = ((p.piece < V ? p.piece : V) + 63) / 64;
     const bool one = p.piece >= V && !loss_packs(T, N, V);

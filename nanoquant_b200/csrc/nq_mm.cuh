@@ -495,8 +495,8 @@ struct MmOperand {
 
 // Width of the tiles: the multiple of `unit` up to 256 that takes least time, in columns of a k step.
 // Pairs of CTAs: whole rounds of tiles over the pairs; a tile costs its columns and some 220 more, for its rows pass through L2 to the SMs as often as
-// there are tiles.  us at 128 / 160 / 192 / 224 / 256 columns: int8 12288 x 4096, 512 tokens 32.1 / 34.3 / 30.6 / 31.6 / 33.2, 4096 tokens 172 / 157 / 146 / 141 /
-// 139, 4096 x 12288, 2048 tokens 102 / 89 / 95 / 100 / 85; the loss of 2048 tokens at 128256 x 2048 895 / 792 / 731 / 704 / 681.
+// there are tiles.  us at 128 / 160 / 192 / 224 / 256 columns: int8 12288 x 4096, 512 tokens 32.1 / 34.3 / 30.6 / 31.6 / 33.2, 2048 tokens 111 / 93 / 85 / 86 (taken) /
+// 97, 4096 tokens 172 / 157 / 146 / 141 / 139, 4096 x 12288, 2048 tokens 102 / 89 / 95 / 100 / 85; the loss of 2048 tokens at 128256 x 2048 895 / 792 / 731 / 704 / 681.
 // Single CTAs have up to 128 rows and are bound by the memory that B streams from, as long as a step has enough of it: its four MMAs take as long for
 // 16 columns as for some 100 (they fetch 128 rows of A all the same).  The last tile's latency is what narrow tiles save.  One token, int8, us at
 // 32 / 64 / 96 / 128 / 176 / 208 / 256 columns: 128256 x 2048 94 / 52 / 46.4 / 44.5 / 50.5 / 51.6 / 48.6, 151936 x 4096 200 / 108 / 94.8 / 97.4 / 97.0 /
