@@ -176,9 +176,16 @@ def as_tiles(bits: torch.Tensor, cols: int) -> torch.Tensor:
     return tiles
 
 
+def _refuse_trace(what: str) -> None:
+    """For calls that are no operators: to ``torch.jit.trace`` their results are constants, or memory that nobody fills."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: it is no operator of the dispatcher")
+
+
 def gemv_forward(x: torch.Tensor, s_in: torch.Tensor, v_tiles: torch.Tensor, s_mid: Optional[torch.Tensor],
                  u_tiles: torch.Tensor, s_out: torch.Tensor, R: int) -> torch.Tensor:
     """The decode path on the current stream at any token count; ``x`` is ``[T, N]``."""
+    _refuse_trace("gemv_forward")
     x, s_in, s_mid, s_out = (_stored(t) for t in (x, s_in, s_mid, s_out))
     T, N = x.shape
     M = s_out.size(0)
@@ -549,6 +556,7 @@ def group_forward(xs, layers, T: int, dtype: torch.dtype, device: torch.device, 
     optional ``biases[i]`` ``[M_i]`` and ``residuals[i]`` ``[T, M_i]`` (added in fp32 behind the output scale).  The
     outputs are written side by side into one ``[T, sum(M_i)]`` buffer (``out`` or a fresh one); returns its
     per-linear column views."""
+    _refuse_trace("a launch group, or a linear with a bias or residual,")
     n = len(layers)
     xs = [_stored(x) for x in xs]
     layers = [tuple(_stored(t) for t in lay[:5]) + (lay[5],) for lay in layers]
@@ -602,6 +610,7 @@ def linear_forward(x: torch.Tensor, s_in: torch.Tensor, v_tiles: torch.Tensor, s
     if bias is not None or residual is not None:
         return group_forward([x], [(s_in, v_tiles, s_mid, u_tiles, s_out, R)], T, x.dtype, x.device,
                              [bias], [residual])[0]
+    _refuse_trace("linear_forward")
     x, s_in, s_mid, s_out = (_stored(t) for t in (x, s_in, s_mid, s_out))
     y = torch.empty((T, M), dtype=x.dtype, device=x.device)
     if T == 0:

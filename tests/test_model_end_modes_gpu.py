@@ -75,6 +75,34 @@ def test_trace_records_a_quantised_linear():
             assert torch.equal(traced(y), lin(y))
 
 
+def test_trace_of_what_is_no_operator_is_refused():
+    """Launch groups, and linears with a bias or residual: a trace would hold constants, or memory that nobody fills."""
+    from tests.test_model_gpu import oc, fill
+    from nanoquant_b200 import ops
+    from nanoquant_b200.modules.group import LinearGroup
+    from nanoquant_b200.modules.linear import NanoQuantLinear
+
+    lins = []
+    for bias in (False, False, True):
+        lin = NanoQuantLinear(256, 128, 64, has_scale_mid=True)
+        fill(lin, oc.synth_linear(256, 64, 128, 2, seed=3))
+        lin = lin.cuda()
+        if bias:
+            lin.bias = torch.nn.Parameter(torch.randn(128, device="cuda").bfloat16(), requires_grad=False)
+        lin._prepare_kernel("gemv", torch.bfloat16)
+        lins.append(lin)
+    group = LinearGroup(lins[:2])
+    s_in, v, s_mid, u, s_out, rank, _ = lins[0].launch_operands()
+    x = torch.randn(2, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        for fn in (lambda x: lins[2](x), lambda x: group(x)[1], lambda x: ops.linear_forward(x, s_in, v, s_mid, u, s_out, rank),
+                   lambda x: ops.gemv_forward(x, s_in, v, s_mid, u, s_out, rank)):
+            assert torch.isfinite(fn(x)).all()
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                torch.jit.trace(fn, (x,))
+            assert torch.isfinite(fn(x)).all()
+
+
 @pytest.mark.parametrize("name", ["rms", "rms_plain", "layer", "quantize", "int8", "dense", "loss", "each", "chain"])
 def test_one_graph_under_torch_compile(name):
     from nanoquant_b200 import ops
