@@ -412,6 +412,74 @@ int nq_linear_ce_bwd(const void* h, const void* w, const void* targets, int targ
                      int dtype, nq_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
+ * Between the projections of a decoder layer: head norms and rotation, the paged cache, attention
+ * ------------------------------------------------------------------------ */
+
+/* Queries and keys of T tokens in ONE launch: an RMS norm over each head's D elements where there is a weight, x^ = x / sqrt(mean(x^2) + eps) w, then
+ * the rotation of the first R of them by the token's position p,
+ *     (a, b) -> (a cos - b sin, b cos + a sin) scaling,   angle = p inv_freq[i]   (formed and reduced in 64 bits)
+ * with elements (i, i + R/2) as pairs, or (2i, 2i + 1) where `interleaved`.  fp32 arithmetic, one rounding of the result.
+ * With a cache the keys (the same way) and the values (as they are) of token t go to position p of sequence `sequences[t]` (t itself where it is
+ * NULL): slot p % page_size of page block_table[sequence][p / page_size] of k_cache and v_cache.  A negative position is padding: nothing is stored, the
+ * query is zero.  What would lie outside the table or the cache is not stored.  Of tokens with the same place in one call any one's key, and any one's
+ * value, may stay.  Without a cache (k_cache NULL) keys go to k_out and there are no values.
+ * q, k, v: [T, heads, D] with the strides between tokens and heads in elements, multiples of 8, 16-byte aligned, D a multiple of 8 up to
+ * nq_head_max_columns(); q_out and k_out dense.  q, or k, may be NULL (with its heads 0).  inv_freq [R/2] fp32; R even, 0 (inv_freq unused) .. D.
+ * Weights in the heads' dtype or fp32.  Cache: 16-bit [pages, page_size, k_heads, D] by its strides (page, slot, head; multiples of 8), pages of
+ * 2^n >= 8 tokens.  block_table: int32, table_stride between rows.
+ * replaces: the q_norm / k_norm / apply_rotary_pos_emb calls and the StaticCache update of the HF model forward around the quantised projections
+ * (src/nanoquant/kernel/test_decode.py:385-422). */
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out, *k_out;
+    void *k_cache, *v_cache;
+    const void* positions;          /* T int32 or int64 (position_bits) */
+    const int32_t* sequences;
+    const int32_t* block_table;
+    const float* inv_freq;
+    const void *q_weight, *k_weight;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;             /* strides */
+    int64_t kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head;
+    int64_t table_stride, pages, T;
+    int position_bits, seqs, max_pages, page_size;
+    int q_heads, k_heads, D, R;
+    int interleaved, weight_dtype, dtype;
+    float eps, scaling;
+} nq_heads_desc;
+int nq_head_max_columns(void);
+int nq_heads_fwd(const nq_heads_desc* desc_host, nq_stream_t stream);
+
+/* Attention: o = sum_j p_j v_j with p = softmax(scale q . k_j) over the tokens j that a query sees, heads q_heads / k_heads of which share a key head.
+ * The query at place r of its sequence sees the tokens r - window < j <= r (window 0: no limit; without `causal` all of the sequence's j > r - window).
+ * A query that sees nothing gives zeros.  What lies outside its sequence (rows of other sequences, slots behind the last token) does not enter, whatever it
+ * holds.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type.
+ * A sequence that the table or the cache does not hold (a page outside the cache, a length beyond the table) is NaN in all its outputs.
+ *
+ * nq_paged_attention_fwd: one query per sequence, q [seqs, q_heads, D], at place lengths[s] - 1 of the `lengths[s]` tokens in the cache (0 or
+ * less: no token).  scratch: nq_paged_attention_scratch_bytes(), any contents, 16-byte aligned; up to the same order of sums for the same sizes and lengths.
+ * nq_prompt_attention_fwd: packed prompts, q [T, q_heads, D]; sequence s has the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32, not decreasing, seqs + 1
+ * of them).  Rows of no sequence are zeros.  Keys and values are packed likewise (k, v [Tk, k_heads, D] by cu_seqlens_k, NULL: cu_seqlens), or those in
+ * the cache, `lengths[s]` per sequence (block_table not NULL; k and v are then the cache).  The last row of a sequence is at the place of its last
+ * key: rows before the first key see nothing.  `status_word` as in nq_onebit_gemm_fwd.
+ * Strides, alignment, pages and block_table as in nq_heads_desc; out dense.
+ * replaces: the attention of the HF model forward between the quantised projections (src/nanoquant/kernel/test_decode.py:385-422). */
+typedef struct {
+    const void *q, *k, *v;
+    void* out;
+    const int32_t *cu_seqlens, *cu_seqlens_k, *lengths, *block_table;
+    int64_t q_token, q_head;                                               /* strides */
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;                /* (packed: k_slot and v_slot between tokens, k_page and v_page unused) */
+    int64_t table_stride, pages, T, Tk;
+    int seqs, max_pages, page_size;
+    int q_heads, k_heads, D;
+    int window, causal, dtype;
+    float scale;
+} nq_attention_desc;
+size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int D, int64_t max_tokens);
+int nq_paged_attention_fwd(const nq_attention_desc* desc_host, void* scratch, size_t scratch_bytes, nq_stream_t stream);
+int nq_prompt_attention_fwd(const nq_attention_desc* desc_host, void* status_word, nq_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
  * Measurement probes (no counterpart in the reference; nothing on the hot path calls them)
  * ------------------------------------------------------------------------ */
 

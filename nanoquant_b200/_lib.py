@@ -34,6 +34,23 @@ class LinearDesc(ctypes.Structure):
                 ("bias", c_void_p), ("residual", c_void_p), ("ldr", c_int64)]
 
 
+class HeadsDesc(ctypes.Structure):
+    """``nq_heads_desc``."""
+    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "q_out", "k_out", "k_cache", "v_cache", "positions", "sequences", "block_table", "inv_freq",
+                                        "q_weight", "k_weight")] + \
+               [(n, c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "kc_page", "kc_slot", "kc_head", "vc_page", "vc_slot", "vc_head",
+                                       "table_stride", "pages", "T")] + \
+               [(n, c_int) for n in ("position_bits", "seqs", "max_pages", "page_size", "q_heads", "k_heads", "D", "R", "interleaved", "weight_dtype", "dtype")] + \
+               [("eps", ctypes.c_float), ("scaling", ctypes.c_float)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """``nq_attention_desc``."""
+    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "out", "cu_seqlens", "cu_seqlens_k", "lengths", "block_table")] + \
+               [(n, c_int64) for n in ("q_token", "q_head", "k_page", "k_slot", "k_head", "v_page", "v_slot", "v_head", "table_stride", "pages", "T", "Tk")] + \
+               [(n, c_int) for n in ("seqs", "max_pages", "page_size", "q_heads", "k_heads", "D", "window", "causal", "dtype")] + [("scale", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/nanoquant_b200.h
 SIGNATURES = {
     "nq_abi_version": (c_int, []),
@@ -86,6 +103,11 @@ SIGNATURES = {
     "nq_linear_ce_bwd_scratch_bytes": (c_size_t, [c_int64] * 3),
     "nq_linear_ce_bwd": (c_int, [c_void_p] * 3 + [c_int, c_int64] + [c_void_p] * 3 + [c_int64] + [c_void_p] * 3 + [c_size_t, c_void_p] +
                          [c_int64] * 7 + [c_int, c_int, c_void_p]),
+    "nq_head_max_columns": (c_int, []),
+    "nq_heads_fwd": (c_int, [ctypes.POINTER(HeadsDesc), c_void_p]),
+    "nq_paged_attention_scratch_bytes": (c_size_t, [c_int] * 4 + [c_int64]),
+    "nq_paged_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_size_t, c_void_p]),
+    "nq_prompt_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_void_p]),
     "nq_gemv_max_tokens": (c_int, []),
     "nq_linear_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "nq_linear_fwd": (c_int, [c_void_p] * 8 + [c_size_t, c_int, c_int, c_int, c_int, c_int, c_void_p]),

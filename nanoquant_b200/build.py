@@ -21,7 +21,7 @@ EXT_SOURCE = "nq_torch.cpp"
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 
 SOURCES = ["nq_core.cu", "nq_pack.cu", "nq_gemv.cu", "nq_gemm.cu", "nq_wgemm.cu", "nq_pgemm.cu", "nq_batch.cu", "nq_comm.cu", "nq_dense.cu", "nq_probe.cu",
-           "nq_norm.cu", "nq_int8.cu", "nq_loss.cu"]
+           "nq_norm.cu", "nq_int8.cu", "nq_loss.cu", "nq_heads.cu", "nq_paged.cu", "nq_prompt.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

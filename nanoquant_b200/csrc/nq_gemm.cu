@@ -162,6 +162,22 @@ int mm_encode_columns(CUtensorMap* map, const void* p, int type, int64_t inner, 
     return mm_encode_box(map, p, type, dims, strides, box);
 }
 
+int mm_encode_heads(CUtensorMap* map, const void* p, int type, const HeadSizes& sizes, const HeadStrides& strides, const HeadBox& box) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return NQ_ERR_UNSUPPORTED;
+    cuuint64_t n[4], bytes[3];
+    cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 4; ++i) {
+        n[i] = (cuuint64_t)sizes.n[i];
+        b[i] = (cuuint32_t)box.n[i];
+    }
+    // (the stride of a single element means nothing, but has to be a valid one)
+    for (int i = 0; i < 3; ++i) bytes[i] = n[i + 1] == 1 ? (cuuint64_t)(sizes.n[0] * 2) : (cuuint64_t)strides.n[i] * 2;
+    const CUresult r = enc(map, type == kMmBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), n, bytes, b, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? NQ_OK : NQ_ERR_UNSUPPORTED;
+}
+
 // The kernel of a stage, with its plan.  (An intermediate in the GEMMs' column order is theirs.)
 static int pick_kernel(const StageJob* jobs, int n, int T, int order, WgemmPlan& w, PgemmPlan& p) {
     if (order == 0 && T <= batch_max_tokens(jobs, n)) return NQ_KERNEL_BATCH;

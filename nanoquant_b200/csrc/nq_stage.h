@@ -75,5 +75,10 @@ enum : int { kMmF16 = 0, kMmBf16 = 1, kMmS8 = 2 };
 int mm_encode(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int box_inner, int box_outer);
 // The same matrix as [inner / 64][outer][64], for one load of `boxes` columns of 64 x 64 elements (inner a multiple of 64).
 int mm_encode_columns(CUtensorMap* map, const void* p, int type, int64_t inner, int64_t outer, int64_t stride, int boxes);
+// A tensor of 16-bit heads: sizes from the inner (contiguous) one on, strides of the outer three in elements, 128-byte swizzle.
+struct HeadSizes { int64_t n[4]; };
+struct HeadStrides { int64_t n[3]; };
+struct HeadBox { int n[4]; };
+int mm_encode_heads(CUtensorMap* map, const void* p, int type, const HeadSizes& sizes, const HeadStrides& strides, const HeadBox& box);
 
 }  // namespace nq

@@ -912,6 +912,286 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// between the projections of a decoder layer: head norms and rotation, the paged cache, attention
+// ---------------------------------------------------------------------------------------------------------------
+// Heads [..., heads, D] as the kernels read them: 16-bit elements, D a multiple of 8 and dense, heads and tokens (evenly spaced) multiples of 8 elements apart,
+// a 16-byte boundary.  False: not so.
+struct Heads {
+    int64_t tokens, heads, D, token, head;
+};
+bool as_heads(const Tensor& t, Heads& h) {
+    const int64_t n = t.dim();
+    if (n < 2 || !is_16bit(t.scalar_type())) return false;
+    h.D = t.size(n - 1);
+    h.heads = t.size(n - 2);
+    if (h.D == 0 || h.D % 8 != 0 || h.D > nq_head_max_columns() || h.heads == 0 || t.stride(n - 1) != 1 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15)) return false;
+    h.head = h.heads > 1 ? t.stride(n - 2) : h.D;
+    h.tokens = 1;
+    h.token = h.head * h.heads;
+    int64_t next = -1;
+    for (int64_t k = n - 3; k >= 0; --k) {
+        if (t.size(k) == 1) continue;
+        if (next < 0) h.token = t.stride(k);
+        else if (t.stride(k) != next) return false;
+        next = t.stride(k) * t.size(k);
+        h.tokens *= t.size(k);
+    }
+    return h.head >= h.D && h.head % 8 == 0 && h.token >= h.D && h.token % 8 == 0;
+}
+bool is_index(const Tensor& t, at::ScalarType type, int64_t dim, int dev) {
+    return t.scalar_type() == type && t.dim() == dim && t.get_device() == dev && (dim == 0 || t.size(dim - 1) <= 1 || t.stride(dim - 1) == 1) && t.numel() > 0;
+}
+// A cache [pages, page_size, heads, D], and the table that leads to its pages.
+bool cache_takes(const Tensor& k, const Tensor& v, const Tensor& table, const Heads& h, at::ScalarType type, int dev) {
+    if (k.dim() != 4 || v.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != type || v.scalar_type() != type || k.get_device() != dev || v.get_device() != dev ||
+        k.size(2) != h.heads || k.size(3) != h.D || k.numel() == 0 || !is_index(table, at::kInt, 2, dev))
+        return false;
+    const int64_t page = k.size(1);
+    if (page < 8 || (page & (page - 1)) != 0 || (table.size(0) > 1 && table.stride(0) < table.size(1))) return false;
+    for (const Tensor* t : {&k, &v}) {
+        if (t->stride(3) != 1 || (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15)) return false;
+        for (int i = 0; i < 3; ++i)
+            if (t->size(i) > 1 && (t->stride(i) % 8 != 0 || t->stride(i) < h.D)) return false;
+    }
+    return true;
+}
+int64_t cache_stride(const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : t.size(3); }
+const void* data(const Tensor* t) { return t ? t->const_data_ptr() : nullptr; }
+
+struct HeadsArgs {
+    const Tensor *q, *k, *v, *k_cache, *v_cache, *table, *positions, *sequences, *inv_freq, *wq, *wk;
+    double eps, scaling;
+    bool interleaved;
+};
+bool heads_takes(const HeadsArgs& a) {
+    Heads q{}, k{}, v{};
+    const Tensor& first = a.q ? *a.q : *a.k;
+    const int dev = first.get_device();
+    const at::ScalarType type = first.scalar_type();
+    if (!as_heads(*a.k, k) || (a.q && !as_heads(*a.q, q)) || (a.v && !as_heads(*a.v, v))) return false;
+    for (const Tensor* t : {a.q, a.k, a.v})
+        if (t && (t->scalar_type() != type || t->get_device() != dev || t->size(-1) != k.D)) return false;
+    const Tensor& p = *a.positions;
+    if (p.get_device() != dev || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || !p.is_contiguous()) return false;
+    for (const Tensor* t : {a.q, a.k, a.v})
+        if (t && t->sizes().slice(0, t->dim() - 2) != p.sizes()) return false;
+    if (a.inv_freq && (a.inv_freq->scalar_type() != at::kFloat || a.inv_freq->dim() != 1 || !a.inv_freq->is_contiguous() || a.inv_freq->get_device() != dev || 2 * a.inv_freq->size(0) > k.D))
+        return false;
+    if (a.wq && !a.q) return false;
+    const Tensor* any = a.wq ? a.wq : a.wk;
+    for (const Tensor* w : {a.wq, a.wk})
+        if (w && ((w->scalar_type() != type && w->scalar_type() != at::kFloat) || w->scalar_type() != any->scalar_type() || w->dim() != 1 || w->size(0) != k.D || !w->is_contiguous() ||
+                  w->get_device() != dev || (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15)))
+            return false;
+    if (!a.k_cache) return true;
+    if (v.heads != k.heads || !cache_takes(*a.k_cache, *a.v_cache, *a.table, k, type, dev)) return false;
+    return a.sequences ? a.sequences->sizes() == p.sizes() && a.sequences->scalar_type() == at::kInt && a.sequences->is_contiguous() && a.sequences->get_device() == dev : true;
+}
+// (q', k'), undefined where there is none
+std::array<Tensor, 2> heads_launch(const HeadsArgs& a) {
+    Heads q{}, k{}, v{};
+    as_heads(*a.k, k);
+    if (a.q) as_heads(*a.q, q);
+    if (a.v) as_heads(*a.v, v);
+    std::array<Tensor, 2> out;
+    if (a.q) out[0] = new_output(a.q->sizes(), *a.q);
+    if (!a.k_cache) out[1] = new_output(a.k->sizes(), *a.k);
+    if (a.positions->numel() == 0) return out;
+    nq_heads_desc d{};
+    d.q = data(a.q); d.k = data(a.k); d.v = data(a.v);
+    d.q_out = a.q ? out[0].mutable_data_ptr() : nullptr;
+    d.k_out = a.k_cache ? nullptr : out[1].mutable_data_ptr();
+    d.positions = data(a.positions);
+    d.inv_freq = a.inv_freq && a.inv_freq->numel() ? static_cast<const float*>(data(a.inv_freq)) : nullptr;
+    d.q_weight = data(a.wq); d.k_weight = data(a.wk);
+    d.q_token = q.token; d.q_head = q.head; d.k_token = k.token; d.k_head = k.head; d.v_token = v.token; d.v_head = v.head;
+    d.T = a.positions->numel();
+    d.position_bits = a.positions->scalar_type() == at::kLong ? 64 : 32;
+    d.q_heads = (int)q.heads; d.k_heads = (int)k.heads; d.D = (int)k.D;
+    d.R = a.inv_freq ? 2 * (int)a.inv_freq->size(0) : 0;
+    d.interleaved = a.interleaved;
+    d.dtype = dtype_id(a.k->scalar_type());
+    const Tensor* w = a.wq ? a.wq : a.wk;
+    d.weight_dtype = w && w->scalar_type() == at::kFloat ? (int)NQ_F32 : d.dtype;
+    d.eps = (float)a.eps; d.scaling = (float)a.scaling;
+    if (a.k_cache) {
+        const Tensor &kc = *a.k_cache, &vc = *a.v_cache;
+        d.k_cache = kc.mutable_data_ptr(); d.v_cache = vc.mutable_data_ptr();
+        d.sequences = static_cast<const int32_t*>(data(a.sequences));
+        d.block_table = static_cast<const int32_t*>(data(a.table));
+        d.kc_page = cache_stride(kc, 0); d.kc_slot = cache_stride(kc, 1); d.kc_head = cache_stride(kc, 2);
+        d.vc_page = cache_stride(vc, 0); d.vc_slot = cache_stride(vc, 1); d.vc_head = cache_stride(vc, 2);
+        d.table_stride = a.table->size(0) > 1 ? a.table->stride(0) : a.table->size(1);
+        d.pages = kc.size(0); d.page_size = (int)kc.size(1);
+        d.seqs = (int)a.table->size(0); d.max_pages = (int)a.table->size(1);
+    }
+    const int dev = a.k->get_device();
+    OnDevice on(dev);
+    const int st = nq_heads_fwd(&d, stream_of(dev));
+    if (st < 0) fail(st, "nq_heads_fwd");
+    for (const Tensor* c : {a.k_cache, a.v_cache})
+        if (c && !c->is_inference()) c->unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+// Whether autograd would record the call: there is no gradient to record.
+bool wants_gradient(std::initializer_list<const Tensor*> inputs) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : inputs)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+// An argument that may be None; false: neither that nor a plain tensor.
+bool maybe(PyObject* o, const Tensor*& t) {
+    t = o == Py_None ? nullptr : plain(o);
+    return t || o == Py_None;
+}
+// qk_norm_rope(q, k, positions, inv_freq, q_weight | None, k_weight | None, eps, interleaved, scaling) -> (q, k) or None
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 9, "qk_norm_rope takes 9 arguments");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    HeadsArgs h{};
+    h.q = plain(a[0]); h.k = plain(a[1]); h.positions = plain(a[2]); h.inv_freq = plain(a[3]);
+    if (!h.q || !h.k || !h.positions || !h.inv_freq || !maybe(a[4], h.wq) || !maybe(a[5], h.wk) || wants_gradient({h.q, h.k, h.inv_freq, h.wq, h.wk}) || !heads_takes(h)) Py_RETURN_NONE;
+    h.eps = PyFloat_AsDouble(a[6]);
+    h.interleaved = PyObject_IsTrue(a[7]) == 1;
+    h.scaling = PyFloat_AsDouble(a[8]);
+    if (PyErr_Occurred()) return nullptr;
+    refuse_tangents("qk_norm_rope", {h.q, h.k, h.inv_freq, h.wq, h.wk});
+    const auto out = heads_launch(h);
+    PyObject* q = THPVariable_Wrap(out[0]);
+    PyObject* k = q ? THPVariable_Wrap(out[1]) : nullptr;
+    return k ? Py_BuildValue("(NN)", q, k) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+// append_kv(q | None, k, v, k_cache, v_cache, block_table, positions, sequences | None, inv_freq | None, q_weight | None, k_weight | None, eps, interleaved, scaling) -> q,
+// True (there is none), or None
+PyObject* py_append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 14, "append_kv takes 14 arguments");
+    if (!exact_plain(a[1])) Py_RETURN_NONE;
+    HeadsArgs h{};
+    h.k = plain(a[1]); h.v = plain(a[2]); h.k_cache = plain(a[3]); h.v_cache = plain(a[4]); h.table = plain(a[5]); h.positions = plain(a[6]);
+    if (!maybe(a[0], h.q) || !h.k || !h.v || !h.k_cache || !h.v_cache || !h.table || !h.positions || !maybe(a[7], h.sequences) || !maybe(a[8], h.inv_freq) || !maybe(a[9], h.wq) ||
+        !maybe(a[10], h.wk) || wants_gradient({h.q, h.k, h.v, h.k_cache, h.v_cache, h.inv_freq, h.wq, h.wk}) || !heads_takes(h))
+        Py_RETURN_NONE;
+    h.eps = PyFloat_AsDouble(a[11]);
+    h.interleaved = PyObject_IsTrue(a[12]) == 1;
+    h.scaling = PyFloat_AsDouble(a[13]);
+    if (PyErr_Occurred()) return nullptr;
+    refuse_tangents("append_kv", {h.q, h.k, h.v, h.k_cache, h.v_cache, h.inv_freq, h.wq, h.wk});
+    const auto out = heads_launch(h);
+    if (!h.q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(out[0]);
+    END_HANDLE_TH_ERRORS
+}
+
+struct AttentionArgs {
+    const Tensor *q, *k, *v, *cu, *cu_k, *table, *lengths;
+    double scale;
+    int64_t window;
+    bool causal;
+};
+bool attention_takes(const AttentionArgs& a) {
+    Heads q, k, v;
+    const int dev = a.q->get_device();
+    const at::ScalarType type = a.q->scalar_type();
+    if (a.q->dim() != 3 || !as_heads(*a.q, q)) return false;
+    if (a.table) {
+        if (a.k->dim() != 4) return false;
+        k = Heads{0, a.k->size(2), q.D, 0, 0};
+        if (!cache_takes(*a.k, *a.v, *a.table, k, type, dev) || !is_index(*a.lengths, at::kInt, 1, dev) || a.lengths->size(0) != a.table->size(0)) return false;
+    } else {
+        if (a.k->dim() != 3 || !as_heads(*a.k, k) || !as_heads(*a.v, v) || a.k->sizes() != a.v->sizes() || k.D != q.D || k.tokens == 0) return false;
+        for (const Tensor* t : {a.k, a.v})
+            if (t->scalar_type() != type || t->get_device() != dev) return false;
+    }
+    if (q.heads % k.heads != 0) return false;
+    if (!a.cu) return a.lengths->size(0) == a.q->size(0);
+    const int64_t seqs = a.cu->size(0) - 1;
+    if (q.heads / k.heads > 128 || !is_index(*a.cu, at::kInt, 1, dev) || seqs < 1 || (a.cu_k && (!is_index(*a.cu_k, at::kInt, 1, dev) || a.cu_k->size(0) != seqs + 1))) return false;
+    return !a.table || a.table->size(0) == seqs;
+}
+Tensor attention_launch(const AttentionArgs& a) {
+    Heads q, k, v;
+    as_heads(*a.q, q);
+    Tensor out = new_output(a.q->sizes(), *a.q);
+    if (a.q->size(0) == 0) return out;
+    nq_attention_desc d{};
+    d.q = data(a.q); d.k = data(a.k); d.v = data(a.v);
+    d.out = out.mutable_data_ptr();
+    d.cu_seqlens = static_cast<const int32_t*>(data(a.cu));
+    d.cu_seqlens_k = static_cast<const int32_t*>(data(a.cu_k));
+    d.lengths = static_cast<const int32_t*>(data(a.lengths));
+    d.block_table = static_cast<const int32_t*>(data(a.table));
+    d.q_token = q.token; d.q_head = q.head;
+    d.T = a.q->size(0);
+    d.q_heads = (int)q.heads; d.D = (int)q.D;
+    d.window = (int)a.window; d.causal = a.causal; d.scale = (float)a.scale;
+    d.dtype = dtype_id(a.q->scalar_type());
+    d.seqs = (int)(a.cu ? a.cu->size(0) - 1 : a.q->size(0));
+    if (a.table) {
+        d.k_page = cache_stride(*a.k, 0); d.k_slot = cache_stride(*a.k, 1); d.k_head = cache_stride(*a.k, 2);
+        d.v_page = cache_stride(*a.v, 0); d.v_slot = cache_stride(*a.v, 1); d.v_head = cache_stride(*a.v, 2);
+        d.table_stride = a.table->size(0) > 1 ? a.table->stride(0) : a.table->size(1);
+        d.pages = a.k->size(0); d.page_size = (int)a.k->size(1); d.k_heads = (int)a.k->size(2);
+        d.max_pages = (int)a.table->size(1);
+    } else {
+        as_heads(*a.k, k);
+        as_heads(*a.v, v);
+        d.k_slot = k.token; d.k_head = k.head; d.v_slot = v.token; d.v_head = v.head;
+        d.Tk = k.tokens; d.k_heads = (int)k.heads;
+    }
+    const int dev = a.q->get_device();
+    OnDevice on(dev);
+    int st;
+    if (a.cu) {
+        st = nq_prompt_attention_fwd(&d, status_header(dev), stream_of(dev));
+        if (st < 0) fail(st, "nq_prompt_attention_fwd");
+    } else {
+        const size_t bytes = nq_paged_attention_scratch_bytes(d.seqs, d.q_heads, d.k_heads, d.D, (int64_t)d.max_pages * d.page_size);
+        const Tensor scratch = bytes ? new_bytes((int64_t)bytes, *a.q) : Tensor();
+        st = nq_paged_attention_fwd(&d, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, stream_of(dev));
+        if (st < 0) fail(st, "nq_paged_attention_fwd");
+    }
+    return out;
+}
+// prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k | None, block_table | None, lengths | None, causal, scale, window) -> o or None
+PyObject* py_prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 10, "prompt_attention takes 10 arguments");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    AttentionArgs t{};
+    t.q = plain(a[0]); t.k = plain(a[1]); t.v = plain(a[2]); t.cu = plain(a[3]);
+    if (!t.q || !t.k || !t.v || !t.cu || !maybe(a[4], t.cu_k) || !maybe(a[5], t.table) || !maybe(a[6], t.lengths) || !t.table != !t.lengths || (t.table && t.cu_k) ||
+        wants_gradient({t.q, t.k, t.v}) || !attention_takes(t))
+        Py_RETURN_NONE;
+    t.causal = PyObject_IsTrue(a[7]) == 1;
+    t.scale = PyFloat_AsDouble(a[8]);
+    t.window = PyLong_AsLongLong(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    refuse_tangents("prompt_attention", {t.q, t.k, t.v});
+    return THPVariable_Wrap(attention_launch(t));
+    END_HANDLE_TH_ERRORS
+}
+// paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window) -> o or None
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 7, "paged_attention takes 7 arguments");
+    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    AttentionArgs t{};
+    t.q = plain(a[0]); t.k = plain(a[1]); t.v = plain(a[2]); t.table = plain(a[3]); t.lengths = plain(a[4]);
+    t.causal = true;
+    if (!t.q || !t.k || !t.v || !t.table || !t.lengths || wants_gradient({t.q, t.k, t.v}) || !attention_takes(t)) Py_RETURN_NONE;
+    t.scale = PyFloat_AsDouble(a[5]);
+    t.window = PyLong_AsLongLong(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    refuse_tangents("paged_attention", {t.q, t.k, t.v});
+    return THPVariable_Wrap(attention_launch(t));
+    END_HANDLE_TH_ERRORS
+}
+
 // The same as operators of the dispatcher, for what records calls (torch.compile, torch.jit.trace); schemas, shapes for tracing and derivatives: nanoquant_b200/ops.py.
 Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
 OptTensor dense(const OptTensor& t) { return t ? OptTensor(dense(*t)) : t; }
@@ -978,8 +1258,57 @@ std::tuple<Tensor, Tensor> op_linear_cross_entropy_backward(const Tensor& grad, 
     const auto d = loss_gradients(grad, h, w, t, lse, count, LossArgs{ignore, (int)reduction}, want);
     return {or_none(d[0], h), or_none(d[1], h)};
 }
+// Heads that the kernels do not read in place are copied.
+Tensor heads_in_place(const Tensor& t_) {
+    const Tensor t = t_.resolve_neg();
+    Heads h;
+    return as_heads(t, h) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+OptTensor heads_in_place(const OptTensor& t) { return t ? OptTensor(heads_in_place(*t)) : t; }
+Tensor at_boundary(const Tensor& t_) {
+    const Tensor t = dense(t_);
+    return reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15 ? t.clone() : t;
+}
+OptTensor at_boundary(const OptTensor& t) { return t ? OptTensor(at_boundary(*t)) : t; }
+std::tuple<Tensor, Tensor> op_qk_norm_rope(const Tensor& q_, const Tensor& k_, const Tensor& p_, const Tensor& f_, const OptTensor& wq_, const OptTensor& wk_, double eps, bool interleaved,
+                                           double scaling) {
+    const Tensor q = heads_in_place(q_), k = heads_in_place(k_), p = dense(p_), f = dense(f_);
+    const OptTensor wq = at_boundary(wq_), wk = at_boundary(wk_);
+    const HeadsArgs a{&q, &k, nullptr, nullptr, nullptr, nullptr, &p, nullptr, &f, pointer(wq), pointer(wk), eps, scaling, interleaved};
+    TORCH_CHECK(heads_takes(a), "nanoquant_b200::qk_norm_rope: 16-bit heads of one type and size, a position for each token, fp32 frequencies");
+    const auto out = heads_launch(a);
+    return {out[0], out[1]};
+}
+Tensor op_append_kv(const OptTensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& p_, const OptTensor& s_,
+                    const OptTensor& f_, const OptTensor& wq_, const OptTensor& wk_, double eps, bool interleaved, double scaling) {
+    const OptTensor q = heads_in_place(q_), s = dense(s_), f = dense(f_), wq = at_boundary(wq_), wk = at_boundary(wk_);
+    const Tensor k = heads_in_place(k_), v = heads_in_place(v_), table = dense(table_), p = dense(p_);
+    const HeadsArgs a{pointer(q), &k, &v, &kc, &vc, &table, &p, pointer(s), pointer(f), pointer(wq), pointer(wk), eps, scaling, interleaved};
+    TORCH_CHECK(!kc.is_neg() && !vc.is_neg() && heads_takes(a),
+                "nanoquant_b200::append_kv: 16-bit heads of one type and size, a cache [pages, page_size, heads, D] of them, an int32 table of pages, a position for each token");
+    return or_none(heads_launch(a)[0], k);
+}
+Tensor op_prompt_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_, const OptTensor& cu_k_, const OptTensor& table_, const OptTensor& lengths_, bool causal,
+                           double scale, int64_t window) {
+    const Tensor q = heads_in_place(q_), k = table_ ? k_.resolve_neg() : heads_in_place(k_), v = table_ ? v_.resolve_neg() : heads_in_place(v_), cu = dense(cu_);
+    const OptTensor cu_k = dense(cu_k_), table = dense(table_), lengths = dense(lengths_);
+    const AttentionArgs a{&q, &k, &v, &cu, pointer(cu_k), pointer(table), pointer(lengths), scale, window, causal};
+    TORCH_CHECK(!table_.has_value() == !lengths_.has_value() && !(table_ && cu_k_) && attention_takes(a),
+                "nanoquant_b200::prompt_attention: 16-bit heads of one type and size, packed or in a cache with its table and lengths, int32 starts of the sequences");
+    return attention_launch(a);
+}
+Tensor op_paged_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& table_, const Tensor& lengths_, double scale, int64_t window) {
+    const Tensor q = heads_in_place(q_), k = k_.resolve_neg(), v = v_.resolve_neg(), table = dense(table_), lengths = dense(lengths_);
+    const AttentionArgs a{&q, &k, &v, nullptr, nullptr, &table, &lengths, scale, window, true};
+    TORCH_CHECK(attention_takes(a), "nanoquant_b200::paged_attention: 16-bit heads of one type and size, a cache [pages, page_size, heads, D], an int32 table of pages and lengths");
+    return attention_launch(a);
+}
 TORCH_LIBRARY_IMPL(nanoquant_b200, CUDA, m) {
     m.impl("norm", op_norm);
+    m.impl("qk_norm_rope", op_qk_norm_rope);
+    m.impl("append_kv", op_append_kv);
+    m.impl("prompt_attention", op_prompt_attention);
+    m.impl("paged_attention", op_paged_attention);
     m.impl("norm_backward", op_norm_backward);
     m.impl("quantize_rows", op_quantize_rows);
     m.impl("int8_linear", op_int8_linear);
@@ -1112,6 +1441,10 @@ PyMethodDef kMethods[] = {
     {"quantize_rows", (PyCFunction)(void*)py_quantize_rows, METH_FASTCALL, nullptr},
     {"int8_linear_forward", (PyCFunction)(void*)py_int8_linear_forward, METH_FASTCALL, nullptr},
     {"linear_cross_entropy", (PyCFunction)(void*)py_linear_cross_entropy, METH_FASTCALL, nullptr},
+    {"qk_norm_rope", (PyCFunction)(void*)py_qk_norm_rope, METH_FASTCALL, nullptr},
+    {"append_kv", (PyCFunction)(void*)py_append_kv, METH_FASTCALL, nullptr},
+    {"prompt_attention", (PyCFunction)(void*)py_prompt_attention, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void*)py_paged_attention, METH_FASTCALL, nullptr},
     {"repack", (PyCFunction)(void*)py_repack, METH_FASTCALL, nullptr},
     {"pack_rows", (PyCFunction)(void*)py_pack_rows, METH_FASTCALL, nullptr},
     {"words_to", (PyCFunction)(void*)py_words_to, METH_FASTCALL, nullptr},

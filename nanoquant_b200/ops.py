@@ -399,6 +399,260 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     return loss.reshape(targets.shape) if reduction == "none" else loss
 
 
+# --- between the projections of a decoder layer: head norms and rotation, the paged cache, attention ---
+
+def _no_gradient(what: str, *inputs) -> None:
+    """The quantised linears around these calls have no backward pass, and neither have they: a call that autograd would record is refused."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or with inputs that need none")
+
+
+def _check_heads(t, name: str, like=None, heads=None) -> None:
+    _check_16bit(t, name)
+    if t.dim() < 2 or t.size(-1) == 0 or t.size(-2) == 0 or t.size(-1) % 8 or t.size(-1) > _HEAD_MAX_COLUMNS:
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected [..., heads, D] with D a multiple of 8 up to {_HEAD_MAX_COLUMNS}")
+    if like is not None:
+        _check_like(t, name, like, (like.dtype,), (*like.shape[:-2], t.size(-2) if heads is None else heads, like.size(-1)))
+
+
+def _check_index(t, name: str, like, dtypes, shape) -> None:
+    if t is None:
+        raise RuntimeError(f"{name} is missing")
+    _check_like(t, name, like, dtypes, shape)
+
+
+def _check_cache(k_cache, v_cache, block_table, like, heads=None) -> None:
+    """A cache ``[pages, page_size, heads, D]`` that is read and written in place, and its table."""
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _check_16bit(t, name)
+        if t.dim() != 4 or t.numel() == 0:
+            raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected [pages, page_size, heads, D]")
+        _check_like(t, name, like, (like.dtype,), (*t.shape[:2], t.size(2) if heads is None else heads, like.size(-1)))
+        page = t.size(1)
+        if page < 8 or page & (page - 1):
+            raise RuntimeError(f"{name} has pages of {page} tokens, expected a power of two from 8 on")
+        if t.stride(3) != 1 or any(t.size(i) > 1 and (t.stride(i) % 8 or t.stride(i) < t.size(3)) for i in range(3)) or \
+                (not _recorded() and (t.is_neg() or t.data_ptr() % 16)):
+            raise RuntimeError(f"{name} is used in place: dense heads at multiples of 8 elements, from a 16-byte boundary on")
+    if k_cache.shape != v_cache.shape:
+        raise RuntimeError(f"k_cache has shape {tuple(k_cache.shape)}, v_cache {tuple(v_cache.shape)}")
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 or block_table.numel() == 0:
+        raise RuntimeError("block_table must be a CUDA [sequences, pages] matrix of int32")
+    _check_like(block_table, "block_table", like, (torch.int32,), block_table.shape)
+
+
+def _check_turn(like, inv_freq, q_weight, k_weight) -> None:
+    D = like.size(-1)
+    if inv_freq is not None:
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1 or 2 * inv_freq.size(0) > D:
+            raise RuntimeError(f"inv_freq must be a CUDA vector of at most {D // 2} fp32 frequencies")
+        _check_like(inv_freq, "inv_freq", like, (torch.float32,), inv_freq.shape)
+    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _check_like(t, name, like, (like.dtype, torch.float32), (D,))
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise RuntimeError("q_weight and k_weight must be of one type")
+
+
+_INT = (torch.int32, torch.int64)
+_HEAD_MAX_COLUMNS = 256         # nq_head_max_columns()
+_WINDOW_MOST = 1 << 30          # beyond any sequence
+
+
+def _scale_of(scale, D: int) -> float:
+    if scale is None:
+        return D ** -0.5
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"scale should be positive, but {scale} was given")
+    return float(scale)
+
+
+def _window_of(window) -> int:
+    if window is None:
+        return 0
+    if window < 1:
+        raise ValueError(f"window should be at least 1, or None, but {window} was given")
+    return min(int(window), _WINDOW_MOST)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False, scaling: float = 1.0):
+    """Queries and keys behind their projections, ``(q', k')`` in one launch (``nq_heads_fwd``): an RMS norm of each head where there is a weight,
+    then the rotation by the token's position.
+
+    ``q`` ``[..., heads, D]`` and ``k`` ``[..., key heads, D]`` fp16 / bf16 with the same leading dimensions (views of a launch group's outputs are read in
+    place), D a multiple of 8 up to 256; ``positions`` ``[...]`` int64 or int32, any values; ``inv_freq`` ``[R / 2]`` fp32, the model's frequencies:
+    the first R of the D elements are rotated by ``position * inv_freq[i]`` (in 64 bits), elements ``(i, i + R/2)`` as pairs, or with ``interleaved``
+    ``(2i, 2i + 1)``, and multiplied by ``scaling``.  ``q_weight`` and ``k_weight`` ``[D]`` in the type of the heads or fp32; without one there is no
+    norm.  fp32 arithmetic, one rounding.  Inference: no gradient."""
+    if not torch.compiler.is_compiling():
+        r = _lib.ext().qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, scaling)
+        if r is not None:
+            return r
+    _check_heads(q, "q")
+    _check_heads(k, "k", q)
+    _check_index(positions, "positions", q, _INT, q.shape[:-2])
+    _check_index(inv_freq, "inv_freq", q, (torch.float32,), getattr(inv_freq, "shape", ()))
+    _check_turn(q, inv_freq, q_weight, k_weight)
+    _no_gradient("qk_norm_rope", q, k, inv_freq, q_weight, k_weight)
+    args = (positions, inv_freq, q_weight, k_weight)
+    if _recorded():
+        return torch.ops.nanoquant_b200.qk_norm_rope(q, k, *args, eps, interleaved, scaling)
+    r = _lib.ext().qk_norm_rope(_heads_in_place(q), _heads_in_place(k), *(_at_boundary(t) for t in args), eps, interleaved, scaling)
+    if r is None:
+        raise _not_plain("qk_norm_rope")
+    return r
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
+              sequences: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+              q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+              scaling: float = 1.0) -> Optional[torch.Tensor]:
+    """Keys, normed and rotated on the way as in :func:`qk_norm_rope`, and values of new tokens into a paged cache, in place; with ``q`` the
+    queries are normed and rotated in the same launch and returned (``nq_heads_fwd``).
+
+    ``k`` and ``v`` ``[..., key heads, D]``; ``k_cache`` and ``v_cache`` ``[pages, page_size, key heads, D]`` (pages of 8, 16, 32, ... tokens; any order of the
+    dimensions in memory but the last); ``block_table`` ``[sequences, n]`` int32.  Token t goes to ``positions[t]`` of sequence ``sequences[t]`` (int32; left
+    out: token t is one of sequence t): slot ``positions[t] % page_size`` of page ``block_table[sequence, positions[t] // page_size]``.  A negative position
+    is padding: nothing is stored, its query is zero.  What lies outside the table or the cache is not stored (attention over such a sequence is
+    NaN).  The places of one call have to differ.  Without ``inv_freq`` nothing is rotated.  Inference: no gradient."""
+    args = (block_table, positions, sequences, inv_freq, q_weight, k_weight)
+    if not torch.compiler.is_compiling():
+        r = _lib.ext().append_kv(q, k, v, k_cache, v_cache, *args, eps, interleaved, scaling)
+        if r is not None:
+            return None if q is None else r
+    _check_heads(k, "k")
+    _check_heads(v, "v", k, k.size(-2))
+    if q is not None:
+        _check_heads(q, "q", k)
+    elif q_weight is not None:
+        raise RuntimeError("q_weight needs q")
+    _check_cache(k_cache, v_cache, block_table, k, k.size(-2))
+    _check_index(positions, "positions", k, _INT, k.shape[:-2])
+    if sequences is not None:
+        _check_like(sequences, "sequences", k, (torch.int32,), positions.shape)
+    _check_turn(k, inv_freq, q_weight, k_weight)
+    _no_gradient("append_kv", q, k, v, k_cache, v_cache, inv_freq, q_weight, k_weight)
+    if _recorded():
+        r = torch.ops.nanoquant_b200.append_kv(q, k, v, k_cache, v_cache, *args, eps, interleaved, scaling)
+    else:
+        r = _lib.ext().append_kv(_heads_in_place(q), _heads_in_place(k), _heads_in_place(v), k_cache, v_cache, *(_at_boundary(t) for t in args), eps, interleaved, scaling)
+        if r is None:
+            raise _not_plain("append_kv")
+    return None if q is None else r
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, cu_seqlens_k: Optional[torch.Tensor] = None,
+                     block_table: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, causal: bool = True,
+                     scale: Optional[float] = None, window: Optional[int] = None) -> torch.Tensor:
+    """Attention of packed prompts of different lengths, ``[T, heads, D]`` (``nq_prompt_attention_fwd``).
+
+    ``q`` ``[T, heads, D]`` fp16 / bf16, the tokens of sequence s in rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` (int32, ``[sequences + 1]``, not
+    decreasing); rows of no sequence come back as zeros.  ``k`` and ``v`` ``[Tk, key heads, D]``, packed by ``cu_seqlens_k`` (left out: as the queries);
+    or, with ``block_table`` and ``lengths`` (int32, tokens of each sequence in the cache, the new ones included), the paged cache that :func:`append_kv` fills: a
+    piece of a prompt behind what the cache holds already.  At most 128 heads share a key head.  The last query of a sequence is at the place of
+    its last key and sees, with ``causal``, all keys up to its own place, with ``window`` only the last ``window`` of these; a query that sees nothing gives zeros.
+    ``scale`` of the scores: ``D ** -0.5`` where left out.  Scores and softmax in fp32, the weights rounded to 16 bits for the product with ``v``.  What lies behind a
+    sequence, in rows or pages, has no influence; a sequence that the table or the cache does not hold is NaN.  Inference: no gradient."""
+    window = _window_of(window)
+    scale = _scale_of(scale, q.shape[-1] if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1)
+    args = (cu_seqlens, cu_seqlens_k, block_table, lengths)
+    if not torch.compiler.is_compiling():
+        r = _lib.ext().prompt_attention(q, k, v, *args, causal, scale, window)
+        if r is not None:
+            return r
+    _check_heads(q, "q")
+    if q.dim() != 3:
+        raise RuntimeError(f"q has shape {tuple(q.shape)}, expected [tokens, heads, D]")
+    _check_index(cu_seqlens, "cu_seqlens", q, (torch.int32,), getattr(cu_seqlens, "shape", ()))
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+        raise RuntimeError("cu_seqlens must hold the starts of one sequence at least, and the end of the last")
+    if (block_table is None) != (lengths is None):
+        raise RuntimeError("block_table and lengths go together")
+    if block_table is not None:
+        if cu_seqlens_k is not None:
+            raise RuntimeError("the lengths of the sequences in a cache are `lengths`, not cu_seqlens_k")
+        _check_cache(k, v, block_table, q)
+        _check_index(lengths, "lengths", q, (torch.int32,), (cu_seqlens.numel() - 1,))
+        _check_like(block_table, "block_table", q, (torch.int32,), (cu_seqlens.numel() - 1, block_table.size(1)))
+    else:
+        _check_heads(k, "k")
+        if k.dim() != 3 or k.size(0) == 0:
+            raise RuntimeError(f"k has shape {tuple(k.shape)}, expected [tokens, key heads, D] with one token at least")
+        _check_like(k, "k", q, (q.dtype,), (*k.shape[:2], q.size(-1)))
+        _check_like(v, "v", q, (q.dtype,), k.shape)
+        if v is None:
+            raise RuntimeError("v must be a CUDA tensor")
+        if cu_seqlens_k is not None:
+            _check_like(cu_seqlens_k, "cu_seqlens_k", q, (torch.int32,), cu_seqlens.shape)
+    _check_shared(q, k.size(-2))
+    if q.size(1) // k.size(-2) > 128:
+        raise RuntimeError(f"{q.size(1)} heads for {k.size(-2)} key heads: at most 128 can share one")
+    _no_gradient("prompt_attention", q, k, v)
+    if _recorded():
+        return torch.ops.nanoquant_b200.prompt_attention(q, k, v, *args, causal, scale, window)
+    cached = block_table is not None
+    r = _lib.ext().prompt_attention(_heads_in_place(q), k if cached else _heads_in_place(k), v if cached else _heads_in_place(v), *(_at_boundary(t) for t in args),
+                                    causal, scale, window)
+    if r is None:
+        raise _not_plain("prompt_attention")
+    return r
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: Optional[float] = None, window: Optional[int] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over the paged cache that :func:`append_kv` fills, ``[sequences, heads, D]`` (``nq_paged_attention_fwd``).
+
+    ``q`` ``[sequences, heads, D]``; ``lengths`` int32, the tokens of each sequence in the cache, the new one included (0 or less: a padded row, which gives zeros);
+    the rest as in :func:`prompt_attention`.  Lengths and table are read on the device: a captured call follows them.  Inference: no gradient."""
+    window = _window_of(window)
+    scale = _scale_of(scale, q.shape[-1] if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1)
+    if not torch.compiler.is_compiling():
+        r = _lib.ext().paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window)
+        if r is not None:
+            return r
+    _check_heads(q, "q")
+    if q.dim() != 3:
+        raise RuntimeError(f"q has shape {tuple(q.shape)}, expected [sequences, heads, D]")
+    _check_cache(k_cache, v_cache, block_table, q)
+    _check_shared(q, k_cache.size(2))
+    if q.size(0) == 0 and block_table.size(0) == 0:
+        return torch.empty_like(q)
+    _check_index(lengths, "lengths", q, (torch.int32,), (q.size(0),))
+    _check_like(block_table, "block_table", q, (torch.int32,), (q.size(0), block_table.size(1)))
+    _no_gradient("paged_attention", q, k_cache, v_cache)
+    if _recorded():
+        return torch.ops.nanoquant_b200.paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window)
+    r = _lib.ext().paged_attention(_heads_in_place(q), k_cache, v_cache, _at_boundary(block_table), _at_boundary(lengths), scale, window)
+    if r is None:
+        raise _not_plain("paged_attention")
+    return r
+
+
+def _check_shared(q, heads: int) -> None:
+    if q.size(1) % heads:
+        raise RuntimeError(f"{q.size(1)} heads are no multiple of {heads} key heads")
+
+
+def _heads_in_place(t):
+    """Heads that the kernels cannot read where they lie (strides that are no multiples of 8 elements, expanded or reversed dimensions) are copied."""
+    if t is None:
+        return None
+    t = t.resolve_neg()
+    even = t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(n == 1 or (s % 8 == 0 and s >= t.size(-1)) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    step = None
+    for n, s in reversed(list(zip(t.shape[:-2], t.stride()[:-2]))):
+        if n > 1:
+            even, step = even and step in (None, s), n * s
+    return t if even else t.clone(memory_format=torch.contiguous_format)
+
+
+def _at_boundary(t):
+    if t is None:
+        return None
+    t = t.resolve_neg().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 # The same calls as operators of the dispatcher, for what records calls: implementations in csrc/nq_torch.cpp, shapes for tracing and derivatives here.
 _RECORDED_OPS = {
     "norm": "(Tensor x, Tensor? weight, Tensor? bias, float eps, bool center) -> (Tensor, Tensor)",
@@ -409,6 +663,13 @@ _RECORDED_OPS = {
     "linear_cross_entropy": "(Tensor h, Tensor weight, Tensor targets, int ignore_index, int reduction) -> (Tensor, Tensor, Tensor)",
     "linear_cross_entropy_backward": "(Tensor grad, Tensor h, Tensor weight, Tensor targets, Tensor lse, Tensor count, int ignore_index, int reduction, "
                                      "bool[2] want) -> (Tensor, Tensor)",
+    "qk_norm_rope": "(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, Tensor? q_weight, Tensor? k_weight, float eps, bool interleaved, float scaling) "
+                    "-> (Tensor, Tensor)",
+    "append_kv": "(Tensor? q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor positions, Tensor? sequences, "
+                 "Tensor? inv_freq, Tensor? q_weight, Tensor? k_weight, float eps, bool interleaved, float scaling) -> Tensor",
+    "prompt_attention": "(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor? cu_seqlens_k, Tensor? block_table, Tensor? lengths, bool causal, float scale, "
+                        "int window) -> Tensor",
+    "paged_attention": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lengths, float scale, int window) -> Tensor",
 }
 
 
@@ -479,13 +740,26 @@ def _linear_cross_entropy_gradients(ctx, grad, *_):
     return (*(t if wanted else None for t, wanted in zip(d, want)), None, None, None)
 
 
+def _qk_norm_rope_fake(q, k, *_):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+def _append_kv_fake(q, k, *_):
+    return k.new_empty((0,)) if q is None else q.new_empty(q.shape)
+
+
+def _attention_fake(q, *_):
+    return q.new_empty(q.shape)
+
+
 def _define_recorded_ops() -> None:
     name = "nanoquant_b200::{}".format
     for op, schema in _RECORDED_OPS.items():
         torch.library.define(name(op), schema)
     for op, fake in (("norm", _norm_fake), ("norm_backward", _norm_backward_fake), ("quantize_rows", _quantize_rows_fake), ("int8_linear", _head_fake),
                      ("dense_gemv", _head_fake), ("linear_cross_entropy", _linear_cross_entropy_fake),
-                     ("linear_cross_entropy_backward", _linear_cross_entropy_backward_fake)):
+                     ("linear_cross_entropy_backward", _linear_cross_entropy_backward_fake), ("qk_norm_rope", _qk_norm_rope_fake),
+                     ("append_kv", _append_kv_fake), ("prompt_attention", _attention_fake), ("paged_attention", _attention_fake)):
         torch.library.register_fake(name(op))(fake)
     torch.library.register_autograd(name("norm"), _norm_gradients, setup_context=_norm_setup)
     torch.library.register_autograd(name("linear_cross_entropy"), _linear_cross_entropy_gradients, setup_context=_linear_cross_entropy_setup)

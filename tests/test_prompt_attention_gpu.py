@@ -1,0 +1,210 @@
+"""Attention of packed prompts (`ops.prompt_attention`), over themselves, other keys or a paged cache, against its definition in 64 bits."""
+import pytest
+import torch
+
+from tests.attention_util import DTYPES, attention64, check_attention, paged, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def starts(lengths, first=0):
+    return torch.tensor([first + sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=torch.int32, device="cuda")
+
+
+def expected(q, ks, vs, lengths, window=None, scale=None, causal=True, first=0):
+    """Rows of no sequence: zeros."""
+    out = [torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(3)]
+    at = first
+    for s, n in enumerate(lengths):
+        place = torch.arange(n, device="cuda") + len(ks[s]) - n
+        for o, part in zip(out, attention64(q[at:at + n], ks[s], vs[s], place, scale, window, causal)):
+            o[at:at + n] = part
+        at += n
+    return out
+
+
+def make(lengths, H, K, D, dtype, seed=0, sharp=1.5):
+    T = sum(lengths)
+    qkv = rand(seed, T, H + 2 * K, D)
+    qkv[:, :H] *= sharp
+    qkv = qkv.to(dtype)
+    return qkv[:, :H], qkv[:, H:H + K], qkv[:, H + K:]
+
+
+CASES = [([1], 1, 1, 64), ([128], 1, 1, 128), ([256], 2, 2, 128), ([257, 1, 127], 4, 1, 128), ([1, 2, 3, 37, 129, 300], 8, 2, 64), ([5, 0, 0, 70], 6, 3, 128), ([515], 14, 2, 64),
+         ([300, 20], 71, 1, 64), ([200], 7, 1, 128), ([333, 64], 8, 8, 80), ([140, 3], 6, 2, 96), ([260, 65, 1], 4, 2, 256), ([130], 12, 4, 192), ([50, 9], 3, 1, 8), ([90], 100, 1, 24),
+         ([1100, 900], 8, 2, 128), ([2049], 4, 4, 64), ([700], 2, 1, 256)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,H,K,D", CASES)
+def test_against_definition(lengths, H, K, D, dtype):
+    from nanoquant_b200 import ops
+
+    q, k, v = make(lengths, H, K, D, dtype)
+    cu = starts(lengths)
+    ks, vs = k.split(lengths), v.split(lengths)
+    got = ops.prompt_attention(q, k, v, cu)
+    assert got.shape == q.shape and got.is_contiguous()
+    check_attention(got, expected(q, ks, vs, lengths))
+    assert torch.equal(got, ops.prompt_attention(q, k, v, cu))
+
+
+@pytest.mark.parametrize("causal,window", [(False, None), (True, 1), (True, 100), (True, 513), (False, 64)])
+@pytest.mark.parametrize("H,K,D", [(8, 2, 128), (2, 2, 64), (4, 1, 256)])
+def test_masks(H, K, D, causal, window):
+    from nanoquant_b200 import ops
+
+    lengths = [700, 3, 130]
+    q, k, v = make(lengths, H, K, D, torch.bfloat16)
+    got = ops.prompt_attention(q, k, v, starts(lengths), causal=causal, window=window, scale=0.2)
+    check_attention(got, expected(q, k.split(lengths), v.split(lengths), lengths, window, 0.2, causal))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_other_numbers_of_keys_than_queries(D, causal):
+    """More keys: a prefix; fewer: rows that see nothing; none."""
+    from nanoquant_b200 import ops
+
+    lengths, keys = [130, 300, 20, 5, 260], [400, 100, 0, 6, 259]
+    q = make(lengths, 4, 2, D, torch.float16)[0]
+    k, v = make(keys, 4, 2, D, torch.float16, seed=1)[1:]
+    got = ops.prompt_attention(q, k, v, starts(lengths), starts(keys), causal=causal)
+    check_attention(got, expected(q, k.split(keys), v.split(keys), lengths, causal=causal))
+    assert (got[430:450] == 0).all()
+    if causal:
+        assert (got[130:330] == 0).all() and (got[455] == 0).all()
+
+
+def test_rows_of_no_sequence_are_zero():
+    from nanoquant_b200 import ops
+
+    lengths = [40, 300]
+    q, k, v = make([7] + lengths + [1000], 4, 2, 128, torch.bfloat16)
+    k[-1000:], v[-1000:], v[:7] = float("nan"), float("nan"), float("inf")
+    spoil = torch.full((1347, 4, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
+    del spoil                                                      # (what the allocator is likely to hand out next)
+    got = ops.prompt_attention(q, k, v, starts(lengths, 7))
+    check_attention(got, expected(q, k[7:347].split(lengths), v[7:347].split(lengths), lengths, first=7))
+    assert (got[:7] == 0).all() and (got[347:] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_neighbours_have_no_influence(D):
+    """NaN and infinities in the sequences beside one, in the rows of the same step."""
+    from nanoquant_b200 import ops
+
+    lengths = [30, 100, 77]
+    q, k, v = make(lengths, 4, 2, D, torch.float16)
+    want = [t[30:130] for t in expected(q, k.split(lengths), v.split(lengths), lengths)]
+    for t in (q, k, v):
+        t[:30], t[130:] = float("nan"), float("inf")
+    check_attention(ops.prompt_attention(q, k, v, starts(lengths))[30:130], want)
+
+
+def piece(new, total, H, K, D, page, dtype, seed=0, order="pages"):
+    k = [rand(seed + 10 * s, n, K, D, dtype=dtype) for s, n in enumerate(total)]
+    v = [rand(seed + 10 * s + 1, n, K, D, dtype=dtype) for s, n in enumerate(total)]
+    q = rand(seed + 3, sum(new), H, D, dtype=dtype, scale=1.5)
+    kc, vc, table = paged(k, v, total, page, seed, order)
+    return q, k, v, kc, vc, table, torch.tensor(total, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,total,H,K,D,page,window", [
+    ([1], [1], 1, 1, 64, 16, None), ([100, 1, 30], [100, 500, 31], 8, 2, 128, 16, None), ([64], [1000], 4, 4, 64, 8, None), ([300, 2], [900, 130], 8, 2, 128, 128, None), ([70], [333], 4, 1, 80, 32, None),
+    ([33, 0, 5], [97, 40, 5], 4, 2, 256, 16, None), ([200], [700], 4, 2, 128, 1024, None), ([150, 4], [800, 300], 8, 2, 128, 16, 100), ([9], [600], 2, 1, 64, 64, 50), ([40], [300], 2, 1, 256, 128, 70),
+    ([12], [5], 4, 2, 128, 16, None), ([17], [0], 4, 2, 64, 16, None)])
+def test_paged(new, total, H, K, D, page, window, dtype):
+    """A piece of a prompt behind what the cache holds; everything that no query sees is NaN, and places in the table that are not needed do not exist."""
+    from nanoquant_b200 import ops
+
+    q, k, v, kc, vc, table, n = piece(new, total, H, K, D, page, dtype, order="heads" if page == 16 else "pages")
+    want = expected(q, k, v, new, window)
+    if window:
+        for s, m in enumerate(total):                             # pages wholly in front of the first query's window
+            table[s, :max(0, m - new[s] + 1 - window) // page] = -1
+    check_attention(ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, window=window), want)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_sequences_that_are_not_there_are_nan(D):
+    from nanoquant_b200 import ops
+
+    new, total = [10, 200, 3, 40], [100, 300, 60, 64]
+    q, k, v, kc, vc, table, n = piece(new, total, 4, 2, D, 16, torch.bfloat16)
+    want = expected(q, k, v, new)
+    table[1, 3] = kc.size(0)
+    n[2] = 16 * table.size(1) + 1
+    got = ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n)
+    assert torch.isnan(got[10:213]).all()
+    rows = torch.cat((torch.arange(10), torch.arange(213, 253))).cuda()
+    check_attention(got[rows], [t[rows] for t in want])
+
+
+def test_maximum_that_keeps_growing():
+    """Scores that grow along the sequence by more than the maximum may lag, step after step, and ones that fall."""
+    from nanoquant_b200 import ops
+
+    n, H, D = 1500, 2, 128
+    for sign in (1, -1):
+        q, k, v = make([n], H, H, D, torch.float16)
+        q, k = q.clone(), k.clone()
+        q[..., 0] = 16.0
+        k[..., 0] = sign * torch.arange(n, device="cuda")[:, None] * (3.0 / 64)      # products to 2^10.2, scaled below 2^6.7
+        want = expected(q, [k], [v], [n])
+        o, avg, all_v = want
+        got = ops.prompt_attention(q, k, v, starts([n]))
+        assert ((got.double() - o).abs() <= 2.0 ** -11 * o.abs() + (2.0 ** -10 + 2.0 ** -11) * avg + 2.0 ** -25 * (1 + all_v)).all()
+
+
+def test_more_sequences_than_a_warp():
+    from nanoquant_b200 import ops
+
+    lengths = [(7 * i) % 23 for i in range(150)]
+    q, k, v = make(lengths, 4, 2, 64, torch.bfloat16)
+    check_attention(ops.prompt_attention(q, k, v, starts(lengths)), expected(q, k.split(lengths), v.split(lengths), lengths))
+
+
+def test_layouts():
+    from nanoquant_b200 import ops
+
+    lengths = [100, 60]
+    q, k, v = make(lengths, 4, 2, 64, torch.float16)
+    want = ops.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), starts(lengths))
+    odd = rand(0, 160, 4, 65, dtype=torch.float16)[..., 1:]
+    odd[:, :4] = q
+    wide = starts(lengths).repeat_interleave(2)[::2]
+    for a, b, c in ((odd, k, v), (q.transpose(0, 1).contiguous().transpose(0, 1), k.transpose(0, 1).contiguous().transpose(0, 1), v), (q, k.permute(2, 0, 1).contiguous().permute(1, 2, 0), v)):
+        assert torch.equal(ops.prompt_attention(a, b, c, wide), want)
+    same = ops.prompt_attention(q, k[:, :1].expand(160, 4, 64), v[:, :1].expand(160, 4, 64), starts(lengths))
+    # (a row's sums do not depend on the heads beside it)
+    assert torch.equal(same, ops.prompt_attention(q, k[:, :1].repeat(1, 4, 1), v[:, :1].repeat(1, 4, 1), starts(lengths)))
+    assert ops.prompt_attention(q[:0], k, v, starts([0])).shape == (0, 4, 64)
+
+
+def test_refusals():
+    from nanoquant_b200 import ops
+
+    lengths = [30, 40]
+    q, k, v = make(lengths, 8, 2, 64, torch.float16)
+    cu = starts(lengths)
+    kc, vc, table = paged(k.split(lengths), v.split(lengths), lengths, 16)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for match, call in (
+            ("CUDA", lambda: ops.prompt_attention(q.cpu(), k, v, cu)), ("Half or BFloat16", lambda: ops.prompt_attention(q.float(), k, v, cu)), ("k is", lambda: ops.prompt_attention(q, k.bfloat16(), v, cu)),
+            ("v has shape", lambda: ops.prompt_attention(q, k, v[:-1], cu)), ("no multiple", lambda: ops.prompt_attention(q[:, :7], k, v, cu)), ("expected \\[tokens", lambda: ops.prompt_attention(q[None], k, v, cu)),
+            ("cu_seqlens", lambda: ops.prompt_attention(q, k, v, cu.long())), ("cu_seqlens", lambda: ops.prompt_attention(q, k, v, cu[:1])), ("cu_seqlens", lambda: ops.prompt_attention(q, k, v, None)),
+            ("cu_seqlens_k", lambda: ops.prompt_attention(q, k, v, cu, cu[:2])), ("go together", lambda: ops.prompt_attention(q, kc, vc, cu, block_table=table)), ("go together", lambda: ops.prompt_attention(q, k, v, cu, lengths=n)),
+            ("cu_seqlens_k", lambda: ops.prompt_attention(q, kc, vc, cu, cu, table, n)), ("lengths", lambda: ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=n[:1])),
+            ("block_table", lambda: ops.prompt_attention(q, kc, vc, cu, block_table=table[:1], lengths=n)), ("k has shape", lambda: ops.prompt_attention(q, k[:0], v[:0], cu)),
+            ("128", lambda: ops.prompt_attention(rand(0, 4, 130, 64, dtype=torch.float16), k[:4, :1], v[:4, :1], cu)), ("expected \\[pages", lambda: ops.prompt_attention(q, k, v, cu, block_table=table, lengths=n))):
+        with pytest.raises(RuntimeError, match=match):
+            call()
+    for kw in (dict(scale=0.0), dict(scale=float("inf")), dict(window=0)):
+        with pytest.raises(ValueError):
+            ops.prompt_attention(q, k, v, cu, **kw)
+    k.requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.prompt_attention(q, k, v, cu)
