@@ -6,11 +6,11 @@
 // mma.sync.m16n8k16 (up to 16; the instruction's rate is far above what memory delivers, and few rows would leave tcgen05's 128 idle).
 //
 // Work.  The tokens that a sequence's query sees are cut into steps of 16.  An item is a sequence, a key head and up to 16 of its query heads; the steps of all
-// items lie one behind the other, and every CTA takes the same number of them, found from the lengths on the device: batches of any lengths fill the
-// SMs evenly, and a captured graph follows the lengths.  Within a CTA each of the four warps takes a contiguous quarter of the CTA's part of an item,
-// with a ring of steps of its own in shared memory (cp.async), its own running maximum, sum and accumulators: no barrier in the loop.  The warps' results are
-// joined through shared memory.  An item that lies in several CTAs leaves fp32 results (m, sum, unnormalised o) in the scratch, which a
-// second, overlapped launch joins in the order of the CTAs.  Batches without long sequences take whole items and need no second launch.
+// items lie one behind the other, and every warp takes the same number of them, found from the lengths on the device: batches of any lengths fill the
+// SMs evenly, and a captured graph follows the lengths.  A warp has a ring of steps of its own in shared memory (cp.async, which runs on into the next item),
+// its own running maximum, sum and accumulators: nothing in the loop waits for another warp.  An item that lies in several warps leaves fp32 results
+// (m, sum, unnormalised o) in the scratch, which a second, overlapped launch joins in their order.  Caches without room for long sequences take a CTA per item, its
+// steps divided among the four warps and their results joined through shared memory: one launch.
 //
 // The weights p are rounded to the operands' type for the product with the values: 2^-9 (bf16) or 2^-12 (fp16) of each, which the average over
 // tokens does not enlarge.  Sums of p are fp32 sums of the rounded values.
@@ -21,22 +21,24 @@ namespace nq {
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStep = 16;                  // tokens
 constexpr int kPagedRows = 16;                  // query heads of an item at most
-constexpr int kPagedWhole = 256;                // caches of up to so many tokens a sequence: whole items
+constexpr int kPagedWhole = 256;                // caches of up to so many tokens a sequence: a CTA per item
+constexpr int kPagedJoinThreads = 128;
 
 struct PagedParams {
     nq_attention_desc d;
     int shift;                                  // log2(page_size)
     int rows, chunks;                           // query heads to a key head; items of 16 of them
-    int whole;                                  // every CTA takes whole items
+    int warps;                                  // of the split kernel
+    int items;                                  // (of all sequences)
     float factor;                               // scale log2(e)
-    float* part;                                // [CTAs][2][16][DP + 2]
+    float* part;                                // [warps][2][16][DP + 2]
 };
 
-// Steps of a sequence's items, and what a step covers.
+// Steps of a sequence's items, and what they cover.
 struct PagedRange {
     int begin, end;                             // tokens seen
     int first, steps;                           // steps of 16 tokens; one at least, so that somebody writes the result
-    bool bad;                                   // the table does not hold the sequence
+    int bad;                                    // the table does not hold the sequence
 };
 __device__ __forceinline__ PagedRange paged_range(const nq_attention_desc& d, int s, int shift) {
     PagedRange r;
@@ -50,23 +52,78 @@ __device__ __forceinline__ PagedRange paged_range(const nq_attention_desc& d, in
     return r;
 }
 
-// The sequence that step `at` of all steps lies in, and the steps ahead of it; all steps where `at` is negative.  By the whole CTA.
+// Where a step of all steps lies.
 struct PagedPlace {
+    long long before;                           // steps ahead of the sequence
     int seq;
-    long long before, total;
+    PagedRange range;
 };
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums) {       // inclusive
+struct PagedPlan {
+    PagedPlace place[kPagedWarps];
+    long long sums[kPagedWarps];
+};
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {       // inclusive, over kPagedThreads threads
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
     }
+    __syncthreads();                            // (the sums before have been read)
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) v += warp_sums[w];
-    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) {
+        if (w < warp) v += warp_sums[w];
+        total += warp_sums[w];
+    }
     return v;
+}
+// Steps of all items, and a warp's share of them.  By the whole CTA.  `first`: the sequence of this thread, for batches of up to kPagedThreads.
+__device__ __forceinline__ long long paged_total(const PagedParams& P, PagedPlan& plan, long long& n, long long& sum, PagedRange& range) {
+    const int per_seq = P.d.k_heads * P.chunks;
+    long long total = 0;
+    for (int s0 = 0; s0 < P.d.seqs; s0 += kPagedThreads) {
+        const int s = s0 + threadIdx.x;
+        n = 0;
+        if (s < P.d.seqs) {
+            range = paged_range(P.d, s, P.shift);
+            n = (long long)range.steps * per_seq;
+        }
+        long long some;
+        sum = block_scan(n, plan.sums, some) + total;
+        total += some;
+    }
+    return total;
+}
+// The sequences that the steps unit(0) .. unit(COUNT - 1) lie in (those that are below the total).
+template <int COUNT, class Unit>
+__device__ __forceinline__ void paged_find(const PagedParams& P, PagedPlan& plan, long long n, long long sum, PagedRange range, Unit unit) {
+    const int per_seq = P.d.k_heads * P.chunks;
+    auto look = [&](int s) {
+#pragma unroll
+        for (int w = 0; w < COUNT; ++w)
+            if (n > 0 && sum - n <= unit(w) && unit(w) < sum) plan.place[w] = {sum - n, s, range};
+    };
+    if (P.d.seqs <= kPagedThreads) {
+        look(threadIdx.x);
+    } else {
+        long long before = 0;
+        for (int s0 = 0; s0 < P.d.seqs; s0 += kPagedThreads) {
+            const int s = s0 + threadIdx.x;
+            n = 0;
+            if (s < P.d.seqs) {
+                range = paged_range(P.d, s, P.shift);
+                n = (long long)range.steps * per_seq;
+            }
+            long long some;
+            sum = block_scan(n, plan.sums, some) + before;
+            before += some;
+            look(s);
+        }
+    }
+    __syncthreads();
 }
 
 template <bool BF16>
@@ -97,7 +154,8 @@ template <int DP> struct PagedShape {
     static constexpr int kStages = DP == 64 ? 4 : 3;
     static constexpr int kWarpBytes = 2 * kStages * kTileBytes;
     static constexpr int kSmem = kPagedWarps * kWarpBytes;
-    static constexpr int kPart = kPagedRows * (DP + 2);           // floats of a partial result
+    static constexpr int kRow = DP + 2;                           // floats of a head's result: o, m, sum
+    static constexpr int kPart = kPagedRows * kRow;
     static constexpr int kCtasPerSm = DP == 64 ? 3 : DP == 128 ? 2 : 1;
     static_assert(kPagedWarps * kPart * 4 <= kSmem, "the warps' results fit the rings");
 };
@@ -105,332 +163,320 @@ template <int DP> struct PagedShape {
 template <int DP>
 __device__ __forceinline__ uint32_t paged_at(uint32_t base, int r, int c) { return base + r * PagedShape<DP>::kRowBytes + ((c ^ (r & 7)) << 4); }
 
-template <int DP, bool BF16>
-__global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) paged_kernel(const __grid_constant__ PagedParams P) {
-    using S = PagedShape<DP>;
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long scan[kPagedWarps];
-    __shared__ long long place[2];
-    const nq_attention_desc& d = P.d;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
-    const int per_seq = d.k_heads * P.chunks;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    // this CTA's steps: [unit, unit_end) of all items' steps
-    long long unit, unit_end, seq_before;          // (seq_before: steps ahead of the sequence, of one of its items' kind)
-    int seq;
-    if (P.whole) {
-        seq = blockIdx.x / per_seq;
-        const int steps = paged_range(d, seq, P.shift).steps;
-        seq_before = 0;
-        unit = (long long)(blockIdx.x - seq * per_seq) * steps;
-        unit_end = unit + steps;
-    } else {
-        long long total = 0;
-        for (int s0 = 0; s0 < d.seqs; s0 += kPagedThreads) {
-            const int s = s0 + threadIdx.x;
-            const long long sum = block_scan(s < d.seqs ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, scan);
-            if (threadIdx.x == kPagedThreads - 1) place[0] = sum;
-            __syncthreads();
-            total += place[0];
-            __syncthreads();
-        }
-        long long share = (total + gridDim.x - 1) / gridDim.x;
-        share = max(share, (long long)kPagedWarps);
-        unit = share * blockIdx.x;
-        unit_end = min(unit + share, total);
-        if (unit >= unit_end) return;
-        long long before = 0;
-        seq = 0;
-        seq_before = 0;
-        for (int s0 = 0; s0 < d.seqs; s0 += kPagedThreads) {
-            const int s = s0 + threadIdx.x;
-            const long long n = s < d.seqs ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, sum = block_scan(n, scan) + before;
-            if (n > 0 && sum - n <= unit && unit < sum) {
-                place[0] = s;
-                place[1] = sum - n;
-            }
-            if (threadIdx.x == kPagedThreads - 1) scan[0] = sum;
-            __syncthreads();
-            before = scan[0];
-            if (before > unit) {
-                seq = (int)place[0];
-                seq_before = place[1];
-                break;
-            }
-            __syncthreads();
-        }
-        __syncthreads();
-    }
-
-    while (unit < unit_end) {
-        const PagedRange R = paged_range(d, seq, P.shift);
-        const long long seq_steps = (long long)R.steps * per_seq;
-        if (unit >= seq_before + seq_steps) {      // (whole: never)
-            seq_before += seq_steps;
-            ++seq;
-            continue;
-        }
-        const int item = (int)((unit - seq_before) / R.steps), from = (int)(unit - seq_before - (long long)item * R.steps);
-        const int to = (int)min((long long)R.steps, from + (unit_end - unit));
-        const int kh = item / P.chunks, chunk = item - kh * P.chunks;
-        const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
-
-        // this warp's steps
-        const int mine = (to - from + kPagedWarps - 1) / kPagedWarps;
-        const int s0 = from + warp * mine, s1 = min(s0 + mine, to);
+// The pages of 32 steps of an item, held by the lanes of a warp: the one of lane i's step, and (pages of 8 tokens) of its second half.
+struct PagedPages {
+    int page0, page1, from;
+    // `to`: steps from there on are not wanted.  False: a page outside the cache.
+    __device__ __forceinline__ bool look(const nq_attention_desc& d, int shift, int seq, const PagedRange& R, int s, int to) {
         const int* table = d.block_table + (long long)seq * d.table_stride;
-        const uint16_t* kbase = static_cast<const uint16_t*>(d.k) + (long long)kh * d.k_head;
-        const uint16_t* vbase = static_cast<const uint16_t*>(d.v) + (long long)kh * d.v_head;
-        bool bad = R.bad;
-
-        // pages of the next 32 steps' first and (pages of 8) second halves: lane i those of step i
-        int page0 = 0, page1 = 0;
-        auto pages = [&](int s) {                  // steps s .. s + 31
-            const int t = (R.first + s + lane) * kPagedStep;
-            auto look = [&](int token) {
-                // (only pages that hold a token that is seen)
-                if (s + lane >= s1 || token >= R.end || token + min(d.page_size, kPagedStep) <= R.begin) return 0;
-                const int p = __ldcg(table + (token >> P.shift));
-                if (p < 0 || p >= d.pages) { bad = true; return 0; }
-                return p;
-            };
-            page0 = look(t);
-            page1 = d.page_size < kPagedStep ? look(t + 8) : page0;
+        const int lane = threadIdx.x & 31, mine = s + lane;
+        bool bad = false;
+        auto one = [&](int token) {
+            // (only pages that hold a token that is seen)
+            if (mine >= to || token >= R.end || token + min(d.page_size, kPagedStep) <= R.begin) return 0;
+            const int p = __ldcg(table + (token >> shift));
+            if (p < 0 || p >= d.pages) { bad = true; return 0; }
+            return p;
         };
-        auto load = [&](int s, int stage) {        // step s, whose page is held by lane (s - s0) % 32
-            const int src = (s - s0) & 31;
-            const int pa = __shfl_sync(0xffffffffu, page0, src), pb = __shfl_sync(0xffffffffu, page1, src);
-            const uint32_t kt = ring + stage * 2 * S::kTileBytes, vt = kt + S::kTileBytes;
-            constexpr int kRowsAtOnce = 32 / S::kChunks > 0 ? 32 / S::kChunks : 1;
-            const int c = lane % S::kChunks, r0 = lane / S::kChunks;
-            const int token0 = (R.first + s) * kPagedStep;
+        const int t = mine < to ? (R.first + mine) * kPagedStep : 0;
+        page0 = one(t);
+        page1 = d.page_size < kPagedStep ? one(t + 8) : page0;
+        from = s;
+        return !__any_sync(0xffffffffu, bad);
+    }
+};
+// Keys and values of step s into a stage.
+template <int DP>
+__device__ __forceinline__ void paged_load(const nq_attention_desc& d, const PagedRange& R, const PagedPages& pages, int kh, int s, uint32_t kt) {
+    using S = PagedShape<DP>;
+    const int lane = threadIdx.x & 31, src = s - pages.from;
+    const int pa = __shfl_sync(0xffffffffu, pages.page0, src), pb = __shfl_sync(0xffffffffu, pages.page1, src);
+    constexpr int kRowsAtOnce = 32 / S::kChunks;
+    const int c = lane % S::kChunks, r0 = lane / S::kChunks;
+    const int token0 = (R.first + s) * kPagedStep, slot0 = token0 & (d.page_size - 1);
+    const uint16_t* kbase = static_cast<const uint16_t*>(d.k) + (long long)kh * d.k_head + 8 * c;
+    const uint16_t* vbase = static_cast<const uint16_t*>(d.v) + (long long)kh * d.v_head + 8 * c;
+    const bool column = 8 * c < d.D;
 #pragma unroll
-            for (int i = 0; i < kPagedStep; i += kRowsAtOnce) {
-                const int r = r0 + i, token = token0 + r;
-                const bool live = token >= R.begin && token < R.end && 8 * c < d.D;
-                const long long page = r < 8 ? pa : pb, slot = token & (d.page_size - 1);
-                copy16(paged_at<DP>(kt, r, c), live ? kbase + page * d.k_page + slot * d.k_slot + 8 * c : kbase, live);
-            }
+    for (int kv = 0; kv < 2; ++kv) {
+        const uint16_t* base = kv ? vbase : kbase;
+        const long long page_step = kv ? d.v_page : d.k_page, slot_step = kv ? d.v_slot : d.k_slot;
+        const uint16_t* at0 = base + pa * page_step + slot0 * slot_step;
+        const uint16_t* at1 = base + pb * page_step + (d.page_size < kPagedStep ? 0 : slot0 + 8) * slot_step;
 #pragma unroll
-            for (int i = 0; i < kPagedStep; i += kRowsAtOnce) {
-                const int r = r0 + i, token = token0 + r;
-                const bool live = token >= R.begin && token < R.end && 8 * c < d.D;
-                const long long page = r < 8 ? pa : pb, slot = token & (d.page_size - 1);
-                copy16(paged_at<DP>(vt, r, c), live ? vbase + page * d.v_page + slot * d.v_slot + 8 * c : vbase, live);
-            }
-        };
-        if (s0 < s1) pages(s0);
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) {
-            if (s0 + i < s1) load(s0 + i, i);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+        for (int i = 0; i < kPagedStep; i += kRowsAtOnce) {
+            const int r = r0 + i, token = token0 + r;
+            const bool live = token >= R.begin && token < R.end && column;
+            const uint16_t* at = (r < 8 ? at0 : at1) + (r & 7) * slot_step;
+            copy16(paged_at<DP>(kt + kv * S::kTileBytes, r, c), live ? at : base, live);
         }
+    }
+}
+// Up to 16 heads' queries, accumulators, maxima and sums, as MMA fragments: lane (g, q) has the heads g and g + 8.
+template <int DP, bool BF16>
+struct PagedHeads {
+    uint32_t a[DP / 16][4];
+    float o[DP / 8][4], m[2], l[2];
 
-        // queries: rows g and g + 8 of the MMA
-        uint32_t a[DP / 16][4];
-        {
-            const uint16_t* qp = static_cast<const uint16_t*>(d.q) + (long long)seq * d.q_token + (long long)h0 * d.q_head;
+    __device__ __forceinline__ void start(const nq_attention_desc& d, int seq, int h0, int rows) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+        const uint16_t* qp = static_cast<const uint16_t*>(d.q) + (long long)seq * d.q_token + (long long)h0 * d.q_head;
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
+        for (int k = 0; k < DP / 16; ++k) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = g + 8 * (i & 1), col = 16 * k + 2 * q + 8 * (i >> 1);
-                    a[k][i] = row < rows && col < d.D ? __ldcg(reinterpret_cast<const unsigned*>(qp + (long long)row * d.q_head + col)) : 0u;
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int row = g + 8 * (i & 1), col = 16 * k + 2 * q + 8 * (i >> 1);
+                a[k][i] = row < rows && col < d.D ? __ldcg(reinterpret_cast<const unsigned*>(qp + (long long)row * d.q_head + col)) : 0u;
             }
         }
-        float o[DP / 8][4] = {};
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-        for (int s = s0, stage = 0; s < s1; ++s) {
-            const int ahead = s + S::kStages - 1;
-            if (ahead < s1) {
-                if (((ahead - s0) & 31) == 0) pages(ahead);
-                load(ahead, stage == 0 ? S::kStages - 1 : stage - 1);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
-            __syncwarp();
-            const uint32_t kt = ring + stage * 2 * S::kTileBytes, vt = kt + S::kTileBytes;
-            float c[2][4] = {};
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                uint32_t b[4];
-                // matrices: keys 0-7 and 8-15 (lanes 8-15 / 24-31: the second 8 columns)
-                ldmatrix4(b, paged_at<DP>(kt, (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-                paged_mma<BF16>(c[0], a[k], b[0], b[1]);
-                paged_mma<BF16>(c[1], a[k], b[2], b[3]);
-            }
-            // lane: heads g (c[.][0..1]) and g + 8 (c[.][2..3]), tokens 8 n + 2 q + (i & 1)
-            const int token0 = (R.first + s) * kPagedStep;
-            if (token0 < R.begin || token0 + kPagedStep > R.end) {
+        for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int token = token0 + 8 * (i >> 2) + 2 * q + (i & 1);
-                    if (token < R.begin || token >= R.end) c[i >> 2][i & 3] = -INFINITY;
-                }
-            }
-            uint32_t p[4];
+            for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+    }
+    __device__ __forceinline__ void step(const PagedRange& R, int s, float factor, uint32_t kt) {
+        using S = PagedShape<DP>;
+        const int lane = threadIdx.x & 31, q = lane & 3;
+        const uint32_t vt = kt + S::kTileBytes;
+        float c[2][4] = {};
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float top = fmaxf(fmaxf(c[0][2 * r], c[0][2 * r + 1]), fmaxf(c[1][2 * r], c[1][2 * r + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float to_m = fmaxf(m[r], top * P.factor), base = to_m == -INFINITY ? 0.f : to_m;
-                const float shrink = exp2_approx(m[r] - base);          // (0 at first, exactly 1 where m stays)
-                m[r] = to_m;
-                float e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = exp2_approx(fmaf(c[i >> 1][2 * r + (i & 1)], P.factor, -base));
-                p[r] = head_pack<BF16>(e[0], e[1]);
-                p[2 + r] = head_pack<BF16>(e[2], e[3]);
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum += head_float<BF16>(i < 2 ? p[r] : p[2 + r], i & 1);
-                l[r] = l[r] * shrink + sum;
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n) {
-                    o[n][2 * r] *= shrink;
-                    o[n][2 * r + 1] *= shrink;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < DP / 16; ++n) {
-                uint32_t b[4];
-                // matrices (transposed): tokens 0-7 and 8-15 of columns 16 n .., then of 16 n + 8 ..
-                ldmatrix4_trans(b, paged_at<DP>(vt, (lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
-                paged_mma<BF16>(o[2 * n], p, b[0], b[1]);
-                paged_mma<BF16>(o[2 * n + 1], p, b[2], b[3]);
-            }
-            __syncwarp();                          // the stage may be filled again
-            if (++stage == S::kStages) stage = 0;
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t b[4];
+            // matrices: keys 0-7 and 8-15 (lanes 8-15 / 24-31: the second 8 columns)
+            ldmatrix4(b, paged_at<DP>(kt, (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+            paged_mma<BF16>(c[0], a[k], b[0], b[1]);
+            paged_mma<BF16>(c[1], a[k], b[2], b[3]);
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        // lane: heads g (c[.][0..1]) and g + 8 (c[.][2..3]), tokens 8 n + 2 q + (i & 1)
+        const int token0 = (R.first + s) * kPagedStep;
+        if (token0 < R.begin || token0 + kPagedStep > R.end) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int token = token0 + 8 * (i >> 2) + 2 * q + (i & 1);
+                if (token < R.begin || token >= R.end) c[i >> 2][i & 3] = -INFINITY;
+            }
+        }
+        uint32_t p[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float top = fmaxf(fmaxf(c[0][2 * r], c[0][2 * r + 1]), fmaxf(c[1][2 * r], c[1][2 * r + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float to_m = fmaxf(m[r], top * factor), base = to_m == -INFINITY ? 0.f : to_m;
+            const float shrink = exp2_approx(m[r] - base);          // (0 at first, exactly 1 where m stays)
+            m[r] = to_m;
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = exp2_approx(fmaf(c[i >> 1][2 * r + (i & 1)], factor, -base));
+            p[r] = head_pack<BF16>(e[0], e[1]);
+            p[2 + r] = head_pack<BF16>(e[2], e[3]);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += head_float<BF16>(i < 2 ? p[r] : p[2 + r], i & 1);
+            l[r] = l[r] * shrink + sum;
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+                o[n][2 * r] *= shrink;
+                o[n][2 * r + 1] *= shrink;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+            uint32_t b[4];
+            // matrices (transposed): tokens 0-7 and 8-15 of columns 16 n .., then of 16 n + 8 ..
+            ldmatrix4_trans(b, paged_at<DP>(vt, (lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
+            paged_mma<BF16>(o[2 * n], p, b[0], b[1]);
+            paged_mma<BF16>(o[2 * n + 1], p, b[2], b[3]);
+        }
+    }
+    // The sums over the lanes of a row; NaN for a sequence that is not there.
+    __device__ __forceinline__ void finish(bool bad) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (bad) l[r] = __int_as_float(0x7fffffff);
         }
-        // a page outside the cache: NaN from here on
-        if (__syncthreads_or(bad)) l[0] = l[1] = __int_as_float(0x7fffffff);
-        // the warps' results through their rings
-        float* box = reinterpret_cast<float*>(smem) + warp * S::kPart;
+    }
+    __device__ __forceinline__ void save(float* box, int rows) const {
+        const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int row = g + 8 * r;
-            float* at = box + row * (DP + 2);
+            float* at = box + row * PagedShape<DP>::kRow;
             if (row < rows) {
 #pragma unroll
                 for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float2*>(at + 8 * n + 2 * q) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
                 if (q == 0) *reinterpret_cast<float2*>(at + DP) = make_float2(m[r], l[r]);
             }
         }
-        __syncthreads();
-        const bool all = from == 0 && to == R.steps;
-        float* part = P.part + ((long long)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * S::kPart;
-        const float* boxes = reinterpret_cast<const float*>(smem);
-        for (int i = threadIdx.x; i < rows * (DP / 2); i += kPagedThreads) {
-            const int row = i / (DP / 2), col = 2 * (i - row * (DP / 2));
-            const float* at = boxes + row * (DP + 2);
-            float top = -INFINITY;
+    }
+    __device__ __forceinline__ void store(const nq_attention_desc& d, int seq, int h0, int rows) const {
+        const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
 #pragma unroll
-            for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, at[w * S::kPart + DP]);
-            const float base = top == -INFINITY ? 0.f : top;
-            float sum = 0.f;
-            float2 v = make_float2(0.f, 0.f);
+        for (int r = 0; r < 2; ++r) {
+            const int row = g + 8 * r;
+            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+            uint16_t* at = static_cast<uint16_t*>(d.out) + ((long long)seq * d.q_heads + h0 + row) * d.D;
+            if (row < rows) {
 #pragma unroll
-            for (int w = 0; w < kPagedWarps; ++w) {
-                const float e = exp2_approx(at[w * S::kPart + DP] - base);
-                const float2 u = *reinterpret_cast<const float2*>(at + w * S::kPart + col);
-                sum += at[w * S::kPart + DP + 1] * e;
-                v.x += u.x * e;
-                v.y += u.y * e;
-            }
-            if (all) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                if (col < d.D)
-                    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(d.out) + ((long long)seq * d.q_heads + h0 + row) * d.D + col) = head_pack<BF16>(v.x * inv, v.y * inv);
-            } else {
-                *reinterpret_cast<float2*>(part + row * (DP + 2) + col) = v;
-                if (col == 0) *reinterpret_cast<float2*>(part + row * (DP + 2) + DP) = make_float2(top, sum);
+                for (int n = 0; n < DP / 8; ++n)
+                    if (8 * n < d.D) *reinterpret_cast<uint32_t*>(at + 8 * n + 2 * q) = head_pack<BF16>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
             }
         }
-        __syncthreads();                           // the rings are filled again
-        unit += to - from;
+    }
+};
+
+// Long caches: a warp has the steps [share W, share (W + 1)) of all items' steps.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) paged_split_kernel(const __grid_constant__ PagedParams P) {
+    using S = PagedShape<DP>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ PagedPlan plan;
+    const nq_attention_desc& d = P.d;
+    const int warp = threadIdx.x >> 5;
+    const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
+    const int per_seq = d.k_heads * P.chunks, W = blockIdx.x * kPagedWarps + warp;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    long long n, sum;
+    PagedRange range;
+    const long long total = paged_total(P, plan, n, sum, range), share = (total + P.warps - 1) / P.warps;
+    paged_find<kPagedWarps>(P, plan, n, sum, range, [&](int w) { return share * (blockIdx.x * kPagedWarps + w); });
+    const long long unit = share * W;
+    if (unit >= total) return;                  // (no barrier behind this)
+    const int count = (int)min(share, total - unit);
+
+    struct Cursor {
+        PagedRange R;
+        int seq, item, s;                       // item of the sequence; the next step
+    } load, at;
+    {
+        const PagedPlace& p = plan.place[warp];
+        load.R = p.range;
+        load.seq = p.seq;
+        load.item = (int)((unit - p.before) / load.R.steps);
+        load.s = (int)(unit - p.before - (long long)load.item * load.R.steps);
+    }
+    at = load;
+    auto advance = [&](Cursor& c) {             // (true: behind the last step of an item)
+        if (++c.s < c.R.steps) return false;
+        c.s = 0;
+        if (++c.item == per_seq) {
+            c.item = 0;
+            if (++c.seq < d.seqs) c.R = paged_range(d, c.seq, P.shift);
+        }
+        return true;
+    };
+    PagedPages pages;
+    bool fresh = true;
+    unsigned bad_items = 0, load_items = 0;     // (bit i: the i-th item from here on, modulo 32, has a page outside the cache; a ring holds far fewer)
+    auto load_next = [&](int i, int stage) {    // step i of this warp's
+        if (fresh || load.s - pages.from >= 32) {
+            const bool ok = pages.look(d, P.shift, load.seq, load.R, load.s, min(load.R.steps, load.s + (count - i)));
+            if (!ok) bad_items |= 1u << (load_items & 31);
+            fresh = false;
+        }
+        paged_load<DP>(d, load.R, pages, load.item / P.chunks, load.s, ring + stage * 2 * S::kTileBytes);
+        if (advance(load)) {
+            fresh = true;
+            ++load_items;
+            bad_items &= ~(1u << (load_items & 31));
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+        if (i < count) load_next(i, i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    PagedHeads<DP, BF16> heads;
+    unsigned at_items = 0;
+    bool begin = true;                          // of an item, here
+    int from = at.s;
+    for (int i = 0, stage = 0; i < count; ++i) {
+        const int kh = at.item / P.chunks, chunk = at.item - kh * P.chunks;
+        const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
+        if (begin) {
+            heads.start(d, at.seq, h0, rows);
+            from = at.s;
+            begin = false;
+        }
+        if (i + S::kStages - 1 < count) load_next(i + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+        __syncwarp();
+        heads.step(at.R, at.s, P.factor, ring + stage * 2 * S::kTileBytes);
+        __syncwarp();                           // the stage may be filled again
+        if (++stage == S::kStages) stage = 0;
+        const int seq = at.seq;
+        const bool seq_bad = at.R.bad != 0, last = at.s + 1 == at.R.steps;
+        if (last || i + 1 == count) {
+            heads.finish(seq_bad || (bad_items >> (at_items & 31) & 1u));
+            if (from == 0 && last) heads.store(d, seq, h0, rows);
+            else heads.save(P.part + ((long long)W * 2 + (from == 0 ? 1 : 0)) * S::kPart, rows);
+            ++at_items;
+            begin = true;
+        }
+        advance(at);
     }
 }
 
-// The results of an item that lies in several CTAs of the kernel above, by the CTA of the same number as the first of them.
+// Short caches: a CTA per item, a quarter of its steps to a warp.
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_constant__ PagedParams P) {
+__global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) paged_whole_kernel(const __grid_constant__ PagedParams P) {
     using S = PagedShape<DP>;
-    __shared__ long long scan[kPagedWarps];
-    __shared__ long long place[2];
+    extern __shared__ __align__(128) unsigned char smem[];
     const nq_attention_desc& d = P.d;
-    const int per_seq = d.k_heads * P.chunks;
-    // (the lengths are older than the kernel above, which has waited for what wrote them before it let this one start)
-    long long total = 0;
-    for (int s0 = 0; s0 < d.seqs; s0 += kPagedThreads) {
-        const int s = s0 + threadIdx.x;
-        const long long sum = block_scan(s < d.seqs ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, scan);
-        if (threadIdx.x == kPagedThreads - 1) place[0] = sum;
-        __syncthreads();
-        total += place[0];
-        __syncthreads();
-    }
-    long long share = (total + gridDim.x - 1) / gridDim.x;
-    share = max(share, (long long)kPagedWarps);
-    const long long last = share * (blockIdx.x + 1) - 1;       // this CTA's last step
-    bool split = last < total - 1;
-    long long begin = 0, end = 0;
-    int seq = 0, item = 0;
-    if (split) {
-        long long before = 0, seq_before = 0;
-        for (int s0 = 0; s0 < d.seqs; s0 += kPagedThreads) {
-            const int s = s0 + threadIdx.x;
-            const long long n = s < d.seqs ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, sum = block_scan(n, scan) + before;
-            if (n > 0 && sum - n <= last && last < sum) {
-                place[0] = s;
-                place[1] = sum - n;
-            }
-            if (threadIdx.x == kPagedThreads - 1) scan[0] = sum;
-            __syncthreads();
-            before = scan[0];
-            if (before > last) {
-                seq = (int)place[0];
-                seq_before = place[1];
-                break;
-            }
-            __syncthreads();
-        }
-        const int steps = paged_range(d, seq, P.shift).steps;
-        item = (int)((last - seq_before) / steps);
-        begin = seq_before + (long long)item * steps;
-        end = begin + steps;
-        split = end > last + 1 && begin >= share * blockIdx.x;
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!split) return;
-    const int count = (int)((end - 1) / share) - (int)blockIdx.x + 1;
+    const int warp = threadIdx.x >> 5;
+    const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
+    const int per_seq = d.k_heads * P.chunks, seq = blockIdx.x / per_seq, item = blockIdx.x - seq * per_seq;
     const int kh = item / P.chunks, chunk = item - kh * P.chunks;
     const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
-    // the first piece is its CTA's second result, the others are their CTAs' first
-    auto piece = [&](int i) { return P.part + ((long long)(blockIdx.x + i) * 2 + (i == 0)) * S::kPart; };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    PagedHeads<DP, BF16> heads;
+    heads.start(d, seq, h0, rows);
+    const PagedRange R = paged_range(d, seq, P.shift);
+    const int mine = (R.steps + kPagedWarps - 1) / kPagedWarps, s0 = warp * mine, s1 = min(s0 + mine, R.steps);
+    static_assert(kPagedWhole / kPagedStep / kPagedWarps <= 32, "one look at the table");
+    PagedPages pages;
+    bool bad = R.bad != 0;
+    if (!pages.look(d, P.shift, seq, R, s0, s1)) bad = true;
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+        if (s0 + i < s1) paged_load<DP>(d, R, pages, kh, s0 + i, ring + i * 2 * S::kTileBytes);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    for (int s = s0, stage = 0; s < s1; ++s) {
+        const int ahead = s + S::kStages - 1;
+        if (ahead < s1) paged_load<DP>(d, R, pages, kh, ahead, ring + (stage == 0 ? S::kStages - 1 : stage - 1) * 2 * S::kTileBytes);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+        __syncwarp();
+        heads.step(R, s, P.factor, ring + stage * 2 * S::kTileBytes);
+        __syncwarp();
+        if (++stage == S::kStages) stage = 0;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    heads.finish(__syncthreads_or(bad));
+    heads.save(reinterpret_cast<float*>(smem) + warp * S::kPart, rows);
+    __syncthreads();
     for (int i = threadIdx.x; i < rows * (DP / 2); i += kPagedThreads) {
         const int row = i / (DP / 2), col = 2 * (i - row * (DP / 2));
+        const float* at = reinterpret_cast<const float*>(smem) + row * S::kRow;
         float top = -INFINITY;
-        for (int k = 0; k < count; ++k) top = fmaxf(top, __ldcg(piece(k) + row * (DP + 2) + DP));
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, at[w * S::kPart + DP]);
         const float base = top == -INFINITY ? 0.f : top;
         float sum = 0.f;
         float2 v = make_float2(0.f, 0.f);
-        for (int k = 0; k < count; ++k) {
-            const float* at = piece(k) + row * (DP + 2);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + DP)), u = __ldcg(reinterpret_cast<const float2*>(at + col));
-            const float e = exp2_approx(ml.x - base);
-            sum += ml.y * e;
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) {
+            const float e = exp2_approx(at[w * S::kPart + DP] - base);
+            const float2 u = *reinterpret_cast<const float2*>(at + w * S::kPart + col);
+            sum += at[w * S::kPart + DP + 1] * e;
             v.x += u.x * e;
             v.y += u.y * e;
         }
@@ -440,29 +486,139 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_
     }
 }
 
+// The results of items that lie in several warps of the split kernel.  A CTA has one such item (of few items: the one of its number; of many: the one whose first
+// part is at the end of the warp of its number), all of its heads or (gridDim.y) one of them.  The pieces' weights 2^(m - largest m) first, then sums
+// over the pieces, column by column, by groups of threads that take turns and add up in their order.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kPagedJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams P) {
+    using S = PagedShape<DP>;
+    static_assert(kPagedJoinThreads == kPagedThreads, "the scan");
+    constexpr int kPairs = DP / 2, kGroups = kPagedJoinThreads / kPairs;
+    extern __shared__ float weight[];            // of the pieces
+    __shared__ PagedPlan plan;
+    __shared__ float top_of[kPagedWarps], sum_of[kPagedWarps];
+    __shared__ float2 partial[kPagedJoinThreads];
+    const nq_attention_desc& d = P.d;
+    const int per_seq = d.k_heads * P.chunks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // (the lengths are older than the kernel above, which has waited for what wrote them before it let this one start)
+    long long n, sum;
+    PagedRange range;
+    const long long total = paged_total(P, plan, n, sum, range), share = (total + P.warps - 1) / P.warps;
+    long long begin = 0, end = 0;
+    int seq, item;
+    const bool by_item = P.items <= P.warps;
+    if (by_item) {
+        // steps ahead of the sequence: the last one's sum minus its own
+        seq = blockIdx.x / per_seq;
+        item = blockIdx.x - seq * per_seq;
+        if (d.seqs <= kPagedThreads) {
+            if ((int)threadIdx.x == seq) plan.place[0] = {sum - n, seq, range};
+        } else {
+            long long before = 0;
+            for (int s0 = 0; s0 < seq; s0 += kPagedThreads) {
+                const int s = s0 + threadIdx.x;
+                long long some;
+                block_scan(s < seq ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, plan.sums, some);
+                before += some;
+            }
+            if (threadIdx.x == 0) plan.place[0] = {before, seq, paged_range(d, seq, P.shift)};
+        }
+        __syncthreads();
+    } else {
+        paged_find<1>(P, plan, n, sum, range, [&](int) { return share * (blockIdx.x + 1) - 1; });
+        if (share * (blockIdx.x + 1) - 1 >= total) {      // (the warp has none, or not all, of its steps: nothing of an item behind it)
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            return;
+        }
+        seq = plan.place[0].seq;
+        item = (int)((share * (blockIdx.x + 1) - 1 - plan.place[0].before) / plan.place[0].range.steps);
+    }
+    begin = plan.place[0].before + (long long)item * plan.place[0].range.steps;
+    end = begin + plan.place[0].range.steps;
+    const long long first = begin / share, last = (end - 1) / share;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (first == last || (!by_item && first != blockIdx.x)) return;
+    const int count = (int)(last - first) + 1;
+    const int kh = item / P.chunks, chunk = item - kh * P.chunks;
+    const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
+    const int col = 2 * (threadIdx.x % kPairs), group = threadIdx.x / kPairs;
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+        // the first piece is its warp's second result, the others are their warps' first
+        auto piece = [&](int i) { return P.part + ((first + i) * 2 + (i == 0)) * S::kPart + row * S::kRow; };
+        float top = -INFINITY;
+        for (int k = threadIdx.x; k < count; k += kPagedJoinThreads) top = fmaxf(top, __ldcg(piece(k) + DP));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        __syncthreads();                         // (the row before is done)
+        if (lane == 0) top_of[warp] = top;
+        __syncthreads();
+        for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, top_of[w]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float l = 0.f;
+        for (int k = threadIdx.x; k < count; k += kPagedJoinThreads) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(k) + DP));
+            const float e = exp2_approx(ml.x - base);
+            weight[k] = e;
+            l += ml.y * e;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) sum_of[warp] = l;
+        __syncthreads();
+        l = 0.f;
+        for (int w = 0; w < kPagedWarps; ++w) l += sum_of[w];
+        float2 v = make_float2(0.f, 0.f);
+#pragma unroll 8
+        for (int k = group; k < count; k += kGroups) {
+            const float2 u = __ldcg(reinterpret_cast<const float2*>(piece(k) + col));
+            const float e = weight[k];
+            v.x += u.x * e;
+            v.y += u.y * e;
+        }
+        if constexpr (kGroups > 1) {
+            partial[threadIdx.x] = v;
+            __syncthreads();
+            if (group == 0)
+                for (int k = 1; k < kGroups; ++k) {
+                    v.x += partial[threadIdx.x + k * kPairs].x;
+                    v.y += partial[threadIdx.x + k * kPairs].y;
+                }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (group == 0 && col < d.D)
+            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(d.out) + ((long long)seq * d.q_heads + h0 + row) * d.D + col) = head_pack<BF16>(v.x * inv, v.y * inv);
+    }
+}
+
 static int padded_columns(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int paged_ctas(int dp) { return sm_count() * (dp == 64 ? PagedShape<64>::kCtasPerSm : dp == 128 ? PagedShape<128>::kCtasPerSm : PagedShape<256>::kCtasPerSm); }
 
 template <int DP, bool BF16>
-static int paged_launch(PagedParams& P, int items, cudaStream_t stream) {
+static int paged_launch(PagedParams& P, bool whole, cudaStream_t stream) {
     static bool attr_set[64];
     int dev = 0;
     NQ_CUDA_TRY(cudaGetDevice(&dev));
-    const void* fn = (const void*)paged_kernel<DP, BF16>;
+    const void *split_fn = (const void*)paged_split_kernel<DP, BF16>, *whole_fn = (const void*)paged_whole_kernel<DP, BF16>;
     if (!attr_set[dev & 63]) {
-        NQ_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DP>::kSmem));
+        NQ_CUDA_TRY(cudaFuncSetAttribute(split_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DP>::kSmem));
+        NQ_CUDA_TRY(cudaFuncSetAttribute(whole_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DP>::kSmem));
         attr_set[dev & 63] = true;
     }
+    P.warps = paged_ctas(DP) * kPagedWarps;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(P.whole ? items : paged_ctas(DP)));
+    cfg.gridDim = dim3((unsigned)(whole ? P.items : paged_ctas(DP)));
     cfg.blockDim = dim3(kPagedThreads);
     cfg.dynamicSmemBytes = PagedShape<DP>::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     void* args[] = {&P};
-    const int st = launch_dependent(cfg, attr, 0, fn, args);
-    if (st != NQ_OK || P.whole) return st;
-    cfg.dynamicSmemBytes = 0;
+    const int st = launch_dependent(cfg, attr, 0, whole ? whole_fn : split_fn, args);
+    if (st != NQ_OK || whole) return st;
+    // a CTA for each head while that makes no more of them than the SMs take at once
+    const int joins = P.items < P.warps ? P.items : P.warps, rows = P.rows < kPagedRows ? P.rows : kPagedRows;
+    cfg.gridDim = dim3((unsigned)joins, (unsigned)((int64_t)joins * rows <= 16 * sm_count() ? rows : 1));
+    cfg.blockDim = dim3(kPagedJoinThreads);
+    cfg.dynamicSmemBytes = P.warps * sizeof(float);
     return launch_dependent(cfg, attr, 0, (const void*)paged_join_kernel<DP, BF16>, args);
 }
 
@@ -493,7 +649,7 @@ size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int 
     using namespace nq;
     if (seqs <= 0 || q_heads <= 0 || k_heads <= 0 || D <= 0 || D > kHeadMaxCols || max_tokens <= kPagedWhole) return 0;
     const int dp = padded_columns(D);
-    return (size_t)paged_ctas(dp) * 2 * kPagedRows * (dp + 2) * sizeof(float);
+    return (size_t)paged_ctas(dp) * kPagedWarps * 2 * kPagedRows * (dp + 2) * sizeof(float);
 }
 
 int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t scratch_bytes, nq_stream_t stream) {
@@ -503,7 +659,7 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     int st = attention_check(d);
     if (st == NQ_OK) st = attention_cache_check(d);
     if (st != NQ_OK) return st;
-    PagedParams P{d, log2_of(d.page_size), d.q_heads / d.k_heads, 0, 0, d.scale * 1.44269504088896340736f, static_cast<float*>(scratch)};
+    PagedParams P{d, log2_of(d.page_size), d.q_heads / d.k_heads, 0, 0, 0, d.scale * 1.44269504088896340736f, static_cast<float*>(scratch)};
     P.chunks = (P.rows + kPagedRows - 1) / kPagedRows;
     const int64_t most = (int64_t)d.max_pages * d.page_size, items = (int64_t)d.seqs * d.k_heads * P.chunks;
     if (most > 0x7fffff00 || items > 0x3fffffff) return NQ_ERR_TOO_LARGE;
@@ -513,12 +669,13 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
         if (!aligned16(scratch)) return NQ_ERR_ALIGN;
         if (scratch_bytes < need) return NQ_ERR_SCRATCH;
     }
-    P.whole = need == 0;
+    P.items = (int)items;
+    const bool whole = need == 0;
     const bool bf = d.dtype == NQ_BF16;
     switch (padded_columns(d.D)) {
-        case 64: return bf ? paged_launch<64, true>(P, (int)items, as_stream(stream)) : paged_launch<64, false>(P, (int)items, as_stream(stream));
-        case 128: return bf ? paged_launch<128, true>(P, (int)items, as_stream(stream)) : paged_launch<128, false>(P, (int)items, as_stream(stream));
-        default: return bf ? paged_launch<256, true>(P, (int)items, as_stream(stream)) : paged_launch<256, false>(P, (int)items, as_stream(stream));
+        case 64: return bf ? paged_launch<64, true>(P, whole, as_stream(stream)) : paged_launch<64, false>(P, whole, as_stream(stream));
+        case 128: return bf ? paged_launch<128, true>(P, whole, as_stream(stream)) : paged_launch<128, false>(P, whole, as_stream(stream));
+        default: return bf ? paged_launch<256, true>(P, whole, as_stream(stream)) : paged_launch<256, false>(P, whole, as_stream(stream));
     }
 }
 
