@@ -22,7 +22,6 @@ constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStep = 16;                  // tokens
 constexpr int kPagedRows = 16;                  // query heads of an item at most
 constexpr int kPagedWhole = 256;                // caches of up to so many tokens a sequence: a CTA per item
-constexpr int kPagedJoinThreads = 128;
 
 struct PagedParams {
     nq_attention_desc d;
@@ -60,9 +59,9 @@ struct PagedPlace {
 };
 struct PagedPlan {
     PagedPlace place[kPagedWarps];
-    long long sums[kPagedWarps];
+    long long sums[32];
 };
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {       // inclusive, over kPagedThreads threads
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {       // inclusive
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -73,18 +72,17 @@ __device__ __forceinline__ long long block_scan(long long v, long long* warp_sum
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
     total = 0;
-#pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) {
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
         if (w < warp) v += warp_sums[w];
         total += warp_sums[w];
     }
     return v;
 }
-// Steps of all items, and a warp's share of them.  By the whole CTA.  `first`: the sequence of this thread, for batches of up to kPagedThreads.
+// Steps of all items, and a warp's share of them.  By the whole CTA.  n, sum and range: of this thread's sequence, for batches of up to as many.
 __device__ __forceinline__ long long paged_total(const PagedParams& P, PagedPlan& plan, long long& n, long long& sum, PagedRange& range) {
     const int per_seq = P.d.k_heads * P.chunks;
     long long total = 0;
-    for (int s0 = 0; s0 < P.d.seqs; s0 += kPagedThreads) {
+    for (int s0 = 0; s0 < P.d.seqs; s0 += blockDim.x) {
         const int s = s0 + threadIdx.x;
         n = 0;
         if (s < P.d.seqs) {
@@ -106,11 +104,11 @@ __device__ __forceinline__ void paged_find(const PagedParams& P, PagedPlan& plan
         for (int w = 0; w < COUNT; ++w)
             if (n > 0 && sum - n <= unit(w) && unit(w) < sum) plan.place[w] = {sum - n, s, range};
     };
-    if (P.d.seqs <= kPagedThreads) {
+    if (P.d.seqs <= (int)blockDim.x) {
         look(threadIdx.x);
     } else {
         long long before = 0;
-        for (int s0 = 0; s0 < P.d.seqs; s0 += kPagedThreads) {
+        for (int s0 = 0; s0 < P.d.seqs; s0 += blockDim.x) {
             const int s = s0 + threadIdx.x;
             n = 0;
             if (s < P.d.seqs) {
@@ -487,35 +485,32 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
 }
 
 // The results of items that lie in several warps of the split kernel.  A CTA has one such item (of few items: the one of its number; of many: the one whose first
-// part is at the end of the warp of its number), all of its heads or (gridDim.y) one of them.  The pieces' weights 2^(m - largest m) first, then sums
-// over the pieces, column by column, by groups of threads that take turns and add up in their order.
-template <int DP, bool BF16>
-__global__ void __launch_bounds__(kPagedJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams P) {
+// part is at the end of the warp of its number), all of its heads or (gridDim.y) one of them.  The pieces' weights 2^(m - largest m) first, while
+// the first pieces are already on their way, then sums over the pieces, column by column, by groups of threads that take turns and add up in their order.
+template <int DP, bool BF16, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_constant__ PagedParams P) {
     using S = PagedShape<DP>;
-    static_assert(kPagedJoinThreads == kPagedThreads, "the scan");
-    constexpr int kPairs = DP / 2, kGroups = kPagedJoinThreads / kPairs;
+    constexpr int kPairs = DP / 2, kGroups = THREADS / kPairs, kWarps = THREADS / 32, kAhead = 8;
     extern __shared__ float weight[];            // of the pieces
     __shared__ PagedPlan plan;
-    __shared__ float top_of[kPagedWarps], sum_of[kPagedWarps];
-    __shared__ float2 partial[kPagedJoinThreads];
+    __shared__ float top_of[kWarps], sum_of[kWarps];
+    __shared__ float2 partial[THREADS];
     const nq_attention_desc& d = P.d;
     const int per_seq = d.k_heads * P.chunks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // (the lengths are older than the kernel above, which has waited for what wrote them before it let this one start)
     long long n, sum;
     PagedRange range;
     const long long total = paged_total(P, plan, n, sum, range), share = (total + P.warps - 1) / P.warps;
-    long long begin = 0, end = 0;
     int seq, item;
     const bool by_item = P.items <= P.warps;
     if (by_item) {
-        // steps ahead of the sequence: the last one's sum minus its own
         seq = blockIdx.x / per_seq;
         item = blockIdx.x - seq * per_seq;
-        if (d.seqs <= kPagedThreads) {
+        if (d.seqs <= THREADS) {
             if ((int)threadIdx.x == seq) plan.place[0] = {sum - n, seq, range};
         } else {
             long long before = 0;
-            for (int s0 = 0; s0 < seq; s0 += kPagedThreads) {
+            for (int s0 = 0; s0 < seq; s0 += THREADS) {
                 const int s = s0 + threadIdx.x;
                 long long some;
                 block_scan(s < seq ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, plan.sums, some);
@@ -533,8 +528,7 @@ __global__ void __launch_bounds__(kPagedJoinThreads) paged_join_kernel(const __g
         seq = plan.place[0].seq;
         item = (int)((share * (blockIdx.x + 1) - 1 - plan.place[0].before) / plan.place[0].range.steps);
     }
-    begin = plan.place[0].before + (long long)item * plan.place[0].range.steps;
-    end = begin + plan.place[0].range.steps;
+    const long long begin = plan.place[0].before + (long long)item * plan.place[0].range.steps, end = begin + plan.place[0].range.steps;
     const long long first = begin / share, last = (end - 1) / share;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (first == last || (!by_item && first != blockIdx.x)) return;
@@ -545,18 +539,27 @@ __global__ void __launch_bounds__(kPagedJoinThreads) paged_join_kernel(const __g
     for (int row = blockIdx.y; row < rows; row += gridDim.y) {
         // the first piece is its warp's second result, the others are their warps' first
         auto piece = [&](int i) { return P.part + ((first + i) * 2 + (i == 0)) * S::kPart + row * S::kRow; };
-        float top = -INFINITY;
-        for (int k = threadIdx.x; k < count; k += kPagedJoinThreads) top = fmaxf(top, __ldcg(piece(k) + DP));
+        auto numbers = [&](int k) { return k < count ? __ldcg(reinterpret_cast<const float2*>(piece(k) + DP)) : make_float2(-INFINITY, 0.f); };
+        const float2 mine = numbers(threadIdx.x);
+        float2 u[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int k = group + i * kGroups;
+            u[i] = k < count ? __ldcg(reinterpret_cast<const float2*>(piece(k) + col)) : make_float2(0.f, 0.f);
+        }
+        float top = mine.x;
+        for (int k = threadIdx.x + THREADS; k < count; k += THREADS) top = fmaxf(top, numbers(k).x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         __syncthreads();                         // (the row before is done)
         if (lane == 0) top_of[warp] = top;
         __syncthreads();
-        for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, top_of[w]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, top_of[w]);
         const float base = top == -INFINITY ? 0.f : top;
         float l = 0.f;
-        for (int k = threadIdx.x; k < count; k += kPagedJoinThreads) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(k) + DP));
+        for (int k = threadIdx.x; k < count; k += THREADS) {
+            const float2 ml = k == (int)threadIdx.x ? mine : numbers(k);
             const float e = exp2_approx(ml.x - base);
             weight[k] = e;
             l += ml.y * e;
@@ -566,19 +569,28 @@ __global__ void __launch_bounds__(kPagedJoinThreads) paged_join_kernel(const __g
         if (lane == 0) sum_of[warp] = l;
         __syncthreads();
         l = 0.f;
-        for (int w = 0; w < kPagedWarps; ++w) l += sum_of[w];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) l += sum_of[w];
         float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int k = group + i * kGroups;
+            if (k < count) {
+                v.x += u[i].x * weight[k];
+                v.y += u[i].y * weight[k];
+            }
+        }
 #pragma unroll 8
-        for (int k = group; k < count; k += kGroups) {
-            const float2 u = __ldcg(reinterpret_cast<const float2*>(piece(k) + col));
-            const float e = weight[k];
-            v.x += u.x * e;
-            v.y += u.y * e;
+        for (int k = group + kAhead * kGroups; k < count; k += kGroups) {
+            const float2 w = __ldcg(reinterpret_cast<const float2*>(piece(k) + col));
+            v.x += w.x * weight[k];
+            v.y += w.y * weight[k];
         }
         if constexpr (kGroups > 1) {
             partial[threadIdx.x] = v;
             __syncthreads();
             if (group == 0)
+#pragma unroll
                 for (int k = 1; k < kGroups; ++k) {
                     v.x += partial[threadIdx.x + k * kPairs].x;
                     v.y += partial[threadIdx.x + k * kPairs].y;
@@ -614,12 +626,13 @@ static int paged_launch(PagedParams& P, bool whole, cudaStream_t stream) {
     void* args[] = {&P};
     const int st = launch_dependent(cfg, attr, 0, whole ? whole_fn : split_fn, args);
     if (st != NQ_OK || whole) return st;
-    // a CTA for each head while that makes no more of them than the SMs take at once
+    // a CTA for each head while that makes no more of them than the SMs take at once; more threads where an item has many pieces
     const int joins = P.items < P.warps ? P.items : P.warps, rows = P.rows < kPagedRows ? P.rows : kPagedRows;
-    cfg.gridDim = dim3((unsigned)joins, (unsigned)((int64_t)joins * rows <= 16 * sm_count() ? rows : 1));
-    cfg.blockDim = dim3(kPagedJoinThreads);
+    const bool many = (int64_t)P.items * 8 <= P.warps;
+    cfg.gridDim = dim3((unsigned)joins, (unsigned)((int64_t)joins * rows <= 8 * sm_count() ? rows : 1));
+    cfg.blockDim = dim3(many ? 512 : 128);
     cfg.dynamicSmemBytes = P.warps * sizeof(float);
-    return launch_dependent(cfg, attr, 0, (const void*)paged_join_kernel<DP, BF16>, args);
+    return launch_dependent(cfg, attr, 0, many ? (const void*)paged_join_kernel<DP, BF16, 512> : (const void*)paged_join_kernel<DP, BF16, 128>, args);
 }
 
 // What both attention entry points ask of their cache; 0: fine.
