@@ -2,9 +2,10 @@
 //
 //     x^ = x / sqrt(mean(x^2) + eps) w        (a, b) -> (a cos - b sin, b cos + a sin) scaling,   angle = p f_i
 //
-// Bound by memory: 2 bytes in and 2 out per element, everything read once.  A CTA takes one token.  A head belongs to a group of 4, 8 or 16 lanes with
+// Bound by memory: 2 bytes in and 2 out per element, everything read once.  A head belongs to a group of 4, 8 or 16 lanes with
 // 16 elements each, so that a norm is a few shuffles; the two elements of a pair are in one lane (chunks of 8 that are R/2 apart, or neighbours).
-// The token's angles are computed once, by the CTA's threads side by side while their heads are on the way, and shared by all heads.
+// A CTA takes a range of tokens, eight at a time: their angles and places in the cache are computed once, by the CTA's threads side by side while their first
+// heads are on the way, and shared by all heads; from then on every group has its next head under way while it works on one.
 //
 // Angles.  p f leaves the precision of fp32 for far positions (131072 x 1: an angle is known to 2^-7).  It is formed in 64 bits, where the product of a position
 // below 2^29 and an fp32 frequency is exact, divided by 2 pi and reduced to half a turn there; cospi and sinpi take the rest in fp32.
@@ -17,7 +18,9 @@ struct HeadsParams {
     int shift;               // log2(page_size)
     int group;               // lanes of a head
     int w32;
+    int tokens;              // of a CTA
 };
+constexpr int kHeadsBatch = 8;        // tokens whose angles are in shared memory
 
 enum : int { kHalves = 0, kNeighbours = 1, kHalvesAnywhere = 2 };      // pairs: R/2 apart (whole chunks of 8), neighbours, R/2 apart
 
@@ -41,9 +44,9 @@ __device__ __forceinline__ float head_weight(const void* w, int w32, int c) {
 
 template <bool BF16, int PAIRS>
 __global__ void __launch_bounds__(512) heads_kernel(const __grid_constant__ HeadsParams P) {
-    extern __shared__ float4 turns[];                 // (cos, sin) of two pairs each, pair 8 g + j at [j / 2][g]
+    extern __shared__ float4 all_turns[];             // of a token: (cos, sin) of two pairs each, pair 8 g + j at [j / 2][g]
+    __shared__ long long place[kHeadsBatch];          // page and slot of a token (-1: nowhere; -2: padding)
     const nq_heads_desc& d = P.d;
-    const long long t = blockIdx.x;
     const int lanes = P.group, g = threadIdx.x & (lanes - 1), first = threadIdx.x / lanes, step = blockDim.x / lanes;
     const bool cached = d.k_cache != nullptr;
     const int chunks = d.D >> 3, half = d.R >> 4, heads = d.q_heads + d.k_heads * (cached ? 2 : 1);
@@ -56,47 +59,68 @@ __global__ void __launch_bounds__(512) heads_kernel(const __grid_constant__ Head
     const bool live0 = c0 < chunks, live1 = c1 < chunks;
     const int columns = (d.R / 2 + 7) / 8;            // of `turns`
 
-    auto source = [&](int h) -> const uint16_t* {
-        const uint16_t* p;
-        if (h < d.q_heads) p = static_cast<const uint16_t*>(d.q) + t * d.q_token + (long long)h * d.q_head;
-        else if (h < d.q_heads + d.k_heads) p = static_cast<const uint16_t*>(d.k) + t * d.k_token + (long long)(h - d.q_heads) * d.k_head;
-        else p = static_cast<const uint16_t*>(d.v) + t * d.v_token + (long long)(h - d.q_heads - d.k_heads) * d.v_head;
-        return p;
+    auto source = [&](long long t, int h) -> const uint16_t* {
+        if (h < d.q_heads) return static_cast<const uint16_t*>(d.q) + t * d.q_token + (long long)h * d.q_head;
+        if (h < d.q_heads + d.k_heads) return static_cast<const uint16_t*>(d.k) + t * d.k_token + (long long)(h - d.q_heads) * d.k_head;
+        return static_cast<const uint16_t*>(d.v) + t * d.v_token + (long long)(h - d.q_heads - d.k_heads) * d.v_head;
     };
     const uint4 zero = make_uint4(0, 0, 0, 0);
+    const long long from = (long long)blockIdx.x * P.tokens, to = min(from + P.tokens, (long long)d.T);
+    // a group's heads: those of the token, then those of the next
+    auto forward = [&](long long& t, int& h) {
+        h += step;
+        while (h >= heads) { h -= heads; ++t; }
+    };
+    long long t = from, next_t;
+    int h = first, next_h;
+    while (h >= heads) { h -= heads; ++t; }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint4 r0 = zero, r1 = zero;
-    if (first < heads) {
-        const uint16_t* p = source(first);
+    if (t < to) {
+        const uint16_t* p = source(t, h);
         if (live0) r0 = __ldcg(reinterpret_cast<const uint4*>(p) + c0);
         if (live1) r1 = __ldcg(reinterpret_cast<const uint4*>(p) + c1);
     }
-    const long long pos = d.position_bits == 64 ? static_cast<const long long*>(d.positions)[t] : static_cast<const int*>(d.positions)[t];
-    // where the token lies in the cache: page and slot, or nowhere
-    long long page = -1;
-    if (cached && pos >= 0) {
-        const long long seq = d.sequences ? d.sequences[t] : t, n = pos >> P.shift;
-        if (seq >= 0 && seq < d.seqs && n < d.max_pages) page = d.block_table[seq * d.table_stride + n];
-        if (page >= d.pages) page = -1;
-    }
-    const int slot = (int)(pos & (d.page_size - 1));
-    for (int i = threadIdx.x; i < d.R / 2; i += blockDim.x) {
-        const double turn = (double)pos * (double)d.inv_freq[i] * 0.15915494309189533577;      // 1 / (2 pi)
-        float s, c;
-        sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
-        float2* at = reinterpret_cast<float2*>(turns + ((i & 7) >> 1) * columns + (i >> 3)) + (i & 1);
-        *at = make_float2(c * d.scaling, s * d.scaling);
-    }
-    __syncthreads();
+    for (long long base = from; base < to; base += kHeadsBatch) {
+      const int batch = (int)min((long long)kHeadsBatch, to - base);
+      auto position = [&](long long at) -> long long {
+          return d.position_bits == 64 ? __ldcg(static_cast<const long long*>(d.positions) + at) : __ldcg(static_cast<const int*>(d.positions) + at);
+      };
+      if (base > from) __syncthreads();               // (the angles before are not needed any more)
+      if (cached && (int)threadIdx.x < batch) {
+          const long long at = base + threadIdx.x, pos = position(at);
+          long long page = -1;
+          if (pos >= 0) {
+              const long long seq = d.sequences ? __ldcg(d.sequences + at) : at, n = pos >> P.shift;
+              if (seq >= 0 && seq < d.seqs && n < d.max_pages) page = __ldcg(d.block_table + seq * d.table_stride + n);
+              if (page >= d.pages) page = -1;
+          }
+          place[threadIdx.x] = pos < 0 ? -2 : page < 0 ? -1 : page << P.shift | (pos & (d.page_size - 1));
+      }
+      for (int i = threadIdx.x; i < batch * (d.R / 2); i += blockDim.x) {
+          const int b = i / (d.R / 2), k = i - b * (d.R / 2);
+          const double turn = (double)position(base + b) * (double)d.inv_freq[k] * 0.15915494309189533577;      // 1 / (2 pi)
+          float s, c;
+          sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
+          float2* at = reinterpret_cast<float2*>(all_turns + (b * 4 + ((k & 7) >> 1)) * columns + (k >> 3)) + (k & 1);
+          *at = make_float2(c * d.scaling, s * d.scaling);
+      }
+      __syncthreads();
 
-    for (int h = first; h < heads; h += step) {
+      for (; t < base + batch; t = next_t, h = next_h) {
         uint4 n0 = zero, n1 = zero;                   // the next head's, under way
-        const int next = h + step;
-        if (next < heads) {
-            const uint16_t* p = source(next);
+        next_t = t;
+        next_h = h;
+        forward(next_t, next_h);
+        if (next_t < to) {
+            const uint16_t* p = source(next_t, next_h);
             if (live0) n0 = __ldcg(reinterpret_cast<const uint4*>(p) + c0);
             if (live1) n1 = __ldcg(reinterpret_cast<const uint4*>(p) + c1);
         }
+        const float4* turns = all_turns + (int)(t - base) * 4 * columns;
+        const long long where = cached ? place[t - base] : -1;
+        const long long page = where >= 0 ? where >> P.shift : -1;
+        const int slot = (int)(where & (d.page_size - 1));
         const bool is_q = h < d.q_heads, is_v = h >= d.q_heads + d.k_heads;
         uint16_t* out = nullptr;
         if (is_q) out = static_cast<uint16_t*>(d.q_out) + (t * d.q_heads + h) * d.D;
@@ -160,7 +184,7 @@ __global__ void __launch_bounds__(512) heads_kernel(const __grid_constant__ Head
                 }
             } else {
                 // an element's partner lies anywhere in the head: read again, from L1 or L2
-                const uint16_t* p = source(h);
+                const uint16_t* p = source(t, h);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int c = 16 * g + e, i = c < d.R / 2 ? c : c - d.R / 2;
@@ -174,7 +198,7 @@ __global__ void __launch_bounds__(512) heads_kernel(const __grid_constant__ Head
                     }
                 }
             }
-            const bool padding = cached && pos < 0;
+            const bool padding = where == -2;
             r0 = padding ? zero : make_uint4(head_pack<BF16>(x[0][0], x[0][1]), head_pack<BF16>(x[0][2], x[0][3]), head_pack<BF16>(x[0][4], x[0][5]), head_pack<BF16>(x[0][6], x[0][7]));
             r1 = padding ? zero : make_uint4(head_pack<BF16>(x[1][0], x[1][1]), head_pack<BF16>(x[1][2], x[1][3]), head_pack<BF16>(x[1][4], x[1][5]), head_pack<BF16>(x[1][6], x[1][7]));
         }
@@ -182,6 +206,7 @@ __global__ void __launch_bounds__(512) heads_kernel(const __grid_constant__ Head
         if (out && live1) reinterpret_cast<uint4*>(out)[c1] = r1;
         r0 = n0;
         r1 = n1;
+      }
     }
 }
 
@@ -212,14 +237,17 @@ int nq_heads_fwd(const nq_heads_desc* desc, nq_stream_t stream) {
                     (const char*)d.q_weight, (const char*)d.k_weight) ||
         !aligned_to(4, (const char*)d.inv_freq, (const char*)d.sequences, (const char*)d.block_table) || !aligned_to((unsigned)d.position_bits / 8, (const char*)d.positions))
         return NQ_ERR_ALIGN;
-    HeadsParams P{d, log2_of(cached ? d.page_size : 8), 1, d.weight_dtype == NQ_F32};
+    HeadsParams P{d, log2_of(cached ? d.page_size : 8), 1, d.weight_dtype == NQ_F32, 1};
     while (16 * P.group < d.D) P.group *= 2;
     const int heads = d.q_heads + d.k_heads * (cached ? 2 : 1);
     const int64_t lanes = (int64_t)heads * P.group;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)d.T);
     cfg.blockDim = dim3((unsigned)(lanes >= 512 ? 512 : (lanes + 31) / 32 * 32));
-    cfg.dynamicSmemBytes = (size_t)4 * ((d.R / 2 + 7) / 8) * sizeof(float4);
+    // as many CTAs as fit the SMs at once, a token each at least
+    const int64_t most = (int64_t)sm_count() * (1024 / cfg.blockDim.x > 16 ? 16 : 1024 / cfg.blockDim.x);
+    P.tokens = (int)((d.T + most - 1) / most);
+    cfg.gridDim = dim3((unsigned)((d.T + P.tokens - 1) / P.tokens));
+    cfg.dynamicSmemBytes = (size_t)4 * kHeadsBatch * ((d.R / 2 + 7) / 8) * sizeof(float4);
     cfg.stream = as_stream(stream);
     const int pairs = d.interleaved ? kNeighbours : d.R % 16 == 0 ? kHalves : kHalvesAnywhere;
     const void* fn[2][3] = {{(const void*)heads_kernel<false, kHalves>, (const void*)heads_kernel<false, kNeighbours>, (const void*)heads_kernel<false, kHalvesAnywhere>},
