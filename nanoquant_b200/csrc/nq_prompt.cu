@@ -18,6 +18,8 @@
 // The maximum m is moved, and O multiplied accordingly, only when it grows by more than 2^8: P and its sum have room for that, and the result does not depend on m.
 // The weights P are rounded to the operands' 16-bit type for the product with the values (what the tensor cores take): 2^-9 (bf16) or 2^-12 (fp16) of each, not
 // enlarged by the average over tokens.
+#include <type_traits>
+
 #include "nq_attn.cuh"
 #include "nq_mm.cuh"
 
@@ -53,6 +55,7 @@ template <int DP> struct PromptShape {
 };
 constexpr int kPromptRegsLaunch = 168, kPromptRegsIssue = 56, kPromptRegsSoftmax = 224;      // of a thread: at launch, and after the split
 static_assert(128 * kPromptRegsIssue + 256 * kPromptRegsSoftmax <= 384 * kPromptRegsLaunch, "register split");
+constexpr int kPromptPoly = 2;                                    // of eight pairs of exponentials: on the FMA pipe
 constexpr float kPromptSlack = 8.f;                               // powers of two by which a maximum may be behind
 
 struct PromptBlock {
@@ -79,6 +82,37 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
                    "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two finite x up to 2^7 on the FMA pipe: x = n + f with |f| <= 1/2 (by adding 1.5 2^23, whose last bits then are n), a polynomial in f (minimax of the relative
+// error by Remez' exchange: degree 3 to 7.5e-5 for weights that are rounded to bf16, 2^-9; degree 4 to 2.7e-6 for fp16, 2^-12), and n added to the exponent.
+template <bool BF16>
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
+    float x, y;
+    pair_split(x2, x, y);
+    x2 = pair_of(fmaxf(x, -126.f), fmaxf(y, -126.f));
+    const uint64_t big = pair_of(12582912.f, 12582912.f), minus = pair_of(-1.f, -1.f);
+    const uint64_t t2 = pair_add(x2, big), f2 = pair_fma(pair_add(t2, pair_of(-12582912.f, -12582912.f)), minus, x2);
+    uint64_t p2;
+    if constexpr (BF16) {
+        p2 = pair_fma(f2, pair_of(0.0551716691f, 0.0551716691f), pair_of(0.242611122f, 0.242611122f));
+        p2 = pair_fma(f2, p2, pair_of(0.693260985f, 0.693260985f));
+        p2 = pair_fma(f2, p2, pair_of(0.999928074f, 0.999928074f));
+    } else {
+        p2 = pair_fma(f2, pair_of(0.00957010191f, 0.00957010191f), pair_of(0.0559178603f, 0.0559178603f));
+        p2 = pair_fma(f2, p2, pair_of(0.240247448f, 0.240247448f));
+        p2 = pair_fma(f2, p2, pair_of(0.693121815f, 0.693121815f));
+        p2 = pair_fma(f2, p2, pair_of(0.999999261f, 0.999999261f));
+    }
+    float px, py, tx, ty;
+    pair_split(p2, px, py);
+    pair_split(t2, tx, ty);
+    return pair_of(__uint_as_float(__float_as_uint(px) + (__float_as_uint(tx) << 23)), __uint_as_float(__float_as_uint(py) + (__float_as_uint(ty) << 23)));
+}
+
 // The block that CTA `index` (of a key head) has, by one warp; false: none.
 __device__ __forceinline__ bool prompt_block(const PromptParams& P, int index, int block_tokens, PromptBlock& B) {
     const nq_attention_desc& d = P.d;
@@ -143,12 +177,13 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     auto bar_s = [&](int i) { return bar_q + 16 + 8 * i; };           // S is there (by tile, or with one tile by buffer)
     auto bar_p = [&](int i) { return bar_q + 32 + 8 * i; };           // P is there
     auto bar_o = [&](int i) { return bar_q + 48 + 8 * i; };           // P V has been added (by tile)
+    auto bar_h = [&](int i) { return bar_q + 64 + 8 * i; };           // the second half of P is there (two tiles)
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 256);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 260);
     volatile int* bad_page = reinterpret_cast<volatile int*>(smem + 264);
     volatile int* have = reinterpret_cast<volatile int*>(smem + 268);
     volatile PromptBlock* block = reinterpret_cast<volatile PromptBlock*>(smem + 272);
-    static_assert(8 * kBars + 64 <= 256, "shared memory map");
+    static_assert(8 * kBars + 80 <= 256, "shared memory map");
 
     const int kh = blockIdx.x % d.k_heads, index = blockIdx.x / d.k_heads, block_tokens = kTiles * P.tokens;
     if (warp == 2) {
@@ -160,6 +195,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             mbar_init(bar_s(lane), 1);
             mbar_init(bar_p(lane), 4);
             mbar_init(bar_o(lane), 1);
+            mbar_init(bar_h(lane), 4);
         }
         if (lane == 0) {
             mbar_init(bar_q, 1);
@@ -279,13 +315,13 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                                          kd + (uint64_t)(((k >> 2) * kKeys * 128 + (k & 3) * 32) >> 4), P.idesc_s, k > 0);
                     mm_commit<1>(bar_s(i + b));
                 };
-                auto product_o = [&](int i, int b, uint32_t vt, bool more) {
+                // with 64 keys, `half` 0 or 1 of a step
+                auto product_o = [&](int i, int b, uint32_t vt, int half, bool more) {
                     // values: 64 columns to a 128-byte row, a row to a key; the next 64 columns kKeys rows on
                     const uint64_t vd = (umma_desc_mn(vt) & ~(0x3FFFull << 16)) | ((uint64_t)((kKeys * 128) >> 4) << 16);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        prompt_mma_ts(tmem + Sh::kOCol + i * DP, tmem + (i + b) * kKeys + 8 * k, vd + (uint64_t)((k * 2048) >> 4), P.idesc_o, more || k > 0);
-                    mm_commit<1>(bar_o(i));
+                    for (int k = 0; k < 4; ++k)
+                        prompt_mma_ts(tmem + Sh::kOCol + i * DP, tmem + (i + b) * kKeys + 32 * half + 8 * k, vd + (uint64_t)(((4 * half + k) * 2048) >> 4), P.idesc_o, more || k > 0);
                 };
                 bool ok = wait(bar_q, 0) && wait(bar_full(0), 0);
                 if (ok) {
@@ -308,7 +344,8 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                         }
                         ok = wait(bar_full(nv % kStages), parity(nv)) && wait(bar_p(b), (uint32_t)(j >> 1) & 1u);
                         if (!ok) break;
-                        product_o(0, b, stage(nv), j > 0);
+                        product_o(0, b, stage(nv), 0, j > 0);
+                        mm_commit<1>(bar_o(0));
                     } else {
                         ok = wait(bar_full(nv % kStages), parity(nv));
                         bool keys = false;
@@ -317,7 +354,11 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                             if (!ok || j >= steps[i]) continue;
                             ok = wait(bar_p(i), (uint32_t)j & 1u);
                             if (!ok) continue;
-                            product_o(i, 0, stage(nv), j > 0);
+                            product_o(i, 0, stage(nv), 0, j > 0);
+                            ok = wait(bar_h(i), (uint32_t)j & 1u);
+                            if (!ok) continue;
+                            product_o(i, 0, stage(nv), 1, true);
+                            mm_commit<1>(bar_o(i));
                             if (j + 1 < steps[i]) {
                                 if (!keys) ok = wait(bar_full(nk % kStages), parity(nk));
                                 keys = true;
@@ -371,18 +412,25 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
 #pragma unroll
             for (int c = 0; c < kKeys / 32; ++c) mm_tmem_use(r[c]);
             const int key = k_first + j * kKeys;
-            if (__any_sync(0xffffffffu, key < begin || key + kKeys > end)) {
+            const bool masked = __any_sync(0xffffffffu, key < begin || key + kKeys > end);
+            if (masked) {
                 const int lo = begin - key, hi = end - key;
 #pragma unroll
                 for (int c = 0; c < kKeys; ++c)
                     if (c < lo || c >= hi) r[c >> 5][c & 31] = 0xff800000u;
             }
-            float top[4];
+            float top[4];                          // (NaN where there is one)
 #pragma unroll
             for (int c = 0; c < 4; ++c) top[c] = __uint_as_float(r[0][c]);
 #pragma unroll
-            for (int c = 4; c < kKeys; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(r[c >> 5][c & 31]));
-            const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.factor;
+            for (int c = 4; c < kKeys; c += 8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (c + 4 + e < kKeys) top[e] = max3_or_nan(top[e], __uint_as_float(r[c >> 5][(c & 31) + e]), __uint_as_float(r[(c + 4) >> 5][((c + 4) & 31) + e]));
+                    else top[e] = max_or_nan(top[e], __uint_as_float(r[c >> 5][(c & 31) + e]));
+                }
+            }
+            const float peak = max_or_nan(max_or_nan(top[0], top[1]), max_or_nan(top[2], top[3])) * P.factor;
             const bool grow = peak > m + kPromptSlack;
             if (__any_sync(0xffffffffu, grow)) {
                 const float to = grow ? peak : m, shrink = grow ? exp2_approx(m - to) : 1.f;
@@ -407,34 +455,48 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             const float base = m == -INFINITY ? 0.f : m;
             const uint64_t factor2 = pair_of(P.factor, P.factor), base2 = pair_of(-base, -base);
             uint64_t sum2[2] = {0, 0};
-#pragma unroll
-            for (int c = 0; c < kKeys / 64; ++c) {
+            // FAST: some of the exponentials by the FMA pipe.  (Scores that are not finite or not seen take the others.)
+            auto weights = [&](auto fast, int half) {
                 uint32_t w[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    const uint32_t(&v)[32] = r[2 * c + (e >> 4)];
+                    const uint32_t(&v)[32] = r[2 * half + (e >> 4)];
+                    uint64_t x2 = pair_fma(pair_of(__uint_as_float(v[2 * (e & 15)]), __uint_as_float(v[2 * (e & 15) + 1])), factor2, base2);
                     float x, y;
-                    pair_split(pair_fma(pair_of(__uint_as_float(v[2 * (e & 15)]), __uint_as_float(v[2 * (e & 15) + 1])), factor2, base2), x, y);
-                    x = exp2_approx(x);
-                    y = exp2_approx(y);
-                    sum2[e & 1] = pair_add(sum2[e & 1], pair_of(x, y));
+                    if (decltype(fast)::value && (e & 7) < kPromptPoly) {
+                        x2 = exp2_pair<BF16>(x2);
+                        pair_split(x2, x, y);
+                    } else {
+                        pair_split(x2, x, y);
+                        x = exp2_approx(x);
+                        y = exp2_approx(y);
+                        x2 = pair_of(x, y);
+                    }
+                    sum2[e & 1] = pair_add(sum2[e & 1], x2);
                     w[e] = head_pack<BF16>(x, y);
                 }
-                tmem_st32(s_at + 32 * c, w);
+                tmem_st32(s_at + 32 * half, w);
+            };
+            const bool plain = __any_sync(0xffffffffu, masked || !(fabsf(peak) < INFINITY) || m == -INFINITY);
+#pragma unroll
+            for (int half = 0; half < kKeys / 64; ++half) {
+                if (plain) weights(std::false_type(), half);
+                else weights(std::true_type(), half);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                // (one tile: S(j) says nothing about the P V before this one, and two phases behind would look like none)
+                if (kTiles == 1 && j > 0) {
+                    ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
+                    if (!ok) break;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(half ? bar_h(i) : bar_p(b));
             }
+            if (!ok) break;
             float a0, a1, b0, b1;
             pair_split(sum2[0], a0, a1);
             pair_split(sum2[1], b0, b1);
             l += (a0 + a1) + (b0 + b1);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_fence_before();
-            // (one tile: S(j) says nothing about the P V before this one, and two phases behind would look like none)
-            if (kTiles == 1 && j > 0) {
-                ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
-                if (!ok) break;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p(b));
         }
         if (ok && n > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(n - 1) & 1u, abort_flag, P.status, P.wait_limit);
         tc_fence_after();
