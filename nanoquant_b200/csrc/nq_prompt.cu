@@ -43,6 +43,7 @@ struct alignas(64) PromptParams {
 template <int DP> struct PromptShape {
     static constexpr int kTiles = DP <= 128 ? 2 : 1;
     static constexpr int kKeys = DP <= 128 ? 128 : 64;            // of a step
+    static constexpr int kEarly = kTiles == 2 ? 3 : 2;            // 32s of keys whose weights are handed over first
     static constexpr int kColumns = DP / 64;                      // 128-byte columns of a row
     static constexpr int kTileBytes = 128 * DP * 2;               // queries
     static constexpr int kStageBytes = kKeys * DP * 2;
@@ -53,9 +54,8 @@ template <int DP> struct PromptShape {
     static constexpr int kOCol = 256;                             // tensor memory: S at 0, O from here
     static_assert(kSmem <= 227 * 1024 && kOCol + kTiles * DP <= 512, "shared and tensor memory");
 };
-constexpr int kPromptRegsLaunch = 168, kPromptRegsIssue = 56, kPromptRegsSoftmax = 224;      // of a thread: at launch, and after the split
+constexpr int kPromptRegsLaunch = 168, kPromptRegsIssue = 88, kPromptRegsSoftmax = 208;      // of a thread: at launch, and after the split
 static_assert(128 * kPromptRegsIssue + 256 * kPromptRegsSoftmax <= 384 * kPromptRegsLaunch, "register split");
-constexpr int kPromptPoly = 2;                                    // of eight pairs of exponentials: on the FMA pipe
 constexpr float kPromptSlack = 8.f;                               // powers of two by which a maximum may be behind
 
 struct PromptBlock {
@@ -82,37 +82,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
                    "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 __device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of two finite x up to 2^7 on the FMA pipe: x = n + f with |f| <= 1/2 (by adding 1.5 2^23, whose last bits then are n), a polynomial in f (minimax of the relative
-// error by Remez' exchange: degree 3 to 7.5e-5 for weights that are rounded to bf16, 2^-9; degree 4 to 2.7e-6 for fp16, 2^-12), and n added to the exponent.
-template <bool BF16>
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
-    float x, y;
-    pair_split(x2, x, y);
-    x2 = pair_of(fmaxf(x, -126.f), fmaxf(y, -126.f));
-    const uint64_t big = pair_of(12582912.f, 12582912.f), minus = pair_of(-1.f, -1.f);
-    const uint64_t t2 = pair_add(x2, big), f2 = pair_fma(pair_add(t2, pair_of(-12582912.f, -12582912.f)), minus, x2);
-    uint64_t p2;
-    if constexpr (BF16) {
-        p2 = pair_fma(f2, pair_of(0.0551716691f, 0.0551716691f), pair_of(0.242611122f, 0.242611122f));
-        p2 = pair_fma(f2, p2, pair_of(0.693260985f, 0.693260985f));
-        p2 = pair_fma(f2, p2, pair_of(0.999928074f, 0.999928074f));
-    } else {
-        p2 = pair_fma(f2, pair_of(0.00957010191f, 0.00957010191f), pair_of(0.0559178603f, 0.0559178603f));
-        p2 = pair_fma(f2, p2, pair_of(0.240247448f, 0.240247448f));
-        p2 = pair_fma(f2, p2, pair_of(0.693121815f, 0.693121815f));
-        p2 = pair_fma(f2, p2, pair_of(0.999999261f, 0.999999261f));
-    }
-    float px, py, tx, ty;
-    pair_split(p2, px, py);
-    pair_split(t2, tx, ty);
-    return pair_of(__uint_as_float(__float_as_uint(px) + (__float_as_uint(tx) << 23)), __uint_as_float(__float_as_uint(py) + (__float_as_uint(ty) << 23)));
-}
-
 // The block that CTA `index` (of a key head) has, by one warp; false: none.
 __device__ __forceinline__ bool prompt_block(const PromptParams& P, int index, int block_tokens, PromptBlock& B) {
     const nq_attention_desc& d = P.d;
@@ -177,7 +156,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     auto bar_s = [&](int i) { return bar_q + 16 + 8 * i; };           // S is there (by tile, or with one tile by buffer)
     auto bar_p = [&](int i) { return bar_q + 32 + 8 * i; };           // P is there
     auto bar_o = [&](int i) { return bar_q + 48 + 8 * i; };           // P V has been added (by tile)
-    auto bar_h = [&](int i) { return bar_q + 64 + 8 * i; };           // the second half of P is there (two tiles)
+    auto bar_h = [&](int i) { return bar_q + 64 + 8 * i; };           // the rest of P is there (two tiles)
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 256);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 260);
     volatile int* bad_page = reinterpret_cast<volatile int*>(smem + 264);
@@ -315,13 +294,13 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                                          kd + (uint64_t)(((k >> 2) * kKeys * 128 + (k & 3) * 32) >> 4), P.idesc_s, k > 0);
                     mm_commit<1>(bar_s(i + b));
                 };
-                // with 64 keys, `half` 0 or 1 of a step
-                auto product_o = [&](int i, int b, uint32_t vt, int half, bool more) {
+                // with the keys [16 k0, 16 k1) of a step
+                auto product_o = [&](int i, int b, uint32_t vt, int k0, int k1, bool more) {
                     // values: 64 columns to a 128-byte row, a row to a key; the next 64 columns kKeys rows on
                     const uint64_t vd = (umma_desc_mn(vt) & ~(0x3FFFull << 16)) | ((uint64_t)((kKeys * 128) >> 4) << 16);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        prompt_mma_ts(tmem + Sh::kOCol + i * DP, tmem + (i + b) * kKeys + 32 * half + 8 * k, vd + (uint64_t)(((4 * half + k) * 2048) >> 4), P.idesc_o, more || k > 0);
+                    for (int k = k0; k < k1; ++k)
+                        prompt_mma_ts(tmem + Sh::kOCol + i * DP, tmem + (i + b) * kKeys + 8 * k, vd + (uint64_t)((k * 2048) >> 4), P.idesc_o, more || k > 0);
                 };
                 bool ok = wait(bar_q, 0) && wait(bar_full(0), 0);
                 if (ok) {
@@ -344,7 +323,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                         }
                         ok = wait(bar_full(nv % kStages), parity(nv)) && wait(bar_p(b), (uint32_t)(j >> 1) & 1u);
                         if (!ok) break;
-                        product_o(0, b, stage(nv), 0, j > 0);
+                        product_o(0, b, stage(nv), 0, 2 * Sh::kEarly, j > 0);
                         mm_commit<1>(bar_o(0));
                     } else {
                         ok = wait(bar_full(nv % kStages), parity(nv));
@@ -354,10 +333,10 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                             if (!ok || j >= steps[i]) continue;
                             ok = wait(bar_p(i), (uint32_t)j & 1u);
                             if (!ok) continue;
-                            product_o(i, 0, stage(nv), 0, j > 0);
+                            product_o(i, 0, stage(nv), 0, 2 * Sh::kEarly, j > 0);
                             ok = wait(bar_h(i), (uint32_t)j & 1u);
                             if (!ok) continue;
-                            product_o(i, 0, stage(nv), 1, true);
+                            product_o(i, 0, stage(nv), 2 * Sh::kEarly, kKeys / 16, true);
                             mm_commit<1>(bar_o(i));
                             if (j + 1 < steps[i]) {
                                 if (!keys) ok = wait(bar_full(nk % kStages), parity(nk));
@@ -389,6 +368,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
         }
     } else {
         // ---------------------------------------------------------------- softmax
+        constexpr int kChunks = kKeys / 32, kEarly = Sh::kEarly;
         if constexpr (kTiles == 2) regs_up<kPromptRegsSoftmax>();
         const int i = (warp - 4) >> 2, row = 32 * (warp & 3) + lane;
         const int token = row / P.rows, t = first + i * P.tokens + token;
@@ -396,7 +376,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
         const int begin = sees_begin(t), end = live ? sees_end(t) : 0;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t o_at = tmem + lanes + Sh::kOCol + i * DP;
-        float m = -INFINITY, l = 0.f;
+        float m = live ? -INFINITY : 0.f, l = 0.f;      // (rows that are not there hold nobody up)
         const int n = kTiles == 1 ? most : (i == 0 ? steps[0] : steps[kTiles - 1]);
         bool ok = true;
         for (int j = 0; j < n; ++j) {
@@ -405,98 +385,129 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             if (!ok) break;
             tc_fence_after();
             const uint32_t s_at = tmem + lanes + b * kKeys;
-            uint32_t r[kKeys / 32][32];
-#pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) mm_tmem_start(s_at + 32 * c, r[c]);
-            mm_tmem_landed();
-#pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) mm_tmem_use(r[c]);
             const int key = k_first + j * kKeys;
-            const bool masked = __any_sync(0xffffffffu, key < begin || key + kKeys > end);
-            if (masked) {
-                const int lo = begin - key, hi = end - key;
-#pragma unroll
-                for (int c = 0; c < kKeys; ++c)
-                    if (c < lo || c >= hi) r[c >> 5][c & 31] = 0xff800000u;
-            }
-            float top[4];                          // (NaN where there is one)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) top[c] = __uint_as_float(r[0][c]);
-#pragma unroll
-            for (int c = 4; c < kKeys; c += 8) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (c + 4 + e < kKeys) top[e] = max3_or_nan(top[e], __uint_as_float(r[c >> 5][(c & 31) + e]), __uint_as_float(r[(c + 4) >> 5][((c + 4) & 31) + e]));
-                    else top[e] = max_or_nan(top[e], __uint_as_float(r[c >> 5][(c & 31) + e]));
-                }
-            }
-            const float peak = max_or_nan(max_or_nan(top[0], top[1]), max_or_nan(top[2], top[3])) * P.factor;
-            const bool grow = peak > m + kPromptSlack;
-            if (__any_sync(0xffffffffu, grow)) {
-                const float to = grow ? peak : m, shrink = grow ? exp2_approx(m - to) : 1.f;
-                m = to;
-                if (j > 0) {
-                    l *= shrink;
-                    ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        uint32_t v[32];
-                        mm_tmem_start(o_at + c, v);
-                        mm_tmem_landed();
-                        mm_tmem_use(v);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * shrink);
-                        tmem_st32(o_at + c, v);
-                    }
-                }
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            const uint64_t factor2 = pair_of(P.factor, P.factor), base2 = pair_of(-base, -base);
+            const bool masked = __any_sync(0xffffffffu, live && (key < begin || key + kKeys > end));
+            uint32_t r[kChunks][32], w[16];
             uint64_t sum2[2] = {0, 0};
-            // FAST: some of the exponentials by the FMA pipe.  (Scores that are not finite or not seen take the others.)
-            auto weights = [&](auto fast, int half) {
-                uint32_t w[32];
+            const uint64_t factor2 = pair_of(P.factor, P.factor);
+            auto peaks = [&](int c) {              // (NaN where there is one)
+                float top[4];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const uint32_t(&v)[32] = r[2 * half + (e >> 4)];
-                    uint64_t x2 = pair_fma(pair_of(__uint_as_float(v[2 * (e & 15)]), __uint_as_float(v[2 * (e & 15) + 1])), factor2, base2);
+                for (int u = 0; u < 4; ++u) top[u] = __uint_as_float(r[c][u]);
+#pragma unroll
+                for (int e = 4; e < 28; e += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) top[u] = max3_or_nan(top[u], __uint_as_float(r[c][e + u]), __uint_as_float(r[c][e + 4 + u]));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) top[u] = max_or_nan(top[u], __uint_as_float(r[c][28 + u]));
+                return max_or_nan(max_or_nan(top[0], top[1]), max_or_nan(top[2], top[3]));
+            };
+            // The weights of 32 keys, pairs e0 .. e1 - 1.
+            auto weights = [&](int c, int e0, int e1, uint64_t base2) {
+#pragma unroll
+                for (int e = e0; e < e1; ++e) {
                     float x, y;
-                    if (decltype(fast)::value && (e & 7) < kPromptPoly) {
-                        x2 = exp2_pair<BF16>(x2);
-                        pair_split(x2, x, y);
-                    } else {
-                        pair_split(x2, x, y);
-                        x = exp2_approx(x);
-                        y = exp2_approx(y);
-                        x2 = pair_of(x, y);
-                    }
-                    sum2[e & 1] = pair_add(sum2[e & 1], x2);
+                    pair_split(pair_fma(pair_of(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), factor2, base2), x, y);
+                    x = exp2_approx(x);
+                    y = exp2_approx(y);
+                    sum2[e & 1] = pair_add(sum2[e & 1], pair_of(x, y));
                     w[e] = head_pack<BF16>(x, y);
                 }
-                tmem_st32(s_at + 32 * half, w);
             };
-            const bool plain = __any_sync(0xffffffffu, masked || !(fabsf(peak) < INFINITY) || m == -INFINITY);
-#pragma unroll
-            for (int half = 0; half < kKeys / 64; ++half) {
-                if (plain) weights(std::false_type(), half);
-                else weights(std::true_type(), half);
+            auto total = [&]() {
+                float a0, a1, b0, b1;
+                pair_split(sum2[0], a0, a1);
+                pair_split(sum2[1], b0, b1);
+                return (a0 + a1) + (b0 + b1);
+            };
+            auto stored = [&]() {
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
-                // (one tile: S(j) says nothing about the P V before this one, and two phases behind would look like none)
-                if (kTiles == 1 && j > 0) {
-                    ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
-                    if (!ok) break;
-                }
+            };
+            auto arrive = [&](uint32_t bar) {
                 __syncwarp();
-                if (lane == 0) mbar_arrive(half ? bar_h(i) : bar_p(b));
+                if (lane == 0) mbar_arrive(bar);
+            };
+            // The last 32 keys' weights; the ones before are handed over when half of them are done, by when they have been stored.
+            auto finish = [&](uint64_t base2) {
+                constexpr int c = kChunks - 1;
+                weights(c, 0, 8, base2);
+                if (kEarly < kChunks) {
+                    stored();
+                    arrive(bar_p(b));
+                }
+                weights(c, 8, 16, base2);
+                tmem_st16(s_at + 16 * c, w);
+                stored();
+                // (one tile: S(j) says nothing about the P V before this one, and two phases behind would look like none)
+                if (kTiles == 1 && j > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
+                if (ok) arrive(kEarly < kChunks ? bar_h(b) : bar_p(b));
+            };
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) mm_tmem_start(s_at + 32 * c, r[c]);
+            mm_tmem_landed();
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) mm_tmem_use(r[c]);
+            bool done = false;
+            if (!masked && __all_sync(0xffffffffu, m > -INFINITY)) {
+                // With the maximum as it is, and without looking for this step's: as long as sums of weights stay below 2^12, so does every weight.  (Of the last
+                // 32 keys, whose weights come when the others are gone, the maximum does it.)  Half of the instructions.
+                const uint64_t base2 = pair_of(-m, -m);
+#pragma unroll
+                for (int c = 0; c + 1 < kChunks; ++c) {
+                    weights(c, 0, 16, base2);
+                    tmem_st16(s_at + 16 * c, w);
+                }
+                const bool fine = total() < 4096.f && peaks(kChunks - 1) * P.factor < m + 12.f;
+                done = __all_sync(0xffffffffu, fine || !live);
+                if (done) finish(base2);
+                else sum2[0] = sum2[1] = 0;
+            }
+            if (!done) {
+                float peak = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    if (masked) {
+                        const int lo = begin - key - 32 * c, hi = end - key - 32 * c;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (e < lo || e >= hi) r[c][e] = 0xff800000u;
+                    }
+                    peak = max_or_nan(peak, peaks(c));
+                }
+                peak *= P.factor;
+                const bool grow = peak > m + kPromptSlack;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float to = grow ? peak : m, shrink = grow ? exp2_approx(m - to) : 1.f;
+                    m = to;
+                    if (j > 0) {
+                        l *= shrink;
+                        ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DP; c += 32) {
+                            uint32_t v[32];
+                            mm_tmem_start(o_at + c, v);
+                            mm_tmem_landed();
+                            mm_tmem_use(v);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * shrink);
+                            tmem_st32(o_at + c, v);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : m;
+                const uint64_t base2 = pair_of(-base, -base);
+#pragma unroll
+                for (int c = 0; c + 1 < kChunks; ++c) {
+                    weights(c, 0, 16, base2);
+                    tmem_st16(s_at + 16 * c, w);
+                }
+                finish(base2);
             }
             if (!ok) break;
-            float a0, a1, b0, b1;
-            pair_split(sum2[0], a0, a1);
-            pair_split(sum2[1], b0, b1);
-            l += (a0 + a1) + (b0 + b1);
+            l += total();
         }
         if (ok && n > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(n - 1) & 1u, abort_flag, P.status, P.wait_limit);
         tc_fence_after();
