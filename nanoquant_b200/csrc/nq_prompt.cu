@@ -47,22 +47,48 @@ template <int DP> struct PromptShape {
     static constexpr int kColumns = DP / 64;                      // 128-byte columns of a row
     static constexpr int kTileBytes = 128 * DP * 2;               // queries
     static constexpr int kStageBytes = kKeys * DP * 2;
-    static constexpr int kStages = DP == 64 ? 8 : 5;
+    static constexpr int kStages = DP == 64 ? 8 : 4;
     static constexpr int kThreads = 128 + 128 * kTiles;
-    static constexpr int kQOff = 1024, kRingOff = kQOff + kTiles * kTileBytes;
-    static constexpr int kSmem = 1024 + kRingOff + kStages * kStageBytes;
+    static constexpr int kQOff = 1024, kRingOff = kQOff + kTiles * kTileBytes, kOutOff = kRingOff + kStages * kStageBytes;
+    static constexpr int kSmem = 1024 + kOutOff + 4 * kTiles * kMmStageOut;
     static constexpr int kOCol = 256;                             // tensor memory: S at 0, O from here
     static_assert(kSmem <= 227 * 1024 && kOCol + kTiles * DP <= 512, "shared and tensor memory");
 };
-constexpr int kPromptRegsLaunch = 168, kPromptRegsIssue = 88, kPromptRegsSoftmax = 208;      // of a thread: at launch, and after the split
+constexpr int kPromptRegsLaunch = 168, kPromptRegsIssue = 104, kPromptRegsSoftmax = 200;      // (two tiles) of a thread: at launch, and after the split
 static_assert(128 * kPromptRegsIssue + 256 * kPromptRegsSoftmax <= 384 * kPromptRegsLaunch, "register split");
+constexpr int kPromptAsk = 3;                                     // steps before a block's end, in which the next one is looked up
 constexpr float kPromptSlack = 8.f;                               // powers of two by which a maximum may be behind
 
 struct PromptBlock {
-    int seq, first;                // first token of the block, within the sequence
+    int have;                      // 1; 0: nothing to do; -1: no more blocks
+    int head;                      // key head
+    int first;                     // first token of the block, within the sequence
     int q_len, k_len;
     int q_at, k_at;                // rows of the sequence's first tokens
-    int bad;
+    int seq, bad;
+};
+// What a block has to do.  Query t is at place t + behind.
+template <int DP>
+struct PromptWork : PromptBlock {
+    int behind, k_first;           // (the first key: at the start of a page, or of a step)
+    int steps[PromptShape<DP>::kTiles], most;
+    int tail_rows;                 // of the last step, that the sequence has
+    __device__ __forceinline__ int sees_end(const PromptParams& P, int t) const { return max(0, P.d.causal ? min(k_len, t + behind + 1) : k_len); }
+    __device__ __forceinline__ int sees_begin(const PromptParams& P, int t) const { return P.d.window > 0 ? max(0, t + behind + 1 - P.d.window) : 0; }
+    __device__ __forceinline__ void read(const PromptParams& P, const volatile PromptBlock* b) {
+        have = b->have; head = b->head; first = b->first; q_len = b->q_len; k_len = b->k_len; q_at = b->q_at; k_at = b->k_at; seq = b->seq; bad = b->bad;
+        behind = k_len - q_len;
+        k_first = sees_begin(P, first) & ~(P.piece - 1);
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < PromptShape<DP>::kTiles; ++i) {
+            const int t = first + i * P.tokens, last = min(t + P.tokens, q_len) - 1;
+            steps[i] = have > 0 && t < q_len ? max(0, sees_end(P, last) - k_first + PromptShape<DP>::kKeys - 1) / PromptShape<DP>::kKeys : 0;
+            most = max(most, steps[i]);
+        }
+        tail_rows = k_len - k_first - (most - 1) * PromptShape<DP>::kKeys;
+    }
+    __device__ __forceinline__ bool fix() const { return most > 0 && tail_rows < PromptShape<DP>::kKeys; }
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -121,6 +147,7 @@ __device__ __forceinline__ bool prompt_block(const PromptParams& P, int index, i
             const int last = __shfl_sync(0xffffffffu, sum, src);           // blocks up to this sequence's end
             B.first = (last - 1 - index) * block_tokens;
             B.bad = 0;
+            B.have = 1;
             B.k_at = B.q_at;
             B.k_len = B.q_len;
             if (P.paged) {
@@ -140,6 +167,21 @@ __device__ __forceinline__ bool prompt_block(const PromptParams& P, int index, i
     return false;
 }
 
+// The next block that has not been started takes this CTA's time instead of an SM's own (16 bytes of answer); whether there was one, and its number.
+__device__ __forceinline__ void next_block_ask(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool next_block_get(uint32_t answer, int& block) {
+    uint32_t some, x;
+    asm volatile("{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+                 "ld.shared.b128 a, [%2];\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}" : "=r"(some), "=r"(x) : "r"(answer) : "memory");
+    block = (int)x;
+    return some != 0;
+}
+
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptParams P) {
     using Sh = PromptShape<DP>;
@@ -151,20 +193,24 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto bar_full = [&](int s) { return sbase + 8 * s; };
     auto bar_free = [&](int s) { return sbase + 8 * (kStages + s); };
-    constexpr int kBars = 2 * kStages;
-    const uint32_t bar_q = sbase + 8 * kBars, bar_tail = bar_q + 8;
-    auto bar_s = [&](int i) { return bar_q + 16 + 8 * i; };           // S is there (by tile, or with one tile by buffer)
-    auto bar_p = [&](int i) { return bar_q + 32 + 8 * i; };           // P is there
-    auto bar_o = [&](int i) { return bar_q + 48 + 8 * i; };           // P V has been added (by tile)
-    auto bar_h = [&](int i) { return bar_q + 64 + 8 * i; };           // the rest of P is there (two tiles)
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 256);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 260);
-    volatile int* bad_page = reinterpret_cast<volatile int*>(smem + 264);
-    volatile int* have = reinterpret_cast<volatile int*>(smem + 268);
-    volatile PromptBlock* block = reinterpret_cast<volatile PromptBlock*>(smem + 272);
-    static_assert(8 * kBars + 80 <= 256, "shared memory map");
+    const uint32_t bars = sbase + 16 * kStages;
+    const uint32_t bar_q = bars, bar_q_free = bars + 8, bar_tail = bars + 16, bar_answer = bars + 24;
+    auto bar_s = [&](int i) { return bars + 32 + 8 * i; };            // S is there (by tile, or with one tile by buffer)
+    auto bar_p = [&](int i) { return bars + 48 + 8 * i; };            // P is there, or the first of it
+    auto bar_h = [&](int i) { return bars + 64 + 8 * i; };            // the rest of P is there (two tiles)
+    auto bar_o = [&](int i) { return bars + 80 + 8 * i; };            // P V has been added (by tile)
+    auto bar_info = [&](int i) { return bars + 96 + 8 * i; };         // the number and sequence of a block are there
+    auto bar_info_free = [&](int i) { return bars + 112 + 8 * i; };
+    const uint32_t bar_ask = bars + 128;                              // a block is nearly done
+    static_assert(16 * kStages + 136 <= 272, "shared memory map");
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 272);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 276);
+    volatile int* bad_block = reinterpret_cast<volatile int*>(smem + 280);          // four: the block (counted from 1) that last had a page outside the cache
+    const uint32_t answer = sbase + 304;
+    volatile PromptBlock* info = reinterpret_cast<volatile PromptBlock*>(smem + 320);
+    static_assert(320 + 2 * sizeof(PromptBlock) <= 1024, "shared memory map");
 
-    const int kh = blockIdx.x % d.k_heads, index = blockIdx.x / d.k_heads, block_tokens = kTiles * P.tokens;
+    const int block_tokens = kTiles * P.tokens;
     if (warp == 2) {
         if (lane < kStages) {
             mbar_init(bar_full(lane), 1);
@@ -173,14 +219,19 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
         if (lane < 2) {
             mbar_init(bar_s(lane), 1);
             mbar_init(bar_p(lane), 4);
-            mbar_init(bar_o(lane), 1);
             mbar_init(bar_h(lane), 4);
+            mbar_init(bar_o(lane), 1);
+            mbar_init(bar_info(lane), 1);
+            mbar_init(bar_info_free(lane), 3 + 4 * kTiles);
         }
+        if (lane < 4) bad_block[lane] = 0;
         if (lane == 0) {
             mbar_init(bar_q, 1);
+            mbar_init(bar_q_free, 1);
             mbar_init(bar_tail, 1);
+            mbar_init(bar_answer, 1);
+            mbar_init(bar_ask, 1);
             *abort_flag = 0;
-            *bad_page = 0;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -189,94 +240,116 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(tmem_slot))), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 3) {
-        PromptBlock B;
-        const bool some = prompt_block(P, index, block_tokens, B);
-        if (lane == 0) {
-            *have = some;
-            if (some) {
-                block->seq = B.seq; block->first = B.first; block->q_len = B.q_len; block->k_len = B.k_len;
-                block->q_at = B.q_at; block->k_at = B.k_at; block->bad = B.bad;
-            }
-        }
-        // rows of no sequence
-        const int head = min(max(__ldcg(d.cu_seqlens), 0), (int)d.T), tail = min(max(__ldcg(d.cu_seqlens + d.seqs), head), (int)d.T);
-        const long long per = (long long)d.q_heads * d.D / 8, missing = ((long long)head + (d.T - tail)) * per;
-        for (long long i = (long long)blockIdx.x * 32 + lane; i < missing; i += (long long)gridDim.x * 32) {
-            const long long at = i < head * per ? i : i - head * per + tail * per;
-            static_cast<uint4*>(d.out)[at] = make_uint4(0, 0, 0, 0);
-        }
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-
-    // what the block has to do
-    const bool some = *have;
-    const int first = some ? block->first : 0, q_len = some ? block->q_len : 0, k_len = some ? block->k_len : 0, q_at = block->q_at, k_at = block->k_at;
-    const int behind = k_len - q_len;              // query t is at place t + behind
-    auto sees_end = [&](int t) { return max(0, d.causal ? min(k_len, t + behind + 1) : k_len); };
-    auto sees_begin = [&](int t) { return d.window > 0 ? max(0, t + behind + 1 - d.window) : 0; };
-    // the first key, at the start of a page (or of a step)
-    const int k_first = sees_begin(first) / P.piece * P.piece;
-    int steps[kTiles], most = 0;
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-        const int t = first + i * P.tokens, last = min(t + P.tokens, q_len) - 1;
-        steps[i] = t < q_len ? max(0, (sees_end(last) - k_first + kKeys - 1) / kKeys) : 0;
-        most = max(most, steps[i]);
-    }
-    const int tail_rows = k_len - k_first - (most - 1) * kKeys;          // of the last step, that the sequence has
-    const bool fix = most > 0 && tail_rows < kKeys;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    PromptWork<DP> B;
+    // The next block's description, for a warp that keeps it in registers; false: no more, or a wait has expired.  `n` counts blocks.
+    auto next_info = [&](int n) {
+        if (!mbar_wait_warp(bar_info(n & 1), (uint32_t)(n >> 1) & 1u, abort_flag, P.status, P.wait_limit)) return false;
+        B.read(P, info + (n & 1));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_info_free(n & 1));
+        return B.have >= 0;
+    };
 
     if (warp < 4) {
         if constexpr (kTiles == 2) regs_down<kPromptRegsIssue>();
-        if (warp == 0) {
-            // ------------------------------------------------------------ operands
-            const int* table = d.block_table + (P.paged ? (long long)block->seq * d.table_stride : 0);
-            if (most > 0 && elect_one()) {
-                const uint32_t bytes = (uint32_t)(P.rows * P.tokens * 128 * Sh::kColumns);
-                int tiles = 0;
-                for (int i = 0; i < kTiles; ++i) tiles += steps[i] > 0;
-                mbar_expect_tx(bar_q, tiles * bytes);
-                for (int i = 0; i < kTiles; ++i) {
-                    if (steps[i] == 0) continue;
-                    for (int c = 0; c < Sh::kColumns; ++c)
-                        tma_load_4d(sbase + Sh::kQOff + i * Sh::kTileBytes + c * 128 * 128, &P.map_q, 64 * c, kh * P.rows, q_at + first + i * P.tokens, 0, bar_q);
+        if (warp == 3) {
+            // ------------------------------------------------------------ which blocks
+            int index = blockIdx.x, lives = 0;
+            bool more = true;
+            for (int n = 0;; ++n) {
+                PromptBlock next{};
+                next.have = -1;
+                if (more) {
+                    next.have = 0;
+                    next.head = index % d.k_heads;
+                    prompt_block(P, index / d.k_heads, block_tokens, next);
+                    // rows of no sequence
+                    const int head = min(max(__ldcg(d.cu_seqlens), 0), (int)d.T), tail = min(max(__ldcg(d.cu_seqlens + d.seqs), head), (int)d.T);
+                    const long long per = (long long)d.q_heads * d.D / 8, missing = ((long long)head + (d.T - tail)) * per;
+                    for (long long i = (long long)index * 32 + lane; i < missing; i += (long long)gridDim.x * 32) {
+                        const long long at = i < head * per ? i : i - head * per + tail * per;
+                        static_cast<uint4*>(d.out)[at] = make_uint4(0, 0, 0, 0);
+                    }
                 }
+                if (!mbar_wait_warp(bar_info_free(n & 1), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag, P.status, P.wait_limit)) break;
+                if (lane == 0) {
+                    volatile PromptBlock* to = info + (n & 1);
+                    to->have = next.have; to->head = next.head; to->first = next.first; to->q_len = next.q_len; to->k_len = next.k_len;
+                    to->q_at = next.q_at; to->k_at = next.k_at; to->seq = next.seq; to->bad = next.bad;
+                    mbar_arrive(bar_info(n & 1));
+                }
+                __syncwarp();
+                if (!more) break;
+                // The next one is asked for near the end of this: at once, the first CTAs would take blocks that other SMs are about to start.
+                B.read(P, info + (n & 1));
+                if (B.most > 0 && !mbar_wait_warp(bar_ask, (uint32_t)lives++ & 1u, abort_flag, P.status, P.wait_limit)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(bar_answer, 16);
+                    next_block_ask(answer, bar_answer);
+                }
+                __syncwarp();
+                if (!mbar_wait_warp(bar_answer, (uint32_t)n & 1u, abort_flag, P.status, P.wait_limit)) break;
+                more = next_block_get(answer, index);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
             }
-            __syncwarp();
+        } else if (warp == 0) {
+            // ------------------------------------------------------------ operands
             const int pieces = kKeys / P.piece;
-            int s = 0;
+            int s = 0, lives = 0;
             uint32_t ph = 0;
             bool ok = true;
-            for (int j = 0; j < most && ok; ++j) {
-                const int key = k_first + j * kKeys + lane * P.piece;       // this lane's box
-                const int boxes = P.paged ? min(pieces, (k_len - (k_first + j * kKeys) + P.piece - 1) / P.piece) : 1;
-                int page = 0, row = k_at + key;
-                if (P.paged && lane < boxes) {
-                    page = __ldcg(table + (key >> P.shift));
-                    row = key & (d.page_size - 1);
-                    if (page < 0 || page >= d.pages) { page = 0; *bad_page = 1; }
-                }
-                for (int kv = 0; kv < 2 && ok; ++kv) {
-                    ok = mbar_wait_warp(bar_free(s), ph ^ 1, abort_flag, P.status, P.wait_limit);
-                    if (!ok) break;
-                    const uint32_t bar = kv == 1 && fix && j == most - 1 ? bar_tail : bar_full(s);
-                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * P.piece * 128 * Sh::kColumns));
-                    __syncwarp();
-                    if (lane < boxes) {
-                        const uint32_t dst = sbase + Sh::kRingOff + s * Sh::kStageBytes + lane * P.piece * 128;
-                        for (int c = 0; c < Sh::kColumns; ++c) tma_load_4d(dst + c * kKeys * 128, kv ? &P.map_v : &P.map_k, 64 * c, row, kh, page, bar);
+            for (int n = 0; ok && next_info(n); ++n) {
+                if (B.most == 0) continue;
+                const int* table = d.block_table + (P.paged ? (long long)B.seq * d.table_stride : 0);
+                for (int j = 0; j < B.most && ok; ++j) {
+                    const int key = B.k_first + j * kKeys + lane * P.piece;       // this lane's box
+                    const int boxes = P.paged ? min(pieces, (B.k_len - (B.k_first + j * kKeys) + P.piece - 1) / P.piece) : 1;
+                    int page = 0, row = B.k_at + key;
+                    if (P.paged && lane < boxes) {
+                        page = __ldcg(table + (key >> P.shift));
+                        row = key & (d.page_size - 1);
+                        if (page < 0 || page >= d.pages) { page = 0; bad_block[n & 3] = n + 1; }
                     }
-                    __syncwarp();
-                    if (++s == kStages) { s = 0; ph ^= 1; }
+                    for (int kv = 0; kv < 2 && ok; ++kv) {
+                        ok = mbar_wait_warp(bar_free(s), ph ^ 1, abort_flag, P.status, P.wait_limit);
+                        if (!ok) break;
+                        const uint32_t bar = kv == 1 && B.fix() && j == B.most - 1 ? bar_tail : bar_full(s);
+                        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * P.piece * 128 * Sh::kColumns));
+                        __syncwarp();
+                        if (lane < boxes) {
+                            const uint32_t dst = sbase + Sh::kRingOff + s * Sh::kStageBytes + lane * P.piece * 128;
+                            for (int c = 0; c < Sh::kColumns; ++c) tma_load_4d(dst + c * kKeys * 128, kv ? &P.map_v : &P.map_k, 64 * c, row, B.head, page, bar);
+                        }
+                        __syncwarp();
+                        if (++s == kStages) { s = 0; ph ^= 1; }
+                        if (j == 0 && kv == 0) {
+                            // (the queries behind the first keys, which need not wait for the block before)
+                            ok = mbar_wait_warp(bar_q_free, ((uint32_t)lives & 1u) ^ 1u, abort_flag, P.status, P.wait_limit);
+                            ++lives;
+                            if (ok && elect_one()) {
+                                const uint32_t bytes = (uint32_t)(P.rows * P.tokens * 128 * Sh::kColumns);
+                                int tiles = 0;
+                                for (int i = 0; i < kTiles; ++i) tiles += B.steps[i] > 0;
+                                mbar_expect_tx(bar_q, tiles * bytes);
+                                for (int i = 0; i < kTiles; ++i) {
+                                    if (B.steps[i] == 0) continue;
+                                    for (int c = 0; c < Sh::kColumns; ++c)
+                                        tma_load_4d(sbase + Sh::kQOff + i * Sh::kTileBytes + c * 128 * 128, &P.map_q, 64 * c, B.head * P.rows, B.q_at + B.first + i * P.tokens, 0, bar_q);
+                                }
+                            }
+                            __syncwarp();
+                        }
+                    }
                 }
             }
         } else if (warp == 1) {
-            if (most > 0 && elect_one()) {
+            if (elect_one()) {
                 // -------------------------------------------------------- products
                 auto wait = [&](uint32_t bar, uint32_t parity) {
                     const bool ok = mm_wait<false>(bar, parity, abort_flag, P.status, P.wait_limit);
@@ -302,86 +375,115 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     for (int k = k0; k < k1; ++k)
                         prompt_mma_ts(tmem + Sh::kOCol + i * DP, tmem + (i + b) * kKeys + 8 * k, vd + (uint64_t)((k * 2048) >> 4), P.idesc_o, more || k > 0);
                 };
-                bool ok = wait(bar_q, 0) && wait(bar_full(0), 0);
-                if (ok) {
+                int at = 0, lives = 0;             // places in the ring; blocks with keys
+                int count[kTiles] = {};            // steps of a tile
+                bool ok = true;
+                for (int n = 0; ok; ++n) {
+                    ok = wait(bar_info(n & 1), (uint32_t)(n >> 1) & 1u);
+                    if (!ok) break;
+                    B.read(P, info + (n & 1));
+                    mbar_arrive(bar_info_free(n & 1));
+                    if (B.have < 0) break;
+                    if (B.most == 0) continue;
+                    ok = wait(bar_q, (uint32_t)lives & 1u) && wait(bar_full(at % kStages), parity(at));
+                    ++lives;
+                    if (!ok) break;
 #pragma unroll
                     for (int i = 0; i < kTiles; ++i)
-                        if (steps[i] > 0) product_s(i, 0, stage(0));
-                    mm_commit<1>(bar_free(0));
-                }
-                for (int j = 0; j < most && ok; ++j) {
-                    const int nv = 2 * j + 1, nk = nv + 1;               // places of these values and of the next keys in the ring
-                    const bool next = j + 1 < most;
-                    if constexpr (kTiles == 1) {
-                        // the next S before this P: two buffers
-                        const int b = j & 1;
-                        if (next) {
-                            ok = wait(bar_full(nk % kStages), parity(nk));
-                            if (!ok) break;
-                            product_s(0, b ^ 1, stage(nk));
-                            mm_commit<1>(bar_free(nk % kStages));
-                        }
-                        ok = wait(bar_full(nv % kStages), parity(nv)) && wait(bar_p(b), (uint32_t)(j >> 1) & 1u);
-                        if (!ok) break;
-                        product_o(0, b, stage(nv), 0, 2 * Sh::kEarly, j > 0);
-                        mm_commit<1>(bar_o(0));
-                    } else {
-                        ok = wait(bar_full(nv % kStages), parity(nv));
-                        bool keys = false;
-#pragma unroll
-                        for (int i = 0; i < kTiles; ++i) {
-                            if (!ok || j >= steps[i]) continue;
-                            ok = wait(bar_p(i), (uint32_t)j & 1u);
-                            if (!ok) continue;
-                            product_o(i, 0, stage(nv), 0, 2 * Sh::kEarly, j > 0);
-                            ok = wait(bar_h(i), (uint32_t)j & 1u);
-                            if (!ok) continue;
-                            product_o(i, 0, stage(nv), 2 * Sh::kEarly, kKeys / 16, true);
-                            mm_commit<1>(bar_o(i));
-                            if (j + 1 < steps[i]) {
-                                if (!keys) ok = wait(bar_full(nk % kStages), parity(nk));
-                                keys = true;
-                                if (ok) product_s(i, 0, stage(nk));
+                        if (B.steps[i] > 0) product_s(i, kTiles == 1 ? count[0] & 1 : 0, stage(at));
+                    mm_commit<1>(bar_free(at % kStages));
+                    if (B.most == 1) mm_commit<1>(bar_q_free);
+                    for (int j = 0; j < B.most && ok; ++j) {
+                        const int nv = at + 2 * j + 1, nk = nv + 1;      // places of these values and of the next keys in the ring
+                        if (j == max(0, B.most - kPromptAsk)) mbar_arrive(bar_ask);
+                        const bool next = j + 1 < B.most;
+                        if constexpr (kTiles == 1) {
+                            // the next S before this P: two buffers
+                            const int c = count[0], b = c & 1;
+                            if (next) {
+                                ok = wait(bar_full(nk % kStages), parity(nk));
+                                if (!ok) break;
+                                product_s(0, b ^ 1, stage(nk));
+                                mm_commit<1>(bar_free(nk % kStages));
+                                if (j + 2 == B.most) mm_commit<1>(bar_q_free);
                             }
+                            ok = wait(bar_full(nv % kStages), parity(nv)) && wait(bar_p(b), (uint32_t)(c >> 1) & 1u);
+                            if (!ok) break;
+                            product_o(0, b, stage(nv), 0, 2 * Sh::kEarly, j > 0);
+                            mm_commit<1>(bar_o(0));
+                            ++count[0];
+                        } else {
+                            ok = wait(bar_full(nv % kStages), parity(nv));
+                            bool keys = false;
+#pragma unroll
+                            for (int i = 0; i < kTiles; ++i) {
+                                if (!ok || j >= B.steps[i]) continue;
+                                ok = wait(bar_p(i), (uint32_t)count[i] & 1u);
+                                if (!ok) continue;
+                                product_o(i, 0, stage(nv), 0, 2 * Sh::kEarly, j > 0);
+                                ok = wait(bar_h(i), (uint32_t)count[i] & 1u);
+                                if (!ok) continue;
+                                product_o(i, 0, stage(nv), 2 * Sh::kEarly, kKeys / 16, true);
+                                mm_commit<1>(bar_o(i));
+                                ++count[i];
+                                if (j + 1 < B.steps[i]) {
+                                    if (!keys) ok = wait(bar_full(nk % kStages), parity(nk));
+                                    keys = true;
+                                    if (ok) product_s(i, 0, stage(nk));
+                                }
+                            }
+                            if (!ok) break;
+                            if (next) mm_commit<1>(bar_free(nk % kStages));
+                            if (j + 2 == B.most) mm_commit<1>(bar_q_free);
                         }
-                        if (!ok) break;
-                        if (next) mm_commit<1>(bar_free(nk % kStages));
+                        mm_commit<1>(bar_free(nv % kStages));
                     }
-                    mm_commit<1>(bar_free(nv % kStages));
+                    at += 2 * B.most;
                 }
             }
             __syncwarp();
-        } else if (warp == 2 && fix) {
+        } else {
             // ------------------------------------------------------------ values behind the last token
-            const int n = 2 * most - 1;
-            if (mbar_wait_warp(bar_tail, 0, abort_flag, P.status, P.wait_limit)) {
-                unsigned char* at = smem + Sh::kRingOff + (n % kStages) * Sh::kStageBytes;
-                const int left = (kKeys - tail_rows) * 8;                 // 16-byte units of a column
+            int at = 0, fixes = 0;
+            for (int n = 0; next_info(n); ++n) {
+                const int last = at + 2 * B.most - 1;
+                at += 2 * B.most;
+                if (!B.fix()) continue;
+                if (!mbar_wait_warp(bar_tail, (uint32_t)fixes & 1u, abort_flag, P.status, P.wait_limit)) break;
+                ++fixes;
+                unsigned char* to = smem + Sh::kRingOff + (last % kStages) * Sh::kStageBytes;
+                const int left = (kKeys - B.tail_rows) * 8;               // 16-byte units of a column
                 for (int i = lane; i < left * Sh::kColumns; i += 32) {
                     const int c = i / left;
-                    *reinterpret_cast<uint4*>(at + c * kKeys * 128 + tail_rows * 128 + (i - c * left) * 16) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(to + c * kKeys * 128 + B.tail_rows * 128 + (i - c * left) * 16) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_full(n % kStages));
+                if (lane == 0) mbar_arrive(bar_full(last % kStages));
             }
         }
     } else {
         // ---------------------------------------------------------------- softmax
-        constexpr int kChunks = kKeys / 32, kEarly = Sh::kEarly;
         if constexpr (kTiles == 2) regs_up<kPromptRegsSoftmax>();
+        constexpr int kChunks = kKeys / 32, kEarly = Sh::kEarly;
         const int i = (warp - 4) >> 2, row = 32 * (warp & 3) + lane;
-        const int token = row / P.rows, t = first + i * P.tokens + token;
-        const bool live = token < P.tokens && t < q_len;
-        const int begin = sees_begin(t), end = live ? sees_end(t) : 0;
+        const int token = row / P.rows;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t o_at = tmem + lanes + Sh::kOCol + i * DP;
-        float m = live ? -INFINITY : 0.f, l = 0.f;      // (rows that are not there hold nobody up)
-        const int n = kTiles == 1 ? most : (i == 0 ? steps[0] : steps[kTiles - 1]);
+        const uint32_t out_stage = sbase + Sh::kOutOff + (warp - 4) * kMmStageOut;
+        const int magic = (65536 + P.rows - 1) / P.rows;                 // (x / rows = x magic / 65536 for x < 128)
+        int count = 0;                             // steps of this tile
         bool ok = true;
-        for (int j = 0; j < n; ++j) {
-            const int b = kTiles == 1 ? j & 1 : i;
-            ok = mbar_wait_warp(bar_s(b), (uint32_t)(kTiles == 1 ? j >> 1 : j) & 1u, abort_flag, P.status, P.wait_limit);
+        for (int block = 0; ok && next_info(block); ++block) {
+          if (B.have == 0) continue;
+          const int first = B.first + i * P.tokens, t = first + token, left = B.q_len - first;       // (tokens of the sequence from the tile's first on)
+          const bool live = token < P.tokens && token < left;
+          const int begin = B.sees_begin(P, t), end = live ? B.sees_end(P, t) : 0, k_first = B.k_first;
+          float m = live ? -INFINITY : 0.f, l = 0.f;      // (rows that are not there hold nobody up)
+          const int n = kTiles == 1 ? B.most : (i == 0 ? B.steps[0] : B.steps[kTiles - 1]);
+          for (int j = 0; j < n; ++j, ++count) {
+            const int b = kTiles == 1 ? count & 1 : i;
+            ok = mbar_wait_warp(bar_s(b), (uint32_t)(kTiles == 1 ? count >> 1 : count) & 1u, abort_flag, P.status, P.wait_limit);
             if (!ok) break;
             tc_fence_after();
             const uint32_t s_at = tmem + lanes + b * kKeys;
@@ -440,7 +542,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                 tmem_st16(s_at + 16 * c, w);
                 stored();
                 // (one tile: S(j) says nothing about the P V before this one, and two phases behind would look like none)
-                if (kTiles == 1 && j > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
+                if (kTiles == 1 && j > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(count - 1) & 1u, abort_flag, P.status, P.wait_limit);
                 if (ok) arrive(kEarly < kChunks ? bar_h(b) : bar_p(b));
             };
 #pragma unroll
@@ -482,7 +584,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     m = to;
                     if (j > 0) {
                         l *= shrink;
-                        ok = mbar_wait_warp(bar_o(i), (uint32_t)(j - 1) & 1u, abort_flag, P.status, P.wait_limit);
+                        ok = mbar_wait_warp(bar_o(i), (uint32_t)(count - 1) & 1u, abort_flag, P.status, P.wait_limit);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -508,37 +610,50 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             }
             if (!ok) break;
             l += total();
-        }
-        if (ok && n > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(n - 1) & 1u, abort_flag, P.status, P.wait_limit);
-        tc_fence_after();
-        const bool bad = (some && block->bad) || *bad_page;
-        const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
-        // rows through this tile's queries, which nothing reads any more, 64 columns at a time
-        unsigned char* stage = smem + Sh::kQOff + i * Sh::kTileBytes + (warp & 3) * kMmStageOut;
-        for (int c = 0; c < d.D && ok; c += 64) {
+          }
+          if (!ok) break;
+          if (n > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(count - 1) & 1u, abort_flag, P.status, P.wait_limit);
+          tc_fence_after();
+          const bool bad = B.bad || bad_block[block & 3] == block + 1;
+          const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
+          uint16_t* const out = static_cast<uint16_t*>(d.out) + ((long long)(B.q_at + first) * d.q_heads + B.head * P.rows) * d.D;
+          // 64 columns at a time through shared memory; the next block's first products run meanwhile.  (Places are computed here: kept from block to block they would
+          // take the registers that a step needs.)
+          int ln = lane;
+          asm volatile("" : "+r"(ln));
+          const uint32_t mine = out_stage + ln * 128, u = ln & 7, r0 = ln >> 3;
+#pragma unroll 1
+          for (int c = 0; c < d.D && ok; c += 64) {
+            __syncwarp();                          // (the stores before have read theirs)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                uint32_t v[32] = {}, w[16];
+                uint32_t v[32] = {};
                 if (n > 0) {
                     mm_tmem_start(o_at + c + 32 * half, v);
                     mm_tmem_landed();
                     mm_tmem_use(v);
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = head_pack<BF16>(__uint_as_float(v[2 * e]) * inv, __uint_as_float(v[2 * e + 1]) * inv);
-                mm_stage_row(stage, half, w);
-            }
-            __syncwarp();
-            const int u = lane & 7;
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int rr = 4 * k + (lane >> 3), full = 32 * (warp & 3) + rr, tok = full / P.rows, h = full - tok * P.rows;
-                if (tok < P.tokens && first + i * P.tokens + tok < q_len && c + 8 * u < d.D) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((u ^ (rr & 7)) << 4));
-                    uint16_t* out = static_cast<uint16_t*>(d.out) + ((long long)(q_at + first + i * P.tokens + tok) * d.q_heads + kh * P.rows + h) * d.D;
-                    *reinterpret_cast<uint4*>(out + c + 8 * u) = v;
+                    for (int e = 0; e < 4; ++e) w[e] = head_pack<BF16>(__uint_as_float(v[8 * q + 2 * e]) * inv, __uint_as_float(v[8 * q + 2 * e + 1]) * inv);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(mine + (((4 * half + q) ^ u) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                 }
             }
+            __syncwarp();
+            const bool column = c + 8 * (int)u < d.D;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int rr = 4 * k + r0, full = 32 * (warp & 3) + rr, tok = (full * magic) >> 16, h = full - tok * P.rows;
+                if (tok < P.tokens && tok < left && column) {
+                    uint4 x;
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(out_stage + rr * 128 + ((u ^ (rr & 7)) << 4)) : "memory");
+                    *reinterpret_cast<uint4*>(out + ((long long)tok * d.q_heads + h) * d.D + c + 8 * u) = x;
+                }
+            }
+          }
+          tc_fence_before();
         }
     }
     // On an expired wait, give the copies in flight a bounded time to land before shared memory is released.
