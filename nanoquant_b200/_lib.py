@@ -107,7 +107,8 @@ SIGNATURES = {
     "nq_heads_fwd": (c_int, [ctypes.POINTER(HeadsDesc), c_void_p]),
     "nq_paged_attention_scratch_bytes": (c_size_t, [c_int] * 4 + [c_int64]),
     "nq_paged_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_size_t, c_void_p]),
-    "nq_prompt_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_void_p]),
+    "nq_prompt_attention_scratch_bytes": (c_size_t, [ctypes.POINTER(AttentionDesc)]),
+    "nq_prompt_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_size_t, c_void_p, c_void_p]),
     "nq_gemv_max_tokens": (c_int, []),
     "nq_linear_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "nq_linear_fwd": (c_int, [c_void_p] * 8 + [c_size_t, c_int, c_int, c_int, c_int, c_int, c_void_p]),

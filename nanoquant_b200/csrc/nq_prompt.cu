@@ -34,7 +34,9 @@ struct alignas(64) PromptParams {
     int rows, tokens;              // query heads to a key head; tokens of a tile
     int piece, shift;              // keys of one box; log2(page_size)
     int paged;
+    int splits, least;             // parts of a block's steps at most; steps of a part at least
     float factor;                  // scale log2(e)
+    float* part;                   // (splits > 1) [block][key head][part][tile]: PromptShape::kPart floats
     uint32_t idesc_s, idesc_o;
     unsigned wait_limit;
     unsigned* status;
@@ -52,6 +54,7 @@ template <int DP> struct PromptShape {
     static constexpr int kQOff = 1024, kRingOff = kQOff + kTiles * kTileBytes, kOutOff = kRingOff + kStages * kStageBytes;
     static constexpr int kSmem = 1024 + kOutOff + 4 * kTiles * kMmStageOut;
     static constexpr int kOCol = 256;                             // tensor memory: S at 0, O from here
+    static constexpr int kPart = 128 * (DP + 2);                  // of a tile: [columns of four][row][4], then maxima and sums of the rows
     static_assert(kSmem <= 227 * 1024 && kOCol + kTiles * DP <= 512, "shared and tensor memory");
 };
 constexpr int kPromptRegsLaunch = 168, kPromptRegsIssue = 104, kPromptRegsSoftmax = 200;      // (two tiles) of a thread: at launch, and after the split
@@ -66,6 +69,8 @@ struct PromptBlock {
     int q_len, k_len;
     int q_at, k_at;                // rows of the sequence's first tokens
     int seq, bad;
+    int part, parts;               // of the block's steps
+    int number;                    // of the block, in all of them of this key head
 };
 // What a block has to do.  Query t is at place t + behind.
 template <int DP>
@@ -77,6 +82,10 @@ struct PromptWork : PromptBlock {
     __device__ __forceinline__ int sees_begin(const PromptParams& P, int t) const { return P.d.window > 0 ? max(0, t + behind + 1 - P.d.window) : 0; }
     __device__ __forceinline__ void read(const PromptParams& P, const volatile PromptBlock* b) {
         have = b->have; head = b->head; first = b->first; q_len = b->q_len; k_len = b->k_len; q_at = b->q_at; k_at = b->k_at; seq = b->seq; bad = b->bad;
+        part = b->part; number = b->number;
+        divide(P);
+    }
+    __device__ __forceinline__ void divide(const PromptParams& P) {
         behind = k_len - q_len;
         k_first = sees_begin(P, first) & ~(P.piece - 1);
         most = 0;
@@ -85,6 +94,21 @@ struct PromptWork : PromptBlock {
             const int t = first + i * P.tokens, last = min(t + P.tokens, q_len) - 1;
             steps[i] = have > 0 && t < q_len ? max(0, sees_end(P, last) - k_first + PromptShape<DP>::kKeys - 1) / PromptShape<DP>::kKeys : 0;
             most = max(most, steps[i]);
+        }
+        parts = 1;
+        if (P.splits > 1 && most > P.least) {      // this part's steps
+            const int size = max((most + P.splits - 1) / P.splits, P.least), from = part * size;
+            parts = (most + size - 1) / size;
+            if (part >= parts) have = 0;
+            most = have > 0 ? min(most - from, size) : 0;
+            k_first += from * PromptShape<DP>::kKeys;
+#pragma unroll
+            for (int i = 0; i < PromptShape<DP>::kTiles; ++i) steps[i] = min(max(steps[i] - from, 0), most);
+        } else if (part > 0) {
+            have = min(have, 0);
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < PromptShape<DP>::kTiles; ++i) steps[i] = 0;
         }
         tail_rows = k_len - k_first - (most - 1) * PromptShape<DP>::kKeys;
     }
@@ -265,9 +289,12 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                 PromptBlock next{};
                 next.have = -1;
                 if (more) {
+                    const int unit = index / d.k_heads;
                     next.have = 0;
-                    next.head = index % d.k_heads;
-                    prompt_block(P, index / d.k_heads, block_tokens, next);
+                    next.head = index - unit * d.k_heads;
+                    next.number = unit / P.splits;
+                    next.part = unit - next.number * P.splits;
+                    prompt_block(P, next.number, block_tokens, next);
                     // rows of no sequence
                     const int head = min(max(__ldcg(d.cu_seqlens), 0), (int)d.T), tail = min(max(__ldcg(d.cu_seqlens + d.seqs), head), (int)d.T);
                     const long long per = (long long)d.q_heads * d.D / 8, missing = ((long long)head + (d.T - tail)) * per;
@@ -280,7 +307,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                 if (lane == 0) {
                     volatile PromptBlock* to = info + (n & 1);
                     to->have = next.have; to->head = next.head; to->first = next.first; to->q_len = next.q_len; to->k_len = next.k_len;
-                    to->q_at = next.q_at; to->k_at = next.k_at; to->seq = next.seq; to->bad = next.bad;
+                    to->q_at = next.q_at; to->k_at = next.k_at; to->seq = next.seq; to->bad = next.bad; to->part = next.part; to->number = next.number;
                     mbar_arrive(bar_info(n & 1));
                 }
                 __syncwarp();
@@ -615,6 +642,24 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
           if (n > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(count - 1) & 1u, abort_flag, P.status, P.wait_limit);
           tc_fence_after();
           const bool bad = B.bad || bad_block[block & 3] == block + 1;
+          if (B.parts > 1) {
+            // This part's sums, unnormalised, a row to a thread; joined with the others' by the kernel behind.
+            float* const to = P.part + ((((long long)B.number * d.k_heads + B.head) * P.splits + B.part) * kTiles + i) * Sh::kPart + row * 4;
+#pragma unroll 1
+            for (int c = 0; c < d.D && n > 0 && ok; c += 32) {
+                uint32_t v[32];
+                mm_tmem_start(o_at + c, v);
+                mm_tmem_landed();
+                mm_tmem_use(v);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(to + (long long)(c + e) * 128) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
+            float* const numbers = to - row * 4 + 128 * DP + row;
+            numbers[0] = l > 0.f || bad || l != l ? m : -INFINITY;
+            numbers[128] = bad ? __int_as_float(0x7fffffff) : l;
+            tc_fence_before();
+            continue;
+          }
           const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
           uint16_t* const out = static_cast<uint16_t*>(d.out) + ((long long)(B.q_at + first) * d.q_heads + B.head * P.rows) * d.D;
           // 64 columns at a time through shared memory; the next block's first products run meanwhile.  (Places are computed here: kept from block to block they would
@@ -669,6 +714,70 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     }
 }
 
+// The parts of blocks that have several.  A CTA has a quarter of a tile's rows, 32, of one key head: four threads to a row, which take turns by four columns.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant__ PromptParams P) {
+    using Sh = PromptShape<DP>;
+    constexpr int kTiles = Sh::kTiles;
+    const nq_attention_desc& d = P.d;
+    const int number = blockIdx.x / d.k_heads, head = blockIdx.x - number * d.k_heads, i = blockIdx.y >> 2;
+    const int row = 32 * (blockIdx.y & 3) + (threadIdx.x & 31), quarter = threadIdx.x >> 5;
+    // (the lengths are older than the kernel before)
+    PromptWork<DP> B;
+    B.have = 0;
+    prompt_block(P, number, kTiles * P.tokens, B);
+    B.head = head;
+    B.part = 0;
+    B.number = number;
+    B.divide(P);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int token = row / P.rows, h = row - token * P.rows, t = B.first + i * P.tokens + token;
+    if (B.have <= 0 || B.parts <= 1 || token >= P.tokens || t >= B.q_len) return;
+    const float* at = P.part + ((((long long)number * d.k_heads + head) * P.splits) * kTiles + i) * Sh::kPart + row * 4;
+    const long long step = (long long)kTiles * Sh::kPart;
+    auto number_of = [&](int p, int k) { return __ldcg(at + p * step - row * 4 + 128 * DP + 128 * k + row); };
+    float top = -INFINITY;
+    for (int p = 0; p < B.parts; ++p) top = fmaxf(top, number_of(p, 0));
+    const float base = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    for (int p = 0; p < B.parts; ++p) l += number_of(p, 1) * exp2_approx(number_of(p, 0) - base);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* out = static_cast<uint16_t*>(d.out) + ((long long)(B.q_at + t) * d.q_heads + head * P.rows + h) * d.D;
+    for (int c = 8 * quarter; c < d.D; c += 32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+        for (int p = 0; p < B.parts; ++p) {
+            const float w = exp2_approx(number_of(p, 0) - base) * inv;
+            if (w == 0.f) continue;                // (a part that saw nothing has left no sums)
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(at + p * step + (long long)c * 128)), y = __ldcg(reinterpret_cast<const float4*>(at + p * step + (long long)(c + 4) * 128));
+            a.x += x.x * w; a.y += x.y * w; a.z += x.z * w; a.w += x.w * w;
+            b.x += y.x * w; b.y += y.y * w; b.z += y.z * w; b.w += y.w * w;
+        }
+        *reinterpret_cast<uint4*>(out + c) = make_uint4(head_pack<BF16>(a.x, a.y), head_pack<BF16>(a.z, a.w), head_pack<BF16>(b.x, b.y), head_pack<BF16>(b.z, b.w));
+    }
+}
+
+// Parts of a block's steps.  Blocks are dealt out as CTAs become free, so that there should be at least two for every SM; a part has eight steps at least (of a prompt
+// over itself, whose blocks see half of it: counted twice), for its sums pass through memory.
+template <int DP>
+static int prompt_splits(const nq_attention_desc& d, int tokens) {
+    using Sh = PromptShape<DP>;
+    const int64_t block = (int64_t)Sh::kTiles * tokens, blocks = ((d.T + block - 1) / block + d.seqs) * d.k_heads;
+    const int64_t keys = d.block_table ? (int64_t)d.max_pages * d.page_size : d.Tk, steps = keys / Sh::kKeys, wanted = 2 * (int64_t)sm_count();
+    int64_t n = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
+    const int64_t most = steps / (d.block_table || d.cu_seqlens_k ? 8 : 16);
+    n = n < most ? n : most;
+    return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+template <int DP>
+static size_t prompt_scratch(const nq_attention_desc& d) {
+    using Sh = PromptShape<DP>;
+    const int tokens = 128 / (d.q_heads / d.k_heads), splits = prompt_splits<DP>(d, tokens);
+    const int64_t block = (int64_t)Sh::kTiles * tokens, blocks = ((d.T + block - 1) / block + d.seqs) * d.k_heads;
+    return splits == 1 ? 0 : (size_t)(blocks * splits * Sh::kTiles) * Sh::kPart * sizeof(float);
+}
+static size_t prompt_scratch_of(const nq_attention_desc& d) { return d.D <= 64 ? prompt_scratch<64>(d) : d.D <= 128 ? prompt_scratch<128>(d) : prompt_scratch<256>(d); }
+
 template <int DP, bool BF16>
 static int prompt_launch(PromptParams& P, cudaStream_t stream) {
     using Sh = PromptShape<DP>;
@@ -698,7 +807,9 @@ static int prompt_launch(PromptParams& P, cudaStream_t stream) {
     if (st != NQ_OK) return st;
     st = mm_encode_heads(&P.map_v, d.v, type, {d.D, rows, d.k_heads, pages}, {d.v_slot, d.v_head, d.v_page}, {64, P.piece, 1, 1});
     if (st != NQ_OK) return st;
-    const int64_t block = (int64_t)Sh::kTiles * P.tokens, ctas = ((d.T + block - 1) / block + d.seqs) * d.k_heads;
+    P.splits = prompt_splits<DP>(d, P.tokens);
+    P.least = 4;
+    const int64_t block = (int64_t)Sh::kTiles * P.tokens, blocks = ((d.T + block - 1) / block + d.seqs) * d.k_heads, ctas = blocks * P.splits;
     if (ctas > 0x7fffffff) return NQ_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
@@ -707,38 +818,62 @@ static int prompt_launch(PromptParams& P, cudaStream_t stream) {
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     void* args[] = {&P};
-    return launch_dependent(cfg, attr, 0, fn, args);
+    st = launch_dependent(cfg, attr, 0, fn, args);
+    if (st != NQ_OK || P.splits == 1) return st;
+    cfg.gridDim = dim3((unsigned)blocks, 4 * Sh::kTiles);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    return launch_dependent(cfg, attr, 0, (const void*)prompt_join_kernel<DP, BF16>, args);
 }
 
-}  // namespace nq
-
-extern "C" int nq_prompt_attention_fwd(const nq_attention_desc* desc, void* status_word, nq_stream_t stream) {
-    using namespace nq;
-    if (!desc || !status_word) return NQ_ERR_NULL;
-    const nq_attention_desc& d = *desc;
+// What does not need a pointer that is followed.
+static int prompt_check(const nq_attention_desc& d) {
     int st = attention_check(d);
     if (st != NQ_OK) return st;
     if (!d.cu_seqlens) return NQ_ERR_NULL;
     if (d.T <= 0 || d.q_heads / d.k_heads > 128) return NQ_ERR_SHAPE;
     if (d.T > 0x3fffffff || d.Tk > 0x3fffffff) return NQ_ERR_TOO_LARGE;
-    if (!aligned_to(4, (const char*)d.cu_seqlens, (const char*)d.cu_seqlens_k) || !aligned16(status_word)) return NQ_ERR_ALIGN;
+    if (!aligned_to(4, (const char*)d.cu_seqlens, (const char*)d.cu_seqlens_k)) return NQ_ERR_ALIGN;
+    if (!d.block_table) return d.Tk <= 0 ? NQ_ERR_SHAPE : NQ_OK;
+    st = attention_cache_check(d);
+    if (st != NQ_OK) return st;
+    return (int64_t)d.max_pages * d.page_size > 0x3fffffff ? NQ_ERR_TOO_LARGE : NQ_OK;
+}
+
+}  // namespace nq
+
+extern "C" {
+
+size_t nq_prompt_attention_scratch_bytes(const nq_attention_desc* desc) {
+    return desc && nq::prompt_check(*desc) == NQ_OK ? nq::prompt_scratch_of(*desc) : 0;
+}
+
+int nq_prompt_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t scratch_bytes, void* status_word, nq_stream_t stream) {
+    using namespace nq;
+    if (!desc || !status_word) return NQ_ERR_NULL;
+    const nq_attention_desc& d = *desc;
+    const int st = prompt_check(d);
+    if (st != NQ_OK) return st;
+    if (!aligned16(status_word)) return NQ_ERR_ALIGN;
+    const size_t need = prompt_scratch_of(d);
+    if (need) {
+        if (!scratch) return NQ_ERR_NULL;
+        if (!aligned16(scratch)) return NQ_ERR_ALIGN;
+        if (scratch_bytes < need) return NQ_ERR_SCRATCH;
+    }
     PromptParams P{};
+    P.part = static_cast<float*>(scratch);
     P.d = d;
     P.rows = d.q_heads / d.k_heads;
     P.paged = d.block_table != nullptr;
     P.factor = d.scale * 1.44269504088896340736f;
     P.wait_limit = gemm_wait_limit();
     P.status = static_cast<unsigned*>(status_word) + 2;
-    if (P.paged) {
-        st = attention_cache_check(d);
-        if (st != NQ_OK) return st;
-        if ((int64_t)d.max_pages * d.page_size > 0x3fffffff) return NQ_ERR_TOO_LARGE;
-        P.shift = log2_of(d.page_size);
-    } else if (d.Tk <= 0) {
-        return NQ_ERR_SHAPE;
-    }
+    if (P.paged) P.shift = log2_of(d.page_size);
     const bool bf = d.dtype == NQ_BF16;
     if (d.D <= 64) return bf ? prompt_launch<64, true>(P, as_stream(stream)) : prompt_launch<64, false>(P, as_stream(stream));
     if (d.D <= 128) return bf ? prompt_launch<128, true>(P, as_stream(stream)) : prompt_launch<128, false>(P, as_stream(stream));
     return bf ? prompt_launch<256, true>(P, as_stream(stream)) : prompt_launch<256, false>(P, as_stream(stream));
 }
+
+}  // extern "C"

@@ -80,9 +80,16 @@ def test_paged_attention_refusals():
 
 def test_prompt_attention_refusals():
     L = _lib.lib()
-    call = lambda d, status=P: L.nq_prompt_attention_fwd(ctypes.byref(_lib.AttentionDesc(**d)), status, None)
-    assert L.nq_prompt_attention_fwd(None, P, None) == _lib.NQ_ERR_NULL
+    call = lambda d, status=P, scratch=None, n=0: L.nq_prompt_attention_fwd(ctypes.byref(_lib.AttentionDesc(**d)), scratch, n, status, None)
+    assert L.nq_prompt_attention_fwd(None, None, 0, P, None) == _lib.NQ_ERR_NULL
     more = [("cu_seqlens", None, "NULL"), ("cu_seqlens", P + 2, "ALIGN"), ("T", 0, "SHAPE"), (("q_heads", "k_heads"), (129, 1), "SHAPE"), ("T", 1 << 30, "TOO_LARGE")]
     refused(call, PACKED, COMMON + more + [("Tk", 0, "SHAPE"), ("cu_seqlens_k", P + 2, "ALIGN"), ("Tk", 1 << 30, "TOO_LARGE")])
     refused(call, PAGED, COMMON + more + CACHE + [(("max_pages", "page_size"), (1 << 20, 1 << 10), "TOO_LARGE")])
     assert call(PACKED, None) == _lib.NQ_ERR_NULL and call(PACKED, P + 4) == _lib.NQ_ERR_ALIGN
+    size = lambda **kw: L.nq_prompt_attention_scratch_bytes(ctypes.byref(_lib.AttentionDesc(**{**PAGED, **kw})))
+    need = size(max_pages=1024)                                   # few tokens behind a long cache: parts of it by several CTAs
+    assert need > 0 and need % 16 == 0 and size() == 0 and size(D=60) == 0 and L.nq_prompt_attention_scratch_bytes(None) == 0
+    long = dict(PAGED, max_pages=1024)
+    assert call(long) == _lib.NQ_ERR_NULL and call(long, P, P + 4, need) == _lib.NQ_ERR_ALIGN and call(long, P, P, need - 1) == _lib.NQ_ERR_SCRATCH
+    for kw in (dict(T=100000), dict(T=100), dict(T=1, seqs=1000), dict(q_heads=64, k_heads=64, D=256), dict(q_heads=128, k_heads=1)):
+        assert size(max_pages=1 << 16, **kw) < 1 << 28, kw         # whatever the sizes

@@ -128,6 +128,33 @@ def test_paged(new, total, H, K, D, page, window, dtype):
     check_attention(ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, window=window), want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,total,H,K,D,page,window", [
+    ([1], [3001], 8, 2, 128, 16, None), ([16, 2, 0], [5000, 100, 2000], 4, 2, 64, 32, None), ([70, 200, 3], [4000, 900, 33], 8, 1, 128, 64, None), ([5, 9], [2500, 2600], 4, 2, 256, 16, None),
+    ([100], [9000], 6, 2, 80, 128, 2500), ([130], [2048], 14, 2, 96, 8, None)])
+def test_few_tokens_behind_a_long_cache(new, total, H, K, D, page, window, dtype):
+    """The keys of a block go to several CTAs, whose sums a second launch joins: parts that a tile or a row sees nothing of among them."""
+    import ctypes
+
+    from nanoquant_b200 import _lib, ops
+
+    q, k, v, kc, vc, table, n = piece(new, total, H, K, D, page, dtype)
+    d = _lib.AttentionDesc(q=1 << 16, k=1 << 16, v=1 << 16, out=1 << 16, cu_seqlens=1 << 16, lengths=1 << 16, block_table=1 << 16, k_slot=8, v_slot=8, table_stride=1, pages=kc.size(0),
+                           max_pages=table.size(1), page_size=page, T=len(q), seqs=len(new), q_heads=H, k_heads=K, D=D, causal=1, scale=1.0)
+    assert _lib.lib().nq_prompt_attention_scratch_bytes(ctypes.byref(d)) > 0
+    want = expected(q, k, v, new, window)
+    got = ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, window=window)
+    check_attention(got, want)
+    assert torch.equal(got, ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, window=window))
+    packed = ops.prompt_attention(q, torch.cat(k), torch.cat(v), starts(new), starts(total), window=window)
+    check_attention(packed, want)
+    if total[0] < 5000:                                           # a page outside the cache: NaN, wherever the part is that has it
+        table[0, total[0] // page // 2] = -1
+        bad = ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, window=window)
+        assert torch.isnan(bad[:new[0]]).all()
+        check_attention(bad[new[0]:], [t[new[0]:] for t in want])
+
+
 @pytest.mark.parametrize("D", [64, 256])
 def test_sequences_that_are_not_there_are_nan(D):
     from nanoquant_b200 import ops
