@@ -1050,7 +1050,7 @@ bool maybe(PyObject* o, const Tensor*& t) {
 PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 9, "qk_norm_rope takes 9 arguments");
-    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    if (!exact_plain(a[0]) || !THPVariable_CheckExact(a[1])) Py_RETURN_NONE;
     HeadsArgs h{};
     h.q = plain(a[0]); h.k = plain(a[1]); h.positions = plain(a[2]); h.inv_freq = plain(a[3]);
     if (!h.q || !h.k || !h.positions || !h.inv_freq || !maybe(a[4], h.wq) || !maybe(a[5], h.wk) || wants_gradient({h.q, h.k, h.inv_freq, h.wq, h.wk}) || !heads_takes(h)) Py_RETURN_NONE;
@@ -1070,7 +1070,7 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 14, "append_kv takes 14 arguments");
-    if (!exact_plain(a[1])) Py_RETURN_NONE;
+    if (!exact_plain(a[1]) || !THPVariable_CheckExact(a[2]) || !(a[0] == Py_None || THPVariable_CheckExact(a[0]))) Py_RETURN_NONE;
     HeadsArgs h{};
     h.k = plain(a[1]); h.v = plain(a[2]); h.k_cache = plain(a[3]); h.v_cache = plain(a[4]); h.table = plain(a[5]); h.positions = plain(a[6]);
     if (!maybe(a[0], h.q) || !h.k || !h.v || !h.k_cache || !h.v_cache || !h.table || !h.positions || !maybe(a[7], h.sequences) || !maybe(a[8], h.inv_freq) || !maybe(a[9], h.wq) ||
@@ -1163,7 +1163,7 @@ Tensor attention_launch(const AttentionArgs& a) {
 PyObject* py_prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 10, "prompt_attention takes 10 arguments");
-    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    if (!exact_plain(a[0]) || !THPVariable_CheckExact(a[1]) || !THPVariable_CheckExact(a[2])) Py_RETURN_NONE;
     AttentionArgs t{};
     t.q = plain(a[0]); t.k = plain(a[1]); t.v = plain(a[2]); t.cu = plain(a[3]);
     if (!t.q || !t.k || !t.v || !t.cu || !maybe(a[4], t.cu_k) || !maybe(a[5], t.table) || !maybe(a[6], t.lengths) || !t.table != !t.lengths || (t.table && t.cu_k) ||
@@ -1181,7 +1181,7 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 7, "paged_attention takes 7 arguments");
-    if (!exact_plain(a[0])) Py_RETURN_NONE;
+    if (!exact_plain(a[0]) || !THPVariable_CheckExact(a[1]) || !THPVariable_CheckExact(a[2])) Py_RETURN_NONE;
     AttentionArgs t{};
     t.q = plain(a[0]); t.k = plain(a[1]); t.v = plain(a[2]); t.table = plain(a[3]); t.lengths = plain(a[4]);
     t.causal = true;
