@@ -596,11 +596,18 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                 float peak = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
-                    if (masked) {
+                    if (masked) {                  // (most 32s of a step are seen by all of a warp's rows, or end for them without a beginning)
                         const int lo = begin - key - 32 * c, hi = end - key - 32 * c;
+                        if (__any_sync(0xffffffffu, hi < 32)) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (e < lo || e >= hi) r[c][e] = 0xff800000u;
+                            for (int e = 0; e < 32; ++e)
+                                if (e >= hi) r[c][e] = 0xff800000u;
+                        }
+                        if (__any_sync(0xffffffffu, lo > 0)) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (e < lo) r[c][e] = 0xff800000u;
+                        }
                     }
                     peak = max_or_nan(peak, peaks(c));
                 }
