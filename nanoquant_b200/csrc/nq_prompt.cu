@@ -669,39 +669,47 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
           }
           const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
           uint16_t* const out = static_cast<uint16_t*>(d.out) + ((long long)(B.q_at + first) * d.q_heads + B.head * P.rows) * d.D;
-          // 64 columns at a time through shared memory; the next block's first products run meanwhile.  (Places are computed here: kept from block to block they would
-          // take the registers that a step needs.)
+          // 64 columns at a time through shared memory, so that eight lanes store a row's 128 bytes (every thread its own row kept the load and store unit busy for 4000 clk);
+          // the next block's first products run meanwhile.  (Places are computed here: kept from block to block they would take the registers that a step needs.)
           int ln = lane;
           asm volatile("" : "+r"(ln));
-          const uint32_t mine = out_stage + ln * 128, u = ln & 7, r0 = ln >> 3;
-#pragma unroll 1
-          for (int c = 0; c < d.D && ok; c += 64) {
+          const uint32_t mine = out_stage + ln * 128, u = ln & 7, r0 = ln >> 3, theirs = out_stage + r0 * 128;
+          int place[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int full = 32 * (warp & 3) + 4 * k + r0, tok = (full * magic) >> 16;
+            place[k] = tok < P.tokens && tok < left ? (tok * d.q_heads + full - tok * P.rows) * d.D + 8 * (int)u : -1;
+          }
+#pragma unroll
+          for (int c = 0; c < DP; c += 64) {
+            if (c >= d.D || !ok) break;
+            uint32_t v[2][32] = {};
+            if (n > 0) {
+                mm_tmem_start(o_at + c, v[0]);
+                mm_tmem_start(o_at + c + 32, v[1]);
+                mm_tmem_landed();
+                mm_tmem_use(v[0]);
+                mm_tmem_use(v[1]);
+            }
             __syncwarp();                          // (the stores before have read theirs)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t v[32] = {};
-                if (n > 0) {
-                    mm_tmem_start(o_at + c + 32 * half, v);
-                    mm_tmem_landed();
-                    mm_tmem_use(v);
-                }
+            for (int q = 0; q < 8; ++q) {
+                uint32_t w[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = head_pack<BF16>(__uint_as_float(v[8 * q + 2 * e]) * inv, __uint_as_float(v[8 * q + 2 * e + 1]) * inv);
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(mine + (((4 * half + q) ^ u) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                }
+                for (int e = 0; e < 4; ++e)
+                    w[e] = head_pack<BF16>(__uint_as_float(v[q >> 2][8 * (q & 3) + 2 * e]) * inv, __uint_as_float(v[q >> 2][8 * (q & 3) + 2 * e + 1]) * inv);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(mine + ((q ^ u) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
             }
             __syncwarp();
             const bool column = c + 8 * (int)u < d.D;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const int rr = 4 * k + r0, full = 32 * (warp & 3) + rr, tok = (full * magic) >> 16, h = full - tok * P.rows;
-                if (tok < P.tokens && tok < left && column) {
+                if (place[k] >= 0 && column) {
                     uint4 x;
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(out_stage + rr * 128 + ((u ^ (rr & 7)) << 4)) : "memory");
-                    *reinterpret_cast<uint4*>(out + ((long long)tok * d.q_heads + h) * d.D + c + 8 * u) = x;
+                    // (row 4 k + r0, unit u)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(theirs + k * 512 + ((u ^ ((4 * k + r0) & 7)) << 4)) : "memory");
+                    *reinterpret_cast<uint4*>(out + place[k] + c) = x;
                 }
             }
           }
