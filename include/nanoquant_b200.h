@@ -460,8 +460,8 @@ int nq_heads_fwd(const nq_heads_desc* desc_host, nq_stream_t stream);
  * nq_prompt_attention_fwd: packed prompts, q [T, q_heads, D]; sequence s has the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32, not decreasing, seqs + 1
  * of them).  Rows of no sequence are zeros.  Keys and values are packed likewise (k, v [Tk, k_heads, D] by cu_seqlens_k, NULL: cu_seqlens), or those in
  * the cache, `lengths[s]` per sequence (block_table not NULL; k and v are then the cache).  The last row of a sequence is at the place of its last
- * key: rows before the first key see nothing.  `status_word` as in nq_onebit_gemm_fwd.
- * scratch: ..._scratch_bytes() (0 where none is needed, or for a refused description), any contents, 16-byte aligned.  The order of sums depends on the sizes and
+ * key: rows before the first key see nothing.
+ * `status_word` as in nq_onebit_gemm_fwd.  scratch: ..._scratch_bytes() (0 where none is needed, or for a refused description), any contents, 16-byte aligned.  The order of sums depends on the sizes and
  * the lengths alone.  Strides, alignment, pages and block_table as in nq_heads_desc; out dense.
  * replaces: the attention of the HF model forward between the quantised projections (src/nanoquant/kernel/test_decode.py:385-422). */
 typedef struct {
@@ -477,7 +477,7 @@ typedef struct {
     float scale;
 } nq_attention_desc;
 size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int D, int64_t max_tokens);
-int nq_paged_attention_fwd(const nq_attention_desc* desc_host, void* scratch, size_t scratch_bytes, nq_stream_t stream);
+int nq_paged_attention_fwd(const nq_attention_desc* desc_host, void* scratch, size_t scratch_bytes, void* status_word, nq_stream_t stream);
 size_t nq_prompt_attention_scratch_bytes(const nq_attention_desc* desc_host);
 int nq_prompt_attention_fwd(const nq_attention_desc* desc_host, void* scratch, size_t scratch_bytes, void* status_word, nq_stream_t stream);
 

@@ -106,7 +106,7 @@ SIGNATURES = {
     "nq_head_max_columns": (c_int, []),
     "nq_heads_fwd": (c_int, [ctypes.POINTER(HeadsDesc), c_void_p]),
     "nq_paged_attention_scratch_bytes": (c_size_t, [c_int] * 4 + [c_int64]),
-    "nq_paged_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_size_t, c_void_p]),
+    "nq_paged_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_size_t, c_void_p, c_void_p]),
     "nq_prompt_attention_scratch_bytes": (c_size_t, [ctypes.POINTER(AttentionDesc)]),
     "nq_prompt_attention_fwd": (c_int, [ctypes.POINTER(AttentionDesc), c_void_p, c_size_t, c_void_p, c_void_p]),
     "nq_gemv_max_tokens": (c_int, []),

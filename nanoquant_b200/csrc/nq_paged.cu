@@ -1,20 +1,23 @@
 // Attention of one new token per sequence over a paged cache.
 //
-//     o[h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale log2(e) q[h] . k_j - m),   m the largest of these exponents so far
+//     o[h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale log2(e) q[h] . k_j - m),   m the largest of these exponents so far, less 8 at most
 //
 // Bound by memory: keys and values are read once, for all the query heads that share them: 4 D bytes for 4 D G operations.  Those G heads are the rows of
 // mma.sync.m16n8k16 (up to 16; the instruction's rate is far above what memory delivers, and few rows would leave tcgen05's 128 idle).
 //
 // Work.  The tokens that a sequence's query sees are cut into steps of 16.  An item is a sequence, a key head and up to 16 of its query heads; the steps of all
 // items lie one behind the other, and every warp takes the same number of them, found from the lengths on the device: batches of any lengths fill the
-// SMs evenly, and a captured graph follows the lengths.  A warp has a ring of steps of its own in shared memory (cp.async, which runs on into the next item),
-// its own running maximum, sum and accumulators: nothing in the loop waits for another warp.  An item that lies in several warps leaves fp32 results
+// SMs evenly, and a captured graph follows the lengths.  A warp has a ring of steps of its own in shared memory (TMA boxes of 16 tokens x 64
+// columns; it runs on into the next item), its own running maximum, sum and accumulators: nothing in the loop waits for another warp.  (Copied by cp.async, 16 bytes a lane,
+// a step was 650 instructions, 1.3 us of a warp alone, and 6.0 TB/s; by bulk copies of 256-byte rows 4.4 TB/s.)  An item that lies in several warps leaves fp32 results
 // (m, sum, unnormalised o) in the scratch, which a second, overlapped launch joins in their order.  Caches without room for long sequences take a CTA per item, its
 // steps divided among the four warps and their results joined through shared memory: one launch.
 //
 // The weights p are rounded to the operands' type for the product with the values: 2^-9 (bf16) or 2^-12 (fp16) of each, which the average over
 // tokens does not enlarge.  Sums of p are fp32 sums of the rounded values.
 #include "nq_attn.cuh"
+#include "nq_stage.h"
+#include "nq_tcgen05.cuh"
 
 namespace nq {
 
@@ -23,13 +26,16 @@ constexpr int kPagedStep = 16;                  // tokens
 constexpr int kPagedRows = 16;                  // query heads of an item at most
 constexpr int kPagedWhole = 256;                // caches of up to so many tokens a sequence: a CTA per item
 
-struct PagedParams {
+struct alignas(64) PagedParams {
+    CUtensorMap map_k, map_v;
     nq_attention_desc d;
     int shift;                                  // log2(page_size)
     int rows, chunks;                           // query heads to a key head; items of 16 of them
     int warps;                                  // of the split kernel
     int items;                                  // (of all sequences)
     float factor;                               // scale log2(e)
+    unsigned wait_limit;
+    unsigned* status;
     float* part;                                // [warps][2][16][DP + 2]
 };
 
@@ -139,27 +145,42 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// 16 bytes to shared memory, or zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
-    const int n = live ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void paged_box(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
 }
-
 template <int DP> struct PagedShape {
-    static constexpr int kChunks = DP / 8;                        // 16-byte chunks of a row
-    static constexpr int kRowBytes = 2 * DP;
-    static constexpr int kTileBytes = kPagedStep * kRowBytes;     // of keys, or of values
+    static constexpr int kColumns = DP / 64;                      // boxes of 64 columns: rows of 128 bytes, 128-byte swizzle
+    static constexpr int kBoxBytes = kPagedStep * 128;
+    static constexpr int kTileBytes = kColumns * kBoxBytes;       // of keys, or of values
     static constexpr int kStages = DP == 64 ? 4 : 3;
     static constexpr int kWarpBytes = 2 * kStages * kTileBytes;
-    static constexpr int kSmem = kPagedWarps * kWarpBytes;
+    static constexpr int kBarOff = kPagedWarps * kWarpBytes;
+    static constexpr int kSmem = 1024 + kBarOff + 8 * kPagedWarps * kStages;
     static constexpr int kRow = DP + 2;                           // floats of a head's result: o, m, sum
     static constexpr int kPart = kPagedRows * kRow;
     static constexpr int kCtasPerSm = DP == 64 ? 3 : DP == 128 ? 2 : 1;
-    static_assert(kPagedWarps * kPart * 4 <= kSmem, "the warps' results fit the rings");
+    static_assert(kPagedWarps * kPart * 4 <= kBarOff, "the warps' results fit the rings");
+    static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory");
 };
-// Chunk c of row r: eight rows' same chunk lie in different banks.
+// A barrier for every stage of a CTA's warps.
 template <int DP>
-__device__ __forceinline__ uint32_t paged_at(uint32_t base, int r, int c) { return base + r * PagedShape<DP>::kRowBytes + ((c ^ (r & 7)) << 4); }
+__device__ __forceinline__ void paged_rings(uint32_t smem) {
+    using S = PagedShape<DP>;
+    if (threadIdx.x < kPagedWarps * S::kStages) mbar_init(smem + S::kBarOff + 8 * threadIdx.x, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+}
+// Waits for a stage by a whole warp; false after `limit` more attempts of some 4 us, which sets the status word.
+__device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, unsigned* status, unsigned limit) {
+    for (unsigned i = 0; i <= limit; ++i)
+        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+    if ((threadIdx.x & 31) == 0) atomicExch(status, (unsigned)(-NQ_ERR_TIMEOUT));
+    // (the copies in flight get a bounded time to land before shared memory is released)
+    for (unsigned i = 0; i < (1u << 20); ++i) __nanosleep(64);
+    return false;
+}
 
 // The pages of 32 steps of an item, held by the lanes of a warp: the one of lane i's step, and (pages of 8 tokens) of its second half.
 struct PagedPages {
@@ -183,32 +204,55 @@ struct PagedPages {
         return !__any_sync(0xffffffffu, bad);
     }
 };
-// Keys and values of step s into a stage.
+// Keys and values of step s into a stage: a box for each page (one, or two pages of 8) and 64 columns.
 template <int DP>
-__device__ __forceinline__ void paged_load(const nq_attention_desc& d, const PagedRange& R, const PagedPages& pages, int kh, int s, uint32_t kt) {
+__device__ __forceinline__ void paged_load(const PagedParams& P, const PagedRange& R, const PagedPages& pages, int kh, int s, uint32_t kt, uint32_t bar) {
     using S = PagedShape<DP>;
-    const int lane = threadIdx.x & 31, src = s - pages.from;
+    const nq_attention_desc& d = P.d;
+    const int src = s - pages.from;
     const int pa = __shfl_sync(0xffffffffu, pages.page0, src), pb = __shfl_sync(0xffffffffu, pages.page1, src);
-    constexpr int kRowsAtOnce = 32 / S::kChunks;
-    const int c = lane % S::kChunks, r0 = lane / S::kChunks;
-    const int token0 = (R.first + s) * kPagedStep, slot0 = token0 & (d.page_size - 1);
-    const uint16_t* kbase = static_cast<const uint16_t*>(d.k) + (long long)kh * d.k_head + 8 * c;
-    const uint16_t* vbase = static_cast<const uint16_t*>(d.v) + (long long)kh * d.v_head + 8 * c;
-    const bool column = 8 * c < d.D;
+    if (elect_one()) {
+        const int token = (R.first + s) * kPagedStep, slot = token & (d.page_size - 1);
+        if (d.page_size >= kPagedStep) {
+            mbar_expect_tx(bar, 2 * S::kTileBytes);
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        const uint16_t* base = kv ? vbase : kbase;
-        const long long page_step = kv ? d.v_page : d.k_page, slot_step = kv ? d.v_slot : d.k_slot;
-        const uint16_t* at0 = base + pa * page_step + slot0 * slot_step;
-        const uint16_t* at1 = base + pb * page_step + (d.page_size < kPagedStep ? 0 : slot0 + 8) * slot_step;
+            for (int c = 0; c < S::kColumns; ++c) {
+                paged_box(kt + c * S::kBoxBytes, &P.map_k, 64 * c, slot, kh, pa, bar);
+                paged_box(kt + S::kTileBytes + c * S::kBoxBytes, &P.map_v, 64 * c, slot, kh, pa, bar);
+            }
+        } else {
+            // (a page that holds nothing that is seen is not looked at)
+            const bool second = token + 8 < R.end, first = token + 8 > R.begin;
+            mbar_expect_tx(bar, (uint32_t)((int)first + (int)second) * S::kTileBytes);
 #pragma unroll
-        for (int i = 0; i < kPagedStep; i += kRowsAtOnce) {
-            const int r = r0 + i, token = token0 + r;
-            const bool live = token >= R.begin && token < R.end && column;
-            const uint16_t* at = (r < 8 ? at0 : at1) + (r & 7) * slot_step;
-            copy16(paged_at<DP>(kt + kv * S::kTileBytes, r, c), live ? at : base, live);
+            for (int c = 0; c < S::kColumns; ++c) {
+                if (first) {
+                    paged_box(kt + c * S::kBoxBytes, &P.map_k, 64 * c, 0, kh, pa, bar);
+                    paged_box(kt + S::kTileBytes + c * S::kBoxBytes, &P.map_v, 64 * c, 0, kh, pa, bar);
+                }
+                if (second) {
+                    paged_box(kt + c * S::kBoxBytes + 1024, &P.map_k, 64 * c, 0, kh, pb, bar);
+                    paged_box(kt + S::kTileBytes + c * S::kBoxBytes + 1024, &P.map_v, 64 * c, 0, kh, pb, bar);
+                }
+            }
         }
     }
+    __syncwarp();
+}
+// Values of a landed step's tokens that are not seen: zeros, for their weights are, which a NaN would survive.
+template <int DP>
+__device__ __forceinline__ void paged_clear(const PagedRange& R, int s, uint32_t kt) {
+    using S = PagedShape<DP>;
+    const int lane = threadIdx.x & 31, token0 = (R.first + s) * kPagedStep;
+    if (token0 >= R.begin && token0 + kPagedStep <= R.end) return;
+    const int token = token0 + (lane & 15);
+    if (token < R.begin || token >= R.end) {
+        const uint32_t at = kt + S::kTileBytes + (lane & 15) * 128 + (lane >> 4) * 64;
+        for (int c = 0; c < S::kColumns; ++c)
+            for (int u = 0; u < 4; ++u) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + c * S::kBoxBytes + 16 * u), "r"(0) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // (before a later copy to the same place)
+    __syncwarp();
 }
 // Up to 16 heads' queries, accumulators, maxima and sums, as MMA fragments: lane (g, q) has the heads g and g + 8.
 template <int DP, bool BF16>
@@ -237,13 +281,15 @@ struct PagedHeads {
     __device__ __forceinline__ void step(const PagedRange& R, int s, float factor, uint32_t kt) {
         using S = PagedShape<DP>;
         const int lane = threadIdx.x & 31, q = lane & 3;
-        const uint32_t vt = kt + S::kTileBytes;
+        // 16 bytes number u of row r are at u ^ (r & 7)
+        const uint32_t k_at = kt + ((lane & 7) + ((lane >> 4) << 3)) * 128, k_unit = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
+        const uint32_t v_at = kt + S::kTileBytes + ((lane & 7) + (((lane >> 3) & 1) << 3)) * 128, v_unit = ((lane >> 4) ^ (lane & 7)) << 4;
         float c[2][4] = {};
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
             uint32_t b[4];
             // matrices: keys 0-7 and 8-15 (lanes 8-15 / 24-31: the second 8 columns)
-            ldmatrix4(b, paged_at<DP>(kt, (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+            ldmatrix4(b, k_at + (k >> 2) * S::kBoxBytes + (k_unit ^ (32 * (k & 3))));
             paged_mma<BF16>(c[0], a[k], b[0], b[1]);
             paged_mma<BF16>(c[1], a[k], b[2], b[3]);
         }
@@ -256,35 +302,45 @@ struct PagedHeads {
                 if (token < R.begin || token >= R.end) c[i >> 2][i & 3] = -INFINITY;
             }
         }
+        float top[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(fmaxf(c[0][2 * r], c[0][2 * r + 1]), fmaxf(c[1][2 * r], c[1][2 * r + 1]));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * factor;
+        }
+        // The maximum is moved, and o multiplied, only when it grows by more than 2^8: weights and sums have room for that.
+        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if (!(top[r] > m[r] + 8.f)) continue;
+                const float shrink = exp2_approx(m[r] - top[r]);      // (0 at first)
+                m[r] = top[r];
+                l[r] *= shrink;
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n) {
+                    o[n][2 * r] *= shrink;
+                    o[n][2 * r + 1] *= shrink;
+                }
+            }
+        }
         uint32_t p[4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            float top = fmaxf(fmaxf(c[0][2 * r], c[0][2 * r + 1]), fmaxf(c[1][2 * r], c[1][2 * r + 1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float to_m = fmaxf(m[r], top * factor), base = to_m == -INFINITY ? 0.f : to_m;
-            const float shrink = exp2_approx(m[r] - base);          // (0 at first, exactly 1 where m stays)
-            m[r] = to_m;
+            const float base = m[r] == -INFINITY ? 0.f : m[r];
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = exp2_approx(fmaf(c[i >> 1][2 * r + (i & 1)], factor, -base));
             p[r] = head_pack<BF16>(e[0], e[1]);
             p[2 + r] = head_pack<BF16>(e[2], e[3]);
-            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum += head_float<BF16>(i < 2 ? p[r] : p[2 + r], i & 1);
-            l[r] = l[r] * shrink + sum;
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-                o[n][2 * r] *= shrink;
-                o[n][2 * r + 1] *= shrink;
-            }
+            for (int i = 0; i < 4; ++i) l[r] += head_float<BF16>(i < 2 ? p[r] : p[2 + r], i & 1);
         }
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
             uint32_t b[4];
             // matrices (transposed): tokens 0-7 and 8-15 of columns 16 n .., then of 16 n + 8 ..
-            ldmatrix4_trans(b, paged_at<DP>(vt, (lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
+            ldmatrix4_trans(b, v_at + (n >> 2) * S::kBoxBytes + (v_unit ^ (32 * (n & 3))));
             paged_mma<BF16>(o[2 * n], p, b[0], b[1]);
             paged_mma<BF16>(o[2 * n + 1], p, b[2], b[3]);
         }
@@ -331,11 +387,12 @@ struct PagedHeads {
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) paged_split_kernel(const __grid_constant__ PagedParams P) {
     using S = PagedShape<DP>;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ unsigned char smem_raw[];
     __shared__ PagedPlan plan;
     const nq_attention_desc& d = P.d;
     const int warp = threadIdx.x >> 5;
-    const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem + warp * S::kWarpBytes, bars = smem + S::kBarOff + 8 * warp * S::kStages;
+    paged_rings<DP>(smem);
     const int per_seq = d.k_heads * P.chunks, W = blockIdx.x * kPagedWarps + warp;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -369,7 +426,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
         }
         return true;
     };
-    PagedPages pages;
+    PagedPages pages{};
     bool fresh = true;
     unsigned bad_items = 0, load_items = 0;     // (bit i: the i-th item from here on, modulo 32, has a page outside the cache; a ring holds far fewer)
     auto load_next = [&](int i, int stage) {    // step i of this warp's
@@ -378,7 +435,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
             if (!ok) bad_items |= 1u << (load_items & 31);
             fresh = false;
         }
-        paged_load<DP>(d, load.R, pages, load.item / P.chunks, load.s, ring + stage * 2 * S::kTileBytes);
+        paged_load<DP>(P, load.R, pages, load.item / P.chunks, load.s, ring + stage * 2 * S::kTileBytes, bars + 8 * stage);
         if (advance(load)) {
             fresh = true;
             ++load_items;
@@ -386,12 +443,11 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
         }
     };
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
+    for (int i = 0; i < S::kStages - 1; ++i)
         if (i < count) load_next(i, i);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
     PagedHeads<DP, BF16> heads;
     unsigned at_items = 0;
+    uint32_t phase = 0;
     bool begin = true;                          // of an item, here
     int from = at.s;
     for (int i = 0, stage = 0; i < count; ++i) {
@@ -403,12 +459,11 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
             begin = false;
         }
         if (i + S::kStages - 1 < count) load_next(i + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
-        __syncwarp();
+        if (!paged_wait(bars + 8 * stage, phase, P.status, P.wait_limit)) return;
+        paged_clear<DP>(at.R, at.s, ring + stage * 2 * S::kTileBytes);
         heads.step(at.R, at.s, P.factor, ring + stage * 2 * S::kTileBytes);
         __syncwarp();                           // the stage may be filled again
-        if (++stage == S::kStages) stage = 0;
+        if (++stage == S::kStages) { stage = 0; phase ^= 1; }
         const int seq = at.seq;
         const bool seq_bad = at.R.bad != 0, last = at.s + 1 == at.R.steps;
         if (last || i + 1 == count) {
@@ -426,10 +481,12 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) paged_whole_kernel(const __grid_constant__ PagedParams P) {
     using S = PagedShape<DP>;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* const boxes = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const nq_attention_desc& d = P.d;
     const int warp = threadIdx.x >> 5;
-    const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
+    const uint32_t smem = smem_u32(boxes), ring = smem + warp * S::kWarpBytes, bars = smem + S::kBarOff + 8 * warp * S::kStages;
+    paged_rings<DP>(smem);
     const int per_seq = d.k_heads * P.chunks, seq = blockIdx.x / per_seq, item = blockIdx.x - seq * per_seq;
     const int kh = item / P.chunks, chunk = item - kh * P.chunks;
     const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
@@ -439,31 +496,28 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     const PagedRange R = paged_range(d, seq, P.shift);
     const int mine = (R.steps + kPagedWarps - 1) / kPagedWarps, s0 = warp * mine, s1 = min(s0 + mine, R.steps);
     static_assert(kPagedWhole / kPagedStep / kPagedWarps <= 32, "one look at the table");
-    PagedPages pages;
+    PagedPages pages{};
     bool bad = R.bad != 0;
     if (!pages.look(d, P.shift, seq, R, s0, s1)) bad = true;
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-        if (s0 + i < s1) paged_load<DP>(d, R, pages, kh, s0 + i, ring + i * 2 * S::kTileBytes);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    for (int i = 0; i < S::kStages - 1; ++i)
+        if (s0 + i < s1) paged_load<DP>(P, R, pages, kh, s0 + i, ring + i * 2 * S::kTileBytes, bars + 8 * i);
+    uint32_t phase = 0;
     for (int s = s0, stage = 0; s < s1; ++s) {
-        const int ahead = s + S::kStages - 1;
-        if (ahead < s1) paged_load<DP>(d, R, pages, kh, ahead, ring + (stage == 0 ? S::kStages - 1 : stage - 1) * 2 * S::kTileBytes);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
-        __syncwarp();
+        const int ahead = s + S::kStages - 1, to = stage == 0 ? S::kStages - 1 : stage - 1;
+        if (ahead < s1) paged_load<DP>(P, R, pages, kh, ahead, ring + to * 2 * S::kTileBytes, bars + 8 * to);
+        if (!paged_wait(bars + 8 * stage, phase, P.status, P.wait_limit)) break;
+        paged_clear<DP>(R, s, ring + stage * 2 * S::kTileBytes);
         heads.step(R, s, P.factor, ring + stage * 2 * S::kTileBytes);
         __syncwarp();
-        if (++stage == S::kStages) stage = 0;
+        if (++stage == S::kStages) { stage = 0; phase ^= 1; }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     heads.finish(__syncthreads_or(bad));
-    heads.save(reinterpret_cast<float*>(smem) + warp * S::kPart, rows);
+    heads.save(reinterpret_cast<float*>(boxes) + warp * S::kPart, rows);
     __syncthreads();
     for (int i = threadIdx.x; i < rows * (DP / 2); i += kPagedThreads) {
         const int row = i / (DP / 2), col = 2 * (i - row * (DP / 2));
-        const float* at = reinterpret_cast<const float*>(smem) + row * S::kRow;
+        const float* at = reinterpret_cast<const float*>(boxes) + row * S::kRow;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, at[w * S::kPart + DP]);
@@ -665,14 +719,22 @@ size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int 
     return (size_t)paged_ctas(dp) * kPagedWarps * 2 * kPagedRows * (dp + 2) * sizeof(float);
 }
 
-int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t scratch_bytes, nq_stream_t stream) {
+int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t scratch_bytes, void* status_word, nq_stream_t stream) {
     using namespace nq;
-    if (!desc) return NQ_ERR_NULL;
+    if (!desc || !status_word) return NQ_ERR_NULL;
     const nq_attention_desc& d = *desc;
     int st = attention_check(d);
     if (st == NQ_OK) st = attention_cache_check(d);
     if (st != NQ_OK) return st;
-    PagedParams P{d, log2_of(d.page_size), d.q_heads / d.k_heads, 0, 0, 0, d.scale * 1.44269504088896340736f, static_cast<float*>(scratch)};
+    if (!aligned16(status_word)) return NQ_ERR_ALIGN;
+    PagedParams P{};
+    P.d = d;
+    P.shift = log2_of(d.page_size);
+    P.rows = d.q_heads / d.k_heads;
+    P.factor = d.scale * 1.44269504088896340736f;
+    P.wait_limit = gemm_wait_limit();
+    P.status = static_cast<unsigned*>(status_word) + 2;
+    P.part = static_cast<float*>(scratch);
     P.chunks = (P.rows + kPagedRows - 1) / kPagedRows;
     const int64_t most = (int64_t)d.max_pages * d.page_size, items = (int64_t)d.seqs * d.k_heads * P.chunks;
     if (most > 0x7fffff00 || items > 0x3fffffff) return NQ_ERR_TOO_LARGE;
@@ -685,6 +747,10 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     P.items = (int)items;
     const bool whole = need == 0;
     const bool bf = d.dtype == NQ_BF16;
+    const int type = bf ? kMmBf16 : kMmF16, box = d.page_size < kPagedStep ? d.page_size : kPagedStep;
+    st = mm_encode_heads(&P.map_k, d.k, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.k_slot, d.k_head, d.k_page}, {64, box, 1, 1});
+    if (st == NQ_OK) st = mm_encode_heads(&P.map_v, d.v, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.v_slot, d.v_head, d.v_page}, {64, box, 1, 1});
+    if (st != NQ_OK) return st;
     switch (padded_columns(d.D)) {
         case 64: return bf ? paged_launch<64, true>(P, whole, as_stream(stream)) : paged_launch<64, false>(P, whole, as_stream(stream));
         case 128: return bf ? paged_launch<128, true>(P, whole, as_stream(stream)) : paged_launch<128, false>(P, whole, as_stream(stream));

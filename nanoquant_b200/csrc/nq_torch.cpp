@@ -1154,7 +1154,7 @@ Tensor attention_launch(const AttentionArgs& a) {
     } else {
         const size_t bytes = nq_paged_attention_scratch_bytes(d.seqs, d.q_heads, d.k_heads, d.D, (int64_t)d.max_pages * d.page_size);
         const Tensor scratch = bytes ? new_bytes((int64_t)bytes, *a.q) : Tensor();
-        st = nq_paged_attention_fwd(&d, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, stream_of(dev));
+        st = nq_paged_attention_fwd(&d, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, status_header(dev), stream_of(dev));
         if (st < 0) fail(st, "nq_paged_attention_fwd");
     }
     return out;

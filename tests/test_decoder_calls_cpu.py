@@ -72,10 +72,11 @@ def test_paged_attention_refusals():
     need = L.nq_paged_attention_scratch_bytes(2, 8, 2, 64, 640)
     assert need > 0 and need % 16 == 0 and L.nq_paged_attention_scratch_bytes(2, 8, 2, 64, 256) == 0 and L.nq_paged_attention_scratch_bytes(0, 8, 2, 64, 640) == 0
     assert L.nq_paged_attention_scratch_bytes(1000, 8, 2, 64, 1 << 20) == need                  # by CTAs, not by sequences
-    assert L.nq_paged_attention_fwd(None, P, need, None) == _lib.NQ_ERR_NULL
-    call = lambda d, scratch=P, n=need: L.nq_paged_attention_fwd(ctypes.byref(_lib.AttentionDesc(**d)), scratch, n, None)
+    assert L.nq_paged_attention_fwd(None, P, need, P, None) == _lib.NQ_ERR_NULL
+    call = lambda d, scratch=P, n=need, status=P: L.nq_paged_attention_fwd(ctypes.byref(_lib.AttentionDesc(**d)), scratch, n, status, None)
     refused(call, PAGED, COMMON + CACHE + [("block_table", None, "NULL"), (("max_pages", "page_size"), (1 << 20, 1 << 12), "TOO_LARGE")])
     assert call(PAGED, None) == _lib.NQ_ERR_NULL and call(PAGED, P + 4) == _lib.NQ_ERR_ALIGN and call(PAGED, P, need - 1) == _lib.NQ_ERR_SCRATCH
+    assert call(PAGED, P, need, None) == _lib.NQ_ERR_NULL and call(PAGED, P, need, P + 4) == _lib.NQ_ERR_ALIGN
 
 
 def test_prompt_attention_refusals():
