@@ -173,8 +173,10 @@ int mm_encode_heads(CUtensorMap* map, const void* p, int type, const HeadSizes& 
     }
     // (the stride of a single element means nothing, but has to be a valid one)
     for (int i = 0; i < 3; ++i) bytes[i] = n[i + 1] == 1 ? (cuuint64_t)(sizes.n[0] * 2) : (cuuint64_t)strides.n[i] * 2;
+    // (a head of up to 64 columns is one line of the L2 cache: the line behind it is another head's, which is read elsewhere)
+    const CUtensorMapL2promotion promotion = sizes.n[0] <= 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
     const CUresult r = enc(map, type == kMmBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), n, bytes, b, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? NQ_OK : NQ_ERR_UNSUPPORTED;
 }
 

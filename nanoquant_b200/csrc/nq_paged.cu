@@ -5,16 +5,22 @@
 // Bound by memory: keys and values are read once, for all the query heads that share them: 4 D bytes for 4 D G operations.  Those G heads are the rows of
 // mma.sync.m16n8k16 (up to 16; the instruction's rate is far above what memory delivers, and few rows would leave tcgen05's 128 idle).
 //
-// Work.  The tokens that a sequence's query sees are cut into steps of 16.  An item is a sequence, a key head and up to 16 of its query heads; the steps of all
-// items lie one behind the other, and every warp takes the same number of them, found from the lengths on the device: batches of any lengths fill the
-// SMs evenly, and a captured graph follows the lengths.  A warp has a ring of steps of its own in shared memory (TMA boxes of 16 tokens x 64
-// columns; it runs on into the next item), its own running maximum, sum and accumulators: nothing in the loop waits for another warp.  (Copied by cp.async, 16 bytes a lane,
-// a step was 650 instructions, 1.3 us of a warp alone, and 6.0 TB/s; by bulk copies of 256-byte rows 4.4 TB/s.)  An item that lies in several warps leaves fp32 results
-// (m, sum, unnormalised o) in the scratch, which a second, overlapped launch joins in their order.  Caches without room for long sequences take a CTA per item, its
-// steps divided among the four warps and their results joined through shared memory: one launch.
+// Work.  The tokens that a sequence's query sees are cut into steps of 16 (heads of up to 64 columns: 32).  An item is a sequence, a key head and up to
+// 16 of its query heads; the steps of all items lie one behind the other, and every warp takes the same number of them, found from the lengths on the
+// device: batches of any lengths fill the SMs evenly, and a captured graph follows the lengths.  A warp has a ring of steps of its own in shared memory
+// (TMA boxes of a page's tokens x 64 columns; it runs on into the next item), its own running maximum, sum and accumulators: nothing in the loop waits
+// for another warp.  (Copied by cp.async, 16 bytes a lane, the same steps were as fast when full, 150 us against 153 for 4 sequences of up to 131072
+// tokens, but 650 instructions each where these have 400; bulk copies of 256-byte rows took 206 us.)  An item that lies in several warps leaves fp32
+// results (m, sum, unnormalised o) in the scratch, which a second, overlapped launch joins in their order.  Caches without room for long sequences take
+// a CTA per item, its steps divided among the four warps and their results joined through shared memory: one launch.
+//
+// Measured: 32 sequences of up to 4096 tokens, 32 heads of 128, fp16: 106 us, 5.97 TB/s; 4 of up to 131072, 64 heads on 8, bf16: 153 us, 5.96 TB/s, of
+// which 12 us are start, join and the uneven end (each further token: 6.7 TB/s, a plain copy's rate); one of 1000, 32 heads on 8: 8.3 us, two launches.
 //
 // The weights p are rounded to the operands' type for the product with the values: 2^-9 (bf16) or 2^-12 (fp16) of each, which the average over
 // tokens does not enlarge.  Sums of p are fp32 sums of the rounded values.
+#include <algorithm>
+
 #include "nq_attn.cuh"
 #include "nq_stage.h"
 #include "nq_tcgen05.cuh"
@@ -22,7 +28,6 @@
 namespace nq {
 
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
-constexpr int kPagedStep = 16;                  // tokens
 constexpr int kPagedRows = 16;                  // query heads of an item at most
 constexpr int kPagedWhole = 256;                // caches of up to so many tokens a sequence: a CTA per item
 
@@ -30,6 +35,7 @@ struct alignas(64) PagedParams {
     CUtensorMap map_k, map_v;
     nq_attention_desc d;
     int shift;                                  // log2(page_size)
+    int step, box;                              // tokens of a step, and of a box of it (a page's at most)
     int rows, chunks;                           // query heads to a key head; items of 16 of them
     int warps;                                  // of the split kernel
     int items;                                  // (of all sequences)
@@ -42,18 +48,19 @@ struct alignas(64) PagedParams {
 // Steps of a sequence's items, and what they cover.
 struct PagedRange {
     int begin, end;                             // tokens seen
-    int first, steps;                           // steps of 16 tokens; one at least, so that somebody writes the result
+    int first, steps;                           // of PagedParams::step tokens; one at least, so that somebody writes the result
     int bad;                                    // the table does not hold the sequence
 };
-__device__ __forceinline__ PagedRange paged_range(const nq_attention_desc& d, int s, int shift) {
+__device__ __forceinline__ PagedRange paged_range(const PagedParams& P, int s) {
+    const nq_attention_desc& d = P.d;
     PagedRange r;
     const int n = __ldcg(d.lengths + s);
     r.end = max(n, 0);
-    r.bad = (long long)r.end > ((long long)d.max_pages << shift);
+    r.bad = (long long)r.end > ((long long)d.max_pages << P.shift);
     if (r.bad) r.end = 0;
     r.begin = d.window > 0 ? max(r.end - d.window, 0) : 0;
-    r.first = r.begin / kPagedStep;
-    r.steps = max((r.end + kPagedStep - 1) / kPagedStep - r.first, 1);
+    r.first = r.begin / P.step;
+    r.steps = max((r.end + P.step - 1) / P.step - r.first, 1);
     return r;
 }
 
@@ -92,7 +99,7 @@ __device__ __forceinline__ long long paged_total(const PagedParams& P, PagedPlan
         const int s = s0 + threadIdx.x;
         n = 0;
         if (s < P.d.seqs) {
-            range = paged_range(P.d, s, P.shift);
+            range = paged_range(P, s);
             n = (long long)range.steps * per_seq;
         }
         long long some;
@@ -118,7 +125,7 @@ __device__ __forceinline__ void paged_find(const PagedParams& P, PagedPlan& plan
             const int s = s0 + threadIdx.x;
             n = 0;
             if (s < P.d.seqs) {
-                range = paged_range(P.d, s, P.shift);
+                range = paged_range(P, s);
                 n = (long long)range.steps * per_seq;
             }
             long long some;
@@ -149,17 +156,21 @@ __device__ __forceinline__ void paged_box(uint32_t dst, const CUtensorMap* map, 
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
 }
+// A warp's step is bound by its own latency, so what counts is how many warps an SM has, each with one step on its way while it works on another:
+// three CTAs of rings of 2 (columns up to 128) moved 5.97 TB/s at 32 sequences of up to 4096 tokens and 32 heads of 128, two of rings of 3 moved
+// 5.8; with heads of 64, 8 x 131072 tokens, 5.8 TB/s instead of 5.5 (one CTA: 2.7).  Of 64 columns a step has 32 tokens: with 16 and four CTAs an SM, 5.55.
 template <int DP> struct PagedShape {
     static constexpr int kColumns = DP / 64;                      // boxes of 64 columns: rows of 128 bytes, 128-byte swizzle
-    static constexpr int kBoxBytes = kPagedStep * 128;
-    static constexpr int kTileBytes = kColumns * kBoxBytes;       // of keys, or of values
-    static constexpr int kStages = DP == 64 ? 4 : 3;
+    static constexpr int kStep = DP == 64 ? 32 : 16;              // tokens of a step
+    static constexpr int kColumnBytes = kStep * 128;
+    static constexpr int kTileBytes = kColumns * kColumnBytes;    // of keys, or of values
+    static constexpr int kStages = DP <= 128 ? 2 : 3;
     static constexpr int kWarpBytes = 2 * kStages * kTileBytes;
     static constexpr int kBarOff = kPagedWarps * kWarpBytes;
     static constexpr int kSmem = 1024 + kBarOff + 8 * kPagedWarps * kStages;
     static constexpr int kRow = DP + 2;                           // floats of a head's result: o, m, sum
     static constexpr int kPart = kPagedRows * kRow;
-    static constexpr int kCtasPerSm = DP == 64 ? 3 : DP == 128 ? 2 : 1;
+    static constexpr int kCtasPerSm = DP <= 128 ? 3 : 1;
     static_assert(kPagedWarps * kPart * 4 <= kBarOff, "the warps' results fit the rings");
     static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory");
 };
@@ -182,59 +193,47 @@ __device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, unsign
     return false;
 }
 
-// The pages of 32 steps of an item, held by the lanes of a warp: the one of lane i's step, and (pages of 8 tokens) of its second half.
+// The pages of 32 boxes of an item, one after the other, held by the lanes of a warp.
 struct PagedPages {
-    int page0, page1, from;
-    // `to`: steps from there on are not wanted.  False: a page outside the cache.
-    __device__ __forceinline__ bool look(const nq_attention_desc& d, int shift, int seq, const PagedRange& R, int s, int to) {
-        const int* table = d.block_table + (long long)seq * d.table_stride;
-        const int lane = threadIdx.x & 31, mine = s + lane;
-        bool bad = false;
-        auto one = [&](int token) {
-            // (only pages that hold a token that is seen)
-            if (mine >= to || token >= R.end || token + min(d.page_size, kPagedStep) <= R.begin) return 0;
-            const int p = __ldcg(table + (token >> shift));
-            if (p < 0 || p >= d.pages) { bad = true; return 0; }
-            return p;
-        };
-        const int t = mine < to ? (R.first + mine) * kPagedStep : 0;
-        page0 = one(t);
-        page1 = d.page_size < kPagedStep ? one(t + 8) : page0;
+    int page, from, until;                      // until: the step behind the last whose pages are here
+    // From step s on; `to`: steps from there on are not wanted.  False: a page outside the cache.
+    template <int STEP>
+    __device__ __forceinline__ bool look(const PagedParams& P, int seq, const PagedRange& R, int s, int to) {
+        const nq_attention_desc& d = P.d;
+        const int boxes = STEP / P.box, lane = threadIdx.x & 31;
+        until = s + 32 / boxes;
         from = s;
+        const int token = (R.first + s) * STEP + lane * P.box;
+        // (only pages that hold a token that is seen)
+        page = 0;
+        bool bad = false;
+        if (s + lane / boxes < to && token < R.end && token + P.box > R.begin) {
+            const int p = __ldcg(d.block_table + (long long)seq * d.table_stride + (token >> P.shift));
+            if (p < 0 || p >= d.pages) bad = true;
+            else page = p;
+        }
         return !__any_sync(0xffffffffu, bad);
     }
 };
-// Keys and values of step s into a stage: a box for each page (one, or two pages of 8) and 64 columns.
+// Keys and values of step s into a stage: boxes of a page's tokens and 64 columns.
 template <int DP>
 __device__ __forceinline__ void paged_load(const PagedParams& P, const PagedRange& R, const PagedPages& pages, int kh, int s, uint32_t kt, uint32_t bar) {
     using S = PagedShape<DP>;
     const nq_attention_desc& d = P.d;
-    const int src = s - pages.from;
-    const int pa = __shfl_sync(0xffffffffu, pages.page0, src), pb = __shfl_sync(0xffffffffu, pages.page1, src);
-    if (elect_one()) {
-        const int token = (R.first + s) * kPagedStep, slot = token & (d.page_size - 1);
-        if (d.page_size >= kPagedStep) {
-            mbar_expect_tx(bar, 2 * S::kTileBytes);
+    const int boxes = S::kStep / P.box, lane = threadIdx.x & 31, token = (R.first + s) * S::kStep + lane * P.box;
+    const int page = __shfl_sync(0xffffffffu, pages.page, ((s - pages.from) * boxes + lane) & 31);
+    // (a page that holds nothing that is seen is not looked at; of no tokens at all the first box is, so that something arrives)
+    const bool mine = lane < boxes && ((token < R.end && token + P.box > R.begin) || (lane == 0 && R.end <= token));
+    const unsigned all = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(all) * P.box * 256 * S::kColumns));
+    __syncwarp();
+    if (mine) {
+        const uint32_t dst = kt + lane * P.box * 128;
+        const int slot = token & (d.page_size - 1);
 #pragma unroll
-            for (int c = 0; c < S::kColumns; ++c) {
-                paged_box(kt + c * S::kBoxBytes, &P.map_k, 64 * c, slot, kh, pa, bar);
-                paged_box(kt + S::kTileBytes + c * S::kBoxBytes, &P.map_v, 64 * c, slot, kh, pa, bar);
-            }
-        } else {
-            // (a page that holds nothing that is seen is not looked at)
-            const bool second = token + 8 < R.end, first = token + 8 > R.begin;
-            mbar_expect_tx(bar, (uint32_t)((int)first + (int)second) * S::kTileBytes);
-#pragma unroll
-            for (int c = 0; c < S::kColumns; ++c) {
-                if (first) {
-                    paged_box(kt + c * S::kBoxBytes, &P.map_k, 64 * c, 0, kh, pa, bar);
-                    paged_box(kt + S::kTileBytes + c * S::kBoxBytes, &P.map_v, 64 * c, 0, kh, pa, bar);
-                }
-                if (second) {
-                    paged_box(kt + c * S::kBoxBytes + 1024, &P.map_k, 64 * c, 0, kh, pb, bar);
-                    paged_box(kt + S::kTileBytes + c * S::kBoxBytes + 1024, &P.map_v, 64 * c, 0, kh, pb, bar);
-                }
-            }
+        for (int c = 0; c < S::kColumns; ++c) {
+            paged_box(dst + c * S::kColumnBytes, &P.map_k, 64 * c, slot, kh, page, bar);
+            paged_box(dst + S::kTileBytes + c * S::kColumnBytes, &P.map_v, 64 * c, slot, kh, page, bar);
         }
     }
     __syncwarp();
@@ -243,13 +242,13 @@ __device__ __forceinline__ void paged_load(const PagedParams& P, const PagedRang
 template <int DP>
 __device__ __forceinline__ void paged_clear(const PagedRange& R, int s, uint32_t kt) {
     using S = PagedShape<DP>;
-    const int lane = threadIdx.x & 31, token0 = (R.first + s) * kPagedStep;
-    if (token0 >= R.begin && token0 + kPagedStep <= R.end) return;
-    const int token = token0 + (lane & 15);
-    if (token < R.begin || token >= R.end) {
-        const uint32_t at = kt + S::kTileBytes + (lane & 15) * 128 + (lane >> 4) * 64;
-        for (int c = 0; c < S::kColumns; ++c)
-            for (int u = 0; u < 4; ++u) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + c * S::kBoxBytes + 16 * u), "r"(0) : "memory");
+    const int lane = threadIdx.x & 31, token0 = (R.first + s) * S::kStep;
+    if (token0 >= R.begin && token0 + S::kStep <= R.end) return;
+    for (int r = lane; r < S::kStep * S::kColumns; r += 32) {
+        const int token = token0 + r % S::kStep;
+        if (token < R.begin || token >= R.end)
+            for (int u = 0; u < 8; ++u)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(kt + S::kTileBytes + r / S::kStep * S::kColumnBytes + r % S::kStep * 128 + 16 * u), "r"(0) : "memory");
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // (before a later copy to the same place)
     __syncwarp();
@@ -280,24 +279,28 @@ struct PagedHeads {
     }
     __device__ __forceinline__ void step(const PagedRange& R, int s, float factor, uint32_t kt) {
         using S = PagedShape<DP>;
+        constexpr int kSub = S::kStep / 16;
         const int lane = threadIdx.x & 31, q = lane & 3;
         // 16 bytes number u of row r are at u ^ (r & 7)
         const uint32_t k_at = kt + ((lane & 7) + ((lane >> 4) << 3)) * 128, k_unit = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
         const uint32_t v_at = kt + S::kTileBytes + ((lane & 7) + (((lane >> 3) & 1) << 3)) * 128, v_unit = ((lane >> 4) ^ (lane & 7)) << 4;
-        float c[2][4] = {};
+        float c[2 * kSub][4] = {};
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-            uint32_t b[4];
-            // matrices: keys 0-7 and 8-15 (lanes 8-15 / 24-31: the second 8 columns)
-            ldmatrix4(b, k_at + (k >> 2) * S::kBoxBytes + (k_unit ^ (32 * (k & 3))));
-            paged_mma<BF16>(c[0], a[k], b[0], b[1]);
-            paged_mma<BF16>(c[1], a[k], b[2], b[3]);
+#pragma unroll
+            for (int t = 0; t < kSub; ++t) {
+                uint32_t b[4];
+                // matrices: keys 0-7 and 8-15 (lanes 8-15 / 24-31: the second 8 columns)
+                ldmatrix4(b, k_at + 2048 * t + (k >> 2) * S::kColumnBytes + (k_unit ^ (32 * (k & 3))));
+                paged_mma<BF16>(c[2 * t], a[k], b[0], b[1]);
+                paged_mma<BF16>(c[2 * t + 1], a[k], b[2], b[3]);
+            }
         }
         // lane: heads g (c[.][0..1]) and g + 8 (c[.][2..3]), tokens 8 n + 2 q + (i & 1)
-        const int token0 = (R.first + s) * kPagedStep;
-        if (token0 < R.begin || token0 + kPagedStep > R.end) {
+        const int token0 = (R.first + s) * S::kStep;
+        if (token0 < R.begin || token0 + S::kStep > R.end) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8 * kSub; ++i) {
                 const int token = token0 + 8 * (i >> 2) + 2 * q + (i & 1);
                 if (token < R.begin || token >= R.end) c[i >> 2][i & 3] = -INFINITY;
             }
@@ -305,7 +308,9 @@ struct PagedHeads {
         float top[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            top[r] = fmaxf(fmaxf(c[0][2 * r], c[0][2 * r + 1]), fmaxf(c[1][2 * r], c[1][2 * r + 1]));
+            top[r] = fmaxf(c[0][2 * r], c[0][2 * r + 1]);
+#pragma unroll
+            for (int n = 1; n < 2 * kSub; ++n) top[r] = fmaxf(top[r], fmaxf(c[n][2 * r], c[n][2 * r + 1]));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * factor;
         }
@@ -324,25 +329,31 @@ struct PagedHeads {
                 }
             }
         }
-        uint32_t p[4];
+        uint32_t p[kSub][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const float base = m[r] == -INFINITY ? 0.f : m[r];
-            float e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = exp2_approx(fmaf(c[i >> 1][2 * r + (i & 1)], factor, -base));
-            p[r] = head_pack<BF16>(e[0], e[1]);
-            p[2 + r] = head_pack<BF16>(e[2], e[3]);
+            for (int t = 0; t < kSub; ++t) {
+                float e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) l[r] += head_float<BF16>(i < 2 ? p[r] : p[2 + r], i & 1);
+                for (int i = 0; i < 4; ++i) e[i] = exp2_approx(fmaf(c[2 * t + (i >> 1)][2 * r + (i & 1)], factor, -base));
+                p[t][r] = head_pack<BF16>(e[0], e[1]);
+                p[t][2 + r] = head_pack<BF16>(e[2], e[3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l[r] += head_float<BF16>(i < 2 ? p[t][r] : p[t][2 + r], i & 1);
+            }
         }
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
-            uint32_t b[4];
-            // matrices (transposed): tokens 0-7 and 8-15 of columns 16 n .., then of 16 n + 8 ..
-            ldmatrix4_trans(b, v_at + (n >> 2) * S::kBoxBytes + (v_unit ^ (32 * (n & 3))));
-            paged_mma<BF16>(o[2 * n], p, b[0], b[1]);
-            paged_mma<BF16>(o[2 * n + 1], p, b[2], b[3]);
+#pragma unroll
+            for (int t = 0; t < kSub; ++t) {
+                uint32_t b[4];
+                // matrices (transposed): tokens 0-7 and 8-15 of columns 16 n .., then of 16 n + 8 ..
+                ldmatrix4_trans(b, v_at + 2048 * t + (n >> 2) * S::kColumnBytes + (v_unit ^ (32 * (n & 3))));
+                paged_mma<BF16>(o[2 * n], p[t], b[0], b[1]);
+                paged_mma<BF16>(o[2 * n + 1], p[t], b[2], b[3]);
+            }
         }
     }
     // The sums over the lanes of a row; NaN for a sequence that is not there.
@@ -408,6 +419,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     struct Cursor {
         PagedRange R;
         int seq, item, s;                       // item of the sequence; the next step
+        int kh, chunk;                          // of the item
     } load, at;
     {
         const PagedPlace& p = plan.place[warp];
@@ -415,14 +427,17 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
         load.seq = p.seq;
         load.item = (int)((unit - p.before) / load.R.steps);
         load.s = (int)(unit - p.before - (long long)load.item * load.R.steps);
+        load.kh = load.item / P.chunks;
+        load.chunk = load.item - load.kh * P.chunks;
     }
     at = load;
     auto advance = [&](Cursor& c) {             // (true: behind the last step of an item)
         if (++c.s < c.R.steps) return false;
         c.s = 0;
+        if (++c.chunk == P.chunks) { c.chunk = 0; ++c.kh; }
         if (++c.item == per_seq) {
-            c.item = 0;
-            if (++c.seq < d.seqs) c.R = paged_range(d, c.seq, P.shift);
+            c.item = c.kh = 0;
+            if (++c.seq < d.seqs) c.R = paged_range(P, c.seq);
         }
         return true;
     };
@@ -430,12 +445,12 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     bool fresh = true;
     unsigned bad_items = 0, load_items = 0;     // (bit i: the i-th item from here on, modulo 32, has a page outside the cache; a ring holds far fewer)
     auto load_next = [&](int i, int stage) {    // step i of this warp's
-        if (fresh || load.s - pages.from >= 32) {
-            const bool ok = pages.look(d, P.shift, load.seq, load.R, load.s, min(load.R.steps, load.s + (count - i)));
+        if (fresh || load.s >= pages.until) {
+            const bool ok = pages.look<S::kStep>(P, load.seq, load.R, load.s, min(load.R.steps, load.s + (count - i)));
             if (!ok) bad_items |= 1u << (load_items & 31);
             fresh = false;
         }
-        paged_load<DP>(P, load.R, pages, load.item / P.chunks, load.s, ring + stage * 2 * S::kTileBytes, bars + 8 * stage);
+        paged_load<DP>(P, load.R, pages, load.kh, load.s, ring + stage * 2 * S::kTileBytes, bars + 8 * stage);
         if (advance(load)) {
             fresh = true;
             ++load_items;
@@ -449,11 +464,11 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     unsigned at_items = 0;
     uint32_t phase = 0;
     bool begin = true;                          // of an item, here
-    int from = at.s;
+    int from = at.s, h0 = 0, rows = 0;
     for (int i = 0, stage = 0; i < count; ++i) {
-        const int kh = at.item / P.chunks, chunk = at.item - kh * P.chunks;
-        const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
         if (begin) {
+            h0 = at.kh * P.rows + at.chunk * kPagedRows;
+            rows = min(kPagedRows, P.rows - at.chunk * kPagedRows);
             heads.start(d, at.seq, h0, rows);
             from = at.s;
             begin = false;
@@ -493,12 +508,12 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     asm volatile("griddepcontrol.wait;" ::: "memory");
     PagedHeads<DP, BF16> heads;
     heads.start(d, seq, h0, rows);
-    const PagedRange R = paged_range(d, seq, P.shift);
+    const PagedRange R = paged_range(P, seq);
     const int mine = (R.steps + kPagedWarps - 1) / kPagedWarps, s0 = warp * mine, s1 = min(s0 + mine, R.steps);
-    static_assert(kPagedWhole / kPagedStep / kPagedWarps <= 32, "one look at the table");
+    static_assert(kPagedWhole / 8 / kPagedWarps <= 32, "one look at the table");
     PagedPages pages{};
     bool bad = R.bad != 0;
-    if (!pages.look(d, P.shift, seq, R, s0, s1)) bad = true;
+    if (!pages.look<S::kStep>(P, seq, R, s0, s1)) bad = true;
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i)
         if (s0 + i < s1) paged_load<DP>(P, R, pages, kh, s0 + i, ring + i * 2 * S::kTileBytes, bars + 8 * i);
@@ -567,10 +582,10 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_consta
             for (int s0 = 0; s0 < seq; s0 += THREADS) {
                 const int s = s0 + threadIdx.x;
                 long long some;
-                block_scan(s < seq ? (long long)paged_range(d, s, P.shift).steps * per_seq : 0, plan.sums, some);
+                block_scan(s < seq ? (long long)paged_range(P, s).steps * per_seq : 0, plan.sums, some);
                 before += some;
             }
-            if (threadIdx.x == 0) plan.place[0] = {before, seq, paged_range(d, seq, P.shift)};
+            if (threadIdx.x == 0) plan.place[0] = {before, seq, paged_range(P, seq)};
         }
         __syncthreads();
     } else {
@@ -660,7 +675,7 @@ static int padded_columns(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int paged_ctas(int dp) { return sm_count() * (dp == 64 ? PagedShape<64>::kCtasPerSm : dp == 128 ? PagedShape<128>::kCtasPerSm : PagedShape<256>::kCtasPerSm); }
 
 template <int DP, bool BF16>
-static int paged_launch(PagedParams& P, bool whole, cudaStream_t stream) {
+static int paged_launch(PagedParams& P, bool whole, int64_t most_steps, cudaStream_t stream) {
     static bool attr_set[64];
     int dev = 0;
     NQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -670,9 +685,11 @@ static int paged_launch(PagedParams& P, bool whole, cudaStream_t stream) {
         NQ_CUDA_TRY(cudaFuncSetAttribute(whole_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DP>::kSmem));
         attr_set[dev & 63] = true;
     }
-    P.warps = paged_ctas(DP) * kPagedWarps;
+    // (no more CTAs than the table has steps for: one sequence of 1000 tokens takes 126 of the 444)
+    const int ctas = (int)std::min<int64_t>(paged_ctas(DP), (most_steps + kPagedWarps - 1) / kPagedWarps);
+    P.warps = ctas * kPagedWarps;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(whole ? P.items : paged_ctas(DP)));
+    cfg.gridDim = dim3((unsigned)(whole ? P.items : ctas));
     cfg.blockDim = dim3(kPagedThreads);
     cfg.dynamicSmemBytes = PagedShape<DP>::kSmem;
     cfg.stream = stream;
@@ -747,14 +764,17 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     P.items = (int)items;
     const bool whole = need == 0;
     const bool bf = d.dtype == NQ_BF16;
-    const int type = bf ? kMmBf16 : kMmF16, box = d.page_size < kPagedStep ? d.page_size : kPagedStep;
-    st = mm_encode_heads(&P.map_k, d.k, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.k_slot, d.k_head, d.k_page}, {64, box, 1, 1});
-    if (st == NQ_OK) st = mm_encode_heads(&P.map_v, d.v, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.v_slot, d.v_head, d.v_page}, {64, box, 1, 1});
+    const int type = bf ? kMmBf16 : kMmF16;
+    P.step = padded_columns(d.D) == 64 ? PagedShape<64>::kStep : PagedShape<128>::kStep;
+    P.box = d.page_size < P.step ? d.page_size : P.step;
+    st = mm_encode_heads(&P.map_k, d.k, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.k_slot, d.k_head, d.k_page}, {64, P.box, 1, 1});
+    if (st == NQ_OK) st = mm_encode_heads(&P.map_v, d.v, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.v_slot, d.v_head, d.v_page}, {64, P.box, 1, 1});
     if (st != NQ_OK) return st;
+    const int64_t most_steps = items * ((most + P.step - 1) / P.step);
     switch (padded_columns(d.D)) {
-        case 64: return bf ? paged_launch<64, true>(P, whole, as_stream(stream)) : paged_launch<64, false>(P, whole, as_stream(stream));
-        case 128: return bf ? paged_launch<128, true>(P, whole, as_stream(stream)) : paged_launch<128, false>(P, whole, as_stream(stream));
-        default: return bf ? paged_launch<256, true>(P, whole, as_stream(stream)) : paged_launch<256, false>(P, whole, as_stream(stream));
+        case 64: return bf ? paged_launch<64, true>(P, whole, most_steps, as_stream(stream)) : paged_launch<64, false>(P, whole, most_steps, as_stream(stream));
+        case 128: return bf ? paged_launch<128, true>(P, whole, most_steps, as_stream(stream)) : paged_launch<128, false>(P, whole, most_steps, as_stream(stream));
+        default: return bf ? paged_launch<256, true>(P, whole, most_steps, as_stream(stream)) : paged_launch<256, false>(P, whole, most_steps, as_stream(stream));
     }
 }
 

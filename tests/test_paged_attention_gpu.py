@@ -69,6 +69,23 @@ def test_what_is_not_seen_has_no_influence(page):
     check_attention(ops.paged_attention(q, kc, vc, table, n, window=window), want)
 
 
+@pytest.mark.parametrize("page,window", [(8, 70), (8, 3), (16, 33), (32, 40), (64, 64)])
+def test_narrow_heads_and_pages_that_are_not_seen(page, window):
+    """Heads of 64 columns, whose steps have several pages: those outside a window are NaN, or do not exist, one after the other in a step."""
+    from nanoquant_b200 import ops
+
+    lengths = [301, 40, 1000, 67, 0, 9]
+    q, k, v, kc, vc, table, n = make(lengths, 8, 2, 64, page, torch.bfloat16)
+    want = expected(q, k, v, window)
+    for s, m in enumerate(lengths):
+        for t in range(max(0, m - window)):
+            p = table[s, t // page].item()
+            kc[p, t % page] = float("nan")
+            vc[p, t % page] = float("inf")
+        table[s, :max(0, m - window) // page] = -1
+    check_attention(ops.paged_attention(q, kc, vc, table, n, window=window), want)
+
+
 @pytest.mark.parametrize("width", [16, 100])
 def test_sequences_that_are_not_there_are_nan(width):
     """A page outside the cache, a length beyond the table: NaN in all of that sequence's outputs, the others untouched."""
