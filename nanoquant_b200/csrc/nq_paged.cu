@@ -754,7 +754,7 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     P.part = static_cast<float*>(scratch);
     P.chunks = (P.rows + kPagedRows - 1) / kPagedRows;
     const int64_t most = (int64_t)d.max_pages * d.page_size, items = (int64_t)d.seqs * d.k_heads * P.chunks;
-    if (most > 0x7fffff00 || items > 0x3fffffff) return NQ_ERR_TOO_LARGE;
+    if (most > 0x3fffffff || items > 0x3fffffff) return NQ_ERR_TOO_LARGE;
     const size_t need = nq_paged_attention_scratch_bytes(d.seqs, d.q_heads, d.k_heads, d.D, most);
     if (need) {
         if (!scratch) return NQ_ERR_NULL;

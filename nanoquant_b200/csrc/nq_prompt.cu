@@ -12,10 +12,19 @@
 //
 //   warp 0       queries, then keys and values in turn into a ring of stages, by TMA (128-byte swizzle), a box for each page of a cache
 //   warp 1       products: S into tensor memory, then P (from tensor memory, over its S) times V into O, also there
-//   warp 2       values behind a sequence's last token are set to zero in shared memory: their weights are zero, which a NaN would survive
+//   warp 2       values that no query of the block sees, ahead of a window or behind the last token, are set to zero in shared memory: their weights are
+//                zero, which a NaN would survive
+//   warp 3       which block is next: the CTAs that fit the SMs take the grid's other blocks over one by one (cluster launch control), so that long and short
+//                blocks fill the SMs evenly; asked for three steps ahead of a block's end (at its start, the first CTAs took blocks that other SMs were about
+//                to start: 143 us instead of 118 for four pieces of 512 tokens behind up to 16384)
 //   warps 4-11   softmax, four warps to a tile, a row to a thread; the next S of a tile is ordered behind its P V, the other tile's products run meanwhile
 //
-// The maximum m is moved, and O multiplied accordingly, only when it grows by more than 2^8: P and its sum have room for that, and the result does not depend on m.
+// The maximum m is moved, and O multiplied accordingly, only when it grows by more than 2^8: P and its sum have room for that, and the result does not depend on
+// m.  Where no row of a warp has a mask in a step, its weights are formed with m as it is, without looking for the step's maximum, and only done again when their sum
+// says that it has been left behind by more than 2^12 (half of the instructions of a step).  Results leave through shared memory, 128 bytes of a row at a time.
+//
+// Few tokens behind many keys are too few blocks for the SMs: a block's steps are then divided among up to 16 CTAs, whose sums a second launch joins.
+//
 // The weights P are rounded to the operands' 16-bit type for the product with the values (what the tensor cores take): 2^-9 (bf16) or 2^-12 (fp16) of each, not
 // enlarged by the average over tokens.
 #include <type_traits>
@@ -77,6 +86,7 @@ template <int DP>
 struct PromptWork : PromptBlock {
     int behind, k_first;           // (the first key: at the start of a page, or of a step)
     int steps[PromptShape<DP>::kTiles], most;
+    int front_rows;                // of the first step, ahead of what any query of the block sees
     int tail_rows;                 // of the last step, that the sequence has
     __device__ __forceinline__ int sees_end(const PromptParams& P, int t) const { return max(0, P.d.causal ? min(k_len, t + behind + 1) : k_len); }
     __device__ __forceinline__ int sees_begin(const PromptParams& P, int t) const { return P.d.window > 0 ? max(0, t + behind + 1 - P.d.window) : 0; }
@@ -88,6 +98,7 @@ struct PromptWork : PromptBlock {
     __device__ __forceinline__ void divide(const PromptParams& P) {
         behind = k_len - q_len;
         k_first = sees_begin(P, first) & ~(P.piece - 1);
+        front_rows = sees_begin(P, first) - k_first;
         most = 0;
 #pragma unroll
         for (int i = 0; i < PromptShape<DP>::kTiles; ++i) {
@@ -102,6 +113,7 @@ struct PromptWork : PromptBlock {
             if (part >= parts) have = 0;
             most = have > 0 ? min(most - from, size) : 0;
             k_first += from * PromptShape<DP>::kKeys;
+            if (part > 0) front_rows = 0;
 #pragma unroll
             for (int i = 0; i < PromptShape<DP>::kTiles; ++i) steps[i] = min(max(steps[i] - from, 0), most);
         } else if (part > 0) {
@@ -112,7 +124,7 @@ struct PromptWork : PromptBlock {
         }
         tail_rows = k_len - k_first - (most - 1) * PromptShape<DP>::kKeys;
     }
-    __device__ __forceinline__ bool fix() const { return most > 0 && tail_rows < PromptShape<DP>::kKeys; }
+    __device__ __forceinline__ bool fix(int j) const { return (j == 0 && front_rows > 0) || (j == most - 1 && tail_rows < PromptShape<DP>::kKeys); }
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -217,8 +229,9 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto bar_full = [&](int s) { return sbase + 8 * s; };
     auto bar_free = [&](int s) { return sbase + 8 * (kStages + s); };
-    const uint32_t bars = sbase + 16 * kStages;
-    const uint32_t bar_q = bars, bar_q_free = bars + 8, bar_tail = bars + 16, bar_answer = bars + 24;
+    auto bar_fix = [&](int s) { return sbase + 8 * (2 * kStages + s); };      // values are there, some of which are to become zeros
+    const uint32_t bars = sbase + 24 * kStages;
+    const uint32_t bar_q = bars, bar_q_free = bars + 8, bar_answer = bars + 24;
     auto bar_s = [&](int i) { return bars + 32 + 8 * i; };            // S is there (by tile, or with one tile by buffer)
     auto bar_p = [&](int i) { return bars + 48 + 8 * i; };            // P is there, or the first of it
     auto bar_h = [&](int i) { return bars + 64 + 8 * i; };            // the rest of P is there (two tiles)
@@ -226,19 +239,20 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     auto bar_info = [&](int i) { return bars + 96 + 8 * i; };         // the number and sequence of a block are there
     auto bar_info_free = [&](int i) { return bars + 112 + 8 * i; };
     const uint32_t bar_ask = bars + 128;                              // a block is nearly done
-    static_assert(16 * kStages + 136 <= 272, "shared memory map");
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 272);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 276);
-    volatile int* bad_block = reinterpret_cast<volatile int*>(smem + 280);          // four: the block (counted from 1) that last had a page outside the cache
-    const uint32_t answer = sbase + 304;
-    volatile PromptBlock* info = reinterpret_cast<volatile PromptBlock*>(smem + 320);
-    static_assert(320 + 2 * sizeof(PromptBlock) <= 1024, "shared memory map");
+    static_assert(24 * kStages + 136 <= 336, "shared memory map");
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 336);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 340);
+    volatile int* bad_block = reinterpret_cast<volatile int*>(smem + 344);          // four: the block (counted from 1) that last had a page outside the cache
+    const uint32_t answer = sbase + 368;
+    volatile PromptBlock* info = reinterpret_cast<volatile PromptBlock*>(smem + 384);
+    static_assert(384 + 2 * sizeof(PromptBlock) <= 1024, "shared memory map");
 
     const int block_tokens = kTiles * P.tokens;
     if (warp == 2) {
         if (lane < kStages) {
             mbar_init(bar_full(lane), 1);
             mbar_init(bar_free(lane), 1);
+            mbar_init(bar_fix(lane), 1);
         }
         if (lane < 2) {
             mbar_init(bar_s(lane), 1);
@@ -252,7 +266,6 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
         if (lane == 0) {
             mbar_init(bar_q, 1);
             mbar_init(bar_q_free, 1);
-            mbar_init(bar_tail, 1);
             mbar_init(bar_answer, 1);
             mbar_init(bar_ask, 1);
             *abort_flag = 0;
@@ -346,7 +359,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     for (int kv = 0; kv < 2 && ok; ++kv) {
                         ok = mbar_wait_warp(bar_free(s), ph ^ 1, abort_flag, P.status, P.wait_limit);
                         if (!ok) break;
-                        const uint32_t bar = kv == 1 && B.fix() && j == B.most - 1 ? bar_tail : bar_full(s);
+                        const uint32_t bar = kv == 1 && B.fix(j) ? bar_fix(s) : bar_full(s);
                         if (lane == 0) mbar_expect_tx(bar, (uint32_t)(boxes * P.piece * 128 * Sh::kColumns));
                         __syncwarp();
                         if (lane < boxes) {
@@ -470,23 +483,31 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             }
             __syncwarp();
         } else {
-            // ------------------------------------------------------------ values behind the last token
-            int at = 0, fixes = 0;
-            for (int n = 0; next_info(n); ++n) {
-                const int last = at + 2 * B.most - 1;
-                at += 2 * B.most;
-                if (!B.fix()) continue;
-                if (!mbar_wait_warp(bar_tail, (uint32_t)fixes & 1u, abort_flag, P.status, P.wait_limit)) break;
-                ++fixes;
-                unsigned char* to = smem + Sh::kRingOff + (last % kStages) * Sh::kStageBytes;
-                const int left = (kKeys - B.tail_rows) * 8;               // 16-byte units of a column
-                for (int i = lane; i < left * Sh::kColumns; i += 32) {
-                    const int c = i / left;
-                    *reinterpret_cast<uint4*>(to + c * kKeys * 128 + B.tail_rows * 128 + (i - c * left) * 16) = make_uint4(0, 0, 0, 0);
+            // ------------------------------------------------------------ values that no query of a block sees
+            int at = 0;
+            uint32_t phases = 0;                   // of the stages' barriers, a bit each
+            bool ok = true;
+            for (int n = 0; ok && next_info(n); ++n) {
+                for (int j = 0; j < B.most && ok; j = j == 0 && B.most > 1 ? B.most - 1 : B.most) {
+                    if (!B.fix(j)) continue;
+                    const int s = (at + 2 * j + 1) % kStages;
+                    ok = mbar_wait_warp(bar_fix(s), phases >> s & 1u, abort_flag, P.status, P.wait_limit);
+                    if (!ok) break;
+                    phases ^= 1u << s;
+                    unsigned char* to = smem + Sh::kRingOff + s * Sh::kStageBytes;
+                    auto clear = [&](int row, int rows) {
+                        for (int i = lane; i < 8 * rows * Sh::kColumns; i += 32) {           // 16 bytes each
+                            const int c = i / (8 * rows);
+                            *reinterpret_cast<uint4*>(to + c * kKeys * 128 + row * 128 + (i - c * 8 * rows) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    };
+                    if (j == 0) clear(0, B.front_rows);
+                    if (j == B.most - 1 && B.tail_rows < kKeys) clear(B.tail_rows, kKeys - B.tail_rows);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_full(s));
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_full(last % kStages));
+                at += 2 * B.most;
             }
         }
     } else {

@@ -235,3 +235,25 @@ def test_refusals():
     k.requires_grad_()
     with pytest.raises(RuntimeError, match="no gradient"):
         ops.prompt_attention(q, k, v, cu)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,total,page,window", [
+    ([3, 1, 20], [300, 77, 500], 16, 70), ([5], [131], 128, 40), ([2, 300], [1000, 900], 1024, 100), ([1], [4001], 64, 3500), ([1, 2, 1, 1], [130, 131, 200, 90], 8, 3)])
+def test_what_no_query_sees_has_no_influence(new, total, page, window, D):
+    """Tokens ahead of the first query's window that were never stored, in pages that do not exist or that it shares with others: keys NaN, values NaN or infinite."""
+    from nanoquant_b200 import ops
+
+    q, k, v, kc, vc, table, n = piece(new, total, 4, 2, D, page, torch.bfloat16)
+    want = expected(q, k, v, new, window=window)
+    for s, (m, t) in enumerate(zip(new, total)):
+        unseen = max(0, t - m + 1 - window)
+        for i in range(unseen):
+            p = table[s, i // page].item()
+            kc[p, i % page], vc[p, i % page] = float("nan"), float("inf") if i % 2 else float("nan")
+        table[s, :unseen // page] = -1
+    check_attention(ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, window=window), want)
+    for x, y, m, t in zip(k, v, new, total):
+        x[:max(0, t - m + 1 - window)], y[:max(0, t - m + 1 - window)] = float("nan"), float("nan")
+    check_attention(ops.prompt_attention(q, torch.cat(k), torch.cat(v), starts(new), starts(total), window=window), want)
+
