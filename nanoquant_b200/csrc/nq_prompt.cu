@@ -818,14 +818,17 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant_
     }
 }
 
-// Parts of a block's steps.  Blocks are dealt out as CTAs become free, so that there should be at least two for every SM; a part has eight steps at least (of a prompt
-// over itself, whose blocks see half of it: counted twice), for its sums pass through memory.
+// Parts of a block's steps.  Blocks are dealt out as CTAs become free, so that a few for every SM are enough: below 1.5 of them (`blocks` counts a block to each
+// sequence more than there may be) they are cut to make two.  128 tokens behind 2048, eight times, 32 heads on 8 of 128 (192 blocks): 32 us cut and 37 whole; 8192 tokens
+// over themselves, 8 heads on 1 (257): 140 and 115; 512 behind up to 4096, four times (288): 116 both.  A part has eight steps at least, for its sums pass through
+// memory (16 tokens behind 16384: 26 us, and with sixteen steps 36; 128 behind 2048: with four 36); of a prompt over itself, whose blocks see half of it, sixteen
+// (2048 tokens: 40 us, with eight 63).  Sixteen parts at most (16 tokens behind 131072: 109 us, up to ten parts 164, up to 32 176).
 template <int DP>
 static int prompt_splits(const nq_attention_desc& d, int tokens) {
     using Sh = PromptShape<DP>;
     const int64_t block = (int64_t)Sh::kTiles * tokens, blocks = ((d.T + block - 1) / block + d.seqs) * d.k_heads;
     const int64_t keys = d.block_table ? (int64_t)d.max_pages * d.page_size : d.Tk, steps = keys / Sh::kKeys, wanted = 2 * (int64_t)sm_count();
-    int64_t n = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
+    int64_t n = 4 * blocks >= 3 * wanted ? 1 : (wanted + blocks - 1) / blocks;
     const int64_t most = steps / (d.block_table || d.cu_seqlens_k ? 8 : 16);
     n = n < most ? n : most;
     return (int)(n < 1 ? 1 : n > kPromptParts ? kPromptParts : n);
