@@ -28,8 +28,8 @@
 namespace nq {
 
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
+constexpr int kPagedWhole = 1024;               // tokens of a sequence that a single CTA takes at most
 constexpr int kPagedRows = 16;                  // query heads of an item at most
-constexpr int kPagedWhole = 256;                // caches of up to so many tokens a sequence: a CTA per item
 
 struct alignas(64) PagedParams {
     CUtensorMap map_k, map_v;
@@ -671,6 +671,11 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_consta
     }
 }
 
+// Whether the table has room for short sequences only: a CTA per item and one launch instead of two, but nothing evens out the lengths.  Heads of 128, 32 on 8, all
+// sequences of one length, us whole and split: 1 x 100 tokens 5.0 and 7.3; 1 x 250 7.1 and 7.5; 1 x 500 10.8 and 7.9; 16 x 500 10.8 and 14.4; 16 x 1000 17.8 and 17.3;
+// 32 x 1000 25.2 and 31.2; 128 x 1000 89.5 and 98; 16 x 2000 33 and 30; 64 x 2000 100 and 97.
+static bool paged_whole(int64_t items, int64_t most) { return most <= 256 || (most <= kPagedWhole && 8 * items >= most); }
+static int64_t paged_items(int64_t seqs, int q_heads, int k_heads) { return seqs * k_heads * ((q_heads / k_heads + kPagedRows - 1) / kPagedRows); }
 static int padded_columns(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int paged_ctas(int dp) { return sm_count() * (dp == 64 ? PagedShape<64>::kCtasPerSm : dp == 128 ? PagedShape<128>::kCtasPerSm : PagedShape<256>::kCtasPerSm); }
 
@@ -697,9 +702,10 @@ static int paged_launch(PagedParams& P, bool whole, int64_t most_steps, cudaStre
     void* args[] = {&P};
     const int st = launch_dependent(cfg, attr, 0, whole ? whole_fn : split_fn, args);
     if (st != NQ_OK || whole) return st;
-    // a CTA for each head while that makes no more of them than the SMs take at once; more threads where an item has many pieces
+    // A CTA for each head while that makes no more of them than the SMs take at once; more threads where an item has many pieces (sequences of 1000 tokens, 32 heads on 8:
+    // one of them 8.7 us, with 128 threads 10.8; sixteen 17.4 with 128 and 21.8 with 512).
     const int joins = P.items < P.warps ? P.items : P.warps, rows = P.rows < kPagedRows ? P.rows : kPagedRows;
-    const bool many = (int64_t)P.items * 8 <= P.warps;
+    const bool many = (int64_t)P.items * 32 <= P.warps;
     cfg.gridDim = dim3((unsigned)joins, (unsigned)((int64_t)joins * rows <= 8 * sm_count() ? rows : 1));
     cfg.blockDim = dim3(many ? 512 : 128);
     cfg.dynamicSmemBytes = P.warps * sizeof(float);
@@ -731,7 +737,7 @@ extern "C" {
 
 size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int D, int64_t max_tokens) {
     using namespace nq;
-    if (seqs <= 0 || q_heads <= 0 || k_heads <= 0 || D <= 0 || D > kHeadMaxCols || max_tokens <= kPagedWhole) return 0;
+    if (seqs <= 0 || q_heads <= 0 || k_heads <= 0 || D <= 0 || D > kHeadMaxCols || paged_whole(paged_items(seqs, q_heads, k_heads), max_tokens)) return 0;
     const int dp = padded_columns(D);
     return (size_t)paged_ctas(dp) * kPagedWarps * 2 * kPagedRows * (dp + 2) * sizeof(float);
 }
@@ -753,7 +759,7 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     P.status = static_cast<unsigned*>(status_word) + 2;
     P.part = static_cast<float*>(scratch);
     P.chunks = (P.rows + kPagedRows - 1) / kPagedRows;
-    const int64_t most = (int64_t)d.max_pages * d.page_size, items = (int64_t)d.seqs * d.k_heads * P.chunks;
+    const int64_t most = (int64_t)d.max_pages * d.page_size, items = paged_items(d.seqs, d.q_heads, d.k_heads);
     if (most > 0x3fffffff || items > 0x3fffffff) return NQ_ERR_TOO_LARGE;
     const size_t need = nq_paged_attention_scratch_bytes(d.seqs, d.q_heads, d.k_heads, d.D, most);
     if (need) {

@@ -35,6 +35,18 @@ def test_against_definition(lengths, H, K, D, page, window, dtype):
     assert torch.equal(got, ops.paged_attention(q, kc, vc, table, n, window=window))          # the same order of sums
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page,width", [(8, 128), (16, 64), (512, 2), (1024, 1), (8, 129), (16, 65)])
+def test_many_sequences_of_middling_length(page, width, D):
+    """Tables of 1024 tokens for 128 key heads in all, which one launch takes, and of more, which two do."""
+    from nanoquant_b200 import ops
+
+    lengths = [1, 1024, 0, 513, 300, 1000, 16, 777] * 8
+    q, k, v, kc, vc, table, n = make(lengths, 4, 2, D, page, torch.bfloat16, width=width)
+    check_attention(ops.paged_attention(q, kc, vc, table, n), expected(q, k, v, None))
+    check_attention(ops.paged_attention(q, kc, vc, table, n, window=301), expected(q, k, v, 301))
+
+
 @pytest.mark.parametrize("width", [None, 400])
 def test_order_of_the_cache_and_width_of_the_table(width):
     """Heads outside the tokens of a page, keys and values in one tensor, rows of the table apart, a table far wider than the sequences: the same numbers within the bound (a wide
