@@ -6,16 +6,18 @@
 // mma.sync.m16n8k16 (up to 16; the instruction's rate is far above what memory delivers, and few rows would leave tcgen05's 128 idle).
 //
 // Work.  The tokens that a sequence's query sees are cut into steps of 16 (heads of up to 64 columns: 32).  An item is a sequence, a key head and up to
-// 16 of its query heads; the steps of all items lie one behind the other, and every warp takes the same number of them, found from the lengths on the
-// device: batches of any lengths fill the SMs evenly, and a captured graph follows the lengths.  A warp has a ring of steps of its own in shared memory
-// (TMA boxes of a page's tokens x 64 columns; it runs on into the next item), its own running maximum, sum and accumulators: nothing in the loop waits
-// for another warp.  (Copied by cp.async, 16 bytes a lane, the same steps were as fast when full, 150 us against 153 for 4 sequences of up to 131072
-// tokens, but 650 instructions each where these have 400; bulk copies of 256-byte rows took 206 us.)  An item that lies in several warps leaves fp32
-// results (m, sum, unnormalised o) in the scratch, which a second, overlapped launch joins in their order.  Caches without room for long sequences take
-// a CTA per item, its steps divided among the four warps and their results joined through shared memory: one launch.
+// 16 of its query heads.  The steps of all sequences lie one behind the other; a group of warps, one for each key head, takes the same number of them as
+// every other group, found from the lengths on the device: batches of any lengths fill the SMs evenly, and a captured graph follows the lengths.  (What
+// the heads of a token have in the cache lies side by side and is read at the same time; with one head's steps after the other's, 32 heads on 8 of 64
+// columns ran at 5.8 TB/s instead of 6.4 to 6.7, and 64 on 8 of 128 at 6.4 instead of 6.7.)  A warp has a ring of steps of its own in shared memory (TMA
+// boxes of a page's tokens x 64 columns; it runs on into the next sequence), its own running maximum, sum and accumulators: nothing in the loop waits
+// for another warp.  (Copied by cp.async, 16 bytes a lane, the same steps were as fast, but of 650 instructions each; bulk copies of 256-byte rows took
+// 206 us where these take 153.)  An item that lies in several groups leaves fp32 results (m, sum, unnormalised o) in the scratch, which a second,
+// overlapped launch joins in their order.  Where the table has room for short sequences only, a CTA takes an item, its steps divided among the four warps
+// and their results joined through shared memory: one launch.
 //
-// Measured: 32 sequences of up to 4096 tokens, 32 heads of 128, fp16: 106 us, 5.97 TB/s; 4 of up to 131072, 64 heads on 8, bf16: 153 us, 5.96 TB/s, of
-// which 12 us are start, join and the uneven end (each further token: 6.7 TB/s, a plain copy's rate); one of 1000, 32 heads on 8: 8.3 us, two launches.
+// Measured: 32 sequences of up to 4096 tokens, 32 heads of 128, fp16: 105 us, 6.05 TB/s; 4 of up to 131072, 64 heads on 8, bf16: 151 us, 6.03 TB/s, of
+// which some 10 us are start, join and the uneven end (each further token: 6.9 TB/s); one of 1000, 32 heads on 8: 8.5 us, two launches.
 //
 // The weights p are rounded to the operands' type for the product with the values: 2^-9 (bf16) or 2^-12 (fp16) of each, which the average over
 // tokens does not enlarge.  Sums of p are fp32 sums of the rounded values.
@@ -37,12 +39,13 @@ struct alignas(64) PagedParams {
     int shift;                                  // log2(page_size)
     int step, box;                              // tokens of a step, and of a box of it (a page's at most)
     int rows, chunks;                           // query heads to a key head; items of 16 of them
-    int warps;                                  // of the split kernel
+    int groups;                                 // of the split kernel: a warp for each key head and 16 of its query heads (`per_seq` of them)
+    int piece;                                  // floats of an item's result
     int items;                                  // (of all sequences)
     float factor;                               // scale log2(e)
     unsigned wait_limit;
     unsigned* status;
-    float* part;                                // [warps][2][16][DP + 2]
+    float* part;                                // [groups][per_seq][2][query heads of an item][DP + 2]
 };
 
 // Steps of a sequence's items, and what they cover.
@@ -91,16 +94,15 @@ __device__ __forceinline__ long long block_scan(long long v, long long* warp_sum
     }
     return v;
 }
-// Steps of all items, and a warp's share of them.  By the whole CTA.  n, sum and range: of this thread's sequence, for batches of up to as many.
+// Steps of all sequences.  By the whole CTA.  n, sum and range: of this thread's sequence, for batches of up to as many.
 __device__ __forceinline__ long long paged_total(const PagedParams& P, PagedPlan& plan, long long& n, long long& sum, PagedRange& range) {
-    const int per_seq = P.d.k_heads * P.chunks;
     long long total = 0;
     for (int s0 = 0; s0 < P.d.seqs; s0 += blockDim.x) {
         const int s = s0 + threadIdx.x;
         n = 0;
         if (s < P.d.seqs) {
             range = paged_range(P, s);
-            n = (long long)range.steps * per_seq;
+            n = range.steps;
         }
         long long some;
         sum = block_scan(n, plan.sums, some) + total;
@@ -111,7 +113,6 @@ __device__ __forceinline__ long long paged_total(const PagedParams& P, PagedPlan
 // The sequences that the steps unit(0) .. unit(COUNT - 1) lie in (those that are below the total).
 template <int COUNT, class Unit>
 __device__ __forceinline__ void paged_find(const PagedParams& P, PagedPlan& plan, long long n, long long sum, PagedRange range, Unit unit) {
-    const int per_seq = P.d.k_heads * P.chunks;
     auto look = [&](int s) {
 #pragma unroll
         for (int w = 0; w < COUNT; ++w)
@@ -126,7 +127,7 @@ __device__ __forceinline__ void paged_find(const PagedParams& P, PagedPlan& plan
             n = 0;
             if (s < P.d.seqs) {
                 range = paged_range(P, s);
-                n = (long long)range.steps * per_seq;
+                n = range.steps;
             }
             long long some;
             sum = block_scan(n, plan.sums, some) + before;
@@ -157,8 +158,8 @@ __device__ __forceinline__ void paged_box(uint32_t dst, const CUtensorMap* map, 
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
 }
 // A warp's step is bound by its own latency, so what counts is how many warps an SM has, each with one step on its way while it works on another:
-// three CTAs of rings of 2 (columns up to 128) moved 5.97 TB/s at 32 sequences of up to 4096 tokens and 32 heads of 128, two of rings of 3 moved
-// 5.8; with heads of 64, 8 x 131072 tokens, 5.8 TB/s instead of 5.5 (one CTA: 2.7).  Of 64 columns a step has 32 tokens: with 16 and four CTAs an SM, 5.55.
+// three CTAs of rings of 2 (columns up to 128) took 106 us for 32 sequences of up to 4096 tokens and 32 heads of 128, two of rings of 3 108.5; with heads of 64,
+// 8 x 131072 tokens, 369 us and 390 (one CTA: 783).  Of 64 columns a step has 32 tokens: with 16 and four CTAs an SM, 387.  (All before the heads were read side by side.)
 template <int DP> struct PagedShape {
     static constexpr int kColumns = DP / 64;                      // boxes of 64 columns: rows of 128 bytes, 128-byte swizzle
     static constexpr int kStep = DP == 64 ? 32 : 16;              // tokens of a step
@@ -394,7 +395,8 @@ struct PagedHeads {
     }
 };
 
-// Long caches: a warp has the steps [share W, share (W + 1)) of all items' steps.
+// Long caches: the warps of group g have the steps [share g, share (g + 1)) of all sequences' steps, each for its key head: what lies side by side in the cache is
+// read at the same time.
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) paged_split_kernel(const __grid_constant__ PagedParams P) {
     using S = PagedShape<DP>;
@@ -404,41 +406,28 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     const int warp = threadIdx.x >> 5;
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem + warp * S::kWarpBytes, bars = smem + S::kBarOff + 8 * warp * S::kStages;
     paged_rings<DP>(smem);
-    const int per_seq = d.k_heads * P.chunks, W = blockIdx.x * kPagedWarps + warp;
+    const int per_seq = d.k_heads * P.chunks, W = blockIdx.x * kPagedWarps + warp, group = W / per_seq, item = W - group * per_seq;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     long long n, sum;
     PagedRange range;
-    const long long total = paged_total(P, plan, n, sum, range), share = (total + P.warps - 1) / P.warps;
-    paged_find<kPagedWarps>(P, plan, n, sum, range, [&](int w) { return share * (blockIdx.x * kPagedWarps + w); });
-    const long long unit = share * W;
+    const long long total = paged_total(P, plan, n, sum, range), share = (total + P.groups - 1) / P.groups;
+    paged_find<kPagedWarps>(P, plan, n, sum, range, [&](int w) { return share * ((blockIdx.x * kPagedWarps + w) / per_seq); });
+    const long long unit = share * group;
     if (unit >= total) return;                  // (no barrier behind this)
     const int count = (int)min(share, total - unit);
 
+    const int kh = item / P.chunks, chunk = item - kh * P.chunks;
+    const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
     struct Cursor {
         PagedRange R;
-        int seq, item, s;                       // item of the sequence; the next step
-        int kh, chunk;                          // of the item
-    } load, at;
-    {
-        const PagedPlace& p = plan.place[warp];
-        load.R = p.range;
-        load.seq = p.seq;
-        load.item = (int)((unit - p.before) / load.R.steps);
-        load.s = (int)(unit - p.before - (long long)load.item * load.R.steps);
-        load.kh = load.item / P.chunks;
-        load.chunk = load.item - load.kh * P.chunks;
-    }
-    at = load;
-    auto advance = [&](Cursor& c) {             // (true: behind the last step of an item)
+        int seq, s;                             // the next step of the sequence
+    } load{plan.place[warp].range, plan.place[warp].seq, (int)(unit - plan.place[warp].before)}, at = load;
+    auto advance = [&](Cursor& c) {             // (true: behind the last step of a sequence)
         if (++c.s < c.R.steps) return false;
         c.s = 0;
-        if (++c.chunk == P.chunks) { c.chunk = 0; ++c.kh; }
-        if (++c.item == per_seq) {
-            c.item = c.kh = 0;
-            if (++c.seq < d.seqs) c.R = paged_range(P, c.seq);
-        }
+        if (++c.seq < d.seqs) c.R = paged_range(P, c.seq);
         return true;
     };
     PagedPages pages{};
@@ -450,7 +439,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
             if (!ok) bad_items |= 1u << (load_items & 31);
             fresh = false;
         }
-        paged_load<DP>(P, load.R, pages, load.kh, load.s, ring + stage * 2 * S::kTileBytes, bars + 8 * stage);
+        paged_load<DP>(P, load.R, pages, kh, load.s, ring + stage * 2 * S::kTileBytes, bars + 8 * stage);
         if (advance(load)) {
             fresh = true;
             ++load_items;
@@ -464,11 +453,9 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
     unsigned at_items = 0;
     uint32_t phase = 0;
     bool begin = true;                          // of an item, here
-    int from = at.s, h0 = 0, rows = 0;
+    int from = at.s;
     for (int i = 0, stage = 0; i < count; ++i) {
         if (begin) {
-            h0 = at.kh * P.rows + at.chunk * kPagedRows;
-            rows = min(kPagedRows, P.rows - at.chunk * kPagedRows);
             heads.start(d, at.seq, h0, rows);
             from = at.s;
             begin = false;
@@ -484,7 +471,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
         if (last || i + 1 == count) {
             heads.finish(seq_bad || (bad_items >> (at_items & 31) & 1u));
             if (from == 0 && last) heads.store(d, seq, h0, rows);
-            else heads.save(P.part + ((long long)W * 2 + (from == 0 ? 1 : 0)) * S::kPart, rows);
+            else heads.save(P.part + ((long long)W * 2 + (from == 0 ? 1 : 0)) * P.piece, rows);
             ++at_items;
             begin = true;
         }
@@ -569,12 +556,12 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_consta
     // (the lengths are older than the kernel above, which has waited for what wrote them before it let this one start)
     long long n, sum;
     PagedRange range;
-    const long long total = paged_total(P, plan, n, sum, range), share = (total + P.warps - 1) / P.warps;
-    int seq, item;
-    const bool by_item = P.items <= P.warps;
+    const long long total = paged_total(P, plan, n, sum, range), share = (total + P.groups - 1) / P.groups;
+    int seq;
+    const bool by_item = d.seqs <= P.groups;
+    const int number = blockIdx.x / per_seq, item = blockIdx.x - number * per_seq;       // of a sequence, or of a group
     if (by_item) {
-        seq = blockIdx.x / per_seq;
-        item = blockIdx.x - seq * per_seq;
+        seq = number;
         if (d.seqs <= THREADS) {
             if ((int)threadIdx.x == seq) plan.place[0] = {sum - n, seq, range};
         } else {
@@ -582,32 +569,31 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_consta
             for (int s0 = 0; s0 < seq; s0 += THREADS) {
                 const int s = s0 + threadIdx.x;
                 long long some;
-                block_scan(s < seq ? (long long)paged_range(P, s).steps * per_seq : 0, plan.sums, some);
+                block_scan(s < seq ? (long long)paged_range(P, s).steps : 0, plan.sums, some);
                 before += some;
             }
             if (threadIdx.x == 0) plan.place[0] = {before, seq, paged_range(P, seq)};
         }
         __syncthreads();
     } else {
-        paged_find<1>(P, plan, n, sum, range, [&](int) { return share * (blockIdx.x + 1) - 1; });
-        if (share * (blockIdx.x + 1) - 1 >= total) {      // (the warp has none, or not all, of its steps: nothing of an item behind it)
+        paged_find<1>(P, plan, n, sum, range, [&](int) { return share * (number + 1) - 1; });
+        if (share * (number + 1) - 1 >= total) {          // (the group has none, or not all, of its steps: nothing of an item behind it)
             asm volatile("griddepcontrol.wait;" ::: "memory");
             return;
         }
         seq = plan.place[0].seq;
-        item = (int)((share * (blockIdx.x + 1) - 1 - plan.place[0].before) / plan.place[0].range.steps);
     }
-    const long long begin = plan.place[0].before + (long long)item * plan.place[0].range.steps, end = begin + plan.place[0].range.steps;
+    const long long begin = plan.place[0].before, end = begin + plan.place[0].range.steps;
     const long long first = begin / share, last = (end - 1) / share;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (first == last || (!by_item && first != blockIdx.x)) return;
+    if (first == last || (!by_item && first != number)) return;
     const int count = (int)(last - first) + 1;
     const int kh = item / P.chunks, chunk = item - kh * P.chunks;
     const int h0 = kh * P.rows + chunk * kPagedRows, rows = min(kPagedRows, P.rows - chunk * kPagedRows);
     const int col = 2 * (threadIdx.x % kPairs), group = threadIdx.x / kPairs;
     for (int row = blockIdx.y; row < rows; row += gridDim.y) {
         // the first piece is its warp's second result, the others are their warps' first
-        auto piece = [&](int i) { return P.part + ((first + i) * 2 + (i == 0)) * S::kPart + row * S::kRow; };
+        auto piece = [&](int i) { return P.part + (((first + i) * per_seq + item) * 2 + (i == 0)) * P.piece + row * S::kRow; };
         auto numbers = [&](int k) { return k < count ? __ldcg(reinterpret_cast<const float2*>(piece(k) + DP)) : make_float2(-INFINITY, 0.f); };
         const float2 mine = numbers(threadIdx.x);
         float2 u[kAhead];
@@ -671,16 +657,22 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_consta
     }
 }
 
+static int padded_columns(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+static int paged_ctas(int dp) { return sm_count() * (dp == 64 ? PagedShape<64>::kCtasPerSm : dp == 128 ? PagedShape<128>::kCtasPerSm : PagedShape<256>::kCtasPerSm); }
+
 // Whether the table has room for short sequences only: a CTA per item and one launch instead of two, but nothing evens out the lengths.  Heads of 128, 32 on 8, all
 // sequences of one length, us whole and split: 1 x 100 tokens 5.0 and 7.3; 1 x 250 7.1 and 7.5; 1 x 500 10.8 and 7.9; 16 x 500 10.8 and 14.4; 16 x 1000 17.8 and 17.3;
 // 32 x 1000 25.2 and 31.2; 128 x 1000 89.5 and 98; 16 x 2000 33 and 30; 64 x 2000 100 and 97.
 static bool paged_whole(int64_t items, int64_t most) { return most <= 256 || (most <= kPagedWhole && 8 * items >= most); }
+// Groups of warps: as many as fit the SMs at once, or, of so many heads that this would leave warps over, four times as many.
+static int64_t paged_groups(int dp, int64_t per_seq) {
+    const int64_t warps = (int64_t)paged_ctas(dp) * kPagedWarps;
+    return 16 * per_seq <= warps ? warps / per_seq : (4 * warps + per_seq - 1) / per_seq;
+}
+static int paged_piece(int q_heads, int k_heads, int dp) { return std::min(q_heads / k_heads, kPagedRows) * (dp + 2); }
 static int64_t paged_items(int64_t seqs, int q_heads, int k_heads) { return seqs * k_heads * ((q_heads / k_heads + kPagedRows - 1) / kPagedRows); }
-static int padded_columns(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-static int paged_ctas(int dp) { return sm_count() * (dp == 64 ? PagedShape<64>::kCtasPerSm : dp == 128 ? PagedShape<128>::kCtasPerSm : PagedShape<256>::kCtasPerSm); }
-
 template <int DP, bool BF16>
-static int paged_launch(PagedParams& P, bool whole, int64_t most_steps, cudaStream_t stream) {
+static int paged_launch(PagedParams& P, bool whole, cudaStream_t stream) {
     static bool attr_set[64];
     int dev = 0;
     NQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -690,11 +682,9 @@ static int paged_launch(PagedParams& P, bool whole, int64_t most_steps, cudaStre
         NQ_CUDA_TRY(cudaFuncSetAttribute(whole_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DP>::kSmem));
         attr_set[dev & 63] = true;
     }
-    // (no more CTAs than the table has steps for: one sequence of 1000 tokens takes 126 of the 444)
-    const int ctas = (int)std::min<int64_t>(paged_ctas(DP), (most_steps + kPagedWarps - 1) / kPagedWarps);
-    P.warps = ctas * kPagedWarps;
+    const int per_seq = P.d.k_heads * P.chunks;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(whole ? P.items : ctas));
+    cfg.gridDim = dim3((unsigned)(whole ? P.items : (P.groups * per_seq + kPagedWarps - 1) / kPagedWarps));
     cfg.blockDim = dim3(kPagedThreads);
     cfg.dynamicSmemBytes = PagedShape<DP>::kSmem;
     cfg.stream = stream;
@@ -704,11 +694,11 @@ static int paged_launch(PagedParams& P, bool whole, int64_t most_steps, cudaStre
     if (st != NQ_OK || whole) return st;
     // A CTA for each head while that makes no more of them than the SMs take at once; more threads where an item has many pieces (sequences of 1000 tokens, 32 heads on 8:
     // one of them 8.7 us, with 128 threads 10.8; sixteen 17.4 with 128 and 21.8 with 512).
-    const int joins = P.items < P.warps ? P.items : P.warps, rows = P.rows < kPagedRows ? P.rows : kPagedRows;
-    const bool many = (int64_t)P.items * 32 <= P.warps;
+    const int joins = P.d.seqs <= P.groups ? P.items : P.groups * per_seq, rows = P.rows < kPagedRows ? P.rows : kPagedRows;
+    const bool many = (int64_t)P.d.seqs * 32 <= P.groups;
     cfg.gridDim = dim3((unsigned)joins, (unsigned)((int64_t)joins * rows <= 8 * sm_count() ? rows : 1));
     cfg.blockDim = dim3(many ? 512 : 128);
-    cfg.dynamicSmemBytes = P.warps * sizeof(float);
+    cfg.dynamicSmemBytes = P.groups * sizeof(float);
     return launch_dependent(cfg, attr, 0, many ? (const void*)paged_join_kernel<DP, BF16, 512> : (const void*)paged_join_kernel<DP, BF16, 128>, args);
 }
 
@@ -739,7 +729,8 @@ size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int 
     using namespace nq;
     if (seqs <= 0 || q_heads <= 0 || k_heads <= 0 || D <= 0 || D > kHeadMaxCols || paged_whole(paged_items(seqs, q_heads, k_heads), max_tokens)) return 0;
     const int dp = padded_columns(D);
-    return (size_t)paged_ctas(dp) * kPagedWarps * 2 * kPagedRows * (dp + 2) * sizeof(float);
+    const int64_t per_seq = paged_items(1, q_heads, k_heads);
+    return (size_t)(paged_groups(dp, per_seq) * per_seq) * 2 * paged_piece(q_heads, k_heads, dp) * sizeof(float);
 }
 
 int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t scratch_bytes, void* status_word, nq_stream_t stream) {
@@ -776,11 +767,14 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     st = mm_encode_heads(&P.map_k, d.k, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.k_slot, d.k_head, d.k_page}, {64, P.box, 1, 1});
     if (st == NQ_OK) st = mm_encode_heads(&P.map_v, d.v, type, {d.D, d.page_size, d.k_heads, d.pages}, {d.v_slot, d.v_head, d.v_page}, {64, P.box, 1, 1});
     if (st != NQ_OK) return st;
-    const int64_t most_steps = items * ((most + P.step - 1) / P.step);
-    switch (padded_columns(d.D)) {
-        case 64: return bf ? paged_launch<64, true>(P, whole, most_steps, as_stream(stream)) : paged_launch<64, false>(P, whole, most_steps, as_stream(stream));
-        case 128: return bf ? paged_launch<128, true>(P, whole, most_steps, as_stream(stream)) : paged_launch<128, false>(P, whole, most_steps, as_stream(stream));
-        default: return bf ? paged_launch<256, true>(P, whole, most_steps, as_stream(stream)) : paged_launch<256, false>(P, whole, most_steps, as_stream(stream));
+    // (no more groups than the table has steps for: one sequence of 1000 tokens takes 63 of the 222)
+    const int dp = padded_columns(d.D);
+    P.groups = (int)std::min<int64_t>(paged_groups(dp, (int64_t)d.k_heads * P.chunks), d.seqs * ((most + P.step - 1) / P.step));
+    P.piece = paged_piece(d.q_heads, d.k_heads, dp);
+    switch (dp) {
+        case 64: return bf ? paged_launch<64, true>(P, whole, as_stream(stream)) : paged_launch<64, false>(P, whole, as_stream(stream));
+        case 128: return bf ? paged_launch<128, true>(P, whole, as_stream(stream)) : paged_launch<128, false>(P, whole, as_stream(stream));
+        default: return bf ? paged_launch<256, true>(P, whole, as_stream(stream)) : paged_launch<256, false>(P, whole, as_stream(stream));
     }
 }
 
