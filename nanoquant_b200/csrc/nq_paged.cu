@@ -11,7 +11,7 @@
 // the heads of a token have in the cache lies side by side and is read at the same time; with one head's steps after the other's, 32 heads on 8 of 64
 // columns ran at 5.8 TB/s instead of 6.4 to 6.7, and 64 on 8 of 128 at 6.4 instead of 6.7.)  A warp has a ring of steps of its own in shared memory (TMA
 // boxes of a page's tokens x 64 columns; it runs on into the next sequence), its own running maximum, sum and accumulators: nothing in the loop waits
-// for another warp.  (Copied by cp.async, 16 bytes a lane, the same steps were as fast, but of 650 instructions each; bulk copies of 256-byte rows took
+// for another warp.  (Copied by cp.async, 16 bytes a lane, the same steps were as fast, but of 650 instructions each instead of 370; bulk copies of 256-byte rows took
 // 206 us where these take 153.)  An item that lies in several groups leaves fp32 results (m, sum, unnormalised o) in the scratch, which a second,
 // overlapped launch joins in their order.  Where the table has room for short sequences only, a CTA takes an item, its steps divided among the four warps
 // and their results joined through shared memory: one launch.
