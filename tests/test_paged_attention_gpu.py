@@ -47,6 +47,19 @@ def test_many_sequences_of_middling_length(page, width, D):
     check_attention(ops.paged_attention(q, kc, vc, table, n, window=301), expected(q, k, v, 301))
 
 
+@pytest.mark.parametrize("lengths,H,K,D,page,width", [
+    ([20, 0, 700] * 50, 32, 32, 64, 16, 130), ([1500, 3, 0, 900], 128, 128, 64, 16, None), ([300, 1, 64] * 20, 128, 128, 8, 16, 70), ([40, 1100, 7] * 45, 8, 4, 128, 32, 40),
+    ([5, 2000, 0, 130] * 120, 2, 1, 64, 64, 64), ([1200, 80], 60, 20, 256, 16, None), ([700], 300, 150, 8, 8, 200), ([2100, 9] * 3, 200, 5, 128, 64, None)])
+def test_more_sequences_or_heads_than_the_warps_take_at_once(lengths, H, K, D, page, width):
+    """Key heads by which the warps do not divide, more of them than get groups of their own, more sequences than groups."""
+    from nanoquant_b200 import ops
+
+    q, k, v, kc, vc, table, n = make(lengths, H, K, D, page, torch.bfloat16, width=width)
+    got = ops.paged_attention(q, kc, vc, table, n)
+    check_attention(got, expected(q, k, v))
+    assert torch.equal(got, ops.paged_attention(q, kc, vc, table, n))
+
+
 @pytest.mark.parametrize("width", [None, 400])
 def test_order_of_the_cache_and_width_of_the_table(width):
     """Heads outside the tokens of a page, keys and values in one tensor, rows of the table apart, a table far wider than the sequences: the same numbers within the bound (a wide
