@@ -451,8 +451,8 @@ int nq_heads_fwd(const nq_heads_desc* desc_host, nq_stream_t stream);
 
 /* Attention: o = sum_j p_j v_j with p = softmax(scale q . k_j) over the tokens j that a query sees, heads q_heads / k_heads of which share a key head.
  * The query at place r of its sequence sees the tokens r - window < j <= r (window 0: no limit; without `causal` all of the sequence's j > r - window).
- * A query that sees nothing gives zeros.  What lies outside its sequence (rows of other sequences, slots behind the last token) does not enter, whatever it
- * holds.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type.
+ * A query that sees nothing gives zeros.  What no query of a sequence sees (rows of other sequences, slots behind the last token or ahead of every window)
+ * does not enter, whatever it holds; of prompts, an infinite or NaN value that some query sees may make NaN of those that do not.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type.
  * A sequence that the table or the cache does not hold (a page outside the cache, a length beyond the table) is NaN in all its outputs.
  *
  * nq_paged_attention_fwd: one query per sequence, q [seqs, q_heads, D], at place lengths[s] - 1 of the `lengths[s]` tokens in the cache (0 or
@@ -461,8 +461,8 @@ int nq_heads_fwd(const nq_heads_desc* desc_host, nq_stream_t stream);
  * of them).  Rows of no sequence are zeros.  Keys and values are packed likewise (k, v [Tk, k_heads, D] by cu_seqlens_k, NULL: cu_seqlens), or those in
  * the cache, `lengths[s]` per sequence (block_table not NULL; k and v are then the cache).  The last row of a sequence is at the place of its last
  * key: rows before the first key see nothing.
- * `status_word` as in nq_onebit_gemm_fwd.  scratch: ..._scratch_bytes() (0 where none is needed, or for a refused description), any contents, 16-byte aligned.  The order of sums depends on the sizes and
- * the lengths alone.  Strides, alignment, pages and block_table as in nq_heads_desc; out dense.
+ * max_pages x page_size: up to 2^30 tokens.  `status_word` as in nq_onebit_gemm_fwd.  scratch: ..._scratch_bytes() (0 where none is needed, or for a
+ * refused description), any contents, 16-byte aligned.  The order of sums depends on the sizes and the lengths alone.  Strides, alignment, pages and block_table as in nq_heads_desc; out dense.
  * replaces: the attention of the HF model forward between the quantised projections (src/nanoquant/kernel/test_decode.py:385-422). */
 typedef struct {
     const void *q, *k, *v;

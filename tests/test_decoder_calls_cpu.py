@@ -94,3 +94,11 @@ def test_prompt_attention_refusals():
     assert call(long) == _lib.NQ_ERR_NULL and call(long, P, P + 4, need) == _lib.NQ_ERR_ALIGN and call(long, P, P, need - 1) == _lib.NQ_ERR_SCRATCH
     for kw in (dict(T=100000), dict(T=100), dict(T=1, seqs=1000), dict(q_heads=64, k_heads=64, D=256), dict(q_heads=128, k_heads=1)):
         assert size(max_pages=1 << 16, **kw) < 1 << 28, kw         # whatever the sizes
+
+
+def test_sequences_in_a_cache_have_up_to_two_to_the_30_tokens():
+    """Windows are cut to that, and so are the tables that a window could be too short for."""
+    L = _lib.lib()
+    d = _lib.AttentionDesc(**{**PAGED, "max_pages": 1 << 26, "table_stride": 1 << 26})
+    assert L.nq_paged_attention_fwd(ctypes.byref(d), P, 1 << 40, P, None) == _lib.NQ_ERR_TOO_LARGE
+    assert L.nq_prompt_attention_fwd(ctypes.byref(d), P, 1 << 40, P, None) == _lib.NQ_ERR_TOO_LARGE
