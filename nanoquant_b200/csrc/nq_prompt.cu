@@ -611,8 +611,12 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                 }
                 const bool fine = total() < 4096.f && peaks(kChunks - 1) * P.factor < m + 12.f;
                 done = __all_sync(0xffffffffu, fine || !live);
-                if (done) finish(base2);
-                else sum2[0] = sum2[1] = 0;
+                if (done) {
+                    finish(base2);
+                } else {                           // (the same columns are stored once more: nothing else orders two stores to tensor memory)
+                    sum2[0] = sum2[1] = 0;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
             }
             if (!done) {
                 float peak = -INFINITY;

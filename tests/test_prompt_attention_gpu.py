@@ -257,3 +257,27 @@ def test_what_no_query_sees_has_no_influence(new, total, page, window, D):
         x[:max(0, t - m + 1 - window)], y[:max(0, t - m + 1 - window)] = float("nan"), float("nan")
     check_attention(ops.prompt_attention(q, torch.cat(k), torch.cat(v), starts(new), starts(total), window=window), want)
 
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("where", ["step", "last"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_maximum_left_behind_in_a_step_without_masks(D, where, dtype):
+    """Scores that rise by 2^16 with every step of keys, or in a step's last 32 keys: weights that were formed with the maximum before are formed, and stored, once more."""
+    from nanoquant_b200 import ops
+
+    n, step = 520, 128 if D <= 128 else 64
+    q, k, v = (rand(i, n, 2, D, scale=s).to(dtype) for i, s in ((0, 0.1), (1, 1.0), (2, 1.0)))
+    at = torch.arange(n, device="cuda")
+    q[..., 0] = 16.0
+    k[..., 0] = (at // step + (at % step >= step - 32) * (where == "last"))[:, None].to(dtype)
+    scale = 0.69314718                                            # 16 powers of two a step, 2^7.2 at most: natural exponents below 2^6.7
+    o, avg, all_v = expected(q, [k], [v], [n], scale=scale)
+    # (as check_attention has it, with scores of up to 2^6.7: up to 16 products of 16 columns, each cut off at 2^-23 of them, are 2^-12.3 of a weight, and as much of the sum)
+    u = torch.finfo(dtype).eps / 2
+    for causal in (True, False):
+        want = (o, avg, all_v) if causal else expected(q, [k], [v], [n], scale=scale, causal=False)
+        got = ops.prompt_attention(q, k, v, starts([n]), causal=causal, scale=scale)
+        bound = u * want[0].abs() + (2 * u + 2.0 ** -11) * want[1] + (2.0 ** -25 if dtype == torch.float16 else 0.0) * (1 + want[2])
+        assert ((got.double() - want[0]).abs() <= bound * (1 + 2.0 ** -8)).all()
+        assert torch.equal(got, ops.prompt_attention(q, k, v, starts([n]), causal=causal, scale=scale))
