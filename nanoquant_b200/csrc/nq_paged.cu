@@ -671,6 +671,11 @@ static int64_t paged_groups(int dp, int64_t per_seq) {
 }
 static int paged_piece(int q_heads, int k_heads, int dp) { return std::min(q_heads / k_heads, kPagedRows) * (dp + 2); }
 static int64_t paged_items(int64_t seqs, int q_heads, int k_heads) { return seqs * k_heads * ((q_heads / k_heads + kPagedRows - 1) / kPagedRows); }
+// What paged_groups and the like can count: the sizes of every description that is taken.
+static bool paged_sizes_ok(int seqs, int q_heads, int k_heads, int D, int64_t max_tokens) {
+    return seqs > 0 && q_heads > 0 && k_heads > 0 && q_heads % k_heads == 0 && q_heads <= 1 << 16 && D > 0 && D % 8 == 0 && D <= kHeadMaxCols && max_tokens > 0 && max_tokens <= 0x3fffffff &&
+           paged_items(seqs, q_heads, k_heads) <= 0x3fffffff;
+}
 template <int DP, bool BF16>
 static int paged_launch(PagedParams& P, bool whole, cudaStream_t stream) {
     static bool attr_set[64];
@@ -727,7 +732,7 @@ extern "C" {
 
 size_t nq_paged_attention_scratch_bytes(int seqs, int q_heads, int k_heads, int D, int64_t max_tokens) {
     using namespace nq;
-    if (seqs <= 0 || q_heads <= 0 || k_heads <= 0 || D <= 0 || D > kHeadMaxCols || paged_whole(paged_items(seqs, q_heads, k_heads), max_tokens)) return 0;
+    if (!paged_sizes_ok(seqs, q_heads, k_heads, D, max_tokens) || paged_whole(paged_items(seqs, q_heads, k_heads), max_tokens)) return 0;
     const int dp = padded_columns(D);
     const int64_t per_seq = paged_items(1, q_heads, k_heads);
     return (size_t)(paged_groups(dp, per_seq) * per_seq) * 2 * paged_piece(q_heads, k_heads, dp) * sizeof(float);
@@ -751,7 +756,7 @@ int nq_paged_attention_fwd(const nq_attention_desc* desc, void* scratch, size_t 
     P.part = static_cast<float*>(scratch);
     P.chunks = (P.rows + kPagedRows - 1) / kPagedRows;
     const int64_t most = (int64_t)d.max_pages * d.page_size, items = paged_items(d.seqs, d.q_heads, d.k_heads);
-    if (most > 0x3fffffff || items > 0x3fffffff) return NQ_ERR_TOO_LARGE;
+    if (!paged_sizes_ok(d.seqs, d.q_heads, d.k_heads, d.D, most)) return NQ_ERR_TOO_LARGE;      // (what else it asks for has been checked)
     const size_t need = nq_paged_attention_scratch_bytes(d.seqs, d.q_heads, d.k_heads, d.D, most);
     if (need) {
         if (!scratch) return NQ_ERR_NULL;

@@ -2,6 +2,8 @@
 import ctypes
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 
@@ -102,3 +104,12 @@ def test_sequences_in_a_cache_have_up_to_two_to_the_30_tokens():
     d = _lib.AttentionDesc(**{**PAGED, "max_pages": 1 << 26, "table_stride": 1 << 26})
     assert L.nq_paged_attention_fwd(ctypes.byref(d), P, 1 << 40, P, None) == _lib.NQ_ERR_TOO_LARGE
     assert L.nq_prompt_attention_fwd(ctypes.byref(d), P, 1 << 40, P, None) == _lib.NQ_ERR_TOO_LARGE
+
+
+@pytest.mark.parametrize("sizes", [(1, 1, 2, 128, 1 << 17), (1, 7, 2, 128, 1 << 17), (1, 8, 2, 60, 1 << 17), (1, 8, 2, 264, 1 << 17), (1, 8, 0, 64, 1 << 17), (1, 0, 2, 64, 1 << 17), (1, -8, -2, 64, 1 << 17),
+                                   (1, (1 << 16) + 2, 2, 64, 1 << 17), (1 << 30, 8, 2, 64, 1 << 17), (1, 8, 2, 64, 1 << 30), (1, 8, 2, 64, 0), (1, 8, 2, 64, -1 << 20), (-3, 8, 2, 64, 1 << 17)])
+def test_paged_attention_asks_for_no_scratch_for_what_it_refuses(sizes):
+    """In a process of its own: fewer query heads than key heads ended it (a division by zero)."""
+    code = f"from nanoquant_b200 import _lib; print(_lib.lib().nq_paged_attention_scratch_bytes(*{sizes!r}))"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert (r.returncode, r.stdout.strip()) == (0, "0"), (r.returncode, r.stderr[-300:])
