@@ -13,7 +13,7 @@
 //   warp 0       queries, then keys and values in turn into a ring of stages, by TMA (128-byte swizzle), a box for each page of a cache
 //   warp 1       products: S into tensor memory, then P (from tensor memory, over its S) times V into O, also there
 //   warp 2       values that no query of the block sees, ahead of a window or behind the last token, are set to zero in shared memory: their weights are
-//                zero, which a NaN would survive
+//                zero, which a NaN would survive; and whether the cache has all pages of the sequence, also those that other blocks read: beside the products
 //   warp 3       which block is next: the CTAs that fit the SMs take the grid's other blocks over one by one (cluster launch control), so that long and short
 //                blocks fill the SMs evenly; asked for three steps ahead of a block's end (at its start, the first CTAs took blocks that other SMs were about
 //                to start: 143 us instead of 118 for four pieces of 512 tokens behind up to 16384)
@@ -240,13 +240,16 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
     auto bar_info = [&](int i) { return bars + 96 + 8 * i; };         // the number and sequence of a block are there
     auto bar_info_free = [&](int i) { return bars + 112 + 8 * i; };
     const uint32_t bar_ask = bars + 128;                              // a block is nearly done
-    static_assert(24 * kStages + 136 <= 336, "shared memory map");
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 336);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 340);
-    volatile int* bad_block = reinterpret_cast<volatile int*>(smem + 344);          // four: the block (counted from 1) that last had a page outside the cache
-    const uint32_t answer = sbase + 368;
-    volatile PromptBlock* info = reinterpret_cast<volatile PromptBlock*>(smem + 384);
-    static_assert(384 + 2 * sizeof(PromptBlock) <= 1024, "shared memory map");
+    // The pages of a block's sequence have been looked at.  Four in turn: warp 2 has at most two blocks more than the softmax warps, for a description waits until they
+    // have read the last but one.
+    auto bar_pages = [&](int n) { return bars + 136 + 8 * (n & 3); };
+    static_assert(24 * kStages + 168 <= 368, "shared memory map");
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + 368);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 372);
+    volatile int* bad_pages = reinterpret_cast<volatile int*>(smem + 376);          // four in turn: one of them lies outside the cache
+    const uint32_t answer = sbase + 400;
+    volatile PromptBlock* info = reinterpret_cast<volatile PromptBlock*>(smem + 416);
+    static_assert(416 + 2 * sizeof(PromptBlock) <= 1024, "shared memory map");
 
     const int block_tokens = kTiles * P.tokens;
     if (warp == 2) {
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             mbar_init(bar_info(lane), 1);
             mbar_init(bar_info_free(lane), 3 + 4 * kTiles);
         }
-        if (lane < 4) bad_block[lane] = 0;
+        if (lane < 4) mbar_init(bar_pages(lane), 1);
         if (lane == 0) {
             mbar_init(bar_q, 1);
             mbar_init(bar_q_free, 1);
@@ -355,7 +358,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     if (P.paged && lane < boxes) {
                         page = __ldcg(table + (key >> P.shift));
                         row = key & (d.page_size - 1);
-                        if (page < 0 || page >= d.pages) { page = 0; bad_block[n & 3] = n + 1; }
+                        if (page < 0 || page >= d.pages) page = 0;                // (which warp 2 finds, too)
                     }
                     for (int kv = 0; kv < 2 && ok; ++kv) {
                         ok = mbar_wait_warp(bar_free(s), ph ^ 1, abort_flag, P.status, P.wait_limit);
@@ -484,12 +487,35 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             }
             __syncwarp();
         } else {
-            // ------------------------------------------------------------ values that no query of a block sees
+            // ------------------------------------------------------------ values that no query of a block sees, pages that are not there
+            // (a part of a block looks at its share of the pages: the join behind sees all parts)
+            auto look = [&](int n) {
+                const int* table = d.block_table + (long long)B.seq * d.table_stride;
+                const int page0 = B.sees_begin(P, 0) >> P.shift, pages = B.have > 0 ? ((B.k_len + d.page_size - 1) >> P.shift) - page0 : 0;
+                const int to = page0 + (int)((long long)pages * (B.part + 1) / B.parts);
+                bool bad = false;
+#pragma unroll 8
+                for (int i = page0 + (int)((long long)pages * B.part / B.parts) + lane; i < to; i += 32) {
+                    const int page = __ldcg(table + i);
+                    bad |= page < 0 || page >= d.pages;
+                }
+                bad = __any_sync(0xffffffffu, bad);
+                if (lane == 0) {
+                    bad_pages[n & 3] = bad;
+                    mbar_arrive(bar_pages(n));
+                }
+                __syncwarp();
+            };
             int at = 0;
             uint32_t phases = 0;                   // of the stages' barriers, a bit each
             bool ok = true;
             for (int n = 0; ok && next_info(n); ++n) {
+                bool looked = !P.paged;
                 for (int j = 0; j < B.most && ok; j = j == 0 && B.most > 1 ? B.most - 1 : B.most) {
+                    if (j > 0 && !looked) {
+                        look(n);
+                        looked = true;
+                    }
                     if (!B.fix(j)) continue;
                     const int s = (at + 2 * j + 1) % kStages;
                     ok = mbar_wait_warp(bar_fix(s), phases >> s & 1u, abort_flag, P.status, P.wait_limit);
@@ -508,6 +534,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_full(s));
                 }
+                if (!looked) look(n);
                 at += 2 * B.most;
             }
         }
@@ -674,7 +701,8 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
           if (!ok) break;
           if (n > 0) ok = mbar_wait_warp(bar_o(i), (uint32_t)(count - 1) & 1u, abort_flag, P.status, P.wait_limit);
           tc_fence_after();
-          const bool bad = B.bad || bad_block[block & 3] == block + 1;
+          if (ok && P.paged) ok = mbar_wait_warp(bar_pages(block), (uint32_t)(block >> 2) & 1u, abort_flag, P.status, P.wait_limit);
+          const bool bad = B.bad || (P.paged && bad_pages[block & 3]);
           if (B.parts > 1) {
             // This part's sums, unnormalised, a row to a thread; joined with the others' by the kernel behind.
             float* const to = P.part + ((((long long)B.number * d.k_heads + B.head) * P.splits + B.part) * kTiles + i) * Sh::kPart + row * 4;

@@ -553,7 +553,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     its last key and sees, with ``causal``, all keys up to its own place, with ``window`` only the last ``window`` of these; a query that sees nothing gives zeros.
     ``scale`` of the scores: ``D ** -0.5`` where left out.  Scores and softmax in fp32, the weights rounded to 16 bits for the product with ``v``.  What no query of a
     sequence sees, behind it or ahead of a window, has no influence, in rows or pages; of the keys that one sees, an infinite or NaN value may make NaN of the queries
-    that do not, too (as a product with zero weights does).  A sequence that the table or the cache does not hold is NaN.  Inference: no gradient."""
+    that do not, too (as a product with zero weights does).  A sequence that the table or the cache does not hold (one page that some query of it sees is enough) is NaN
+    in all its rows.  Inference: no gradient."""
     window = _window_of(window)
     scale = _scale_of(scale, q.shape[-1] if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1)
     args = (cu_seqlens, cu_seqlens_k, block_table, lengths)

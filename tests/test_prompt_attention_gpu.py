@@ -281,3 +281,33 @@ def test_maximum_left_behind_in_a_step_without_masks(D, where, dtype):
         bound = u * want[0].abs() + (2 * u + 2.0 ** -11) * want[1] + (2.0 ** -25 if dtype == torch.float16 else 0.0) * (1 + want[2])
         assert ((got.double() - want[0]).abs() <= bound * (1 + 2.0 ** -8)).all()
         assert torch.equal(got, ops.prompt_attention(q, k, v, starts([n]), causal=causal, scale=scale))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,total,page,window", [
+    ([400, 30], [500, 30], 16, None), ([300, 5], [300, 900], 8, None), ([40, 3], [60, 70], 64, None), ([700, 9], [900, 40], 32, 100), ([20, 1], [6000, 300], 16, None), ([30], [4000], 8, 3000),
+    ([300, 7], [40, 7], 16, None), ([600] + [8] * 300, [600] + [40] * 300, 16, None)])
+def test_a_page_that_is_not_there_makes_its_whole_sequence_nan(new, total, page, window, D):
+    """The first and the last page that some query of the sequence sees, one that only a few of them do: NaN in all of its outputs, those ahead of the page and those that see nothing among
+    them, in every run; the other sequences are as without it.  Pages ahead of every window are not looked at."""
+    from nanoquant_b200 import ops
+
+    q, k, v, kc, vc, table, n = piece(new, total, 4, 2, D, page, torch.bfloat16)
+    cu = starts(new)
+    fine = ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=n, window=window)
+    check_attention(fine, expected(q, k, v, new, window))
+    first = max(0, total[0] - new[0] + 1 - window) // page if window else 0
+    last = (total[0] - 1) // page
+    for at in sorted({first, (first + last) // 2, last}):
+        for wrong in (-1, kc.size(0), 2 ** 31 - 1):
+            bad = table.clone()
+            bad[0, at] = wrong
+            bad[0, :first] = wrong                                # (nobody sees those)
+            for _ in range(3):
+                got = ops.prompt_attention(q, kc, vc, cu, block_table=bad, lengths=n, window=window)
+                assert torch.isnan(got[:new[0]]).all(), (at, wrong)
+                assert torch.equal(got[new[0]:], fine[new[0]:])
+    bad = table.clone()
+    bad[0, :first] = -1
+    bad[0, last + 1:] = kc.size(0)                                # (nor what lies behind the last token)
+    assert torch.equal(ops.prompt_attention(q, kc, vc, cu, block_table=bad, lengths=n, window=window), fine)
