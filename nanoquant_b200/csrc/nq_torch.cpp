@@ -940,12 +940,13 @@ bool as_heads(const Tensor& t, Heads& h) {
     return h.head >= h.D && h.head % 8 == 0 && h.token >= h.D && h.token % 8 == 0;
 }
 bool is_index(const Tensor& t, at::ScalarType type, int64_t dim, int dev) {
-    return t.scalar_type() == type && t.dim() == dim && t.get_device() == dev && (dim == 0 || t.size(dim - 1) <= 1 || t.stride(dim - 1) == 1) && t.numel() > 0;
+    return t.scalar_type() == type && t.dim() == dim && t.get_device() == dev && (dim == 0 || t.size(dim - 1) <= 1 || t.stride(dim - 1) == 1);
 }
-// A cache [pages, page_size, heads, D], and the table that leads to its pages.
-bool cache_takes(const Tensor& k, const Tensor& v, const Tensor& table, const Heads& h, at::ScalarType type, int dev) {
+// A cache [pages, page_size, heads, D], and the table that leads to its pages.  (A table of no sequences is one for a call without tokens.)
+bool cache_takes(const Tensor& k, const Tensor& v, const Tensor& table, const Heads& h, at::ScalarType type, int dev, bool no_tokens) {
     if (k.dim() != 4 || v.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != type || v.scalar_type() != type || k.get_device() != dev || v.get_device() != dev ||
-        k.size(2) != h.heads || k.size(3) != h.D || k.numel() == 0 || !is_index(table, at::kInt, 2, dev))
+        k.size(2) != h.heads || k.size(3) != h.D || k.numel() == 0 || !is_index(table, at::kInt, 2, dev) ||
+        (table.numel() == 0 && !(no_tokens && table.size(0) == 0)))
         return false;
     const int64_t page = k.size(1);
     if (page < 8 || (page & (page - 1)) != 0 || (table.size(0) > 1 && table.stride(0) < table.size(1))) return false;
@@ -985,7 +986,7 @@ bool heads_takes(const HeadsArgs& a) {
                   w->get_device() != dev || (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15)))
             return false;
     if (!a.k_cache) return true;
-    if (v.heads != k.heads || !cache_takes(*a.k_cache, *a.v_cache, *a.table, k, type, dev)) return false;
+    if (v.heads != k.heads || !cache_takes(*a.k_cache, *a.v_cache, *a.table, k, type, dev, p.numel() == 0)) return false;
     return a.sequences ? a.sequences->sizes() == p.sizes() && a.sequences->scalar_type() == at::kInt && a.sequences->is_contiguous() && a.sequences->get_device() == dev : true;
 }
 // (q', k'), undefined where there is none
@@ -1101,9 +1102,9 @@ bool attention_takes(const AttentionArgs& a) {
     if (a.table) {
         if (a.k->dim() != 4) return false;
         k = Heads{0, a.k->size(2), q.D, 0, 0};
-        if (!cache_takes(*a.k, *a.v, *a.table, k, type, dev) || !is_index(*a.lengths, at::kInt, 1, dev) || a.lengths->size(0) != a.table->size(0)) return false;
+        if (!cache_takes(*a.k, *a.v, *a.table, k, type, dev, q.tokens == 0) || !is_index(*a.lengths, at::kInt, 1, dev) || a.lengths->size(0) != a.table->size(0)) return false;
     } else {
-        if (a.k->dim() != 3 || !as_heads(*a.k, k) || !as_heads(*a.v, v) || a.k->sizes() != a.v->sizes() || k.D != q.D || k.tokens == 0) return false;
+        if (a.k->dim() != 3 || !as_heads(*a.k, k) || !as_heads(*a.v, v) || a.k->sizes() != a.v->sizes() || k.D != q.D || (k.tokens == 0 && q.tokens > 0)) return false;
         for (const Tensor* t : {a.k, a.v})
             if (t->scalar_type() != type || t->get_device() != dev) return false;
     }

@@ -422,7 +422,7 @@ def _check_index(t, name: str, like, dtypes, shape) -> None:
 
 
 def _check_cache(k_cache, v_cache, block_table, like, heads=None) -> None:
-    """A cache ``[pages, page_size, heads, D]`` that is read and written in place, and its table."""
+    """A cache ``[pages, page_size, heads, D]`` that is read and written in place, and its table (of no sequences only for a call without tokens)."""
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _check_16bit(t, name)
         if t.dim() != 4 or t.numel() == 0:
@@ -436,7 +436,7 @@ def _check_cache(k_cache, v_cache, block_table, like, heads=None) -> None:
             raise RuntimeError(f"{name} is used in place: dense heads at multiples of 8 elements, from a 16-byte boundary on")
     if k_cache.shape != v_cache.shape:
         raise RuntimeError(f"k_cache has shape {tuple(k_cache.shape)}, v_cache {tuple(v_cache.shape)}")
-    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 or block_table.numel() == 0:
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 or (block_table.numel() == 0 and (block_table.size(0) > 0 or like.numel() > 0)):
         raise RuntimeError("block_table must be a CUDA [sequences, pages] matrix of int32")
     _check_like(block_table, "block_table", like, (torch.int32,), block_table.shape)
 
@@ -578,7 +578,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         _check_like(block_table, "block_table", q, (torch.int32,), (cu_seqlens.numel() - 1, block_table.size(1)))
     else:
         _check_heads(k, "k")
-        if k.dim() != 3 or k.size(0) == 0:
+        if k.dim() != 3 or (k.size(0) == 0 and q.size(0) > 0):
             raise RuntimeError(f"k has shape {tuple(k.shape)}, expected [tokens, key heads, D] with one token at least")
         _check_like(k, "k", q, (q.dtype,), (*k.shape[:2], q.size(-1)))
         _check_like(v, "v", q, (q.dtype,), k.shape)
@@ -617,8 +617,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise RuntimeError(f"q has shape {tuple(q.shape)}, expected [sequences, heads, D]")
     _check_cache(k_cache, v_cache, block_table, q)
     _check_shared(q, k_cache.size(2))
-    if q.size(0) == 0 and block_table.size(0) == 0:
-        return torch.empty_like(q)
     _check_index(lengths, "lengths", q, (torch.int32,), (q.size(0),))
     _check_like(block_table, "block_table", q, (torch.int32,), (q.size(0), block_table.size(1)))
     _no_gradient("paged_attention", q, k_cache, v_cache)

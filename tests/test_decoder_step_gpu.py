@@ -369,3 +369,36 @@ def test_wait_that_runs_out():
             assert L.nq_gemm_set_wait_limit(old) == 1
         scratch.zero_()
         assert torch.equal(ops.prompt_attention(q, k, v, cu), want) and status() == 0
+
+
+@pytest.mark.parametrize("how", ["eager", "compile", "trace"])
+def test_calls_without_tokens(how):
+    """A decode step, or a batch of prompts, of no sequences: its table has no rows, with or without columns."""
+    from nanoquant_b200 import ops
+
+    q, k, v = (rand(i, 3, n, D, dtype=torch.bfloat16)[:0] for i, n in ((0, H), (1, K), (2, K)))
+    cache = [torch.zeros((4, PAGE, K, D), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    freq = 1e4 ** (torch.arange(0, D, 2, device="cuda").float() / -D)
+    for columns in (5, 0):
+        table = torch.zeros((0, columns), dtype=torch.int32, device="cuda")
+
+        def step(q, k, v, table, none):
+            turned_q = ops.append_kv(k, v, *cache, table, none, None, freq, q=q)
+            fresh_q, fresh_k = ops.qk_norm_rope(q, k, none, freq)
+            start = torch.zeros(2, dtype=torch.int32, device="cuda")
+            return turned_q, fresh_q, fresh_k, ops.paged_attention(turned_q, *cache, table, none), ops.prompt_attention(fresh_q, fresh_k, v, start)
+
+        run = {"eager": step, "compile": torch.compile(step, backend="aot_eager", fullgraph=True), "trace": step if how != "trace" else torch.jit.trace(step, (q, k, v, table, none), check_trace=False)}[how]
+        got = run(q, k, v, table, none)
+        assert [t.shape[0] for t in got] == [0] * 5 and [t.shape[1:] for t in got] == [(H, D), (H, D), (K, D), (H, D), (H, D)]
+        assert all((c == 0).all() for c in cache)
+    # what is wrong with a call is said without tokens too
+    with pytest.raises(RuntimeError, match="lengths"):
+        ops.paged_attention(q, *cache, table, none.long())
+    with pytest.raises(RuntimeError, match="block_table"):
+        ops.paged_attention(q, *cache, torch.zeros((2, 0), dtype=torch.int32, device="cuda"), none)
+    with pytest.raises(RuntimeError, match="block_table"):
+        ops.append_kv(rand(1, 3, K, D, dtype=torch.bfloat16), rand(2, 3, K, D, dtype=torch.bfloat16), *cache, table, torch.zeros(3, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="no multiple"):
+        ops.paged_attention(q[:, :7], *cache, table, none)
