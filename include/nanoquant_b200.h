@@ -451,8 +451,9 @@ int nq_heads_fwd(const nq_heads_desc* desc_host, nq_stream_t stream);
 
 /* Attention: o = sum_j p_j v_j with p = softmax(scale q . k_j) over the tokens j that a query sees, heads q_heads / k_heads of which share a key head.
  * The query at place r of its sequence sees the tokens r - window < j <= r (window 0: no limit; without `causal` all of the sequence's j > r - window).
- * A query that sees nothing gives zeros.  What no query of a sequence sees (rows of other sequences, slots behind the last token or ahead of every window)
- * does not enter, whatever it holds; of prompts, an infinite or NaN value that some query sees may make NaN of those that do not.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type.
+ * A query that sees nothing gives zeros; one whose scores are all minus infinity is NaN, as a softmax of these is.  What no query of a sequence sees (rows of
+ * other sequences, slots behind the last token or ahead of every window) does not enter, whatever it holds; of prompts, an infinite or NaN value that some
+ * query sees may make NaN of those that do not.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type.
  * A sequence that the table or the cache does not hold (a length beyond the table; among the pages with a token that one of its queries sees, one outside the
  * cache) is NaN in all its outputs, those of queries that do not see the page too.
  *

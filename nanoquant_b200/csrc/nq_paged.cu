@@ -379,12 +379,13 @@ struct PagedHeads {
             }
         }
     }
-    __device__ __forceinline__ void store(const nq_attention_desc& d, int seq, int h0, int rows) const {
+    // (no sum: there is no token, or only scores of minus infinity: 0 x infinity, as a softmax of these is)
+    __device__ __forceinline__ void store(const nq_attention_desc& d, int seq, int h0, int rows, bool tokens) const {
         const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int row = g + 8 * r;
-            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+            const float inv = l[r] == 0.f && !tokens ? 0.f : 1.f / l[r];
             uint16_t* at = static_cast<uint16_t*>(d.out) + ((long long)seq * d.q_heads + h0 + row) * d.D;
             if (row < rows) {
 #pragma unroll
@@ -467,10 +468,10 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
         __syncwarp();                           // the stage may be filled again
         if (++stage == S::kStages) { stage = 0; phase ^= 1; }
         const int seq = at.seq;
-        const bool seq_bad = at.R.bad != 0, last = at.s + 1 == at.R.steps;
+        const bool seq_bad = at.R.bad != 0, tokens = at.R.end > 0, last = at.s + 1 == at.R.steps;
         if (last || i + 1 == count) {
             heads.finish(seq_bad || (bad_items >> (at_items & 31) & 1u));
-            if (from == 0 && last) heads.store(d, seq, h0, rows);
+            if (from == 0 && last) heads.store(d, seq, h0, rows, tokens);
             else heads.save(P.part + ((long long)W * 2 + (from == 0 ? 1 : 0)) * P.piece, rows);
             ++at_items;
             begin = true;
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedShape<DP>::kCtasPerSm) pag
             v.x += u.x * e;
             v.y += u.y * e;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f && R.end == 0 ? 0.f : 1.f / sum;
         if (col < d.D)
             *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(d.out) + ((long long)seq * d.q_heads + h0 + row) * d.D + col) = head_pack<BF16>(v.x * inv, v.y * inv);
     }
@@ -651,7 +652,7 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const __grid_consta
                     v.y += partial[threadIdx.x + k * kPairs].y;
                 }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = 1.f / l;               // (an item of several groups has tokens; no sum: only scores of minus infinity, 0 x infinity)
         if (group == 0 && col < d.D)
             *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(d.out) + ((long long)seq * d.q_heads + h0 + row) * d.D + col) = head_pack<BF16>(v.x * inv, v.y * inv);
     }

@@ -721,7 +721,8 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             tc_fence_before();
             continue;
           }
-          const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
+          // (no sum: nothing is seen, or only scores of minus infinity: 0 x infinity, as a softmax of these is)
+          const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f && begin >= end ? 0.f : 1.f / l;
           uint16_t* const out = static_cast<uint16_t*>(d.out) + ((long long)(B.q_at + first) * d.q_heads + B.head * P.rows) * d.D;
           // 64 columns at a time through shared memory, so that eight lanes store a row's 128 bytes (every thread its own row kept the load and store unit busy for 4000 clk);
           // the next block's first products run meanwhile.  (Places are computed here: kept from block to block they would take the registers that a step needs.)
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant_
                     w[p] = exp2_approx(w[p] - base);
                     l += sums[p] * w[p];
                 }
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = l == 0.f && B.sees_begin(P, t) >= B.sees_end(P, t) ? 0.f : 1.f / l;
 #pragma unroll
                 for (int p = 0; p < kPromptParts; ++p) w[p] *= inv;
             }

@@ -550,7 +550,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     decreasing); rows of no sequence come back as zeros.  ``k`` and ``v`` ``[Tk, key heads, D]``, packed by ``cu_seqlens_k`` (left out: as the queries);
     or, with ``block_table`` and ``lengths`` (int32, tokens of each sequence in the cache, the new ones included), the paged cache that :func:`append_kv` fills: a
     piece of a prompt behind what the cache holds already.  At most 128 heads share a key head.  The last query of a sequence is at the place of
-    its last key and sees, with ``causal``, all keys up to its own place, with ``window`` only the last ``window`` of these; a query that sees nothing gives zeros.
+    its last key and sees, with ``causal``, all keys up to its own place, with ``window`` only the last ``window`` of these; a query that sees nothing gives zeros, and
+    one whose scores are all minus infinity NaN.
     ``scale`` of the scores: ``D ** -0.5`` where left out.  Scores and softmax in fp32, the weights rounded to 16 bits for the product with ``v``.  What no query of a
     sequence sees, behind it or ahead of a window, has no influence, in rows or pages; of the keys that one sees, an infinite or NaN value may make NaN of the queries
     that do not, too (as a product with zero weights does).  A sequence that the table or the cache does not hold (one page that some query of it sees is enough) is NaN

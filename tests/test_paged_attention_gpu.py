@@ -180,3 +180,23 @@ def test_refusals():
     q.requires_grad_()
     with pytest.raises(RuntimeError, match="no gradient"):
         ops.paged_attention(q, kc, vc, table, n)
+
+
+@pytest.mark.parametrize("width", [None, 1000])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_of_minus_infinity(D, width):
+    """As torch's softmax has them: next to finite ones a weight of zero, and NaN where all of a query are so (which is not one that sees nothing); with a wide table by several CTAs."""
+    from nanoquant_b200 import ops
+
+    lengths, infinite = [250, 250, 1, 0, 130, 40], [250, 240, 1, 0, 0, 39]
+    q, k, v, kc, vc, table, n = make(lengths, 4, 2, D, 16, torch.bfloat16, width=width)
+    q[..., 0] = -1.0
+    for s, m in enumerate(infinite):
+        for t in range(m):
+            kc[table[s, t // 16].item(), t % 16, :, 0] = float("inf")
+    got = ops.paged_attention(q, kc, vc, table, n)
+    assert torch.isnan(got[[0, 2]]).all() and (got[3] == 0).all()
+    some = [1, 4, 5]
+    check_attention(got[some], expected(q[some], [k[s][infinite[s]:] for s in some], [v[s][infinite[s]:] for s in some]))
+    got = ops.paged_attention(q, kc, vc, table, n, window=11)
+    assert torch.isnan(got[[0, 2]]).all() and (got[3] == 0).all() and not torch.isnan(got[some]).any()

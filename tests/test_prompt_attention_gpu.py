@@ -311,3 +311,32 @@ def test_a_page_that_is_not_there_makes_its_whole_sequence_nan(new, total, page,
     bad[0, :first] = -1
     bad[0, last + 1:] = kc.size(0)                                # (nor what lies behind the last token)
     assert torch.equal(ops.prompt_attention(q, kc, vc, cu, block_table=bad, lengths=n, window=window), fine)
+
+
+@pytest.mark.parametrize("behind", [0, 300, 3000])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_of_minus_infinity(D, behind):
+    """As torch's softmax has them: next to finite ones a weight of zero, and NaN for a query whose scores are all so (which is not one that sees nothing)."""
+    from nanoquant_b200 import ops
+
+    new, first = (200, 130) if not behind else (20, behind + 7)
+    total = new + behind
+    q, k, v, kc, vc, table, n = piece([new], [total], 4, 2, D, 16, torch.bfloat16)
+    place = torch.arange(new, device="cuda") + behind
+    q[..., 0] = -1.0
+    k[0][:first, :, 0] = float("inf")
+    kc[table[0].long()] = torch.cat((k[0], k[0].new_zeros(table.size(1) * 16 - total, 2, D))).view(-1, 16, 2, D)
+    some = place >= first
+    want = attention64(q[some], k[0][first:], v[0][first:], place[some] - first)
+    cu = starts([new])
+    for got in (ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=n), ops.prompt_attention(q, k[0], v[0], cu, starts([total]))):
+        assert torch.isnan(got[~some]).all()
+        check_attention(got[some], want)
+    got = ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=n, window=2)
+    assert torch.isnan(got[~some]).all() and not torch.isnan(got[some]).any()
+    k[0][..., 0] = float("inf")
+    kc[table[0].long(), ..., 0] = float("inf")
+    for causal in (True, False):
+        assert torch.isnan(ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=n, causal=causal)).all()
+        assert torch.isnan(ops.prompt_attention(q, k[0], v[0], cu, starts([total]), causal=causal)).all()
+    assert (ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=torch.zeros_like(n)) == 0).all()
