@@ -453,7 +453,8 @@ int nq_heads_fwd(const nq_heads_desc* desc_host, nq_stream_t stream);
  * The query at place r of its sequence sees the tokens r - window < j <= r (window 0: no limit; without `causal` all of the sequence's j > r - window).
  * A query that sees nothing gives zeros; one whose scores are all minus infinity is NaN, as a softmax of these is.  What no query of a sequence sees (rows of
  * other sequences, slots behind the last token or ahead of every window) does not enter, whatever it holds; of prompts, an infinite or NaN value that some
- * query sees may make NaN of those that do not.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type.
+ * query sees may make NaN of those that do not.  Scores, softmax and sums in fp32, one rounding of o; the weights p are multiplied in the operands' 16-bit type
+ * (fp16: each to 2^-12 of itself or, of prompts, 2^-28, of single queries 2^-32 of the largest one).
  * A sequence that the table or the cache does not hold (a length beyond the table; among the pages with a token that one of its queries sees, one outside the
  * cache) is NaN in all its outputs, those of queries that do not see the page too.
  *

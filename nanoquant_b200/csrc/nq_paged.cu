@@ -1,6 +1,6 @@
 // Attention of one new token per sequence over a paged cache.
 //
-//     o[h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale log2(e) q[h] . k_j - m),   m the largest of these exponents so far, less 8 at most
+//     o[h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale log2(e) q[h] . k_j - m),   m the largest of these exponents so far, less 8 at most (fp16: less 7 to 15)
 //
 // Bound by memory: keys and values are read once, for all the query heads that share them: 4 D bytes for 4 D G operations.  Those G heads are the rows of
 // mma.sync.m16n8k16 (up to 16; the instruction's rate is far above what memory delivers, and few rows would leave tcgen05's 128 idle).
@@ -20,7 +20,9 @@
 // which some 10 us are start, join and the uneven end (each further token: 6.9 TB/s); one of 1000, 32 heads on 8: 8.5 us, two launches.
 //
 // The weights p are rounded to the operands' type for the product with the values: 2^-9 (bf16) or 2^-12 (fp16) of each, which the average over
-// tokens does not enlarge.  Sums of p are fp32 sums of the rounded values.
+// tokens does not enlarge.  fp16 has subnormals below 2^-14, where a rounding is 2^-25 whatever the weight, and nothing below 2^-25: its weights are formed 2^7 times as
+// large (m is kept that much below the maximum; 2^(8 + 7) is the most that fp16 holds), so that this is 2^-32 of the largest weight for each token.  Sums of p are
+// fp32 sums of the rounded values.
 #include <algorithm>
 
 #include "nq_attn.cuh"
@@ -316,12 +318,13 @@ struct PagedHeads {
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * factor;
         }
         // The maximum is moved, and o multiplied, only when it grows by more than 2^8: weights and sums have room for that.
-        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+        constexpr float kLift = BF16 ? 0.f : 7.f, kBehind = 8.f + kLift;
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kBehind || top[1] > m[1] + kBehind)) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                if (!(top[r] > m[r] + 8.f)) continue;
-                const float shrink = exp2_approx(m[r] - top[r]);      // (0 at first)
-                m[r] = top[r];
+                if (!(top[r] > m[r] + kBehind)) continue;
+                const float to = top[r] - kLift, shrink = exp2_approx(m[r] - to);      // (0 at first)
+                m[r] = to;
                 l[r] *= shrink;
 #pragma unroll
                 for (int n = 0; n < DP / 8; ++n) {

@@ -26,7 +26,9 @@
 // Few tokens behind many keys are too few blocks for the SMs: a block's steps are then divided among up to 16 CTAs, whose sums a second launch joins.
 //
 // The weights P are rounded to the operands' 16-bit type for the product with the values (what the tensor cores take): 2^-9 (bf16) or 2^-12 (fp16) of each, not
-// enlarged by the average over tokens.
+// enlarged by the average over tokens.  fp16 has subnormals below 2^-14, where a rounding is 2^-25 whatever the weight, and nothing below 2^-25: its weights are formed 2^3
+// times as large (m is kept that much below the maximum; 2^(12 + 3) is the most that fp16 holds), so that this is 2^-28 of the largest weight for each key (formed
+// as they are, weights of 2^-25.2 are all lost, however many).  The sum l is of the weights ahead of this rounding.
 #include <type_traits>
 
 #include "nq_attn.cuh"
@@ -71,6 +73,7 @@ static_assert(128 * kPromptRegsIssue + 256 * kPromptRegsSoftmax <= 384 * kPrompt
 constexpr int kPromptAsk = 3;                                     // steps before a block's end, in which the next one is looked up
 constexpr int kPromptParts = 16;                                  // of a block at most
 constexpr float kPromptSlack = 8.f;                               // powers of two by which a maximum may be behind
+constexpr float kPromptMost = 12.f;                               // and by which weights may exceed 1 where it is not looked for
 
 struct PromptBlock {
     int have;                      // 1; 0: nothing to do; -1: no more blocks
@@ -542,6 +545,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
         // ---------------------------------------------------------------- softmax
         if constexpr (kTiles == 2) regs_up<kPromptRegsSoftmax>();
         constexpr int kChunks = kKeys / 32, kEarly = Sh::kEarly;
+        constexpr float kLift = BF16 ? 0.f : 3.f, kMostWeight = BF16 ? 4096.f : 32768.f;       // 2^(kPromptMost + kLift)
         const int i = (warp - 4) >> 2, row = 32 * (warp & 3) + lane;
         const int token = row / P.rows;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     weights(c, 0, 16, base2);
                     tmem_st16(s_at + 16 * c, w);
                 }
-                const bool fine = total() < 4096.f && peaks(kChunks - 1) * P.factor < m + 12.f;
+                const bool fine = total() < kMostWeight && peaks(kChunks - 1) * P.factor < m + (kPromptMost + kLift);
                 done = __all_sync(0xffffffffu, fine || !live);
                 if (done) {
                     finish(base2);
@@ -665,9 +669,9 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     peak = max_or_nan(peak, peaks(c));
                 }
                 peak *= P.factor;
-                const bool grow = peak > m + kPromptSlack;
+                const bool grow = peak > m + (kPromptSlack + kLift);
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float to = grow ? peak : m, shrink = grow ? exp2_approx(m - to) : 1.f;
+                    const float to = grow ? peak - kLift : m, shrink = grow ? exp2_approx(m - to) : 1.f;
                     m = to;
                     if (j > 0) {
                         l *= shrink;

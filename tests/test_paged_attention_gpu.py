@@ -200,3 +200,24 @@ def test_scores_of_minus_infinity(D, width):
     check_attention(got[some], expected(q[some], [k[s][infinite[s]:] for s in some], [v[s][infinite[s]:] for s in some]))
     got = ops.paged_attention(q, kc, vc, table, n, window=11)
     assert torch.isnan(got[[0, 2]]).all() and (got[3] == 0).all() and not torch.isnan(got[some]).any()
+
+
+@pytest.mark.parametrize("width", [None, 1000])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_small_weights(D, width):
+    """fp16: one key 2^25.2 above all others, which by themselves make up the result.  A weight's subnormal half step is 2^-32 of the largest weight (they are formed 2^7 times as large)."""
+    from nanoquant_b200 import ops
+
+    lengths = [250, 17, 100]
+    q, k, v, kc, vc, table, n = make(lengths, 4, 2, D, 16, torch.float16, width=width)
+    q[:], q[..., 0] = 0.0, 1.0
+    for s, m in enumerate(lengths):
+        k[s][:], k[s][0, :, 0] = 0.0, 25.1875
+        v[s].abs_()[0] = 0.0
+        at = table[s, torch.arange(m, device="cuda") // 16].long(), torch.arange(m, device="cuda") % 16
+        kc[at], vc[at] = k[s], v[s]
+    scale = 0.69314718
+    o, avg, all_v = expected(q, k, v, scale=scale)
+    got = ops.paged_attention(q, kc, vc, table, n, scale=scale)
+    bound = 2.0 ** -11 * o + (2.0 ** -10 + 2.0 ** -12) * avg + 2.0 ** -32 * all_v + 2.0 ** -25           # (the last: half a step of the result)
+    assert ((got.double() - o).abs() <= bound * (1 + 2.0 ** -8)).all()

@@ -340,3 +340,20 @@ def test_scores_of_minus_infinity(D, behind):
         assert torch.isnan(ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=n, causal=causal)).all()
         assert torch.isnan(ops.prompt_attention(q, k[0], v[0], cu, starts([total]), causal=causal)).all()
     assert (ops.prompt_attention(q, kc, vc, cu, block_table=table, lengths=torch.zeros_like(n)) == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_small_weights(D):
+    """fp16: one key 2^25.2 above all others, which by themselves make up the result.  A weight's subnormal half step is 2^-28 of the largest weight (they are formed 2^3 times as large)."""
+    from nanoquant_b200 import ops
+
+    n = 1000
+    q, k, v = (torch.zeros((n, 2, D), dtype=torch.float16, device="cuda") for _ in range(3))
+    q[..., 0], k[0, :, 0], v[1:] = 1.0, 25.1875, rand(0, n - 1, 2, D).abs().half()
+    scale = 0.69314718
+    cu = starts([n])
+    o, avg, all_v = expected(q, [k], [v], [n], scale=scale)
+    got = ops.prompt_attention(q, k, v, cu, scale=scale)
+    bound = 2.0 ** -11 * o + (2.0 ** -10 + 2.0 ** -12) * avg + 2.0 ** -28 * all_v + 2.0 ** -25           # (the last: half a step of the result)
+    assert ((got.double() - o).abs() <= bound * (1 + 2.0 ** -8)).all()
+    check_attention(ops.prompt_attention(q, k, v, cu, scale=scale, causal=False), expected(q, [k], [v], [n], scale=scale, causal=False))
