@@ -402,3 +402,10 @@ def test_calls_without_tokens(how):
         ops.append_kv(rand(1, 3, K, D, dtype=torch.bfloat16), rand(2, 3, K, D, dtype=torch.bfloat16), *cache, table, torch.zeros(3, dtype=torch.int32, device="cuda"))
     with pytest.raises(RuntimeError, match="no multiple"):
         ops.paged_attention(q[:, :7], *cache, table, none)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_vmap_is_refused(name):
+    x, fn = calls()[name]
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(fn)(torch.stack((x, x)))

@@ -357,3 +357,44 @@ def test_many_small_weights(D):
     bound = 2.0 ** -11 * o + (2.0 ** -10 + 2.0 ** -12) * avg + 2.0 ** -28 * all_v + 2.0 ** -25           # (the last: half a step of the result)
     assert ((got.double() - o).abs() <= bound * (1 + 2.0 ** -8)).all()
     check_attention(ops.prompt_attention(q, k, v, cu, scale=scale, causal=False), expected(q, [k], [v], [n], scale=scale, causal=False))
+
+
+def parts_of(q, kc, table, seqs, K):
+    """Scratch of a call over the cache: none where no block is cut."""
+    import ctypes
+
+    from nanoquant_b200 import _lib
+
+    d = _lib.AttentionDesc(q=1 << 16, k=1 << 16, v=1 << 16, out=1 << 16, cu_seqlens=1 << 16, lengths=1 << 16, block_table=1 << 16, k_slot=8, v_slot=8, table_stride=1, pages=kc.size(0),
+                           max_pages=table.size(1), page_size=kc.size(1), T=len(q), seqs=seqs, q_heads=q.size(1), k_heads=K, D=q.size(2), causal=1, scale=1.0)
+    return _lib.lib().nq_prompt_attention_scratch_bytes(ctypes.byref(d))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new,total,H,K,D,page,window", [
+    ([40, 3, 1], [2000, 2, 700], 8, 2, 128, 16, None), ([300, 5], [100, 90], 4, 2, 64, 16, None), ([200, 2], [900, 4000], 4, 1, 256, 64, None), ([30, 30], [1500, 3], 4, 2, 96, 8, 300),
+    ([600], [600], 8, 2, 64, 32, None)])
+def test_tables_far_wider_than_the_sequences(new, total, H, K, D, page, window, causal):
+    """A table for 65536 tokens, by whose width blocks are cut: lengths that give many parts, one, or none; fewer keys than queries; every query over all keys (as over another text's)."""
+    from nanoquant_b200 import ops
+
+    q, k, v, kc, vc, table, n = piece(new, total, H, K, D, page, torch.bfloat16)
+    wide = torch.full((len(new), 65536 // page), -9, dtype=torch.int32, device="cuda")
+    wide[:, :table.size(1)] = table
+    assert parts_of(q, kc, wide, len(new), K) > 0
+    want = expected(q, k, v, new, window, causal=causal)
+    got = ops.prompt_attention(q, kc, vc, starts(new), block_table=wide, lengths=n, causal=causal, window=window)
+    check_attention(got, want)
+    assert torch.equal(got, ops.prompt_attention(q, kc, vc, starts(new), block_table=wide, lengths=n, causal=causal, window=window))
+    check_attention(ops.prompt_attention(q, kc, vc, starts(new), block_table=table, lengths=n, causal=causal, window=window), want)
+
+
+def test_few_queries_over_all_keys_of_another_text():
+    """Packed keys, no causal order, blocks cut along the keys."""
+    from nanoquant_b200 import ops
+
+    new, total = [9, 70, 1], [5000, 2000, 3000]
+    q = make(new, 8, 2, 128, torch.float16)[0]
+    k, v = make(total, 8, 2, 128, torch.float16, seed=1)[1:]
+    got = ops.prompt_attention(q, k, v, starts(new), starts(total), causal=False)
+    check_attention(got, expected(q, k.split(total), v.split(total), new, causal=False))
