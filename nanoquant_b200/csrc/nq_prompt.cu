@@ -513,12 +513,8 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             uint32_t phases = 0;                   // of the stages' barriers, a bit each
             bool ok = true;
             for (int n = 0; ok && next_info(n); ++n) {
-                bool looked = !P.paged;
+                if (P.paged) look(n);              // (a description comes some steps before the block before it is done)
                 for (int j = 0; j < B.most && ok; j = j == 0 && B.most > 1 ? B.most - 1 : B.most) {
-                    if (j > 0 && !looked) {
-                        look(n);
-                        looked = true;
-                    }
                     if (!B.fix(j)) continue;
                     const int s = (at + 2 * j + 1) % kStages;
                     ok = mbar_wait_warp(bar_fix(s), phases >> s & 1u, abort_flag, P.status, P.wait_limit);
@@ -537,7 +533,6 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_full(s));
                 }
-                if (!looked) look(n);
                 at += 2 * B.most;
             }
         }
@@ -559,7 +554,7 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
           const int first = B.first + i * P.tokens, t = first + token, left = B.q_len - first;       // (tokens of the sequence from the tile's first on)
           const bool live = token < P.tokens && token < left;
           const int begin = B.sees_begin(P, t), end = live ? B.sees_end(P, t) : 0, k_first = B.k_first;
-          float m = live ? -INFINITY : 0.f, l = 0.f;      // (rows that are not there hold nobody up)
+          float m = live && begin < end ? -INFINITY : 0.f, l = 0.f;      // (rows that are not there, or see nothing, hold nobody up)
           const int n = kTiles == 1 ? B.most : (i == 0 ? B.steps[0] : B.steps[kTiles - 1]);
           for (int j = 0; j < n; ++j, ++count) {
             const int b = kTiles == 1 ? count & 1 : i;
@@ -725,8 +720,8 @@ __global__ void __launch_bounds__(PromptShape<DP>::kThreads, 1) prompt_kernel(co
             tc_fence_before();
             continue;
           }
-          // (no sum: nothing is seen, or only scores of minus infinity: 0 x infinity, as a softmax of these is)
-          const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f && begin >= end ? 0.f : 1.f / l;
+          // (no sum: nothing is seen, or, without a maximum, only scores of minus infinity: 0 x infinity, as a softmax of these is)
+          const float inv = bad ? __int_as_float(0x7fffffff) : l == 0.f && m > -INFINITY ? 0.f : 1.f / l;
           uint16_t* const out = static_cast<uint16_t*>(d.out) + ((long long)(B.q_at + first) * d.q_heads + B.head * P.rows) * d.D;
           // 64 columns at a time through shared memory, so that eight lanes store a row's 128 bytes (every thread its own row kept the load and store unit busy for 4000 clk);
           // the next block's first products run meanwhile.  (Places are computed here: kept from block to block they would take the registers that a step needs.)
