@@ -9,15 +9,15 @@
 // 16 of its query heads.  The steps of all sequences lie one behind the other; a group of warps, one for each key head, takes the same number of them as
 // every other group, found from the lengths on the device: batches of any lengths fill the SMs evenly, and a captured graph follows the lengths.  (What
 // the heads of a token have in the cache lies side by side and is read at the same time; with one head's steps after the other's, 32 heads on 8 of 64
-// columns ran at 5.8 TB/s instead of 6.4 to 6.7, and 64 on 8 of 128 at 6.4 instead of 6.7.)  A warp has a ring of steps of its own in shared memory (TMA
+// columns ran at 5.8 TB/s instead of 6.5, and 64 on 8 of 128 at 6.4 instead of 6.65: eight sequences of 131072 tokens.)  A warp has a ring of steps of its own in shared memory (TMA
 // boxes of a page's tokens x 64 columns; it runs on into the next sequence), its own running maximum, sum and accumulators: nothing in the loop waits
 // for another warp.  (Copied by cp.async, 16 bytes a lane, the same steps were as fast, but of 650 instructions each instead of 370; bulk copies of 256-byte rows took
 // 206 us where these take 153.)  An item that lies in several groups leaves fp32 results (m, sum, unnormalised o) in the scratch, which a second,
 // overlapped launch joins in their order.  Where the table has room for short sequences only, a CTA takes an item, its steps divided among the four warps
 // and their results joined through shared memory: one launch.
 //
-// Measured: 32 sequences of up to 4096 tokens, 32 heads of 128, fp16: 105 us, 6.05 TB/s; 4 of up to 131072, 64 heads on 8, bf16: 151 us, 6.03 TB/s, of
-// which some 10 us are start, join and the uneven end (each further token: 6.9 TB/s); one of 1000, 32 heads on 8: 8.5 us, two launches.
+// Measured: 32 sequences of up to 4096 tokens, 32 heads of 128, fp16: 107 us, 5.9 TB/s; 4 of up to 131072, 64 heads on 8, bf16: 154 us, 5.9 TB/s, of
+// which some 10 us are start, join and the uneven end; one of 1000, 32 heads on 8: 8.7 us, two launches.
 //
 // The weights p are rounded to the operands' type for the product with the values: 2^-9 (bf16) or 2^-12 (fp16) of each, which the average over
 // tokens does not enlarge.  fp16 has subnormals below 2^-14, where a rounding is 2^-25 whatever the weight, and nothing below 2^-25: its weights are formed 2^7 times as

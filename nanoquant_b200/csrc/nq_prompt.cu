@@ -16,7 +16,7 @@
 //                zero, which a NaN would survive; and whether the cache has all pages of the sequence, also those that other blocks read: beside the products
 //   warp 3       which block is next: the CTAs that fit the SMs take the grid's other blocks over one by one (cluster launch control), so that long and short
 //                blocks fill the SMs evenly; asked for three steps ahead of a block's end (at its start, the first CTAs took blocks that other SMs were about
-//                to start: 143 us instead of 118 for four pieces of 512 tokens behind up to 16384)
+//                to start: 138 us instead of 113 for four pieces of 512 tokens behind up to 4096)
 //   warps 4-11   softmax, four warps to a tile, a row to a thread; the next S of a tile is ordered behind its P V, the other tile's products run meanwhile
 //
 // The maximum m is moved, and O multiplied accordingly, only when it grows by more than 2^8: P and its sum have room for that, and the result does not depend on
@@ -850,11 +850,14 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant_
     }
 }
 
-// Parts of a block's steps.  Blocks are dealt out as CTAs become free, so that a few for every SM are enough: below 1.5 of them (`blocks` counts a block to each
-// sequence more than there may be) they are cut to make two.  128 tokens behind 2048, eight times, 32 heads on 8 of 128 (192 blocks): 32 us cut and 37 whole; 8192 tokens
-// over themselves, 8 heads on 1 (257): 140 and 115; 512 behind up to 4096, four times (288): 116 both.  A part has eight steps at least, for its sums pass through
-// memory (16 tokens behind 16384: 26 us, and with sixteen steps 36; 128 behind 2048: with four 36); of a prompt over itself, whose blocks see half of it, sixteen
-// (2048 tokens: 40 us, with eight 63).  Sixteen parts at most (16 tokens behind 131072: 109 us, up to ten parts 164, up to 32 176).
+// Parts of a block's steps.  Blocks are dealt out as CTAs become free; below 1.5 of them for an SM (`blocks` counts a block to each sequence more than there may be) they
+// are cut to make two.  Cut by this rule and whole, us in a graph, 32 heads on 8 of 128, bf16, pages of 64: 128 tokens behind 2048 26 and 34, behind 8192 29 and 112; four times
+// that 31 and 35, 82 and 122; eight times (128 blocks with work) 56 and 37, 155 and 139.  So parts that the SMs take all at once gain much, and a second turn of them
+// costs more than it gains on short caches; which it is depends on the lengths, which the host does not have.  Above the line: four pieces of 512 tokens behind 4096, 126 whole and
+// 155 in two; 8192 tokens over themselves, 489 and 630.  Sixteen parts at most (16 tokens behind 131072: 112 us, ten parts 172, eight 202).
+// A part has eight steps at least of the keys that there may be (of a prompt over itself, whose blocks see half of it, sixteen: 2048 tokens whole 39 us, in two 59), and
+// four of those that there are, where the table is wider than the sequences: of 2048 tokens and a table for 131072, 128 queries take 22 us in parts of four steps, 28 of eight, 38 of
+// sixteen, and 16 queries 18, 23, 33.
 template <int DP>
 static int prompt_splits(const nq_attention_desc& d, int tokens) {
     using Sh = PromptShape<DP>;
@@ -904,7 +907,7 @@ static int prompt_launch(PromptParams& P, cudaStream_t stream) {
     st = mm_encode_heads(&P.map_v, d.v, type, {d.D, rows, d.k_heads, pages}, {d.v_slot, d.v_head, d.v_page}, {64, P.piece, 1, 1});
     if (st != NQ_OK) return st;
     P.splits = prompt_splits<DP>(d, P.tokens);
-    P.least = 4;
+    P.least = 4;                   // (measured at prompt_splits)
     const int64_t block = (int64_t)Sh::kTiles * P.tokens, blocks = ((d.T + block - 1) / block + d.seqs) * d.k_heads, ctas = blocks * P.splits;
     if (ctas > 0x7fffffff) return NQ_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
